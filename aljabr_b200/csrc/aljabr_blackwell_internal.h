@@ -209,6 +209,74 @@ cudaError_t launch_rmsnorm(float* out, const float* x, const float* w, int n, fl
 cudaError_t launch_host_pull(float* dst, const float* src_mapped, size_t n, int sms, cudaStream_t stream);
 cudaError_t launch_silu_ffn(float* out, const float* gate, const float* up, int n, int sms, cudaStream_t stream);
 
+// 4-bit KV cache (kv4.cuh describes the layout).  Rows in (append, type of k /
+// v, strides in elements between tokens, k_out / v_out the values stored) and
+// out (read); slot = page * page_size + position, -1 skips.
+struct Kv4Rows {
+    uint8_t* cache;
+    int pages, page_size, kv_heads, head_dim;
+    const int* slots;
+    int tokens;
+    int type;                // ALJ_KV_F32 / ALJ_KV_BF16
+    const void* k;
+    const void* v;
+    long long k_stride, v_stride;
+    void* k_out;             // [tokens][kv_heads * head_dim]
+    void* v_out;
+    int vec, vec_out;        // 16-byte accesses on the inputs / outputs
+};
+bool kv4_supported(int page_size, int kv_heads, int head_dim);
+long long kv4_cache_bytes(int pages, int page_size, int kv_heads, int head_dim);
+cudaError_t launch_kv4_append(const Kv4Rows& p, cudaStream_t stream);
+cudaError_t launch_kv4_read(const Kv4Rows& p, cudaStream_t stream);
+
+// Attention over it (kv4_attention.cu): q [batch][q_len] rows of kv_heads *
+// group heads, q_stride elements apart; query t of sequence b sees positions
+// up to lens[b] + len_add - q_len + t (window > 0: the last `window` of them).
+constexpr int kKv4MaxBatch = 2048;
+constexpr int kKv4MaxRows = 1024;    // q_len * group: a chunk of a prompt belongs to the prefill attention
+struct Kv4Attn {
+    void* out;               // [batch][q_len][kv_heads * group][head_dim], q's type
+    const void* q;
+    long long q_stride;
+    int type;
+    const uint8_t* cache;
+    int pages, page_size, kv_heads, head_dim, group;
+    const int* table;        // [batch][table_stride] page ids; null: sequence b is page b
+    int table_stride;
+    const int* lens;
+    int len_add;
+    int batch, q_len, window;
+    float scale, soft_cap;
+    // set by the launcher
+    int row_tiles, page_shift;
+    unsigned int* counters;  // zero before and after a call
+    float* part;
+};
+size_t kv4_attention_workspace_bytes(int q_rows, int head_dim, int sms);
+cudaError_t launch_kv4_attention(const Kv4Attn& a, void* workspace, int sms, cudaStream_t stream);
+
+// Logits step (logits.cu).
+struct LogitsArgs {
+    float* out;
+    const void* logits;
+    int type;                // ALJ_KV_F32 / ALJ_KV_BF16
+    int rows, vocab;
+    long long in_stride, out_stride;
+    const int* history;      // [rows][history_stride], history_len[rows] of them live; may be null
+    const int* history_len;
+    int history_stride;
+    const float* penalties;  // [rows][3] repetition, frequency, presence
+    const int* bias_tokens;  // [rows][bias_stride], bias_len[rows] of them live; may be null
+    const float* bias_values;
+    const int* bias_len;
+    int bias_stride;
+    const uint32_t* allow;   // [rows][allow_stride] words, bit t % 32 of word t / 32; may be null
+    int allow_stride;
+    int* token;              // [rows]; may be null
+};
+cudaError_t launch_logits(const LogitsArgs& a, int sms, cudaStream_t stream);
+
 int sm_count_for_current_device();
 
 }  // namespace alj

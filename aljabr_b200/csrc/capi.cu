@@ -559,6 +559,56 @@ int run_attention(DeviceState* st, float* dout, const float* dq, const void* k, 
     return launch_status(launch_attention(p, stream, true), "decode attention");
 }
 
+// Shared checks of the 4-bit KV cache's entry points.
+int kv4_check_cache(int pages, int page_size, int kv_heads, int head_dim) {
+    if (pages < 1 || page_size < 1 || kv_heads < 1 || head_dim < 1)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4: pages=%d page_size=%d kv_heads=%d head_dim=%d", pages, page_size, kv_heads, head_dim);
+    if (!kv4_supported(page_size, kv_heads, head_dim))
+        return fail(ALJ_ERR_UNSUPPORTED, "kv4: head_dim %d (64, 128 or 256), page_size %d (a multiple of 16)", head_dim, page_size);
+    if (static_cast<long long>(pages) * page_size > 0x7fffffffLL || kv_heads > 65536)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4: %d pages of %d positions exceed 2^31 - 1 slots, or %d kv heads", pages, page_size, kv_heads);
+    return ALJ_OK;
+}
+
+int kv4_check_heads(int q_len, int q_heads, int kv_heads, int head_dim) {
+    if (q_len < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: q_len=%d, q_heads=%d must be a positive multiple of kv_heads=%d", q_len,
+                    q_heads, kv_heads);
+    if (!kv4_supported(16, kv_heads, head_dim))
+        return fail(ALJ_ERR_UNSUPPORTED, "kv4_attention: head_dim %d (64, 128 or 256)", head_dim);
+    if (static_cast<long long>(q_len) * (q_heads / kv_heads) > kKv4MaxRows)
+        return fail(ALJ_ERR_UNSUPPORTED, "kv4_attention: q_len * q_heads / kv_heads = %lld rows (at most %d)",
+                    static_cast<long long>(q_len) * (q_heads / kv_heads), kKv4MaxRows);
+    return ALJ_OK;
+}
+
+int kv4_rows(Kv4Rows* p, void* cache, int pages, int page_size, int kv_heads, int head_dim, int type, const int* slots,
+             int tokens, void* k_out, void* v_out) {
+    const int rc = kv4_check_cache(pages, page_size, kv_heads, head_dim);
+    if (rc) return rc;
+    if (type != ALJ_KV_F32 && type != ALJ_KV_BF16)
+        return fail(ALJ_ERR_UNSUPPORTED, "kv4: row type %d (ALJ_KV_F32 or ALJ_KV_BF16)", type);
+    if (tokens < 0 || static_cast<long long>(tokens) * kv_heads * head_dim > (1LL << 38))
+        return fail(ALJ_ERR_BAD_DIMS, "kv4: %d tokens", tokens);
+    if (tokens > 0 && (!cache || !slots)) return fail(ALJ_ERR_BAD_ARG, "kv4: null cache or slots");
+    const uintptr_t out = reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out);
+    if ((reinterpret_cast<uintptr_t>(cache) & 15) || out % (type == ALJ_KV_BF16 ? 2 : 4))
+        return fail(ALJ_ERR_BAD_ARG, "kv4: cache must be 16-byte aligned, rows to their elements");
+    *p = Kv4Rows{};
+    p->cache = static_cast<uint8_t*>(cache);
+    p->pages = pages;
+    p->page_size = page_size;
+    p->kv_heads = kv_heads;
+    p->head_dim = head_dim;
+    p->slots = slots;
+    p->tokens = tokens;
+    p->type = type;
+    p->k_out = k_out;
+    p->v_out = v_out;
+    p->vec_out = (out & 15) == 0;
+    return ALJ_OK;
+}
+
 // The binding's elementwise glue (rmsnorm, silu_ffn): operands that are
 // device, managed or registered memory are used in place; plain host
 // operands are staged through the device scratch.  Blocks until out is
@@ -1314,6 +1364,157 @@ int aljabr_blackwell_decode_attention_dev(float* out, const float* q, const void
     std::lock_guard<std::mutex> g(st->mu);   // the split scratch is shared per device
     return run_attention(st, out, q, k_cache, v_cache, kv_dtype, cache_head_stride, head_dim, kv_heads, q_heads, head_dim,
                          seq_len, start_pos, scale, pick_stream(st, stream), &st->dscratch);
+}
+
+long long aljabr_blackwell_kv4_cache_size(int pages, int page_size, int kv_heads, int head_dim) {
+    const int rc = kv4_check_cache(pages, page_size, kv_heads, head_dim);
+    return rc ? rc : kv4_cache_bytes(pages, page_size, kv_heads, head_dim);
+}
+
+int aljabr_blackwell_kv4_append_dev(void* cache, int pages, int page_size, int kv_heads, int head_dim, const void* k,
+                                    const void* v, int kv_dtype, long long k_stride, long long v_stride,
+                                    const int* slots, int tokens, void* k_back, void* v_back, void* stream) {
+    Kv4Rows p;
+    const int rc = kv4_rows(&p, cache, pages, page_size, kv_heads, head_dim, kv_dtype, slots, tokens, k_back, v_back);
+    if (rc) return rc;
+    if (!k_back != !v_back) return fail(ALJ_ERR_BAD_ARG, "kv4_append: k_back and v_back go together");
+    if (tokens == 0) return ALJ_OK;
+    if (!k || !v) return fail(ALJ_ERR_BAD_ARG, "kv4_append: null k or v");
+    const long long row = static_cast<long long>(kv_heads) * head_dim;
+    if (k_stride < row || v_stride < row)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4_append: strides %lld, %lld < kv_heads * head_dim = %lld", k_stride, v_stride, row);
+    const uintptr_t e = kv_dtype == ALJ_KV_BF16 ? 2 : 4;
+    const uintptr_t kp = reinterpret_cast<uintptr_t>(k), vp = reinterpret_cast<uintptr_t>(v);
+    if ((kp | vp) % e) return fail(ALJ_ERR_BAD_ARG, "kv4_append: k or v not aligned to its elements");
+    p.k = k;
+    p.v = v;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
+    p.vec = ((kp | vp | static_cast<uintptr_t>(k_stride) * e | static_cast<uintptr_t>(v_stride) * e) & 15) == 0;
+    int err = 0;
+    DeviceState* st = state(&err);
+    if (!st) return err;
+    return launch_status(launch_kv4_append(p, pick_stream(st, stream)), "kv4_append");
+}
+
+int aljabr_blackwell_kv4_read_dev(void* k_out, void* v_out, int kv_dtype, const void* cache, int pages, int page_size,
+                                  int kv_heads, int head_dim, const int* slots, int tokens, void* stream) {
+    Kv4Rows p;
+    const int rc = kv4_rows(&p, const_cast<void*>(cache), pages, page_size, kv_heads, head_dim, kv_dtype, slots, tokens,
+                            k_out, v_out);
+    if (rc) return rc;
+    if (tokens == 0) return ALJ_OK;
+    if (!k_out && !v_out) return fail(ALJ_ERR_BAD_ARG, "kv4_read: null k_out and v_out");
+    int err = 0;
+    DeviceState* st = state(&err);
+    if (!st) return err;
+    return launch_status(launch_kv4_read(p, pick_stream(st, stream)), "kv4_read");
+}
+
+long long aljabr_blackwell_kv4_attention_workspace_size(int q_len, int q_heads, int kv_heads, int head_dim) {
+    const int rc = kv4_check_heads(q_len, q_heads, kv_heads, head_dim);
+    if (rc) return rc;
+    const int sms = sm_count_for_current_device();
+    return static_cast<long long>(kv4_attention_workspace_bytes(q_len * (q_heads / kv_heads), head_dim, sms));
+}
+
+int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, long long q_stride, const void* cache,
+                                       int pages, int page_size, int kv_heads, int head_dim, const int* block_table,
+                                       int table_stride, const int* seq_lens, int batch, int q_len, int q_heads,
+                                       int window, float scale, float soft_cap, void* workspace,
+                                       long long workspace_bytes, void* stream) {
+    int rc = kv4_check_cache(pages, page_size, kv_heads, head_dim);
+    if (rc) return rc;
+    rc = kv4_check_heads(q_len, q_heads, kv_heads, head_dim);
+    if (rc) return rc;
+    if (q_dtype != ALJ_KV_F32 && q_dtype != ALJ_KV_BF16)
+        return fail(ALJ_ERR_UNSUPPORTED, "kv4_attention: q type %d (ALJ_KV_F32 or ALJ_KV_BF16)", q_dtype);
+    if (batch < 0 || batch > kKv4MaxBatch)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: batch %d outside [0, %d]", batch, kKv4MaxBatch);
+    if (window < 0) return fail(ALJ_ERR_BAD_ARG, "kv4_attention: window %d < 0", window);
+    if (!(soft_cap >= 0.0f)) return fail(ALJ_ERR_BAD_ARG, "kv4_attention: soft_cap must be >= 0");
+    if (batch == 0) return ALJ_OK;
+    if (!out || !q || !cache || !seq_lens || !workspace) return fail(ALJ_ERR_BAD_ARG, "kv4_attention: null pointer");
+    if (block_table ? table_stride < 1 : batch > pages)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: table_stride %d, batch %d, pages %d", table_stride, batch, pages);
+    const uintptr_t e = q_dtype == ALJ_KV_BF16 ? 2 : 4;
+    if (q_stride < static_cast<long long>(q_heads) * head_dim)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: q_stride %lld < q_heads * head_dim", q_stride);
+    if (reinterpret_cast<uintptr_t>(q) % e || ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(cache)) & 15))
+        return fail(ALJ_ERR_BAD_ARG, "kv4_attention: out and cache must be 16-byte aligned, q to its elements");
+    int err = 0;
+    DeviceState* st = state(&err);
+    if (!st) return err;
+    const size_t need = kv4_attention_workspace_bytes(q_len * (q_heads / kv_heads), head_dim, st->sms);
+    if (workspace_bytes < static_cast<long long>(need) || (reinterpret_cast<uintptr_t>(workspace) & 255))
+        return fail(ALJ_ERR_BAD_ARG, "kv4_attention: workspace %lld bytes (need %zu, 256-byte aligned)", workspace_bytes, need);
+    Kv4Attn a = {};
+    a.out = out;
+    a.q = q;
+    a.q_stride = q_stride;
+    a.type = q_dtype;
+    a.cache = static_cast<const uint8_t*>(cache);
+    a.pages = pages;
+    a.page_size = page_size;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.group = q_heads / kv_heads;
+    a.table = block_table;
+    a.table_stride = table_stride;
+    a.lens = seq_lens;
+    a.batch = batch;
+    a.q_len = q_len;
+    a.window = window;
+    a.scale = scale;
+    a.soft_cap = soft_cap;
+    return launch_status(launch_kv4_attention(a, workspace, st->sms, pick_stream(st, stream)), "kv4_attention");
+}
+
+int aljabr_blackwell_logits_process_dev(float* out, long long out_stride, const void* logits, int logits_dtype,
+                                        long long logits_stride, int rows, int vocab, const int* history,
+                                        const int* history_len, int history_stride, const float* penalties,
+                                        const int* bias_tokens, const float* bias_values, const int* bias_len,
+                                        int bias_stride, const unsigned int* allow, int allow_stride, int* token,
+                                        void* stream) {
+    if (rows < 0 || rows > 65535 || vocab < 1 || vocab > (1 << 28))
+        return fail(ALJ_ERR_BAD_DIMS, "logits_process: rows=%d (0..65535) vocab=%d (1..2^28)", rows, vocab);
+    if (logits_dtype != ALJ_KV_F32 && logits_dtype != ALJ_KV_BF16)
+        return fail(ALJ_ERR_UNSUPPORTED, "logits_process: logits type %d (ALJ_KV_F32 or ALJ_KV_BF16)", logits_dtype);
+    if (out_stride < vocab || logits_stride < vocab)
+        return fail(ALJ_ERR_BAD_DIMS, "logits_process: strides %lld, %lld < vocab %d", out_stride, logits_stride, vocab);
+    if (rows == 0) return ALJ_OK;
+    if (!out || !logits) return fail(ALJ_ERR_BAD_ARG, "logits_process: null out or logits");
+    if (out == logits && (logits_dtype != ALJ_KV_F32 || out_stride != logits_stride))
+        return fail(ALJ_ERR_BAD_ARG, "logits_process: in place needs fp32 logits and equal strides");
+    if (history && (!history_len || !penalties || history_stride < 1))
+        return fail(ALJ_ERR_BAD_ARG, "logits_process: history needs history_len, penalties and history_stride >= 1");
+    if (bias_tokens && (!bias_values || !bias_len || bias_stride < 1))
+        return fail(ALJ_ERR_BAD_ARG, "logits_process: bias_tokens needs bias_values, bias_len and bias_stride >= 1");
+    if (allow && allow_stride < (vocab + 31) / 32)
+        return fail(ALJ_ERR_BAD_DIMS, "logits_process: allow_stride %d < %d words", allow_stride, (vocab + 31) / 32);
+    LogitsArgs a;
+    a.out = out;
+    a.logits = logits;
+    a.type = logits_dtype;
+    a.rows = rows;
+    a.vocab = vocab;
+    a.in_stride = logits_stride;
+    a.out_stride = out_stride;
+    a.history = history;
+    a.history_len = history_len;
+    a.history_stride = history_stride;
+    a.penalties = penalties;
+    a.bias_tokens = bias_tokens;
+    a.bias_values = bias_values;
+    a.bias_len = bias_len;
+    a.bias_stride = bias_stride;
+    a.allow = allow;
+    a.allow_stride = allow_stride;
+    a.token = token;
+    int err = 0;
+    DeviceState* st = state(&err);
+    if (!st) return err;
+    return launch_status(launch_logits(a, st->sms, pick_stream(st, stream)), "logits_process");
 }
 
 int aljabr_blackwell_rmsnorm(float* out, const float* x, const float* weight, int N, float eps) {

@@ -201,7 +201,8 @@ __global__ void swiglu_kernel(const float* gate, float* up, int n) {
 // Split-half RoPE (GGUFVectorOps.rope, GGUFVectorOps.java:383-440) on the
 // rank's q and k heads, then the KV store at `pos`
 // (GgufKvCacheWriteExecution.storeToken).  rope[pos * D/2 + i] holds
-// (cos, sin) of the reference's angle, computed on the host once.
+// (cos, sin) of the reference's angle, computed on the host once.  A 4-bit
+// cache (ALJ_KV_Q4) is written by the append launch that follows.
 __global__ void rope_store_kernel(float* q, float* k, const float* v, void* kc, void* vc, const int* io,
                                   const float2* rope, int hq, int hkv, int D, int kv_dtype) {
     pdl_launch_dependents();
@@ -225,12 +226,13 @@ __global__ void rope_store_kernel(float* q, float* k, const float* v, void* kc, 
             if (kv_dtype == ALJ_KV_BF16) {
                 static_cast<__nv_bfloat16*>(kc)[off] = __float2bfloat16_rn(r0);
                 static_cast<__nv_bfloat16*>(kc)[off + half] = __float2bfloat16_rn(r1);
-            } else {
+            } else if (kv_dtype == ALJ_KV_F32) {
                 static_cast<float*>(kc)[off] = r0;
                 static_cast<float*>(kc)[off + half] = r1;
             }
         }
     }
+    if (kv_dtype == ALJ_KV_Q4) return;
     for (int idx = blockIdx.x * blockDim.x + threadIdx.x; idx < stride; idx += gridDim.x * blockDim.x) {
         const long long off = static_cast<long long>(pos) * stride + idx;
         if (kv_dtype == ALJ_KV_BF16) static_cast<__nv_bfloat16*>(vc)[off] = __float2bfloat16_rn(v[idx]);
@@ -378,7 +380,8 @@ struct DecodeModel {
     bool output_set = false;
     float* norms = nullptr;            // [layers][2][H] then [H]
     float2* rope = nullptr;            // [max_ctx][D/2] (cos, sin)
-    void *kc = nullptr, *vc = nullptr; // [layers][max_ctx][hkv*D]
+    void *kc = nullptr, *vc = nullptr; // [layers][max_ctx][hkv*D]; 4-bit: kc holds [layers] caches of one page
+    void* kv4_work = nullptr;          // workspace of the 4-bit cache's attention
     float *x, *xn, *q, *k, *vv, *att_l, *att, *delta_l, *delta, *h_l, *hh, *logits_l, *logits, *scratch;
     float* norm_partials = nullptr;    // [matvec_max_ctas()] per-CTA sums of squares
     bool defer_norm = false;           // RMSNorm scale applied by the consuming matvec (one GPU)
@@ -405,6 +408,10 @@ struct DecodeModel {
            arena_bytes = 0;
     std::mutex mu;
 
+    // a 4-bit cache is one page of max_ctx positions, rounded up to the tile of 16
+    bool kv4() const { return kv_dtype == ALJ_KV_Q4; }
+    int kv4_page() const { return (max_ctx + 15) / 16 * 16; }
+    size_t kv4_layer_bytes() const { return static_cast<size_t>(kv4_cache_bytes(1, kv4_page(), hkv, D)); }
     size_t kv_elem() const { return kv_dtype == ALJ_KV_BF16 ? 2 : 4; }
     size_t kv_layer_elems() const { return static_cast<size_t>(max_ctx) * hkv * D; }
 };
@@ -517,6 +524,48 @@ bool typed_fusable(const DecodeModel& m) {
     return ok(m.head, m.H, m.v);
 }
 
+// One layer's 4-bit cache as the arguments of its row kernels: fp32 rows.
+Kv4Rows kv4_layer_rows(const DecodeModel& m, int layer, const int* slots, int tokens) {
+    Kv4Rows r = {};
+    r.cache = static_cast<uint8_t*>(m.kc) + static_cast<size_t>(layer) * m.kv4_layer_bytes();
+    r.pages = 1;
+    r.page_size = m.kv4_page();
+    r.kv_heads = m.hkv;
+    r.head_dim = m.D;
+    r.slots = slots;
+    r.tokens = tokens;
+    r.type = ALJ_KV_F32;
+    r.k_stride = r.v_stride = static_cast<long long>(m.hkv) * m.D;
+    r.vec = r.vec_out = 1;
+    return r;
+}
+
+// The layer's new K and V into its 4-bit cache at *io (the position is the
+// slot), then attention over [0, *io].
+cudaError_t record_kv4_attention(DecodeModel& m, int layer, int sms) {
+    Kv4Rows r = kv4_layer_rows(m, layer, m.io, 1);
+    r.k = m.k;
+    r.v = m.vv;
+    REC(launch_kv4_append(r, m.stream));
+    Kv4Attn a = {};
+    a.out = m.att;
+    a.q = m.q;
+    a.q_stride = static_cast<long long>(m.hq) * m.D;
+    a.type = ALJ_KV_F32;
+    a.cache = r.cache;
+    a.pages = 1;
+    a.page_size = r.page_size;
+    a.kv_heads = m.hkv;
+    a.head_dim = m.D;
+    a.group = m.hq / m.hkv;
+    a.lens = m.io;
+    a.len_add = 1;
+    a.batch = 1;
+    a.q_len = 1;
+    a.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(m.D)));
+    return launch_kv4_attention(a, m.kv4_work, sms, m.stream);
+}
+
 cudaError_t record_step(DecodeModel& m) {
     if (m.typed) m.defer_norm = typed_fusable(m);
     const int D = m.D;
@@ -545,7 +594,9 @@ cudaError_t record_step(DecodeModel& m) {
         REC(launch_small(rope_store_kernel, std::max(1, ((m.hq + m.hkv) * D / 2 + 255) / 256), 256, m.stream, m.q,
                          m.k, static_cast<const float*>(m.vv), kc, vc, static_cast<const int*>(m.io),
                          static_cast<const float2*>(m.rope), m.hq, m.hkv, D, m.kv_dtype));
-        {   // attention (GgufDecodePass.java:368-389)
+        if (m.kv4()) {
+            REC(record_kv4_attention(m, l, sms));
+        } else {   // attention (GgufDecodePass.java:368-389)
             AttnParams a = {};
             a.out = m.T > 1 ? m.att_l : m.att;
             a.q = m.q;
@@ -850,6 +901,58 @@ bool setup_p2p(DecodeModel* m) {
     return true;
 }
 
+// Device rows [n][hkv * D] of K and of V and the slots 0 .. n - 1, for moving
+// fp32 rows into and out of a layer's 4-bit cache.
+struct Kv4Staging {
+    float *k = nullptr, *v = nullptr;
+    int* slots = nullptr;
+    ~Kv4Staging() {
+        cudaFree(k);
+        cudaFree(v);
+        cudaFree(slots);
+    }
+    cudaError_t make(const DecodeModel& m, int n) {
+        const size_t bytes = static_cast<size_t>(n) * m.hkv * m.D * 4;
+        std::vector<int> at(n);
+        for (int i = 0; i < n; ++i) at[i] = i;
+        REC(cudaMalloc(&k, bytes));
+        REC(cudaMalloc(&v, bytes));
+        REC(cudaMalloc(&slots, n * sizeof(int)));
+        REC(cudaMemcpyAsync(slots, at.data(), n * sizeof(int), cudaMemcpyHostToDevice, m.stream));
+        return cudaStreamSynchronize(m.stream);
+    }
+};
+
+cudaError_t sync_kv4(DecodeModel& m, int layer, int seq_len, const void* k, const void* v) {
+    Kv4Staging st;
+    REC(st.make(m, seq_len));
+    const size_t bytes = static_cast<size_t>(seq_len) * m.hkv * m.D * 4;
+    REC(cudaMemcpyAsync(st.k, k, bytes, cudaMemcpyDefault, m.stream));
+    REC(cudaMemcpyAsync(st.v, v, bytes, cudaMemcpyDefault, m.stream));
+    Kv4Rows r = kv4_layer_rows(m, layer, st.slots, seq_len);
+    r.k = st.k;
+    r.v = st.v;
+    REC(launch_kv4_append(r, m.stream));
+    return cudaStreamSynchronize(m.stream);
+}
+
+// Every layer's [max_ctx][hkv * D] values, fp32, to host memory.
+cudaError_t read_kv4(DecodeModel& m, float* k_out, float* v_out) {
+    Kv4Staging st;
+    REC(st.make(m, m.max_ctx));
+    const size_t elems = m.kv_layer_elems();
+    for (int l = 0; l < m.layers; ++l) {
+        Kv4Rows r = kv4_layer_rows(m, l, st.slots, m.max_ctx);
+        r.k_out = st.k;
+        r.v_out = st.v;
+        REC(launch_kv4_read(r, m.stream));
+        if (k_out) REC(cudaMemcpyAsync(k_out + l * elems, st.k, elems * 4, cudaMemcpyDeviceToHost, m.stream));
+        if (v_out) REC(cudaMemcpyAsync(v_out + l * elems, st.v, elems * 4, cudaMemcpyDeviceToHost, m.stream));
+        REC(cudaStreamSynchronize(m.stream));
+    }
+    return cudaSuccess;
+}
+
 void destroy(DecodeModel* m) {
     cudaSetDevice(m->device);
     if (m->stream) cudaStreamSynchronize(m->stream);
@@ -860,6 +963,7 @@ void destroy(DecodeModel* m) {
     if (m->comm) g_nccl.commDestroy(m->comm);
     cudaFree(m->kc);
     cudaFree(m->vc);
+    cudaFree(m->kv4_work);
     cudaFree(m->act_base);
     cudaFree(m->norms);
     cudaFree(m->rope);
@@ -911,7 +1015,9 @@ int aljabr_blackwell_decode_model_create(const int* dims, float eps, float rope_
     if (m->H % 256 || m->F % 256 || (m->Hq * m->D) % 256 || !matvec_tma_supported(FMT_NF4, m->H, m->group) ||
         !matvec_tma_supported(FMT_NF4, m->F, m->group) || !matvec_tma_supported(FMT_NF4, m->Hq * m->D, m->group))
         return decode_fail(ALJ_ERR_UNSUPPORTED, "decode step needs hidden, ffn, heads*head_dim multiples of 256 and NF4 group 64/128");
-    if (m->kv_dtype != ALJ_KV_BF16 && m->kv_dtype != ALJ_KV_F32) return decode_fail(ALJ_ERR_UNSUPPORTED, "kv dtype");
+    if (m->kv_dtype != ALJ_KV_BF16 && m->kv_dtype != ALJ_KV_F32 && m->kv_dtype != ALJ_KV_Q4)
+        return decode_fail(ALJ_ERR_UNSUPPORTED, "kv dtype");
+    if (m->kv4() && T > 1) return decode_fail(ALJ_ERR_UNSUPPORTED, "the 4-bit KV cache needs tp_world 1");
     const int G = m->Hq / m->Hkv;
     if (!(m->D == 64 || m->D == 128 || m->D == 256) || !(G == 1 || G == 2 || G == 4 || G == 8))
         return decode_fail(ALJ_ERR_UNSUPPORTED, "decode attention needs head_dim 64/128/256 and group 1/2/4/8");
@@ -929,12 +1035,16 @@ int aljabr_blackwell_decode_model_create(const int* dims, float eps, float rope_
                     matvec_lut_supported(FMT_NF4, m->F, m->group);
 
     auto ok = [&](cudaError_t e) { return e == cudaSuccess; };
-    const size_t kvb = static_cast<size_t>(m->layers) * m->kv_layer_elems() * m->kv_elem();
+    const size_t kvb = m->kv4() ? m->layers * m->kv4_layer_bytes()
+                                : static_cast<size_t>(m->layers) * m->kv_layer_elems() * m->kv_elem();
+    const size_t vcb = m->kv4() ? 0 : kvb;
+    const size_t k4w = m->kv4() ? kv4_attention_workspace_bytes(G, m->D, sm_count_for_current_device()) : 0;
     const size_t acts = static_cast<size_t>(m->H) + m->hq * m->D + 2 * m->hkv * m->D + m->hq * m->D + m->Hq * m->D +
                         m->h + m->H + m->f + m->F + m->v + m->V + m->H + matvec_max_ctas() + 4 +
                         attention_scratch_floats(m->hq, m->D, m->splits) + 64;
     if (!ok(cudaStreamCreateWithFlags(&m->stream, cudaStreamNonBlocking)) || !ok(cudaMalloc(&m->kc, kvb)) ||
-        !ok(cudaMalloc(&m->vc, kvb)) || !ok(cudaMalloc(&m->act_base, acts * 4)) ||
+        (vcb && !ok(cudaMalloc(&m->vc, vcb))) || (k4w && !ok(cudaMalloc(&m->kv4_work, k4w))) ||
+        !ok(cudaMalloc(&m->act_base, acts * 4)) ||
         !ok(cudaMalloc(&m->norms, (static_cast<size_t>(m->layers) * 2 + 1) * m->H * 4)) ||
         !ok(cudaMalloc(&m->io, 8 * sizeof(int))) || !ok(cudaMallocHost(&m->host_io, 8 * sizeof(int))) ||
         !ok(cudaMalloc(&m->rope, static_cast<size_t>(m->max_ctx) * (m->D / 2) * sizeof(float2))) ||
@@ -945,7 +1055,8 @@ int aljabr_blackwell_decode_model_create(const int* dims, float eps, float rope_
         return decode_fail(ALJ_ERR_NO_MEMORY, "allocating the decode model's KV cache / activations failed");
     }
     cudaMemsetAsync(m->kc, 0, kvb, m->stream);
-    cudaMemsetAsync(m->vc, 0, kvb, m->stream);
+    if (vcb) cudaMemsetAsync(m->vc, 0, vcb, m->stream);
+    if (k4w) cudaMemsetAsync(m->kv4_work, 0, k4w, m->stream);   // arrival counters
     cudaMemsetAsync(m->act_base, 0, acts * 4, m->stream);
     {
         // RoPE angle table exactly as GGUFVectorOps.rope (GGUFVectorOps.java:425-431):
@@ -1178,6 +1289,13 @@ int aljabr_blackwell_sync_kv_cache(unsigned long long handle, int layer, int seq
     if (!k || !v) return decode_fail(ALJ_ERR_BAD_ARG, "null K or V");
     std::lock_guard<std::mutex> g(m->mu);
     cudaSetDevice(m->device);
+    if (m->kv4()) {
+        if (seq_len == 0) return ALJ_OK;
+        const cudaError_t e4 = sync_kv4(*m, layer, seq_len, k, v);
+        if (e4 == cudaErrorMemoryAllocation) return decode_fail(ALJ_ERR_NO_MEMORY, "staging the rows of the 4-bit cache failed");
+        if (e4 != cudaSuccess) return decode_fail(ALJ_ERR_CUDA, cudaGetErrorString(e4));
+        return ALJ_OK;
+    }
     const size_t bytes = static_cast<size_t>(seq_len) * m->hkv * m->D * m->kv_elem();
     const size_t off = static_cast<size_t>(layer) * m->kv_layer_elems() * m->kv_elem();
     cudaError_t e = cudaMemcpyAsync(static_cast<uint8_t*>(m->kc) + off, k, bytes, cudaMemcpyDefault, m->stream);
@@ -1194,10 +1312,25 @@ int aljabr_blackwell_decode_read_state(unsigned long long handle, float* x_out, 
     cudaSetDevice(m->device);
     const size_t kvb = static_cast<size_t>(m->layers) * m->kv_layer_elems() * m->kv_elem();
     cudaError_t e = cudaStreamSynchronize(m->stream);
+    if (e == cudaSuccess && m->kv4() && (k_cache_out || v_cache_out)) {
+        e = read_kv4(*m, static_cast<float*>(k_cache_out), static_cast<float*>(v_cache_out));
+        if (e == cudaErrorMemoryAllocation) return decode_fail(ALJ_ERR_NO_MEMORY, "staging the rows of the 4-bit cache failed");
+        k_cache_out = v_cache_out = nullptr;
+    }
     if (e == cudaSuccess && x_out) e = cudaMemcpy(x_out, m->x, static_cast<size_t>(m->H) * 4, cudaMemcpyDeviceToHost);
     if (e == cudaSuccess && k_cache_out) e = cudaMemcpy(k_cache_out, m->kc, kvb, cudaMemcpyDeviceToHost);
     if (e == cudaSuccess && v_cache_out) e = cudaMemcpy(v_cache_out, m->vc, kvb, cudaMemcpyDeviceToHost);
     if (e != cudaSuccess) return decode_fail(ALJ_ERR_CUDA, cudaGetErrorString(e));
+    return ALJ_OK;
+}
+
+int aljabr_blackwell_decode_logits(unsigned long long handle, const float** logits) {
+    DecodeModel* m = find(handle);
+    if (!m) return decode_fail(ALJ_ERR_BAD_ARG, "unknown decode model handle");
+    if (!logits) return decode_fail(ALJ_ERR_BAD_ARG, "null logits");
+    std::lock_guard<std::mutex> g(m->mu);
+    if (m->steps_run == 0) return decode_fail(ALJ_ERR_NOT_INITIALIZED, "no step has run");
+    *logits = m->logits;
     return ALJ_OK;
 }
 

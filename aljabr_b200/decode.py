@@ -142,6 +142,47 @@ class LlamaNf4Decoder:
                     out.ctypes.data)
         return out
 
+    def generate(self, token: int, pos: int, n_tokens: int, history=(), penalties=(1.0, 0.0, 0.0), bias=None,
+                 allow=None) -> np.ndarray:
+        """Greedy decode of n_tokens with the logits step between tokens: repetition / frequency / presence
+        penalties over `history` and everything emitted so far, `bias` ({token: value}), and `allow`, which gives
+        the grammar's words (uint32, bit t % 32 of word t / 32) for the tokens emitted so far, or None.  Stops
+        early when the grammar allows nothing.  Runs on cache and logits where they are (kv_dtype KV_Q4 too)."""
+        import torch
+        from .kv4 import current_stream
+        dev, V = torch.device("cuda", torch.cuda.current_device()), self.shape.vocab
+        hist = torch.zeros(1, max(1, len(history) + n_tokens + 1), dtype=torch.int32, device=dev)
+        seen = list(history) + [token]
+        hist[0, :len(seen)] = torch.tensor(seen, dtype=torch.int32)
+        live = torch.zeros(1, dtype=torch.int32, device=dev)
+        pen = torch.tensor([penalties], dtype=torch.float32, device=dev)
+        out, best = torch.empty(V, dtype=torch.float32, device=dev), torch.empty(1, dtype=torch.int32, device=dev)
+        bt = bv = bl = words = None
+        if bias:
+            bt = torch.tensor(list(bias), dtype=torch.int32, device=dev)
+            bv = torch.tensor(list(bias.values()), dtype=torch.float32, device=dev)
+            bl = torch.tensor([len(bias)], dtype=torch.int32, device=dev)
+        ptr = (lambda t: None if t is None else t.data_ptr())
+        logits, emitted = ctypes.c_void_p(), []
+        for i in range(n_tokens):
+            self.step(token, pos + i)
+            if i == 0:
+                native.call("aljabr_blackwell_decode_logits", ctypes.c_ulonglong(self.handle), ctypes.byref(logits))
+            if allow is not None:
+                words = torch.from_numpy(np.ascontiguousarray(allow(emitted), dtype=np.uint32).view(np.int32)).to(dev)
+            live.fill_(len(seen))
+            native.call("aljabr_blackwell_logits_process_dev", out.data_ptr(), V, logits, native.KV_F32, V, 1, V,
+                        hist.data_ptr(), live.data_ptr(), hist.shape[1], pen.data_ptr(), ptr(bt), ptr(bv), ptr(bl),
+                        0 if bt is None else bt.numel(), ptr(words), 0 if words is None else words.numel(),
+                        best.data_ptr(), current_stream(dev))
+            token = int(best)
+            if token < 0:
+                break
+            hist[0, len(seen)] = token
+            seen.append(token)
+            emitted.append(token)
+        return np.array(emitted, np.int32)
+
     def read_state(self):
         s = self.shape
         kv_heads = s.kv_heads // self.tp_world

@@ -1,0 +1,155 @@
+"""The 4-bit KV cache (aljabr_blackwell_kv4_*): quantise rows as they are
+written, read them back, and attend over them.
+
+A cache is a pool of pages; a sequence owns pages through a block table, or
+one page of max_ctx positions each (no table).  The serving loop of one layer:
+
+    cache = Kv4Cache(pages, page_size, kv_heads, head_dim)
+    cache.append(k, v, slots)                      # new rows -> 4 bits
+    out = cache.attend(q, seq_lens, block_table)   # q: [batch, q_len, q_heads, head_dim]
+
+Tensors are torch CUDA tensors on the cache's device; every call is ordered on
+torch's current stream of that device (or `stream`, a raw cudaStream_t).  The
+layout and the arithmetic are described in include/aljabr_blackwell.h.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import native
+
+_DTYPES = {torch.float32: native.KV_F32, torch.bfloat16: native.KV_BF16}
+_LEGACY_STREAM = 1      # cudaStreamLegacy: the C-ABI reads 0 as "the library's own stream"
+
+
+def current_stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream or _LEGACY_STREAM
+
+
+def dtype_id(t: torch.Tensor, what: str) -> int:
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        raise native.UnsupportedOperation(native.ALJ_ERR_UNSUPPORTED, f"{what} is {t.dtype}: float32 or bfloat16")
+    return d
+
+
+def bad(message: str) -> native.ProviderError:
+    return native.ProviderError(native.ALJ_ERR_BAD_ARG, message)
+
+
+class Kv4Cache:
+    """`pages` pages of `page_size` positions of `kv_heads` heads in 4 bits.
+
+    `data`: uint8 storage to use (for example another process's or layer's
+    share of one allocation); a zeroed buffer is allocated without it.
+    """
+
+    def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, device="cuda", data=None):
+        size = native.lib().aljabr_blackwell_kv4_cache_size(pages, page_size, kv_heads, head_dim)
+        if size < 0:
+            native.check(int(size))
+        if data is None:
+            data = torch.zeros(size, dtype=torch.uint8, device=device)
+        if data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() < size or data.device.type != "cuda":
+            raise bad(f"cache data must be {size} contiguous uint8 on a CUDA device")
+        self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
+        self.data, self.device, self.bytes = data, data.device, size
+        native.call("aljabr_blackwell_init", self.device.index or 0)
+        self._shape = (data.data_ptr(), pages, page_size, kv_heads, head_dim)
+        self._work = {}      # stream -> (workspace, bytes): calls on one stream never overlap
+
+    # -- checks ----------------------------------------------------------------
+    def _rows(self, t: torch.Tensor, tokens: int, what: str) -> int:
+        """Elements between the rows of t: [tokens, kv_heads, head_dim] or [tokens, kv_heads * head_dim]."""
+        row = self.kv_heads * self.head_dim
+        if t.device != self.device or t.dim() not in (2, 3) or t.shape[0] != tokens or t[0:1].numel() != row * min(tokens, 1):
+            raise bad(f"{what} must be [{tokens}, {self.kv_heads}, {self.head_dim}] on {self.device}, not {tuple(t.shape)}")
+        st = t.stride()
+        if st[-1] != 1 or (t.dim() == 3 and st[1] != self.head_dim and self.kv_heads > 1):
+            raise bad(f"{what}: the heads of a row must be contiguous (strides {st})")
+        return st[0] if tokens > 1 else row
+
+    def _ints(self, t: torch.Tensor, shape: tuple, what: str) -> int:
+        if t.dtype != torch.int32 or t.device != self.device or tuple(t.shape) != shape or not t.is_contiguous():
+            raise bad(f"{what} must be contiguous int32 {shape} on {self.device}")
+        return t.data_ptr()
+
+    def _dense(self, t, tokens: int, dtype, what: str):
+        if t is None:
+            return None
+        if t.dtype != dtype or not t.is_contiguous() or t.device != self.device or \
+                t.numel() != tokens * self.kv_heads * self.head_dim:
+            raise bad(f"{what} must be contiguous {dtype} [{tokens}, {self.kv_heads}, {self.head_dim}] on {self.device}")
+        return t.data_ptr()
+
+    # -- rows ------------------------------------------------------------------
+    def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_back=None, v_back=None, stream=None):
+        """Quantise the rows k, v into slots[i] = page * page_size + position (-1: skip the row).
+
+        k_back / v_back (both or neither) receive the values the cache now holds."""
+        n = slots.shape[0]
+        kind = dtype_id(k, "k")
+        if v.dtype != k.dtype:
+            raise bad(f"k is {k.dtype}, v is {v.dtype}")
+        ks, vs = self._rows(k, n, "k"), self._rows(v, n, "v")
+        native.call("aljabr_blackwell_kv4_append_dev", *self._shape, k.data_ptr(), v.data_ptr(), kind, ks, vs,
+                    self._ints(slots, (n,), "slots"), n, self._dense(k_back, n, k.dtype, "k_back"),
+                    self._dense(v_back, n, k.dtype, "v_back"), stream or current_stream(self.device))
+
+    def read(self, slots: torch.Tensor, dtype=torch.float32, k_out=None, v_out=None, stream=None):
+        """Rows of the given slots as (k, v), [n, kv_heads, head_dim] each; zeros where a slot is -1."""
+        n = slots.shape[0]
+        if k_out is None and v_out is None:
+            k_out, v_out = (torch.empty(n, self.kv_heads, self.head_dim, dtype=dtype, device=self.device) for _ in range(2))
+        some = k_out if k_out is not None else v_out
+        native.call("aljabr_blackwell_kv4_read_dev", self._dense(k_out, n, some.dtype, "k_out"),
+                    self._dense(v_out, n, some.dtype, "v_out"), dtype_id(some, "k_out"), *self._shape,
+                    self._ints(slots, (n,), "slots"), n, stream or current_stream(self.device))
+        return k_out, v_out
+
+    # -- attention -------------------------------------------------------------
+    def _workspace(self, q_len: int, q_heads: int, stream: int):
+        need = native.lib().aljabr_blackwell_kv4_attention_workspace_size(q_len, q_heads, self.kv_heads, self.head_dim)
+        if need < 0:
+            native.check(int(need))
+        have = self._work.get(stream)
+        if have is None or have[1] < need:
+            # zeroed on torch's current stream; another stream's kernels neither wait for that nor hold the
+            # old buffer, so there the device is waited for, once
+            new = (torch.zeros(need, dtype=torch.uint8, device=self.device), need)
+            if stream != current_stream(self.device):
+                torch.cuda.synchronize(self.device)
+            have = self._work[stream] = new
+        return have
+
+    def attend(self, q: torch.Tensor, seq_lens: torch.Tensor, block_table=None, window: int = 0, scale=None,
+               soft_cap: float = 0.0, out=None, stream=None) -> torch.Tensor:
+        """Attention of q [batch, q_len, q_heads, head_dim], whose rows are the last q_len of seq_lens[b] positions.
+
+        block_table: int32 [batch, pages a sequence], or None where sequence b is page b.  scale: 1 / sqrt(head_dim)
+        by default.  Returns out, contiguous, of q's type."""
+        if q.dim() != 4 or q.shape[3] != self.head_dim or q.device != self.device:
+            raise bad(f"q must be [batch, q_len, q_heads, {self.head_dim}] on {self.device}, not {tuple(q.shape)}")
+        batch, q_len, q_heads, D = q.shape
+        st = q.stride()
+        row = q_heads * D
+        q_stride = st[1] if q_len > 1 else st[0] if batch > 1 else row
+        if st[3] != 1 or (q_heads > 1 and st[2] != D) or (q_len > 1 and batch > 1 and st[0] != q_len * st[1]):
+            raise bad(f"q: the heads of a token must be contiguous and the tokens evenly spaced (strides {st})")
+        kind = dtype_id(q, "q")
+        if out is None:
+            out = torch.empty(batch, q_len, q_heads, D, dtype=q.dtype, device=self.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous():
+            raise bad(f"out must be contiguous {q.dtype} {tuple(q.shape)} on {self.device}")
+        table, width = None, 0
+        if block_table is not None:
+            width = block_table.shape[-1]
+            table = self._ints(block_table, (batch, width), "block_table")
+        stream = stream or current_stream(self.device)
+        work, size = self._workspace(q_len, q_heads, stream)
+        native.call("aljabr_blackwell_kv4_attention_dev", out.data_ptr(), q.data_ptr(), kind, q_stride, *self._shape,
+                    table, width, self._ints(seq_lens, (batch,), "seq_lens"), batch, q_len, q_heads, window,
+                    1.0 / math.sqrt(D) if scale is None else scale, soft_cap, work.data_ptr(), size, stream)
+        return out

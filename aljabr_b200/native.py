@@ -32,6 +32,7 @@ TYPE_Q4_K = 12
 TYPE_Q6_K = 14
 KV_F32 = 0
 KV_BF16 = 1
+KV_Q4 = 2
 
 
 class ProviderError(RuntimeError):
@@ -103,6 +104,14 @@ SIGNATURES = {
     "aljabr_blackwell_gemm_q_pack": (_i, [_i, _p, _p, _i, _i, _p]),
     "aljabr_blackwell_gemm_q_workspace_size": (_ll, [_i, _i]),
     "aljabr_blackwell_gemm_q_dev": (_i, [_i, _i, _p, _p, _p, _p, _p, _i, _i, _p, _ll, _p]),
+    "aljabr_blackwell_kv4_cache_size": (_ll, [_i, _i, _i, _i]),
+    "aljabr_blackwell_kv4_append_dev": (_i, [_p, _i, _i, _i, _i, _p, _p, _i, _ll, _ll, _p, _i, _p, _p, _p]),
+    "aljabr_blackwell_kv4_read_dev": (_i, [_p, _p, _i, _p, _i, _i, _i, _i, _p, _i, _p]),
+    "aljabr_blackwell_kv4_attention_workspace_size": (_ll, [_i, _i, _i, _i]),
+    "aljabr_blackwell_kv4_attention_dev": (_i, [_p, _p, _i, _ll, _p, _i, _i, _i, _i, _p, _i, _p, _i, _i, _i, _i, _f, _f,
+                                                _p, _ll, _p]),
+    "aljabr_blackwell_logits_process_dev": (_i, [_p, _ll, _p, _i, _ll, _i, _i, _p, _p, _i, _p, _p, _p, _p, _i, _p, _i,
+                                                 _p, _p]),
     "aljabr_blackwell_nccl_unique_id": (_i, [_p, _i]),
     "aljabr_blackwell_decode_model_create": (_i, [ctypes.POINTER(_i), _f, _f, _i, _i, _p,
                                                   ctypes.POINTER(ctypes.c_ulonglong)]),
@@ -114,6 +123,7 @@ SIGNATURES = {
     "aljabr_blackwell_decode_run": (_i, [ctypes.c_ulonglong, _i, _i, _i, _p]),
     "aljabr_blackwell_sync_kv_cache": (_i, [ctypes.c_ulonglong, _i, _i, _p, _p]),
     "aljabr_blackwell_decode_read_state": (_i, [ctypes.c_ulonglong, _p, _p, _p]),
+    "aljabr_blackwell_decode_logits": (_i, [ctypes.c_ulonglong, _p]),
     "aljabr_blackwell_decode_model_destroy": (_i, [ctypes.c_ulonglong]),
 }
 

@@ -76,6 +76,7 @@ extern "C" {
 /* ---- KV-cache element types --------------------------------------------- */
 #define ALJ_KV_F32  0   /* the reference's fp32 cache (KVCache.java:22-23)  */
 #define ALJ_KV_BF16 1   /* bf16 cache (half the bytes)                      */
+#define ALJ_KV_Q4   2   /* 4-bit cache (see "4-bit KV cache"); decode models */
 
 /* ---- lifecycle (BlackwellBinding.java:52-78 names) ----------------------- */
 /* Select `device_id` for the calling thread and create its state.  Replaces
@@ -322,6 +323,87 @@ int aljabr_blackwell_gemm_q_dev(int type, int nseg, float* const* y, const int* 
                                 const int* rows, const float* x, int M, int K, void* workspace,
                                 long long workspace_bytes, void* stream);
 
+/* ---- 4-bit KV cache --------------------------------------------------------
+ * No counterpart in the reference, whose caches are fp32.  A cache is one
+ * device buffer of `pages` pages of `page_size` positions (a multiple of 16;
+ * pages * page_size < 2^31), kv4_cache_size bytes, 16-byte aligned.  head_dim
+ * D is 64, 128 or 256.  Values are kept in groups of 32 along D as
+ * d * (c - 8), d fp16, c a 4-bit code (4.5 bits a value, the Q4_0 arithmetic):
+ *   ext = the extreme of larger magnitude (the negative one on a tie),
+ *   d   = fp16(ext / -8), saturated at +-65504; NaN if the group holds a NaN
+ *         or an infinity (the group then reads back as NaN),
+ *   c   = clamp(rint(x * (1 / d)) + 8, 0, 15), ties to even; d = 0: c = 8.
+ * Layout of a page, for each kv head in turn, with NG = D / 32:
+ *   K codes  [page_size][D / 2]: word (c, g), c < 4, at byte 4 (c NG + g),
+ *            dims 32 g + 8 c + i in bits 4 i;
+ *   V codes  [page_size][D / 2]: halfword (r, g), r < 8, at byte 2 (r NG + g),
+ *            dims 32 g + 4 r + i in bits 4 i;
+ *   K scales [page_size][NG] fp16, then V scales [page_size][NG] fp16.
+ *
+ * kv4_append_dev writes `tokens` rows of K and V (kv_dtype ALJ_KV_F32 or
+ * ALJ_KV_BF16, [kv_heads * head_dim] each, k_stride / v_stride elements
+ * apart, so columns of a fused q|k|v buffer will do) at slots[i] = page *
+ * page_size + position (device int32; -1 skips the row; a slot must not occur
+ * twice in a call).  k_back / v_back, both or neither, receive the values the
+ * cache now holds, [tokens][kv_heads * head_dim] of kv_dtype (zeros for
+ * skipped rows): the rows for a prompt's own attention, so that it sees what
+ * later tokens will see.
+ * kv4_read_dev reads rows back the same way (zeros for -1); either output may
+ * be NULL.
+ * kv4_attention_dev: q_len query tokens (usually 1) of each of `batch`
+ * sequences attend over the cache; q and out are q_dtype (ALJ_KV_F32 /
+ * ALJ_KV_BF16), q rows [q_heads * head_dim] q_stride elements apart, out
+ * [batch][q_len][q_heads * head_dim], 16-byte aligned.  seq_lens[b] (device)
+ * counts the cached positions with the q_len new ones, which are appended
+ * before the call: query t sees positions up to seq_lens[b] - q_len + t,
+ * with window > 0 only the last `window` of them; a query that sees nothing
+ * is zero.  Position p of sequence b is at block_table[b * table_stride + p /
+ * page_size] (device), or with block_table NULL in page b.  soft_cap > 0
+ * applies tanh(s / cap) * cap to the scaled scores.  fp32 queries are
+ * computed to fp32 accuracy, bf16 ones to bf16's.  q_len * q_heads / kv_heads
+ * is at most 1024, batch at most 2048.  The results do not depend on timing.
+ * workspace: kv4_attention_workspace_size bytes of device memory, 256-byte
+ * aligned, used by one call at a time; its first kilobytes are arrival
+ * counters that must be zero before the first call and are zero after each.
+ * On the device, slots, page ids and lengths outside the cache are not
+ * followed: the row or page counts as absent (zeros), a length is cut, and
+ * bit 1 of aljabr_blackwell_device_status is set.
+ * All are stream-ordered (NULL = the library's stream) and allocate nothing. */
+long long aljabr_blackwell_kv4_cache_size(int pages, int page_size, int kv_heads, int head_dim);
+int aljabr_blackwell_kv4_append_dev(void* cache, int pages, int page_size, int kv_heads, int head_dim, const void* k,
+                                    const void* v, int kv_dtype, long long k_stride, long long v_stride,
+                                    const int* slots, int tokens, void* k_back, void* v_back, void* stream);
+int aljabr_blackwell_kv4_read_dev(void* k_out, void* v_out, int kv_dtype, const void* cache, int pages, int page_size,
+                                  int kv_heads, int head_dim, const int* slots, int tokens, void* stream);
+long long aljabr_blackwell_kv4_attention_workspace_size(int q_len, int q_heads, int kv_heads, int head_dim);
+int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, long long q_stride, const void* cache,
+                                       int pages, int page_size, int kv_heads, int head_dim, const int* block_table,
+                                       int table_stride, const int* seq_lens, int batch, int q_len, int q_heads,
+                                       int window, float scale, float soft_cap, void* workspace,
+                                       long long workspace_bytes, void* stream);
+
+/* ---- logits step -----------------------------------------------------------
+ * For each of `rows` rows of `vocab` logits (ALJ_KV_F32 or ALJ_KV_BF16, rows
+ * logits_stride elements apart), into out (fp32; may be `logits` itself):
+ *   for tokens in the row's history, n times: l = l > 0 ? l / rep : l * rep,
+ *     then l = (l - freq * n) - pres, with {rep, freq, pres} = penalties[row];
+ *   l = l + bias for the row's listed tokens (a token listed more than once
+ *     gets the sum of its entries);
+ *   l = -inf where the row's `allow` bit (bit t % 32 of word t / 32) is 0;
+ *   token[row] = the lowest index of the largest value.  NaN never wins; -1
+ *     if no token is allowed or all allowed ones are NaN.
+ * history [rows][history_stride] with history_len[row] live entries, entries
+ * outside [0, vocab) ignored; bias_tokens / bias_values [rows][bias_stride]
+ * with bias_len[row]; allow [rows][allow_stride words].  history, bias_tokens,
+ * allow and token may each be NULL.  Device pointers, stream-ordered.  No
+ * counterpart in the reference's native code: its samplers run on the host. */
+int aljabr_blackwell_logits_process_dev(float* out, long long out_stride, const void* logits, int logits_dtype,
+                                        long long logits_stride, int rows, int vocab, const int* history,
+                                        const int* history_len, int history_stride, const float* penalties,
+                                        const int* bias_tokens, const float* bias_values, const int* bias_len,
+                                        int bias_stride, const unsigned int* allow, int allow_stride, int* token,
+                                        void* stream);
+
 /* Same computation as aljabr_blackwell_decode_attention_dev, for callers that
  * may not allocate device memory at call time.  No counterpart in the
  * reference: its attention runs on the host and needs no device scratch.
@@ -352,7 +434,9 @@ int aljabr_blackwell_decode_attention_noalloc(float* out, const float* q, const 
  * models can coexist.
  *
  * dims = {layers, hidden, q_heads, kv_heads, head_dim, ffn, vocab, max_ctx,
- *         nf4_group, kv_dtype}.  With tp_world > 1 every weight passed in is
+ *         nf4_group, kv_dtype}.  kv_dtype ALJ_KV_Q4 keeps each layer's K and
+ * V in 4 bits (tp_world 1): sync_kv_cache then takes fp32 rows and
+ * quantises them, decode_read_state returns fp32 values.  With tp_world > 1 every weight passed in is
  * this rank's contiguous row block ([rows/tp_world] of each matrix; the
  * q/k/v row blocks are whole heads), the KV cache holds this rank's heads,
  * and nccl_id is the 128-byte id from aljabr_blackwell_nccl_unique_id,
@@ -396,6 +480,11 @@ int aljabr_blackwell_decode_run(unsigned long long handle, int token, int pos, i
  * or a restored session; aljabr_metal_sync_kv_cache).  k, v: host or device
  * memory holding seq_len x (kv_heads/tp * head_dim) elements of kv_dtype. */
 int aljabr_blackwell_sync_kv_cache(unsigned long long handle, int layer, int seq_len, const void* k, const void* v);
+/* Device address of the last step's logits (float[vocab]), for the logits
+ * step (aljabr_blackwell_logits_process_dev) to pick the next token
+ * on the device.  decode_step_token has finished writing them when it
+ * returns; the next step overwrites them. */
+int aljabr_blackwell_decode_logits(unsigned long long handle, const float** logits);
 /* Copy the residual stream x (float[hidden]) and this rank's KV caches
  * ([layers][max_ctx][kv_heads/tp*head_dim] of kv_dtype) to host memory;
  * any pointer may be NULL. */
