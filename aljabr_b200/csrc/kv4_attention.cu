@@ -14,11 +14,14 @@
 //     K codes are the B operand of S^T = q K^T without being converted: a
 //     nibble masked out of its word is the fp16 subnormal c * 2^-24 (or
 //     16 c * 2^-24), exact, so 8 codes cost 4 LOP3 and a shift.  The slots
-//     with the factor 16 have q / 16 on the other side, and the offset -8
-//     enters as the accumulator's start value, -8 * sum of the group's q.
-//   * q is scaled by a power of two into fp16's range; fp32 queries take two
-//     fp16 parts (22 bits) in the two row halves of the A operand, bf16
-//     queries are exact in one.
+//     with the factor 16 have q / 16 on the other side.  The offset -8 is
+//     sum_g dK[p, g] * (-8 sum_{j in g} q_j): one more MMA with the fp16
+//     scales as they are stored for its B operand.
+//   * q is scaled by a power of two into fp16's range.  bf16 queries are
+//     exact in one part; fp32 queries take two parts in the two row halves of
+//     the A operand, each a multiple of a fixed step of the row (2^-11 and
+//     2^-22 of its largest value), so that the tensor cores' sums of a group
+//     are exact integers and their truncation does not enter.
 //   * The accumulator layout of S^T (row = query, columns = positions) is the
 //     B operand layout of O^T = V^T P^T, so probabilities never leave their
 //     lane.  V's group scales are folded into P before it is rounded:
@@ -37,16 +40,16 @@
 // Work split: the positions of each sequence are cut into chunks of 128
 // (a 16-position tile for each of the 8 warps); all chunks of all (sequence,
 // kv head, row tile) items form one line that is dealt out evenly to the
-// resident CTAs, whatever the lengths are.  A CTA keeps an item's running
-// softmax in registers; where an item ends inside a CTA the warps merge in
-// shared memory, and an item cut over several CTAs is joined by the CTA that
-// arrives last, in CTA order, so results do not depend on timing.  Each warp
-// feeds itself through a private ring of tiles filled by cp.async; warps meet
-// only at item ends.
+// resident CTAs, whatever the lengths are (starting and ending an item counts
+// as kItemCost chunks).  A CTA keeps an item's running softmax in registers;
+// where an item ends inside a CTA the warps merge in shared memory, and an
+// item cut over several CTAs is joined by the CTA that arrives last, in CTA
+// order, so results do not depend on timing.  Each warp feeds itself through
+// a private ring of tiles, four bulk copies a tile; warps meet only at item
+// ends.
 #include "kv4.cuh"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace alj {
 namespace {
@@ -56,28 +59,27 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kTilePos = 16;
 constexpr int kChunkTiles = kWarps;
 constexpr int kStages = 3;
+constexpr int kItemCost = 2;     // chunks that an item's start and end are worth
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.0f;    // a row's maximum is raised only when a score exceeds it by 2^8
 
+// d = a b + c; the form without c starts from zero.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-// 16 bytes global -> shared; `bytes` 0 writes zeros and reads nothing.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
@@ -136,23 +138,11 @@ struct Cfg {
     static constexpr int MROW = SG * 32 + 4;                // floats a row in the merge buffer; + 4: no bank conflicts
     static constexpr int MERGE = kWarps * ROWS * MROW * 4;
     static constexpr int QFRAG = NA * NG * 2 * 32 * 16;
-    static constexpr int QSUM = 2 * ROWS * NG * 4;          // [part][row][g]
-    static constexpr int MISC = (kWarps * ROWS * 2 + kWarps + ROWS * 2 + 8) * 4;
-    static constexpr int SMEM = RING + MERGE + QFRAG + QSUM + MISC;   // + the per-sequence tables
+    static constexpr int QSUM = NA * 32 * 16;               // offset fragments
+    static constexpr int BARS = kStages * kWarps * 8;
+    static constexpr int MISC = (kWarps * ROWS * 2 + kWarps + ROWS + 8) * 4;
+    static constexpr int SMEM = RING + MERGE + QFRAG + QSUM + BARS + MISC;   // + the per-sequence tables
 };
-
-// 16-byte chunk i of a tile's K rows / V rows -> its place.  K: the two rows
-// that fall into one bank line at D = 256 swap halves.  V: a lane reads row
-// 2 c + .. at r * 2 NG bytes, c = 0..3, and rows 2 c share banks without the
-// swizzle.
-template <int NG>
-__device__ __forceinline__ int k_chunk(int i) {
-    return NG == 8 ? i ^ ((i >> 3) & 1) : i;
-}
-template <int NG>
-__device__ __forceinline__ int v_chunk(int i) {
-    return i ^ (((i >> (NG == 8 ? 4 : 3)) & 3) << 1);
-}
 
 // One place on the line of chunks: sequence b, item h = kv head * row tiles +
 // row tile, chunk ch of that item.
@@ -161,7 +151,7 @@ struct Cursor {
 };
 
 struct Tables {      // per sequence, in shared memory
-    const int* pre;  // [batch + 1] chunks before it (of one item)
+    const int* pre;  // [batch + 1] chunks and item costs before it (of one item)
     const int* len;  // [batch]
 };
 
@@ -174,7 +164,7 @@ __device__ __forceinline__ int chunks_of(const Kv4Attn& p, int len) {
 }
 __device__ __forceinline__ void load_seq(Cursor& c, const Kv4Attn& p, const Tables& t) {
     c.len = t.len[c.b];
-    c.chunks = t.pre[c.b + 1] - t.pre[c.b];
+    c.chunks = t.pre[c.b + 1] - t.pre[c.b] - kItemCost;
     c.first = first_tile(p, c.len);
 }
 __device__ __forceinline__ void step(Cursor& c, const Kv4Attn& p, const Tables& t, int items) {
@@ -185,41 +175,36 @@ __device__ __forceinline__ void step(Cursor& c, const Kv4Attn& p, const Tables& 
     if (++c.b < p.batch) load_seq(c, p, t);
 }
 
-// Issue the copies of this warp's tile at cursor c into `stage`.
+// Issue the copies of this warp's tile at cursor c into `stage`: lane 0 the K
+// codes, lane 1 the V codes, lanes 2 and 3 their scales.  Returns false, with
+// nothing issued, where there is no tile (past the end, or a page id outside
+// the cache).
 template <int NG>
-__device__ __forceinline__ void load_tile(const Kv4Attn& p, const Cursor& c, uint32_t stage, int warp, int lane) {
+__device__ __forceinline__ bool load_tile(const Kv4Attn& p, const Cursor& c, uint8_t* stage, uint64_t* bar, int warp,
+                                          int lane) {
     using F = Cfg<NG, 1, 1>;
     const int pos = (c.first + c.ch * kChunkTiles + warp) * kTilePos;
-    const uint8_t* src = p.cache;
-    long long kc = 0, vc = 0, ks = 0, vs = 0;
-    int n = 0;
-    if (pos < c.len) {
-        const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
-        const int page = p.table ? __ldg(p.table + static_cast<long long>(c.b) * p.table_stride + pi) : c.b;
-        if (page >= 0 && page < p.pages) {
-            const int off = pos - pi * p.page_size;
-            const int kvh = p.row_tiles == 1 ? c.h : c.h / p.row_tiles;
-            src += (static_cast<long long>(page) * p.kv_heads + kvh) * kv4_block_bytes(p.page_size, F::D);
-            const long long row = 16LL * NG, all = row * p.page_size;
-            kc = off * row;
-            vc = all + kc;
-            ks = 2 * all + off * (2LL * NG);
-            vs = ks + p.page_size * (2LL * NG);
-            n = 16;
-        } else {
-            record_fault(ALJ_FAULT_BOUNDS);   // the tile stays zero
-        }
+    if (pos >= c.len) return false;
+    const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
+    const int page = p.table ? __ldg(p.table + static_cast<long long>(c.b) * p.table_stride + pi) : c.b;
+    if (page < 0 || page >= p.pages) {
+        record_fault(ALJ_FAULT_BOUNDS);
+        return false;
     }
-#pragma unroll
-    for (int i = 0; i < NG / 2; ++i) {
-        const int ch = i * 32 + lane;
-        cp_async16(stage + 16 * k_chunk<NG>(ch), src + kc + 16 * ch, n);
-        cp_async16(stage + F::CODES + 16 * v_chunk<NG>(ch), src + vc + 16 * ch, n);
+    if (lane == 0) mbar_arrive_expect_tx(bar, F::STAGE);
+    __syncwarp();
+    if (lane < 4) {
+        const uint32_t off = pos - pi * p.page_size, ps = p.page_size;
+        const int kvh = p.row_tiles == 1 ? c.h : c.h / p.row_tiles;
+        // sections of a block start at 0, 16 NG ps, 32 NG ps and 34 NG ps bytes
+        const uint32_t row = lane < 2 ? 16 * NG : 2 * NG;
+        const uint32_t section = (lane < 2 ? 16 * NG * lane : 28 * NG + 2 * NG * lane);
+        const uint8_t* src = p.cache + (static_cast<long long>(page) * p.kv_heads + kvh) * kv4_block_bytes(p.page_size, F::D) +
+                             static_cast<unsigned long long>(section) * ps + static_cast<unsigned long long>(row) * off;
+        const uint32_t dst = lane < 2 ? F::CODES * lane : 2 * F::CODES + F::SCALES * (lane - 2);
+        bulk_g2s(stage + dst, src, row * kTilePos, bar);
     }
-    if (lane < 4 * NG) {
-        const int ch = lane < 2 * NG ? lane : lane - 2 * NG;
-        cp_async16(stage + 2 * F::CODES + 16 * lane, src + (lane < 2 * NG ? ks : vs) + 16 * ch, n);
-    }
+    return true;
 }
 
 template <int NG, int RT, int PARTS>
@@ -230,11 +215,12 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
     uint8_t* const ring = smem;
     float* const s_merge = reinterpret_cast<float*>(smem + F::RING);
     uint4* const s_q = reinterpret_cast<uint4*>(smem + F::RING + F::MERGE);
-    float* const s_qsum = reinterpret_cast<float*>(smem + F::RING + F::MERGE + F::QFRAG);
-    float* const s_ml = s_qsum + F::QSUM / 4;                 // [warp][row][max, sum]
-    int* const s_e = reinterpret_cast<int*>(s_ml + kWarps * ROWS * 2);   // [warp] exponent
-    float* const s_fac = reinterpret_cast<float*>(s_e + kWarps);         // [row] score factor
-    int* const s_misc = reinterpret_cast<int*>(s_fac + 2 * ROWS);
+    uint4* const s_off = s_q + F::QFRAG / 16;                 // offset fragments
+    uint64_t* const s_bar = reinterpret_cast<uint64_t*>(s_off + F::QSUM / 16);
+    float* const s_ml = reinterpret_cast<float*>(s_bar + kStages * kWarps);   // [warp][row][max, sum]
+    int* const s_e = reinterpret_cast<int*>(s_ml + kWarps * ROWS * 2);        // [warp]
+    float* const s_fac = reinterpret_cast<float*>(s_e + kWarps);              // [row] score factor
+    int* const s_misc = reinterpret_cast<int*>(s_fac + ROWS);
     int* const s_pre = s_misc + 8;
     int* const s_len = s_pre + p.batch + 1;
 
@@ -243,6 +229,12 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
     const int R = p.q_len * p.group;               // rows that share a kv head
     const int items = p.kv_heads * p.row_tiles;    // items of a sequence
     pdl_launch_dependents();
+    uint64_t* const bars = s_bar + warp * kStages;
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) mbar_init(bars + i, 1);
+        fence_mbar_init();
+    }
+    for (int i = threadIdx.x; i < (F::QFRAG + F::QSUM) / 16; i += kThreads) s_q[i] = make_uint4(0u, 0u, 0u, 0u);
     pdl_wait();
 
     // lengths (clamped to what the table can address) and the prefix of chunks
@@ -260,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
                 len = len < 0 ? 0 : cap;
             }
             s_len[b] = len;
-            n = chunks_of(p, len);
+            n = chunks_of(p, len) + kItemCost;
         }
         int incl = n;
 #pragma unroll
@@ -283,34 +275,53 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
     const long long total = static_cast<long long>(s_pre[p.batch]) * items;
     const long long ctas = min(static_cast<long long>(gridDim.x), total);
     if (static_cast<long long>(blockIdx.x) >= ctas) return;
-    const long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
+    // The line with its item costs is dealt out evenly; chunk numbers (u) count
+    // real chunks only.
+    auto chunks_before = [&](int b) { return static_cast<long long>(s_pre[b] - kItemCost * b) * items; };
+    auto real = [&](long long x) {                 // real chunks before place x of the line
+        if (x >= total) return chunks_before(p.batch);
+        int lo = 0, hi = p.batch - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (static_cast<long long>(s_pre[mid]) * items <= x) lo = mid;
+            else hi = mid - 1;
+        }
+        const int width = s_pre[lo + 1] - s_pre[lo];
+        const long long rest = x - static_cast<long long>(s_pre[lo]) * items;
+        const long long h = rest / width;
+        return chunks_before(lo) + h * (width - kItemCost) + max(0, static_cast<int>(rest - h * width) - kItemCost);
+    };
+    const long long u0 = real(total * blockIdx.x / ctas), u1 = real(total * (blockIdx.x + 1) / ctas);
+    if (u0 >= u1) return;
 
     Cursor at;
     {
         int lo = 0, hi = p.batch - 1;              // the sequence of chunk u0
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (static_cast<long long>(s_pre[mid]) * items <= u0) lo = mid;
+            if (chunks_before(mid) <= u0) lo = mid;
             else hi = mid - 1;
         }
         at.b = lo;
         load_seq(at, p, tab);
-        const long long rest = u0 - static_cast<long long>(s_pre[lo]) * items;
+        const long long rest = u0 - chunks_before(lo);
         at.h = static_cast<int>(rest / at.chunks);
         at.ch = static_cast<int>(rest - static_cast<long long>(at.h) * at.chunks);
     }
     Cursor ahead = at;
-    const uint32_t my_ring = smem_u32(ring) + warp * (kStages * F::STAGE);
+    uint8_t* const my_ring = ring + warp * (kStages * F::STAGE);
     long long next = u0;                           // first chunk not yet asked for
+    uint32_t have = 0, phase = 0;                  // per ring slot: a tile was asked for; the barrier's next parity
+    bool dead = false;                             // a copy never arrived: stop waiting, the fault is recorded
+    auto ask = [&](int slot) {
+        if (next >= u1) return;
+        const bool some = load_tile<NG>(p, ahead, my_ring + slot * F::STAGE, bars + slot, warp, lane);
+        have = some ? have | (1u << slot) : have & ~(1u << slot);
+        step(ahead, p, tab, items);
+        ++next;
+    };
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-        if (next < u1) {
-            load_tile<NG>(p, ahead, my_ring + s * F::STAGE, warp, lane);
-            step(ahead, p, tab, items);
-            ++next;
-        }
-        cp_commit();
-    }
+    for (int i = 0; i < kStages - 1; ++i) ask(i);
     int fill = kStages - 1, use = 0;               // ring slots
 
     long long u = u0;
@@ -318,8 +329,12 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
         // ---------------------------------------------------------- item start
         const int kvh = at.h / p.row_tiles, row0 = (at.h - kvh * p.row_tiles) * ROWS;
         const int item_b = at.b, len = at.len;
-        const long long item0 = static_cast<long long>(s_pre[item_b]) * items + static_cast<long long>(at.h) * at.chunks;
+        const long long item0 = chunks_before(item_b) + static_cast<long long>(at.h) * at.chunks;
         const long long item1 = item0 + at.chunks;
+        // the item's place on the line, for the CTAs that share it
+        const long long line0 = static_cast<long long>(s_pre[item_b]) * items +
+                                static_cast<long long>(at.h) * (at.chunks + kItemCost) + kItemCost;
+        const long long line1 = line0 + at.chunks;
         const long long seg0 = u, seg1 = min(u1, item1);
         const int rows = min(ROWS, R - row0);
         __syncthreads();                           // the previous item's tables are read
@@ -349,22 +364,19 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
             // lane j of a group: slot (c = j / 8, i = j % 8).  MMA step (i & 3) >> 1; k index within it
             const int i8 = lane & 7, cc = lane >> 3, st = (i8 & 3) >> 1;
             const bool odd = i8 & 1;               // second k half, codes carry a factor 16
+            const int half_at = i8 >> 2;           // low or high half of the pair
+            const __half sixteenth = __ushort_as_half(0x2C00);
+            float sum[NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const float y = x[g] * up;
-                const __half h = __float2half_rn(y);
+                const float y = x[g] * up;         // |y| < 2^15
+                // PARTS 2: multiples of 16 and of 2^-7 -- 11 bits each, so that a group's sum of products is exact
+                const __half h = __float2half_rn(PARTS == 2 ? rintf(y * 0.0625f) * 16.0f : y);
                 const float hf = __half2float(h);
-                const __half l = __float2half_rn((y - hf) * 2048.0f);
-                float sum_h = hf, sum_l = __half2float(l);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    sum_h += __shfl_xor_sync(0xffffffffu, sum_h, o);
-                    if (PARTS == 2) sum_l += __shfl_xor_sync(0xffffffffu, sum_l, o);
-                }
-                const __half sixteenth = __ushort_as_half(0x2C00);
+                const __half l = __float2half_rn(rintf((y - hf) * 128.0f) * 16.0f);
+                sum[g] = PARTS == 2 ? fmaf(__half2float(l), 1.0f / 2048.0f, hf) : hf;
                 const __half hs = odd ? __hmul(h, sixteenth) : h, ls = odd ? __hmul(l, sixteenth) : l;
                 // register of the fragment: a0 / a2 rows 0-7, a1 / a3 rows 8-15; a2, a3 the second k half
-                const int half_at = i8 >> 2;       // low or high half of the pair
                 auto put = [&](int na, int reg, __half v) {
                     reinterpret_cast<__half*>(s_q + ((na * NG + g) * 2 + st) * 32 + (row & 7) * 4 + cc)[2 * reg + half_at] = v;
                 };
@@ -373,12 +385,22 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
                     put(row >> 3, odd ? 3 : 1, ls);
                 } else {
                     put(0, (odd ? 2 : 0) + (row >> 3), hs);
-                    if (RT == 1) put(0, odd ? 3 : 1, __ushort_as_half(0));
                 }
-                if (lane == 0) {
-                    s_qsum[row * NG + g] = sum_h * (-8.0f * 5.9604644775390625e-8f);   // -8 sum * 2^-24
-                    if (PARTS == 2) s_qsum[(ROWS + row) * NG + g] = sum_l * (-8.0f * 5.9604644775390625e-8f);
-                }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                for (int g = 0; g < NG; ++g) sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], o);
+            // offset fragment: k = g holds the group sum * 2^-6 in fp16, k = NG + g what that rounding left
+            if (lane < 2 * NG) {
+                float v = 0.0f;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) v = (lane & (NG - 1)) == g ? sum[g] * 0.015625f : v;
+                const __half h = __float2half_rn(v);
+                const __half w = lane < NG ? h : __float2half_rn(v - __half2float(h));
+                const int na = PARTS == 2 ? row >> 3 : 0;
+                const int reg = (lane >= 8 ? 2 : 0) + (PARTS == 2 ? 0 : row >> 3);
+                reinterpret_cast<__half*>(s_off + na * 32 + (row & 7) * 4 + ((lane & 7) >> 1))[2 * reg + (lane & 1)] = w;
             }
             if (lane == 0) s_fac[row] = p.scale * pow2i(24 - f);
         }
@@ -402,16 +424,13 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
         const int any_lo = p.window > 0 ? all_hi - p.window + 1 : 0;
         constexpr bool kQRegs = NA == 1 && NG <= 4;
         uint4 qreg[kQRegs ? NG * 2 : 1];
-        float init[kQRegs ? NG : 1][2];
         if constexpr (kQRegs) {
 #pragma unroll
             for (int i = 0; i < NG * 2; ++i) qreg[i] = s_q[i * 32 + lane];
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                init[g][0] = s_qsum[r * NG + g];
-                init[g][1] = PARTS == 2 ? s_qsum[(ROWS + r) * NG + g] : RT == 2 ? s_qsum[(r + 8) * NG + g] : 0.0f;
-            }
         }
+        uint4 oreg[NA];
+#pragma unroll
+        for (int n = 0; n < NA; ++n) oreg[n] = s_off[n * 32 + lane];
         float acc[2 * NG][RT][4];
 #pragma unroll
         for (int i = 0; i < 2 * NG; ++i)
@@ -420,123 +439,113 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[i][a][j] = 0.0f;
         int E = 0;                                 // exponent field the P' scaling is made for
+        float sigma = pow2i(20);
 
-        auto tile = [&](const uint8_t* st, int pos, auto masked_tag) {
-            constexpr bool MASKED = decltype(masked_tag)::value;
+        // A lane's columns of S^T and P: slots (h, j) of tile halves h are the
+        // positions 8 h + 2 c4 + (j ^ (c4 & 1)).  The swap for odd c4 spreads the
+        // V rows of one load over both halves of the banks.
+        const int swap = c4 & 1;
+        auto tile = [&](const uint8_t* st, int pos) {
             const uint8_t* kcode = st;
             const uint8_t* vcode = st + F::CODES;
             const uint8_t* kscale = st + 2 * F::CODES;
             const uint8_t* vscale = kscale + F::SCALES;
-            // ---- scores: s[a][2 h + j] of position pos + 8 h + 2 c4 + j
             float s[RT][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                const int krow = 8 * h + (r ^ ((r >> 1) & 1));     // the position of column r
                 uint32_t kw[NG];
-                if constexpr (NG == 8) {
-                    const int row = 8 * h + r;
-                    uint32_t t[4];
-                    lds_words<4>(kcode + 16 * k_chunk<NG>(row * 8 + c4 * 2), t);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) kw[i] = t[i];
-                    lds_words<4>(kcode + 16 * k_chunk<NG>(row * 8 + c4 * 2 + 1), t);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) kw[4 + i] = t[i];
-                } else {
-                    lds_words<NG>(kcode + (8 * h + r) * 16 * NG + c4 * 4 * NG, kw);
-                }
-                uint32_t dk[NG];                   // scales of positions 2 c4 and 2 c4 + 1
-                lds_words<NG>(kscale + (8 * h + 2 * c4) * 2 * NG, dk);
-                float part[NA][4];
+                lds_words<NG>(kcode + krow * 16 * NG + c4 * 4 * NG, kw);
+                uint32_t d0w[NG / 2], d1w[NG / 2];
+                lds_words<NG / 2>(kscale + (8 * h + 2 * c4 + swap) * 2 * NG, d0w);
+                lds_words<NG / 2>(kscale + (8 * h + 2 * c4 + 1 - swap) * 2 * NG, d1w);
+                // offset: B = the scales of position `krow`, k = g and again NG + g
+                uint32_t ob = 0u;
+                if (NG > 2 || c4 < 2) ob = *reinterpret_cast<const uint32_t*>(kscale + krow * 2 * NG + 4 * (c4 & (NG / 2 - 1)));
+                float off[NA][4], part[NA][4];
 #pragma unroll
                 for (int n = 0; n < NA; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) part[n][j] = 0.0f;
+                    mma_f16_zero(off[n], oreg[n].x, oreg[n].y, oreg[n].z, oreg[n].w, ob, NG == 8 ? ob : 0u);
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     const uint32_t w8 = kw[g] >> 8;
                     const uint32_t b0 = kw[g] & 0x000F000Fu, b1 = kw[g] & 0x00F000F0u;
                     const uint32_t b2 = w8 & 0x000F000Fu, b3 = w8 & 0x00F000F0u;
-                    // group g of position 2 c4 is half g of the first NG halves, of 2 c4 + 1 of the next
-                    const uint32_t w0 = dk[g / 2], w1 = dk[NG / 2 + g / 2];
-                    const float d0 = g & 1 ? half_hi(w0) : half_lo(w0);
-                    const float d1 = g & 1 ? half_hi(w1) : half_lo(w1);
+                    const float d0 = g & 1 ? half_hi(d0w[g / 2]) : half_lo(d0w[g / 2]);
+                    const float d1 = g & 1 ? half_hi(d1w[g / 2]) : half_lo(d1w[g / 2]);
 #pragma unroll
                     for (int n = 0; n < NA; ++n) {
                         uint4 a0, a1;
-                        float i0, i1;
                         if constexpr (kQRegs) {
                             a0 = qreg[2 * g];
                             a1 = qreg[2 * g + 1];
-                            i0 = init[g][0];
-                            i1 = init[g][1];
                         } else {
                             a0 = s_q[((n * NG + g) * 2) * 32 + lane];
                             a1 = s_q[((n * NG + g) * 2 + 1) * 32 + lane];
-                            i0 = s_qsum[(r + 8 * n) * NG + g];
-                            i1 = PARTS == 2 ? s_qsum[(ROWS + r + 8 * n) * NG + g] : RT == 2 ? s_qsum[(r + 8) * NG + g] : 0.0f;
                         }
-                        float x[4] = {i0, i0, i1, i1};
-                        mma_f16(x, a0.x, a0.y, a0.z, a0.w, b0, b1);
+                        float x[4];
+                        mma_f16_zero(x, a0.x, a0.y, a0.z, a0.w, b0, b1);
                         mma_f16(x, a1.x, a1.y, a1.z, a1.w, b2, b3);
-                        part[n][0] = fmaf(d0, x[0], part[n][0]);
-                        part[n][1] = fmaf(d1, x[1], part[n][1]);
-                        if (PARTS == 2 || RT == 2) {
-                            part[n][2] = fmaf(d0, x[2], part[n][2]);
-                            part[n][3] = fmaf(d1, x[3], part[n][3]);
+                        if (g == 0) {
+                            part[n][0] = d0 * x[0];
+                            part[n][1] = d1 * x[1];
+                            part[n][2] = d0 * x[2];
+                            part[n][3] = d1 * x[3];
+                        } else {
+                            part[n][0] = fmaf(d0, x[0], part[n][0]);
+                            part[n][1] = fmaf(d1, x[1], part[n][1]);
+                            if (PARTS == 2 || RT == 2) {
+                                part[n][2] = fmaf(d0, x[2], part[n][2]);
+                                part[n][3] = fmaf(d1, x[3], part[n][3]);
+                            }
                         }
                     }
                 }
+                // offset in the units of the products: -8 * 2^6 * 2^-24
 #pragma unroll
                 for (int a = 0; a < RT; ++a)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float v = PARTS == 2 ? fmaf(part[a][2 + j], 1.0f / 2048.0f, part[a][j]) : part[0][2 * a + j];
-                        v *= fac[a];
-                        if (p.soft_cap > 0.0f) v = tanhf(v / p.soft_cap) * p.soft_cap * kLog2e;
-                        s[a][2 * h + j] = v;
+                        const float v = PARTS == 2 ? fmaf(part[a][2 + j], 1.0f / 2048.0f, part[a][j]) : part[0][2 * a + j];
+                        const float o = PARTS == 2 ? off[a][j] : off[0][2 * a + j];
+                        s[a][2 * h + j] = fmaf(o, -3.0517578125e-5f, v) * fac[a];
                     }
             }
-            // ---- masks
-            uint32_t dv[4][NG / 2];                // V scales of the lane's 4 positions, two groups a word
+            if (p.soft_cap > 0.0f) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t w[NG];
-                lds_words<NG>(vscale + (8 * h + 2 * c4) * 2 * NG, w);
+                for (int a = 0; a < RT; ++a)
 #pragma unroll
-                for (int i = 0; i < NG / 2; ++i) {
-                    dv[2 * h][i] = w[i];
-                    dv[2 * h + 1][i] = w[NG / 2 + i];
-                }
+                    for (int j = 0; j < 4; ++j) s[a][j] = tanhf(s[a][j] / p.soft_cap) * p.soft_cap * kLog2e;
             }
-            bool seen[RT][4];
-            if constexpr (MASKED) {
+            // largest V scale: the tile's scale words are dealt out over the lanes
+            uint32_t top = 0u;
+            if (NG >= 4 || lane < 16) {
+                constexpr int NW = NG == 8 ? 2 : 1;
+                uint32_t w[NW];
+                lds_words<NW>(vscale + lane * 4 * NW, w);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at_pos = pos + (j >> 1) * 8 + 2 * c4 + (j & 1);
+                for (int i = 0; i < NW; ++i) top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+            }
+            // a tile at the edge of what some row sees: masks; what no row sees, and NaN scales, do not set the range
+            uint32_t keep[RT][2];
 #pragma unroll
-                    for (int a = 0; a < RT; ++a) {
-                        seen[a][j] = at_pos <= hi[a] && at_pos >= lo[a];
-                        s[a][j] = seen[a][j] ? s[a][j] : -INFINITY;
+            for (int a = 0; a < RT; ++a) keep[a][0] = keep[a][1] = 0xFFFFFFFFu;
+            if (pos < all_lo || pos + kTilePos - 1 > all_hi) {
+                const int word_pos = pos + (NG == 2 ? lane : lane >> 1);   // the position of the lane's scale words
+                if (word_pos >= len || word_pos < any_lo || top >= 0x7C00u) top = 0u;
+#pragma unroll
+                for (int a = 0; a < RT; ++a)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int at0 = pos + 8 * h + 2 * c4 + swap, at1 = pos + 8 * h + 2 * c4 + 1 - swap;
+                        const bool see0 = at0 <= hi[a] && at0 >= lo[a], see1 = at1 <= hi[a] && at1 >= lo[a];
+                        s[a][2 * h] = see0 ? s[a][2 * h] : -INFINITY;
+                        s[a][2 * h + 1] = see1 ? s[a][2 * h + 1] : -INFINITY;
+                        keep[a][h] = (see0 ? 0x0000FFFFu : 0u) | (see1 ? 0xFFFF0000u : 0u);
                     }
-                }
             }
             // ---- running maximum and the exponent of the V scales
-            uint32_t top = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t t = 0;
-#pragma unroll
-                for (int i = 0; i < NG / 2; ++i) t = __vmaxu2(t, dv[j][i] & 0x7FFF7FFFu);
-                if constexpr (MASKED) {            // what no row sees, and NaN scales, do not set the range
-                    const int at_pos = pos + (j >> 1) * 8 + 2 * c4 + (j & 1);
-                    const bool out = at_pos >= len || at_pos < any_lo;
-                    t = out ? 0u : t;
-                    if ((t & 0xFFFFu) >= 0x7C00u) t &= 0xFFFF0000u;
-                    if ((t >> 16) >= 0x7C00u) t &= 0xFFFFu;
-                }
-                top = __vmaxu2(top, t);
-            }
-            const int e_tile = static_cast<int>(__reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16)) >> 10);
+            const int e_tile = static_cast<int>(__reduce_max_sync(0xffffffffu, top) >> 10);
             float mx[RT];
             bool raise = e_tile > E;
 #pragma unroll
@@ -551,6 +560,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
                 const int e_new = max(E, e_tile);
                 const float shrink = pow2i(E - e_new);
                 E = e_new;
+                sigma = pow2i(20 - E);
 #pragma unroll
                 for (int a = 0; a < RT; ++a) {
                     const float mn = fmaxf(m[a], mx[a]);
@@ -569,7 +579,6 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
                     }
                 }
             }
-            const float sigma = pow2i(20 - E);
 #pragma unroll
             for (int a = 0; a < RT; ++a) {
                 const float ms = m[a] == -INFINITY ? 0.0f : m[a];
@@ -579,13 +588,13 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[a][j] *= sigma;
             }
-            // ---- output: V rows of positions (2 c4, 2 c4 + 1) and (8 + 2 c4, ..), nibbles of row block r
-            uint32_t vw[4][NG / 2];
+            // ---- output: V rows of the lane's positions, nibbles of row block r
+            uint32_t vw[4][NG / 2], dv[4][NG / 2];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int row = (j >> 1) * 8 + 2 * c4 + (j & 1);
-                const int byte = row * 16 * NG + r * 2 * NG;
-                lds_words<NG / 2>(vcode + 16 * v_chunk<NG>(byte >> 4) + (byte & 15), vw[j]);
+                const int row = (j >> 1) * 8 + 2 * c4 + ((j & 1) ^ swap);
+                lds_words<NG / 2>(vcode + row * 16 * NG + r * 2 * NG, vw[j]);
+                lds_words<NG / 2>(vscale + row * 2 * NG, dv[j]);
             }
             const __half2 kOff = bits_h2(0x64086408u);          // 1032
             const __half2 kDiv = bits_h2(0x2C002C00u), kOff16 = bits_h2(0xD480D480u);   // 1/16, -72
@@ -597,15 +606,12 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t w0 = dv[2 * h][g / 2], w1 = dv[2 * h + 1][g / 2];
-                        float x0 = s[a][2 * h] * (g & 1 ? half_hi(w0) : half_lo(w0));
-                        float x1 = s[a][2 * h + 1] * (g & 1 ? half_hi(w1) : half_lo(w1));
-                        if constexpr (MASKED) {    // a masked position's scale may be anything
-                            x0 = seen[a][2 * h] ? x0 : 0.0f;
-                            x1 = seen[a][2 * h + 1] ? x1 : 0.0f;
-                        }
+                        const float x0 = s[a][2 * h] * (g & 1 ? half_hi(w0) : half_lo(w0));
+                        const float x1 = s[a][2 * h + 1] * (g & 1 ? half_hi(w1) : half_lo(w1));
                         const __half2 hh = __floats2half2_rn(x0, x1);
-                        bh[a][h] = h2_bits(hh);
-                        if (PARTS == 2) bl[a][h] = h2_bits(__floats2half2_rn(x0 - __low2float(hh), x1 - __high2float(hh)));
+                        bh[a][h] = h2_bits(hh) & keep[a][h];       // a masked position's scale may be anything
+                        if (PARTS == 2)
+                            bl[a][h] = h2_bits(__floats2half2_rn(x0 - __low2float(hh), x1 - __high2float(hh))) & keep[a][h];
                     }
                 uint32_t f[2][4];                  // [position half][nibble]: the integers c - 8
 #pragma unroll
@@ -623,8 +629,8 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
                     for (int a = 0; a < RT; ++a) {
                         float (&o)[4] = acc[2 * g + q2][a];
                         if constexpr (PARTS == 2) {
-                            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma_f16(x, f[0][2 * q2], f[0][2 * q2 + 1], f[1][2 * q2], f[1][2 * q2 + 1], bl[a][0], bl[a][1]);
+                            float x[4];
+                            mma_f16_zero(x, f[0][2 * q2], f[0][2 * q2 + 1], f[1][2 * q2], f[1][2 * q2 + 1], bl[a][0], bl[a][1]);
                             mma_f16(x, f[0][2 * q2], f[0][2 * q2 + 1], f[1][2 * q2], f[1][2 * q2 + 1], bh[a][0], bh[a][1]);
 #pragma unroll
                             for (int j = 0; j < 4; ++j) o[j] += x[j];
@@ -638,20 +644,12 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
         // ---------------------------------------------------------- the item's chunks
         for (; u < seg1; ++u) {
             __syncwarp();                          // the slot below was read by every lane
-            if (next < u1) {
-                load_tile<NG>(p, ahead, my_ring + fill * F::STAGE, warp, lane);
-                step(ahead, p, tab, items);
-                ++next;
-            }
-            cp_commit();
+            ask(fill);
             fill = fill + 1 == kStages ? 0 : fill + 1;
-            cp_wait<kStages - 1>();
-            __syncwarp();
-            const int pos = (at.first + at.ch * kChunkTiles + warp) * kTilePos;
-            const uint8_t* st = ring + warp * (kStages * F::STAGE) + use * F::STAGE;
-            if (pos < len) {
-                if (pos >= all_lo && pos + kTilePos - 1 <= all_hi) tile(st, pos, std::false_type{});
-                else tile(st, pos, std::true_type{});
+            if ((have >> use) & 1u) {
+                if (!dead) dead = !mbar_wait(bars + use, (phase >> use) & 1u);
+                phase ^= 1u << use;
+                tile(my_ring + use * F::STAGE, (at.first + at.ch * kChunkTiles + warp) * kTilePos);
             }
             use = use + 1 == kStages ? 0 : use + 1;
             step(at, p, tab, items);
@@ -735,8 +733,8 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
         if (whole) continue;
 
         // ---------------------------------------------------------- join an item cut over CTAs
-        const int cta0 = static_cast<int>(((item0 + 1) * ctas - 1) / total);
-        const int cta1 = static_cast<int>((item1 * ctas - 1) / total);
+        const int cta0 = static_cast<int>(((line0 + 1) * ctas - 1) / total);
+        const int cta1 = static_cast<int>((line1 * ctas - 1) / total);
         __threadfence();
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -748,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
         if (!s_misc[1]) continue;
         __threadfence();
         const int n = cta1 - cta0 + 1;
-        const int slot0 = total * cta0 / ctas == item0 ? 0 : 1;   // only the first CTA may hold it in its second slot
+        const int slot0 = real(total * cta0 / ctas) == item0 ? 0 : 1;   // only the first CTA may hold it in its second slot
         auto base = [&](int k) { return p.part + (static_cast<long long>(cta0 + k) * 2 + (k == 0 ? slot0 : 0)) * (ROWS * (D + 2)); };
         const int outs = rows * (D / 4);
         const int ways = max(1, min(n, min(kThreads / outs, F::MERGE / 4 / (outs * 4))));   // threads that share one output
@@ -798,7 +796,6 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && RT == 1 ? 2 : 1) kv4_attn
             }
         }
     }
-    cp_wait<0>();
 }
 
 template <int NG, int RT, int PARTS>
