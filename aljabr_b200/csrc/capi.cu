@@ -1437,10 +1437,12 @@ int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, lo
     if (!out || !q || !cache || !seq_lens || !workspace) return fail(ALJ_ERR_BAD_ARG, "kv4_attention: null pointer");
     if (block_table ? table_stride < 1 : batch > pages)
         return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: table_stride %d, batch %d, pages %d", table_stride, batch, pages);
-    // chunks of one sequence over all its items, which the kernel counts in 32 bits
+    // the chunks of all sequences at their longest, which the kernel counts in 32 bits
     const long long cap = block_table ? static_cast<long long>(table_stride) * page_size : page_size;
-    if ((cap / 128 + 4) * kv_heads * (static_cast<long long>(q_len) * (q_heads / kv_heads) / 4 + 1) > 0x7fffffffLL)
-        return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: %d kv heads of sequences of up to %lld positions are too many", kv_heads, cap);
+    const long long items = kv_heads * (static_cast<long long>(q_len) * (q_heads / kv_heads) / 4 + 1);
+    if (static_cast<long long>(batch) * (cap / 128 + 4) > 0x7fffffffLL / items)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: %d sequences of up to %lld positions x %d kv heads are too many", batch, cap,
+                    kv_heads);
     const uintptr_t e = q_dtype == ALJ_KV_BF16 ? 2 : 4;
     if (q_stride < static_cast<long long>(q_heads) * head_dim)
         return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: q_stride %lld < q_heads * head_dim", q_stride);

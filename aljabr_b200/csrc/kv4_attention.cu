@@ -49,10 +49,14 @@
 // as kItemCost chunks).  A CTA keeps an item's running softmax in registers;
 // where an item ends inside a CTA the warps merge in shared memory, and an
 // item cut over several CTAs is joined by the CTA that arrives last, in CTA
-// order, so results do not depend on timing.  A ninth warp feeds the others:
-// it walks the line ahead of them and fills a ring of chunks, each lane one
-// bulk copy (a tile's K codes, V codes, K scales or V scales).  Its address
-// arithmetic, done by each consumer for itself, was half of all instructions.
+// order, so results do not depend on timing.  The ring
+// of chunks is filled two chunks ahead, by the warps in turn: each lane one
+// bulk copy (K codes, V codes, K scales or V scales of the tiles that share a
+// page).  A ninth warp for it would cut every warp from 128 to 96 registers,
+// and address arithmetic in every warp for itself was half of all
+// instructions.  Pages of fewer than 64 positions would take up to 32 such
+// copies a chunk, which one warp issues one after the other (~100 cycles
+// each): there every warp copies its own tile in 16-byte pieces instead.
 #include "kv4.cuh"
 
 #include <algorithm>
@@ -61,11 +65,14 @@ namespace alj {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;         // consumers; one more warp loads
+constexpr int kThreads = kWarps * 32;
 constexpr int kTilePos = 16;
 constexpr int kChunkTiles = kWarps;
-constexpr int kStages = 3;
+constexpr int kStages = 4;
+constexpr int kAhead = 2;        // chunks asked for before their turn
 constexpr int kItemCost = 2;     // chunks that an item's start and end are worth
+constexpr int kMinShare = 2;     // least length of line a CTA is started for
+constexpr int kBulkPage = 64;    // least page size that is loaded by bulk copies
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 2.0f;    // a row's maximum is raised only when a score exceeds it by 2 (log2)
 constexpr float kNone = -1e30f;  // running maximum of a row that has seen nothing
@@ -129,20 +136,19 @@ __device__ __forceinline__ void store4(void* out, bool bf16, long long to, float
     }
 }
 
-// NW consecutive 32-bit words from shared memory (4 NW-byte aligned).
+// NW consecutive 32-bit words from shared memory (aligned to 4 NW bytes, at most 16).
 template <int NW>
-__device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[NW]) {
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[NW]) {
     if constexpr (NW % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < NW / 4; ++i) {
-            const uint4 v = reinterpret_cast<const uint4*>(p)[i];
-            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-        }
+        for (int i = 0; i < NW / 4; ++i)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3])
+                         : "r"(a + 16 * i));
     } else if constexpr (NW == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        w[0] = v.x; w[1] = v.y;
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
     } else {
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a));
     }
 }
 
@@ -205,16 +211,16 @@ __device__ __forceinline__ void step(Cursor& c, const Kv4Attn& p, const Tables& 
     if (++c.b < p.batch) load_seq(c, p, t);
 }
 
-// The loading warp's pass over one chunk: lane 4 w + i copies section i of the
+// A warp's pass over one chunk to load: lane 4 w + i copies section i of the
 // tile of consumer w.
 struct TileSource {
     int pos;     // the tile's first position; at or past the sequence's end there is no tile
     int page;    // its page, or -1
     int off;     // its place in the page
 };
-__device__ __forceinline__ TileSource find_tile(const Kv4Attn& p, const Cursor& c, int lane) {
+__device__ __forceinline__ TileSource find_tile(const Kv4Attn& p, const Cursor& c, int w) {
     TileSource t;
-    t.pos = (c.first + c.ch * kChunkTiles + (lane >> 2)) * kTilePos;
+    t.pos = (c.first + c.ch * kChunkTiles + w) * kTilePos;
     t.page = -1;
     t.off = 0;
     if (t.pos < c.len) {
@@ -254,8 +260,44 @@ __device__ __forceinline__ void load_chunk(const Kv4Attn& p, const TileSource& t
     }
 }
 
+// This warp's own tile in 16-byte pieces; the full barrier counts every lane's
+// arrival, which follows its copies.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+template <int NG>
+__device__ __forceinline__ void load_own(const Kv4Attn& p, const TileSource& t, int kvh, int len, uint32_t stage,
+                                         uint64_t* bar, int warp, int lane) {
+    using F = Cfg<NG, 1, 1>;
+    if (t.pos < len) {
+        const bool ok = t.page >= 0 && t.page < p.pages;
+        if (!ok) record_fault(ALJ_FAULT_BOUNDS);       // reads as zeros
+        const int n = ok ? 16 : 0;
+        const uint8_t* src = p.cache;
+        const unsigned long long plane = 16ull * NG * p.page_size;
+        unsigned long long k = 16u * lane, sc = 0;
+        if (ok) {
+            src += (static_cast<long long>(t.page) * p.kv_heads + kvh) * kv4_block_bytes(p.page_size, F::D);
+            k += 16ull * NG * t.off;
+            // lanes 0 .. 2 NG - 1 the K scales, the next 2 NG the V scales
+            sc = 2 * plane + 2ull * NG * t.off + 16u * lane + (lane >= 2 * NG ? 2ull * NG * p.page_size - F::SCALES : 0ull);
+        }
+        const uint32_t dst = stage + warp * F::CODES + 16 * lane;
+#pragma unroll
+        for (int i = 0; i < NG / 2; ++i) {
+            cp_async16(dst + 512 * i, src + (ok ? k + 512 * i : 0), n);
+            cp_async16(dst + kWarps * F::CODES + 512 * i, src + (ok ? plane + k + 512 * i : 0), n);
+        }
+        if (lane < 4 * NG) {
+            const uint32_t at = lane < 2 * NG ? 16 * lane : kWarps * F::SCALES + 16 * (lane - 2 * NG);
+            cp_async16(stage + 2 * kWarps * F::CODES + warp * F::SCALES + at, src + sc, n);
+        }
+    }
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 template <int NG, int CT, int PARTS>
-__global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4_attn_kernel(const Kv4Attn p) {
+__global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kernel(const Kv4Attn p) {
     using F = Cfg<NG, CT, PARTS>;
     constexpr int D = F::D, ROWS = F::ROWS, COLS = F::COLS;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -273,32 +315,34 @@ __global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4
     int* const s_pre = s_misc + 8;
     int* const s_len = s_pre + p.batch + 1;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = hide(threadIdx.x >> 5), lane = hide(threadIdx.x & 31);
     const int r = lane >> 2, c4 = lane & 3;
     const int R = p.q_len * p.group;               // rows that share a kv head
     const int items = p.kv_heads * p.row_tiles;    // items of a sequence
     pdl_launch_dependents();
+    const bool bulk = p.page_size >= kBulkPage;
     uint64_t* const full = s_bar;
     uint64_t* const empty = s_bar + kStages;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(full + i, 1);
+            mbar_init(full + i, bulk ? 1 : kThreads);
             mbar_init(empty + i, kWarps);
         }
         fence_mbar_init();
         s_misc[0] = 0;
     }
-    for (int i = threadIdx.x; i < (F::QFRAG + F::QOFF) / 8; i += kThreads + 32) s_q[i] = make_uint2(0u, 0u);
+    for (int i = threadIdx.x; i < (F::QFRAG + F::QOFF) / 8; i += kThreads) s_q[i] = make_uint2(0u, 0u);
     __syncthreads();
     pdl_wait();
 
-    // lengths (clamped to what the table can address) and the prefix of chunks
+    // lengths (clamped to what the table can address) and the prefix of chunks and item costs
     const int cap = p.table ? static_cast<int>(min(static_cast<long long>(p.table_stride) * p.page_size, 0x7fffff00LL))
                             : p.page_size;
+    int total = 0;                                 // < 2^31: checked on the host for the longest sequences
     for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
         const int b = b0 + threadIdx.x;
         int n = 0;
-        if (b < p.batch && warp < kWarps) {
+        if (b < p.batch) {
             int len = __ldg(p.lens + b) + p.len_add;
             if (len < 0 || len > cap) {
                 record_fault(ALJ_FAULT_BOUNDS);
@@ -313,45 +357,47 @@ __global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4
             const int up = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += up;
         }
-        if (lane == 31 && warp < kWarps) s_e[warp] = incl;
+        if (b0 > 0) __syncthreads();               // s_e is read
+        if (lane == 31) s_e[warp] = incl;
         __syncthreads();
-        int base = s_misc[0];
-        for (int w = 0; w < min(warp, kWarps); ++w) base += s_e[w];
-        if (b < p.batch && warp < kWarps) s_pre[b] = base + incl - n;
-        __syncthreads();
-        if (threadIdx.x == kThreads - 1) s_misc[0] = base + incl;
-        __syncthreads();
+        int base = total;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const int e = s_e[w];
+            if (w < warp) base += e;
+            total += e;
+        }
+        if (b < p.batch) s_pre[b + 1] = base + incl;
     }
-    if (threadIdx.x == 0) s_pre[p.batch] = s_misc[0];
+    if (threadIdx.x == 0) s_pre[0] = 0;
     __syncthreads();
     const Tables tab = {s_pre, s_len};
-    const long long total = static_cast<long long>(s_pre[p.batch]) * items;
-    const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+    total *= items;
+    const int ctas = min(static_cast<int>(gridDim.x), (total + kMinShare - 1) / kMinShare);
     if (static_cast<int>(blockIdx.x) >= ctas) return;
-    const long long share = total / ctas;
-    const int rem = static_cast<int>(total - share * ctas);
+    const int share = total / ctas, rem = total - share * ctas;
     auto start_of = [&](int c) { return share * c + min(c, rem); };     // CTA c's first place on the line
-    auto cta_at = [&](long long x) {
-        const long long wide = static_cast<long long>(rem) * (share + 1);
-        return static_cast<int>(x < wide ? x / (share + 1) : rem + (x - wide) / share);
+    auto cta_at = [&](int x) {
+        const int wide = rem * (share + 1);
+        return x < wide ? x / (share + 1) : rem + (x - wide) / share;
     };
     // The line with its item costs is dealt out evenly; chunk numbers (u) count
     // real chunks only.
-    auto chunks_before = [&](int b) { return static_cast<long long>(s_pre[b] - kItemCost * b) * items; };
-    auto real = [&](long long x) {                 // real chunks before place x of the line
+    auto chunks_before = [&](int b) { return (s_pre[b] - kItemCost * b) * items; };
+    auto real = [&](int x) {                       // real chunks before place x of the line
         if (x >= total) return chunks_before(p.batch);
         int lo = 0, hi = p.batch - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (static_cast<long long>(s_pre[mid]) * items <= x) lo = mid;
+            if (s_pre[mid] * items <= x) lo = mid;
             else hi = mid - 1;
         }
         const int width = s_pre[lo + 1] - s_pre[lo];
-        const int rest = static_cast<int>(x - static_cast<long long>(s_pre[lo]) * items);
+        const int rest = x - s_pre[lo] * items;
         const int h = rest / width;
         return chunks_before(lo) + h * (width - kItemCost) + max(0, rest - h * width - kItemCost);
     };
-    const long long u0 = real(start_of(blockIdx.x)), u1 = real(start_of(blockIdx.x + 1));
+    const int u0 = real(start_of(blockIdx.x)), u1 = real(start_of(blockIdx.x + 1));
     if (u0 >= u1) return;
 
     Cursor at;
@@ -364,79 +410,78 @@ __global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4
         }
         at.b = lo;
         load_seq(at, p, tab);
-        const int rest = static_cast<int>(u0 - chunks_before(lo));
+        const int rest = u0 - chunks_before(lo);
         at.h = rest / at.chunks;
         at.ch = rest - at.h * at.chunks;
     }
-    if (warp == kWarps) {                          // the loading warp
-        const int n = static_cast<int>(u1 - u0);
-        TileSource t = find_tile(p, at, lane);
-        int slot = 0;
-        uint32_t parity = 1;                       // the first kStages slots are free
-        for (int i = 0; i < n; ++i) {
-            const int kvh = at.h / p.row_tiles, len = at.len;
-            if (i >= kStages && !mbar_wait(empty + slot, parity)) return;
-            load_chunk<NG>(p, t, kvh, len, ring + slot * F::STAGE, full + slot, lane);
-            if (++slot == kStages) {
-                slot = 0;
-                parity ^= 1u;
-            }
-            if (i + 1 < n) {
-                step(at, p, tab, items);
-                t = find_tile(p, at, lane);        // the page id is on its way while the slot empties
-            }
+    // chunk number i of this CTA, at cursor c, into its slot; the slot's last chunk has been read by every warp
+    auto load = [&](int i, const Cursor& c) {
+        const int slot = i % kStages;
+        const TileSource t = find_tile(p, c, lane >> 2);    // the page id is on its way while the slot empties
+        if (i >= kStages && !mbar_wait(empty + slot, (i / kStages - 1) & 1)) return false;
+        load_chunk<NG>(p, t, c.h / p.row_tiles, c.len, ring + slot * F::STAGE, full + slot, lane);
+        return true;
+    };
+    auto load_mine = [&](int i, const Cursor& c) {     // the slot's last tile of this warp has been read by it
+        load_own<NG>(p, find_tile(p, c, warp), c.h / p.row_tiles, c.len, smem_u32(ring) + (i % kStages) * F::STAGE,
+                     full + i % kStages, warp, lane);
+    };
+    const int todo = u1 - u0;
+    if (bulk ? warp < min(kAhead, todo) : true) {
+        Cursor c = at;
+        for (int i = 0; i < min(kAhead, todo); ++i) {
+            if (!bulk) load_mine(i, c);
+            else if (i == warp) load(i, c);
+            step(c, p, tab, items);
         }
-        return;
     }
-    int use = 0;                                   // ring slot
-    uint32_t parity = 0;
+    int done = 0;                                  // chunks of this CTA behind us
     bool dead = false;                             // a chunk never arrived: stop waiting, the fault is recorded
-    long long u = u0;
+    int u = u0;
     while (u < u1) {
         // ---------------------------------------------------------- item start
         const int kvh = at.h / p.row_tiles, row0 = (at.h - kvh * p.row_tiles) * ROWS;
         const int item_b = at.b, len = at.len;
-        const long long item0 = chunks_before(item_b) + static_cast<long long>(at.h) * at.chunks;
-        const long long item1 = item0 + at.chunks;
+        const int item0 = chunks_before(item_b) + at.h * at.chunks, item1 = item0 + at.chunks;
         // the item's place on the line, for the CTAs that share it
-        const long long line0 = static_cast<long long>(s_pre[item_b]) * items +
-                                static_cast<long long>(at.h) * (at.chunks + kItemCost) + kItemCost;
-        const long long line1 = line0 + at.chunks;
-        const long long seg0 = u, seg1 = min(u1, item1);
+        const int line0 = s_pre[item_b] * items + at.h * (at.chunks + kItemCost) + kItemCost;
+        const int line1 = line0 + at.chunks;
+        const int seg0 = u, seg1 = min(u1, item1);
         const int rows = min(ROWS, R - row0);
-        named_bar(1, kThreads);                    // the previous item's tables are read
+        __syncthreads();                    // the previous item's tables are read
 
-        // q rows -> columns in B-fragment order, their group sums, their score factors
-        for (int row = warp; row < ROWS; row += kWarps) {
+        // q rows -> columns in B-fragment order, their group sums, their score factors.  A lane has NG dims of
+        // one group.  (The first warps are busy with the first chunks.)
+        for (int row = (warp - kAhead) & (kWarps - 1); row < ROWS; row += kWarps) {
             float x[NG];
             const int i = row0 + row;
             const bool live = row < rows;
             const int t = live ? i / p.group : 0, hd = live ? i - t * p.group : 0;
             const long long src = (static_cast<long long>(item_b) * p.q_len + t) * p.q_stride +
-                                  static_cast<long long>(kvh * p.group + hd) * D;
+                                  static_cast<long long>(kvh * p.group + hd) * D + lane * NG;
             float big = 0.0f;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                x[g] = 0.0f;
+            for (int k = 0; k < NG; ++k) {
+                x[k] = 0.0f;
                 if (live)
-                    x[g] = PARTS == 2 ? static_cast<const float*>(p.q)[src + 32 * g + lane]
-                                      : __bfloat162float(static_cast<const __nv_bfloat16*>(p.q)[src + 32 * g + lane]);
-                big = fmaxf(big, fabsf(x[g]));
+                    x[k] = PARTS == 2 ? static_cast<const float*>(p.q)[src + k]
+                                      : __bfloat162float(static_cast<const __nv_bfloat16*>(p.q)[src + k]);
+                big = fmaxf(big, fabsf(x[k]));
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
             // big * 2^f in [2^14, 2^15); f kept where both 2^f and the factor below are normal
             const int f = big > 0.0f ? max(-100, min(126, 14 - (static_cast<int>((__float_as_uint(big) >> 23) & 255) - 127))) : 0;
             const float up = pow2i(f);
-            // lane j of a group: slot (c = j / 8, i = j % 8).  MMA step (i & 3) >> 1; k index within it
-            const int i8 = lane & 7, cc = lane >> 3, st = (i8 & 3) >> 1;
-            const bool odd = i8 & 1;               // second k half, codes carry a factor 16
-            const int half_at = i8 >> 2;           // low or high half of the pair
-            const __half sixteenth = __ushort_as_half(0x2C00);
-            float sum[PARTS][NG];
+            constexpr int kSpan = 32 / NG;         // lanes of a group
+            const int g = lane / kSpan;
+            float sum[PARTS] = {};
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const float y = x[g] * up;         // |y| < 2^15
+            for (int k = 0; k < NG; ++k) {
+                const float y = x[k] * up;         // |y| < 2^15
+                // dim j of its group is slot (c = j / 8, i = j % 8): MMA step (i & 3) >> 1, k half i & 1 (where the
+                // codes carry a factor 16), pair c, element i >> 2
+                const int j = (lane % kSpan) * NG + k, c = j >> 3, i8 = j & 7, st = (i8 & 3) >> 1;
                 // PARTS 2: multiples of 16 and of 2^-7 -- 11 bits each, so that a group's sum of products is exact
                 __half v[PARTS];
                 v[0] = __float2half_rn(PARTS == 2 ? rintf(y * 0.0625f) * 16.0f : y);
@@ -444,33 +489,30 @@ __global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4
 #pragma unroll
                 for (int e = 0; e < PARTS; ++e) {
                     const int col = column_of<PARTS>(row, e);
-                    sum[e][g] = __half2float(v[e]);
-                    reinterpret_cast<__half*>(s_q + (((col >> 3) * NG + g) * 2 + st) * 32 + (col & 7) * 4 + cc)[(odd ? 2 : 0) + half_at] =
-                        odd ? __hmul(v[e], sixteenth) : v[e];
+                    sum[e] += __half2float(v[e]);
+                    reinterpret_cast<__half*>(s_q + (((col >> 3) * NG + g) * 2 + st) * 32 + (col & 7) * 4 + c)[2 * (i8 & 1) + (i8 >> 2)] =
+                        __hmul(v[e], __ushort_as_half(i8 & 1 ? 0x2C00 : 0x3C00));     // 1/16 or 1
                 }
             }
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1)
+            for (int o = kSpan / 2; o > 0; o >>= 1)
 #pragma unroll
-                for (int e = 0; e < PARTS; ++e)
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) sum[e][g] += __shfl_xor_sync(0xffffffffu, sum[e][g], o);
+                for (int e = 0; e < PARTS; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
             // offset fragment: k = g holds the group sum * 2^-6 in fp16, k = NG + g what that rounding left
-            if (lane < 2 * NG) {
+            if (lane % kSpan < 2) {
+                const int k = lane % kSpan * NG + g;
 #pragma unroll
                 for (int e = 0; e < PARTS; ++e) {
-                    float v = 0.0f;
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) v = (lane & (NG - 1)) == g ? sum[e][g] * 0.015625f : v;
+                    const float v = sum[e] * 0.015625f;
                     const __half h = __float2half_rn(v);
                     const int col = column_of<PARTS>(row, e);
-                    reinterpret_cast<__half*>(s_off + (col >> 3) * 32 + (col & 7) * 4 + ((lane & 7) >> 1))[(lane >> 3) * 2 + (lane & 1)] =
-                        lane < NG ? h : __float2half_rn(v - __half2float(h));
+                    reinterpret_cast<__half*>(s_off + (col >> 3) * 32 + (col & 7) * 4 + ((k & 7) >> 1))[(k >> 3) * 2 + (k & 1)] =
+                        k < NG ? h : __float2half_rn(v - __half2float(h));
                 }
             }
             if (lane < PARTS) s_fac[column_of<PARTS>(row, lane)] = p.scale * pow2i(24 - f);
         }
-        named_bar(1, kThreads);
+        __syncthreads();
 
         // this lane's columns 2 c4 and 2 c4 + 1 of each tile: the last position their rows see, and the first
         int hi[CT][2];
@@ -514,22 +556,31 @@ __global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4
         int E = 0;
         float limit = shift_of(0) + kLazy;
         const uint32_t m0 = hide(0x000F000Fu), m1 = hide(0x00F000F0u), one = hide(0x64006400u);
+        const uint32_t div16 = hide(0x2C002C00u), off16 = hide(0xD480D480u);     // 1/16, -72
 
-        auto tile = [&](const uint8_t* st, int pos) {
-            const uint8_t* kcode = st + warp * F::CODES;
-            const uint8_t* vcode = kcode + kWarps * F::CODES;
-            const uint8_t* kscale = st + 2 * kWarps * F::CODES + warp * F::SCALES;
-            const uint8_t* vscale = kscale + kWarps * F::SCALES;
-            // ---- scores: y[a][h][j] of row position krow + 8 h and column 2 c4 + j.  Rows r and r ^ 1 are
-            // swapped for every second pair: it spreads the V rows of one load over both halves of the banks.
-            const int krow = r ^ ((r >> 1) & 1);
+        // The lane's places in a slot.  Row positions: krow + 8 h, with rows r and r ^ 1 swapped for every second
+        // pair -- it spreads the V rows of one load over both halves of the banks.
+        const int krow = r ^ ((r >> 1) & 1);
+        const int vrow0 = 2 * c4 + (c4 & 1), vrow1 = 2 * c4 + 1 - (c4 & 1);
+        const uint32_t codes = smem_u32(ring) + warp * F::CODES;
+        const uint32_t scales = smem_u32(ring) + 2 * kWarps * F::CODES + warp * F::SCALES;
+        const uint32_t at_k = codes + krow * 16 * NG + c4 * 4 * NG;
+        const uint32_t at_v0 = codes + kWarps * F::CODES + vrow0 * 16 * NG + r * 2 * NG;
+        const uint32_t at_v1 = codes + kWarps * F::CODES + vrow1 * 16 * NG + r * 2 * NG;
+        const uint32_t at_ks = scales + krow * 2 * NG;
+        const uint32_t at_vs0 = scales + kWarps * F::SCALES + vrow0 * 2 * NG;
+        const uint32_t at_vs1 = scales + kWarps * F::SCALES + vrow1 * 2 * NG;
+        const uint32_t at_top = scales + kWarps * F::SCALES + lane * (NG == 8 ? 8 : 4);
+        auto tile = [&](int slot, int pos) {
+            const uint32_t st = slot * F::STAGE;
+            // ---- scores: y[a][h][j] of row position krow + 8 h and column 2 c4 + j
             float y[CT][2][2];
             {
                 uint32_t kw[2][NG], dw[2][NG / 2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    lds_words<NG>(kcode + (krow + 8 * h) * 16 * NG + c4 * 4 * NG, kw[h]);
-                    lds_words<NG / 2>(kscale + (krow + 8 * h) * 2 * NG, dw[h]);
+                    lds_words<NG>(at_k + st + h * 128 * NG, kw[h]);
+                    lds_words<NG / 2>(at_ks + st + h * 16 * NG, dw[h]);
                 }
                 float off[CT][4], part[CT][4];
                 // offset: A = the scales, k = g and again NG + g
@@ -599,7 +650,7 @@ __global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4
             if (NG >= 4 || lane < 16) {
                 constexpr int NW = NG == 8 ? 2 : 1;
                 uint32_t w[NW];
-                lds_words<NW>(vscale + lane * 4 * NW, w);
+                lds_words<NW>(at_top + st, w);
 #pragma unroll
                 for (int i = 0; i < NW; ++i) top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
             }
@@ -681,12 +732,11 @@ __global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4
             uint32_t vw[4][NG / 2], dv[4][NG / 2];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int row = (j >> 1) * 8 + 2 * c4 + ((j ^ c4) & 1);
-                lds_words<NG / 2>(vcode + row * 16 * NG + r * 2 * NG, vw[j]);
-                lds_words<NG / 2>(vscale + row * 2 * NG, dv[j]);
+                lds_words<NG / 2>((j & 1 ? at_v1 : at_v0) + st + (j >> 1) * 128 * NG, vw[j]);
+                lds_words<NG / 2>((j & 1 ? at_vs1 : at_vs0) + st + (j >> 1) * 16 * NG, dv[j]);
             }
             const __half2 kOff = bits_h2(0x64086408u);          // 1032
-            const __half2 kDiv = bits_h2(0x2C002C00u), kOff16 = bits_h2(0xD480D480u);   // 1/16, -72
+            const __half2 kDiv = bits_h2(div16), kOff16 = bits_h2(off16);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const uint32_t pick = g & 1 ? 0x7632 : 0x5410;
@@ -737,18 +787,22 @@ __global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4
         };
 
         // ---------------------------------------------------------- the item's chunks
-        const int count = static_cast<int>(seg1 - seg0);
-        int pos = (at.first + at.ch * kChunkTiles + warp) * kTilePos;
-        for (int i = 0; i < count; ++i) {
-            if (!dead) dead = !mbar_wait(full + use, parity);
-            if (pos < len) tile(ring + use * F::STAGE, pos);
-            pos += kChunkTiles * kTilePos;
-            __syncwarp();                          // every lane has read the slot
-            if (lane == 0) mbar_arrive(empty + use);
-            if (++use == kStages) {
-                use = 0;
-                parity ^= 1u;
+        const int count = seg1 - seg0;
+        const int pos0 = (at.first + at.ch * kChunkTiles + warp) * kTilePos;
+        for (int i = 0; i < count; ++i, ++done) {
+            if ((!bulk || (done & (kWarps - 1)) == warp) && done + kAhead < todo) {
+                Cursor c = at;
+                c.ch += i;
+                for (int k = 0; k < kAhead; ++k) step(c, p, tab, items);
+                if (!bulk) load_mine(done + kAhead, c);
+                else if (!dead) dead = !load(done + kAhead, c);
             }
+            const int slot = done % kStages;
+            if (!dead) dead = !mbar_wait(full + slot, (done / kStages) & 1);
+            const int pos = pos0 + i * (kChunkTiles * kTilePos);
+            if (pos < len) tile(slot, pos);
+            __syncwarp();                          // every lane has read the slot
+            if (lane == 0) mbar_arrive(empty + slot);
         }
         u = seg1;
         at.ch = at.chunks - 1;                     // on to the next item
@@ -761,7 +815,7 @@ __global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4
 #pragma unroll
                 for (int j = 0; j < 2; ++j) s_m[warp * COLS + 8 * a + 2 * c4 + j] = M[a][j];
         }
-        named_bar(1, kThreads);
+        __syncthreads();
         float wgt[CT][2];                          // this warp's weight for its columns
 #pragma unroll
         for (int a = 0; a < CT; ++a)
@@ -787,7 +841,7 @@ __global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4
         };
 #pragma unroll
         for (int g0 = 0; g0 < NG; g0 += F::SG) {
-            if (g0 > 0) named_bar(1, kThreads);
+            if (g0 > 0) __syncthreads();
 #pragma unroll
             for (int g = g0; g < g0 + F::SG; ++g)
 #pragma unroll
@@ -797,7 +851,7 @@ __global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4
                         *reinterpret_cast<float4*>(s_merge + (warp * COLS + 8 * a + 2 * c4 + j) * F::MROW + (g - g0) * 32 + 4 * r) =
                             make_float4(acc[2 * g][a][j] * wgt[a][j], acc[2 * g][a][2 + j] * wgt[a][j],
                                         acc[2 * g + 1][a][j] * wgt[a][j], acc[2 * g + 1][a][2 + j] * wgt[a][j]);
-            named_bar(1, kThreads);
+            __syncthreads();
             for (int i = threadIdx.x; i < rows * F::SG * 8; i += kThreads) {
                 const int row = i / (F::SG * 8), d4 = i - row * (F::SG * 8), col = column_of<PARTS>(row, 0);
                 float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -829,61 +883,64 @@ __global__ void __launch_bounds__(kThreads + 32, NG <= 4 && CT == 1 ? 2 : 1) kv4
 
         // ---------------------------------------------------------- join an item cut over CTAs
         const int cta0 = cta_at(line0), cta1 = cta_at(line1 - 1);
-        __threadfence();
-        named_bar(1, kThreads);
+        __syncthreads();                           // every thread's partials, made visible by thread 0's release
         if (threadIdx.x == 0) {
             const bool last = arrive_acq_rel(p.counters + cta0) == static_cast<unsigned int>(cta1 - cta0);
             if (last) p.counters[cta0] = 0;
             s_misc[1] = last;
         }
-        named_bar(1, kThreads);
+        __syncthreads();
         if (!s_misc[1]) continue;
-        __threadfence();
         const int n = cta1 - cta0 + 1;
         const int slot0 = real(start_of(cta0)) == item0 ? 0 : 1;   // only the first CTA may hold it in its second slot
         auto base = [&](int k) { return p.part + (static_cast<long long>(cta0 + k) * 2 + (k == 0 ? slot0 : 0)) * (ROWS * (D + 2)); };
-        const int outs = rows * (D / 4);
-        // threads that share one output: each takes a run of the CTAs
-        const int ways = max(1, min(min(n, kThreads / outs), min(F::MERGE / 16 / outs, kWarps * COLS / rows)));
-        const int way = threadIdx.x / outs;
-        for (int i = ways > 1 ? threadIdx.x - way * outs : threadIdx.x; i < outs;
-             i += ways > 1 ? outs : kThreads) {
-            if (ways > 1 && way >= ways) break;
-            const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
+        // the CTAs' weights for each row, a warp a row: w[row][k]; rows' sums in s_way
+        float* const w = s_merge;
+        for (int row = warp; row < rows; row += kWarps) {
             float top = kNone, L = 0.0f;
-            for (int k = 0; k < n; ++k) top = fmaxf(top, __ldcg(base(k) + ROWS * D + row * 2));
+            for (int k = lane; k < n; k += 32) top = fmaxf(top, __ldcg(base(k) + ROWS * D + row * 2));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (int k = lane; k < n; k += 32) {
+                const float2 ml = __ldcg(reinterpret_cast<const float2*>(base(k) + ROWS * D + row * 2));
+                const float f = ex2(ml.x - top);
+                w[row * n + k] = f;
+                L = fmaf(ml.y, f, L);
+            }
+            L = warp_sum(L);
+            if (lane == 0) s_way[row] = L;
+        }
+        // threads that share one output: each takes a run of the CTAs; their sums follow the weights
+        const int outs = rows * (D / 4);
+        const int room = (F::MERGE / 4 - rows * n - 3) / 4;
+        const int ways = max(1, min(min(n, kThreads / outs), room / outs));
+        const int way = ways > 1 ? threadIdx.x / outs : 0;
+        float4* const sums = reinterpret_cast<float4*>(s_merge + (rows * n + 3) / 4 * 4);
+        __syncthreads();
+        for (int i = threadIdx.x - way * outs; i < outs && way < ways; i += kThreads) {
+            const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const int per = (n + ways - 1) / ways, k0 = ways > 1 ? way * per : 0, k1 = min(n, k0 + per);
-#pragma unroll 4
+            const int per = (n + ways - 1) / ways, k0 = way * per, k1 = min(n, k0 + per);
+#pragma unroll 8
             for (int k = k0; k < k1; ++k) {
-                const float* b = base(k);
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>(b + ROWS * D + row * 2));
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(b + row * D + d));
-                const float w = ex2(ml.x - top);
-                L = fmaf(ml.y, w, L);
-                sum.x = fmaf(v.x, w, sum.x); sum.y = fmaf(v.y, w, sum.y);
-                sum.z = fmaf(v.z, w, sum.z); sum.w = fmaf(v.w, w, sum.w);
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(base(k) + row * D + d));
+                const float f = w[row * n + k];
+                sum.x = fmaf(v.x, f, sum.x); sum.y = fmaf(v.y, f, sum.y);
+                sum.z = fmaf(v.z, f, sum.z); sum.w = fmaf(v.w, f, sum.w);
             }
-            if (ways == 1) {
-                store4(p.out, PARTS == 1, out_at(row, d), sum, L == 0.0f ? 0.0f : 1.0f / L);
-            } else {
-                reinterpret_cast<float4*>(s_merge)[way * outs + i] = sum;
-                if (d == 0) s_way[way * rows + row] = L;
-                break;
-            }
+            if (ways == 1) store4(p.out, PARTS == 1, out_at(row, d), sum, s_way[row] == 0.0f ? 0.0f : 1.0f / s_way[row]);
+            else sums[way * outs + i] = sum;
         }
         if (ways > 1) {
-            named_bar(1, kThreads);
+            __syncthreads();
             for (int i = threadIdx.x; i < outs; i += kThreads) {
                 const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
                 float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                float L = 0.0f;
                 for (int k = 0; k < ways; ++k) {
-                    const float4 v = reinterpret_cast<const float4*>(s_merge)[k * outs + i];
+                    const float4 v = sums[k * outs + i];
                     sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-                    L += s_way[k * rows + row];
                 }
-                store4(p.out, PARTS == 1, out_at(row, d), sum, L == 0.0f ? 0.0f : 1.0f / L);
+                store4(p.out, PARTS == 1, out_at(row, d), sum, s_way[row] == 0.0f ? 0.0f : 1.0f / s_way[row]);
             }
         }
     }
@@ -903,10 +960,10 @@ cudaError_t launch_cfg(Kv4Attn p, int sms, int max_ctas, cudaStream_t stream) {
         configured[dev & 63] = true;
     }
     // One wave: two CTAs an SM where registers and 227 KB of shared memory hold two.
-    const int per_sm = NG <= 4 && CT == 1 && 2 * (smem + 1024) <= 227 * 1024 ? 2 : 1;
+    const int per_sm = NG * CT <= 4 && 2 * (smem + 1024) <= 227 * 1024 ? 2 : 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(std::min(per_sm * sms, max_ctas));
-    cfg.blockDim = dim3(kThreads + 32);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
