@@ -8,9 +8,15 @@
 //
 // Bound: one read and one write of the row, so HBM for a batch and latency
 // for one row.  A row belongs to one thread-block cluster, its vocabulary
-// dealt out to the cluster's CTAs in chunks; a CTA counts the history's hits
-// of its chunk in shared memory (integer atomics: their order is immaterial),
-// adds the biases with one warp in list order, and streams the chunk once.
+// dealt out to the cluster's CTAs in chunks of 8192.  A CTA asks for its chunk
+// first, then finds the tokens that need more than a mask: it counts the
+// history's hits of the chunk in shared memory (integer atomics: their order
+// is immaterial), adds the biases with one warp in list order, and lists each
+// such token once.  The chunk is then streamed with a mask, a store and a
+// maximum a logit; the listed tokens are finished by one thread each, so that
+// their divisions are not paid by whole warps.  (Tables read and keys formed
+// for every logit: 75 instructions each, 105 us for 96 x 128256 against the
+// floor of 16.)
 // The greedy token is reduced over the cluster through distributed shared
 // memory: no workspace and no second launch.
 // Every step of the arithmetic is one rounded fp32 operation, as written.
@@ -21,8 +27,8 @@
 namespace alj {
 namespace {
 
-constexpr int kLThreads = 1024;
-constexpr int kPer = 8;                             // logits a thread holds
+constexpr int kLThreads = 512;
+constexpr int kPer = 16;                            // logits a thread holds, in runs of 4
 constexpr int kChunk = kLThreads * kPer;            // vocabulary entries counted at a time
 constexpr int kMaxCluster = 16;
 
@@ -30,11 +36,6 @@ __device__ __forceinline__ unsigned long long order_key(float v, int i) {
     uint32_t b = __float_as_uint(v + 0.0f);         // -0 and +0 tie
     b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
     return (static_cast<unsigned long long>(b) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(i));
-}
-
-template <typename T>
-__device__ __forceinline__ float as_float(T v) {
-    return static_cast<float>(v);
 }
 
 // A thread's kPer entries are 4-wide runs: i = base + 4 thread + 4 kLThreads j + 0..3.
@@ -62,14 +63,32 @@ __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, int
     }
 }
 
+// A float as an unsigned number of the same order; -0 counts as +0.
+__device__ __forceinline__ uint32_t order_bits(float v) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kLThreads) logits_kernel(const LogitsArgs a, int share, int vec_in, int vec_out) {
-    extern __shared__ uint32_t s_count[];           // [kChunk], then the biases [kChunk]
+__global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a, int share, int vec_in, int vec_out) {
+    extern __shared__ uint4 s_tables[];             // hit counts [kChunk], biases [kChunk], listed tokens [kChunk] (16 bits)
+    uint32_t* const s_count = reinterpret_cast<uint32_t*>(s_tables);
     float* const s_bias = reinterpret_cast<float*>(s_count + kChunk);
-    __shared__ unsigned long long s_key[32];
+    uint16_t* const s_list = reinterpret_cast<uint16_t*>(s_bias + kChunk);
+    __shared__ uint32_t s_mark[kChunk / 32];        // tokens in the list
+    __shared__ unsigned long long s_key[kLThreads / 32];
     __shared__ unsigned long long s_best[kMaxCluster];
+    __shared__ uint64_t s_bar;                      // rank 0: the cluster's keys have arrived
+    __shared__ int s_listed;
     const int row = blockIdx.y, rank = blockIdx.x, ranks = gridDim.x;
     const int lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(&s_bar, 1);
+        fence_mbar_init();
+        mbar_arrive_expect_tx(&s_bar, ranks * 8);
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // waited for before the first remote store
     pdl_launch_dependents();
     pdl_wait();
 
@@ -78,73 +97,79 @@ __global__ void __launch_bounds__(kLThreads) logits_kernel(const LogitsArgs a, i
     const int* hist = a.history + static_cast<long long>(row) * a.history_stride;
     const int n_hist = a.history ? max(0, min(__ldg(a.history_len + row), a.history_stride)) : 0;
     const int n_bias = a.bias_tokens ? max(0, min(__ldg(a.bias_len + row), a.bias_stride)) : 0;
-    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
-    if (n_hist > 0) {
-        rep = __ldg(a.penalties + row * 3LL);
-        freq = __ldg(a.penalties + row * 3LL + 1);
-        pres = __ldg(a.penalties + row * 3LL + 2);
-    }
+    const uint32_t* allow = a.allow ? a.allow + static_cast<long long>(row) * a.allow_stride : nullptr;
     const int v0 = min(a.vocab, rank * share), v1 = min(a.vocab, v0 + share);
-    unsigned long long best = 0ull;
+    unsigned long long best = 0ull;                 // 0: no candidate
     for (int c0 = v0; c0 < v1; c0 += kChunk) {
-        const int c1 = min(v1, c0 + kChunk);
+        const int c1 = min(v1, c0 + kChunk), n = c1 - c0;
         float x[kPer / 4][4];
+        uint32_t ok[kPer / 4];
 #pragma unroll
         for (int j = 0; j < kPer / 4; ++j) {
             const int i = c0 + 4 * (j * kLThreads + static_cast<int>(threadIdx.x));
             load4<T>(in + min(i, c1), c1 - i, vec_in != 0, x[j]);
+            ok[j] = 15u;
+            if (allow && i < c1) ok[j] = __ldg(allow + (i >> 5)) >> (i & 31);
+            if (i + 4 > c1) ok[j] &= i < c1 ? (1u << (c1 - i)) - 1u : 0u;
         }
-        if (n_hist > 0) {
-            for (int i = threadIdx.x; i < kChunk; i += kLThreads) s_count[i] = 0u;
-        }
-        if (n_bias > 0) {
-            for (int i = threadIdx.x; i < kChunk; i += kLThreads) s_bias[i] = 0.0f;
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < n_hist; i += kLThreads) {
-            const int t = __ldg(hist + i);
-            if (t >= c0 && t < c1) atomicAdd(s_count + (t - c0), 1u);
-        }
-        if (n_bias > 0 && threadIdx.x >= kLThreads - 32) {   // the last warp, 32 entries at a time, in order
-            for (int i0 = 0; i0 < n_bias; i0 += 32) {
-                const int i = i0 + lane;
-                const int t = i < n_bias ? __ldg(a.bias_tokens + static_cast<long long>(row) * a.bias_stride + i) : -1;
-                const float b = i < n_bias ? __ldg(a.bias_values + static_cast<long long>(row) * a.bias_stride + i) : 0.0f;
-                const bool mine = t >= c0 && t < c1;
-                const unsigned int same = __match_any_sync(0xffffffffu, mine ? t : -1 - lane);
-                float sum = mine ? s_bias[t - c0] : 0.0f;
-                // equal tokens of these 32: the lowest lane adds them all, in lane order
-                const bool leads = (same & ((1u << lane) - 1u)) == 0u;
-                for (int o = 0; o < 32; ++o) {
-                    const float v = __shfl_sync(0xffffffffu, b, o);
-                    if (mine && leads && ((same >> o) & 1u)) sum = __fadd_rn(sum, v);
+        const bool special = n_hist > 0 || n_bias > 0;
+        if (special) {
+            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+            const int words = (n_bias > 0 ? 2 : 1) * kChunk / 4;
+            for (int i = threadIdx.x; i < words; i += kLThreads) s_tables[i] = zero;
+            for (int i = threadIdx.x; i < kChunk / 32; i += kLThreads) s_mark[i] = 0u;
+            if (threadIdx.x == 0) s_listed = 0;
+            __syncthreads();
+            auto list = [&](int t) {
+                const uint32_t bit = 1u << (t & 31);
+                if (!(atomicOr(s_mark + (t >> 5), bit) & bit)) s_list[atomicAdd(&s_listed, 1)] = static_cast<uint16_t>(t);
+            };
+#pragma unroll 8
+            for (int i = threadIdx.x; i < n_hist; i += kLThreads) {
+                const int t = __ldg(hist + i) - c0;
+                if (static_cast<unsigned int>(t) < static_cast<unsigned int>(n)) {
+                    atomicAdd(s_count + t, 1u);
+                    list(t);
                 }
-                if (mine && leads) s_bias[t - c0] = sum;
-                __syncwarp();
             }
+            if (n_bias > 0 && threadIdx.x >= kLThreads - 32) {   // the last warp, 32 entries at a time, in order
+                for (int i0 = 0; i0 < n_bias; i0 += 32) {
+                    const long long i = static_cast<long long>(row) * a.bias_stride + i0 + lane;
+                    const int t = i0 + lane < n_bias ? __ldg(a.bias_tokens + i) - c0 : -1;
+                    const float b = i0 + lane < n_bias ? __ldg(a.bias_values + i) : 0.0f;
+                    const bool mine = static_cast<unsigned int>(t) < static_cast<unsigned int>(n);
+                    const unsigned int same = __match_any_sync(0xffffffffu, mine ? t : -1 - lane);
+                    float sum = mine ? s_bias[t] : 0.0f;
+                    const bool leads = (same & ((1u << lane) - 1u)) == 0u;
+                    if (__any_sync(0xffffffffu, !leads)) {       // equal tokens: the lowest lane adds them in lane order
+                        for (int o = 0; o < 32; ++o) {
+                            const float v = __shfl_sync(0xffffffffu, b, o);
+                            if ((same >> o) & 1u) sum = __fadd_rn(sum, v);
+                        }
+                    } else {
+                        sum = __fadd_rn(sum, b);
+                    }
+                    if (mine && leads) {
+                        s_bias[t] = sum;
+                        list(t);
+                    }
+                    __syncwarp();
+                }
+            }
+            __syncthreads();
         }
-        __syncthreads();
+        // stream the chunk; listed tokens keep their logits and are no candidates yet
+        float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < kPer / 4; ++j) {
-            const int i = c0 + 4 * (j * kLThreads + static_cast<int>(threadIdx.x));
-            if (i >= c1) continue;
-            const uint32_t bits = a.allow ? __ldg(a.allow + static_cast<long long>(row) * a.allow_stride + (i >> 5)) >> (i & 31) : 15u;
+            const int at = 4 * (j * kLThreads + static_cast<int>(threadIdx.x)), i = c0 + at;
+            const uint32_t marks = special && at < n ? s_mark[at >> 5] >> (at & 31) : 0u;
             float y[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float v = x[j][e];
-                const int at = i - c0 + e;
-                if (n_hist > 0) {
-                    const uint32_t n = s_count[at];
-                    if (n > 0u) {
-                        v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-                        v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, static_cast<float>(n))), pres);
-                    }
-                }
-                if (n_bias > 0) v = __fadd_rn(v, s_bias[at]);
-                const bool ok = (bits >> e) & 1u;
-                y[e] = ok ? v : -INFINITY;
-                if (ok && i + e < c1 && v == v) best = max(best, order_key(v, i + e));
+                y[e] = ((ok[j] | marks) >> e) & 1u ? x[j][e] : -INFINITY;
+                x[j][e] = (ok[j] & ~marks) >> e & 1u ? x[j][e] : __int_as_float(0x7FFFFFFF);   // not a candidate
+                top = fmaxf(top, x[j][e]);          // a NaN does not count
             }
             if (vec_out && i + 4 <= c1) {
                 *reinterpret_cast<float4*>(out + i) = make_float4(y[0], y[1], y[2], y[3]);
@@ -154,28 +179,61 @@ __global__ void __launch_bounds__(kLThreads) logits_kernel(const LogitsArgs a, i
                     if (i + e < c1) out[i + e] = y[e];
             }
         }
-        __syncthreads();                            // the tables are reused
+        if (special) {                              // one thread a listed token, after the stores above
+            __syncthreads();
+            for (int k = threadIdx.x; k < s_listed; k += kLThreads) {
+                const int t = s_list[k], i = c0 + t;
+                float v = static_cast<float>(in[i]);
+                const uint32_t hits = s_count[t];
+                if (hits > 0u) {
+                    const float* pen = a.penalties + row * 3LL;
+                    const float rep = __ldg(pen), freq = __ldg(pen + 1), pres = __ldg(pen + 2);
+                    v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+                    v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, static_cast<float>(hits))), pres);
+                }
+                if (n_bias > 0) v = __fadd_rn(v, s_bias[t]);
+                const bool may = !allow || ((__ldg(allow + (i >> 5)) >> (i & 31)) & 1u);
+                out[i] = may ? v : -INFINITY;
+                if (may && v == v) best = max(best, order_key(v, i));
+            }
+        }
+        // the warp's largest streamed candidate and its lowest index
+        if (a.token) {
+            const uint32_t high = __reduce_max_sync(0xffffffffu, order_bits(top));
+            unsigned int first = 0xFFFFFFFFu;
+            if (order_bits(top) == high) {
+#pragma unroll
+                for (int j = kPer / 4 - 1; j >= 0; --j)
+#pragma unroll
+                    for (int e = 3; e >= 0; --e)
+                        if (x[j][e] == top) first = c0 + 4 * (j * kLThreads + static_cast<int>(threadIdx.x)) + e;
+            }
+            first = __reduce_min_sync(0xffffffffu, first);
+            if (first != 0xFFFFFFFFu) best = max(best, (static_cast<unsigned long long>(high) << 32) | (0xFFFFFFFFu - first));
+        }
+        if (c0 + kChunk < v1) __syncthreads();      // the tables are reused
     }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA has started, its barrier is ready
     if (!a.token) return;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     if (lane == 0) s_key[threadIdx.x >> 5] = best;
-    // every CTA of the cluster has started before its shared memory is written
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (threadIdx.x < 32) {
-        best = s_key[lane];
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    best = lane < kLThreads / 32 ? s_key[lane] : 0ull;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-        if (lane == 0) {
-            uint32_t to;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(s_best + rank)), "r"(0));
-            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(best) : "memory");
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane == 0) {                                // to rank 0, which counts the bytes: no fence over the row's stores
+        uint32_t to, bar;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(s_best + rank)));
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(bar) : "r"(smem_u32(&s_bar)));
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.u64 [%0], %1, [%2];" ::"r"(to), "l"(best), "r"(bar)
+                     : "memory");
+        if (rank == 0) {
+            mbar_wait(&s_bar, 0);
+            for (int k = 0; k < ranks; ++k) best = max(best, s_best[k]);
+            a.token[row] = best ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(best)) : -1;
         }
-    }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank == 0 && threadIdx.x == 0) {
-        for (int k = 0; k < ranks; ++k) best = max(best, s_best[k]);
-        a.token[row] = best ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(best)) : -1;
     }
 }
 
@@ -185,17 +243,15 @@ cudaError_t launch_typed(const LogitsArgs& a, int sms, cudaStream_t stream) {
     static bool configured[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
-    const int smem = kChunk * 8;
+    const int smem = kChunk * 10;
     if (!configured[dev & 63]) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         configured[dev & 63] = true;
     }
-    // CTAs a row: up to 16 while that fills no more than the machine once (2
-    // CTAs an SM), else 8, which every GPC can place; no more than a row has
-    // 1024-entry pieces.
-    int ranks = static_cast<long long>(a.rows) * kMaxCluster <= 2LL * sms ? kMaxCluster : 8;
+    // 16 CTAs a row (one chunk each for vocabularies up to 131072); fewer where a row has no 1024 entries for each
+    int ranks = kMaxCluster;
     while (ranks > 1 && (a.vocab + ranks - 1) / ranks < 1024) ranks >>= 1;
     const int share = ((a.vocab + ranks - 1) / ranks + 31) / 32 * 32;   // whole words of the mask
     auto aligned = [](const void* p, long long stride, size_t bytes) {

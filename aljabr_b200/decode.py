@@ -174,7 +174,7 @@ class LlamaNf4Decoder:
             native.call("aljabr_blackwell_logits_process_dev", out.data_ptr(), V, logits, native.KV_F32, V, 1, V,
                         hist.data_ptr(), live.data_ptr(), hist.shape[1], pen.data_ptr(), ptr(bt), ptr(bv), ptr(bl),
                         0 if bt is None else bt.numel(), ptr(words), 0 if words is None else words.numel(),
-                        best.data_ptr(), current_stream(dev))
+                        best.data_ptr(), current_stream(dev.index))
             token = int(best)
             if token < 0:
                 break

@@ -14,8 +14,6 @@ layout and the arithmetic are described in include/aljabr_blackwell.h.
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import native
@@ -24,8 +22,22 @@ _DTYPES = {torch.float32: native.KV_F32, torch.bfloat16: native.KV_BF16}
 _LEGACY_STREAM = 1      # cudaStreamLegacy: the C-ABI reads 0 as "the library's own stream"
 
 
-def current_stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream or _LEGACY_STREAM
+# torch.cuda.current_stream(device).cuda_stream without building the Stream object (2.6 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def current_stream(index: int) -> int:
+    return _raw_stream(index) or _LEGACY_STREAM
+
+
+_several = torch.cuda.device_count() > 1
+
+
+def select_device(index: int) -> None:
+    """The library launches on the calling thread's device; where there are several, each call names its own."""
+    if _several:
+        native.call("aljabr_blackwell_init", index)
 
 
 def dtype_id(t: torch.Tensor, what: str) -> int:
@@ -56,31 +68,37 @@ class Kv4Cache:
             raise bad(f"cache data must be {size} contiguous uint8 on a CUDA device")
         self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
         self.data, self.device, self.bytes = data, data.device, size
-        native.call("aljabr_blackwell_init", self.device.index or 0)
+        self._index = data.get_device()
+        native.call("aljabr_blackwell_init", self._index)
+        lib = native.lib()
+        self._append, self._read = lib.aljabr_blackwell_kv4_append_dev, lib.aljabr_blackwell_kv4_read_dev
+        self._attend, self._work_size = lib.aljabr_blackwell_kv4_attention_dev, lib.aljabr_blackwell_kv4_attention_workspace_size
+        self._row = kv_heads * head_dim
         self._shape = (data.data_ptr(), pages, page_size, kv_heads, head_dim)
         self._work = {}      # stream -> (workspace, bytes): calls on one stream never overlap
 
     # -- checks ----------------------------------------------------------------
     def _rows(self, t: torch.Tensor, tokens: int, what: str) -> int:
         """Elements between the rows of t: [tokens, kv_heads, head_dim] or [tokens, kv_heads * head_dim]."""
-        row = self.kv_heads * self.head_dim
-        if t.device != self.device or t.dim() not in (2, 3) or t.shape[0] != tokens or t[0:1].numel() != row * min(tokens, 1):
-            raise bad(f"{what} must be [{tokens}, {self.kv_heads}, {self.head_dim}] on {self.device}, not {tuple(t.shape)}")
-        st = t.stride()
-        if st[-1] != 1 or (t.dim() == 3 and st[1] != self.head_dim and self.kv_heads > 1):
-            raise bad(f"{what}: the heads of a row must be contiguous (strides {st})")
-        return st[0] if tokens > 1 else row
+        shape, st = t.shape, t.stride()
+        if len(shape) == 3:
+            ok = shape == (tokens, self.kv_heads, self.head_dim) and (st[1] == self.head_dim or self.kv_heads == 1)
+        else:
+            ok = shape == (tokens, self._row)
+        if not ok or t.get_device() != self._index or st[-1] != 1:
+            raise bad(f"{what} must be [{tokens}, {self.kv_heads}, {self.head_dim}] on {self.device} with contiguous rows, "
+                      f"not {tuple(shape)} with strides {st} on {t.device}")
+        return st[0] if tokens > 1 else self._row
 
     def _ints(self, t: torch.Tensor, shape: tuple, what: str) -> int:
-        if t.dtype != torch.int32 or t.device != self.device or tuple(t.shape) != shape or not t.is_contiguous():
+        if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != self._index or not t.is_contiguous():
             raise bad(f"{what} must be contiguous int32 {shape} on {self.device}")
         return t.data_ptr()
 
     def _dense(self, t, tokens: int, dtype, what: str):
         if t is None:
             return None
-        if t.dtype != dtype or not t.is_contiguous() or t.device != self.device or \
-                t.numel() != tokens * self.kv_heads * self.head_dim:
+        if t.dtype is not dtype or not t.is_contiguous() or t.get_device() != self._index or t.numel() != tokens * self._row:
             raise bad(f"{what} must be contiguous {dtype} [{tokens}, {self.kv_heads}, {self.head_dim}] on {self.device}")
         return t.data_ptr()
 
@@ -89,29 +107,35 @@ class Kv4Cache:
         """Quantise the rows k, v into slots[i] = page * page_size + position (-1: skip the row).
 
         k_back / v_back (both or neither) receive the values the cache now holds."""
+        select_device(self._index)
         n = slots.shape[0]
         kind = dtype_id(k, "k")
-        if v.dtype != k.dtype:
+        if v.dtype is not k.dtype:
             raise bad(f"k is {k.dtype}, v is {v.dtype}")
         ks, vs = self._rows(k, n, "k"), self._rows(v, n, "v")
-        native.call("aljabr_blackwell_kv4_append_dev", *self._shape, k.data_ptr(), v.data_ptr(), kind, ks, vs,
-                    self._ints(slots, (n,), "slots"), n, self._dense(k_back, n, k.dtype, "k_back"),
-                    self._dense(v_back, n, k.dtype, "v_back"), stream or current_stream(self.device))
+        rc = self._append(*self._shape, k.data_ptr(), v.data_ptr(), kind, ks, vs, self._ints(slots, (n,), "slots"), n,
+                          self._dense(k_back, n, k.dtype, "k_back"), self._dense(v_back, n, k.dtype, "v_back"),
+                          stream or current_stream(self._index))
+        if rc:
+            native.check(rc)
 
     def read(self, slots: torch.Tensor, dtype=torch.float32, k_out=None, v_out=None, stream=None):
         """Rows of the given slots as (k, v), [n, kv_heads, head_dim] each; zeros where a slot is -1."""
+        select_device(self._index)
         n = slots.shape[0]
         if k_out is None and v_out is None:
             k_out, v_out = (torch.empty(n, self.kv_heads, self.head_dim, dtype=dtype, device=self.device) for _ in range(2))
         some = k_out if k_out is not None else v_out
-        native.call("aljabr_blackwell_kv4_read_dev", self._dense(k_out, n, some.dtype, "k_out"),
-                    self._dense(v_out, n, some.dtype, "v_out"), dtype_id(some, "k_out"), *self._shape,
-                    self._ints(slots, (n,), "slots"), n, stream or current_stream(self.device))
+        rc = self._read(self._dense(k_out, n, some.dtype, "k_out"), self._dense(v_out, n, some.dtype, "v_out"),
+                        dtype_id(some, "k_out"), *self._shape, self._ints(slots, (n,), "slots"), n,
+                        stream or current_stream(self._index))
+        if rc:
+            native.check(rc)
         return k_out, v_out
 
     # -- attention -------------------------------------------------------------
     def _workspace(self, q_len: int, q_heads: int, stream: int):
-        need = native.lib().aljabr_blackwell_kv4_attention_workspace_size(q_len, q_heads, self.kv_heads, self.head_dim)
+        need = self._work_size(q_len, q_heads, self.kv_heads, self.head_dim)
         if need < 0:
             native.check(int(need))
         have = self._work.get(stream)
@@ -119,7 +143,7 @@ class Kv4Cache:
             # zeroed on torch's current stream; another stream's kernels neither wait for that nor hold the
             # old buffer, so there the device is waited for, once
             new = (torch.zeros(need, dtype=torch.uint8, device=self.device), need)
-            if stream != current_stream(self.device):
+            if stream != current_stream(self._index):
                 torch.cuda.synchronize(self.device)
             have = self._work[stream] = new
         return have
@@ -130,26 +154,28 @@ class Kv4Cache:
 
         block_table: int32 [batch, pages a sequence], or None where sequence b is page b.  scale: 1 / sqrt(head_dim)
         by default.  Returns out, contiguous, of q's type."""
-        if q.dim() != 4 or q.shape[3] != self.head_dim or q.device != self.device:
-            raise bad(f"q must be [batch, q_len, q_heads, {self.head_dim}] on {self.device}, not {tuple(q.shape)}")
-        batch, q_len, q_heads, D = q.shape
-        st = q.stride()
-        row = q_heads * D
-        q_stride = st[1] if q_len > 1 else st[0] if batch > 1 else row
+        select_device(self._index)
+        shape, st = q.shape, q.stride()
+        if len(shape) != 4 or shape[3] != self.head_dim or q.get_device() != self._index:
+            raise bad(f"q must be [batch, q_len, q_heads, {self.head_dim}] on {self.device}, not {tuple(shape)} on {q.device}")
+        batch, q_len, q_heads, D = shape
+        q_stride = st[1] if q_len > 1 else st[0] if batch > 1 else q_heads * D
         if st[3] != 1 or (q_heads > 1 and st[2] != D) or (q_len > 1 and batch > 1 and st[0] != q_len * st[1]):
             raise bad(f"q: the heads of a token must be contiguous and the tokens evenly spaced (strides {st})")
         kind = dtype_id(q, "q")
         if out is None:
             out = torch.empty(batch, q_len, q_heads, D, dtype=q.dtype, device=self.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous():
-            raise bad(f"out must be contiguous {q.dtype} {tuple(q.shape)} on {self.device}")
+        elif out.shape != shape or out.dtype is not q.dtype or out.get_device() != self._index or not out.is_contiguous():
+            raise bad(f"out must be contiguous {q.dtype} {tuple(shape)} on {self.device}")
         table, width = None, 0
         if block_table is not None:
             width = block_table.shape[-1]
             table = self._ints(block_table, (batch, width), "block_table")
-        stream = stream or current_stream(self.device)
+        stream = stream or current_stream(self._index)
         work, size = self._workspace(q_len, q_heads, stream)
-        native.call("aljabr_blackwell_kv4_attention_dev", out.data_ptr(), q.data_ptr(), kind, q_stride, *self._shape,
-                    table, width, self._ints(seq_lens, (batch,), "seq_lens"), batch, q_len, q_heads, window,
-                    1.0 / math.sqrt(D) if scale is None else scale, soft_cap, work.data_ptr(), size, stream)
+        rc = self._attend(out.data_ptr(), q.data_ptr(), kind, q_stride, *self._shape, table, width,
+                          self._ints(seq_lens, (batch,), "seq_lens"), batch, q_len, q_heads, window,
+                          D ** -0.5 if scale is None else scale, soft_cap, work.data_ptr(), size, stream)
+        if rc:
+            native.check(rc)
         return out
