@@ -30,6 +30,7 @@ namespace {
 constexpr int kLThreads = 512;
 constexpr int kPer = 16;                            // logits a thread holds, in runs of 4
 constexpr int kChunk = kLThreads * kPer;            // vocabulary entries counted at a time
+constexpr int kSeen = 8;                            // history entries a thread holds
 constexpr int kMaxCluster = 16;
 
 __device__ __forceinline__ unsigned long long order_key(float v, int i) {
@@ -95,8 +96,21 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
     const T* in = static_cast<const T*>(a.logits) + row * a.in_stride;
     float* out = a.out + row * a.out_stride;
     const int* hist = a.history + static_cast<long long>(row) * a.history_stride;
-    const int n_hist = a.history ? max(0, min(__ldg(a.history_len + row), a.history_stride)) : 0;
-    const int n_bias = a.bias_tokens ? max(0, min(__ldg(a.bias_len + row), a.bias_stride)) : 0;
+    // everything that does not depend on the lengths is asked for along with them
+    const int hist_len = a.history ? __ldg(a.history_len + row) : 0;
+    const int bias_len = a.bias_tokens ? __ldg(a.bias_len + row) : 0;
+    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    if (a.history) {
+        rep = __ldg(a.penalties + row * 3LL);
+        freq = __ldg(a.penalties + row * 3LL + 1);
+        pres = __ldg(a.penalties + row * 3LL + 2);
+    }
+    int seen[kSeen];                                // the first history entries
+#pragma unroll
+    for (int j = 0; j < kSeen; ++j) {
+        const int i = j * kLThreads + static_cast<int>(threadIdx.x);
+        seen[j] = a.history && i < a.history_stride ? __ldg(hist + i) : -1;
+    }
     const uint32_t* allow = a.allow ? a.allow + static_cast<long long>(row) * a.allow_stride : nullptr;
     const int v0 = min(a.vocab, rank * share), v1 = min(a.vocab, v0 + share);
     unsigned long long best = 0ull;                 // 0: no candidate
@@ -112,6 +126,7 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
             if (allow && i < c1) ok[j] = __ldg(allow + (i >> 5)) >> (i & 31);
             if (i + 4 > c1) ok[j] &= i < c1 ? (1u << (c1 - i)) - 1u : 0u;
         }
+        const int n_hist = max(0, min(hist_len, a.history_stride)), n_bias = max(0, min(bias_len, a.bias_stride));
         const bool special = n_hist > 0 || n_bias > 0;
         if (special) {
             const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
@@ -124,14 +139,17 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
                 const uint32_t bit = 1u << (t & 31);
                 if (!(atomicOr(s_mark + (t >> 5), bit) & bit)) s_list[atomicAdd(&s_listed, 1)] = static_cast<uint16_t>(t);
             };
-#pragma unroll 8
-            for (int i = threadIdx.x; i < n_hist; i += kLThreads) {
-                const int t = __ldg(hist + i) - c0;
+            auto count = [&](int token) {
+                const int t = token - c0;
                 if (static_cast<unsigned int>(t) < static_cast<unsigned int>(n)) {
                     atomicAdd(s_count + t, 1u);
                     list(t);
                 }
-            }
+            };
+#pragma unroll
+            for (int j = 0; j < kSeen; ++j)
+                if (j * kLThreads + static_cast<int>(threadIdx.x) < n_hist) count(seen[j]);
+            for (int i = kSeen * kLThreads + static_cast<int>(threadIdx.x); i < n_hist; i += kLThreads) count(__ldg(hist + i));
             if (n_bias > 0 && threadIdx.x >= kLThreads - 32) {   // the last warp, 32 entries at a time, in order
                 for (int i0 = 0; i0 < n_bias; i0 += 32) {
                     const long long i = static_cast<long long>(row) * a.bias_stride + i0 + lane;
@@ -158,7 +176,30 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
             }
             __syncthreads();
         }
-        // stream the chunk; listed tokens keep their logits and are no candidates yet
+        // a listed token a thread: asked for before the chunk is streamed, finished after it
+        const int listed = special ? s_listed : 0;
+        auto finish = [&](int t, float v, uint32_t word) {
+            const uint32_t hits = s_count[t];
+            if (hits > 0u) {
+                v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+                v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, static_cast<float>(hits))), pres);
+            }
+            if (n_bias > 0) v = __fadd_rn(v, s_bias[t]);
+            const int i = c0 + t;
+            const bool may = (word >> (i & 31)) & 1u;
+            out[i] = may ? v : -INFINITY;
+            if (may && v == v) best = max(best, order_key(v, i));
+        };
+        auto allowed = [&](int i) { return allow ? __ldg(allow + (i >> 5)) : 0xFFFFFFFFu; };   // its whole word
+        int mine = -1;
+        float mine_v = 0.0f;
+        uint32_t mine_ok = 0u;
+        if (static_cast<int>(threadIdx.x) < listed) {
+            mine = s_list[threadIdx.x];
+            mine_v = static_cast<float>(in[c0 + mine]);
+            mine_ok = allowed(c0 + mine);
+        }
+        // stream the chunk, leaving the listed tokens out
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < kPer / 4; ++j) {
@@ -167,35 +208,22 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
             float y[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                y[e] = ((ok[j] | marks) >> e) & 1u ? x[j][e] : -INFINITY;
+                y[e] = (ok[j] >> e) & 1u ? x[j][e] : -INFINITY;
                 x[j][e] = (ok[j] & ~marks) >> e & 1u ? x[j][e] : __int_as_float(0x7FFFFFFF);   // not a candidate
                 top = fmaxf(top, x[j][e]);          // a NaN does not count
             }
-            if (vec_out && i + 4 <= c1) {
+            if (vec_out && i + 4 <= c1 && (marks & 15u) == 0u) {
                 *reinterpret_cast<float4*>(out + i) = make_float4(y[0], y[1], y[2], y[3]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (i + e < c1) out[i + e] = y[e];
+                    if (i + e < c1 && !((marks >> e) & 1u)) out[i + e] = y[e];
             }
         }
-        if (special) {                              // one thread a listed token, after the stores above
-            __syncthreads();
-            for (int k = threadIdx.x; k < s_listed; k += kLThreads) {
-                const int t = s_list[k], i = c0 + t;
-                float v = static_cast<float>(in[i]);
-                const uint32_t hits = s_count[t];
-                if (hits > 0u) {
-                    const float* pen = a.penalties + row * 3LL;
-                    const float rep = __ldg(pen), freq = __ldg(pen + 1), pres = __ldg(pen + 2);
-                    v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-                    v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, static_cast<float>(hits))), pres);
-                }
-                if (n_bias > 0) v = __fadd_rn(v, s_bias[t]);
-                const bool may = !allow || ((__ldg(allow + (i >> 5)) >> (i & 31)) & 1u);
-                out[i] = may ? v : -INFINITY;
-                if (may && v == v) best = max(best, order_key(v, i));
-            }
+        if (mine >= 0) finish(mine, mine_v, mine_ok);
+        for (int k = kLThreads + static_cast<int>(threadIdx.x); k < listed; k += kLThreads) {
+            const int t = s_list[k];
+            finish(t, static_cast<float>(in[c0 + t]), allowed(c0 + t));
         }
         // the warp's largest streamed candidate and its lowest index
         if (a.token) {
