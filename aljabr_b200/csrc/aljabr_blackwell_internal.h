@@ -250,6 +250,7 @@ struct Kv4Attn {
     float scale, soft_cap;
     // set by the launcher
     int row_tiles, page_shift;
+    unsigned int group_magic;
     unsigned int* counters;  // zero before and after a call
     float* part;
 };

@@ -171,7 +171,7 @@ struct Cfg {
     static constexpr int QFRAG = CT * NG * 2 * 32 * 8;
     static constexpr int QOFF = CT * 32 * 8;                // offset fragments
     static constexpr int BARS = kStages * 2 * 8;            // full and empty
-    static constexpr int MISC = (3 * kWarps * COLS + kWarps + COLS + 8) * 4;
+    static constexpr int MISC = (3 * kWarps * COLS + kWarps + 2 * COLS + 8) * 4;
     static constexpr int SMEM = RING + MERGE + QFRAG + QOFF + BARS + MISC;   // + the per-sequence tables
 };
 // Column of a row's part, and the row of a column.
@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     float* const s_way = s_l + kWarps * COLS;                           // the join's sums
     int* const s_e = reinterpret_cast<int*>(s_way + kWarps * COLS);     // [warp]
     float* const s_fac = reinterpret_cast<float*>(s_e + kWarps);        // [column] score factor
-    int* const s_misc = reinterpret_cast<int*>(s_fac + COLS);
+    int* const s_hi = reinterpret_cast<int*>(s_fac + COLS);             // [column] last position its row sees
+    int* const s_misc = s_hi + COLS;
     int* const s_pre = s_misc + 8;
     int* const s_len = s_pre + p.batch + 1;
 
@@ -381,11 +382,12 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
         const int wide = rem * (share + 1);
         return x < wide ? x / (share + 1) : rem + (x - wide) / share;
     };
-    // The line with its item costs is dealt out evenly; chunk numbers (u) count
-    // real chunks only.
-    auto chunks_before = [&](int b) { return (s_pre[b] - kItemCost * b) * items; };
-    auto real = [&](int x) {                       // real chunks before place x of the line
-        if (x >= total) return chunks_before(p.batch);
+    // The line with its item costs is dealt out evenly.  Lane 0 finds the place where this CTA starts, lane 1 (and
+    // the others) the one where the next does: sequence, item, chunk, and the real chunks before it.
+    Cursor at;
+    int todo;                                      // chunks of this CTA
+    {
+        const int x = start_of(blockIdx.x + min(lane, 1));
         int lo = 0, hi = p.batch - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -393,62 +395,65 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             else hi = mid - 1;
         }
         const int width = s_pre[lo + 1] - s_pre[lo];
-        const int rest = x - s_pre[lo] * items;
-        const int h = rest / width;
-        return chunks_before(lo) + h * (width - kItemCost) + max(0, rest - h * width - kItemCost);
-    };
-    const int u0 = real(start_of(blockIdx.x)), u1 = real(start_of(blockIdx.x + 1));
-    if (u0 >= u1) return;
-
-    Cursor at;
-    {
-        int lo = 0, hi = p.batch - 1;              // the sequence of chunk u0
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (chunks_before(mid) <= u0) lo = mid;
-            else hi = mid - 1;
-        }
-        at.b = lo;
-        load_seq(at, p, tab);
-        const int rest = u0 - chunks_before(lo);
-        at.h = rest / at.chunks;
-        at.ch = rest - at.h * at.chunks;
+        const int rest = x - s_pre[lo] * items;    // x = total: item `items`, chunk 0
+        const int h = rest / width, ch = max(0, rest - h * width - kItemCost);
+        const int before = (s_pre[lo] - kItemCost * lo) * items + h * (width - kItemCost) + ch;
+        todo = __shfl_sync(0xffffffffu, before, 1) - __shfl_sync(0xffffffffu, before, 0);
+        at.b = __shfl_sync(0xffffffffu, lo, 0);
+        at.h = __shfl_sync(0xffffffffu, h, 0);
+        at.ch = __shfl_sync(0xffffffffu, ch, 0);
     }
-    // chunk number i of this CTA, at cursor c, into its slot; the slot's last chunk has been read by every warp
-    auto load = [&](int i, const Cursor& c) {
-        const int slot = i % kStages;
-        const TileSource t = find_tile(p, c, lane >> 2);    // the page id is on its way while the slot empties
-        if (i >= kStages && !mbar_wait(empty + slot, (i / kStages - 1) & 1)) return false;
-        load_chunk<NG>(p, t, c.h / p.row_tiles, c.len, ring + slot * F::STAGE, full + slot, lane);
-        return true;
+    if (todo <= 0) return;
+    load_seq(at, p, tab);
+    bool dead = false;                             // a chunk never arrived: stop waiting, the fault is recorded
+    constexpr bool kQRegs = CT == 1 && NG <= 4;    // q fragments in registers, else read for every tile
+    // PARTS 2: the other part's column is two lanes away and weighs 2^-11 where this one is the high part
+    const float own = PARTS == 1 || c4 < 2 ? 1.0f : 1.0f / 2048.0f, others = c4 < 2 ? 1.0f / 2048.0f : 1.0f;
+    // e: exponent field the shift t is made for.  |dV| < 2^(e - 14) and P <= 2^(t + kLazy): P dV < 2^15, and for bf16,
+    // where P itself is rounded to fp16, P <= 2^15
+    auto shift_of = [](int e) { return PARTS == 2 ? 27 - e : min(13, 27 - e); };
+    auto token_of = [&](int row) { return static_cast<int>((static_cast<unsigned int>(row) * p.group_magic) >> 21); };   // row / group
+
+    // chunk number i of this CTA, at cursor c, into its slot
+    auto ask = [&](int i, const Cursor& c) {
+        const int slot = i % kStages, head = p.row_tiles == 1 ? c.h : c.h / p.row_tiles;
+        const TileSource t = find_tile(p, c, bulk ? lane >> 2 : warp);   // the page id is on its way while the slot empties
+        if (!bulk) {                               // the slot's last tile of this warp has been read by it
+            load_own<NG>(p, t, head, c.len, smem_u32(ring) + slot * F::STAGE, full + slot, warp, lane);
+        } else {
+            if (i >= kStages && !dead) dead = !mbar_wait(empty + slot, (i / kStages - 1) & 1);
+            if (!dead) load_chunk<NG>(p, t, head, c.len, ring + slot * F::STAGE, full + slot, lane);
+        }
     };
-    auto load_mine = [&](int i, const Cursor& c) {     // the slot's last tile of this warp has been read by it
-        load_own<NG>(p, find_tile(p, c, warp), c.h / p.row_tiles, c.len, smem_u32(ring) + (i % kStages) * F::STAGE,
-                     full + i % kStages, warp, lane);
-    };
-    const int todo = u1 - u0;
-    if (bulk ? warp < min(kAhead, todo) : true) {
+    if (!bulk || warp < kAhead) {
         Cursor c = at;
+#pragma unroll 1
         for (int i = 0; i < min(kAhead, todo); ++i) {
-            if (!bulk) load_mine(i, c);
-            else if (i == warp) load(i, c);
+            if (!bulk || i == warp) ask(i, c);
             step(c, p, tab, items);
         }
     }
+    struct Item {
+        int kvh, row0, rows;
+    };
+    auto item_of = [&](const Cursor& c) {
+        Item it;
+        it.kvh = p.row_tiles == 1 ? c.h : c.h / p.row_tiles;
+        it.row0 = (c.h - it.kvh * p.row_tiles) * ROWS;
+        it.rows = min(ROWS, R - it.row0);
+        return it;
+    };
     int done = 0;                                  // chunks of this CTA behind us
-    bool dead = false;                             // a chunk never arrived: stop waiting, the fault is recorded
-    int u = u0;
-    while (u < u1) {
-        // ---------------------------------------------------------- item start
-        const int kvh = at.h / p.row_tiles, row0 = (at.h - kvh * p.row_tiles) * ROWS;
-        const int item_b = at.b, len = at.len;
-        const int item0 = chunks_before(item_b) + at.h * at.chunks, item1 = item0 + at.chunks;
-        // the item's place on the line, for the CTAs that share it
-        const int line0 = s_pre[item_b] * items + at.h * (at.chunks + kItemCost) + kItemCost;
-        const int line1 = line0 + at.chunks;
-        const int seg0 = u, seg1 = min(u1, item1);
-        const int rows = min(ROWS, R - row0);
-        __syncthreads();                    // the previous item's tables are read
+#pragma unroll 1
+    while (done < todo) {
+        // ---------------------------------------------------------- an item begins
+        const int len = at.len;
+        const int count = min(at.chunks - at.ch, todo - done);
+        __syncthreads();                           // the previous item's tables are read
+        int all_lo, all_hi;                        // a tile inside is seen whole by every row
+        {
+        const Item it = item_of(at);
+        const int kvh = it.kvh, row0 = it.row0, rows = it.rows, item_b = at.b;
 
         // q rows -> columns in B-fragment order, their group sums, their score factors.  A lane has NG dims of
         // one group.  (The first warps are busy with the first chunks.)
@@ -456,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             float x[NG];
             const int i = row0 + row;
             const bool live = row < rows;
-            const int t = live ? i / p.group : 0, hd = live ? i - t * p.group : 0;
+            const int t = live ? token_of(i) : 0, hd = live ? i - t * p.group : 0;
             const long long src = (static_cast<long long>(item_b) * p.q_len + t) * p.q_stride +
                                   static_cast<long long>(kvh * p.group + hd) * D + lane * NG;
             float big = 0.0f;
@@ -512,47 +517,37 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             }
             if (lane < PARTS) s_fac[column_of<PARTS>(row, lane)] = p.scale * pow2i(24 - f);
         }
+
+        if (threadIdx.x < COLS) {                  // the last position a column's row sees
+            const int row = PARTS == 1 ? threadIdx.x : 4 * (threadIdx.x >> 3) + (threadIdx.x & 3);
+            s_hi[threadIdx.x] = row < rows ? len - p.q_len + token_of(row0 + row) : -1;
+        }
+        all_hi = len - p.q_len + token_of(row0);
+        all_lo = p.window > 0 ? len - p.q_len + token_of(row0 + rows - 1) - p.window + 1 : 0;
+        }
         __syncthreads();
 
-        // this lane's columns 2 c4 and 2 c4 + 1 of each tile: the last position their rows see, and the first
-        int hi[CT][2];
-        float fac[CT][2], M[CT][2], l[CT][2];
+        // this lane's columns 2 c4 and 2 c4 + 1 of each tile
+        float fac[CT][2], M[CT][2], l[CT][2], acc[2 * NG][CT][4];
+        uint2 qreg[kQRegs ? NG * 2 : 1];
 #pragma unroll
         for (int a = 0; a < CT; ++a)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int col = 8 * a + 2 * c4 + j, row = PARTS == 1 ? col : 4 * a + (col & 3);
-                hi[a][j] = row < rows ? len - p.q_len + (row0 + row) / p.group : -1;
-                fac[a][j] = s_fac[col] * (p.soft_cap > 0.0f ? 1.0f : kLog2e);
+                fac[a][j] = s_fac[8 * a + 2 * c4 + j] * (p.soft_cap > 0.0f ? 1.0f : kLog2e);
                 M[a][j] = kNone;
                 l[a][j] = 0.0f;
             }
-        // PARTS 2: the other part's column is two lanes away and weighs 2^-11 where this one is the high part
-        const float own = PARTS == 1 || c4 < 2 ? 1.0f : 1.0f / 2048.0f, others = c4 < 2 ? 1.0f / 2048.0f : 1.0f;
-        // a tile inside [all_lo, all_hi] is seen whole by every row
-        const int all_hi = len - p.q_len + row0 / p.group;
-        const int all_lo = p.window > 0 ? len - p.q_len + (row0 + rows - 1) / p.group - p.window + 1 : 0;
-        const int any_lo = p.window > 0 ? all_hi - p.window + 1 : 0;
-        constexpr bool kQRegs = CT == 1 && NG <= 4;    // q fragments in registers, else read for every tile
-        uint2 qreg[kQRegs ? NG * 2 : 1];
         if constexpr (kQRegs) {
 #pragma unroll
             for (int i = 0; i < NG * 2; ++i) qreg[i] = s_q[i * 32 + lane];
         }
-        auto q_frag = [&](int a, int g, int st) {
-            if constexpr (kQRegs) return qreg[2 * g + st];
-            return s_q[((a * NG + g) * 2 + st) * 32 + lane];
-        };
-        float acc[2 * NG][CT][4];
 #pragma unroll
         for (int i = 0; i < 2 * NG; ++i)
 #pragma unroll
             for (int a = 0; a < CT; ++a)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[i][a][j] = 0.0f;
-        // e: exponent field the shift t is made for.  |dV| < 2^(e - 14) and P <= 2^(t + kLazy): P dV < 2^15, and
-        // for bf16, where P itself is rounded to fp16, P <= 2^15
-        auto shift_of = [](int e) { return PARTS == 2 ? 27 - e : min(13, 27 - e); };
         int E = 0;
         float limit = shift_of(0) + kLazy;
         const uint32_t m0 = hide(0x000F000Fu), m1 = hide(0x00F000F0u), one = hide(0x64006400u);
@@ -571,6 +566,10 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
         const uint32_t at_vs0 = scales + kWarps * F::SCALES + vrow0 * 2 * NG;
         const uint32_t at_vs1 = scales + kWarps * F::SCALES + vrow1 * 2 * NG;
         const uint32_t at_top = scales + kWarps * F::SCALES + lane * (NG == 8 ? 8 : 4);
+        auto q_frag = [&](int a, int g, int st) {
+            if constexpr (kQRegs) return qreg[2 * g + st];
+            return s_q[((a * NG + g) * 2 + st) * 32 + lane];
+        };
         auto tile = [&](int slot, int pos) {
             const uint32_t st = slot * F::STAGE;
             // ---- scores: y[a][h][j] of row position krow + 8 h and column 2 c4 + j
@@ -637,13 +636,14 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
                             y[a][h][j] = v * fac[a][j];
                         }
             }
-            if (p.soft_cap > 0.0f) {
+            if (p.soft_cap > 0.0f) {               // one value at a time, rotated through: tanhf is long
+#pragma unroll 1
+                for (int k = 0; k < 4 * CT; ++k) {
+                    const float v = tanhf(y[0][0][0] / p.soft_cap) * p.soft_cap * kLog2e;
 #pragma unroll
-                for (int a = 0; a < CT; ++a)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) y[a][h][j] = tanhf(y[a][h][j] / p.soft_cap) * p.soft_cap * kLog2e;
+                    for (int n = 0; n < 4 * CT - 1; ++n) y[n >> 2][(n >> 1) & 1][n & 1] = y[(n + 1) >> 2][((n + 1) >> 1) & 1][(n + 1) & 1];
+                    y[CT - 1][1][1] = v;
+                }
             }
             // largest V scale of the tile: its scale words are dealt out over the lanes
             uint32_t top = 0u;
@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             for (int a = 0; a < CT; ++a) keep[a][0] = keep[a][1] = 0xFFFFFFFFu;
             if (pos < all_lo || pos + kTilePos - 1 > all_hi) {
                 const int word_pos = pos + (NG == 2 ? lane : lane >> 1);   // the position of the lane's scale words
-                if (word_pos >= len || word_pos < any_lo || top >= 0x7C00u) top = 0u;
+                if (word_pos >= len || (p.window > 0 && word_pos <= all_hi - p.window) || top >= 0x7C00u) top = 0u;
 #pragma unroll
                 for (int a = 0; a < CT; ++a)
 #pragma unroll
@@ -669,7 +669,8 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
                         bool see[2];
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            see[j] = at_pos <= hi[a][j] && (p.window == 0 || at_pos > hi[a][j] - p.window);
+                            const int hi = s_hi[8 * a + 2 * c4 + j];
+                            see[j] = at_pos <= hi && (p.window == 0 || at_pos > hi - p.window);
                             y[a][h][j] = see[j] ? y[a][h][j] : -INFINITY;
                         }
                         keep[a][h] = transpose8((see[0] ? 0x0000FFFFu : 0u) | (see[1] ? 0xFFFF0000u : 0u));
@@ -786,16 +787,15 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             }
         };
 
-        // ---------------------------------------------------------- the item's chunks
-        const int count = seg1 - seg0;
+        // ---------------------------------------------------------- its chunks
         const int pos0 = (at.first + at.ch * kChunkTiles + warp) * kTilePos;
+#pragma unroll 1
         for (int i = 0; i < count; ++i, ++done) {
-            if ((!bulk || (done & (kWarps - 1)) == warp) && done + kAhead < todo) {
+            if ((!bulk || ((done + kAhead) & (kWarps - 1)) == warp) && done + kAhead < todo) {
                 Cursor c = at;
                 c.ch += i;
                 for (int k = 0; k < kAhead; ++k) step(c, p, tab, items);
-                if (!bulk) load_mine(done + kAhead, c);
-                else if (!dead) dead = !load(done + kAhead, c);
+                ask(done + kAhead, c);
             }
             const int slot = done % kStages;
             if (!dead) dead = !mbar_wait(full + slot, (done / kStages) & 1);
@@ -804,9 +804,12 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             __syncwarp();                          // every lane has read the slot
             if (lane == 0) mbar_arrive(empty + slot);
         }
-        u = seg1;
+        Cursor was = at;
         at.ch = at.chunks - 1;                     // on to the next item
         step(at, p, tab, items);
+        was.h = hide(was.h);                       // found again, not held in registers over the chunks
+        const Item it = item_of(was);
+        const int kvh = it.kvh, row0 = it.row0, rows = it.rows;
 
         // ---------------------------------------------------------- merge the warps
         if (r == 0) {
@@ -831,13 +834,16 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
                 for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                 if (r == 0) s_l[warp * COLS + col] = sum * wgt[a][j];
             }
-        const bool whole = seg0 == item0 && seg1 == item1;
-        const int slot = seg0 == u0 ? 0 : 1;
-        float* const part = p.part + (static_cast<long long>(blockIdx.x) * 2 + slot) * (ROWS * (D + 2));
+        const bool whole = count == was.chunks;
+        // the item's place on the line, for the CTAs that share it: the first of them keeps its part in its second
+        // slot (no other item can begin there and go on), the others in their first
+        const int line0 = s_pre[was.b] * items + was.h * (was.chunks + kItemCost) + kItemCost;
+        const int cta0 = whole ? 0 : cta_at(line0);
+        float* const part = p.part + (static_cast<long long>(blockIdx.x) * 2 + (static_cast<int>(blockIdx.x) == cta0 ? 1 : 0)) * (ROWS * (D + 2));
         // element of the output that row `row`, dim d of this item has
         auto out_at = [&](int row, int d) {
-            const int ri = row0 + row, t = ri / p.group, hd = ri - t * p.group;
-            return (((static_cast<long long>(item_b) * p.q_len + t) * p.kv_heads + kvh) * p.group + hd) * D + d;
+            const int ri = row0 + row, t = token_of(ri), hd = ri - t * p.group;
+            return (((static_cast<long long>(was.b) * p.q_len + t) * p.kv_heads + kvh) * p.group + hd) * D + d;
         };
 #pragma unroll
         for (int g0 = 0; g0 < NG; g0 += F::SG) {
@@ -882,7 +888,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
         if (whole) continue;
 
         // ---------------------------------------------------------- join an item cut over CTAs
-        const int cta0 = cta_at(line0), cta1 = cta_at(line1 - 1);
+        const int cta1 = cta_at(line0 + was.chunks - 1);
         __syncthreads();                           // every thread's partials, made visible by thread 0's release
         if (threadIdx.x == 0) {
             const bool last = arrive_acq_rel(p.counters + cta0) == static_cast<unsigned int>(cta1 - cta0);
@@ -892,42 +898,46 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
         __syncthreads();
         if (!s_misc[1]) continue;
         const int n = cta1 - cta0 + 1;
-        const int slot0 = real(start_of(cta0)) == item0 ? 0 : 1;   // only the first CTA may hold it in its second slot
-        auto base = [&](int k) { return p.part + (static_cast<long long>(cta0 + k) * 2 + (k == 0 ? slot0 : 0)) * (ROWS * (D + 2)); };
-        // the CTAs' weights for each row, a warp a row: w[row][k]; rows' sums in s_way
-        float* const w = s_merge;
-        for (int row = warp; row < rows; row += kWarps) {
-            float top = kNone, L = 0.0f;
-            for (int k = lane; k < n; k += 32) top = fmaxf(top, __ldcg(base(k) + ROWS * D + row * 2));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            for (int k = lane; k < n; k += 32) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>(base(k) + ROWS * D + row * 2));
-                const float f = ex2(ml.x - top);
-                w[row * n + k] = f;
-                L = fmaf(ml.y, f, L);
-            }
-            L = warp_sum(L);
-            if (lane == 0) s_way[row] = L;
-        }
-        // threads that share one output: each takes a run of the CTAs; their sums follow the weights
+        auto base = [&](int k) { return p.part + (static_cast<long long>(cta0 + k) * 2 + (k == 0 ? 1 : 0)) * (ROWS * (D + 2)); };
+        // Threads that share one output take a run of the CTAs each.  The CTAs' weights first: w[row][k], a warp a
+        // row, the rows' sums in s_way.
         const int outs = rows * (D / 4);
         const int room = (F::MERGE / 4 - rows * n - 3) / 4;
         const int ways = max(1, min(min(n, kThreads / outs), room / outs));
         const int way = ways > 1 ? threadIdx.x / outs : 0;
+        const int per = (n + ways - 1) / ways, k0 = way * per, k1 = min(n, k0 + per);
+        const int first = threadIdx.x - way * outs;
+        float* const w = s_merge;
+#pragma unroll 1
+        for (int row = warp; row < rows; row += kWarps) {
+            float2 ml = make_float2(kNone, 0.0f);      // the lane's CTA, and what came before it
+            for (int k = lane; k < n; k += 32) {
+                const float2 x = __ldcg(reinterpret_cast<const float2*>(base(k) + ROWS * D + row * 2));
+                w[row * n + k] = x.x;
+                const float top = fmaxf(ml.x, x.x);
+                ml.y = fmaf(ml.y, ex2(ml.x - top), x.y * ex2(x.x - top));
+                ml.x = top;
+            }
+            float top = ml.x;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float L = warp_sum(ml.y * ex2(ml.x - top));
+            for (int k = lane; k < n; k += 32) w[row * n + k] = ex2(w[row * n + k] - top);
+            if (lane == 0) s_way[row] = L;
+        }
         float4* const sums = reinterpret_cast<float4*>(s_merge + (rows * n + 3) / 4 * 4);
         __syncthreads();
-        for (int i = threadIdx.x - way * outs; i < outs && way < ways; i += kThreads) {
+#pragma unroll 1
+        for (int i = first; i < outs && way < ways; i += kThreads) {
             const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const int per = (n + ways - 1) / ways, k0 = way * per, k1 = min(n, k0 + per);
-#pragma unroll 8
-            for (int k = k0; k < k1; ++k) {
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(base(k) + row * D + d));
+            auto add = [&](int k, float4 v) {
                 const float f = w[row * n + k];
                 sum.x = fmaf(v.x, f, sum.x); sum.y = fmaf(v.y, f, sum.y);
                 sum.z = fmaf(v.z, f, sum.z); sum.w = fmaf(v.w, f, sum.w);
-            }
+            };
+#pragma unroll 4
+            for (int k = k0; k < k1; ++k) add(k, __ldcg(reinterpret_cast<const float4*>(base(k) + row * D + d)));
             if (ways == 1) store4(p.out, PARTS == 1, out_at(row, d), sum, s_way[row] == 0.0f ? 0.0f : 1.0f / s_way[row]);
             else sums[way * outs + i] = sum;
         }
@@ -997,6 +1007,7 @@ cudaError_t launch_kv4_attention(const Kv4Attn& a, void* workspace, int sms, cud
     const int rows = p.q_len * p.group, tr = tile_rows(rows, p.head_dim, wide);
     const bool two = tr > (wide ? 4 : 8);
     p.row_tiles = (rows + tr - 1) / tr;
+    p.group_magic = ((1u << 21) + p.group - 1) / p.group;   // row / group for row < 2048, exact as row * group < 2^21
     p.page_shift = (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctz(p.page_size) : -1;
     p.counters = static_cast<unsigned int*>(workspace);
     p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (static_cast<size_t>(ctas) * 4 + 255) / 256 * 256);
