@@ -71,7 +71,6 @@ constexpr int kChunkTiles = kWarps;
 constexpr int kStages = 4;
 constexpr int kAhead = 2;        // chunks asked for before their turn
 constexpr int kItemCost = 2;     // chunks that an item's start and end are worth
-constexpr int kMinShare = 2;     // least length of line a CTA is started for
 constexpr int kBulkPage = 64;    // least page size that is loaded by bulk copies
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 2.0f;    // a row's maximum is raised only when a score exceeds it by 2 (log2)
@@ -374,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     __syncthreads();
     const Tables tab = {s_pre, s_len};
     total *= items;
-    const int ctas = min(static_cast<int>(gridDim.x), (total + kMinShare - 1) / kMinShare);
+    const int ctas = min(static_cast<int>(gridDim.x), total);
     if (static_cast<int>(blockIdx.x) >= ctas) return;
     const int share = total / ctas, rem = total - share * ctas;
     auto start_of = [&](int c) { return share * c + min(c, rem); };     // CTA c's first place on the line
@@ -408,6 +407,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     bool dead = false;                             // a chunk never arrived: stop waiting, the fault is recorded
     constexpr bool kQRegs = CT == 1 && NG <= 4;    // q fragments in registers, else read for every tile
     // PARTS 2: the other part's column is two lanes away and weighs 2^-11 where this one is the high part
+    const float inv_cap = p.soft_cap > 0.0f ? 1.0f / p.soft_cap : 0.0f;
     const float own = PARTS == 1 || c4 < 2 ? 1.0f : 1.0f / 2048.0f, others = c4 < 2 ? 1.0f / 2048.0f : 1.0f;
     // e: exponent field the shift t is made for.  |dV| < 2^(e - 14) and P <= 2^(t + kLazy): P dV < 2^15, and for bf16,
     // where P itself is rounded to fp16, P <= 2^15
@@ -556,16 +556,14 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
         // The lane's places in a slot.  Row positions: krow + 8 h, with rows r and r ^ 1 swapped for every second
         // pair -- it spreads the V rows of one load over both halves of the banks.
         const int krow = r ^ ((r >> 1) & 1);
-        const int vrow0 = 2 * c4 + (c4 & 1), vrow1 = 2 * c4 + 1 - (c4 & 1);
+        const int vrow0 = 2 * c4 + (c4 & 1);       // and vrow0 ^ 1
         const uint32_t codes = smem_u32(ring) + warp * F::CODES;
         const uint32_t scales = smem_u32(ring) + 2 * kWarps * F::CODES + warp * F::SCALES;
-        const uint32_t at_k = codes + krow * 16 * NG + c4 * 4 * NG;
-        const uint32_t at_v0 = codes + kWarps * F::CODES + vrow0 * 16 * NG + r * 2 * NG;
-        const uint32_t at_v1 = codes + kWarps * F::CODES + vrow1 * 16 * NG + r * 2 * NG;
-        const uint32_t at_ks = scales + krow * 2 * NG;
-        const uint32_t at_vs0 = scales + kWarps * F::SCALES + vrow0 * 2 * NG;
-        const uint32_t at_vs1 = scales + kWarps * F::SCALES + vrow1 * 2 * NG;
-        const uint32_t at_top = scales + kWarps * F::SCALES + lane * (NG == 8 ? 8 : 4);
+        const uint32_t at_k = hide(codes + krow * 16 * NG + c4 * 4 * NG);
+        const uint32_t at_v = hide(codes + kWarps * F::CODES + vrow0 * 16 * NG + r * 2 * NG);
+        const uint32_t at_ks = hide(scales + krow * 2 * NG);
+        const uint32_t at_vs = hide(scales + kWarps * F::SCALES + vrow0 * 2 * NG);
+        const uint32_t at_top = hide(scales + kWarps * F::SCALES + lane * (NG == 8 ? 8 : 4));
         auto q_frag = [&](int a, int g, int st) {
             if constexpr (kQRegs) return qreg[2 * g + st];
             return s_q[((a * NG + g) * 2 + st) * 32 + lane];
@@ -639,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             if (p.soft_cap > 0.0f) {               // one value at a time, rotated through: tanhf is long
 #pragma unroll 1
                 for (int k = 0; k < 4 * CT; ++k) {
-                    const float v = tanhf(y[0][0][0] / p.soft_cap) * p.soft_cap * kLog2e;
+                    const float v = tanhf(y[0][0][0] * inv_cap) * (p.soft_cap * kLog2e);
 #pragma unroll
                     for (int n = 0; n < 4 * CT - 1; ++n) y[n >> 2][(n >> 1) & 1][n & 1] = y[(n + 1) >> 2][((n + 1) >> 1) & 1][(n + 1) & 1];
                     y[CT - 1][1][1] = v;
@@ -733,8 +731,8 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             uint32_t vw[4][NG / 2], dv[4][NG / 2];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                lds_words<NG / 2>((j & 1 ? at_v1 : at_v0) + st + (j >> 1) * 128 * NG, vw[j]);
-                lds_words<NG / 2>((j & 1 ? at_vs1 : at_vs0) + st + (j >> 1) * 16 * NG, dv[j]);
+                lds_words<NG / 2>(((at_v + st) ^ (j & 1 ? 16 * NG : 0)) + (j >> 1) * 128 * NG, vw[j]);   // slots start at even rows
+                lds_words<NG / 2>(((at_vs + st) ^ (j & 1 ? 2 * NG : 0)) + (j >> 1) * 16 * NG, dv[j]);
             }
             const __half2 kOff = bits_h2(0x64086408u);          // 1032
             const __half2 kDiv = bits_h2(div16), kOff16 = bits_h2(off16);
