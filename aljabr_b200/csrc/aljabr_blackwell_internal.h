@@ -223,7 +223,8 @@ struct Kv4Rows {
     long long k_stride, v_stride;
     void* k_out;             // [tokens][kv_heads * head_dim]
     void* v_out;
-    int vec, vec_out;        // 16-byte accesses on the inputs / outputs
+    int vec, vec_out;        // alignment of the inputs' / outputs' rows: 2 for 32 bytes, 1 for 16, 0
+    int page_shift;          // set by the launcher
 };
 bool kv4_supported(int page_size, int kv_heads, int head_dim);
 long long kv4_cache_bytes(int pages, int page_size, int kv_heads, int head_dim);

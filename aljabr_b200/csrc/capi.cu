@@ -582,14 +582,16 @@ int kv4_check_heads(int q_len, int q_heads, int kv_heads, int head_dim) {
     return ALJ_OK;
 }
 
+int kv4_align(uintptr_t bits) { return (bits & 31) == 0 ? 2 : (bits & 15) == 0 ? 1 : 0; }
+
 int kv4_rows(Kv4Rows* p, void* cache, int pages, int page_size, int kv_heads, int head_dim, int type, const int* slots,
              int tokens, void* k_out, void* v_out) {
     const int rc = kv4_check_cache(pages, page_size, kv_heads, head_dim);
     if (rc) return rc;
     if (type != ALJ_KV_F32 && type != ALJ_KV_BF16)
         return fail(ALJ_ERR_UNSUPPORTED, "kv4: row type %d (ALJ_KV_F32 or ALJ_KV_BF16)", type);
-    if (tokens < 0 || static_cast<long long>(tokens) * kv_heads * head_dim > (1LL << 38))
-        return fail(ALJ_ERR_BAD_DIMS, "kv4: %d tokens", tokens);
+    if (tokens < 0 || static_cast<long long>(tokens) * kv_heads > 0x7fffffffLL - 32)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4: %d tokens x %d kv heads", tokens, kv_heads);
     if (tokens > 0 && (!cache || !slots)) return fail(ALJ_ERR_BAD_ARG, "kv4: null cache or slots");
     const uintptr_t out = reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out);
     if ((reinterpret_cast<uintptr_t>(cache) & 15) || out % (type == ALJ_KV_BF16 ? 2 : 4))
@@ -605,7 +607,7 @@ int kv4_rows(Kv4Rows* p, void* cache, int pages, int page_size, int kv_heads, in
     p->type = type;
     p->k_out = k_out;
     p->v_out = v_out;
-    p->vec_out = (out & 15) == 0;
+    p->vec_out = kv4_align(out);
     return ALJ_OK;
 }
 
@@ -1390,7 +1392,7 @@ int aljabr_blackwell_kv4_append_dev(void* cache, int pages, int page_size, int k
     p.v = v;
     p.k_stride = k_stride;
     p.v_stride = v_stride;
-    p.vec = ((kp | vp | static_cast<uintptr_t>(k_stride) * e | static_cast<uintptr_t>(v_stride) * e) & 15) == 0;
+    p.vec = kv4_align(kp | vp | static_cast<uintptr_t>(k_stride) * e | static_cast<uintptr_t>(v_stride) * e);
     int err = 0;
     DeviceState* st = state(&err);
     if (!st) return err;

@@ -536,7 +536,7 @@ Kv4Rows kv4_layer_rows(const DecodeModel& m, int layer, const int* slots, int to
     r.tokens = tokens;
     r.type = ALJ_KV_F32;
     r.k_stride = r.v_stride = static_cast<long long>(m.hkv) * m.D;
-    r.vec = r.vec_out = 1;
+    r.vec = r.vec_out = 1;      // the activations start on 16-byte boundaries
     return r;
 }
 

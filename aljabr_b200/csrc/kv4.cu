@@ -7,7 +7,10 @@
 //
 // Both are streams: a thread owns 8 consecutive dims of K and of V of one
 // (token, kv head), a quad owns a group of 32, so the extremes need two
-// shuffles and nothing is staged.  Each byte is touched once.
+// shuffles and nothing is staged.  Each byte is touched once, and HBM is the
+// bound as long as a thread's ~64 bytes cost it few hundred instructions:
+// head_dim is a template parameter (rows by shifts), a code is four
+// operations (kv4_rounded).
 #include "kv4.cuh"
 
 #include <algorithm>
@@ -17,12 +20,20 @@ namespace {
 
 constexpr int kRowThreads = 256;
 
+// 8 consecutive elements.  `vec`: 2 for 32-byte aligned rows (one 32-byte
+// access a lane, whole sectors: two 16-byte stores each cover half of every
+// sector, and read-back of 49152 rows took 88 us with them), 1 for 16-byte
+// aligned ones, 0 for the rest.  bf16 rows need 16 bytes a lane.
 template <typename T>
-struct Wide;   // 8 consecutive elements
+struct Wide;
 template <>
 struct Wide<float> {
-    static __device__ __forceinline__ void load(const float* p, bool vec, float (&v)[8]) {
-        if (vec) {
+    static __device__ __forceinline__ void load(const float* p, int vec, float (&v)[8]) {
+        if (vec == 2) {
+            asm volatile("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                         : "l"(p));
+        } else if (vec == 1) {
             const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
             v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
             v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -31,8 +42,12 @@ struct Wide<float> {
             for (int i = 0; i < 8; ++i) v[i] = __ldg(p + i);
         }
     }
-    static __device__ __forceinline__ void store(float* p, bool vec, const float (&v)[8]) {
-        if (vec) {
+    static __device__ __forceinline__ void store(float* p, int vec, const float (&v)[8]) {
+        if (vec == 2) {
+            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                         "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                         : "memory");
+        } else if (vec == 1) {
             reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
             reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
         } else {
@@ -43,7 +58,7 @@ struct Wide<float> {
 };
 template <>
 struct Wide<__nv_bfloat16> {
-    static __device__ __forceinline__ void load(const __nv_bfloat16* p, bool vec, float (&v)[8]) {
+    static __device__ __forceinline__ void load(const __nv_bfloat16* p, int vec, float (&v)[8]) {
         if (vec) {
             const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
             const uint32_t w[4] = {a.x, a.y, a.z, a.w};
@@ -58,7 +73,7 @@ struct Wide<__nv_bfloat16> {
         }
     }
     // one rounding to bf16, the type the caller asked the values in
-    static __device__ __forceinline__ void store(__nv_bfloat16* p, bool vec, const float (&v)[8]) {
+    static __device__ __forceinline__ void store(__nv_bfloat16* p, int vec, const float (&v)[8]) {
         if (vec) {
             uint32_t w[4];
 #pragma unroll
@@ -74,48 +89,62 @@ struct Wide<__nv_bfloat16> {
     }
 };
 
-struct Where {          // one thread's place: token, head, 8 dims
-    long long token;
-    int head, j;        // dims 8 j ..
-    int slot;           // -1: skip
+struct Where {          // one thread's place: token, head, 8 dims 8 j ..
+    int token, head, j;
+    long long block;    // its page's block for the head, in bytes; -1: skip
+    int off;            // position in the page
 };
 
+template <int D>
 __device__ __forceinline__ bool place(const Kv4Rows& p, Where& w) {
-    const int per_row = p.head_dim / 8;
-    const long long i = static_cast<long long>(blockIdx.x) * kRowThreads + threadIdx.x;
-    w.j = static_cast<int>(i % per_row);
-    const long long row = i / per_row;
-    w.head = static_cast<int>(row % p.kv_heads);
-    w.token = row / p.kv_heads;
-    if (w.token >= p.tokens) return false;   // whole quads only: per_row is a multiple of 8
-    w.slot = __ldg(p.slots + w.token);
-    if (w.slot >= 0 && w.slot >= static_cast<long long>(p.pages) * p.page_size) {
+    constexpr int kLanes = D / 8;
+    const unsigned int row = blockIdx.x * (kRowThreads / kLanes) + threadIdx.x / kLanes;   // < 2^31: checked on the host
+    w.j = threadIdx.x % kLanes;
+    w.token = row / static_cast<unsigned int>(p.kv_heads);
+    w.head = row - w.token * p.kv_heads;
+    w.block = -1;
+    if (w.token >= p.tokens) return false;         // whole rows, so whole quads
+    const int slot = __ldg(p.slots + w.token);
+    if (slot < 0) return true;
+    const int page = p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
+    if (page >= p.pages) {
         record_fault(ALJ_FAULT_BOUNDS);
-        w.slot = -1;
+        return true;
     }
+    w.off = slot - page * p.page_size;
+    w.block = (static_cast<long long>(page) * p.kv_heads + w.head) * kv4_block_bytes(p.page_size, D);
     return true;
 }
 
-__device__ __forceinline__ uint32_t pack8(const float (&x)[8], float inv) {
+// Codes of 8 values as a word, and the values they stand for back in x.
+__device__ __forceinline__ uint32_t encode8(float (&x)[8], float inv, float d, bool finite) {
     uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= kv4_code(x[i], inv) << (4 * i);
-    return w;
+    for (int i = 0; i < 8; ++i) {
+        const float r = kv4_rounded(x[i], inv);
+        w |= (__float_as_uint(r) & 15u) << (4 * i);
+        x[i] = __fadd_rn(__fmul_rn(__fadd_rn(r, -kKv4Round), d), 0.0f);   // as kv4_value
+    }
+    return finite ? w : 0x88888888u;
 }
 __device__ __forceinline__ void unpack8(uint32_t w, float d, float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = kv4_value((w >> (4 * i)) & 15u, d);
 }
 
-// Extremes of a group over its quad and the scale they give.  `finite` from
-// x - x: zero for every finite x, NaN for an infinity or a NaN.
-__device__ __forceinline__ __half group_scale(const float (&x)[8]) {
+// A group's scale from its extremes over the quad.  `finite` from x * 0: zero
+// for every finite x, NaN for an infinity or a NaN.
+struct Group {
+    __half d;
+    bool finite;
+};
+__device__ __forceinline__ Group group_of(const float (&x)[8]) {
     float mn = x[0], mx = x[0], nan = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         mn = fminf(mn, x[i]);
         mx = fmaxf(mx, x[i]);
-        nan += x[i] - x[i];
+        nan = fmaf(x[i], 0.0f, nan);
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
@@ -123,83 +152,85 @@ __device__ __forceinline__ __half group_scale(const float (&x)[8]) {
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         nan += __shfl_xor_sync(0xffffffffu, nan, o);
     }
-    return kv4_scale(mn, mx, nan == 0.0f);
+    Group g;
+    g.finite = nan == 0.0f;
+    g.d = kv4_scale(mn, mx, g.finite);
+    return g;
 }
 
-template <typename T>
+template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Rows p) {
     pdl_launch_dependents();
     pdl_wait();
+    constexpr int NG = D / 32;
     Where w;
-    const bool live = place(p, w);
-    const int NG = p.head_dim / 32, g = w.j >> 2, c = w.j & 3;
-    const bool vec = p.vec != 0;
+    const bool live = place<D>(p, w);
+    const int g = w.j >> 2, c = w.j & 3;
     float k[8] = {}, v[8] = {};
-    const bool write = live && w.slot >= 0;
+    const bool write = live && w.block >= 0;
     if (write) {
-        Wide<T>::load(static_cast<const T*>(p.k) + w.token * p.k_stride + w.head * p.head_dim + 8 * w.j, vec, k);
-        Wide<T>::load(static_cast<const T*>(p.v) + w.token * p.v_stride + w.head * p.head_dim + 8 * w.j, vec, v);
+        const int col = w.head * D + 8 * w.j;
+        Wide<T>::load(static_cast<const T*>(p.k) + w.token * p.k_stride + col, p.vec, k);
+        Wide<T>::load(static_cast<const T*>(p.v) + w.token * p.v_stride + col, p.vec, v);
     }
     // every lane takes part in the shuffles below; a skipped row's zeros are not stored
-    const __half dk = group_scale(k), dv = group_scale(v);
-    const uint32_t kw = pack8(k, kv4_inverse(dk)), vw = pack8(v, kv4_inverse(dv));
+    const Group gk = group_of(k), gv = group_of(v);
+    const uint32_t kw = encode8(k, kv4_inverse(gk.d), __half2float(gk.d), gk.finite);
+    const uint32_t vw = encode8(v, kv4_inverse(gv.d), __half2float(gv.d), gv.finite);
     // V halfwords (2 c, g) and (2 c + 1, g): lanes of groups g and g ^ 1 trade
     // one each, so a lane stores the adjacent pair (r, g & ~1), (r, g | 1)
     const uint32_t other = __shfl_xor_sync(0xffffffffu, vw, 4);
     const uint32_t vpair = g & 1 ? __byte_perm(other, vw, 0x7632) : __byte_perm(vw, other, 0x5410);
     if (write) {
-        const int page = w.slot / p.page_size, off = w.slot - page * p.page_size;
-        uint8_t* blk = p.cache + (static_cast<long long>(page) * p.kv_heads + w.head) * kv4_block_bytes(p.page_size, p.head_dim);
-        const int row = p.head_dim / 2;
-        uint8_t* kc = blk + static_cast<long long>(off) * row;
-        uint8_t* vc = kc + static_cast<long long>(p.page_size) * row;
+        uint8_t* blk = p.cache + w.block;
+        uint8_t* kc = blk + w.off * (D / 2LL);
+        uint8_t* vc = kc + p.page_size * (D / 2LL);
         *reinterpret_cast<uint32_t*>(kc + 4 * (c * NG + g)) = kw;
         *reinterpret_cast<uint32_t*>(vc + 2 * ((2 * c + (g & 1)) * NG + (g & ~1))) = vpair;
-        __half* sc = reinterpret_cast<__half*>(blk + 2LL * p.page_size * row);
-        if (c == 0) sc[static_cast<long long>(off) * NG + g] = dk;
-        if (c == 1) sc[static_cast<long long>(p.page_size + off) * NG + g] = dv;
+        __half* sc = reinterpret_cast<__half*>(blk + p.page_size * static_cast<long long>(D));
+        if (c == 0) sc[w.off * static_cast<long long>(NG) + g] = gk.d;
+        if (c == 1) sc[(p.page_size + w.off) * static_cast<long long>(NG) + g] = gv.d;
     }
-    if (live && p.k_out) {
-        const long long at = (w.token * p.kv_heads + w.head) * p.head_dim + 8 * w.j;
-        unpack8(kw, write ? __half2float(dk) : 0.0f, k);
-        unpack8(vw, write ? __half2float(dv) : 0.0f, v);
-        Wide<T>::store(static_cast<T*>(p.k_out) + at, p.vec_out != 0, k);
-        Wide<T>::store(static_cast<T*>(p.v_out) + at, p.vec_out != 0, v);
+    if (live && p.k_out) {                         // a skipped row's zeros stand for zeros
+        const long long at = (static_cast<long long>(w.token) * p.kv_heads + w.head) * D + 8 * w.j;
+        Wide<T>::store(static_cast<T*>(p.k_out) + at, p.vec_out, k);
+        Wide<T>::store(static_cast<T*>(p.v_out) + at, p.vec_out, v);
     }
 }
 
-template <typename T>
+template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(const Kv4Rows p) {
     pdl_launch_dependents();
     pdl_wait();
+    constexpr int NG = D / 32;
     Where w;
-    if (!place(p, w)) return;
-    const int NG = p.head_dim / 32, g = w.j >> 2, c = w.j & 3;
+    if (!place<D>(p, w)) return;
+    const int g = w.j >> 2, c = w.j & 3;
     float k[8] = {}, v[8] = {};
-    if (w.slot >= 0) {
-        const int page = w.slot / p.page_size, off = w.slot - page * p.page_size;
-        const uint8_t* blk = p.cache + (static_cast<long long>(page) * p.kv_heads + w.head) * kv4_block_bytes(p.page_size, p.head_dim);
-        const int row = p.head_dim / 2;
-        const uint8_t* kc = blk + static_cast<long long>(off) * row;
-        const uint8_t* vc = kc + static_cast<long long>(p.page_size) * row;
-        const __half* sc = reinterpret_cast<const __half*>(blk + 2LL * p.page_size * row);
-        const uint32_t kw = *reinterpret_cast<const uint32_t*>(kc + 4 * (c * NG + g));
-        const uint32_t v0 = *reinterpret_cast<const uint16_t*>(vc + 2 * (2 * c * NG + g));
-        const uint32_t v1 = *reinterpret_cast<const uint16_t*>(vc + 2 * ((2 * c + 1) * NG + g));
-        const float dk = __half2float(sc[static_cast<long long>(off) * NG + g]);
-        const float dv = __half2float(sc[static_cast<long long>(p.page_size + off) * NG + g]);
+    if (w.block >= 0) {
+        const uint8_t* blk = p.cache + w.block;
+        const uint8_t* kc = blk + w.off * (D / 2LL);
+        const uint8_t* vc = kc + p.page_size * (D / 2LL);
+        const __half* sc = reinterpret_cast<const __half*>(blk + p.page_size * static_cast<long long>(D));
+        const uint32_t kw = __ldg(reinterpret_cast<const uint32_t*>(kc + 4 * (c * NG + g)));
+        const uint32_t v0 = __ldg(reinterpret_cast<const uint16_t*>(vc + 2 * (2 * c * NG + g)));
+        const uint32_t v1 = __ldg(reinterpret_cast<const uint16_t*>(vc + 2 * ((2 * c + 1) * NG + g)));
+        const float dk = __half2float(__ldg(sc + w.off * static_cast<long long>(NG) + g));
+        const float dv = __half2float(__ldg(sc + (p.page_size + w.off) * static_cast<long long>(NG) + g));
         unpack8(kw, dk, k);
         unpack8(v0 | (v1 << 16), dv, v);
     }
-    const long long at = (w.token * p.kv_heads + w.head) * p.head_dim + 8 * w.j;
-    if (p.k_out) Wide<T>::store(static_cast<T*>(p.k_out) + at, p.vec_out != 0, k);
-    if (p.v_out) Wide<T>::store(static_cast<T*>(p.v_out) + at, p.vec_out != 0, v);
+    const long long at = (static_cast<long long>(w.token) * p.kv_heads + w.head) * D + 8 * w.j;
+    if (p.k_out) Wide<T>::store(static_cast<T*>(p.k_out) + at, p.vec_out, k);
+    if (p.v_out) Wide<T>::store(static_cast<T*>(p.v_out) + at, p.vec_out, v);
 }
 
-cudaError_t launch_rows(void (*kernel)(const Kv4Rows), const Kv4Rows& p, cudaStream_t stream) {
-    const long long items = static_cast<long long>(p.tokens) * p.kv_heads * (p.head_dim / 8);
+cudaError_t launch_rows(void (*kernel)(const Kv4Rows), Kv4Rows p, cudaStream_t stream) {
+    p.page_shift = (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctz(p.page_size) : -1;
+    const long long rows = static_cast<long long>(p.tokens) * p.kv_heads;
+    const int per_cta = kRowThreads / (p.head_dim / 8);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned int>((items + kRowThreads - 1) / kRowThreads));
+    cfg.gridDim = dim3(static_cast<unsigned int>((rows + per_cta - 1) / per_cta));
     cfg.blockDim = dim3(kRowThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -221,12 +252,25 @@ long long kv4_cache_bytes(int pages, int page_size, int kv_heads, int head_dim) 
     return static_cast<long long>(pages) * kv_heads * page_size * (head_dim + head_dim / 8);
 }
 
+template <typename T>
+cudaError_t launch_append(const Kv4Rows& p, cudaStream_t stream) {
+    if (p.head_dim == 64) return launch_rows(kv4_append_kernel<T, 64>, p, stream);
+    if (p.head_dim == 128) return launch_rows(kv4_append_kernel<T, 128>, p, stream);
+    return launch_rows(kv4_append_kernel<T, 256>, p, stream);
+}
+template <typename T>
+cudaError_t launch_read(const Kv4Rows& p, cudaStream_t stream) {
+    if (p.head_dim == 64) return launch_rows(kv4_read_kernel<T, 64>, p, stream);
+    if (p.head_dim == 128) return launch_rows(kv4_read_kernel<T, 128>, p, stream);
+    return launch_rows(kv4_read_kernel<T, 256>, p, stream);
+}
+
 cudaError_t launch_kv4_append(const Kv4Rows& p, cudaStream_t stream) {
-    return launch_rows(p.type == ALJ_KV_BF16 ? kv4_append_kernel<__nv_bfloat16> : kv4_append_kernel<float>, p, stream);
+    return p.type == ALJ_KV_BF16 ? launch_append<__nv_bfloat16>(p, stream) : launch_append<float>(p, stream);
 }
 
 cudaError_t launch_kv4_read(const Kv4Rows& p, cudaStream_t stream) {
-    return launch_rows(p.type == ALJ_KV_BF16 ? kv4_read_kernel<__nv_bfloat16> : kv4_read_kernel<float>, p, stream);
+    return p.type == ALJ_KV_BF16 ? launch_read<__nv_bfloat16>(p, stream) : launch_read<float>(p, stream);
 }
 
 }  // namespace alj

@@ -39,11 +39,12 @@ __device__ __forceinline__ float kv4_inverse(__half d) {
     const float f = __half2float(d);
     return f == 0.0f ? 0.0f : __fdiv_rn(1.0f, f);
 }
-// Code of x: x / d to the nearest integer (ties to even), clamped to -8..7,
-// plus 8.  A NaN scale gives code 8.
-__device__ __forceinline__ uint32_t kv4_code(float x, float inv) {
-    const float r = rintf(__fmul_rn(x, inv)) + 8.0f;
-    return r == r ? static_cast<uint32_t>(fminf(fmaxf(r, 0.0f), 15.0f)) : 8u;
+// x / d clamped to -8..7 and rounded to the nearest integer, ties to even, as
+// the sum with 1.5 * 2^23 + 8: its low four bits are the code, and less that
+// number it is the code's integer c - 8.
+constexpr float kKv4Round = 12582920.0f;
+__device__ __forceinline__ float kv4_rounded(float x, float inv) {
+    return __fadd_rn(fminf(fmaxf(__fmul_rn(x, inv), -8.0f), 7.0f), kKv4Round);
 }
 // The value a code stands for; exact in fp32 (4-bit x 11-bit product).  The
 // added zero turns -0 into +0, as the Q4_0 dequantisation does.
