@@ -230,6 +230,8 @@ bool kv4_supported(int page_size, int kv_heads, int head_dim);
 long long kv4_cache_bytes(int pages, int page_size, int kv_heads, int head_dim);
 cudaError_t launch_kv4_append(const Kv4Rows& p, cudaStream_t stream);
 cudaError_t launch_kv4_read(const Kv4Rows& p, cudaStream_t stream);
+// One token of a decode step: RoPE on q (in place) and k, then k and v (fp32, 16-byte aligned) into page 0 at *p.slots.
+cudaError_t launch_kv4_rope_append(const Kv4Rows& p, float* q, const float2* rope, int q_heads, cudaStream_t stream);
 
 // Attention over it (kv4_attention.cu): q [batch][q_len] rows of kv_heads *
 // group heads, q_stride elements apart; query t of sequence b sees positions

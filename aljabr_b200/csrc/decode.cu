@@ -201,8 +201,7 @@ __global__ void swiglu_kernel(const float* gate, float* up, int n) {
 // Split-half RoPE (GGUFVectorOps.rope, GGUFVectorOps.java:383-440) on the
 // rank's q and k heads, then the KV store at `pos`
 // (GgufKvCacheWriteExecution.storeToken).  rope[pos * D/2 + i] holds
-// (cos, sin) of the reference's angle, computed on the host once.  A 4-bit
-// cache (ALJ_KV_Q4) is written by the append launch that follows.
+// (cos, sin) of the reference's angle, computed on the host once.
 __global__ void rope_store_kernel(float* q, float* k, const float* v, void* kc, void* vc, const int* io,
                                   const float2* rope, int hq, int hkv, int D, int kv_dtype) {
     pdl_launch_dependents();
@@ -226,13 +225,12 @@ __global__ void rope_store_kernel(float* q, float* k, const float* v, void* kc, 
             if (kv_dtype == ALJ_KV_BF16) {
                 static_cast<__nv_bfloat16*>(kc)[off] = __float2bfloat16_rn(r0);
                 static_cast<__nv_bfloat16*>(kc)[off + half] = __float2bfloat16_rn(r1);
-            } else if (kv_dtype == ALJ_KV_F32) {
+            } else {
                 static_cast<float*>(kc)[off] = r0;
                 static_cast<float*>(kc)[off + half] = r1;
             }
         }
     }
-    if (kv_dtype == ALJ_KV_Q4) return;
     for (int idx = blockIdx.x * blockDim.x + threadIdx.x; idx < stride; idx += gridDim.x * blockDim.x) {
         const long long off = static_cast<long long>(pos) * stride + idx;
         if (kv_dtype == ALJ_KV_BF16) static_cast<__nv_bfloat16*>(vc)[off] = __float2bfloat16_rn(v[idx]);
@@ -540,13 +538,13 @@ Kv4Rows kv4_layer_rows(const DecodeModel& m, int layer, const int* slots, int to
     return r;
 }
 
-// The layer's new K and V into its 4-bit cache at *io (the position is the
-// slot), then attention over [0, *io].
+// RoPE, the layer's new K and V into its 4-bit cache at *io (the position is
+// the slot), then attention over [0, *io].
 cudaError_t record_kv4_attention(DecodeModel& m, int layer, int sms) {
     Kv4Rows r = kv4_layer_rows(m, layer, m.io, 1);
     r.k = m.k;
     r.v = m.vv;
-    REC(launch_kv4_append(r, m.stream));
+    REC(launch_kv4_rope_append(r, m.q, m.rope, m.hq, m.stream));
     Kv4Attn a = {};
     a.out = m.att;
     a.q = m.q;
@@ -591,7 +589,8 @@ cudaError_t record_step(DecodeModel& m) {
             REC(matvec(m, ws, ys, rows, 3, m.xn, m.H, EPI_STORE, nullptr, nullptr, nullptr, nullptr, l > 0));
         }
         // RoPE on q and k, KV store (GgufDecodePass.java:333-362)
-        REC(launch_small(rope_store_kernel, std::max(1, ((m.hq + m.hkv) * D / 2 + 255) / 256), 256, m.stream, m.q,
+        if (!m.kv4())
+            REC(launch_small(rope_store_kernel, std::max(1, ((m.hq + m.hkv) * D / 2 + 255) / 256), 256, m.stream, m.q,
                          m.k, static_cast<const float*>(m.vv), kc, vc, static_cast<const int*>(m.io),
                          static_cast<const float2*>(m.rope), m.hq, m.hkv, D, m.kv_dtype));
         if (m.kv4()) {

@@ -225,6 +225,59 @@ __global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(const Kv4Rows p) 
     if (p.v_out) Wide<T>::store(static_cast<T*>(p.v_out) + at, p.vec_out, v);
 }
 
+// Decode step: split-half RoPE of one token's q and k heads (the products and
+// sums of rope_store_kernel, decode.cu), then K and V into the cache at
+// position *p.slots.  A thread owns dims 8 t .. and D / 2 + 8 t .. of a head,
+// which RoPE pairs.
+template <int D>
+__global__ void __launch_bounds__(kRowThreads) kv4_rope_append_kernel(const Kv4Rows p, float* q, const float2* rope, int q_heads) {
+    pdl_launch_dependents();
+    pdl_wait();
+    constexpr int kLanes = D / 16, NG = D / 32;
+    const int unit = blockIdx.x * (kRowThreads / kLanes) + threadIdx.x / kLanes, t = threadIdx.x % kLanes;
+    const int pos = __ldg(p.slots);
+    const bool in_cache = pos >= 0 && pos < p.page_size, live = unit < q_heads + 2 * p.kv_heads;
+    if (!in_cache && live) record_fault(ALJ_FAULT_BOUNDS);
+    const bool is_q = unit < q_heads, is_v = unit >= q_heads + p.kv_heads;
+    const int head = is_q ? unit : is_v ? unit - q_heads - p.kv_heads : unit - q_heads;
+    float x[2][8] = {};
+    if (live && in_cache) {
+        const float* src = (is_q ? q : static_cast<const float*>(is_v ? p.v : p.k)) + head * D + 8 * t;
+        Wide<float>::load(src, 1, x[0]);
+        Wide<float>::load(src + D / 2, 1, x[1]);
+        if (!is_v) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float2 cs = rope[static_cast<long long>(pos) * (D / 2) + 8 * t + i];
+                const float a = x[0][i], b = x[1][i];
+                x[0][i] = __fsub_rn(__fmul_rn(a, cs.x), __fmul_rn(b, cs.y));
+                x[1][i] = __fadd_rn(__fmul_rn(a, cs.y), __fmul_rn(b, cs.x));
+            }
+        }
+        if (is_q) {
+            Wide<float>::store(q + head * D + 8 * t, 1, x[0]);
+            Wide<float>::store(q + head * D + D / 2 + 8 * t, 1, x[1]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {                  // every lane takes part in the shuffles
+        const int j = t + e * kLanes, g = j >> 2, c = j & 3;
+        const Group gr = group_of(x[e]);
+        const uint32_t w = encode8(x[e], kv4_inverse(gr.d), __half2float(gr.d), gr.finite);
+        if (!live || !in_cache || is_q) continue;
+        uint8_t* blk = p.cache + head * kv4_block_bytes(p.page_size, D);
+        uint8_t* row = blk + ((is_v ? p.page_size : 0) + pos) * (D / 2LL);
+        if (is_v) {
+            *reinterpret_cast<uint16_t*>(row + 2 * (2 * c * NG + g)) = static_cast<uint16_t>(w);
+            *reinterpret_cast<uint16_t*>(row + 2 * ((2 * c + 1) * NG + g)) = static_cast<uint16_t>(w >> 16);
+        } else {
+            *reinterpret_cast<uint32_t*>(row + 4 * (c * NG + g)) = w;
+        }
+        if (c == 0)
+            reinterpret_cast<__half*>(blk + p.page_size * static_cast<long long>(D))[((is_v ? p.page_size : 0) + pos) * static_cast<long long>(NG) + g] = gr.d;
+    }
+}
+
 cudaError_t launch_rows(void (*kernel)(const Kv4Rows), Kv4Rows p, cudaStream_t stream) {
     p.page_shift = (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctz(p.page_size) : -1;
     const long long rows = static_cast<long long>(p.tokens) * p.kv_heads;
@@ -271,6 +324,21 @@ cudaError_t launch_kv4_append(const Kv4Rows& p, cudaStream_t stream) {
 
 cudaError_t launch_kv4_read(const Kv4Rows& p, cudaStream_t stream) {
     return p.type == ALJ_KV_BF16 ? launch_read<__nv_bfloat16>(p, stream) : launch_read<float>(p, stream);
+}
+
+cudaError_t launch_kv4_rope_append(const Kv4Rows& p, float* q, const float2* rope, int q_heads, cudaStream_t stream) {
+    const int units = q_heads + 2 * p.kv_heads, per_cta = kRowThreads / (p.head_dim / 16);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((units + per_cta - 1) / per_cta);
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    auto kernel = p.head_dim == 64 ? kv4_rope_append_kernel<64> : p.head_dim == 128 ? kv4_rope_append_kernel<128> : kv4_rope_append_kernel<256>;
+    return cudaLaunchKernelEx(&cfg, kernel, p, q, rope, q_heads);
 }
 
 }  // namespace alj

@@ -22,6 +22,7 @@ run on these hosts: no JDK), over all host threads.
 from __future__ import annotations
 
 import argparse
+import dataclasses
 import json
 import os
 import statistics
@@ -811,7 +812,10 @@ def run_decode(args, rank, world, dev, tokens_per_run=32, runs=4):
 
     from aljabr_b200.decode import LLAMA3_8B, LlamaNf4Decoder, nccl_unique_id
 
-    s = LLAMA3_8B
+    kvkind = getattr(args, "decode_kv", "bf16")
+    s = LLAMA3_8B if kvkind == "bf16" else dataclasses.replace(LLAMA3_8B, kv_dtype=2)   # native.KV_Q4
+    if kvkind != "bf16" and world > 1:
+        raise SystemExit("the 4-bit KV cache runs on one GPU")
     nid = None
     if world > 1:
         obj = [nccl_unique_id() if rank == 0 else None]
@@ -886,8 +890,11 @@ def run_decode(args, rank, world, dev, tokens_per_run=32, runs=4):
         dec.register_output(ec, ea, hc, ha, np.ones(H, np.float32))
     kvd = s.kv_heads // world * s.head_dim
     for layer in range(s.layers):
-        k = torch.randn(s.max_ctx, kvd, device=dev, generator=g).to(torch.bfloat16)
-        v = torch.randn(s.max_ctx, kvd, device=dev, generator=g).to(torch.bfloat16)
+        k = torch.randn(s.max_ctx, kvd, device=dev, generator=g)
+        v = torch.randn(s.max_ctx, kvd, device=dev, generator=g)
+        if kvkind == "bf16":                     # a 4-bit cache takes fp32 rows and quantises them
+            k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
+        torch.cuda.synchronize(dev)
         dec.sync_kv_cache(layer, s.max_ctx, k, v)
         del k, v
     torch.cuda.synchronize(dev)
@@ -916,7 +923,7 @@ def run_decode(args, rank, world, dev, tokens_per_run=32, runs=4):
         torch.distributed.all_reduce(t, op=torch.distributed.ReduceOp.MAX)
         dt_e2e = float(t.item())
     dec.close()
-    kv_bytes = s.layers * (s.max_ctx - tokens_per_run // 2) * kvd * 2 * 2
+    kv_bytes = int(s.layers * (s.max_ctx - tokens_per_run // 2) * kvd * 2 * (2 if kvkind == "bf16" else 18 / 32))
     per_gpu = weight_bytes + kv_bytes
     tok_s = n / dt
     peak, _ = load_peaks()
@@ -930,7 +937,7 @@ def run_decode(args, rank, world, dev, tokens_per_run=32, runs=4):
                                                "q4_0": "GGUF Q4_0 linear + lm_head + embedding",
                                                "q4_k_m": "GGUF Q4_K linear + embedding, Q6_K attn_v / ffn_down / "
                                                          "lm_head (llama.cpp Q4_K_M mix)"}[wkind]
-                      + ", bf16 KV ctx 4096, random weights"}
+                      + f", {'bf16' if kvkind == 'bf16' else '4-bit'} KV ctx 4096, random weights"}
 
 
 # ----------------------------------------------------------------- CPU legs
@@ -1034,6 +1041,8 @@ def main():
     ap.add_argument("--decode-tokens", type=int, default=32)
     ap.add_argument("--decode-weights", default="nf4", choices=["nf4", "q4_0", "q4_k_m"],
                     help="weight formats of the --only decode model (GGUF types on one GPU only)")
+    ap.add_argument("--decode-kv", default="bf16", choices=["bf16", "q4"],
+                    help="KV cache of the --only decode model (4 bits on one GPU only)")
     ap.add_argument("--c5-tokens", default="1,16,64,512",
                     help="token counts of the batched-NF4 (C5) section, comma separated")
     ap.add_argument("--prefill-tokens", default="16,64,512",

@@ -98,7 +98,7 @@ def test_non_finite_groups_read_back_as_nan_and_large_ones_saturate():
 
 def test_strided_and_unaligned_rows():
     rng = np.random.default_rng(2)
-    for dtype, cut in ((torch.float32, 0), (torch.float32, 1), (torch.bfloat16, 0), (torch.bfloat16, 3)):
+    for dtype, cut in ((torch.float32, 0), (torch.float32, 1), (torch.float32, 4), (torch.bfloat16, 0), (torch.bfloat16, 3)):
         wide = torch.from_numpy(rng.normal(size=(20, 3 * 256 + 8)).astype(np.float32)).cuda().to(dtype)
         k, v = wide[:, cut:cut + 256], wide[:, 256 + cut:512 + cut]
         a, b = make(2, 16, 2, 128), make(2, 16, 2, 128)
