@@ -75,7 +75,8 @@ class Kv4Cache:
         self._attend, self._work_size = lib.aljabr_blackwell_kv4_attention_dev, lib.aljabr_blackwell_kv4_attention_workspace_size
         self._row = kv_heads * head_dim
         self._shape = (data.data_ptr(), pages, page_size, kv_heads, head_dim)
-        self._work = {}      # stream -> (workspace, bytes): calls on one stream never overlap
+        self._buffers = {}   # stream -> workspace: calls on one stream never overlap
+        self._work = {}      # (stream, q_len, q_heads) -> its address and size
 
     # -- checks ----------------------------------------------------------------
     def _rows(self, t: torch.Tensor, tokens: int, what: str) -> int:
@@ -85,20 +86,20 @@ class Kv4Cache:
             ok = shape == (tokens, self.kv_heads, self.head_dim) and (st[1] == self.head_dim or self.kv_heads == 1)
         else:
             ok = shape == (tokens, self._row)
-        if not ok or t.get_device() != self._index or st[-1] != 1:
+        if not ok or st[-1] != 1 or t.get_device() != self._index:
             raise bad(f"{what} must be [{tokens}, {self.kv_heads}, {self.head_dim}] on {self.device} with contiguous rows, "
                       f"not {tuple(shape)} with strides {st} on {t.device}")
         return st[0] if tokens > 1 else self._row
 
-    def _ints(self, t: torch.Tensor, shape: tuple, what: str) -> int:
-        if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != self._index or not t.is_contiguous():
-            raise bad(f"{what} must be contiguous int32 {shape} on {self.device}")
+    def _ints(self, t: torch.Tensor, n: int, what: str) -> int:
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != n or t.get_device() != self._index or not t.is_contiguous():
+            raise bad(f"{what} must be contiguous int32 [{n}] on {self.device}")
         return t.data_ptr()
 
     def _dense(self, t, tokens: int, dtype, what: str):
         if t is None:
             return None
-        if t.dtype is not dtype or not t.is_contiguous() or t.get_device() != self._index or t.numel() != tokens * self._row:
+        if t.dtype is not dtype or t.numel() != tokens * self._row or t.get_device() != self._index or not t.is_contiguous():
             raise bad(f"{what} must be contiguous {dtype} [{tokens}, {self.kv_heads}, {self.head_dim}] on {self.device}")
         return t.data_ptr()
 
@@ -107,27 +108,32 @@ class Kv4Cache:
         """Quantise the rows k, v into slots[i] = page * page_size + position (-1: skip the row).
 
         k_back / v_back (both or neither) receive the values the cache now holds."""
-        select_device(self._index)
-        n = slots.shape[0]
-        kind = dtype_id(k, "k")
-        if v.dtype is not k.dtype:
-            raise bad(f"k is {k.dtype}, v is {v.dtype}")
+        if _several:
+            select_device(self._index)
+        n, dtype = slots.numel(), k.dtype
+        kind = _DTYPES.get(dtype)
+        if kind is None:
+            dtype_id(k, "k")
+        if v.dtype is not dtype:
+            raise bad(f"k is {dtype}, v is {v.dtype}")
         ks, vs = self._rows(k, n, "k"), self._rows(v, n, "v")
-        rc = self._append(*self._shape, k.data_ptr(), v.data_ptr(), kind, ks, vs, self._ints(slots, (n,), "slots"), n,
-                          self._dense(k_back, n, k.dtype, "k_back"), self._dense(v_back, n, k.dtype, "v_back"),
+        kb = None if k_back is None else self._dense(k_back, n, dtype, "k_back")
+        vb = None if v_back is None else self._dense(v_back, n, dtype, "v_back")
+        rc = self._append(*self._shape, k.data_ptr(), v.data_ptr(), kind, ks, vs, self._ints(slots, n, "slots"), n, kb, vb,
                           stream or current_stream(self._index))
         if rc:
             native.check(rc)
 
     def read(self, slots: torch.Tensor, dtype=torch.float32, k_out=None, v_out=None, stream=None):
         """Rows of the given slots as (k, v), [n, kv_heads, head_dim] each; zeros where a slot is -1."""
-        select_device(self._index)
-        n = slots.shape[0]
+        if _several:
+            select_device(self._index)
+        n = slots.numel()
         if k_out is None and v_out is None:
             k_out, v_out = (torch.empty(n, self.kv_heads, self.head_dim, dtype=dtype, device=self.device) for _ in range(2))
         some = k_out if k_out is not None else v_out
         rc = self._read(self._dense(k_out, n, some.dtype, "k_out"), self._dense(v_out, n, some.dtype, "v_out"),
-                        dtype_id(some, "k_out"), *self._shape, self._ints(slots, (n,), "slots"), n,
+                        dtype_id(some, "k_out"), *self._shape, self._ints(slots, n, "slots"), n,
                         stream or current_stream(self._index))
         if rc:
             native.check(rc)
@@ -135,18 +141,21 @@ class Kv4Cache:
 
     # -- attention -------------------------------------------------------------
     def _workspace(self, q_len: int, q_heads: int, stream: int):
+        """(address, bytes) of a workspace for this shape of query on this stream."""
         need = self._work_size(q_len, q_heads, self.kv_heads, self.head_dim)
         if need < 0:
             native.check(int(need))
-        have = self._work.get(stream)
-        if have is None or have[1] < need:
+        have = self._buffers.get(stream)
+        if have is None or have.numel() < need:
             # zeroed on torch's current stream; another stream's kernels neither wait for that nor hold the
             # old buffer, so there the device is waited for, once
-            new = (torch.zeros(need, dtype=torch.uint8, device=self.device), need)
+            have = torch.zeros(need, dtype=torch.uint8, device=self.device)
             if stream != current_stream(self._index):
                 torch.cuda.synchronize(self.device)
-            have = self._work[stream] = new
-        return have
+            self._buffers[stream] = have
+            self._work = {k: v for k, v in self._work.items() if k[0] != stream}
+        got = self._work[stream, q_len, q_heads] = (have.data_ptr(), have.numel())
+        return got
 
     def attend(self, q: torch.Tensor, seq_lens: torch.Tensor, block_table=None, window: int = 0, scale=None,
                soft_cap: float = 0.0, out=None, stream=None) -> torch.Tensor:
@@ -154,7 +163,8 @@ class Kv4Cache:
 
         block_table: int32 [batch, pages a sequence], or None where sequence b is page b.  scale: 1 / sqrt(head_dim)
         by default.  Returns out, contiguous, of q's type."""
-        select_device(self._index)
+        if _several:
+            select_device(self._index)
         shape, st = q.shape, q.stride()
         if len(shape) != 4 or shape[3] != self.head_dim or q.get_device() != self._index:
             raise bad(f"q must be [batch, q_len, q_heads, {self.head_dim}] on {self.device}, not {tuple(shape)} on {q.device}")
@@ -170,12 +180,16 @@ class Kv4Cache:
         table, width = None, 0
         if block_table is not None:
             width = block_table.shape[-1]
-            table = self._ints(block_table, (batch, width), "block_table")
+            if block_table.dtype is not torch.int32 or block_table.shape != (batch, width) or \
+                    block_table.get_device() != self._index or not block_table.is_contiguous():
+                raise bad(f"block_table must be contiguous int32 [{batch}, pages a sequence] on {self.device}")
+            table = block_table.data_ptr()
         stream = stream or current_stream(self._index)
-        work, size = self._workspace(q_len, q_heads, stream)
+        have = self._work.get((stream, q_len, q_heads))
+        work, size = have if have is not None else self._workspace(q_len, q_heads, stream)
         rc = self._attend(out.data_ptr(), q.data_ptr(), kind, q_stride, *self._shape, table, width,
-                          self._ints(seq_lens, (batch,), "seq_lens"), batch, q_len, q_heads, window,
-                          D ** -0.5 if scale is None else scale, soft_cap, work.data_ptr(), size, stream)
+                          self._ints(seq_lens, batch, "seq_lens"), batch, q_len, q_heads, window,
+                          D ** -0.5 if scale is None else scale, soft_cap, work, size, stream)
         if rc:
             native.check(rc)
         return out

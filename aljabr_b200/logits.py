@@ -5,7 +5,17 @@ from __future__ import annotations
 import torch
 
 from . import native
-from .kv4 import bad, current_stream, dtype_id, select_device
+from .kv4 import _several, bad, current_stream, dtype_id, select_device
+
+
+_process = native.lib().aljabr_blackwell_logits_process_dev
+_I32, _F32 = torch.int32, torch.float32
+
+
+def _ptr(t, dtype, count, dev, what):
+    if t.dtype is not dtype or t.numel() != count or t.get_device() != dev or not t.is_contiguous():
+        raise bad(f"{what} must be {count} contiguous {dtype} on device {dev}, not {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
 def process_logits(logits: torch.Tensor, history=None, history_len=None, penalties=None, bias_tokens=None,
@@ -21,14 +31,8 @@ def process_logits(logits: torch.Tensor, history=None, history_len=None, penalti
     if len(shape) != 2 or st[1] != 1 or dev < 0:
         raise bad("logits must be a [rows, vocab] CUDA tensor with contiguous rows")
     rows, vocab = shape
-    select_device(dev)
-
-    def ptr(t, dtype, shape, what):
-        if t is None:
-            return None
-        if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
-            raise bad(f"{what} must be contiguous {dtype} {shape} on {logits.device}")
-        return t.data_ptr()
+    if _several:
+        select_device(dev)
 
     if out is None:
         out = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
@@ -36,17 +40,26 @@ def process_logits(logits: torch.Tensor, history=None, history_len=None, penalti
         raise bad(f"out must be float32 [{rows}, {vocab}] on {logits.device} with contiguous rows")
     if token is None:
         token = torch.empty(rows, dtype=torch.int32, device=logits.device)
-    nh = 0 if history is None else history.shape[-1]
-    nb = 0 if bias_tokens is None else bias_tokens.shape[-1]
-    na = 0 if allow is None else allow.shape[-1]
-    i32, f32 = torch.int32, torch.float32
-    rc = native.lib().aljabr_blackwell_logits_process_dev(
-        out.data_ptr(), out.stride(0) if rows > 1 else vocab, logits.data_ptr(), dtype_id(logits, "logits"),
-        st[0] if rows > 1 else vocab, rows, vocab, ptr(history, i32, (rows, nh), "history"),
-        ptr(history_len, i32, (rows,), "history_len"), nh, ptr(penalties, f32, (rows, 3), "penalties"),
-        ptr(bias_tokens, i32, (rows, nb), "bias_tokens"), ptr(bias_values, f32, (rows, nb), "bias_values"),
-        ptr(bias_len, i32, (rows,), "bias_len"), nb, ptr(allow, i32, (rows, na), "allow"), na,
-        ptr(token, i32, (rows,), "token"), stream or current_stream(dev))
+    h = hl = pen = bt = bv = bl = al = None
+    nh = nb = na = 0
+    if history is not None:
+        if history_len is None or penalties is None or penalties.shape[-1] != 3:
+            raise bad("a history needs history_len [rows] and penalties [rows, 3]")
+        nh = history.shape[-1]
+        h, hl = _ptr(history, _I32, rows * nh, dev, "history"), _ptr(history_len, _I32, rows, dev, "history_len")
+        pen = _ptr(penalties, _F32, rows * 3, dev, "penalties")
+    if bias_tokens is not None:
+        if bias_values is None or bias_len is None:
+            raise bad("bias_tokens needs bias_values and bias_len")
+        nb = bias_tokens.shape[-1]
+        bt, bv = _ptr(bias_tokens, _I32, rows * nb, dev, "bias_tokens"), _ptr(bias_values, _F32, rows * nb, dev, "bias_values")
+        bl = _ptr(bias_len, _I32, rows, dev, "bias_len")
+    if allow is not None:
+        na = allow.shape[-1]
+        al = _ptr(allow, _I32, rows * na, dev, "allow")
+    rc = _process(out.data_ptr(), out.stride(0) if rows > 1 else vocab, logits.data_ptr(), dtype_id(logits, "logits"),
+                  st[0] if rows > 1 else vocab, rows, vocab, h, hl, nh, pen, bt, bv, bl, nb, al, na,
+                  _ptr(token, _I32, rows, dev, "token"), stream or current_stream(dev))
     if rc:
         native.check(rc)
     return out, token

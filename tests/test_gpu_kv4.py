@@ -255,14 +255,14 @@ def test_results_repeat_and_leave_the_workspace_ready():
     cache, q, sl, table, out, k64, v64 = attend_case(11, 128, 2, 4, 1, 16, [4000, 100, 9000])
     for _ in range(3):
         assert torch.equal(cache.attend(q, sl, table), out)
-    (work, _), = cache._work.values()
+    work, = cache._buffers.values()
     assert int(work[:1024].int().sum()) == 0
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
         again = cache.attend(q, sl, table)
     s.synchronize()
-    assert torch.equal(again, out) and len(cache._work) == 2
+    assert torch.equal(again, out) and len(cache._buffers) == 2
 
 
 def test_call_replays_in_a_graph_with_growing_lengths():
