@@ -57,6 +57,16 @@
 // instructions.  Pages of fewer than 64 positions would take up to 32 such
 // copies a chunk, which one warp issues one after the other (~100 cycles
 // each): there every warp copies its own tile in 16-byte pieces instead.
+//
+// Measured (1965 MHz, measured copy rate 6473 GB/s): two sequences of 131072,
+// 64 query heads on 8 kv heads, D 128, bf16: 80 us, 3.8 TB/s; 32 ragged
+// sequences up to 16384: 56 us, 3.2 TB/s; 4096 positions of one sequence, fp32:
+// 11.3 us.  The long ones are bound by issue: 374 instructions a tile (2304
+// bytes) at 2.45 a clock and SM, ALU pipe 55 % busy, DRAM 44 %; the short ones
+// by the chain launch - lengths - page - tile - merge - join.  Tried and
+// slower: scores of the next tile beside the values of this one (84 us), tiles
+// asked for 3 chunks ahead (88 us), one loop with the item's start inside
+// (116 us: the registers no longer hold).
 #include "kv4.cuh"
 
 #include <algorithm>
@@ -373,8 +383,8 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     __syncthreads();
     const Tables tab = {s_pre, s_len};
     // A chunk costs a CTA about as much as 25 parts cost the one that joins them, so where the line is short an item
-    // of n places is cut into stretches of sqrt(n / 25): one kv head of 32768 positions 23 us with 256 CTAs a chunk
-    // each, 17 with 128.
+    // of n places is cut into stretches of sqrt(n / 25): one kv head of 32768 positions 23 us with 256 CTAs of a
+    // chunk each, 16 so.
     const int stretch = max(1, __float2int_rn(sqrtf(static_cast<float>(total) / (25.0f * p.batch))));
     total *= items;
     const int ctas = min(static_cast<int>(gridDim.x), (total + stretch - 1) / stretch);

@@ -14,9 +14,12 @@
 // is immaterial), adds the biases with one warp in list order, and lists each
 // such token once.  The chunk is then streamed with a mask, a store and a
 // maximum a logit; the listed tokens are finished by one thread each, so that
-// their divisions are not paid by whole warps.  (Tables read and keys formed
-// for every logit: 75 instructions each, 105 us for 96 x 128256 against the
-// floor of 16.)
+// their divisions are not paid by whole warps.  Measured: 96 x 128256 fp32
+// logits with a mask, 4000 history entries and 64 biases a row 61 us (1.7 TB/s;
+// floor 16 us); one such row 5.5 us.  Tables read and keys formed for every
+// logit: 105 us.  What bounds it now is the chain of phases in a CTA (load,
+// count, stream, finish) with 2 CTAs an SM to overlap: 3 CTAs by 40 registers
+// spill (76 us), halves of the chunk scan the history twice (80 us).
 // The greedy token is reduced over the cluster through distributed shared
 // memory: no workspace and no second launch.
 // Every step of the arithmetic is one rounded fp32 operation, as written.
@@ -64,6 +67,15 @@ __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, int
     }
 }
 
+// The 16-byte pieces inside [p, p + bytes) into L2.
+__device__ __forceinline__ void prefetch_l2(const void* p, size_t bytes) {
+    const uintptr_t first = (reinterpret_cast<uintptr_t>(p) + 15) & ~uintptr_t(15);
+    const uintptr_t end = (reinterpret_cast<uintptr_t>(p) + bytes) & ~uintptr_t(15);
+    for (uintptr_t at = first; at < end; at += 16384)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(at), "r"(static_cast<uint32_t>(min(end - at, uintptr_t(16384))))
+                     : "memory");
+}
+
 // A float as an unsigned number of the same order; -0 counts as +0.
 __device__ __forceinline__ uint32_t order_bits(float v) {
     const uint32_t b = __float_as_uint(v + 0.0f);
@@ -71,7 +83,7 @@ __device__ __forceinline__ uint32_t order_bits(float v) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a, int share, int vec_in, int vec_out) {
+__global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a, int share, int vec_in, int vec_out, int ahead) {
     extern __shared__ uint4 s_tables[];             // hit counts [kChunk], biases [kChunk], listed tokens [kChunk] (16 bits)
     uint32_t* const s_count = reinterpret_cast<uint32_t*>(s_tables);
     float* const s_bias = reinterpret_cast<float*>(s_count + kChunk);
@@ -96,6 +108,13 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
     const T* in = static_cast<const T*>(a.logits) + row * a.in_stride;
     float* out = a.out + row * a.out_stride;
     const int* hist = a.history + static_cast<long long>(row) * a.history_stride;
+    // What the CTA that takes this one's place will read, into L2: rows come in order, `ahead` of them at a time.
+    if (threadIdx.x == 0 && row + ahead < a.rows) {
+        const int first = min(a.vocab, rank * share), many = min(a.vocab, first + share) - first;
+        prefetch_l2(static_cast<const T*>(a.logits) + (row + ahead) * a.in_stride + first, many * sizeof(T));
+        if (a.allow) prefetch_l2(a.allow + static_cast<long long>(row + ahead) * a.allow_stride + first / 32, many / 8);
+        if (a.history && rank == 0) prefetch_l2(a.history + static_cast<long long>(row + ahead) * a.history_stride, a.history_stride * 4u);
+    }
     // everything that does not depend on the lengths is asked for along with them
     const int hist_len = a.history ? __ldg(a.history_len + row) : 0;
     const int bias_len = a.bias_tokens ? __ldg(a.bias_len + row) : 0;
@@ -111,6 +130,18 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
         const int i = j * kLThreads + static_cast<int>(threadIdx.x);
         seen[j] = a.history && i < a.history_stride ? __ldg(hist + i) : -1;
     }
+    // the last warp has the biases: the first 64 entries ahead of time
+    const int* bias_tokens = a.bias_tokens + static_cast<long long>(row) * a.bias_stride;
+    const float* bias_values = a.bias_values + static_cast<long long>(row) * a.bias_stride;
+    const bool biaser = a.bias_tokens && threadIdx.x >= kLThreads - 32;
+    int bt[2] = {-1, -1};
+    float bv[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        if (biaser && j * 32 + lane < a.bias_stride) {
+            bt[j] = __ldg(bias_tokens + j * 32 + lane);
+            bv[j] = __ldg(bias_values + j * 32 + lane);
+        }
     const uint32_t* allow = a.allow ? a.allow + static_cast<long long>(row) * a.allow_stride : nullptr;
     const int v0 = min(a.vocab, rank * share), v1 = min(a.vocab, v0 + share);
     unsigned long long best = 0ull;                 // 0: no candidate
@@ -139,22 +170,45 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
                 const uint32_t bit = 1u << (t & 31);
                 if (!(atomicOr(s_mark + (t >> 5), bit) & bit)) s_list[atomicAdd(&s_listed, 1)] = static_cast<uint16_t>(t);
             };
-            auto count = [&](int token) {
-                const int t = token - c0;
+            // A thread's entries first mark and count, all in flight together; then it takes its places in the list
+            // at once.
+            uint32_t old[kSeen];
+#pragma unroll
+            for (int j = 0; j < kSeen; ++j) {
+                const int t = seen[j] - c0;
+                old[j] = 0xFFFFFFFFu;
+                if (static_cast<unsigned int>(t) < static_cast<unsigned int>(n) &&
+                    j * kLThreads + static_cast<int>(threadIdx.x) < n_hist) {
+                    atomicAdd(s_count + t, 1u);
+                    old[j] = atomicOr(s_mark + (t >> 5), 1u << (t & 31));
+                }
+            }
+            uint32_t claimed = 0u;
+#pragma unroll
+            for (int j = 0; j < kSeen; ++j)
+                claimed |= ((old[j] >> ((seen[j] - c0) & 31)) & 1u) ? 0u : 1u << j;
+            if (claimed) {
+                int place = atomicAdd(&s_listed, __popc(claimed));
+#pragma unroll
+                for (int j = 0; j < kSeen; ++j)
+                    if ((claimed >> j) & 1u) s_list[place++] = static_cast<uint16_t>(seen[j] - c0);
+            }
+            for (int i = kSeen * kLThreads + static_cast<int>(threadIdx.x); i < n_hist; i += kLThreads) {
+                const int t = __ldg(hist + i) - c0;
                 if (static_cast<unsigned int>(t) < static_cast<unsigned int>(n)) {
                     atomicAdd(s_count + t, 1u);
                     list(t);
                 }
-            };
-#pragma unroll
-            for (int j = 0; j < kSeen; ++j)
-                if (j * kLThreads + static_cast<int>(threadIdx.x) < n_hist) count(seen[j]);
-            for (int i = kSeen * kLThreads + static_cast<int>(threadIdx.x); i < n_hist; i += kLThreads) count(__ldg(hist + i));
-            if (n_bias > 0 && threadIdx.x >= kLThreads - 32) {   // the last warp, 32 entries at a time, in order
+            }
+            if (n_bias > 0 && biaser) {   // the last warp, 32 entries at a time, in order
                 for (int i0 = 0; i0 < n_bias; i0 += 32) {
-                    const long long i = static_cast<long long>(row) * a.bias_stride + i0 + lane;
-                    const int t = i0 + lane < n_bias ? __ldg(a.bias_tokens + i) - c0 : -1;
-                    const float b = i0 + lane < n_bias ? __ldg(a.bias_values + i) : 0.0f;
+                    int t = -1;
+                    float b = 0.0f;
+                    if (i0 + lane < n_bias) {
+                        t = i0 == 0 ? bt[0] : i0 == 32 ? bt[1] : __ldg(bias_tokens + i0 + lane);
+                        b = i0 == 0 ? bv[0] : i0 == 32 ? bv[1] : __ldg(bias_values + i0 + lane);
+                        t = static_cast<unsigned int>(t) < static_cast<unsigned int>(a.vocab) ? t - c0 : -1;
+                    }
                     const bool mine = static_cast<unsigned int>(t) < static_cast<unsigned int>(n);
                     const unsigned int same = __match_any_sync(0xffffffffu, mine ? t : -1 - lane);
                     float sum = mine ? s_bias[t] : 0.0f;
@@ -300,7 +354,8 @@ cudaError_t launch_typed(const LogitsArgs& a, int sms, cudaStream_t stream) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kernel, a, share, vec_in, vec_out);
+    const int ahead = std::max(1, 2 * sms / ranks);   // rows under way: two CTAs an SM
+    return cudaLaunchKernelEx(&cfg, kernel, a, share, vec_in, vec_out, ahead);
 }
 
 }  // namespace
