@@ -5,7 +5,8 @@ registerDecodeLayer / registerOutput / decodeStepToken,
 engine/gguf/aljabr-gguf-java/.../javabackend/GgufMetalBridge.java:1879-2053)
 for a Llama-shaped model whose linear weights are NF4 or, through
 register_layer_typed / register_output_typed, GGUF Q4_0 / Q8_0 / Q4_K / Q6_K
-with one type per tensor (registerDecodeLayer's typeQ .. typeDown).
+with one type per tensor (registerDecodeLayer's typeQ .. typeDown).  The KV
+cache is bf16, fp32 or, with LlamaShape(kv_dtype=native.KV_Q4), 4 bits.
 
 Weights may be given as numpy arrays (registered as model buffers: copied to
 HBM once, kept alive by this object) or as device addresses (ints, e.g.
