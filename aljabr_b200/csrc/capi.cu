@@ -1510,7 +1510,7 @@ int aljabr_blackwell_logits_process_dev(float* out, long long out_stride, const 
     a.out_stride = out_stride;
     a.history = history;
     a.history_len = history_len;
-    a.history_stride = history_stride;
+    a.history_stride = history ? history_stride : 0;
     a.penalties = penalties;
     a.bias_tokens = bias_tokens;
     a.bias_values = bias_values;

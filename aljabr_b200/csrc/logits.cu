@@ -15,11 +15,12 @@
 // such token once.  The chunk is then streamed with a mask, a store and a
 // maximum a logit; the listed tokens are finished by one thread each, so that
 // their divisions are not paid by whole warps.  Measured: 96 x 128256 fp32
-// logits with a mask, 4000 history entries and 64 biases a row 61 us (1.7 TB/s;
-// floor 16 us); one such row 5.5 us.  Tables read and keys formed for every
-// logit: 105 us.  What bounds it now is the chain of phases in a CTA (load,
-// count, stream, finish) with 2 CTAs an SM to overlap: 3 CTAs by 40 registers
-// spill (76 us), halves of the chunk scan the history twice (80 us).
+// logits with a mask, 4000 history entries and 64 biases a row 58 us (1.8 TB/s;
+// floor 16 us); one row with 300 entries 5.7 us.  Tables read and keys formed
+// for every logit: 105 us.  What bounds it now is the chain of phases in a CTA
+// (load, count, stream, finish) with 2 CTAs an SM to overlap: issue slots 44 %
+// busy, DRAM 12 %.  3 CTAs by 40 registers spill (76 us), halves of the chunk
+// scan the history twice (80 us).
 // The greedy token is reduced over the cluster through distributed shared
 // memory: no workspace and no second launch.
 // Every step of the arithmetic is one rounded fp32 operation, as written.
@@ -94,8 +95,10 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
     __shared__ uint64_t s_bar;                      // rank 0: the cluster's keys have arrived
     __shared__ int s_listed;
     const int row = blockIdx.y, rank = blockIdx.x, ranks = gridDim.x;
-    const int lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+r"(tid));                  // kept in a register, not read again where it is used
+    const int lane = tid & 31;
+    if (tid == 0) {
         mbar_init(&s_bar, 1);
         fence_mbar_init();
         mbar_arrive_expect_tx(&s_bar, ranks * 8);
@@ -109,7 +112,7 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
     float* out = a.out + row * a.out_stride;
     const int* hist = a.history + static_cast<long long>(row) * a.history_stride;
     // What the CTA that takes this one's place will read, into L2: rows come in order, `ahead` of them at a time.
-    if (threadIdx.x == 0 && row + ahead < a.rows) {
+    if (tid == 0 && row + ahead < a.rows) {
         const int first = min(a.vocab, rank * share), many = min(a.vocab, first + share) - first;
         prefetch_l2(static_cast<const T*>(a.logits) + (row + ahead) * a.in_stride + first, many * sizeof(T));
         if (a.allow) prefetch_l2(a.allow + static_cast<long long>(row + ahead) * a.allow_stride + first / 32, many / 8);
@@ -127,13 +130,13 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
     int seen[kSeen];                                // the first history entries
 #pragma unroll
     for (int j = 0; j < kSeen; ++j) {
-        const int i = j * kLThreads + static_cast<int>(threadIdx.x);
-        seen[j] = a.history && i < a.history_stride ? __ldg(hist + i) : -1;
+        const int i = j * kLThreads + tid;
+        seen[j] = i < a.history_stride ? __ldg(hist + i) : -1;   // the stride is 0 without a history
     }
     // the last warp has the biases: the first 64 entries ahead of time
     const int* bias_tokens = a.bias_tokens + static_cast<long long>(row) * a.bias_stride;
     const float* bias_values = a.bias_values + static_cast<long long>(row) * a.bias_stride;
-    const bool biaser = a.bias_tokens && threadIdx.x >= kLThreads - 32;
+    const bool biaser = a.bias_tokens && tid >= kLThreads - 32;
     int bt[2] = {-1, -1};
     float bv[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -147,53 +150,54 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
     unsigned long long best = 0ull;                 // 0: no candidate
     for (int c0 = v0; c0 < v1; c0 += kChunk) {
         const int c1 = min(v1, c0 + kChunk), n = c1 - c0;
+        const bool quads = vec_in && vec_out && n % 4 == 0;   // every run of 4 is whole or absent
         float x[kPer / 4][4];
         uint32_t ok[kPer / 4];
 #pragma unroll
         for (int j = 0; j < kPer / 4; ++j) {
-            const int i = c0 + 4 * (j * kLThreads + static_cast<int>(threadIdx.x));
-            load4<T>(in + min(i, c1), c1 - i, vec_in != 0, x[j]);
-            ok[j] = 15u;
-            if (allow && i < c1) ok[j] = __ldg(allow + (i >> 5)) >> (i & 31);
-            if (i + 4 > c1) ok[j] &= i < c1 ? (1u << (c1 - i)) - 1u : 0u;
+            const int at = 4 * (j * kLThreads + tid), i = c0 + at;
+            ok[j] = 0u;
+            if (quads) {
+                x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.0f;
+                if (at < n) {
+                    load4<T>(in + i, 4, true, x[j]);
+                    ok[j] = 15u;
+                    if (allow) ok[j] = __ldg(allow + (i >> 5)) >> (i & 31);
+                }
+            } else {
+                load4<T>(in + min(i, c1), c1 - i, vec_in != 0, x[j]);
+                if (at < n) ok[j] = allow ? __ldg(allow + (i >> 5)) >> (i & 31) : 15u;
+                if (at + 4 > n && at < n) ok[j] &= (1u << (n - at)) - 1u;
+            }
         }
         const int n_hist = max(0, min(hist_len, a.history_stride)), n_bias = max(0, min(bias_len, a.bias_stride));
         const bool special = n_hist > 0 || n_bias > 0;
         if (special) {
             const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
             const int words = (n_bias > 0 ? 2 : 1) * kChunk / 4;
-            for (int i = threadIdx.x; i < words; i += kLThreads) s_tables[i] = zero;
-            for (int i = threadIdx.x; i < kChunk / 32; i += kLThreads) s_mark[i] = 0u;
-            if (threadIdx.x == 0) s_listed = 0;
+            for (int i = tid; i < words; i += kLThreads) s_tables[i] = zero;
+            for (int i = tid; i < kChunk / 32; i += kLThreads) s_mark[i] = 0u;
+            if (tid == 0) s_listed = 0;
             __syncthreads();
             auto list = [&](int t) {
                 const uint32_t bit = 1u << (t & 31);
                 if (!(atomicOr(s_mark + (t >> 5), bit) & bit)) s_list[atomicAdd(&s_listed, 1)] = static_cast<uint16_t>(t);
             };
-            // A thread's entries first mark and count, all in flight together; then it takes its places in the list
-            // at once.
-            uint32_t old[kSeen];
-#pragma unroll
-            for (int j = 0; j < kSeen; ++j) {
-                const int t = seen[j] - c0;
-                old[j] = 0xFFFFFFFFu;
-                if (static_cast<unsigned int>(t) < static_cast<unsigned int>(n) &&
-                    j * kLThreads + static_cast<int>(threadIdx.x) < n_hist) {
-                    atomicAdd(s_count + t, 1u);
-                    old[j] = atomicOr(s_mark + (t >> 5), 1u << (t & 31));
-                }
-            }
-            uint32_t claimed = 0u;
+            // A thread's entries in this chunk, few of them: found together, counted one after the other
+            uint32_t here = 0u;
 #pragma unroll
             for (int j = 0; j < kSeen; ++j)
-                claimed |= ((old[j] >> ((seen[j] - c0) & 31)) & 1u) ? 0u : 1u << j;
-            if (claimed) {
-                int place = atomicAdd(&s_listed, __popc(claimed));
-#pragma unroll
-                for (int j = 0; j < kSeen; ++j)
-                    if ((claimed >> j) & 1u) s_list[place++] = static_cast<uint16_t>(seen[j] - c0);
+                if (static_cast<unsigned int>(seen[j] - c0) < static_cast<unsigned int>(n)) here |= 1u << j;
+            const int mine_in = (n_hist - tid + kLThreads - 1) / kLThreads;   // this thread's entries
+            if (mine_in < kSeen) here &= (1u << max(0, mine_in)) - 1u;
+            while (here) {
+                const int j = __ffs(here) - 1;
+                here &= here - 1u;
+                const int t = __ldg(hist + j * kLThreads + tid) - c0;   // read again: registers have no index
+                atomicAdd(s_count + t, 1u);
+                list(t);
             }
-            for (int i = kSeen * kLThreads + static_cast<int>(threadIdx.x); i < n_hist; i += kLThreads) {
+            for (int i = kSeen * kLThreads + tid; i < n_hist; i += kLThreads) {
                 const int t = __ldg(hist + i) - c0;
                 if (static_cast<unsigned int>(t) < static_cast<unsigned int>(n)) {
                     atomicAdd(s_count + t, 1u);
@@ -248,34 +252,38 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
         int mine = -1;
         float mine_v = 0.0f;
         uint32_t mine_ok = 0u;
-        if (static_cast<int>(threadIdx.x) < listed) {
-            mine = s_list[threadIdx.x];
+        if (tid < listed) {
+            mine = s_list[tid];
             mine_v = static_cast<float>(in[c0 + mine]);
             mine_ok = allowed(c0 + mine);
         }
-        // stream the chunk, leaving the listed tokens out
+        // stream the chunk; a listed token's logit is written as it is and replaced below
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < kPer / 4; ++j) {
-            const int at = 4 * (j * kLThreads + static_cast<int>(threadIdx.x)), i = c0 + at;
-            const uint32_t marks = special && at < n ? s_mark[at >> 5] >> (at & 31) : 0u;
-            float y[4];
+            const int at = 4 * (j * kLThreads + tid);
+            const uint32_t marks = special && at < n ? (s_mark[at >> 5] >> (at & 31)) & 15u : 0u;
+            const uint32_t keep = ok[j] | marks;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                y[e] = (ok[j] >> e) & 1u ? x[j][e] : -INFINITY;
-                x[j][e] = (ok[j] & ~marks) >> e & 1u ? x[j][e] : __int_as_float(0x7FFFFFFF);   // not a candidate
-                top = fmaxf(top, x[j][e]);          // a NaN does not count
-            }
-            if (vec_out && i + 4 <= c1 && (marks & 15u) == 0u) {
-                *reinterpret_cast<float4*>(out + i) = make_float4(y[0], y[1], y[2], y[3]);
+            for (int e = 0; e < 4; ++e) x[j][e] = (keep >> e) & 1u ? x[j][e] : -INFINITY;
+            if (quads) {
+                if (at < n) *reinterpret_cast<float4*>(out + c0 + at) = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
+            } else if (vec_out && at + 4 <= n) {
+                *reinterpret_cast<float4*>(out + c0 + at) = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (i + e < c1 && !((marks >> e) & 1u)) out[i + e] = y[e];
+                    if (at + e < n) out[c0 + at + e] = x[j][e];
             }
+            if (marks) {                            // no candidate here
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[j][e] = (marks >> e) & 1u ? -INFINITY : x[j][e];
+            }
+            top = fmaxf(top, fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])));   // a NaN does not count
         }
+        if (special) __syncthreads();               // the logits above are written
         if (mine >= 0) finish(mine, mine_v, mine_ok);
-        for (int k = kLThreads + static_cast<int>(threadIdx.x); k < listed; k += kLThreads) {
+        for (int k = kLThreads + tid; k < listed; k += kLThreads) {
             const int t = s_list[k];
             finish(t, static_cast<float>(in[c0 + t]), allowed(c0 + t));
         }
@@ -283,12 +291,20 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
         if (a.token) {
             const uint32_t high = __reduce_max_sync(0xffffffffu, order_bits(top));
             unsigned int first = 0xFFFFFFFFu;
-            if (order_bits(top) == high) {
+            if (high == order_bits(-INFINITY)) {    // rarely: nothing above -inf; a logit of -inf that is allowed counts
+                for (int j = 0; j < kPer; ++j) {
+                    const int at = 4 * ((j >> 2) * kLThreads + tid) + (j & 3);
+                    if (at >= n || (special && (s_mark[at >> 5] >> (at & 31)) & 1u)) continue;
+                    if (((allowed(c0 + at) >> ((c0 + at) & 31)) & 1u) && out[c0 + at] == -INFINITY &&
+                        (a.out != a.logits ? static_cast<float>(in[c0 + at]) == -INFINITY : true))
+                        first = min(first, static_cast<unsigned int>(c0 + at));
+                }
+            } else if (order_bits(top) == high) {
 #pragma unroll
                 for (int j = kPer / 4 - 1; j >= 0; --j)
 #pragma unroll
                     for (int e = 3; e >= 0; --e)
-                        if (x[j][e] == top) first = c0 + 4 * (j * kLThreads + static_cast<int>(threadIdx.x)) + e;
+                        if (x[j][e] == top) first = c0 + 4 * (j * kLThreads + tid) + e;
             }
             first = __reduce_min_sync(0xffffffffu, first);
             if (first != 0xFFFFFFFFu) best = max(best, (static_cast<unsigned long long>(high) << 32) | (0xFFFFFFFFu - first));
@@ -299,9 +315,9 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_kernel(const LogitsArgs a
     if (!a.token) return;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) s_key[threadIdx.x >> 5] = best;
+    if (lane == 0) s_key[tid >> 5] = best;
     __syncthreads();
-    if (threadIdx.x >= 32) return;
+    if (tid >= 32) return;
     best = lane < kLThreads / 32 ? s_key[lane] : 0ull;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));

@@ -64,6 +64,30 @@ def test_restored_cache_continues_alike():
         b.close()
 
 
+def test_context_that_is_no_multiple_of_a_tile():
+    """max_ctx 21: the cache is padded to 32 positions, the model still ends at 21."""
+    from aljabr_b200 import native
+    from aljabr_b200.decode import LlamaShape
+    native.call("aljabr_blackwell_init", 0)
+    shape = LlamaShape(**{**SHAPES["small"], "max_ctx": 21}, kv_dtype=2)
+    weights = _model(43, shape)
+    a, b = _build(shape, *weights), _build(shape, *weights)
+    try:
+        run = a.run(9, 0, 21)
+        token = 9
+        for pos in range(21):
+            token, _ = b.step(token, pos)
+            assert token == run[pos]
+        _, ka, va = a.read_state()
+        _, kb, vb = b.read_state()
+        assert ka.shape[1] == 21 and np.array_equal(ka, kb) and np.array_equal(va, vb) and np.abs(ka[:, 20]).max() > 0
+        with pytest.raises(native.ProviderError):
+            a.step(1, 21)
+    finally:
+        a.close()
+        b.close()
+
+
 def test_generate_applies_the_rules():
     from tests.test_gpu_logits import reference
     shape, (a, b) = _pair("small", 2, 2)

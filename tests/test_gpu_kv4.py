@@ -234,6 +234,39 @@ def test_queries_of_any_size(factor):
     check(cache.attend(qf, sl, table), qf, k64, v64, [150])
 
 
+def test_non_finite_queries_stay_in_their_rows():
+    for dtype in (torch.float32, torch.bfloat16):
+        cache, q, sl, table, out, _, _ = attend_case(16, 128, 2, 4, 1, 16, [70], dtype=dtype)
+        bad = q.clone()
+        bad[0, 0, 1, 5], bad[0, 0, 6, 0] = float("nan"), float("inf")
+        got = cache.attend(bad, sl, table)
+        assert torch.isnan(got[0, 0, [1, 6]]).all()
+        rest = [0, 2, 3, 4, 5, 7]
+        assert torch.equal(got[0, 0, rest], out[0, 0, rest])
+
+
+def test_wrapper_refusals():
+    cache = make(4, 16, 2, 64)
+    k = torch.zeros(3, 2, 64, device="cuda")
+    slots = torch.arange(3, dtype=torch.int32, device="cuda")
+    q = torch.zeros(1, 1, 4, 64, device="cuda")
+    lens, table = torch.ones(1, dtype=torch.int32, device="cuda"), torch.zeros(1, 4, dtype=torch.int32, device="cuda")
+    bad = native.ProviderError
+    for call in (lambda: cache.append(k.cpu(), k, slots), lambda: cache.append(k, k[:2], slots),
+                 lambda: cache.append(k, k.bfloat16(), slots), lambda: cache.append(k.half(), k.half(), slots),
+                 lambda: cache.append(k, k, slots.long()), lambda: cache.append(k, k, slots, k_back=torch.empty_like(k)),
+                 lambda: cache.append(k.transpose(1, 2), k, slots), lambda: cache.read(slots, dtype=torch.float16),
+                 lambda: cache.read(slots[::2]), lambda: cache.attend(q[0], lens, table),
+                 lambda: cache.attend(q, lens.long(), table), lambda: cache.attend(q, lens, table[:, ::2]),
+                 lambda: cache.attend(q, lens, table, out=torch.empty(1, 1, 4, 64, device="cuda", dtype=torch.bfloat16)),
+                 lambda: cache.attend(torch.zeros(1, 1, 3, 64, device="cuda"), lens, table),
+                 lambda: cache.attend(q, lens, table, window=-1)):
+        with pytest.raises(bad):
+            call()
+    with pytest.raises(native.UnsupportedOperation):
+        make(4, 16, 2, 96)
+
+
 def test_values_of_very_different_size():
     """A first position with nearly all the weight and tiny values, as attention sinks have."""
     rng = np.random.default_rng(10)

@@ -127,6 +127,36 @@ def test_ties_nan_and_empty_rows():
     assert np.isneginf(out[5]).all() and np.isnan(out[3]).all()
 
 
+def test_rows_with_nothing_above_minus_infinity():
+    """All allowed logits -inf: the lowest allowed index that is no listed token is as good as any, so the lowest of all
+    allowed ones wins; in place too."""
+    from aljabr_b200.logits import process_logits
+    x = np.full((2, 20000), -np.inf, np.float32)
+    allow = np.zeros((2, 20000), bool)
+    allow[0, [13000, 400, 19999]] = True
+    allow[1, [7, 9]] = True
+    for in_place in (False, True):
+        t = torch.from_numpy(x).cuda()
+        out, token = run(t, hist=[[400], [9]], pen=[[1.1, 0.1, 0.1]] * 2, allow=allow, **({"out": t} if in_place else {}))
+        assert token.tolist() == [400, 7] and np.isneginf(out).all()
+
+
+def test_wrapper_refusals():
+    from aljabr_b200 import native
+    from aljabr_b200.logits import process_logits
+    x = torch.zeros(2, 64, device="cuda")
+    h, n, p = torch.zeros(2, 4, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.ones(2, 3, device="cuda")
+    for kw in (dict(history=h), dict(history=h, history_len=n), dict(history=h, history_len=n[:1], penalties=p),
+               dict(history=h.long(), history_len=n, penalties=p), dict(history=h, history_len=n, penalties=p.t()),
+               dict(bias_tokens=h), dict(allow=h[:, :1]), dict(allow=h.cpu()), dict(out=x.bfloat16()), dict(token=n.long())):
+        with pytest.raises(native.ProviderError):
+            process_logits(x, **kw)
+    with pytest.raises(native.ProviderError):
+        process_logits(x.cpu())
+    with pytest.raises(native.UnsupportedOperation):
+        process_logits(x.half())
+
+
 def test_strided_rows_and_long_histories():
     rng = np.random.default_rng(4)
     wide = torch.from_numpy(rng.normal(size=(4, 9001)).astype(np.float32)).cuda()
