@@ -81,6 +81,7 @@ constexpr int kChunkTiles = kWarps;
 constexpr int kStages = 4;
 constexpr int kAhead = 2;        // chunks asked for before their turn
 constexpr int kItemCost = 2;     // chunks that an item's start and end are worth
+constexpr int kWholeItem = 4;    // chunks of an item that is not cut
 constexpr int kBulkPage = 64;    // least page size that is loaded by bulk copies
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 2.0f;    // a row's maximum is raised only when a score exceeds it by 2 (log2)
@@ -384,8 +385,10 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     const Tables tab = {s_pre, s_len};
     // A chunk costs a CTA about as much as 25 parts cost the one that joins them, so where the line is short an item
     // of n places is cut into stretches of sqrt(n / 25): one kv head of 32768 positions 23 us with 256 CTAs of a
-    // chunk each, 16 so.
-    const int stretch = max(1, __float2int_rn(sqrtf(static_cast<float>(total) / (25.0f * p.batch))));
+    // chunk each, 16 so.  The join itself costs as much as three chunks, so items of up to kWholeItem chunks are left
+    // whole: 257 positions 9.1 us in three parts, 7.2 whole.
+    const int width = (total + p.batch - 1) / p.batch;
+    const int stretch = width <= kItemCost + kWholeItem ? width : max(1, __float2int_rn(sqrtf(width / 25.0f)));
     total *= items;
     const int ctas = min(static_cast<int>(gridDim.x), (total + stretch - 1) / stretch);
     if (static_cast<int>(blockIdx.x) >= ctas) return;
