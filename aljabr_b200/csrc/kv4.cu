@@ -10,9 +10,10 @@
 // shuffles and nothing is staged.  Each byte is touched once, and HBM is the
 // bound as long as a thread's ~64 bytes cost it few hundred instructions:
 // head_dim is a template parameter (rows by shifts), a code is four
-// operations (kv4_rounded).  Measured: 16384 rows of 8 x 128, fp32 in and
-// back, 51 us (5.6 TB/s, 87 % of the measured copy rate); 49152 rows read back
-// as fp32 77 us (6.0 TB/s, 92 %).
+// operations (kv4_rounded), and 40 registers let 48 warps an SM wait for
+// their loads (50 registers: 48 us).  Measured: 16384 rows of 8 x 128, fp32 in
+// and back, 46.4 us (6.2 TB/s, 96 % of the measured copy rate); 49152 rows read
+// back as fp32 72.5 us (6.3 TB/s, 98 %).
 #include "kv4.cuh"
 
 #include <algorithm>
@@ -20,7 +21,7 @@
 namespace alj {
 namespace {
 
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 128;   // 256 threads: 51 us in, 76 us out at the sizes above; 64: 46 and 102
 
 // 8 consecutive elements.  `vec`: 2 for 32-byte aligned rows (one 32-byte
 // access a lane, whole sectors: two 16-byte stores each cover half of every
@@ -161,7 +162,7 @@ __device__ __forceinline__ Group group_of(const float (&x)[8]) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Rows p) {
+__global__ void __launch_bounds__(kRowThreads, 12) kv4_append_kernel(const Kv4Rows p) {
     pdl_launch_dependents();
     pdl_wait();
     constexpr int NG = D / 32;
