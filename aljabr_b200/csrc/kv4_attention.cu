@@ -54,17 +54,18 @@
 // bulk copy (K codes, V codes, K scales or V scales of the tiles that share a
 // page).  A ninth warp for it would cut every warp from 128 to 96 registers,
 // and address arithmetic in every warp for itself was half of all
-// instructions.  Pages of fewer than 64 positions would take up to 32 such
-// copies a chunk, which one warp issues one after the other (~100 cycles
-// each): there every warp copies its own tile in 16-byte pieces instead.
+// instructions.
+// For pages of 16 that is 32 copies a chunk, issued one after the other, and
+// still faster than 16-byte pieces copied by every warp for itself (8 sequences
+// of 8192: 33 us against 36; pages of 32: 30 against 35).
 //
 // Measured (1965 MHz, measured copy rate 6473 GB/s): two sequences of 131072,
-// 64 query heads on 8 kv heads, D 128, bf16: 80 us, 3.8 TB/s; 32 ragged
-// sequences up to 16384: 56 us, 3.2 TB/s; 4096 positions of one sequence, fp32:
-// 11.3 us.  The long ones are bound by issue: 374 instructions a tile (2304
+// 64 query heads on 8 kv heads, D 128, bf16: 79 us, 3.8 TB/s; 32 ragged
+// sequences up to 16384: 54.5 us, 3.3 TB/s; 4096 positions of one sequence, fp32:
+// 11.4 us.  The long ones are bound by issue: 374 instructions a tile (2304
 // bytes) at 2.45 a clock and SM, ALU pipe 55 % busy, DRAM 44 %; the short ones
 // by the chain launch - lengths - page - tile - merge - join.  Tried and
-// slower: scores of the next tile beside the values of this one (84 us), tiles
+// slower, against 80 us: scores of the next tile beside the values of this one (84 us), tiles
 // asked for 3 chunks ahead (88 us), one loop with the item's start inside
 // (116 us: the registers no longer hold).
 #include "kv4.cuh"
@@ -82,7 +83,6 @@ constexpr int kStages = 4;
 constexpr int kAhead = 2;        // chunks asked for before their turn
 constexpr int kItemCost = 2;     // chunks that an item's start and end are worth
 constexpr int kWholeItem = 4;    // chunks of an item that is not cut
-constexpr int kBulkPage = 64;    // least page size that is loaded by bulk copies
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 2.0f;    // a row's maximum is raised only when a score exceeds it by 2 (log2)
 constexpr float kNone = -1e30f;  // running maximum of a row that has seen nothing
@@ -270,42 +270,6 @@ __device__ __forceinline__ void load_chunk(const Kv4Attn& p, const TileSource& t
     }
 }
 
-// This warp's own tile in 16-byte pieces; the full barrier counts every lane's
-// arrival, which follows its copies.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-template <int NG>
-__device__ __forceinline__ void load_own(const Kv4Attn& p, const TileSource& t, int kvh, int len, uint32_t stage,
-                                         uint64_t* bar, int warp, int lane) {
-    using F = Cfg<NG, 1, 1>;
-    if (t.pos < len) {
-        const bool ok = t.page >= 0 && t.page < p.pages;
-        if (!ok) record_fault(ALJ_FAULT_BOUNDS);       // reads as zeros
-        const int n = ok ? 16 : 0;
-        const uint8_t* src = p.cache;
-        const unsigned long long plane = 16ull * NG * p.page_size;
-        unsigned long long k = 16u * lane, sc = 0;
-        if (ok) {
-            src += (static_cast<long long>(t.page) * p.kv_heads + kvh) * kv4_block_bytes(p.page_size, F::D);
-            k += 16ull * NG * t.off;
-            // lanes 0 .. 2 NG - 1 the K scales, the next 2 NG the V scales
-            sc = 2 * plane + 2ull * NG * t.off + 16u * lane + (lane >= 2 * NG ? 2ull * NG * p.page_size - F::SCALES : 0ull);
-        }
-        const uint32_t dst = stage + warp * F::CODES + 16 * lane;
-#pragma unroll
-        for (int i = 0; i < NG / 2; ++i) {
-            cp_async16(dst + 512 * i, src + (ok ? k + 512 * i : 0), n);
-            cp_async16(dst + kWarps * F::CODES + 512 * i, src + (ok ? plane + k + 512 * i : 0), n);
-        }
-        if (lane < 4 * NG) {
-            const uint32_t at = lane < 2 * NG ? 16 * lane : kWarps * F::SCALES + 16 * (lane - 2 * NG);
-            cp_async16(stage + 2 * kWarps * F::CODES + warp * F::SCALES + at, src + sc, n);
-        }
-    }
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 template <int NG, int CT, int PARTS>
 __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kernel(const Kv4Attn p) {
     using F = Cfg<NG, CT, PARTS>;
@@ -331,12 +295,11 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     const int R = p.q_len * p.group;               // rows that share a kv head
     const int items = p.kv_heads * p.row_tiles;    // items of a sequence
     pdl_launch_dependents();
-    const bool bulk = p.page_size >= kBulkPage;
     uint64_t* const full = s_bar;
     uint64_t* const empty = s_bar + kStages;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(full + i, bulk ? 1 : kThreads);
+            mbar_init(full + i, 1);
             mbar_init(empty + i, kWarps);
         }
         fence_mbar_init();
@@ -434,19 +397,15 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     // chunk number i of this CTA, at cursor c, into its slot
     auto ask = [&](int i, const Cursor& c) {
         const int slot = i % kStages, head = p.row_tiles == 1 ? c.h : c.h / p.row_tiles;
-        const TileSource t = find_tile(p, c, bulk ? lane >> 2 : warp);   // the page id is on its way while the slot empties
-        if (!bulk) {                               // the slot's last tile of this warp has been read by it
-            load_own<NG>(p, t, head, c.len, smem_u32(ring) + slot * F::STAGE, full + slot, warp, lane);
-        } else {
-            if (i >= kStages && !dead) dead = !mbar_wait(empty + slot, (i / kStages - 1) & 1);
-            if (!dead) load_chunk<NG>(p, t, head, c.len, ring + slot * F::STAGE, full + slot, lane);
-        }
+        const TileSource t = find_tile(p, c, lane >> 2);   // the page id is on its way while the slot empties
+        if (i >= kStages && !dead) dead = !mbar_wait(empty + slot, (i / kStages - 1) & 1);
+        if (!dead) load_chunk<NG>(p, t, head, c.len, ring + slot * F::STAGE, full + slot, lane);
     };
-    if (!bulk || warp < kAhead) {
+    if (warp < kAhead) {
         Cursor c = at;
 #pragma unroll 1
         for (int i = 0; i < min(kAhead, todo); ++i) {
-            if (!bulk || i == warp) ask(i, c);
+            if (i == warp) ask(i, c);
             step(c, p, tab, items);
         }
     }
@@ -806,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
         const int pos0 = (at.first + at.ch * kChunkTiles + warp) * kTilePos;
 #pragma unroll 1
         for (int i = 0; i < count; ++i, ++done) {
-            if ((!bulk || ((done + kAhead) & (kWarps - 1)) == warp) && done + kAhead < todo) {
+            if (((done + kAhead) & (kWarps - 1)) == warp && done + kAhead < todo) {
                 Cursor c = at;
                 c.ch += i;
                 for (int k = 0; k < kAhead; ++k) step(c, p, tab, items);
@@ -1000,7 +959,9 @@ cudaError_t launch_cfg(Kv4Attn p, int sms, int max_ctas, cudaStream_t stream) {
 }
 
 // Rows a CTA serves at once: a column tile holds 8 bf16 or 4 fp32 rows; two
-// tiles where the rows need them and the accumulators fit (D <= 128).
+// tiles where the rows need them and the accumulators fit (D <= 128): 8
+// sequences of 8192 with 16 bf16 rows 44 us in one pass of two tiles, 49 in two
+// of one; 8 fp32 rows 46 against 55.
 int tile_rows(int rows, int head_dim, bool wide) {
     const int one = wide ? 4 : 8;
     return rows > one && head_dim <= 128 ? 2 * one : one;
