@@ -141,19 +141,22 @@ class Kv4Cache:
 
     # -- attention -------------------------------------------------------------
     def _workspace(self, q_len: int, q_heads: int, stream: int):
-        """(address, bytes) of a workspace for this shape of query on this stream."""
-        need = self._work_size(q_len, q_heads, self.kv_heads, self.head_dim)
+        """(address, bytes) of this stream's workspace.
+
+        A captured graph keeps the address, so a buffer is made once, as large as any accepted call needs (a few MB),
+        and lives as long as the cache."""
+        need = self._work_size(q_len, q_heads, self.kv_heads, self.head_dim)   # the call's own, for its refusals
         if need < 0:
             native.check(int(need))
         have = self._buffers.get(stream)
-        if have is None or have.numel() < need:
-            # zeroed on torch's current stream; another stream's kernels neither wait for that nor hold the
-            # old buffer, so there the device is waited for, once
-            have = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        if have is None:
+            most = self._work_size(native.KV4_MAX_ROWS, self.kv_heads, self.kv_heads, self.head_dim)
+            # zeroed on torch's current stream; another stream's kernels do not wait for that, so there the device is
+            # waited for, once
+            have = torch.zeros(most, dtype=torch.uint8, device=self.device)
             if stream != current_stream(self._index):
                 torch.cuda.synchronize(self.device)
             self._buffers[stream] = have
-            self._work = {k: v for k, v in self._work.items() if k[0] != stream}
         got = self._work[stream, q_len, q_heads] = (have.data_ptr(), have.numel())
         return got
 

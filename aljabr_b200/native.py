@@ -33,6 +33,7 @@ TYPE_Q6_K = 14
 KV_F32 = 0
 KV_BF16 = 1
 KV_Q4 = 2
+KV4_MAX_ROWS = 1024      # q_len * q_heads / kv_heads of one kv4_attention call
 
 
 class ProviderError(RuntimeError):
