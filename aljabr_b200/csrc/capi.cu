@@ -1478,6 +1478,19 @@ int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, lo
     return launch_status(launch_kv4_attention(a, workspace, st->sms, pick_stream(st, stream)), "kv4_attention");
 }
 
+int aljabr_blackwell_stream_capture_id(void* stream, unsigned long long* id) {
+    if (!id) return fail(ALJ_ERR_BAD_ARG, "stream_capture_id: null id");
+    *id = 0;
+    int err = 0;
+    DeviceState* st = state(&err);
+    if (!st) return err;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long got = 0;
+    const int rc = launch_status(cudaStreamGetCaptureInfo(pick_stream(st, stream), &status, &got), "stream_capture_id");
+    if (rc == ALJ_OK && status == cudaStreamCaptureStatusActive) *id = got;
+    return rc;
+}
+
 int aljabr_blackwell_logits_process_dev(float* out, long long out_stride, const void* logits, int logits_dtype,
                                         long long logits_stride, int rows, int vocab, const int* history,
                                         const int* history_len, int history_stride, const float* penalties,

@@ -9,10 +9,13 @@ one page of max_ctx positions each (no table).  The serving loop of one layer:
     out = cache.attend(q, seq_lens, block_table)   # q: [batch, q_len, q_heads, head_dim]
 
 Tensors are torch CUDA tensors on the cache's device; every call is ordered on
-torch's current stream of that device (or `stream`, a raw cudaStream_t).  The
-layout and the arithmetic are described in include/aljabr_blackwell.h.
+torch's current stream of that device (or `stream`, a raw cudaStream_t), and
+may be captured with torch.cuda.graph.  The layout and the arithmetic are
+described in include/aljabr_blackwell.h.
 """
 from __future__ import annotations
+
+import ctypes
 
 import torch
 
@@ -38,6 +41,18 @@ def select_device(index: int) -> None:
     """The library launches on the calling thread's device; where there are several, each call names its own."""
     if _several:
         native.call("aljabr_blackwell_init", index)
+
+
+def capture_id(index: int, stream: int) -> int:
+    """Id of the graph capture that `stream` of device `index` takes part in; 0 where it is in none."""
+    if stream == current_stream(index) and not torch.cuda.is_current_stream_capturing():
+        return 0
+    got = ctypes.c_ulonglong(0)
+    native.call("aljabr_blackwell_stream_capture_id", stream, ctypes.byref(got))
+    return got.value
+
+
+_captured = {}      # (device, stream) -> capture id, its workspaces
 
 
 def dtype_id(t: torch.Tensor, what: str) -> int:
@@ -141,24 +156,38 @@ class Kv4Cache:
 
     # -- attention -------------------------------------------------------------
     def _workspace(self, q_len: int, q_heads: int, stream: int):
-        """(address, bytes) of this stream's workspace.
-
-        A captured graph keeps the address, so a buffer is made once, as large as any accepted call needs (a few MB),
-        and lives as long as the cache."""
-        need = self._work_size(q_len, q_heads, self.kv_heads, self.head_dim)   # the call's own, for its refusals
-        if need < 0:
-            native.check(int(need))
+        """(address, bytes) of this stream's workspace: made once, as large as any accepted call needs (a few MB), and
+        kept as long as the cache, since kernels under way may hold its address."""
         have = self._buffers.get(stream)
         if have is None:
-            most = self._work_size(native.KV4_MAX_ROWS, self.kv_heads, self.kv_heads, self.head_dim)
+            have = self._make_workspace(q_len, q_heads)
             # zeroed on torch's current stream; another stream's kernels do not wait for that, so there the device is
             # waited for, once
-            have = torch.zeros(most, dtype=torch.uint8, device=self.device)
             if stream != current_stream(self._index):
                 torch.cuda.synchronize(self.device)
             self._buffers[stream] = have
         got = self._work[stream, q_len, q_heads] = (have.data_ptr(), have.numel())
         return got
+
+    def _make_workspace(self, q_len: int, q_heads: int) -> torch.Tensor:
+        need = self._work_size(q_len, q_heads, self.kv_heads, self.head_dim)   # the call's own, for its refusals
+        if need < 0:
+            native.check(int(need))
+        most = self._work_size(native.KV4_MAX_ROWS, self.kv_heads, self.kv_heads, self.head_dim)
+        return torch.zeros(most, dtype=torch.uint8, device=self.device)
+
+    def _captured_workspace(self, capture: int, q_len: int, q_heads: int, stream: int):
+        """(address, bytes) for calls recorded into a graph.  Its zeroing is a node of that graph, which may run on any
+        stream: so it belongs to this capture's calls on this stream (of all caches: they follow one another) and to
+        nothing else.  torch's graph keeps the memory; here it is held until the stream's next capture."""
+        key = self._index, stream
+        owner, have = _captured.get(key, (0, []))
+        if owner != capture:
+            _captured[key] = capture, (have := [])
+        need = self._work_size(q_len, q_heads, self.kv_heads, self.head_dim)
+        if not have or have[-1].numel() < need:
+            have.append(self._make_workspace(q_len, q_heads))
+        return have[-1].data_ptr(), have[-1].numel()
 
     def attend(self, q: torch.Tensor, seq_lens: torch.Tensor, block_table=None, window: int = 0, scale=None,
                soft_cap: float = 0.0, out=None, stream=None) -> torch.Tensor:
@@ -188,8 +217,12 @@ class Kv4Cache:
                 raise bad(f"block_table must be contiguous int32 [{batch}, pages a sequence] on {self.device}")
             table = block_table.data_ptr()
         stream = stream or current_stream(self._index)
-        have = self._work.get((stream, q_len, q_heads))
-        work, size = have if have is not None else self._workspace(q_len, q_heads, stream)
+        capture = capture_id(self._index, stream)
+        if capture:
+            work, size = self._captured_workspace(capture, q_len, q_heads, stream)
+        else:
+            have = self._work.get((stream, q_len, q_heads))
+            work, size = have if have is not None else self._workspace(q_len, q_heads, stream)
         rc = self._attend(out.data_ptr(), q.data_ptr(), kind, q_stride, *self._shape, table, width,
                           self._ints(seq_lens, batch, "seq_lens"), batch, q_len, q_heads, window,
                           D ** -0.5 if scale is None else scale, soft_cap, work, size, stream)

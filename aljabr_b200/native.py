@@ -111,6 +111,7 @@ SIGNATURES = {
     "aljabr_blackwell_kv4_attention_workspace_size": (_ll, [_i, _i, _i, _i]),
     "aljabr_blackwell_kv4_attention_dev": (_i, [_p, _p, _i, _ll, _p, _i, _i, _i, _i, _p, _i, _p, _i, _i, _i, _i, _f, _f,
                                                 _p, _ll, _p]),
+    "aljabr_blackwell_stream_capture_id": (_i, [_p, _p]),
     "aljabr_blackwell_logits_process_dev": (_i, [_p, _ll, _p, _i, _ll, _i, _i, _p, _p, _i, _p, _p, _p, _p, _i, _p, _i,
                                                  _p, _p]),
     "aljabr_blackwell_nccl_unique_id": (_i, [_p, _i]),

@@ -381,6 +381,10 @@ int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, lo
                                        int table_stride, const int* seq_lens, int batch, int q_len, int q_heads,
                                        int window, float scale, float soft_cap, void* workspace,
                                        long long workspace_bytes, void* stream);
+/* *id: the graph capture that `stream` takes part in, 0 if none.  A workspace
+ * that is zeroed inside a capture is zero only in that graph's replays, so a
+ * host keeps those apart by this id. */
+int aljabr_blackwell_stream_capture_id(void* stream, unsigned long long* id);
 
 /* ---- logits step -----------------------------------------------------------
  * For each of `rows` rows of `vocab` logits (ALJ_KV_F32 or ALJ_KV_BF16, rows

@@ -36,3 +36,47 @@ def test_a_graph_survives_a_later_call_with_more_rows():
         torch.cuda.synchronize()
         assert torch.equal(out, want)
     assert all(bool((t == 0x5A).all()) for t in others)
+
+
+def test_graphs_of_a_stream_that_was_not_warmed_up():
+    """Two batch sizes captured on one stream with nothing run on it before, replayed in reverse, with plain calls on the
+    stream between and both at once on two streams."""
+    cache, q, sl, table, want, _, _ = attend_case(31, 128, 2, 4, 1, 16, [4000, 100, 9000, 2500])
+    side = torch.cuda.Stream()
+    graphs = []
+    for n in (4, 2):
+        out = torch.zeros_like(q[:n])
+        graphs.append((capture(side, lambda: cache.attend(q[:n], sl[:n], table[:n], out=out)), out, n))
+    few = cache.attend(q[:2], sl[:2], table[:2])
+    for graph, out, n in reversed(graphs):
+        graph.replay()
+        with torch.cuda.stream(side):
+            plain = cache.attend(q, sl, table)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want if n == 4 else few) and torch.equal(plain, want)
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for _, out, _ in graphs:
+        out.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for stream, (graph, _, _) in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(graphs[0][1], want) and torch.equal(graphs[1][1], few)
+
+
+def test_one_graph_of_several_caches_and_row_counts():
+    a, q, sl, table, want, _, _ = attend_case(32, 128, 2, 4, 1, 16, [3000, 5000])
+    b, qb, slb, tb, want_b, _, _ = attend_case(33, 64, 1, 2, 7, 32, [700, 6000])
+    outs = torch.zeros_like(q), torch.zeros_like(qb)
+
+    def both():
+        a.attend(q, sl, table, out=outs[0])
+        b.attend(qb, slb, tb, out=outs[1])
+
+    graph = capture(torch.cuda.Stream(), both)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want_b)

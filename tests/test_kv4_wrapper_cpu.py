@@ -22,6 +22,8 @@ def cache(monkeypatch):
     c._work_size = lambda q_len, q_heads, kv_heads, head_dim: 1024 if q_len * q_heads // kv_heads <= 8 else 2048
     c._append = c._read = c._attend = lambda *a: 0
     monkeypatch.setattr(kv4, "current_stream", lambda index: 7)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: None)
     return c
 
 
@@ -43,3 +45,33 @@ def test_no_accepted_call_needs_more_than_the_most_rows(D):
     most = size(native.KV4_MAX_ROWS, 2, 2, D)
     assert all(size(rows, 2, 2, D) <= most for rows in range(1, native.KV4_MAX_ROWS))
     assert size(native.KV4_MAX_ROWS + 1, 2, 2, D) == native.ALJ_ERR_UNSUPPORTED
+
+
+def attend(cache, stream=None, rows=1):
+    """The workspace address that a call of the wrapper hands to the library."""
+    got = []
+    cache._attend = lambda *a: got.append(a[-3]) or 0
+    cache.attend(torch.zeros(1, rows, 2, 64), torch.ones(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32), stream=stream)
+    return got[0]
+
+
+def test_each_capture_has_a_workspace_of_its_own(cache, monkeypatch):
+    """Two graphs captured one after the other on one stream, and calls before, between and after them: a buffer whose
+    zeroing is a node of one graph must serve nothing else, and no graph the buffer of plain calls."""
+    capture = 0
+    monkeypatch.setattr(kv4, "capture_id", lambda index, stream: capture, raising=False)
+    capture = 11
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capture != 0)
+    first = attend(cache)
+    assert attend(cache) == first                       # calls of one stream in one graph follow one another
+    other_branch = attend(cache, stream=8)
+    capture = 0
+    plain = attend(cache)
+    kept = dict(cache._buffers)
+    capture = 12
+    second = attend(cache)
+    assert attend(cache) == second and second != plain
+    capture = 0
+    assert attend(cache) == plain and cache._buffers == kept
+    assert plain not in (first, other_branch) and first != other_branch
+    assert len(cache._buffers) == 1
