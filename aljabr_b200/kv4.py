@@ -9,9 +9,10 @@ one page of max_ctx positions each (no table).  The serving loop of one layer:
     out = cache.attend(q, seq_lens, block_table)   # q: [batch, q_len, q_heads, head_dim]
 
 Tensors are torch CUDA tensors on the cache's device; every call is ordered on
-torch's current stream of that device (or `stream`, a raw cudaStream_t), and
-may be captured with torch.cuda.graph.  The layout and the arithmetic are
-described in include/aljabr_blackwell.h.
+torch's current stream of that device (or `stream`, a raw cudaStream_t: what
+the call is given must be ready there and live until it has run), and may be
+captured with torch.cuda.graph.  The layout and the arithmetic are described
+in include/aljabr_blackwell.h.
 """
 from __future__ import annotations
 
@@ -43,13 +44,23 @@ def select_device(index: int) -> None:
         native.call("aljabr_blackwell_init", index)
 
 
-def capture_id(index: int, stream: int) -> int:
-    """Id of the graph capture that `stream` of device `index` takes part in; 0 where it is in none."""
-    if stream == current_stream(index) and not torch.cuda.is_current_stream_capturing():
-        return 0
+def capture_id(stream: int) -> int:
+    """Id of the graph capture that `stream` takes part in; 0 where it is in none."""
     got = ctypes.c_ulonglong(0)
     native.call("aljabr_blackwell_stream_capture_id", stream, ctypes.byref(got))
     return got.value
+
+
+def new_output(shape, dtype, device, index: int, stream: int) -> torch.Tensor:
+    """A tensor that a call on `stream` writes and that the caller reads on torch's current stream: of the allocator's
+    pool of the first, so that no work pending on the second still uses its memory, and not given out again before
+    the second is done with it."""
+    if stream == current_stream(index):
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device)):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    t.record_stream(torch.cuda.current_stream(device))
+    return t
 
 
 _captured = {}      # (device, stream) -> capture id, its workspaces
@@ -144,12 +155,12 @@ class Kv4Cache:
         if _several:
             select_device(self._index)
         n = slots.numel()
+        stream = stream or current_stream(self._index)
         if k_out is None and v_out is None:
-            k_out, v_out = (torch.empty(n, self.kv_heads, self.head_dim, dtype=dtype, device=self.device) for _ in range(2))
+            k_out, v_out = (new_output((n, self.kv_heads, self.head_dim), dtype, self.device, self._index, stream) for _ in range(2))
         some = k_out if k_out is not None else v_out
         rc = self._read(self._dense(k_out, n, some.dtype, "k_out"), self._dense(v_out, n, some.dtype, "v_out"),
-                        dtype_id(some, "k_out"), *self._shape, self._ints(slots, n, "slots"), n,
-                        stream or current_stream(self._index))
+                        dtype_id(some, "k_out"), *self._shape, self._ints(slots, n, "slots"), n, stream)
         if rc:
             native.check(rc)
         return k_out, v_out
@@ -205,8 +216,10 @@ class Kv4Cache:
         if st[3] != 1 or (q_heads > 1 and st[2] != D) or (q_len > 1 and batch > 1 and st[0] != q_len * st[1]):
             raise bad(f"q: the heads of a token must be contiguous and the tokens evenly spaced (strides {st})")
         kind = dtype_id(q, "q")
+        current = current_stream(self._index)
+        stream = stream or current
         if out is None:
-            out = torch.empty(batch, q_len, q_heads, D, dtype=q.dtype, device=self.device)
+            out = new_output((batch, q_len, q_heads, D), q.dtype, self.device, self._index, stream)
         elif out.shape != shape or out.dtype is not q.dtype or out.get_device() != self._index or not out.is_contiguous():
             raise bad(f"out must be contiguous {q.dtype} {tuple(shape)} on {self.device}")
         table, width = None, 0
@@ -216,8 +229,9 @@ class Kv4Cache:
                     block_table.get_device() != self._index or not block_table.is_contiguous():
                 raise bad(f"block_table must be contiguous int32 [{batch}, pages a sequence] on {self.device}")
             table = block_table.data_ptr()
-        stream = stream or current_stream(self._index)
-        capture = capture_id(self._index, stream)
+        capture = 0      # the legacy stream is never captured: no question asked there (0.8 us)
+        if stream != _LEGACY_STREAM and (stream != current or torch.cuda.is_current_stream_capturing()):
+            capture = capture_id(stream)
         if capture:
             work, size = self._captured_workspace(capture, q_len, q_heads, stream)
         else:

@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from . import native
-from .kv4 import _several, bad, current_stream, dtype_id, select_device
+from .kv4 import _several, bad, current_stream, dtype_id, new_output, select_device
 
 
 _process = native.lib().aljabr_blackwell_logits_process_dev
@@ -33,13 +33,13 @@ def process_logits(logits: torch.Tensor, history=None, history_len=None, penalti
     rows, vocab = shape
     if _several:
         select_device(dev)
-
+    stream = stream or current_stream(dev)
     if out is None:
-        out = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
+        out = new_output((rows, vocab), torch.float32, logits.device, dev, stream)
     elif out.dtype is not torch.float32 or out.shape != shape or out.stride(1) != 1 or out.get_device() != dev:
         raise bad(f"out must be float32 [{rows}, {vocab}] on {logits.device} with contiguous rows")
     if token is None:
-        token = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        token = new_output((rows,), torch.int32, logits.device, dev, stream)
     h = hl = pen = bt = bv = bl = al = None
     nh = nb = na = 0
     if history is not None:
@@ -59,7 +59,7 @@ def process_logits(logits: torch.Tensor, history=None, history_len=None, penalti
         al = _ptr(allow, _I32, rows * na, dev, "allow")
     rc = _process(out.data_ptr(), out.stride(0) if rows > 1 else vocab, logits.data_ptr(), dtype_id(logits, "logits"),
                   st[0] if rows > 1 else vocab, rows, vocab, h, hl, nh, pen, bt, bv, bl, nb, al, na,
-                  _ptr(token, _I32, rows, dev, "token"), stream or current_stream(dev))
+                  _ptr(token, _I32, rows, dev, "token"), stream)
     if rc:
         native.check(rc)
     return out, token

@@ -80,3 +80,27 @@ def test_one_graph_of_several_caches_and_row_counts():
         graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want) and torch.equal(outs[1], want_b)
+
+
+def test_calls_on_a_stream_of_their_own():
+    """`stream=`: the results, and outputs that do not take memory from work still pending on the current stream."""
+    from aljabr_b200.logits import process_logits
+    cache, q, sl, table, want, _, _ = attend_case(34, 128, 2, 4, 1, 16, [4000, 100])
+    slots = torch.arange(64, dtype=torch.int32, device="cuda")
+    rows = cache.read(slots)
+    logits = torch.randn(3, 5000, device="cuda")
+    plain = process_logits(logits)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(20):
+        # a block of the output's size, freed while the current stream has yet to read it
+        block = torch.zeros(want.numel(), device="cuda")
+        torch.cuda._sleep(2_000_000)
+        copy = block.clone()
+        del block
+        out = cache.attend(q, sl, table, stream=side.cuda_stream)
+        k, v = cache.read(slots, stream=side.cuda_stream)
+        got, token = process_logits(logits, stream=side.cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(k, rows[0]) and torch.equal(v, rows[1])
+        assert torch.equal(got, plain[0]) and torch.equal(token, plain[1]) and not copy.any()

@@ -51,7 +51,8 @@ def attend(cache, stream=None, rows=1):
     """The workspace address that a call of the wrapper hands to the library."""
     got = []
     cache._attend = lambda *a: got.append(a[-3]) or 0
-    cache.attend(torch.zeros(1, rows, 2, 64), torch.ones(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32), stream=stream)
+    q = torch.zeros(1, rows, 2, 64)
+    cache.attend(q, torch.ones(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32), out=q, stream=stream)
     return got[0]
 
 
@@ -59,7 +60,7 @@ def test_each_capture_has_a_workspace_of_its_own(cache, monkeypatch):
     """Two graphs captured one after the other on one stream, and calls before, between and after them: a buffer whose
     zeroing is a node of one graph must serve nothing else, and no graph the buffer of plain calls."""
     capture = 0
-    monkeypatch.setattr(kv4, "capture_id", lambda index, stream: capture, raising=False)
+    monkeypatch.setattr(kv4, "capture_id", lambda stream: capture, raising=False)
     capture = 11
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capture != 0)
     first = attend(cache)
@@ -75,3 +76,45 @@ def test_each_capture_has_a_workspace_of_its_own(cache, monkeypatch):
     assert attend(cache) == plain and cache._buffers == kept
     assert plain not in (first, other_branch) and first != other_branch
     assert len(cache._buffers) == 1
+
+
+def test_outputs_belong_to_the_stream_that_writes_them(cache, monkeypatch):
+    """With `stream` given, an output from the allocator's pool of torch's current stream could be a block whose last
+    reader there has not run yet; and its own readers there must keep it from being handed out again."""
+    from contextlib import contextmanager
+    at, made, readers = [7], [], []
+    real = torch.empty
+
+    @contextmanager
+    def switch(s):
+        at.append(s)
+        yield
+        at.pop()
+
+    def empty(*a, **kw):
+        made.append(at[-1])
+        return real(*a, **kw)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda s, device=None: s)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: at[-1])
+    monkeypatch.setattr(torch.cuda, "stream", switch)
+    monkeypatch.setattr(torch, "empty", empty)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: readers.append(s))
+    monkeypatch.setattr(kv4, "capture_id", lambda stream: 0)
+    q, lens, slots = torch.zeros(1, 1, 2, 64), torch.ones(1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    table = torch.zeros(1, 1, dtype=torch.int32)
+    cache.attend(q, lens, table)
+    cache.read(slots)
+    assert made == [7, 7, 7] and readers == []
+    made.clear()
+    cache.attend(q, lens, table, stream=9)
+    cache.read(slots, stream=9)
+    assert made == [9, 9, 9] and readers == [7, 7, 7]
+    from aljabr_b200 import logits
+    monkeypatch.setattr(logits, "_process", lambda *a: 0)
+    monkeypatch.setattr(logits, "current_stream", lambda index: 7)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    made.clear(), readers.clear()
+    logits.process_logits(torch.zeros(2, 33))
+    assert made == [7, 7] and readers == []
+    logits.process_logits(torch.zeros(2, 33), stream=9)
+    assert made == [7, 7, 9, 9] and readers == [7, 7]
