@@ -201,8 +201,13 @@ struct Tables {      // per sequence, in shared memory
     const int* len;  // [batch]
 };
 
+// First of the p.window positions before `end`: a window may be as long as an int holds, so it is only taken from what
+// is longer.
+__device__ __forceinline__ int window_start(const Kv4Attn& p, int end) {
+    return p.window > 0 && end > p.window ? end - p.window : 0;
+}
 __device__ __forceinline__ int first_tile(const Kv4Attn& p, int len) {
-    return p.window > 0 ? max(0, len - p.q_len - p.window + 1) / kTilePos : 0;
+    return window_start(p, len - p.q_len + 1) / kTilePos;
 }
 __device__ __forceinline__ int chunks_of(const Kv4Attn& p, int len) {
     const int tiles = (len + kTilePos - 1) / kTilePos - first_tile(p, len);
@@ -499,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             s_hi[threadIdx.x] = row < rows ? len - p.q_len + token_of(row0 + row) : -1;
         }
         all_hi = len - p.q_len + token_of(row0);
-        all_lo = p.window > 0 ? len - p.q_len + token_of(row0 + rows - 1) - p.window + 1 : 0;
+        all_lo = window_start(p, len - p.q_len + token_of(row0 + rows - 1) + 1);
         }
         __syncthreads();
 
@@ -634,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             for (int a = 0; a < CT; ++a) keep[a][0] = keep[a][1] = 0xFFFFFFFFu;
             if (pos < all_lo || pos + kTilePos - 1 > all_hi) {
                 const int word_pos = pos + (NG == 2 ? lane : lane >> 1);   // the position of the lane's scale words
-                if (word_pos >= len || (p.window > 0 && word_pos <= all_hi - p.window) || top >= 0x7C00u) top = 0u;
+                if (word_pos >= len || (p.window > 0 && all_hi - word_pos >= p.window) || top >= 0x7C00u) top = 0u;
 #pragma unroll
                 for (int a = 0; a < CT; ++a)
 #pragma unroll
@@ -644,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             const int hi = s_hi[8 * a + 2 * c4 + j];
-                            see[j] = at_pos <= hi && (p.window == 0 || at_pos > hi - p.window);
+                            see[j] = at_pos <= hi && (p.window == 0 || hi - at_pos < p.window);
                             y[a][h][j] = see[j] ? y[a][h][j] : -INFINITY;
                         }
                         keep[a][h] = transpose8((see[0] ? 0x0000FFFFu : 0u) | (see[1] ? 0xFFFF0000u : 0u));

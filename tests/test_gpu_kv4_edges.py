@@ -1,0 +1,33 @@
+"""Edges of the 4-bit cache's attention, against 64 bits: values, scores and
+queries of very unequal size, and arguments at the ends of their ranges."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests import kv4_ref as ref
+from tests.test_gpu_kv4 import attend_case, check, fault_bits, make
+
+pytestmark = pytest.mark.gpu
+
+
+def one_sequence(k, v, dtype=torch.float32):
+    """A cache of one sequence of the rows k, v [n][hkv][D], its table and length, and the values it holds."""
+    n, hkv, D = k.shape
+    pages = -(-n // 16)
+    cache = make(pages, 16, hkv, D, fill=0xFF)
+    cache.append(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), torch.arange(n, dtype=torch.int32, device="cuda"))
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    return (cache, table, torch.tensor([n], dtype=torch.int32, device="cuda"), ref.values(*ref.quantise(k)),
+            ref.values(*ref.quantise(v)))
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 5, 5000])
+def test_a_window_longer_than_every_sequence_is_none(window):
+    """Sequences shorter than their new tokens, empty ones among them, with a window that 32 bits barely hold."""
+    for T in (1, 3, 7):
+        lens = [0, 1, 2, 300, 4000]
+        cache, q, sl, table, out, k64, v64 = attend_case(23, 128, 2, 2, T, 16, lens)
+        assert torch.equal(cache.attend(q, sl, table, window=window), out)
+        check(out, q, k64, v64, lens)
+    assert fault_bits() == 0
