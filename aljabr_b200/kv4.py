@@ -229,6 +229,8 @@ class Kv4Cache:
                     block_table.get_device() != self._index or not block_table.is_contiguous():
                 raise bad(f"block_table must be contiguous int32 [{batch}, pages a sequence] on {self.device}")
             table = block_table.data_ptr()
+        if window:       # ctypes would take its low 32 bits
+            window = max(-1, min(window, 0x7FFFFFFF))
         capture = 0      # the legacy stream is never captured: no question asked there (0.8 us)
         if stream != _LEGACY_STREAM and (stream != current or torch.cuda.is_current_stream_capturing()):
             capture = capture_id(stream)

@@ -118,3 +118,19 @@ def test_outputs_belong_to_the_stream_that_writes_them(cache, monkeypatch):
     assert made == [7, 7] and readers == []
     logits.process_logits(torch.zeros(2, 33), stream=9)
     assert made == [7, 7, 9, 9] and readers == [7, 7]
+
+
+@pytest.mark.parametrize("window,passed", [(0, 0), (7, 7), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31, 2 ** 31 - 1),
+                                           (2 ** 32 + 5, 2 ** 31 - 1), (2 ** 63 - 1, 2 ** 31 - 1), (-1, -1), (-2 ** 32, None)])
+def test_a_window_that_an_int_does_not_hold(cache, monkeypatch, window, passed):
+    """ctypes would cut it to its low 32 bits: 2^32 + 5 to a window of 5.  Longer than any sequence is no window."""
+    from aljabr_b200 import native
+    got = []
+    cache._attend = lambda *a: got.append(a[-6]) or 0
+    q = torch.zeros(1, 1, 2, 64)
+    args = q, torch.ones(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32)
+    monkeypatch.setattr(kv4, "capture_id", lambda stream: 0)
+    import ctypes
+    cache.attend(*args, window=window, out=q)
+    sent = ctypes.c_int(got[0]).value
+    assert sent == passed if passed is not None else sent < 0
