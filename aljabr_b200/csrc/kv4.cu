@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kRowThreads, 12) kv4_append_kernel(const Kv4Ro
         *reinterpret_cast<uint32_t*>(vc + 2 * ((2 * c + (g & 1)) * NG + (g & ~1))) = vpair;
         __half* sc = reinterpret_cast<__half*>(blk + p.page_size * static_cast<long long>(D));
         if (c == 0) sc[w.off * static_cast<long long>(NG) + g] = gk.d;
-        if (c == 1) sc[(p.page_size + w.off) * static_cast<long long>(NG) + g] = gv.d;
+        if (c == 1) sc[(static_cast<long long>(p.page_size) + w.off) * NG + g] = gv.d;
     }
     if (live && p.k_out) {                         // a skipped row's zeros stand for zeros
         const long long at = (static_cast<long long>(w.token) * p.kv_heads + w.head) * D + 8 * w.j;
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(const Kv4Rows p) 
         const uint32_t v0 = __ldg(reinterpret_cast<const uint16_t*>(vc + 2 * (2 * c * NG + g)));
         const uint32_t v1 = __ldg(reinterpret_cast<const uint16_t*>(vc + 2 * ((2 * c + 1) * NG + g)));
         const float dk = __half2float(__ldg(sc + w.off * static_cast<long long>(NG) + g));
-        const float dv = __half2float(__ldg(sc + (p.page_size + w.off) * static_cast<long long>(NG) + g));
+        const float dv = __half2float(__ldg(sc + (static_cast<long long>(p.page_size) + w.off) * NG + g));
         unpack8(kw, dk, k);
         unpack8(v0 | (v1 << 16), dv, v);
     }
@@ -269,7 +269,8 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rope_append_kernel(const Kv4R
         const uint32_t w = encode8(x[e], kv4_inverse(gr.d), __half2float(gr.d), gr.finite);
         if (!live || !in_cache || is_q) continue;
         uint8_t* blk = p.cache + head * kv4_block_bytes(p.page_size, D);
-        uint8_t* row = blk + ((is_v ? p.page_size : 0) + pos) * (D / 2LL);
+        const long long at = (is_v ? static_cast<long long>(p.page_size) : 0) + pos;   // row of the block
+        uint8_t* row = blk + at * (D / 2);
         if (is_v) {
             *reinterpret_cast<uint16_t*>(row + 2 * (2 * c * NG + g)) = static_cast<uint16_t>(w);
             *reinterpret_cast<uint16_t*>(row + 2 * ((2 * c + 1) * NG + g)) = static_cast<uint16_t>(w >> 16);
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rope_append_kernel(const Kv4R
             *reinterpret_cast<uint32_t*>(row + 4 * (c * NG + g)) = w;
         }
         if (c == 0)
-            reinterpret_cast<__half*>(blk + p.page_size * static_cast<long long>(D))[((is_v ? p.page_size : 0) + pos) * static_cast<long long>(NG) + g] = gr.d;
+            reinterpret_cast<__half*>(blk + p.page_size * static_cast<long long>(D))[at * NG + g] = gr.d;
     }
 }
 

@@ -314,9 +314,9 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     __syncthreads();
     pdl_wait();
 
-    // lengths (clamped to what the table can address) and the prefix of chunks and item costs
-    const int cap = p.table ? static_cast<int>(min(static_cast<long long>(p.table_stride) * p.page_size, 0x7fffff00LL))
-                            : p.page_size;
+    // lengths (clamped to what the table or page can address, less what the last chunk counts past the end) and the
+    // prefix of chunks and item costs
+    const int cap = static_cast<int>(min(p.table ? static_cast<long long>(p.table_stride) * p.page_size : p.page_size, 0x7fffff00LL));
     int total = 0;                                 // < 2^31: checked on the host for the longest sequences
     for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
         const int b = b0 + threadIdx.x;

@@ -31,3 +31,25 @@ def test_a_window_longer_than_every_sequence_is_none(window):
         assert torch.equal(cache.attend(q, sl, table, window=window), out)
         check(out, q, k64, v64, lens)
     assert fault_bits() == 0
+
+
+def test_a_page_of_more_than_2_to_the_30_positions():
+    """The scales of V lie page_size + position rows into their section: a sum beyond 31 bits.  77 GB."""
+    from aljabr_b200.kv4 import Kv4Cache
+    ps, D, n = 2 ** 30 + 16, 64, 20
+    if torch.cuda.mem_get_info()[0] < ps * 72 + 2 ** 30:
+        pytest.skip("needs 78 GB")
+    cache = Kv4Cache(1, ps, 1, D, data=torch.empty(ps * 72, dtype=torch.uint8, device="cuda"))
+    rng = np.random.default_rng(24)
+    k, v = (rng.normal(size=(n, 1, D)).astype(np.float32) for _ in range(2))
+    slots = torch.arange(ps - n, ps, dtype=torch.int32, device="cuda")
+    cache.append(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), slots)
+    k64, v64 = ref.values(*ref.quantise(k)), ref.values(*ref.quantise(v))
+    for got, want in zip(cache.read(slots), (k64, v64)):
+        assert np.array_equal(got.cpu().numpy(), want.astype(np.float32))
+    q = torch.from_numpy(rng.normal(size=(1, 1, 2, D)).astype(np.float32)).cuda()
+    out = cache.attend(q, torch.tensor([ps], dtype=torch.int32, device="cuda"), window=n)
+    check(out, q, [k64], [v64], [n])
+    del cache
+    torch.cuda.empty_cache()
+    assert fault_bits() == 0
