@@ -1,0 +1,53 @@
+"""What the decode wrapper takes and refuses before the library sees an
+address: the library's calls are stubs, no GPU."""
+import numpy as np
+import pytest
+
+from aljabr_b200 import decode, native
+
+
+def decoder(monkeypatch, kv_dtype):
+    """A one-layer model of 2 kv heads x 64, and the calls it makes."""
+    d = object.__new__(decode.LlamaNf4Decoder)
+    d.shape = decode.LlamaShape(1, 256, 4, 2, 64, 512, 1000, 32, kv_dtype=kv_dtype)
+    d.tp_world, d.tp_rank, d.handle = 1, 0, 1
+    calls = []
+    monkeypatch.setattr(native, "call", lambda name, *a: calls.append((name, a)))
+    return d, calls
+
+
+@pytest.mark.parametrize("kv_dtype,good,wrong", [
+    (native.KV_Q4, [np.float32], [np.uint16, np.float16, np.float64]),
+    (native.KV_F32, [np.float32], [np.uint16, np.float64]),
+    (native.KV_BF16, [np.uint16, np.int16], [np.float32, np.float16])])
+def test_cache_rows_of_another_type_are_refused(monkeypatch, kv_dtype, good, wrong):
+    """The library reads 4 (or 2) bytes an element from the address it is given."""
+    d, calls = decoder(monkeypatch, kv_dtype)
+    for t in good:
+        rows = np.zeros((7, 128), t)
+        d.sync_kv_cache(0, 7, rows, rows)
+        d.sync_kv_cache(0, 5, rows, rows)                     # the first rows of a longer buffer
+    d.sync_kv_cache(0, 7, 1 << 20, 1 << 20)                   # an address is the caller's own word
+    assert len(calls) == 2 * len(good) + 1
+    ok = np.zeros((7, 128), good[0])
+    for t in wrong:
+        bad = np.zeros((7, 128), t)
+        for k, v in ((bad, bad), (ok, bad), (bad, ok)):
+            with pytest.raises(native.ProviderError):
+                d.sync_kv_cache(0, 7, k, v)
+    with pytest.raises(native.ProviderError):
+        d.sync_kv_cache(0, 8, ok, ok)                         # fewer rows than it says
+    assert len(calls) == 2 * len(good) + 1
+
+
+def test_cache_rows_as_tensors(monkeypatch):
+    torch = pytest.importorskip("torch")
+    for kv_dtype, good, wrong in ((native.KV_Q4, torch.float32, torch.bfloat16), (native.KV_BF16, torch.bfloat16, torch.float32),
+                                  (native.KV_BF16, torch.int16, torch.half)):
+        d, calls = decoder(monkeypatch, kv_dtype)
+        rows = torch.zeros(3, 128, dtype=good)
+        d.sync_kv_cache(0, 3, rows, rows)
+        for bad in (rows.to(wrong), torch.zeros(128, 3, dtype=good).t(), rows[:2]):
+            with pytest.raises(native.ProviderError):
+                d.sync_kv_cache(0, 3, bad, bad)
+        assert len(calls) == 1 and calls[0][1][3].value == rows.data_ptr()
