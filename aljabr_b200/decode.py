@@ -119,14 +119,13 @@ class LlamaNf4Decoder:
     def sync_kv_cache(self, layer: int, seq_len: int, k, v):
         """Rows [seq_len][kv_heads/tp * head_dim] of K and V, or more, into a layer's cache: fp32 for kv_dtype KV_F32 and
         KV_Q4, bf16 (or its bits as 16-bit integers) for KV_BF16.  Arrays, tensors, or addresses, which are not checked."""
+        k, v = (a if isinstance(a, (int, np.integer)) or hasattr(a, "data_ptr") else np.ascontiguousarray(a) for a in (k, v))
         native.call("aljabr_blackwell_sync_kv_cache", ctypes.c_ulonglong(self.handle), layer, seq_len,
                     ctypes.c_void_p(self._cache_rows(k, seq_len, "k")), ctypes.c_void_p(self._cache_rows(v, seq_len, "v")))
 
     def _cache_rows(self, a, seq_len: int, what: str) -> int:
         if isinstance(a, (int, np.integer)):
             return int(a)
-        if not hasattr(a, "data_ptr"):
-            a = np.ascontiguousarray(a)
         types = ("bfloat16", "int16", "uint16") if self.shape.kv_dtype == native.KV_BF16 else ("float32",)
         need = seq_len * (self.shape.kv_heads // self.tp_world) * self.shape.head_dim
         tensor = hasattr(a, "data_ptr")

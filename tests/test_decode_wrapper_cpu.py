@@ -1,5 +1,7 @@
 """What the decode wrapper takes and refuses before the library sees an
 address: the library's calls are stubs, no GPU."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -51,3 +53,19 @@ def test_cache_rows_as_tensors(monkeypatch):
             with pytest.raises(native.ProviderError):
                 d.sync_kv_cache(0, 3, bad, bad)
         assert len(calls) == 1 and calls[0][1][3].value == rows.data_ptr()
+
+
+def test_strided_arrays_are_copied_and_outlive_the_call(monkeypatch):
+    d, _ = decoder(monkeypatch, native.KV_Q4)
+    k = np.arange(2 * 7 * 128, dtype=np.float32).reshape(7, 256)[:, 128:]
+    v = np.arange(2 * 7 * 128, dtype=np.float32).reshape(7, 2, 128)[:, 0] + 0.5
+    seen = []
+
+    def call(name, handle, layer, n, kp, vp):
+        other = [np.full(7 * 128, -1.0, np.float32) for _ in range(64)]     # what would take a freed copy's place
+        for p in (kp, vp):
+            seen.append(np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctypes.c_float)), (7, 128)).copy())
+        assert len(other) == 64
+    monkeypatch.setattr(native, "call", call)
+    d.sync_kv_cache(0, 7, k, v)
+    assert np.array_equal(seen[0], k) and np.array_equal(seen[1], v)
