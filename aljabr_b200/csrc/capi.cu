@@ -831,6 +831,21 @@ int aljabr_blackwell_device_get(int device_id) {
     return state(&err) ? ALJ_OK : err;
 }
 
+int aljabr_blackwell_device_swap(int device_id, int* previous) {
+    if (!previous || device_id < -1) return fail(ALJ_ERR_BAD_ARG, "device_swap: device %d, previous %p", device_id, static_cast<void*>(previous));
+    const int before = t_device;
+    if (device_id >= 0) {
+        const int rc = aljabr_blackwell_device_get(device_id);
+        if (rc) {
+            t_device = before;
+            return rc;
+        }
+    }
+    t_device = device_id;
+    *previous = before;
+    return ALJ_OK;
+}
+
 int aljabr_blackwell_device_name(char* buf, int buf_len, int device_id) {
     if (!buf || buf_len <= 0) return fail(ALJ_ERR_BAD_ARG, "null buffer");
     int count = 0;

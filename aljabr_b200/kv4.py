@@ -17,6 +17,7 @@ in include/aljabr_blackwell.h.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -35,13 +36,35 @@ def current_stream(index: int) -> int:
     return _raw_stream(index) or _LEGACY_STREAM
 
 
-_several = torch.cuda.device_count() > 1
+class selected:
+    """Device `index` selected in the library, which launches on the calling thread's device, and in CUDA; on leaving,
+    both choices are the caller's again."""
+
+    def __init__(self, index: int):
+        self.index, self.library = index, ctypes.c_int(-1)
+
+    def __enter__(self):
+        self.cuda = torch.cuda.current_device()
+        native.call("aljabr_blackwell_device_swap", self.index, ctypes.byref(self.library))
+
+    def __exit__(self, *exc):
+        native.call("aljabr_blackwell_device_swap", self.library.value, ctypes.byref(ctypes.c_int(-1)))
+        torch.cuda.set_device(self.cuda)
 
 
-def select_device(index: int) -> None:
-    """The library launches on the calling thread's device; where there are several, each call names its own."""
-    if _several:
-        native.call("aljabr_blackwell_init", index)
+def selecting(call, index_of):
+    """`call` on the device that index_of finds in its arguments; where there is one device, `call` itself."""
+    if torch.cuda.device_count() <= 1:
+        return call
+
+    @functools.wraps(call)
+    def on_device(*args, **kwargs):
+        index = index_of(*args, **kwargs)
+        if index < 0:
+            return call(*args, **kwargs)      # not a CUDA tensor: refused there
+        with selected(index):
+            return call(*args, **kwargs)
+    return on_device
 
 
 def capture_id(stream: int) -> int:
@@ -95,7 +118,8 @@ class Kv4Cache:
         self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
         self.data, self.device, self.bytes = data, data.device, size
         self._index = data.get_device()
-        native.call("aljabr_blackwell_init", self._index)
+        with selected(self._index):
+            native.call("aljabr_blackwell_init", self._index)      # refuses other GPUs than the library's
         lib = native.lib()
         self._append, self._read = lib.aljabr_blackwell_kv4_append_dev, lib.aljabr_blackwell_kv4_read_dev
         self._attend, self._work_size = lib.aljabr_blackwell_kv4_attention_dev, lib.aljabr_blackwell_kv4_attention_workspace_size
@@ -134,8 +158,6 @@ class Kv4Cache:
         """Quantise the rows k, v into slots[i] = page * page_size + position (-1: skip the row).
 
         k_back / v_back (both or neither) receive the values the cache now holds."""
-        if _several:
-            select_device(self._index)
         n, dtype = slots.numel(), k.dtype
         kind = _DTYPES.get(dtype)
         if kind is None:
@@ -152,8 +174,6 @@ class Kv4Cache:
 
     def read(self, slots: torch.Tensor, dtype=torch.float32, k_out=None, v_out=None, stream=None):
         """Rows of the given slots as (k, v), [n, kv_heads, head_dim] each; zeros where a slot is -1."""
-        if _several:
-            select_device(self._index)
         n = slots.numel()
         stream = stream or current_stream(self._index)
         if k_out is None and v_out is None:
@@ -206,8 +226,6 @@ class Kv4Cache:
 
         block_table: int32 [batch, pages a sequence], or None where sequence b is page b.  scale: 1 / sqrt(head_dim)
         by default.  Returns out, contiguous, of q's type."""
-        if _several:
-            select_device(self._index)
         shape, st = q.shape, q.stride()
         if len(shape) != 4 or shape[3] != self.head_dim or q.get_device() != self._index:
             raise bad(f"q must be [batch, q_len, q_heads, {self.head_dim}] on {self.device}, not {tuple(shape)} on {q.device}")
@@ -245,3 +263,7 @@ class Kv4Cache:
         if rc:
             native.check(rc)
         return out
+
+
+for _name in ("append", "read", "attend"):
+    setattr(Kv4Cache, _name, selecting(getattr(Kv4Cache, _name), lambda cache, *_, **__: cache._index))

@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from . import native
-from .kv4 import _several, bad, current_stream, dtype_id, new_output, select_device
+from .kv4 import bad, current_stream, dtype_id, new_output, selecting
 
 
 _process = native.lib().aljabr_blackwell_logits_process_dev
@@ -31,8 +31,6 @@ def process_logits(logits: torch.Tensor, history=None, history_len=None, penalti
     if len(shape) != 2 or st[1] != 1 or dev < 0:
         raise bad("logits must be a [rows, vocab] CUDA tensor with contiguous rows")
     rows, vocab = shape
-    if _several:
-        select_device(dev)
     stream = stream or current_stream(dev)
     if out is None:
         out = new_output((rows, vocab), torch.float32, logits.device, dev, stream)
@@ -63,3 +61,6 @@ def process_logits(logits: torch.Tensor, history=None, history_len=None, penalti
     if rc:
         native.check(rc)
     return out, token
+
+
+process_logits = selecting(process_logits, lambda logits, *_, **__: logits.get_device())

@@ -56,6 +56,7 @@ _sz = ctypes.c_size_t
 
 # name -> (restype, argtypes); every symbol declared in the header is listed.
 SIGNATURES = {
+    "aljabr_blackwell_device_swap": (_i, [_i, _p]),
     "aljabr_blackwell_init": (_i, [_i]),
     "aljabr_blackwell_device_count": (_i, []),
     "aljabr_blackwell_device_get": (_i, [_i]),

@@ -88,6 +88,11 @@ int aljabr_blackwell_device_count(void);
  * aljabr_blackwell_init (FN_DEVICE_GET, BlackwellBinding.java:153-157,
  * bound at :465-466 as (JAVA_INT) -> JAVA_INT).  Returns 0 or an error. */
 int aljabr_blackwell_device_get(int device_id);
+/* The same, and *previous: the device selected before, -1 if none was.  With
+ * device_id -1 none is selected again: the thread's calls follow CUDA's
+ * current device, which stays.  For callers that select one call's device
+ * and put the choice back. */
+int aljabr_blackwell_device_swap(int device_id, int* previous);
 /* Device name into buf, NUL-terminated and truncated to buf_len bytes
  * (FN_DEVICE_NAME; argument order as bound at BlackwellBinding.java:469-470:
  * (ADDRESS buf, JAVA_INT bufSz, JAVA_INT deviceId)).  Returns 0 or an error. */

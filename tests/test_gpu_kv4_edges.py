@@ -5,6 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from aljabr_b200 import native
 from tests import kv4_ref as ref
 from tests.test_gpu_kv4 import attend_case, check, fault_bits, make
 
@@ -53,3 +54,19 @@ def test_a_page_of_more_than_2_to_the_30_positions():
     del cache
     torch.cuda.empty_cache()
     assert fault_bits() == 0
+
+
+def test_device_swap_gives_the_choice_back():
+    import ctypes
+    before, now = ctypes.c_int(7), ctypes.c_int(7)
+    native.call("aljabr_blackwell_device_swap", -1, ctypes.byref(before))
+    try:
+        native.call("aljabr_blackwell_device_swap", 0, ctypes.byref(now))
+        assert now.value == -1
+        for bad in (torch.cuda.device_count(), -2):
+            with pytest.raises(native.ProviderError):
+                native.call("aljabr_blackwell_device_swap", bad, ctypes.byref(now))
+        native.call("aljabr_blackwell_device_swap", -1, ctypes.byref(now))
+        assert now.value == 0
+    finally:
+        native.call("aljabr_blackwell_device_swap", before.value, ctypes.byref(now))
