@@ -243,9 +243,10 @@ class Kv4Cache:
         table, width = None, 0
         if block_table is not None:
             width = block_table.shape[-1]
-            if block_table.dtype is not torch.int32 or block_table.shape != (batch, width) or \
+            # an empty table has no address, which would read as no table
+            if block_table.dtype is not torch.int32 or block_table.shape != (batch, width) or (width == 0 and batch > 0) or \
                     block_table.get_device() != self._index or not block_table.is_contiguous():
-                raise bad(f"block_table must be contiguous int32 [{batch}, pages a sequence] on {self.device}")
+                raise bad(f"block_table must be contiguous int32 [{batch}, 1 or more pages a sequence] on {self.device}")
             table = block_table.data_ptr()
         if window:       # ctypes would take its low 32 bits
             window = max(-1, min(window, 0x7FFFFFFF))

@@ -70,3 +70,11 @@ def test_device_swap_gives_the_choice_back():
         assert now.value == 0
     finally:
         native.call("aljabr_blackwell_device_swap", before.value, ctypes.byref(now))
+
+
+def test_a_table_without_pages_is_refused():
+    """[batch, 0]: an empty tensor has no address, which would stand for 'sequence b is page b'."""
+    cache = make(2, 16, 1, 64)
+    q, lens = torch.zeros(1, 1, 1, 64, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(native.ProviderError):
+        cache.attend(q, lens, torch.zeros(1, 0, dtype=torch.int32, device="cuda"))
