@@ -85,7 +85,7 @@ constexpr int kItemCost = 2;     // chunks that an item's start and end are wort
 constexpr int kWholeItem = 4;    // chunks of an item that is not cut
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 2.0f;    // a row's maximum is raised only when a score exceeds it by 2 (log2)
-constexpr float kNone = -1e30f;  // running maximum of a row that has seen nothing
+constexpr float kNone = -3.4e38f;  // running maximum of a row that has seen nothing: below every finite score
 
 // d = a b + c; the form without c starts from zero.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,

@@ -78,3 +78,14 @@ def test_a_table_without_pages_is_refused():
     q, lens = torch.zeros(1, 1, 1, 64, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
     with pytest.raises(native.ProviderError):
         cache.attend(q, lens, torch.zeros(1, 0, dtype=torch.int32, device="cuda"))
+
+
+def test_scores_far_below_zero_still_sum_to_one():
+    """Equal scores of -1.1e31: the output is the mean of V, not zero."""
+    rng = np.random.default_rng(21)
+    k, v = np.full((40, 1, 128), -1.0, np.float32), rng.normal(size=(40, 1, 128)).astype(np.float32)
+    cache, table, n, k64, v64 = one_sequence(k, v)
+    out = cache.attend(torch.full((1, 1, 2, 128), 1e30, device="cuda"), n, table).double().cpu().numpy()
+    weight, want = np.abs(v64).mean(0)[0], v64.mean(0)[0]
+    # equal scores carry equal errors: what is left is P in two parts and fp32 sums, 2^-18 of sum P |v|
+    assert np.all(np.abs(out[0, 0] - want) <= weight * 2.0 ** -18)
