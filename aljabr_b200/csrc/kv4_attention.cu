@@ -633,13 +633,13 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
 #pragma unroll
                 for (int i = 0; i < NW; ++i) top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
             }
-            // a tile at the edge of what some row sees: masks; what no row sees, and NaN scales, do not set the shift
+            // a tile at the edge of what some row sees: masks; what no row sees does not set the shift
             uint32_t keep[CT][2];
 #pragma unroll
             for (int a = 0; a < CT; ++a) keep[a][0] = keep[a][1] = 0xFFFFFFFFu;
             if (pos < all_lo || pos + kTilePos - 1 > all_hi) {
                 const int word_pos = pos + (NG == 2 ? lane : lane >> 1);   // the position of the lane's scale words
-                if (word_pos >= len || (p.window > 0 && all_hi - word_pos >= p.window) || top >= 0x7C00u) top = 0u;
+                if (word_pos >= len || (p.window > 0 && all_hi - word_pos >= p.window)) top = 0u;
 #pragma unroll
                 for (int a = 0; a < CT; ++a)
 #pragma unroll
@@ -664,6 +664,17 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
                     most = fmaxf(most, fmaxf(y[a][0][j], y[a][1][j]) - M[a][j]);
             const bool raise = most > limit || static_cast<int>(top >> 10) > E;
             if (__any_sync(0xffffffffu, raise)) {
+                if (top >= 0x7C00u) {              // a NaN scale sets no shift, but its words' other groups do
+                    constexpr int NW = NG == 8 ? 2 : 1;
+                    uint32_t w[NW];
+                    lds_words<NW>(at_top + st, w);
+                    top = 0u;
+#pragma unroll
+                    for (int i = 0; i < 2 * NW; ++i) {
+                        const uint32_t h = (w[i >> 1] >> (16 * (i & 1))) & 0x7FFFu;
+                        if (h < 0x7C00u) top = max(top, h);
+                    }
+                }
                 const int e_new = max(E, static_cast<int>(__reduce_max_sync(0xffffffffu, top) >> 10));
                 const float t_old = shift_of(E), t_new = shift_of(e_new);
                 E = e_new;

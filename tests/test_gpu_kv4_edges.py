@@ -89,3 +89,24 @@ def test_scores_far_below_zero_still_sum_to_one():
     weight, want = np.abs(v64).mean(0)[0], v64.mean(0)[0]
     # equal scores carry equal errors: what is left is P in two parts and fp32 sums, 2^-18 of sum P |v|
     assert np.all(np.abs(out[0, 0] - want) <= weight * 2.0 ** -18)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("at", [5, 17])      # a tile that is seen whole, and the sequence's last one
+def test_a_nan_group_of_v_leaves_a_large_neighbour_finite(at, dtype):
+    """A V row with NaN in one group and a scale of 5000 in the next, among rows of scale 0.1."""
+    rng = np.random.default_rng(20)
+    k, v = (rng.normal(size=(20, 1, 128)).astype(np.float32) for _ in range(2))
+    v[at, 0, 32:64] *= 2e4
+    cache, table, n, k64, v64 = one_sequence(k, v)
+    bad = v.copy()
+    bad[at, 0, 7] = np.nan
+    cache.append(torch.from_numpy(k).cuda(), torch.from_numpy(bad).cuda(), torch.arange(20, dtype=torch.int32, device="cuda"))
+    q = torch.from_numpy(rng.normal(size=(1, 1, 2, 128)).astype(np.float32)).cuda().to(dtype)
+    out = cache.attend(q, n, table)
+    assert torch.isnan(out[..., :32]).all()
+    want, weight, delta = ref.attention(q.float().cpu().numpy()[0], k64, v64, 20)
+    # the bound of check() in tests/test_gpu_kv4.py, for the dims outside the NaN group
+    tol = weight * (2 * delta[..., None] * 2.0 ** -20 + 2.0 ** (-18 if dtype == torch.float32 else -10)) + 20 * 2.0 ** -28 * np.abs(v64).max()
+    tol += np.abs(want) * (2.0 ** -8 if dtype == torch.bfloat16 else 0)
+    assert np.all((np.abs(out[0].double().cpu().numpy() - want) <= tol)[..., 32:])
