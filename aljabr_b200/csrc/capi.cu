@@ -1449,7 +1449,8 @@ int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, lo
     if (batch < 0 || batch > kKv4MaxBatch)
         return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: batch %d outside [0, %d]", batch, kKv4MaxBatch);
     if (window < 0) return fail(ALJ_ERR_BAD_ARG, "kv4_attention: window %d < 0", window);
-    if (!(soft_cap >= 0.0f)) return fail(ALJ_ERR_BAD_ARG, "kv4_attention: soft_cap must be >= 0");
+    if (!(soft_cap == 0.0f || (soft_cap >= 1e-30f && soft_cap <= 1e30f)))   // its reciprocal is used
+        return fail(ALJ_ERR_BAD_ARG, "kv4_attention: soft_cap %g is neither 0 (none) nor in [1e-30, 1e30]", soft_cap);
     if (batch == 0) return ALJ_OK;
     if (!out || !q || !cache || !seq_lens || !workspace) return fail(ALJ_ERR_BAD_ARG, "kv4_attention: null pointer");
     if (block_table ? table_stride < 1 : batch > pages)

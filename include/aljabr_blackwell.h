@@ -364,7 +364,7 @@ int aljabr_blackwell_gemm_q_dev(int type, int nseg, float* const* y, const int* 
  * with window > 0 only the last `window` of them; a query that sees nothing
  * is zero.  Position p of sequence b is at block_table[b * table_stride + p /
  * page_size] (device), or with block_table NULL in page b.  soft_cap > 0
- * applies tanh(s / cap) * cap to the scaled scores.  fp32 queries are
+ * (in [1e-30, 1e30]) applies tanh(s / cap) * cap to the scaled scores.  fp32 queries are
  * computed to fp32 accuracy, bf16 ones to bf16's.  q_len * q_heads / kv_heads
  * is at most 1024, batch at most 2048.  The results do not depend on timing.
  * workspace: kv4_attention_workspace_size bytes of device memory, 256-byte
