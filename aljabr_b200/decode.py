@@ -164,6 +164,8 @@ class LlamaNf4Decoder:
         hist[0, :len(seen)] = torch.tensor(seen, dtype=torch.int32)
         live = torch.zeros(1, dtype=torch.int32, device=dev)
         pen = torch.tensor([penalties], dtype=torch.float32, device=dev)
+        if pen.shape != (1, 3):
+            raise native.ProviderError(native.ALJ_ERR_BAD_ARG, f"penalties must be three numbers, not {penalties}")
         out, best = torch.empty(V, dtype=torch.float32, device=dev), torch.empty(1, dtype=torch.int32, device=dev)
         bt = bv = bl = words = None
         if bias:

@@ -69,3 +69,17 @@ def test_strided_arrays_are_copied_and_outlive_the_call(monkeypatch):
     monkeypatch.setattr(native, "call", call)
     d.sync_kv_cache(0, 7, k, v)
     assert np.array_equal(seen[0], k) and np.array_equal(seen[1], v)
+
+
+@pytest.mark.parametrize("penalties", [(1.1,), (1.1, 0.0), (1.0, 0.0, 0.0, 0.0), [(1.0, 0.0, 0.0)]])
+def test_generate_takes_three_penalties(monkeypatch, penalties):
+    """The library reads three numbers from the address it is given."""
+    torch = pytest.importorskip("torch")
+    d, calls = decoder(monkeypatch, native.KV_Q4)
+    real = torch.device
+    monkeypatch.setattr(torch, "device", lambda *a: real("cpu"))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    d.step = lambda token, pos: calls.append(("step", (token, pos)))
+    with pytest.raises(native.ProviderError):
+        d.generate(3, 0, 2, penalties=penalties)
+    assert calls == []
