@@ -153,9 +153,10 @@ class LlamaNf4Decoder:
     def generate(self, token: int, pos: int, n_tokens: int, history=(), penalties=(1.0, 0.0, 0.0), bias=None,
                  allow=None) -> np.ndarray:
         """Greedy decode of n_tokens with the logits step between tokens: repetition / frequency / presence
-        penalties over `history` and everything emitted so far, `bias` ({token: value}), and `allow`, which gives
-        the grammar's words (uint32, bit t % 32 of word t / 32) for the tokens emitted so far, or None.  Stops
-        early when the grammar allows nothing.  Runs on cache and logits where they are (kv_dtype KV_Q4 too)."""
+        penalties over `history` and everything emitted so far, `bias` ({token: value}), and `allow`, a function that
+        gives the grammar's words (uint32, bit t % 32 of word t / 32) after the tokens emitted so far, or None where
+        every token may follow.  Stops early when the grammar allows nothing.  Runs on cache and logits where they
+        are (kv_dtype KV_Q4 too)."""
         import torch
         from .kv4 import current_stream
         dev, V = torch.device("cuda", torch.cuda.current_device()), self.shape.vocab
@@ -167,7 +168,7 @@ class LlamaNf4Decoder:
         if pen.shape != (1, 3):
             raise native.ProviderError(native.ALJ_ERR_BAD_ARG, f"penalties must be three numbers, not {penalties}")
         out, best = torch.empty(V, dtype=torch.float32, device=dev), torch.empty(1, dtype=torch.int32, device=dev)
-        bt = bv = bl = words = None
+        bt = bv = bl = None
         if bias:
             bt = torch.tensor(list(bias), dtype=torch.int32, device=dev)
             bv = torch.tensor(list(bias.values()), dtype=torch.float32, device=dev)
@@ -178,8 +179,9 @@ class LlamaNf4Decoder:
             self.step(token, pos + i)
             if i == 0:
                 native.call("aljabr_blackwell_decode_logits", ctypes.c_ulonglong(self.handle), ctypes.byref(logits))
-            if allow is not None:
-                words = torch.from_numpy(np.ascontiguousarray(allow(emitted), dtype=np.uint32).view(np.int32)).to(dev)
+            mask = None if allow is None else allow(emitted)
+            words = None if mask is None else \
+                torch.from_numpy(np.ascontiguousarray(mask, dtype=np.uint32).view(np.int32)).to(dev)
             live.fill_(len(seen))
             native.call("aljabr_blackwell_logits_process_dev", out.data_ptr(), V, logits, native.KV_F32, V, 1, V,
                         hist.data_ptr(), live.data_ptr(), hist.shape[1], pen.data_ptr(), ptr(bt), ptr(bv), ptr(bl),

@@ -83,3 +83,20 @@ def test_generate_takes_three_penalties(monkeypatch, penalties):
     with pytest.raises(native.ProviderError):
         d.generate(3, 0, 2, penalties=penalties)
     assert calls == []
+
+
+def test_a_grammar_may_allow_everything_for_a_token(monkeypatch):
+    """`allow` gives words, or None where the grammar says nothing about the next token."""
+    torch = pytest.importorskip("torch")
+    d, _ = decoder(monkeypatch, native.KV_Q4)
+    real, masks = torch.device, []
+    monkeypatch.setattr(torch, "device", lambda *a: real("cpu"))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    from aljabr_b200 import kv4
+    monkeypatch.setattr(kv4, "current_stream", lambda index: 1)
+    monkeypatch.setattr(native, "call", lambda name, *a: masks.append((a[15], a[16])) if "logits_process" in name else None)
+    d.step = lambda token, pos: None
+    words = np.full((1000 + 31) // 32, 0xFFFFFFFF, np.uint32)
+    monkeypatch.setattr(torch.Tensor, "__int__", lambda t: 5)
+    got = d.generate(3, 0, 3, allow=lambda emitted: words if len(emitted) == 1 else None)
+    assert got.tolist() == [5, 5, 5] and [m[1] for m in masks] == [0, 32, 0] and masks[0][0] is None and masks[2][0] is None
