@@ -1333,6 +1333,14 @@ int aljabr_blackwell_decode_logits(unsigned long long handle, const float** logi
     return ALJ_OK;
 }
 
+int aljabr_blackwell_decode_device(unsigned long long handle, int* device) {
+    DecodeModel* m = find(handle);
+    if (!m) return decode_fail(ALJ_ERR_BAD_ARG, "unknown decode model handle");
+    if (!device) return decode_fail(ALJ_ERR_BAD_ARG, "null device");
+    *device = m->device;
+    return ALJ_OK;
+}
+
 int aljabr_blackwell_decode_model_destroy(unsigned long long handle) {
     std::unique_ptr<DecodeModel> m;
     {

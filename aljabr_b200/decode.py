@@ -157,16 +157,23 @@ class LlamaNf4Decoder:
         gives the grammar's words (uint32, bit t % 32 of word t / 32) after the tokens emitted so far, or None where
         every token may follow.  Stops early when the grammar allows nothing.  Runs on cache and logits where they
         are (kv_dtype KV_Q4 too)."""
+        from .kv4 import selected
+        if np.shape(penalties) != (3,):
+            raise native.ProviderError(native.ALJ_ERR_BAD_ARG, f"penalties must be three numbers, not {penalties}")
+        device = ctypes.c_int(0)
+        native.call("aljabr_blackwell_decode_device", ctypes.c_ulonglong(self.handle), ctypes.byref(device))
+        with selected(device.value):
+            return self._generate(device.value, token, pos, n_tokens, history, penalties, bias, allow)
+
+    def _generate(self, device: int, token: int, pos: int, n_tokens: int, history, penalties, bias, allow) -> np.ndarray:
         import torch
         from .kv4 import current_stream
-        dev, V = torch.device("cuda", torch.cuda.current_device()), self.shape.vocab
+        dev, V = torch.device("cuda", device), self.shape.vocab
         hist = torch.zeros(1, max(1, len(history) + n_tokens + 1), dtype=torch.int32, device=dev)
         seen = list(history) + [token]
         hist[0, :len(seen)] = torch.tensor(seen, dtype=torch.int32)
         live = torch.zeros(1, dtype=torch.int32, device=dev)
         pen = torch.tensor([penalties], dtype=torch.float32, device=dev)
-        if pen.shape != (1, 3):
-            raise native.ProviderError(native.ALJ_ERR_BAD_ARG, f"penalties must be three numbers, not {penalties}")
         out, best = torch.empty(V, dtype=torch.float32, device=dev), torch.empty(1, dtype=torch.int32, device=dev)
         bt = bv = bl = None
         if bias:

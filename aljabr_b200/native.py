@@ -127,6 +127,7 @@ SIGNATURES = {
     "aljabr_blackwell_sync_kv_cache": (_i, [ctypes.c_ulonglong, _i, _i, _p, _p]),
     "aljabr_blackwell_decode_read_state": (_i, [ctypes.c_ulonglong, _p, _p, _p]),
     "aljabr_blackwell_decode_logits": (_i, [ctypes.c_ulonglong, _p]),
+    "aljabr_blackwell_decode_device": (_i, [ctypes.c_ulonglong, _p]),
     "aljabr_blackwell_decode_model_destroy": (_i, [ctypes.c_ulonglong]),
 }
 

@@ -494,6 +494,8 @@ int aljabr_blackwell_sync_kv_cache(unsigned long long handle, int layer, int seq
  * on the device.  decode_step_token has finished writing them when it
  * returns; the next step overwrites them. */
 int aljabr_blackwell_decode_logits(unsigned long long handle, const float** logits);
+/* The GPU that the model lives on, for what a host runs beside it. */
+int aljabr_blackwell_decode_device(unsigned long long handle, int* device);
 /* Copy the residual stream x (float[hidden]) and this rank's KV caches
  * ([layers][max_ctx][kv_heads/tp*head_dim] of kv_dtype) to host memory;
  * any pointer may be NULL. */

@@ -15,6 +15,8 @@ def decoder(monkeypatch, kv_dtype):
     d.tp_world, d.tp_rank, d.handle = 1, 0, 1
     calls = []
     monkeypatch.setattr(native, "call", lambda name, *a: calls.append((name, a)))
+    torch = pytest.importorskip("torch")
+    monkeypatch.setattr(torch.cuda, "set_device", lambda index: None)
     return d, calls
 
 
@@ -100,3 +102,35 @@ def test_a_grammar_may_allow_everything_for_a_token(monkeypatch):
     monkeypatch.setattr(torch.Tensor, "__int__", lambda t: 5)
     got = d.generate(3, 0, 3, allow=lambda emitted: words if len(emitted) == 1 else None)
     assert got.tolist() == [5, 5, 5] and [m[1] for m in masks] == [0, 32, 0] and masks[0][0] is None and masks[2][0] is None
+
+
+def test_generate_runs_on_the_model_s_device(monkeypatch):
+    """Two models on two GPUs: the thread's device is the last one's.  The logits step of the other must be launched, and
+    its tensors made, where that model is; afterwards the thread's choice is as before."""
+    torch = pytest.importorskip("torch")
+    d, _ = decoder(monkeypatch, native.KV_Q4)
+    real, state, seen = torch.device, {"cuda": 1, "library": 1}, []
+
+    def call(name, *a):
+        if name == "aljabr_blackwell_decode_device":
+            a[1]._obj.value = 0
+        elif name == "aljabr_blackwell_device_swap":
+            a[1]._obj.value, state["library"] = state["library"], a[0]
+            if a[0] >= 0:
+                state["cuda"] = a[0]
+        elif "logits_process" in name:
+            seen.append(dict(state))
+
+    def step(token, pos):
+        state["cuda"] = 0                     # as the library leaves it
+    made = []
+    monkeypatch.setattr(native, "call", call)
+    monkeypatch.setattr(torch, "device", lambda kind, index: made.append(index) or real("cpu"))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["cuda"])
+    monkeypatch.setattr(torch.cuda, "set_device", lambda i: state.update(cuda=i))
+    from aljabr_b200 import kv4
+    monkeypatch.setattr(kv4, "current_stream", lambda index: 1)
+    monkeypatch.setattr(torch.Tensor, "__int__", lambda t: 5)
+    d.step = step
+    d.generate(3, 0, 2)
+    assert made == [0] and seen == [{"cuda": 0, "library": 0}] * 2 and state == {"cuda": 1, "library": 1}
