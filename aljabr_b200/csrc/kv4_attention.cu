@@ -258,6 +258,7 @@ __device__ __forceinline__ void load_chunk(const Kv4Attn& p, const TileSource& t
         record_fault(ALJ_FAULT_BOUNDS);
         if (sec >= 2)
             for (int i = 0; i < F::SCALES / 16; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the slot's next writer is a bulk copy
     }
     const unsigned int tiles = __popc(__ballot_sync(0xffffffffu, ok)) / 4;
     __syncwarp();

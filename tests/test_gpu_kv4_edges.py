@@ -110,3 +110,18 @@ def test_a_nan_group_of_v_leaves_a_large_neighbour_finite(at, dtype):
     tol = weight * (2 * delta[..., None] * 2.0 ** -20 + 2.0 ** (-18 if dtype == torch.float32 else -10)) + 20 * 2.0 ** -28 * np.abs(v64).max()
     tol += np.abs(want) * (2.0 ** -8 if dtype == torch.bfloat16 else 0)
     assert np.all((np.abs(out[0].double().cpu().numpy() - want) <= tol)[..., 32:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_absent_pages_between_others_in_a_long_sequence(dtype):
+    """A page outside the cache counts as zeros: score 0, value 0.  Every slot of the ring is then loaded again."""
+    lens, ps = [9000], 16
+    cache, q, sl, table, _, k64, v64 = attend_case(25, 128, 1, 2, 1, ps, lens, dtype=dtype)
+    gone = [3, 40, 41, 200, 333, 561]
+    for i in gone:
+        table[0, i] = -7 if i % 2 else 10 ** 8
+        k64[0][i * ps:(i + 1) * ps] = 0.0
+        v64[0][i * ps:(i + 1) * ps] = 0.0
+    out = cache.attend(q, sl, table)
+    assert fault_bits() & 2
+    check(out, q, k64, v64, lens)
