@@ -17,14 +17,19 @@
 //   * The K codes are the A operand of S = K q^T without being converted: a
 //     nibble masked out of its word is the fp16 subnormal c * 2^-24 (or
 //     16 c * 2^-24), exact, so 8 codes cost 4 LOP3 and a shift.  The slots
-//     with the factor 16 have q / 16 on the other side.  The offset -8 is
-//     sum_g dK[p, g] * (-8 sum_{j in g} q_j): one more MMA with the fp16
-//     scales as they are stored for its A operand.
+//     with the factor 16 have q / 16 on the other side.
 //   * q is scaled by a power of two into fp16's range.  bf16 queries are
-//     exact in one column; fp32 queries take two, each a multiple of a fixed
-//     step of the row (2^-11 and 2^-22 of its largest value), so that the
-//     tensor cores' sums of a group are exact integers and their truncation
-//     does not enter.  4 fp32 rows, as 8 bf16 ones, fill one MMA's columns.
+//     exact in one column; their offset -8 is sum_g dK[p, g] * (-8 sum_{j in
+//     g} q_j), one more MMA with the fp16 scales as they are stored for its A
+//     operand.  fp32 queries take two columns, each a multiple of a fixed step
+//     of the row's group of 32 (2^-11 and 2^-23 of the group's largest value,
+//     so an element is off by at most 2^-23 of that).  Their groups' sums
+//     start from -8 sum_j q_j and are exact integers: neither the tensor
+//     cores' truncation nor an outlier in another group enters.  (One step for
+//     the whole row loses 1e-4 of the result where q has an outlier of 300;
+//     the group's scales cost 4 FMUL and a shared load a group, 5 % of the
+//     time: 2 sequences of 131072, 32 fp32 heads on 8, 102 us against 96.)
+//     4 fp32 rows, as 8 bf16 ones, fill one MMA's columns.
 //   * P = 2^(S - M), M the running maximum less a shift t: P lies where fp16
 //     is precise, and no other scaling is kept.  One movmatrix turns the
 //     accumulator layout (rows = positions) into the B operand of
@@ -179,7 +184,7 @@ struct Cfg {
     static constexpr int MROW = SG * 32 + 4;                // floats a column in the merge buffer; + 4: no bank conflicts
     static constexpr int MERGE = kWarps * COLS * MROW * 4;
     static constexpr int QFRAG = CT * NG * 2 * 32 * 8;
-    static constexpr int QOFF = CT * 32 * 8;                // offset fragments
+    static constexpr int QOFF = PARTS == 2 ? CT * NG * 64 : CT * 32 * 8;   // per group offsets and scales, or offset fragments
     static constexpr int BARS = kStages * 2 * 8;            // full and empty
     static constexpr int MISC = (3 * kWarps * COLS + kWarps + 2 * COLS + 8) * 4;
     static constexpr int SMEM = RING + MERGE + QFRAG + QOFF + BARS + MISC;   // + the per-sequence tables
@@ -284,7 +289,8 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     uint8_t* const ring = smem;
     float* const s_merge = reinterpret_cast<float*>(smem + F::RING);
     uint2* const s_q = reinterpret_cast<uint2*>(smem + F::RING + F::MERGE);
-    uint2* const s_off = s_q + F::QFRAG / 8;                  // offset fragments
+    uint2* const s_off = s_q + F::QFRAG / 8;                  // PARTS 1: offset fragments
+    float4* const s_group = reinterpret_cast<float4*>(s_off); // PARTS 2: [column tile][group][c4] offsets, scales of 2 columns
     uint64_t* const s_bar = reinterpret_cast<uint64_t*>(s_off + F::QOFF / 8);
     float* const s_m = reinterpret_cast<float*>(s_bar + 2 * kStages);   // [warp][column] running maximum
     float* const s_l = s_m + kWarps * COLS;                             // [warp][column] weighted sum
@@ -392,9 +398,9 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     load_seq(at, p, tab);
     bool dead = false;                             // a chunk never arrived: stop waiting, the fault is recorded
     constexpr bool kQRegs = CT == 1 && NG <= 4;    // q fragments in registers, else read for every tile
-    // PARTS 2: the other part's column is two lanes away and weighs 2^-11 where this one is the high part
+    // PARTS 2: the other part's column is two lanes away and weighs 2^-12 where this one is the high part
     const float inv_cap = p.soft_cap > 0.0f ? 1.0f / p.soft_cap : 0.0f;
-    const float own = PARTS == 1 || c4 < 2 ? 1.0f : 1.0f / 2048.0f, others = c4 < 2 ? 1.0f / 2048.0f : 1.0f;
+    const float own = PARTS == 1 || c4 < 2 ? 1.0f : 1.0f / 4096.0f, others = c4 < 2 ? 1.0f / 4096.0f : 1.0f;
     // e: exponent field the shift t is made for.  |dV| < 2^(e - 14) and P <= 2^(t + kLazy): P dV < 2^15, and for bf16,
     // where P itself is rounded to fp16, P <= 2^15
     auto shift_of = [](int e) { return PARTS == 2 ? 27 - e : min(13, 27 - e); };
@@ -437,8 +443,8 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
         const Item it = item_of(at);
         const int kvh = it.kvh, row0 = it.row0, rows = it.rows, item_b = at.b;
 
-        // q rows -> columns in B-fragment order, their group sums, their score factors.  A lane has NG dims of
-        // one group.  (The first warps are busy with the first chunks.)
+        // q rows -> columns in B-fragment order, their groups' sums and scales, their score factors.  A lane has NG dims
+        // of one group.  (The first warps are busy with the first chunks.)
         for (int row = (warp - kAhead) & (kWarps - 1); row < ROWS; row += kWarps) {
             float x[NG];
             const int i = row0 + row;
@@ -446,7 +452,9 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             const int t = live ? token_of(i) : 0, hd = live ? i - t * p.group : 0;
             const long long src = (static_cast<long long>(item_b) * p.q_len + t) * p.q_stride +
                                   static_cast<long long>(kvh * p.group + hd) * D + lane * NG;
-            float big = 0.0f;
+            constexpr int kSpan = 32 / NG;         // lanes of a group
+            const int g = lane / kSpan;
+            float big = 0.0f, big_g = 0.0f;        // largest value of the row, of the lane's group
 #pragma unroll
             for (int k = 0; k < NG; ++k) {
                 x[k] = 0.0f;
@@ -456,12 +464,17 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
                 big = fmaxf(big, fabsf(x[k]));
             }
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-            // big * 2^f in [2^14, 2^15); f kept where both 2^f and the factor below are normal
-            const int f = big > 0.0f ? max(-100, min(126, 14 - (static_cast<int>((__float_as_uint(big) >> 23) & 255) - 127))) : 0;
-            const float up = pow2i(f);
-            constexpr int kSpan = 32 / NG;         // lanes of a group
-            const int g = lane / kSpan;
+            for (int o = 1; o < 32; o <<= 1) {
+                if (o == kSpan) big_g = big;
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            }
+            // v * 2^f in [2^14, 2^15)
+            auto raise_of = [](float v) { return 14 - (static_cast<int>((__float_as_uint(v) >> 23) & 255) - 127); };
+            // f of the row, kept where both 2^f and the factor below are normal; PARTS 2: fg of the group, at most 2^40
+            // above the row's, so that d * 2^(f - fg) is normal too
+            const int f = big > 0.0f ? max(-100, min(126, raise_of(big))) : 0;
+            const int fg = PARTS == 2 && big_g > 0.0f ? max(-100, min(min(126, f + 40), raise_of(big_g))) : f;
+            const float up = pow2i(fg);
             float sum[PARTS] = {};
 #pragma unroll
             for (int k = 0; k < NG; ++k) {
@@ -469,10 +482,10 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
                 // dim j of its group is slot (c = j / 8, i = j % 8): MMA step (i & 3) >> 1, k half i & 1 (where the
                 // codes carry a factor 16), pair c, element i >> 2
                 const int j = (lane % kSpan) * NG + k, c = j >> 3, i8 = j & 7, st = (i8 & 3) >> 1;
-                // PARTS 2: multiples of 16 and of 2^-7 -- 11 bits each, so that a group's sum of products is exact
+                // PARTS 2: multiples of 16 and of 2^-8 -- 11 bits each, so that a group's sum of products is exact
                 __half v[PARTS];
                 v[0] = __float2half_rn(PARTS == 2 ? rintf(y * 0.0625f) * 16.0f : y);
-                if (PARTS == 2) v[PARTS - 1] = __float2half_rn(rintf((y - __half2float(v[0])) * 128.0f) * 16.0f);
+                if (PARTS == 2) v[PARTS - 1] = __float2half_rn(rintf((y - __half2float(v[0])) * 256.0f) * 16.0f);
 #pragma unroll
                 for (int e = 0; e < PARTS; ++e) {
                     const int col = column_of<PARTS>(row, e);
@@ -485,17 +498,22 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             for (int o = kSpan / 2; o > 0; o >>= 1)
 #pragma unroll
                 for (int e = 0; e < PARTS; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
-            // offset fragment: k = g holds the group sum * 2^-6 in fp16, k = NG + g what that rounding left
-            if (lane % kSpan < 2) {
-                const int k = lane % kSpan * NG + g;
-#pragma unroll
-                for (int e = 0; e < PARTS; ++e) {
-                    const float v = sum[e] * 0.015625f;
-                    const __half h = __float2half_rn(v);
-                    const int col = column_of<PARTS>(row, e);
-                    reinterpret_cast<__half*>(s_off + (col >> 3) * 32 + (col & 7) * 4 + ((k & 7) >> 1))[(k >> 3) * 2 + (k & 1)] =
-                        k < NG ? h : __float2half_rn(v - __half2float(h));
+            if constexpr (PARTS == 2) {
+                // what the group's products start from, in their units: -8 * 2^-24 times its sum, exact; and the
+                // group's scale against the row's
+                if (lane % kSpan < 2) {
+                    const int e = lane % kSpan, col = column_of<PARTS>(row, e);
+                    float* const to = reinterpret_cast<float*>(s_group + ((col >> 3) * NG + g) * 4 + ((col & 7) >> 1)) + (col & 1);
+                    to[0] = (e ? sum[PARTS - 1] : sum[0]) * -4.76837158203125e-7f;
+                    to[2] = pow2i(f - fg);
                 }
+            } else if (lane % kSpan < 2) {
+                // offset fragment: k = g holds the group sum * 2^-6 in fp16, k = NG + g what that rounding left
+                const int k = lane % kSpan * NG + g;
+                const float v = sum[0] * 0.015625f;
+                const __half h = __float2half_rn(v);
+                reinterpret_cast<__half*>(s_off + (row >> 3) * 32 + (row & 7) * 4 + ((k & 7) >> 1))[(k >> 3) * 2 + (k & 1)] =
+                    k < NG ? h : __float2half_rn(v - __half2float(h));
             }
             if (lane < PARTS) s_fac[column_of<PARTS>(row, lane)] = p.scale * pow2i(24 - f);
         }
@@ -562,23 +580,24 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
                     lds_words<NG / 2>(at_ks + st + h * 16 * NG, dw[h]);
                 }
                 float off[CT][4], part[CT][4];
-                // offset: A = the scales, k = g and again NG + g
-                uint32_t o0, o1;
-                if constexpr (NG == 8) {
-                    o0 = c4 & 2 ? (c4 & 1 ? dw[0][3] : dw[0][2]) : (c4 & 1 ? dw[0][1] : dw[0][0]);
-                    o1 = c4 & 2 ? (c4 & 1 ? dw[1][3] : dw[1][2]) : (c4 & 1 ? dw[1][1] : dw[1][0]);
-                } else if constexpr (NG == 4) {
-                    o0 = c4 & 1 ? dw[0][1] : dw[0][0];
-                    o1 = c4 & 1 ? dw[1][1] : dw[1][0];
-                } else {                           // k = 4 .. 7 are empty
-                    o0 = c4 < 2 ? dw[0][0] : 0u;
-                    o1 = c4 < 2 ? dw[1][0] : 0u;
-                }
+                if constexpr (PARTS == 1) {        // offset: A = the scales, k = g and again NG + g
+                    uint32_t o0, o1;
+                    if constexpr (NG == 8) {
+                        o0 = c4 & 2 ? (c4 & 1 ? dw[0][3] : dw[0][2]) : (c4 & 1 ? dw[0][1] : dw[0][0]);
+                        o1 = c4 & 2 ? (c4 & 1 ? dw[1][3] : dw[1][2]) : (c4 & 1 ? dw[1][1] : dw[1][0]);
+                    } else if constexpr (NG == 4) {
+                        o0 = c4 & 1 ? dw[0][1] : dw[0][0];
+                        o1 = c4 & 1 ? dw[1][1] : dw[1][0];
+                    } else {                       // k = 4 .. 7 are empty
+                        o0 = c4 < 2 ? dw[0][0] : 0u;
+                        o1 = c4 < 2 ? dw[1][0] : 0u;
+                    }
 #pragma unroll
-                for (int a = 0; a < CT; ++a) {
-                    const uint2 b = s_off[a * 32 + lane];
-                    if constexpr (NG == 8) mma_f16_zero(off[a], o0, o1, o0, o1, b.x, b.y);
-                    else mma_f16_k8_zero(off[a], o0, o1, b.x);
+                    for (int a = 0; a < CT; ++a) {
+                        const uint2 b = s_off[a * 32 + lane];
+                        if constexpr (NG == 8) mma_f16_zero(off[a], o0, o1, o0, o1, b.x, b.y);
+                        else mma_f16_k8_zero(off[a], o0, o1, b.x);
+                    }
                 }
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
@@ -596,23 +615,32 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
 #pragma unroll
                     for (int a = 0; a < CT; ++a) {
                         const uint2 b0 = q_frag(a, g, 0), b1 = q_frag(a, g, 1);
-                        float x[4];
-                        mma_f16_zero(x, f[0][0], f[1][0], f[0][1], f[1][1], b0.x, b0.y);
+                        float x[4], d[4] = {d0, d0, d1, d1};
+                        if constexpr (PARTS == 2) {
+                            const float4 start = s_group[(a * NG + g) * 4 + c4];
+                            x[0] = x[2] = start.x;
+                            x[1] = x[3] = start.y;
+                            mma_f16(x, f[0][0], f[1][0], f[0][1], f[1][1], b0.x, b0.y);
+                            d[0] = d0 * start.z; d[1] = d0 * start.w;
+                            d[2] = d1 * start.z; d[3] = d1 * start.w;
+                        } else {
+                            mma_f16_zero(x, f[0][0], f[1][0], f[0][1], f[1][1], b0.x, b0.y);
+                        }
                         mma_f16(x, f[0][2], f[1][2], f[0][3], f[1][3], b1.x, b1.y);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            part[a][j] = g == 0 ? (j < 2 ? d0 : d1) * x[j] : fmaf(j < 2 ? d0 : d1, x[j], part[a][j]);
+                        for (int j = 0; j < 4; ++j) part[a][j] = g == 0 ? d[j] * x[j] : fmaf(d[j], x[j], part[a][j]);
                     }
                 }
-                // offset in the units of the products: -8 * 2^6 * 2^-24
+                // PARTS 1: offset in the units of the products: -8 * 2^6 * 2^-24
 #pragma unroll
                 for (int a = 0; a < CT; ++a)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            float v = fmaf(off[a][2 * h + j], -3.0517578125e-5f, part[a][2 * h + j]);
-                            if (PARTS == 2) v = fmaf(v, own, __shfl_xor_sync(0xffffffffu, v, 2) * others);
+                            float v = part[a][2 * h + j];
+                            if constexpr (PARTS == 2) v = fmaf(v, own, __shfl_xor_sync(0xffffffffu, v, 2) * others);
+                            else v = fmaf(off[a][2 * h + j], -3.0517578125e-5f, v);
                             y[a][h][j] = v * fac[a][j];
                         }
             }

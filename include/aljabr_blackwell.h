@@ -364,9 +364,15 @@ int aljabr_blackwell_gemm_q_dev(int type, int nseg, float* const* y, const int* 
  * with window > 0 only the last `window` of them; a query that sees nothing
  * is zero.  Position p of sequence b is at block_table[b * table_stride + p /
  * page_size] (device), or with block_table NULL in page b.  soft_cap > 0
- * (in [1e-30, 1e30]) applies tanh(s / cap) * cap to the scaled scores.  fp32 queries are
- * computed to fp32 accuracy, bf16 ones to bf16's.  q_len * q_heads / kv_heads
- * is at most 1024, batch at most 2048.  The results do not depend on timing.
+ * (in [1e-30, 1e30]) applies tanh(s / cap) * cap to the scaled scores.
+ * Accuracy: sums and softmax statistics are fp32.  An fp32 query element
+ * enters with an error of at most 2^-23 of the largest in its group of 32
+ * dims (an outlier costs its own group's small values their last bits),
+ * softmax weights with 2^-22 of themselves or 2^-28 of the largest V.  For
+ * bf16 queries the weights and their products with V's scales are rounded to
+ * fp16 (2^-11 each), below the output's own rounding of 2^-9.
+ * q_len * q_heads / kv_heads is at most 1024, batch at most 2048.  The results
+ * do not depend on timing.
  * workspace: kv4_attention_workspace_size bytes of device memory, 256-byte
  * aligned, used by one call at a time; its first kilobytes are arrival
  * counters that must be zero before the first call and are zero after each.

@@ -125,3 +125,30 @@ def test_absent_pages_between_others_in_a_long_sequence(dtype):
     out = cache.attend(q, sl, table)
     assert fault_bits() & 2
     check(out, q, k64, v64, lens)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_outliers_of_q_do_not_cost_the_other_groups_their_bits(D):
+    """q 300 times larger in one group of 32 (where K is small), K 100 times larger in another (where q is small).
+
+    Bound of a score: q is off by at most 2^-23 of the largest value of its group of 32, so
+    e = 2^-23 scale sum_g max|q_g| sum_g |k|, plus NG + 8 fp32 roundings of the groups' sums.  The output is then off by
+    at most 2 e + 2^-18 (exp2, P in two parts, sums) of sum P |v|."""
+    rng = np.random.default_rng(22 + D)
+    n, heads, NG = 60, 16, D // 32
+    k, v = (rng.normal(size=(n, 1, D)).astype(np.float32) for _ in range(2))
+    q = rng.normal(size=(1, 1, heads, D)).astype(np.float32)
+    k[..., :32] *= 0.05
+    k[..., D - 5] *= 100
+    q[..., 3] *= 300
+    q[..., D - 32:] *= 0.1
+    cache, table, lens, k64, v64 = one_sequence(k, v)
+    out = cache.attend(torch.from_numpy(q).cuda(), lens, table).double().cpu().numpy()[0]
+    want, weight, _ = ref.attention(q[0], k64, v64, n)
+    scale = D ** -0.5
+    top = np.abs(q[0, 0].astype(np.float64)).reshape(heads, NG, 32).max(-1)
+    size = np.abs(k64[:, 0]).reshape(n, NG, 32).sum(-1)
+    sums = np.abs(np.einsum("hgj,ngj->hng", q[0, 0].astype(np.float64).reshape(heads, NG, 32), k64[:, 0].reshape(n, NG, 32)))
+    e = scale * (2.0 ** -23 * (top @ size.T).max(-1) + (NG + 8) * 2.0 ** -24 * 2 * sums.sum(-1).max(-1))
+    err, tol = np.abs(out[0] - want[0]), weight[0] * (2 * e[:, None] + 2.0 ** -18) + n * 2.0 ** -28 * np.abs(v64).max()
+    assert np.all(err <= tol), float((err / tol).max())
