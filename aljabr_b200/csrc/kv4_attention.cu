@@ -23,12 +23,14 @@
 //     g} q_j), one more MMA with the fp16 scales as they are stored for its A
 //     operand.  fp32 queries take two columns, each a multiple of a fixed step
 //     of the row's group of 32 (2^-11 and 2^-23 of the group's largest value,
-//     so an element is off by at most 2^-23 of that).  Their groups' sums
-//     start from -8 sum_j q_j and are exact integers: neither the tensor
+//     so an element is off by at most 2^-23 of that).  Their groups' sums,
+//     with the offset -8 sum_j q_j, are exact integers: neither the tensor
 //     cores' truncation nor an outlier in another group enters.  (One step for
 //     the whole row loses 1e-4 of the result where q has an outlier of 300;
-//     the group's scales cost 4 FMUL and a shared load a group, 5 % of the
-//     time: 2 sequences of 131072, 32 fp32 heads on 8, 102 us against 96.)
+//     a group's scale and offset cost 4 FFMA and a shared load, asked for ahead
+//     of its products: 8 sequences of 8192, 32 fp32 heads on 8, 33.0 us against
+//     32.7, D 256 53.5 against 51.5.  Loaded after the products, short contexts
+//     took 0.5 us more.)
 //     4 fp32 rows, as 8 bf16 ones, fill one MMA's columns.
 //   * P = 2^(S - M), M the running maximum less a shift t: P lies where fp16
 //     is precise, and no other scaling is kept.  One movmatrix turns the
@@ -499,13 +501,14 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
 #pragma unroll
                 for (int e = 0; e < PARTS; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
             if constexpr (PARTS == 2) {
-                // what the group's products start from, in their units: -8 * 2^-24 times its sum, exact; and the
-                // group's scale against the row's
+                // the group's scale against the row's, and -8 * 2^-24 (the products' units) times its sum, scaled so:
+                // powers of two and an integer of 20 bits, all exact
                 if (lane % kSpan < 2) {
                     const int e = lane % kSpan, col = column_of<PARTS>(row, e);
                     float* const to = reinterpret_cast<float*>(s_group + ((col >> 3) * NG + g) * 4 + ((col & 7) >> 1)) + (col & 1);
-                    to[0] = (e ? sum[PARTS - 1] : sum[0]) * -4.76837158203125e-7f;
-                    to[2] = pow2i(f - fg);
+                    const float u = pow2i(f - fg);
+                    to[0] = (e ? sum[PARTS - 1] : sum[0]) * -4.76837158203125e-7f * u;
+                    to[2] = u;
                 }
             } else if (lane % kSpan < 2) {
                 // offset fragment: k = g holds the group sum * 2^-6 in fp16, k = NG + g what that rounding left
@@ -564,6 +567,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
         const uint32_t at_ks = hide(scales + krow * 2 * NG);
         const uint32_t at_vs = hide(scales + kWarps * F::SCALES + vrow0 * 2 * NG);
         const uint32_t at_top = hide(scales + kWarps * F::SCALES + lane * (NG == 8 ? 8 : 4));
+        const uint32_t at_group = hide(smem_u32(s_group) + c4 * 16);
         auto q_frag = [&](int a, int g, int st) {
             if constexpr (kQRegs) return qreg[2 * g + st];
             return s_q[((a * NG + g) * 2 + st) * 32 + lane];
@@ -615,20 +619,18 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
 #pragma unroll
                     for (int a = 0; a < CT; ++a) {
                         const uint2 b0 = q_frag(a, g, 0), b1 = q_frag(a, g, 1);
-                        float x[4], d[4] = {d0, d0, d1, d1};
-                        if constexpr (PARTS == 2) {
-                            const float4 start = s_group[(a * NG + g) * 4 + c4];
-                            x[0] = x[2] = start.x;
-                            x[1] = x[3] = start.y;
-                            mma_f16(x, f[0][0], f[1][0], f[0][1], f[1][1], b0.x, b0.y);
-                            d[0] = d0 * start.z; d[1] = d0 * start.w;
-                            d[2] = d1 * start.z; d[3] = d1 * start.w;
-                        } else {
-                            mma_f16_zero(x, f[0][0], f[1][0], f[0][1], f[1][1], b0.x, b0.y);
-                        }
+                        float x[4];
+                        uint32_t gr[4];            // the group's offsets and scales, on their way before the products
+                        if constexpr (PARTS == 2) lds_words<4>(at_group + (a * NG + g) * 64, gr);
+                        mma_f16_zero(x, f[0][0], f[1][0], f[0][1], f[1][1], b0.x, b0.y);
                         mma_f16(x, f[0][2], f[1][2], f[0][3], f[1][3], b1.x, b1.y);
+                        if constexpr (PARTS == 2) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) part[a][j] = g == 0 ? d[j] * x[j] : fmaf(d[j], x[j], part[a][j]);
+                            for (int j = 0; j < 4; ++j) x[j] = fmaf(x[j], __uint_as_float(gr[2 + (j & 1)]), __uint_as_float(gr[j & 1]));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            part[a][j] = g == 0 ? (j < 2 ? d0 : d1) * x[j] : fmaf(j < 2 ? d0 : d1, x[j], part[a][j]);
                     }
                 }
                 // PARTS 1: offset in the units of the products: -8 * 2^6 * 2^-24
