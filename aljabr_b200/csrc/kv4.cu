@@ -12,8 +12,8 @@
 // head_dim is a template parameter (rows by shifts), a code is four
 // operations (kv4_rounded), and 40 registers let 48 warps an SM wait for
 // their loads (50 registers: 48 us).  Measured: 16384 rows of 8 x 128, fp32 in
-// and back, 46.4 us (6.2 TB/s, 96 % of the measured copy rate); 49152 rows read
-// back as fp32 72.5 us (6.3 TB/s, 98 %).
+// and back, 46.4 to 47.1 us over several runs (6.1 to 6.2 TB/s, 94 to 96 % of
+// the measured copy rate); 49152 rows read back as fp32 72.5 us (6.3 TB/s, 98 %).
 #include "kv4.cuh"
 
 #include <algorithm>

@@ -42,7 +42,8 @@
 //     the size of V.
 //   * V codes become the exact fp16 integers c - 8 (the sums then stay as
 //     small as the result; adding -8 sum P dV afterwards would lose 2-3 digits
-//     over long contexts): (bits | 1024) - 1032, or (bits | 1024) / 16 - 72.
+//     over long contexts): (bits | 1024) - 1032, or (bits | 1024) / 16 - 72, the
+//     well-known reading of small integers as the low bits of an fp16 number.
 //     Two positions are interleaved by one PRMT, no transposing load needed.
 //   * Rounding points: q parts, P parts, the output type.  Scores, softmax
 //     statistics and sums are fp32.  For fp32 outputs every tile's product is
@@ -68,8 +69,8 @@
 //
 // Measured (1965 MHz, measured copy rate 6473 GB/s): two sequences of 131072,
 // 64 query heads on 8 kv heads, D 128, bf16: 79 us, 3.8 TB/s; 32 ragged
-// sequences up to 16384: 54.5 us, 3.3 TB/s; 4096 positions of one sequence, fp32:
-// 11.4 us.  The long ones are bound by issue: 374 instructions a tile (2304
+// sequences up to 16384: 55 us, 3.3 TB/s; 4096 positions of one sequence, fp32:
+// 11.6 us.  The long ones are bound by issue: 374 instructions a tile (2304
 // bytes) at 2.45 a clock and SM, ALU pipe 55 % busy, DRAM 44 %; the short ones
 // by the chain launch - lengths - page - tile - merge - join.  Tried and
 // slower, against 80 us: scores of the next tile beside the values of this one (84 us), tiles
@@ -88,8 +89,8 @@ constexpr int kTilePos = 16;
 constexpr int kChunkTiles = kWarps;
 constexpr int kStages = 4;
 constexpr int kAhead = 2;        // chunks asked for before their turn
-constexpr int kItemCost = 2;     // chunks that an item's start and end are worth
-constexpr int kWholeItem = 4;    // chunks of an item that is not cut
+constexpr int kItemCost = 2;     // chunks that an item's start and end are worth (4: 80.6 us for 2 x 131072, 80.0 with 2)
+constexpr int kWholeItem = 4;    // chunks of the average item up to which none is cut for want of work
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 2.0f;    // a row's maximum is raised only when a score exceeds it by 2 (log2)
 constexpr float kNone = -3.4e38f;  // running maximum of a row that has seen nothing: below every finite score
@@ -363,7 +364,8 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     // A chunk costs a CTA about as much as 25 parts cost the one that joins them, so where the line is short an item
     // of n places is cut into stretches of sqrt(n / 25): one kv head of 32768 positions 23 us with 256 CTAs of a
     // chunk each, 16 so.  The join itself costs as much as three chunks, so items of up to kWholeItem chunks are left
-    // whole: 257 positions 9.1 us in three parts, 7.2 whole.
+    // whole: 257 positions 9.1 us in three parts, 7.4 whole.  n is the average item: among short sequences a long one
+    // is cut as they are, and dealt out over the CTAs all the same.
     const int width = (total + p.batch - 1) / p.batch;
     const int stretch = width <= kItemCost + kWholeItem ? width : max(1, __float2int_rn(sqrtf(width / 25.0f)));
     total *= items;
@@ -990,7 +992,8 @@ cudaError_t launch_cfg(Kv4Attn p, int sms, int max_ctas, cudaStream_t stream) {
         if (e != cudaSuccess) return e;
         configured[dev & 63] = true;
     }
-    // One wave: two CTAs an SM where registers and 227 KB of shared memory hold two.
+    // One wave: two CTAs an SM where registers and 227 KB of shared memory hold two.  At D 128 the batch's tables leave
+    // room for two up to 552 sequences: 500 of 300 positions 94 us, 600 of them 164 us.
     const int per_sm = NG * CT <= 4 && 2 * (smem + 1024) <= 227 * 1024 ? 2 : 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(std::min(per_sm * sms, max_ctas));
@@ -1008,7 +1011,9 @@ cudaError_t launch_cfg(Kv4Attn p, int sms, int max_ctas, cudaStream_t stream) {
 // Rows a CTA serves at once: a column tile holds 8 bf16 or 4 fp32 rows; two
 // tiles where the rows need them and the accumulators fit (D <= 128): 8
 // sequences of 8192 with 16 bf16 rows 44 us in one pass of two tiles, 49 in two
-// of one; 8 fp32 rows 46 against 55.
+// of one; 8 fp32 rows 47 against 55.  D 256 has room for one tile and one CTA
+// an SM (220 registers a thread, 181 KB of ring and merge buffer): 48 us for 4
+// bf16 rows of the same, 3.2 TB/s.
 int tile_rows(int rows, int head_dim, bool wide) {
     const int one = wide ? 4 : 8;
     return rows > one && head_dim <= 128 ? 2 * one : one;

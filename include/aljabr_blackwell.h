@@ -373,9 +373,11 @@ int aljabr_blackwell_gemm_q_dev(int type, int nseg, float* const* y, const int* 
  * fp16 (2^-11 each), below the output's own rounding of 2^-9.
  * q_len * q_heads / kv_heads is at most 1024, batch at most 2048.  The results
  * do not depend on timing.
- * workspace: kv4_attention_workspace_size bytes of device memory, 256-byte
- * aligned, used by one call at a time; its first kilobytes are arrival
- * counters that must be zero before the first call and are zero after each.
+ * workspace: kv4_attention_workspace_size bytes of device memory (it does not
+ * grow with the batch, and is largest at 1024 rows), 256-byte aligned, used by
+ * one call at a time, replays of captured graphs included; its first kilobytes
+ * are arrival counters that must be zero before the first call and are zero
+ * after each.
  * On the device, slots, page ids and lengths outside the cache are not
  * followed: the row or page counts as absent (zeros), a length is cut, and
  * bit 1 of aljabr_blackwell_device_status is set.
@@ -410,7 +412,8 @@ int aljabr_blackwell_stream_capture_id(void* stream, unsigned long long* id);
  * history [rows][history_stride] with history_len[row] live entries, entries
  * outside [0, vocab) ignored; bias_tokens / bias_values [rows][bias_stride]
  * with bias_len[row]; allow [rows][allow_stride words].  history, bias_tokens,
- * allow and token may each be NULL.  Device pointers, stream-ordered.  No
+ * allow and token may each be NULL; rows at most 65535, vocab at most 2^28.
+ * Device pointers, stream-ordered.  No
  * counterpart in the reference's native code: its samplers run on the host. */
 int aljabr_blackwell_logits_process_dev(float* out, long long out_stride, const void* logits, int logits_dtype,
                                         long long logits_stride, int rows, int vocab, const int* history,
