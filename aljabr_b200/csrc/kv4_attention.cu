@@ -22,8 +22,8 @@
 //     exact in one column; their offset -8 is sum_g dK[p, g] * (-8 sum_{j in
 //     g} q_j), one more MMA with the fp16 scales as they are stored for its A
 //     operand.  fp32 queries take two columns, each a multiple of a fixed step
-//     of the row's group of 32 (2^-11 and 2^-23 of the group's largest value,
-//     so an element is off by at most 2^-23 of that).  Their groups' sums,
+//     of the row's group of 32 (at most 2^-10 and 2^-22 of the group's largest
+//     value, so an element is off by at most 2^-23 of that).  Their groups' sums,
 //     with the offset -8 sum_j q_j, are exact integers: neither the tensor
 //     cores' truncation nor an outlier in another group enters.  (One step for
 //     the whole row loses 1e-4 of the result where q has an outlier of 300;
