@@ -80,7 +80,9 @@ def new_output(shape, dtype, device, index: int, stream: int) -> torch.Tensor:
     the second is done with it."""
     if stream == current_stream(index):
         return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device)):
+    # torch reads an odd number, as the legacy stream's is, as one of its own streams
+    s = torch.cuda.default_stream(device) if stream == _LEGACY_STREAM else torch.cuda.ExternalStream(stream, device)
+    with torch.cuda.stream(s):
         t = torch.empty(shape, dtype=dtype, device=device)
     t.record_stream(torch.cuda.current_stream(device))
     return t

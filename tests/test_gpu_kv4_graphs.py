@@ -104,3 +104,12 @@ def test_calls_on_a_stream_of_their_own():
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(k, rows[0]) and torch.equal(v, rows[1])
         assert torch.equal(got, plain[0]) and torch.equal(token, plain[1]) and not copy.any()
+
+
+def test_the_legacy_stream_named_from_another_one():
+    cache, q, sl, table, want, _, _ = attend_case(35, 128, 2, 4, 1, 16, [4000, 100])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        out = cache.attend(q, sl, table, stream=1)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)

@@ -134,3 +134,19 @@ def test_a_window_that_an_int_does_not_hold(cache, monkeypatch, window, passed):
     cache.attend(*args, window=window, out=q)
     sent = ctypes.c_int(got[0]).value
     assert sent == passed if passed is not None else sent < 0
+
+
+def test_the_legacy_stream_s_outputs_come_from_the_default_stream_s_pool(cache, monkeypatch):
+    """Handle 1 names the legacy stream; torch takes an odd number for one of its own streams, not for a handle."""
+    asked = []
+
+    class Nothing:
+        __enter__ = __exit__ = lambda *a: None
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda s, device=None: asked.append(s))
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: asked.append("default"))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: None)
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: Nothing())
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: None)
+    cache.read(torch.zeros(3, dtype=torch.int32), stream=1)
+    cache.read(torch.zeros(3, dtype=torch.int32), stream=0x7f00)
+    assert asked == ["default"] * 2 + [0x7f00] * 2
