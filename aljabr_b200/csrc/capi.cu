@@ -582,6 +582,12 @@ int kv4_check_heads(int q_len, int q_heads, int kv_heads, int head_dim) {
     return ALJ_OK;
 }
 
+// Whether an address is no multiple of `bytes` (a power of two).
+template <typename... P>
+bool misaligned(uintptr_t bytes, P... p) {
+    return ((reinterpret_cast<uintptr_t>(p) | ...) & (bytes - 1)) != 0;
+}
+
 int kv4_align(uintptr_t bits) { return (bits & 31) == 0 ? 2 : (bits & 15) == 0 ? 1 : 0; }
 
 int kv4_rows(Kv4Rows* p, void* cache, int pages, int page_size, int kv_heads, int head_dim, int type, const int* slots,
@@ -594,8 +600,8 @@ int kv4_rows(Kv4Rows* p, void* cache, int pages, int page_size, int kv_heads, in
         return fail(ALJ_ERR_BAD_DIMS, "kv4: %d tokens x %d kv heads", tokens, kv_heads);
     if (tokens > 0 && (!cache || !slots)) return fail(ALJ_ERR_BAD_ARG, "kv4: null cache or slots");
     const uintptr_t out = reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out);
-    if ((reinterpret_cast<uintptr_t>(cache) & 15) || out % (type == ALJ_KV_BF16 ? 2 : 4))
-        return fail(ALJ_ERR_BAD_ARG, "kv4: cache must be 16-byte aligned, rows to their elements");
+    if (misaligned(16, cache) || misaligned(4, slots) || out % (type == ALJ_KV_BF16 ? 2 : 4))
+        return fail(ALJ_ERR_BAD_ARG, "kv4: cache must be 16-byte aligned, rows and slots to their elements");
     *p = Kv4Rows{};
     p->cache = static_cast<uint8_t*>(cache);
     p->pages = pages;
@@ -1464,8 +1470,8 @@ int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, lo
     const uintptr_t e = q_dtype == ALJ_KV_BF16 ? 2 : 4;
     if (q_stride < static_cast<long long>(q_heads) * head_dim)
         return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: q_stride %lld < q_heads * head_dim", q_stride);
-    if (reinterpret_cast<uintptr_t>(q) % e || ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(cache)) & 15))
-        return fail(ALJ_ERR_BAD_ARG, "kv4_attention: out and cache must be 16-byte aligned, q to its elements");
+    if (misaligned(e, q) || misaligned(16, out, cache) || misaligned(4, block_table, seq_lens))
+        return fail(ALJ_ERR_BAD_ARG, "kv4_attention: out and cache must be 16-byte aligned, q, block_table and seq_lens to their elements");
     int err = 0;
     DeviceState* st = state(&err);
     if (!st) return err;
@@ -1521,6 +1527,9 @@ int aljabr_blackwell_logits_process_dev(float* out, long long out_stride, const 
         return fail(ALJ_ERR_BAD_DIMS, "logits_process: strides %lld, %lld < vocab %d", out_stride, logits_stride, vocab);
     if (rows == 0) return ALJ_OK;
     if (!out || !logits) return fail(ALJ_ERR_BAD_ARG, "logits_process: null out or logits");
+    if (misaligned(4, out, history, history_len, penalties, bias_tokens, bias_values, bias_len, allow, token) ||
+        misaligned(logits_dtype == ALJ_KV_BF16 ? 2 : 4, logits))
+        return fail(ALJ_ERR_BAD_ARG, "logits_process: a buffer is not aligned to its elements");
     if (out == logits && (logits_dtype != ALJ_KV_F32 || out_stride != logits_stride))
         return fail(ALJ_ERR_BAD_ARG, "logits_process: in place needs fp32 logits and equal strides");
     if (history && (!history_len || !penalties || history_stride < 1))
