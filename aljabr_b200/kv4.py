@@ -74,21 +74,25 @@ def capture_id(stream: int) -> int:
     return got.value
 
 
+def torch_stream(stream: int, device):
+    """The handle as torch's object.  Torch reads an odd number, as the legacy stream's is, as one of its own streams."""
+    return torch.cuda.default_stream(device) if stream == _LEGACY_STREAM else torch.cuda.ExternalStream(stream, device)
+
+
 def new_output(shape, dtype, device, index: int, stream: int) -> torch.Tensor:
     """A tensor that a call on `stream` writes and that the caller reads on torch's current stream: of the allocator's
     pool of the first, so that no work pending on the second still uses its memory, and not given out again before
     the second is done with it."""
     if stream == current_stream(index):
         return torch.empty(shape, dtype=dtype, device=device)
-    # torch reads an odd number, as the legacy stream's is, as one of its own streams
-    s = torch.cuda.default_stream(device) if stream == _LEGACY_STREAM else torch.cuda.ExternalStream(stream, device)
-    with torch.cuda.stream(s):
+    with torch.cuda.stream(torch_stream(stream, device)):
         t = torch.empty(shape, dtype=dtype, device=device)
     t.record_stream(torch.cuda.current_stream(device))
     return t
 
 
 _captured = {}      # (device, stream) -> capture id, its workspaces
+_kept = []          # workspaces of captures on streams given by handle
 
 
 def dtype_id(t: torch.Tensor, what: str) -> int:
@@ -193,33 +197,35 @@ class Kv4Cache:
         kept as long as the cache, since kernels under way may hold its address."""
         have = self._buffers.get(stream)
         if have is None:
-            have = self._make_workspace(q_len, q_heads)
-            # zeroed on torch's current stream; another stream's kernels do not wait for that, so there the device is
-            # waited for, once
-            if stream != current_stream(self._index):
-                torch.cuda.synchronize(self.device)
-            self._buffers[stream] = have
+            have = self._buffers[stream] = self._make_workspace(q_len, q_heads, stream)
         got = self._work[stream, q_len, q_heads] = (have.data_ptr(), have.numel())
         return got
 
-    def _make_workspace(self, q_len: int, q_heads: int) -> torch.Tensor:
+    def _make_workspace(self, q_len: int, q_heads: int, stream: int) -> torch.Tensor:
+        """Made and zeroed on the stream whose kernels will use it."""
         need = self._work_size(q_len, q_heads, self.kv_heads, self.head_dim)   # the call's own, for its refusals
         if need < 0:
             native.check(int(need))
         most = self._work_size(native.KV4_MAX_ROWS, self.kv_heads, self.kv_heads, self.head_dim)
-        return torch.zeros(most, dtype=torch.uint8, device=self.device)
+        if stream == current_stream(self._index):
+            return torch.zeros(most, dtype=torch.uint8, device=self.device)
+        with torch.cuda.stream(torch_stream(stream, self.device)):
+            return torch.zeros(most, dtype=torch.uint8, device=self.device)
 
     def _captured_workspace(self, capture: int, q_len: int, q_heads: int, stream: int):
         """(address, bytes) for calls recorded into a graph.  Its zeroing is a node of that graph, which may run on any
         stream: so it belongs to this capture's calls on this stream (of all caches: they follow one another) and to
-        nothing else.  torch's graph keeps the memory; here it is held until the stream's next capture."""
+        nothing else.  torch's graph keeps the memory: here it is held until the stream's next capture, and for good
+        where the stream was given by its handle, since other means of capture keep nothing."""
         key = self._index, stream
         owner, have = _captured.get(key, (0, []))
         if owner != capture:
             _captured[key] = capture, (have := [])
         need = self._work_size(q_len, q_heads, self.kv_heads, self.head_dim)
         if not have or have[-1].numel() < need:
-            have.append(self._make_workspace(q_len, q_heads))
+            have.append(self._make_workspace(q_len, q_heads, stream))
+            if stream != current_stream(self._index):
+                _kept.append(have[-1])
         return have[-1].data_ptr(), have[-1].numel()
 
     def attend(self, q: torch.Tensor, seq_lens: torch.Tensor, block_table=None, window: int = 0, scale=None,

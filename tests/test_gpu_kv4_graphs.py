@@ -113,3 +113,24 @@ def test_the_legacy_stream_named_from_another_one():
         out = cache.attend(q, sl, table, stream=1)
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_a_captured_branch_on_a_stream_given_by_handle():
+    """Two branches of one graph, the second joined from a stream that the call names; cold, so that both make their
+    workspaces in the capture."""
+    cache, q, sl, table, want, _, _ = attend_case(36, 128, 2, 4, 1, 16, [4000, 9000])
+    outs, side, branch = (torch.zeros_like(q), torch.zeros_like(q)), torch.cuda.Stream(), torch.cuda.Stream()
+
+    def both():
+        branch.wait_stream(side)
+        cache.attend(q, sl, table, out=outs[0])
+        cache.attend(q, sl, table, out=outs[1], stream=branch.cuda_stream)
+        side.wait_stream(branch)
+
+    graph = capture(side, both)
+    for _ in range(5):
+        for out in outs:
+            out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want)

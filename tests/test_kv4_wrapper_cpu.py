@@ -2,6 +2,7 @@
 and torch's streams are stubs, the tensors live on the CPU."""
 import gc
 import weakref
+from contextlib import contextmanager
 
 import pytest
 
@@ -24,6 +25,15 @@ def cache(monkeypatch):
     monkeypatch.setattr(kv4, "current_stream", lambda index: 7)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: None)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda s, device=None: s)
+
+    @contextmanager
+    def switch(s):
+        c.at.append(s)
+        yield
+        c.at.pop()
+    c.at = [7]           # torch's current stream, as its context managers set it
+    monkeypatch.setattr(torch.cuda, "stream", switch)
     return c
 
 
@@ -81,7 +91,6 @@ def test_each_capture_has_a_workspace_of_its_own(cache, monkeypatch):
 def test_outputs_belong_to_the_stream_that_writes_them(cache, monkeypatch):
     """With `stream` given, an output from the allocator's pool of torch's current stream could be a block whose last
     reader there has not run yet; and its own readers there must keep it from being handed out again."""
-    from contextlib import contextmanager
     at, made, readers = [7], [], []
     real = torch.empty
 
@@ -150,3 +159,32 @@ def test_the_legacy_stream_s_outputs_come_from_the_default_stream_s_pool(cache, 
     cache.read(torch.zeros(3, dtype=torch.int32), stream=1)
     cache.read(torch.zeros(3, dtype=torch.int32), stream=0x7f00)
     assert asked == ["default"] * 2 + [0x7f00] * 2
+
+
+@pytest.mark.parametrize("capture", [0, 31])
+def test_a_workspace_is_zeroed_on_the_stream_that_uses_it(cache, monkeypatch, capture):
+    """In a capture, zeroing on another stream is a node of no graph or of an unordered branch; outside, a wait for the
+    whole device would be needed."""
+    zeroed, waits, real = [], [], torch.zeros
+    monkeypatch.setattr(kv4, "capture_id", lambda stream: capture)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capture != 0)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: waits.append(1))
+    monkeypatch.setattr(torch, "zeros", lambda *a, **kw: (zeroed.append(cache.at[-1]) if kw.get("dtype") is torch.uint8 else None,
+                                                          real(*a, **kw))[1])
+    kv4._captured.clear()
+    attend(cache)
+    attend(cache, stream=8)
+    assert zeroed == [7, 8] and waits == []
+
+
+def test_a_capture_named_by_its_stream_keeps_its_workspace(cache, monkeypatch):
+    """A stream given by handle may be captured by other means than torch's, whose graphs keep their memory."""
+    capture = 41
+    monkeypatch.setattr(kv4, "capture_id", lambda stream: capture)
+    kv4._captured.clear()
+    first = attend(cache, stream=8)
+    held = [weakref.ref(t) for t in kv4._captured[-1, 8][1]]
+    capture = 42
+    assert attend(cache, stream=8) != first
+    gc.collect()
+    assert held and all(t() is not None for t in held)
