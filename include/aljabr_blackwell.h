@@ -368,7 +368,8 @@ int aljabr_blackwell_gemm_q_dev(int type, int nseg, float* const* y, const int* 
  * Accuracy: sums and softmax statistics are fp32.  An fp32 query element
  * enters with an error of at most 2^-23 of the largest in its group of 32
  * dims (an outlier costs its own group's small values their last bits),
- * softmax weights with 2^-22 of themselves or 2^-28 of the largest V.  For
+ * softmax weights with 2^-22 of themselves or 2^-28 of the largest V.
+ * Queries of 2^115 and more leave its range and may give NaN.  For
  * bf16 queries the weights and their products with V's scales are rounded to
  * fp16 (2^-11 each), below the output's own rounding of 2^-9.
  * q_len * q_heads / kv_heads is at most 1024, batch at most 2048.  The results
