@@ -230,6 +230,22 @@ bool kv4_supported(int page_size, int kv_heads, int head_dim);
 long long kv4_cache_bytes(int pages, int page_size, int kv_heads, int head_dim);
 cudaError_t launch_kv4_append(const Kv4Rows& p, cudaStream_t stream);
 cudaError_t launch_kv4_read(const Kv4Rows& p, cudaStream_t stream);
+// Rows with the rotation of their positions on the way: q [tokens] rows of q_heads heads into q_out, k before it is
+// quantised.  rope: [rope_positions][half] of (cos, sin), half a multiple of 8; a token whose position is below zero is
+// absent (q_out zero, nothing stored).
+struct Kv4Rotate {
+    Kv4Rows rows;
+    const void* q;
+    void* q_out;
+    long long q_stride, q_out_stride;
+    int q_heads;
+    const int* positions;
+    const float2* rope;
+    int rope_positions, half, interleaved;
+    int vec_q, vec_q_out;    // as rows.vec
+    int span, splits;        // set by the launcher
+};
+cudaError_t launch_kv4_rotate_append(const Kv4Rotate& a, int sms, cudaStream_t stream);
 // One token of a decode step: RoPE on q (in place) and k, then k and v (fp32, 16-byte aligned) into page 0 at *p.slots.
 cudaError_t launch_kv4_rope_append(const Kv4Rows& p, float* q, const float2* rope, int q_heads, cudaStream_t stream);
 
@@ -237,6 +253,7 @@ cudaError_t launch_kv4_rope_append(const Kv4Rows& p, float* q, const float2* rop
 // group heads, q_stride elements apart; query t of sequence b sees positions
 // up to lens[b] + len_add - q_len + t (window > 0: the last `window` of them).
 constexpr int kKv4MaxBatch = 2048;
+constexpr int kKv4MaxNodes = 256;    // of a drafted tree
 constexpr int kKv4MaxRows = 1024;    // q_len * group: a chunk of a prompt belongs to the prefill attention
 struct Kv4Attn {
     void* out;               // [batch][q_len][kv_heads * group][head_dim], q's type
@@ -251,6 +268,8 @@ struct Kv4Attn {
     int len_add;
     int batch, q_len, window;
     float scale, soft_cap;
+    const int* parents;      // the q_len tokens are a tree (kv4.cuh): [batch] rows parents_stride apart (0: one for all); null: a chain
+    int parents_stride;
     // set by the launcher
     int row_tiles, page_shift;
     unsigned int group_magic;
@@ -258,7 +277,30 @@ struct Kv4Attn {
     float* part;
 };
 size_t kv4_attention_workspace_bytes(int q_rows, int head_dim, int sms);
+// for trees
+size_t kv4_tree_workspace_bytes(int q_rows, int head_dim, int sms);
 cudaError_t launch_kv4_attention(const Kv4Attn& a, void* workspace, int sms, cudaStream_t stream);
+
+// Acceptance of a drafted tree (kv4_accept.cu): along each sequence's tree from node 0 to the first child whose drafted
+// token is the one picked after its parent, and so on; the path's rows move to the tree's first positions in every cache.
+constexpr int kKv4MaxLayers = 256;
+struct Kv4Accept {
+    uint8_t* cache[kKv4MaxLayers];
+    int layers, pages, page_size, kv_heads, head_dim;
+    const int* table;        // as in Kv4Attn
+    int table_stride;
+    const int* lens;         // [batch] positions, the tree's `nodes` among them
+    int batch, nodes;
+    const int* parents;
+    int parents_stride;
+    const int* drafted;      // [batch][nodes]
+    const int* picked;       // [batch][nodes]
+    int* path;               // [batch][nodes], -1 behind its end
+    int* count;              // [batch]
+    int* token;              // [batch] picked after the path's last node, -1 where there is none
+    int* new_lens;           // [batch]
+};
+cudaError_t launch_kv4_accept(const Kv4Accept& a, cudaStream_t stream);
 
 // Logits step (logits.cu).
 struct LogitsArgs {

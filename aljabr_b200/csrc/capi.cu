@@ -617,6 +617,109 @@ int kv4_rows(Kv4Rows* p, void* cache, int pages, int page_size, int kv_heads, in
     return ALJ_OK;
 }
 
+// Rows that enter the cache: the checks and arguments of both appends.
+int kv4_append_rows(Kv4Rows* p, const char* what, void* cache, int pages, int page_size, int kv_heads, int head_dim,
+                    const void* k, const void* v, int type, long long k_stride, long long v_stride, const int* slots,
+                    int tokens, void* k_back, void* v_back) {
+    const int rc = kv4_rows(p, cache, pages, page_size, kv_heads, head_dim, type, slots, tokens, k_back, v_back);
+    if (rc) return rc;
+    if (!k_back != !v_back) return fail(ALJ_ERR_BAD_ARG, "%s: k_back and v_back go together", what);
+    if (tokens == 0) return ALJ_OK;
+    if (!k || !v) return fail(ALJ_ERR_BAD_ARG, "%s: null k or v", what);
+    const long long row = static_cast<long long>(kv_heads) * head_dim;
+    if (k_stride < row || v_stride < row)
+        return fail(ALJ_ERR_BAD_DIMS, "%s: strides %lld, %lld < kv_heads * head_dim = %lld", what, k_stride, v_stride, row);
+    const uintptr_t e = type == ALJ_KV_BF16 ? 2 : 4;
+    const uintptr_t kp = reinterpret_cast<uintptr_t>(k), vp = reinterpret_cast<uintptr_t>(v);
+    if ((kp | vp) % e) return fail(ALJ_ERR_BAD_ARG, "%s: k or v not aligned to its elements", what);
+    p->k = k;
+    p->v = v;
+    p->k_stride = k_stride;
+    p->v_stride = v_stride;
+    p->vec = kv4_align(kp | vp | static_cast<uintptr_t>(k_stride) * e | static_cast<uintptr_t>(v_stride) * e);
+    return ALJ_OK;
+}
+
+int kv4_check_tree_heads(int nodes, int q_heads, int kv_heads, int head_dim) {
+    if (nodes < 1 || nodes > kKv4MaxNodes)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4: trees have 1 to %d nodes, not %d", kKv4MaxNodes, nodes);
+    return kv4_check_heads(nodes, q_heads, kv_heads, head_dim);
+}
+
+int kv4_check_tree(int batch, const int* parents, int parents_stride, int nodes, const char* what) {
+    if (nodes < 1 || nodes > kKv4MaxNodes)
+        return fail(ALJ_ERR_BAD_DIMS, "%s: trees have 1 to %d nodes, not %d", what, kKv4MaxNodes, nodes);
+    if (batch < 0 || batch > kKv4MaxBatch)
+        return fail(ALJ_ERR_BAD_DIMS, "%s: batch %d outside [0, %d]", what, batch, kKv4MaxBatch);
+    if (batch == 0) return ALJ_OK;
+    if (!parents || misaligned(4, parents)) return fail(ALJ_ERR_BAD_ARG, "%s: parents must be device integers", what);
+    if (parents_stride != 0 && parents_stride < nodes)
+        return fail(ALJ_ERR_BAD_DIMS, "%s: parents_stride %d is neither 0 (one tree for all) nor at least %d", what, parents_stride, nodes);
+    return ALJ_OK;
+}
+
+// Attention over the 4-bit cache: a chain of q_len tokens, or with `parents` a tree of them.
+int kv4_attend(const char* what, void* out, const void* q, int q_dtype, long long q_stride, const void* cache, int pages,
+               int page_size, int kv_heads, int head_dim, const int* block_table, int table_stride, const int* seq_lens,
+               int batch, const int* parents, int parents_stride, int q_len, int q_heads, int window, float scale,
+               float soft_cap, void* workspace, long long workspace_bytes, void* stream) {
+    int rc = kv4_check_cache(pages, page_size, kv_heads, head_dim);
+    if (rc) return rc;
+    rc = parents ? kv4_check_tree_heads(q_len, q_heads, kv_heads, head_dim) : kv4_check_heads(q_len, q_heads, kv_heads, head_dim);
+    if (rc) return rc;
+    if (q_dtype != ALJ_KV_F32 && q_dtype != ALJ_KV_BF16)
+        return fail(ALJ_ERR_UNSUPPORTED, "%s: q type %d (ALJ_KV_F32 or ALJ_KV_BF16)", what, q_dtype);
+    if (batch < 0 || batch > kKv4MaxBatch)
+        return fail(ALJ_ERR_BAD_DIMS, "%s: batch %d outside [0, %d]", what, batch, kKv4MaxBatch);
+    if (window < 0) return fail(ALJ_ERR_BAD_ARG, "%s: window %d < 0", what, window);
+    if (!(soft_cap == 0.0f || (soft_cap >= 1e-30f && soft_cap <= 1e30f)))   // its reciprocal is used
+        return fail(ALJ_ERR_BAD_ARG, "%s: soft_cap %g is neither 0 (none) nor in [1e-30, 1e30]", what, soft_cap);
+    if (batch == 0) return ALJ_OK;
+    if (!out || !q || !cache || !seq_lens || !workspace) return fail(ALJ_ERR_BAD_ARG, "%s: null pointer", what);
+    if (block_table ? table_stride < 1 : batch > pages)
+        return fail(ALJ_ERR_BAD_DIMS, "%s: table_stride %d, batch %d, pages %d", what, table_stride, batch, pages);
+    // the chunks of all sequences at their longest, which the kernel counts in 32 bits
+    const long long cap = block_table ? static_cast<long long>(table_stride) * page_size : page_size;
+    const long long items = kv_heads * (static_cast<long long>(q_len) * (q_heads / kv_heads) / 4 + 1);
+    if (static_cast<long long>(batch) * (cap / 128 + 4) > 0x7fffffffLL / items)
+        return fail(ALJ_ERR_BAD_DIMS, "%s: %d sequences of up to %lld positions x %d kv heads are too many", what, batch, cap,
+                    kv_heads);
+    const uintptr_t e = q_dtype == ALJ_KV_BF16 ? 2 : 4;
+    if (q_stride < static_cast<long long>(q_heads) * head_dim)
+        return fail(ALJ_ERR_BAD_DIMS, "%s: q_stride %lld < q_heads * head_dim", what, q_stride);
+    if (misaligned(e, q) || misaligned(16, out, cache) || misaligned(4, block_table, seq_lens))
+        return fail(ALJ_ERR_BAD_ARG, "%s: out and cache must be 16-byte aligned, q, block_table and seq_lens to their elements", what);
+    int err = 0;
+    DeviceState* st = state(&err);
+    if (!st) return err;
+    const int rows = q_len * (q_heads / kv_heads);
+    const size_t need = parents ? kv4_tree_workspace_bytes(rows, head_dim, st->sms) : kv4_attention_workspace_bytes(rows, head_dim, st->sms);
+    if (workspace_bytes < static_cast<long long>(need) || (reinterpret_cast<uintptr_t>(workspace) & 255))
+        return fail(ALJ_ERR_BAD_ARG, "%s: workspace %lld bytes (need %zu, 256-byte aligned)", what, workspace_bytes, need);
+    Kv4Attn a = {};
+    a.out = out;
+    a.q = q;
+    a.q_stride = q_stride;
+    a.type = q_dtype;
+    a.cache = static_cast<const uint8_t*>(cache);
+    a.pages = pages;
+    a.page_size = page_size;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.group = q_heads / kv_heads;
+    a.table = block_table;
+    a.table_stride = table_stride;
+    a.lens = seq_lens;
+    a.batch = batch;
+    a.q_len = q_len;
+    a.window = window;
+    a.scale = scale;
+    a.soft_cap = soft_cap;
+    a.parents = parents;
+    a.parents_stride = parents_stride;
+    return launch_status(launch_kv4_attention(a, workspace, st->sms, pick_stream(st, stream)), what);
+}
+
 // The binding's elementwise glue (rmsnorm, silu_ffn): operands that are
 // device, managed or registered memory are used in place; plain host
 // operands are staged through the device scratch.  Blocks until out is
@@ -1398,22 +1501,9 @@ int aljabr_blackwell_kv4_append_dev(void* cache, int pages, int page_size, int k
                                     const void* v, int kv_dtype, long long k_stride, long long v_stride,
                                     const int* slots, int tokens, void* k_back, void* v_back, void* stream) {
     Kv4Rows p;
-    const int rc = kv4_rows(&p, cache, pages, page_size, kv_heads, head_dim, kv_dtype, slots, tokens, k_back, v_back);
-    if (rc) return rc;
-    if (!k_back != !v_back) return fail(ALJ_ERR_BAD_ARG, "kv4_append: k_back and v_back go together");
-    if (tokens == 0) return ALJ_OK;
-    if (!k || !v) return fail(ALJ_ERR_BAD_ARG, "kv4_append: null k or v");
-    const long long row = static_cast<long long>(kv_heads) * head_dim;
-    if (k_stride < row || v_stride < row)
-        return fail(ALJ_ERR_BAD_DIMS, "kv4_append: strides %lld, %lld < kv_heads * head_dim = %lld", k_stride, v_stride, row);
-    const uintptr_t e = kv_dtype == ALJ_KV_BF16 ? 2 : 4;
-    const uintptr_t kp = reinterpret_cast<uintptr_t>(k), vp = reinterpret_cast<uintptr_t>(v);
-    if ((kp | vp) % e) return fail(ALJ_ERR_BAD_ARG, "kv4_append: k or v not aligned to its elements");
-    p.k = k;
-    p.v = v;
-    p.k_stride = k_stride;
-    p.v_stride = v_stride;
-    p.vec = kv4_align(kp | vp | static_cast<uintptr_t>(k_stride) * e | static_cast<uintptr_t>(v_stride) * e);
+    const int rc = kv4_append_rows(&p, "kv4_append", cache, pages, page_size, kv_heads, head_dim, k, v, kv_dtype, k_stride,
+                                   v_stride, slots, tokens, k_back, v_back);
+    if (rc || tokens == 0) return rc;
     int err = 0;
     DeviceState* st = state(&err);
     if (!st) return err;
@@ -1446,58 +1536,130 @@ int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, lo
                                        int table_stride, const int* seq_lens, int batch, int q_len, int q_heads,
                                        int window, float scale, float soft_cap, void* workspace,
                                        long long workspace_bytes, void* stream) {
-    int rc = kv4_check_cache(pages, page_size, kv_heads, head_dim);
+    return kv4_attend("kv4_attention", out, q, q_dtype, q_stride, cache, pages, page_size, kv_heads, head_dim, block_table,
+                      table_stride, seq_lens, batch, nullptr, 0, q_len, q_heads, window, scale, soft_cap, workspace,
+                      workspace_bytes, stream);
+}
+
+long long aljabr_blackwell_kv4_tree_attention_workspace_size(int nodes, int q_heads, int kv_heads, int head_dim) {
+    const int rc = kv4_check_tree_heads(nodes, q_heads, kv_heads, head_dim);
     if (rc) return rc;
-    rc = kv4_check_heads(q_len, q_heads, kv_heads, head_dim);
+    const int sms = sm_count_for_current_device();
+    return static_cast<long long>(kv4_tree_workspace_bytes(nodes * (q_heads / kv_heads), head_dim, sms));
+}
+
+int aljabr_blackwell_kv4_tree_attention_dev(void* out, const void* q, int q_dtype, long long q_stride, const void* cache,
+                                            int pages, int page_size, int kv_heads, int head_dim, const int* block_table,
+                                            int table_stride, const int* seq_lens, int batch, const int* parents,
+                                            int parents_stride, int nodes, int q_heads, int window, float scale,
+                                            float soft_cap, void* workspace, long long workspace_bytes, void* stream) {
+    const int rc = kv4_check_tree(batch, parents, parents_stride, nodes, "kv4_tree_attention");
     if (rc) return rc;
-    if (q_dtype != ALJ_KV_F32 && q_dtype != ALJ_KV_BF16)
-        return fail(ALJ_ERR_UNSUPPORTED, "kv4_attention: q type %d (ALJ_KV_F32 or ALJ_KV_BF16)", q_dtype);
-    if (batch < 0 || batch > kKv4MaxBatch)
-        return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: batch %d outside [0, %d]", batch, kKv4MaxBatch);
-    if (window < 0) return fail(ALJ_ERR_BAD_ARG, "kv4_attention: window %d < 0", window);
-    if (!(soft_cap == 0.0f || (soft_cap >= 1e-30f && soft_cap <= 1e30f)))   // its reciprocal is used
-        return fail(ALJ_ERR_BAD_ARG, "kv4_attention: soft_cap %g is neither 0 (none) nor in [1e-30, 1e30]", soft_cap);
-    if (batch == 0) return ALJ_OK;
-    if (!out || !q || !cache || !seq_lens || !workspace) return fail(ALJ_ERR_BAD_ARG, "kv4_attention: null pointer");
-    if (block_table ? table_stride < 1 : batch > pages)
-        return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: table_stride %d, batch %d, pages %d", table_stride, batch, pages);
-    // the chunks of all sequences at their longest, which the kernel counts in 32 bits
-    const long long cap = block_table ? static_cast<long long>(table_stride) * page_size : page_size;
-    const long long items = kv_heads * (static_cast<long long>(q_len) * (q_heads / kv_heads) / 4 + 1);
-    if (static_cast<long long>(batch) * (cap / 128 + 4) > 0x7fffffffLL / items)
-        return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: %d sequences of up to %lld positions x %d kv heads are too many", batch, cap,
-                    kv_heads);
-    const uintptr_t e = q_dtype == ALJ_KV_BF16 ? 2 : 4;
-    if (q_stride < static_cast<long long>(q_heads) * head_dim)
-        return fail(ALJ_ERR_BAD_DIMS, "kv4_attention: q_stride %lld < q_heads * head_dim", q_stride);
-    if (misaligned(e, q) || misaligned(16, out, cache) || misaligned(4, block_table, seq_lens))
-        return fail(ALJ_ERR_BAD_ARG, "kv4_attention: out and cache must be 16-byte aligned, q, block_table and seq_lens to their elements");
+    return kv4_attend("kv4_tree_attention", out, q, q_dtype, q_stride, cache, pages, page_size, kv_heads, head_dim,
+                      block_table, table_stride, seq_lens, batch, parents, parents_stride, nodes, q_heads, window, scale,
+                      soft_cap, workspace, workspace_bytes, stream);
+}
+
+int aljabr_blackwell_kv4_rotate_append_dev(void* cache, int pages, int page_size, int kv_heads, int head_dim, void* q_out,
+                                           long long q_out_stride, const void* q, const void* k, const void* v,
+                                           int kv_dtype, long long q_stride, long long k_stride, long long v_stride,
+                                           int q_heads, const int* slots, const int* positions, const float* rope,
+                                           int rope_positions, int rotary_dim, int interleaved, int tokens, void* k_back,
+                                           void* v_back, void* stream) {
+    Kv4Rotate p = {};
+    int rc = kv4_append_rows(&p.rows, "kv4_rotate_append", cache, pages, page_size, kv_heads, head_dim, k, v, kv_dtype,
+                             k_stride, v_stride, slots, tokens, k_back, v_back);
+    if (rc) return rc;
+    if (q_heads < 1 || (static_cast<long long>(q_heads) + kv_heads) * std::max(tokens, 1) > 0x7fffffffLL - 32)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4_rotate_append: %d query heads x %d tokens", q_heads, tokens);
+    if (rope_positions < 1 || rotary_dim < 16 || rotary_dim > head_dim || rotary_dim % 16)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4_rotate_append: %d positions, rotary_dim %d (a multiple of 16 up to head_dim %d)",
+                    rope_positions, rotary_dim, head_dim);
+    if (tokens == 0) return ALJ_OK;
+    if (!q || !q_out || !positions || !rope) return fail(ALJ_ERR_BAD_ARG, "kv4_rotate_append: null q, q_out, positions or rope");
+    const long long row = static_cast<long long>(q_heads) * head_dim;
+    if (q_stride < row || q_out_stride < row)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4_rotate_append: strides %lld, %lld < q_heads * head_dim = %lld", q_stride, q_out_stride, row);
+    const uintptr_t e = kv_dtype == ALJ_KV_BF16 ? 2 : 4;
+    if (misaligned(e, q, q_out) || misaligned(4, positions) || misaligned(16, rope))
+        return fail(ALJ_ERR_BAD_ARG, "kv4_rotate_append: q, q_out and positions must be aligned to their elements, rope to 16 bytes");
+    p.q = q;
+    p.q_out = q_out;
+    p.q_stride = q_stride;
+    p.q_out_stride = q_out_stride;
+    p.q_heads = q_heads;
+    p.positions = positions;
+    p.rope = reinterpret_cast<const float2*>(rope);
+    p.rope_positions = rope_positions;
+    p.half = rotary_dim / 2;
+    p.interleaved = interleaved != 0;
+    p.vec_q = kv4_align(reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(q_stride) * e);
+    p.vec_q_out = kv4_align(reinterpret_cast<uintptr_t>(q_out) | static_cast<uintptr_t>(q_out_stride) * e);
     int err = 0;
     DeviceState* st = state(&err);
     if (!st) return err;
-    const size_t need = kv4_attention_workspace_bytes(q_len * (q_heads / kv_heads), head_dim, st->sms);
-    if (workspace_bytes < static_cast<long long>(need) || (reinterpret_cast<uintptr_t>(workspace) & 255))
-        return fail(ALJ_ERR_BAD_ARG, "kv4_attention: workspace %lld bytes (need %zu, 256-byte aligned)", workspace_bytes, need);
-    Kv4Attn a = {};
-    a.out = out;
-    a.q = q;
-    a.q_stride = q_stride;
-    a.type = q_dtype;
-    a.cache = static_cast<const uint8_t*>(cache);
+    return launch_status(launch_kv4_rotate_append(p, st->sms, pick_stream(st, stream)), "kv4_rotate_append");
+}
+
+int aljabr_blackwell_kv4_accept_tree_dev(int* path, int* count, int* token, int* new_lens, void* const* caches, int layers,
+                                         int pages, int page_size, int kv_heads, int head_dim, const int* block_table,
+                                         int table_stride, const int* seq_lens, int batch, const int* parents,
+                                         int parents_stride, int nodes, const int* drafted, const int* picked,
+                                         void* stream) {
+    int rc = kv4_check_cache(pages, page_size, kv_heads, head_dim);
+    if (rc) return rc;
+    rc = kv4_check_tree(batch, parents, parents_stride, nodes, "kv4_accept_tree");
+    if (rc) return rc;
+    if (layers < 1 || layers > kKv4MaxLayers)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4_accept_tree: %d layers (1 to %d)", layers, kKv4MaxLayers);
+    if (batch == 0) return ALJ_OK;
+    if (!path || !count || !token || !new_lens || !caches || !seq_lens || !drafted || !picked)
+        return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: null pointer");
+    if (block_table ? table_stride < 1 : batch > pages)
+        return fail(ALJ_ERR_BAD_DIMS, "kv4_accept_tree: table_stride %d, batch %d, pages %d", table_stride, batch, pages);
+    if (misaligned(4, path, count, token, new_lens, block_table, seq_lens, drafted, picked))
+        return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: integers must be aligned to their elements");
+    // every layer's blocks walk for themselves while the first one's write: an output must not be an input
+    const long long all = static_cast<long long>(batch) * nodes;
+    const int* const outs[4] = {path, count, token, new_lens};
+    const long long out_n[4] = {all, batch, batch, batch};
+    const int* const ins[5] = {seq_lens, parents, drafted, picked, block_table};
+    const long long in_n[5] = {batch, static_cast<long long>(parents_stride) * (batch - 1) + nodes, all, all,
+                               static_cast<long long>(table_stride) * batch};
+    for (int o = 0; o < 4; ++o)
+        for (int i = 0; i < 5; ++i)
+            if (ins[i] && outs[o] < ins[i] + in_n[i] && ins[i] < outs[o] + out_n[o])
+                return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: outputs must not overlap the inputs");
+    Kv4Accept a = {};
+    for (int l = 0; l < layers; ++l) {
+        if (!caches[l] || misaligned(16, caches[l]))
+            return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: cache %d must be a 16-byte aligned device address", l);
+        for (int m = 0; m < l; ++m)
+            if (a.cache[m] == caches[l]) return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: caches %d and %d are the same", m, l);
+        a.cache[l] = static_cast<uint8_t*>(caches[l]);
+    }
+    a.layers = layers;
     a.pages = pages;
     a.page_size = page_size;
     a.kv_heads = kv_heads;
     a.head_dim = head_dim;
-    a.group = q_heads / kv_heads;
     a.table = block_table;
     a.table_stride = table_stride;
     a.lens = seq_lens;
     a.batch = batch;
-    a.q_len = q_len;
-    a.window = window;
-    a.scale = scale;
-    a.soft_cap = soft_cap;
-    return launch_status(launch_kv4_attention(a, workspace, st->sms, pick_stream(st, stream)), "kv4_attention");
+    a.nodes = nodes;
+    a.parents = parents;
+    a.parents_stride = parents_stride;
+    a.drafted = drafted;
+    a.picked = picked;
+    a.path = path;
+    a.count = count;
+    a.token = token;
+    a.new_lens = new_lens;
+    int err = 0;
+    DeviceState* st = state(&err);
+    if (!st) return err;
+    return launch_status(launch_kv4_accept(a, pick_stream(st, stream)), "kv4_accept_tree");
 }
 
 int aljabr_blackwell_stream_capture_id(void* stream, unsigned long long* id) {

@@ -98,6 +98,20 @@ struct Where {          // one thread's place: token, head, 8 dims 8 j ..
     int off;            // position in the page
 };
 
+// The block of w.head in the slot's page, -1 for none.
+template <int D>
+__device__ __forceinline__ void find_block(const Kv4Rows& p, int slot, Where& w) {
+    w.block = -1;
+    if (slot < 0) return;
+    const int page = p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
+    if (page >= p.pages) {
+        record_fault(ALJ_FAULT_BOUNDS);
+        return;
+    }
+    w.off = slot - page * p.page_size;
+    w.block = (static_cast<long long>(page) * p.kv_heads + w.head) * kv4_block_bytes(p.page_size, D);
+}
+
 template <int D>
 __device__ __forceinline__ bool place(const Kv4Rows& p, Where& w) {
     constexpr int kLanes = D / 8;
@@ -105,17 +119,11 @@ __device__ __forceinline__ bool place(const Kv4Rows& p, Where& w) {
     w.j = threadIdx.x % kLanes;
     w.token = row / static_cast<unsigned int>(p.kv_heads);
     w.head = row - w.token * p.kv_heads;
-    w.block = -1;
-    if (w.token >= p.tokens) return false;         // whole rows, so whole quads
-    const int slot = __ldg(p.slots + w.token);
-    if (slot < 0) return true;
-    const int page = p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
-    if (page >= p.pages) {
-        record_fault(ALJ_FAULT_BOUNDS);
-        return true;
+    if (w.token >= p.tokens) {                     // whole rows, so whole quads
+        w.block = -1;
+        return false;
     }
-    w.off = slot - page * p.page_size;
-    w.block = (static_cast<long long>(page) * p.kv_heads + w.head) * kv4_block_bytes(p.page_size, D);
+    find_block<D>(p, __ldg(p.slots + w.token), w);
     return true;
 }
 
@@ -161,22 +169,12 @@ __device__ __forceinline__ Group group_of(const float (&x)[8]) {
     return g;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kRowThreads, 12) kv4_append_kernel(const Kv4Rows p) {
-    pdl_launch_dependents();
-    pdl_wait();
+// Quantises a thread's 8 dims of K and of V and stores them at w where `write`; k and v become the values that the
+// codes stand for.  Every lane of the warp takes part.
+template <int D>
+__device__ __forceinline__ void put8(const Kv4Rows& p, const Where& w, bool write, float (&k)[8], float (&v)[8]) {
     constexpr int NG = D / 32;
-    Where w;
-    const bool live = place<D>(p, w);
     const int g = w.j >> 2, c = w.j & 3;
-    float k[8] = {}, v[8] = {};
-    const bool write = live && w.block >= 0;
-    if (write) {
-        const int col = w.head * D + 8 * w.j;
-        Wide<T>::load(static_cast<const T*>(p.k) + w.token * p.k_stride + col, p.vec, k);
-        Wide<T>::load(static_cast<const T*>(p.v) + w.token * p.v_stride + col, p.vec, v);
-    }
-    // every lane takes part in the shuffles below; a skipped row's zeros are not stored
     const Group gk = group_of(k), gv = group_of(v);
     const uint32_t kw = encode8(k, kv4_inverse(gk.d), __half2float(gk.d), gk.finite);
     const uint32_t vw = encode8(v, kv4_inverse(gv.d), __half2float(gv.d), gv.finite);
@@ -194,6 +192,22 @@ __global__ void __launch_bounds__(kRowThreads, 12) kv4_append_kernel(const Kv4Ro
         if (c == 0) sc[w.off * static_cast<long long>(NG) + g] = gk.d;
         if (c == 1) sc[(static_cast<long long>(p.page_size) + w.off) * NG + g] = gv.d;
     }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowThreads, 12) kv4_append_kernel(const Kv4Rows p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    Where w;
+    const bool live = place<D>(p, w);
+    float k[8] = {}, v[8] = {};
+    const bool write = live && w.block >= 0;
+    if (write) {
+        const int col = w.head * D + 8 * w.j;
+        Wide<T>::load(static_cast<const T*>(p.k) + w.token * p.k_stride + col, p.vec, k);
+        Wide<T>::load(static_cast<const T*>(p.v) + w.token * p.v_stride + col, p.vec, v);
+    }
+    put8<D>(p, w, write, k, v);                    // a skipped row's zeros are not stored
     if (live && p.k_out) {                         // a skipped row's zeros stand for zeros
         const long long at = (static_cast<long long>(w.token) * p.kv_heads + w.head) * D + 8 * w.j;
         Wide<T>::store(static_cast<T*>(p.k_out) + at, p.vec_out, k);
@@ -226,6 +240,91 @@ __global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(const Kv4Rows p) 
     const long long at = (static_cast<long long>(w.token) * p.kv_heads + w.head) * D + 8 * w.j;
     if (p.k_out) Wide<T>::store(static_cast<T*>(p.k_out) + at, p.vec_out, k);
     if (p.v_out) Wide<T>::store(static_cast<T*>(p.v_out) + at, p.vec_out, v);
+}
+
+// Rows of new tokens with the position rotation on the way: q is rotated into q_out, k before it is quantised.  A
+// thread owns 8 consecutive dims of a head, as above; the dims they pair with are its own (interleaved) or another
+// lane's of the same row (split halves: one shuffle a value).  A CTA stays with one token for p.span units a row of
+// threads, a unit being a q head or a kv head's K and V, so that the token's cosines and sines are loaded once.
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowThreads) kv4_rotate_append_kernel(const Kv4Rotate p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    constexpr int kLanes = D / 8, kSlots = kRowThreads / kLanes;
+    Where w;
+    w.token = blockIdx.x / p.splits;
+    w.j = threadIdx.x % kLanes;
+    const int first = (blockIdx.x - w.token * p.splits) * (p.span * kSlots) + threadIdx.x / kLanes;
+    const int units = p.q_heads + p.rows.kv_heads;
+    int pos = __ldg(p.positions + w.token);
+    const int slot = __ldg(p.rows.slots + w.token);
+    if (pos >= p.rope_positions) {
+        record_fault(ALJ_FAULT_BOUNDS);
+        pos = -1;
+    }
+    // this thread's pairs: 8 (split halves) or 4 (interleaved) of (cos, sin)
+    const int half8 = p.half >> 3;                 // lanes of one half of the rotated dims
+    const bool turns = w.j < 2 * half8 && pos >= 0;
+    const bool second = !p.interleaved && w.j >= half8;
+    float cs[8], sn[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cs[i] = 1.0f, sn[i] = 0.0f;
+    if (turns) {
+        const int pair = p.interleaved ? 4 * w.j : 8 * (second ? w.j - half8 : w.j);
+        const float4* row = reinterpret_cast<const float4*>(p.rope + static_cast<long long>(pos) * p.half + pair);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i >= 2 && p.interleaved) break;
+            const float4 t = __ldg(row + i);
+            cs[2 * i] = t.x, sn[2 * i] = t.y, cs[2 * i + 1] = t.z, sn[2 * i + 1] = t.w;
+        }
+    }
+    const int lane = threadIdx.x & 31;
+    const int partner = turns && !p.interleaved ? lane + (second ? -half8 : half8) : lane;
+    auto turn = [&](float (&x)[8]) {               // products and sums rounded one by one, as in the decode step
+        if (p.interleaved) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = x[2 * i], b = x[2 * i + 1];
+                if (turns) {
+                    x[2 * i] = __fsub_rn(__fmul_rn(a, cs[i]), __fmul_rn(b, sn[i]));
+                    x[2 * i + 1] = __fadd_rn(__fmul_rn(a, sn[i]), __fmul_rn(b, cs[i]));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float other = __fmul_rn(__shfl_sync(0xffffffffu, x[i], partner), sn[i]), own = __fmul_rn(x[i], cs[i]);
+                if (turns) x[i] = second ? __fadd_rn(other, own) : __fsub_rn(own, other);
+            }
+        }
+    };
+    for (int s = 0; s < p.span; ++s) {
+        const int unit = first + s * kSlots;
+        const bool is_q = unit < p.q_heads, live = unit < units;
+        if (!__any_sync(0xffffffffu, live)) break;
+        w.head = unit - p.q_heads;
+        w.block = -1;
+        if (live && !is_q && pos >= 0) find_block<D>(p.rows, slot, w);
+        const bool write = w.block >= 0;
+        float x[8] = {}, v[8] = {};
+        if (live && is_q && pos >= 0)
+            Wide<T>::load(static_cast<const T*>(p.q) + w.token * p.q_stride + unit * D + 8 * w.j, p.vec_q, x);
+        if (write) {
+            const int col = w.head * D + 8 * w.j;
+            Wide<T>::load(static_cast<const T*>(p.rows.k) + w.token * p.rows.k_stride + col, p.rows.vec, x);
+            Wide<T>::load(static_cast<const T*>(p.rows.v) + w.token * p.rows.v_stride + col, p.rows.vec, v);
+        }
+        turn(x);
+        if (live && is_q) Wide<T>::store(static_cast<T*>(p.q_out) + w.token * p.q_out_stride + unit * D + 8 * w.j, p.vec_q_out, x);
+        if (!__any_sync(0xffffffffu, live && !is_q)) continue;
+        put8<D>(p.rows, w, write, x, v);
+        if (live && !is_q && p.rows.k_out) {
+            const long long at = (static_cast<long long>(w.token) * p.rows.kv_heads + w.head) * D + 8 * w.j;
+            Wide<T>::store(static_cast<T*>(p.rows.k_out) + at, p.rows.vec_out, x);
+            Wide<T>::store(static_cast<T*>(p.rows.v_out) + at, p.rows.vec_out, v);
+        }
+    }
 }
 
 // Decode step: split-half RoPE of one token's q and k heads (the products and
@@ -324,6 +423,31 @@ cudaError_t launch_read(const Kv4Rows& p, cudaStream_t stream) {
 
 cudaError_t launch_kv4_append(const Kv4Rows& p, cudaStream_t stream) {
     return p.type == ALJ_KV_BF16 ? launch_append<__nv_bfloat16>(p, stream) : launch_append<float>(p, stream);
+}
+
+cudaError_t launch_kv4_rotate_append(const Kv4Rotate& a, int sms, cudaStream_t stream) {
+    Kv4Rotate p = a;
+    p.rows.page_shift = (p.rows.page_size & (p.rows.page_size - 1)) == 0 ? __builtin_ctz(p.rows.page_size) : -1;
+    const int slots = kRowThreads / (p.rows.head_dim / 8), units = p.q_heads + p.rows.kv_heads;
+    const int most = (units + slots - 1) / slots;
+    // a CTA a token where those fill the GPU, else one for every `slots` heads
+    p.span = p.rows.tokens >= 4 * sms ? most : 1;
+    p.splits = (most + p.span - 1) / p.span;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned int>(p.rows.tokens) * p.splits);
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const bool bf16 = p.rows.type == ALJ_KV_BF16;
+    auto pick = [&](auto wide, auto narrow) { return bf16 ? narrow : wide; };
+    auto kernel = p.rows.head_dim == 64    ? pick(kv4_rotate_append_kernel<float, 64>, kv4_rotate_append_kernel<__nv_bfloat16, 64>)
+                  : p.rows.head_dim == 128 ? pick(kv4_rotate_append_kernel<float, 128>, kv4_rotate_append_kernel<__nv_bfloat16, 128>)
+                                           : pick(kv4_rotate_append_kernel<float, 256>, kv4_rotate_append_kernel<__nv_bfloat16, 256>);
+    return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 cudaError_t launch_kv4_read(const Kv4Rows& p, cudaStream_t stream) {

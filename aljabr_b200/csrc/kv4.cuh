@@ -52,4 +52,28 @@ __device__ __forceinline__ float kv4_value(uint32_t c, float d) {
     return __fadd_rn(__fmul_rn(static_cast<float>(static_cast<int>(c) - 8), d), 0.0f);
 }
 
+// ---------------------------------------------------------------- trees of drafted tokens
+// A tree of up to kKv4MaxNodes nodes is given by parents[t] < t: -1 for a
+// root, -2 for a node that is absent, as is one whose parent is.  Anything else
+// is no tree: the node counts as absent and a fault is recorded.
+constexpr int kKv4TreeWords = kKv4MaxNodes / 32;
+
+__device__ __forceinline__ int tree_parent(const int* parents, int t) {
+    const int up = __ldg(parents + t);
+    if (up >= -2 && up < t) return up;
+    record_fault(ALJ_FAULT_BOUNDS);
+    return -2;
+}
+__device__ __forceinline__ bool tree_sees(const uint32_t* words, int node) { return (words[node >> 5] >> (node & 31)) & 1u; }
+// Depth of node t, itself counted (0: absent); see: bits of the last `window` nodes of its path (0: of all of it).
+__device__ __forceinline__ int tree_chain(const int* parents, int t, int window, uint32_t* see) {
+    for (int i = 0; i < kKv4TreeWords; ++i) see[i] = 0u;
+    int depth = 0;
+    for (; t >= 0; t = parents[t], ++depth)        // parents come first: at most t steps
+        if (window == 0 || depth < window) see[t >> 5] |= 1u << (t & 31);
+    if (t == -1) return depth;
+    for (int i = 0; i < kKv4TreeWords; ++i) see[i] = 0u;
+    return 0;
+}
+
 }  // namespace alj

@@ -145,6 +145,7 @@ __device__ __forceinline__ uint32_t hide(uint32_t v) {
 // Four outputs sum * inv at element `to`, one rounding where the type is bf16.
 __device__ __forceinline__ void store4(void* out, bool bf16, long long to, float4 sum, float inv) {
     sum.x *= inv; sum.y *= inv; sum.z *= inv; sum.w *= inv;
+    if (inv == 0.0f) sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // a row that sees nothing, whatever its sums are
     if (bf16) {
         const __nv_bfloat162 a = __floats2bfloat162_rn(sum.x, sum.y), b = __floats2bfloat162_rn(sum.z, sum.w);
         *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(out) + to) =
@@ -284,7 +285,9 @@ __device__ __forceinline__ void load_chunk(const Kv4Attn& p, const TileSource& t
     }
 }
 
-template <int NG, int CT, int PARTS>
+// TREE: the q_len new tokens are the nodes of a drafted tree (p.parents): a row sees the positions before the tree, its
+// node's ancestors and its node.
+template <int NG, int CT, int PARTS, bool TREE>
 __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kernel(const Kv4Attn p) {
     using F = Cfg<NG, CT, PARTS>;
     constexpr int D = F::D, ROWS = F::ROWS, COLS = F::COLS;
@@ -304,6 +307,9 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     int* const s_misc = s_hi + COLS;
     int* const s_pre = s_misc + 8;
     int* const s_len = s_pre + p.batch + 1;
+    int* const s_par = s_len + p.batch;                                 // TREE: [node] the sequence's parents,
+    uint32_t* const s_see = reinterpret_cast<uint32_t*>(s_par + kKv4MaxNodes);   // [column] bits of the nodes its row sees,
+    uint32_t* const s_any = s_see + COLS * kKv4TreeWords;               // their union, and the first row's position
 
     const int warp = hide(threadIdx.x >> 5), lane = hide(threadIdx.x & 31);
     const int r = lane >> 2, c4 = lane & 3;
@@ -337,6 +343,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
                 record_fault(ALJ_FAULT_BOUNDS);
                 len = len < 0 ? 0 : cap;
             }
+            if (TREE && len < p.q_len) len = 0;    // no tree is there
             s_len[b] = len;
             n = chunks_of(p, len) + kItemCost;
         }
@@ -523,12 +530,33 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             if (lane < PARTS) s_fac[column_of<PARTS>(row, lane)] = p.scale * pow2i(24 - f);
         }
 
-        if (threadIdx.x < COLS) {                  // the last position a column's row sees
+        if constexpr (TREE) {
+            const int base = len - p.q_len;
+            for (int i = threadIdx.x; i < p.q_len; i += kThreads)
+                s_par[i] = tree_parent(p.parents + static_cast<long long>(item_b) * p.parents_stride, i);
+            if (threadIdx.x <= kKv4TreeWords) s_any[threadIdx.x] = threadIdx.x < kKv4TreeWords ? 0u : 0x7FFFFFFFu;
+            __syncthreads();
+            if (threadIdx.x < COLS) {              // the position that a column's row stands for, and the nodes it sees
+                const int row = PARTS == 1 ? threadIdx.x : 4 * (threadIdx.x >> 3) + (threadIdx.x & 3);
+                uint32_t* const see = s_see + threadIdx.x * kKv4TreeWords;
+                const int depth = row < rows && base >= 0 ? tree_chain(s_par, token_of(row0 + row), p.window, see) : 0;
+                s_hi[threadIdx.x] = depth > 0 ? base + depth - 1 : -1;
+                if (depth > 0) {
+                    for (int i = 0; i < kKv4TreeWords; ++i) atomicOr(s_any + i, see[i]);
+                    atomicMin(s_any + kKv4TreeWords, static_cast<uint32_t>(base + depth - 1));
+                }
+            }
+            all_hi = base - 1;                     // every position before the tree; rows of absent nodes need no care
+            all_lo = window_start(p, len);
+        }
+        if (!TREE && threadIdx.x < COLS) {         // the last position a column's row sees
             const int row = PARTS == 1 ? threadIdx.x : 4 * (threadIdx.x >> 3) + (threadIdx.x & 3);
             s_hi[threadIdx.x] = row < rows ? len - p.q_len + token_of(row0 + row) : -1;
         }
-        all_hi = len - p.q_len + token_of(row0);
-        all_lo = window_start(p, len - p.q_len + token_of(row0 + rows - 1) + 1);
+        if constexpr (!TREE) {
+            all_hi = len - p.q_len + token_of(row0);
+            all_lo = window_start(p, len - p.q_len + token_of(row0 + rows - 1) + 1);
+        }
         }
         __syncthreads();
 
@@ -672,7 +700,14 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             for (int a = 0; a < CT; ++a) keep[a][0] = keep[a][1] = 0xFFFFFFFFu;
             if (pos < all_lo || pos + kTilePos - 1 > all_hi) {
                 const int word_pos = pos + (NG == 2 ? lane : lane >> 1);   // the position of the lane's scale words
-                if (word_pos >= len || (p.window > 0 && all_hi - word_pos >= p.window)) top = 0u;
+                if constexpr (TREE) {
+                    const int node = word_pos - (all_hi + 1);
+                    if (word_pos >= len || (node >= 0 && !tree_sees(s_any, node)) ||
+                        (p.window > 0 && static_cast<int>(s_any[kKv4TreeWords]) - word_pos >= p.window))
+                        top = 0u;
+                } else if (word_pos >= len || (p.window > 0 && all_hi - word_pos >= p.window)) {
+                    top = 0u;
+                }
 #pragma unroll
                 for (int a = 0; a < CT; ++a)
 #pragma unroll
@@ -682,7 +717,13 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             const int hi = s_hi[8 * a + 2 * c4 + j];
-                            see[j] = at_pos <= hi && (p.window == 0 || hi - at_pos < p.window);
+                            if constexpr (TREE) {  // hi: the position the row stands for, -1 where its node is absent
+                                const int node = at_pos - (all_hi + 1);
+                                if (node < 0) see[j] = hi >= 0 && (p.window == 0 || hi - at_pos < p.window);
+                                else see[j] = hi >= 0 && node < p.q_len && tree_sees(s_see + (8 * a + 2 * c4 + j) * kKv4TreeWords, node);
+                            } else {
+                                see[j] = at_pos <= hi && (p.window == 0 || hi - at_pos < p.window);
+                            }
                             y[a][h][j] = see[j] ? y[a][h][j] : -INFINITY;
                         }
                         keep[a][h] = transpose8((see[0] ? 0x0000FFFFu : 0u) | (see[1] ? 0xFFFF0000u : 0u));
@@ -835,6 +876,16 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
         const int kvh = it.kvh, row0 = it.row0, rows = it.rows;
 
         // ---------------------------------------------------------- merge the warps
+        if constexpr (TREE) {                      // absent nodes took part in the tiles that need no masks
+#pragma unroll
+            for (int a = 0; a < CT; ++a)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (s_hi[8 * a + 2 * c4 + j] < 0) {
+                        M[a][j] = kNone;
+                        l[a][j] = 0.0f;
+                    }
+        }
         if (r == 0) {
 #pragma unroll
             for (int a = 0; a < CT; ++a)
@@ -979,16 +1030,17 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     }
 }
 
-template <int NG, int CT, int PARTS>
+template <int NG, int CT, int PARTS, bool TREE>
 cudaError_t launch_cfg(Kv4Attn p, int sms, int max_ctas, cudaStream_t stream) {
     using F = Cfg<NG, CT, PARTS>;
-    const int smem = F::SMEM + (2 * p.batch + 1) * static_cast<int>(sizeof(int));
+    constexpr int kTree = TREE ? (kKv4MaxNodes + F::COLS * kKv4TreeWords + kKv4TreeWords + 1) * 4 : 0;
+    const int smem = F::SMEM + kTree + (2 * p.batch + 1) * static_cast<int>(sizeof(int));
     static bool configured[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
-        const cudaError_t e = cudaFuncSetAttribute(kv4_attn_kernel<NG, CT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   F::SMEM + (2 * kKv4MaxBatch + 1) * static_cast<int>(sizeof(int)));
+        const cudaError_t e = cudaFuncSetAttribute(kv4_attn_kernel<NG, CT, PARTS, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   F::SMEM + kTree + (2 * kKv4MaxBatch + 1) * static_cast<int>(sizeof(int)));
         if (e != cudaSuccess) return e;
         configured[dev & 63] = true;
     }
@@ -1005,7 +1057,7 @@ cudaError_t launch_cfg(Kv4Attn p, int sms, int max_ctas, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv4_attn_kernel<NG, CT, PARTS>, p);
+    return cudaLaunchKernelEx(&cfg, kv4_attn_kernel<NG, CT, PARTS, TREE>, p);
 }
 
 // Rows a CTA serves at once: a column tile holds 8 bf16 or 4 fp32 rows; two
@@ -1028,6 +1080,8 @@ size_t kv4_attention_workspace_bytes(int q_rows, int head_dim, int sms) {
     return (ctas * 4 + 255) / 256 * 256 + ctas * 2 * tile_rows(q_rows, head_dim, false) * (head_dim + 2) * 4;
 }
 
+size_t kv4_tree_workspace_bytes(int q_rows, int head_dim, int sms) { return kv4_attention_workspace_bytes(q_rows, head_dim, sms); }
+
 cudaError_t launch_kv4_attention(const Kv4Attn& a, void* workspace, int sms, cudaStream_t stream) {
     Kv4Attn p = a;
     const int ctas = kv4_attention_max_ctas(sms);
@@ -1039,8 +1093,9 @@ cudaError_t launch_kv4_attention(const Kv4Attn& a, void* workspace, int sms, cud
     p.page_shift = (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctz(p.page_size) : -1;
     p.counters = static_cast<unsigned int*>(workspace);
     p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (static_cast<size_t>(ctas) * 4 + 255) / 256 * 256);
-#define ALJ_KV4(NG, CT)                                                      \
-    return wide ? launch_cfg<NG, CT, 2>(p, sms, ctas, stream) : launch_cfg<NG, CT, 1>(p, sms, ctas, stream)
+#define ALJ_KV4(NG, CT)                                                                                             \
+    return p.parents ? (wide ? launch_cfg<NG, CT, 2, true>(p, sms, ctas, stream) : launch_cfg<NG, CT, 1, true>(p, sms, ctas, stream)) \
+                     : (wide ? launch_cfg<NG, CT, 2, false>(p, sms, ctas, stream) : launch_cfg<NG, CT, 1, false>(p, sms, ctas, stream))
     if (p.head_dim == 256) ALJ_KV4(8, 1);
     if (p.head_dim == 128) {
         if (two) ALJ_KV4(4, 2);

@@ -8,6 +8,14 @@ one page of max_ctx positions each (no table).  The serving loop of one layer:
     cache.append(k, v, slots)                      # new rows -> 4 bits
     out = cache.attend(q, seq_lens, block_table)   # q: [batch, q_len, q_heads, head_dim]
 
+Speculative decoding drafts a tree of tokens a sequence, whose nodes take the
+positions behind it (parents: int32, -1 a root, -2 an absent node).  One step:
+
+    q = cache.append_rotated(q, k, v, slots, positions, rope)    # each layer
+    out = cache.attend_tree(q, seq_lens, parents, block_table)
+    ...                                                          # logits, process_logits: picked
+    path, count, token, lens = accept_tree(caches, seq_lens, parents, drafted, picked, block_table)
+
 Tensors are torch CUDA tensors on the cache's device; every call is ordered on
 torch's current stream of that device (or `stream`, a raw cudaStream_t: what
 the call is given must be ready there and live until it has run), and may be
@@ -91,6 +99,7 @@ def new_output(shape, dtype, device, index: int, stream: int) -> torch.Tensor:
     return t
 
 
+_tree_work = {}     # (device, stream) -> workspace of attend_tree, of all caches: calls on one stream follow one another
 _captured = {}      # (device, stream) -> capture id, its workspaces
 _kept = []          # workspaces of captures on streams given by handle
 
@@ -104,6 +113,11 @@ def dtype_id(t: torch.Tensor, what: str) -> int:
 
 def bad(message: str) -> native.ProviderError:
     return native.ProviderError(native.ALJ_ERR_BAD_ARG, message)
+
+
+_rotate_append = native.lib().aljabr_blackwell_kv4_rotate_append_dev
+_attend_tree = native.lib().aljabr_blackwell_kv4_tree_attention_dev
+_accept_tree = native.lib().aljabr_blackwell_kv4_accept_tree_dev
 
 
 class Kv4Cache:
@@ -178,6 +192,49 @@ class Kv4Cache:
         if rc:
             native.check(rc)
 
+    def append_rotated(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
+                       rope: torch.Tensor, interleaved: bool = False, q_out=None, k_back=None, v_back=None,
+                       stream=None) -> torch.Tensor:
+        """append() with the rotation of q and k by their positions on the way; returns the rotated q.
+
+        q: [tokens, q_heads, head_dim] with contiguous rows, of k's type.  positions: int32 [tokens], below zero where a
+        token is absent (its q is zero, nothing is stored).  rope: float32 [positions, n, 2] of (cos, sin), contiguous;
+        a head's first 2 n dims turn, dims i and i + n a pair, or with `interleaved` 2 i and 2 i + 1.  q_out: of q's
+        shape and type, its rows may be strided, q itself will do."""
+        n, dtype = slots.numel(), k.dtype
+        kind = _DTYPES.get(dtype)
+        if kind is None:
+            dtype_id(k, "k")
+        if v.dtype is not dtype or q.dtype is not dtype:
+            raise bad(f"k is {dtype}, v is {v.dtype}, q is {q.dtype}")
+        ks, vs = self._rows(k, n, "k"), self._rows(v, n, "v")
+        heads = q.shape[1] if q.dim() == 3 else 0
+        qs = self._q_rows(q, n, heads, "q")
+        if rope.dtype is not torch.float32 or rope.dim() != 3 or rope.shape[2] != 2 or rope.get_device() != self._index or \
+                not rope.is_contiguous():
+            raise bad(f"rope must be contiguous float32 [positions, pairs, 2] on {self.device}")
+        kb = None if k_back is None else self._dense(k_back, n, dtype, "k_back")
+        vb = None if v_back is None else self._dense(v_back, n, dtype, "v_back")
+        stream = stream or current_stream(self._index)
+        if q_out is None:
+            q_out = new_output(q.shape, dtype, self.device, self._index, stream)
+        elif q_out.dtype is not dtype:
+            raise bad(f"q is {dtype}, q_out is {q_out.dtype}")
+        rc = _rotate_append(*self._shape, q_out.data_ptr(), self._q_rows(q_out, n, heads, "q_out"), q.data_ptr(), k.data_ptr(),
+                            v.data_ptr(), kind, qs, ks, vs, heads, self._ints(slots, n, "slots"),
+                            self._ints(positions, n, "positions"), rope.data_ptr(), rope.shape[0], 2 * rope.shape[1],
+                            bool(interleaved), n, kb, vb, stream)
+        if rc:
+            native.check(rc)
+        return q_out
+
+    def _q_rows(self, t: torch.Tensor, tokens: int, heads: int, what: str) -> int:
+        shape, st, D = t.shape, t.stride(), self.head_dim
+        if shape != (tokens, heads, D) or st[2] != 1 or (heads > 1 and st[1] != D) or t.get_device() != self._index:
+            raise bad(f"{what} must be [{tokens}, q_heads, {D}] on {self.device} with contiguous rows, "
+                      f"not {tuple(shape)} with strides {st} on {t.device}")
+        return st[0] if tokens > 1 else heads * D
+
     def read(self, slots: torch.Tensor, dtype=torch.float32, k_out=None, v_out=None, stream=None):
         """Rows of the given slots as (k, v), [n, kv_heads, head_dim] each; zeros where a slot is -1."""
         n = slots.numel()
@@ -202,17 +259,28 @@ class Kv4Cache:
         return got
 
     def _make_workspace(self, q_len: int, q_heads: int, stream: int) -> torch.Tensor:
-        """Made and zeroed on the stream whose kernels will use it."""
         need = self._work_size(q_len, q_heads, self.kv_heads, self.head_dim)   # the call's own, for its refusals
         if need < 0:
             native.check(int(need))
-        most = self._work_size(native.KV4_MAX_ROWS, self.kv_heads, self.kv_heads, self.head_dim)
-        if stream == current_stream(self._index):
-            return torch.zeros(most, dtype=torch.uint8, device=self.device)
-        with torch.cuda.stream(torch_stream(stream, self.device)):
-            return torch.zeros(most, dtype=torch.uint8, device=self.device)
+        return self._zeros(self._work_size(native.KV4_MAX_ROWS, self.kv_heads, self.kv_heads, self.head_dim), stream)
 
-    def _captured_workspace(self, capture: int, q_len: int, q_heads: int, stream: int):
+    def _tree_workspace(self, stream: int):
+        """(address, bytes) of this stream's workspace for trees: as large as any accepted call needs, kept for good."""
+        have = _tree_work.get((self._index, stream))
+        if have is None:
+            size, group = native.lib().aljabr_blackwell_kv4_tree_attention_workspace_size, native.KV4_MAX_ROWS // native.KV4_MAX_NODES
+            most = max(size(native.KV4_MAX_NODES, group, 1, D) for D in (64, 128, 256))
+            have = _tree_work[self._index, stream] = self._zeros(int(most), stream)
+        return have.data_ptr(), have.numel()
+
+    def _zeros(self, size: int, stream: int) -> torch.Tensor:
+        """Made and zeroed on the stream whose kernels will use it."""
+        if stream == current_stream(self._index):
+            return torch.zeros(size, dtype=torch.uint8, device=self.device)
+        with torch.cuda.stream(torch_stream(stream, self.device)):
+            return torch.zeros(size, dtype=torch.uint8, device=self.device)
+
+    def _captured_workspace(self, capture: int, q_len: int, q_heads: int, stream: int, tree: bool = False):
         """(address, bytes) for calls recorded into a graph.  Its zeroing is a node of that graph, which may run on any
         stream: so it belongs to this capture's calls on this stream (of all caches: they follow one another) and to
         nothing else.  torch's graph keeps the memory: here it is held until the stream's next capture, and for good
@@ -221,9 +289,10 @@ class Kv4Cache:
         owner, have = _captured.get(key, (0, []))
         if owner != capture:
             _captured[key] = capture, (have := [])
-        need = self._work_size(q_len, q_heads, self.kv_heads, self.head_dim)
+        size = native.lib().aljabr_blackwell_kv4_tree_attention_workspace_size if tree else self._work_size
+        need = size(q_len, q_heads, self.kv_heads, self.head_dim)
         if not have or have[-1].numel() < need:
-            have.append(self._make_workspace(q_len, q_heads, stream))
+            have.append(self._zeros(int(need), stream) if tree else self._make_workspace(q_len, q_heads, stream))
             if stream != current_stream(self._index):
                 _kept.append(have[-1])
         return have[-1].data_ptr(), have[-1].numel()
@@ -234,6 +303,22 @@ class Kv4Cache:
 
         block_table: int32 [batch, pages a sequence], or None where sequence b is page b.  scale: 1 / sqrt(head_dim)
         by default.  Returns out, contiguous, of q's type."""
+        return self._attention(q, seq_lens, None, block_table, window, scale, soft_cap, out, stream)
+
+    def attend_tree(self, q: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor, block_table=None, window: int = 0,
+                    scale=None, soft_cap: float = 0.0, out=None, stream=None) -> torch.Tensor:
+        """Attention of the nodes of drafted trees, the last `nodes` of seq_lens[b] positions: q [batch, nodes, q_heads,
+        head_dim].  A node sees the positions before the tree, its ancestors and itself; zeros where it is absent.
+
+        parents: int32 [batch, nodes], or [nodes] for one tree of all sequences; -1 a root, -2 absent, else an earlier
+        node.  window counts a node by its depth.  The rest as attend()."""
+        nodes = q.shape[1] if q.dim() == 4 else -1
+        if parents.dtype is not torch.int32 or parents.shape not in ((nodes,), (q.shape[0], nodes)) or \
+                parents.get_device() != self._index or not parents.is_contiguous():
+            raise bad(f"parents must be contiguous int32 [{nodes}] or [{q.shape[0]}, {nodes}] on {self.device}")
+        return self._attention(q, seq_lens, parents, block_table, window, scale, soft_cap, out, stream)
+
+    def _attention(self, q, seq_lens, parents, block_table, window, scale, soft_cap, out, stream):
         shape, st = q.shape, q.stride()
         if len(shape) != 4 or shape[3] != self.head_dim or q.get_device() != self._index:
             raise bad(f"q must be [batch, q_len, q_heads, {self.head_dim}] on {self.device}, not {tuple(shape)} on {q.device}")
@@ -262,17 +347,75 @@ class Kv4Cache:
         if stream != _LEGACY_STREAM and (stream != current or torch.cuda.is_current_stream_capturing()):
             capture = capture_id(stream)
         if capture:
-            work, size = self._captured_workspace(capture, q_len, q_heads, stream)
+            work, size = self._captured_workspace(capture, q_len, q_heads, stream, parents is not None)
+        elif parents is not None:
+            work, size = self._tree_workspace(stream)
         else:
             have = self._work.get((stream, q_len, q_heads))
             work, size = have if have is not None else self._workspace(q_len, q_heads, stream)
-        rc = self._attend(out.data_ptr(), q.data_ptr(), kind, q_stride, *self._shape, table, width,
-                          self._ints(seq_lens, batch, "seq_lens"), batch, q_len, q_heads, window,
-                          D ** -0.5 if scale is None else scale, soft_cap, work, size, stream)
+        scale = D ** -0.5 if scale is None else scale
+        lens = self._ints(seq_lens, batch, "seq_lens")
+        if parents is None:
+            rc = self._attend(out.data_ptr(), q.data_ptr(), kind, q_stride, *self._shape, table, width, lens, batch, q_len,
+                              q_heads, window, scale, soft_cap, work, size, stream)
+        else:
+            rc = _attend_tree(out.data_ptr(), q.data_ptr(), kind, q_stride, *self._shape, table, width, lens, batch,
+                              parents.data_ptr(), q_len if parents.dim() == 2 else 0, q_len, q_heads, window, scale, soft_cap,
+                              work, size, stream)
         if rc:
             native.check(rc)
         return out
 
 
-for _name in ("append", "read", "attend"):
+def accept_tree(caches, seq_lens: torch.Tensor, parents: torch.Tensor, drafted: torch.Tensor, picked: torch.Tensor,
+                block_table=None, out=None, stream=None):
+    """Keeps the drafted path that agrees with the model, in every cache of a list (a model's layers, of one shape).
+
+    From node 0, the token emitted last, on to the first child whose drafted token is the one picked after its parent.
+    drafted, picked: int32 [batch, nodes]; seq_lens, parents, block_table as for attend_tree.  The path's rows move to
+    the first positions of the tree.  Returns int32 (path [batch, nodes], -1 behind its end; count [batch]; token
+    [batch], picked after the path's last node; lens [batch], the sequence with its path), written to `out` where
+    that is a result of an earlier call.  A sequence without a tree: count 0, token -1, its length."""
+    caches = [caches] if isinstance(caches, Kv4Cache) else list(caches)
+    if not caches:
+        raise bad("no caches")
+    first = caches[0]
+    if any(c._shape[1:] != first._shape[1:] or c._index != first._index for c in caches):
+        raise bad("the caches of one call must have the same shape and device")
+    if drafted.dim() != 2:
+        raise bad("drafted must be int32 [batch, nodes]")
+    batch, nodes = drafted.shape
+    ints = (lambda t, shapes, what: _int_tensor(t, shapes, what, first))
+    stream = stream or current_stream(first._index)
+    if out is None:
+        out = tuple(new_output(s, torch.int32, first.device, first._index, stream) for s in ((batch, nodes),) + ((batch,),) * 3)
+    table, width = None, 0
+    if block_table is not None:
+        width = block_table.shape[-1]
+        table = ints(block_table, ((batch, max(width, 1)),), "block_table")
+    path, count, token, lens = (ints(t, (s,), w) for t, s, w in zip(out, ((batch, nodes),) + ((batch,),) * 3,
+                                                                    ("path", "count", "token", "lens")))
+    rc = _accept_tree(path, count, token, lens, (ctypes.c_void_p * len(caches))(*[c._shape[0] for c in caches]), len(caches),
+                      *first._shape[1:], table, width, ints(seq_lens, ((batch,),), "seq_lens"), batch,
+                      ints(parents, ((nodes,), (batch, nodes)), "parents"), nodes if parents.dim() == 2 else 0, nodes,
+                      ints(drafted, ((batch, nodes),), "drafted"), ints(picked, ((batch, nodes),), "picked"), stream)
+    if rc:
+        native.check(rc)
+    return out
+
+
+def _int_tensor(t: torch.Tensor, shapes, what: str, cache: Kv4Cache) -> int:
+    if t.dtype is not torch.int32 or t.shape not in shapes or t.get_device() != cache._index or not t.is_contiguous():
+        raise bad(f"{what} must be contiguous int32 {' or '.join(str(list(s)) for s in shapes)} on {cache.device}, "
+                  f"not {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _index_of(caches, *_, **__):
+    caches = [caches] if isinstance(caches, Kv4Cache) else list(caches)
+    return caches[0]._index if caches else -1
+
+
+accept_tree = selecting(accept_tree, _index_of)
+for _name in ("append", "append_rotated", "read", "attend", "attend_tree"):
     setattr(Kv4Cache, _name, selecting(getattr(Kv4Cache, _name), lambda cache, *_, **__: cache._index))

@@ -34,6 +34,8 @@ KV_F32 = 0
 KV_BF16 = 1
 KV_Q4 = 2
 KV4_MAX_ROWS = 1024      # q_len * q_heads / kv_heads of one kv4_attention call
+KV4_MAX_NODES = 256      # of a drafted tree
+KV4_MAX_LAYERS = 256     # caches of one kv4_accept_tree call
 
 
 class ProviderError(RuntimeError):
@@ -112,6 +114,13 @@ SIGNATURES = {
     "aljabr_blackwell_kv4_attention_workspace_size": (_ll, [_i, _i, _i, _i]),
     "aljabr_blackwell_kv4_attention_dev": (_i, [_p, _p, _i, _ll, _p, _i, _i, _i, _i, _p, _i, _p, _i, _i, _i, _i, _f, _f,
                                                 _p, _ll, _p]),
+    "aljabr_blackwell_kv4_rotate_append_dev": (_i, [_p, _i, _i, _i, _i, _p, _ll, _p, _p, _p, _i, _ll, _ll, _ll, _i, _p, _p, _p,
+                                                    _i, _i, _i, _i, _p, _p, _p]),
+    "aljabr_blackwell_kv4_tree_attention_workspace_size": (_ll, [_i, _i, _i, _i]),
+    "aljabr_blackwell_kv4_tree_attention_dev": (_i, [_p, _p, _i, _ll, _p, _i, _i, _i, _i, _p, _i, _p, _i, _p, _i, _i, _i, _i,
+                                                     _f, _f, _p, _ll, _p]),
+    "aljabr_blackwell_kv4_accept_tree_dev": (_i, [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _i, _p, _i, _p, _i, _i, _p, _p,
+                                                  _p]),
     "aljabr_blackwell_stream_capture_id": (_i, [_p, _p]),
     "aljabr_blackwell_logits_process_dev": (_i, [_p, _ll, _p, _i, _ll, _i, _i, _p, _p, _i, _p, _p, _p, _p, _i, _p, _i,
                                                  _p, _p]),

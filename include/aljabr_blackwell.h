@@ -395,6 +395,74 @@ int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, lo
                                        int table_stride, const int* seq_lens, int batch, int q_len, int q_heads,
                                        int window, float scale, float soft_cap, void* workspace,
                                        long long workspace_bytes, void* stream);
+
+/* ---- trees of drafted tokens over the 4-bit cache --------------------------
+ * No counterpart in the reference.  One step of speculative decoding: the
+ * drafted nodes' rows enter the cache at the positions behind the sequence
+ * (kv4_rotate_append_dev), every node attends to its own past
+ * (kv4_tree_attention_dev), the model's logits give a token after each node
+ * (logits_process_dev), and the drafted path that agrees with them is kept
+ * (kv4_accept_tree_dev).
+ *
+ * A tree of `nodes` (1 to 256) nodes is device int32 parents[nodes]: -1 for
+ * a root, -2 for a node that is absent (as is one whose parent is), otherwise
+ * an earlier node.  Sequence b's is at parents + b * parents_stride (0: one tree for
+ * all).  Its nodes are the last `nodes` of the sequence's seq_lens[b]
+ * positions, in node order, absent ones included; base = seq_lens[b] - nodes.
+ * A sequence of fewer positions holds no tree.
+ *
+ * kv4_rotate_append_dev is kv4_append_dev with the position rotation on the
+ * way: tokens have q rows of q_heads heads too (kv_dtype, q_stride elements
+ * apart), and with (c, s) = rope[positions[i]][pair], rope device fp32
+ * [rope_positions][rotary_dim / 2][2], 16-byte aligned, rotary_dim a multiple of 16 up to
+ * head_dim, the first rotary_dim dims of every q and K head become
+ *   (a c - b s, a s + b c) for the dims a, b = pair, pair + rotary_dim / 2,
+ *   or with `interleaved` 2 pair, 2 pair + 1,
+ * products and sums rounded to fp32 one by one, as in the decode step.  The
+ * rotated q goes to q_out (q's type, q_out_stride apart; q itself will do),
+ * K is quantised from the fp32 result.  A token at a position below zero is
+ * absent: q_out zero, nothing stored.  One whose slot is -1 has its q rotated.
+ *
+ * kv4_tree_attention_dev: as kv4_attention_dev, for the nodes of each
+ * sequence's tree (q [batch][nodes]).  A node sees the positions before base,
+ * its ancestors and itself; with window > 0 of these the last `window`, a
+ * node counting as position base + its depth (a root's is 0).  A node that is
+ * absent, or whose sequence holds no tree, is zero.  nodes * q_heads /
+ * kv_heads is at most 1024.  The workspace may be the same as
+ * kv4_attention_dev's where it is large enough.
+ *
+ * kv4_accept_tree_dev: from node 0 (a root: the token emitted last) on to the
+ * first child whose drafted token is the one picked after its parent, as long
+ * as there is one; drafted, picked [batch][nodes].  path [batch][nodes] gets
+ * the nodes (-1 behind them), count their number, token the one picked
+ * after the last, new_lens base + count.  The path's rows move to positions
+ * base, base + 1, .. in each of `layers` (at most 256) caches of equal shape
+ * (host array of device addresses); sequences must not share the pages of
+ * their trees.  A sequence without a tree, or whose node 0 is no root, keeps
+ * nothing of it: count 0, token -1, new_lens base (or seq_lens[b] without a
+ * tree).  Outputs must not overlap inputs.
+ *
+ * Parents, pages, positions and lengths outside their ranges are not followed
+ * and set bit 1 of aljabr_blackwell_device_status, as above.  All are
+ * stream-ordered (NULL = the library's stream) and allocate nothing. */
+int aljabr_blackwell_kv4_rotate_append_dev(void* cache, int pages, int page_size, int kv_heads, int head_dim, void* q_out,
+                                           long long q_out_stride, const void* q, const void* k, const void* v,
+                                           int kv_dtype, long long q_stride, long long k_stride, long long v_stride,
+                                           int q_heads, const int* slots, const int* positions, const float* rope,
+                                           int rope_positions, int rotary_dim, int interleaved, int tokens, void* k_back,
+                                           void* v_back, void* stream);
+long long aljabr_blackwell_kv4_tree_attention_workspace_size(int nodes, int q_heads, int kv_heads, int head_dim);
+int aljabr_blackwell_kv4_tree_attention_dev(void* out, const void* q, int q_dtype, long long q_stride, const void* cache,
+                                            int pages, int page_size, int kv_heads, int head_dim, const int* block_table,
+                                            int table_stride, const int* seq_lens, int batch, const int* parents,
+                                            int parents_stride, int nodes, int q_heads, int window, float scale,
+                                            float soft_cap, void* workspace, long long workspace_bytes, void* stream);
+int aljabr_blackwell_kv4_accept_tree_dev(int* path, int* count, int* token, int* new_lens, void* const* caches, int layers,
+                                         int pages, int page_size, int kv_heads, int head_dim, const int* block_table,
+                                         int table_stride, const int* seq_lens, int batch, const int* parents,
+                                         int parents_stride, int nodes, const int* drafted, const int* picked,
+                                         void* stream);
+
 /* *id: the graph capture that `stream` takes part in, 0 if none.  A workspace
  * that is zeroed inside a capture is zero only in that graph's replays, so a
  * host keeps those apart by this id. */
