@@ -121,6 +121,7 @@ struct DeviceState {
     std::mutex mu;                          // serialises the staging buffers of tb calls
     std::map<uintptr_t, Registered> reg;    // host base -> HBM copy
     std::mutex reg_mu;
+    std::mutex tree_mu;                     // keeps the launches of one tree attention together
     DevBuf dx, dy, dtmp, dscratch, dgemm;
     HostBuf hx, hy;
     std::map<PackKey, PackedQ> qpack;       // guarded by mu
@@ -717,7 +718,10 @@ int kv4_attend(const char* what, void* out, const void* q, int q_dtype, long lon
     a.soft_cap = soft_cap;
     a.parents = parents;
     a.parents_stride = parents_stride;
-    return launch_status(launch_kv4_attention(a, workspace, st->sms, pick_stream(st, stream)), what);
+    if (!parents) return launch_status(launch_kv4_attention(a, workspace, st->sms, pick_stream(st, stream)), what);
+    // two launches share the workspace: another thread's call on this stream must not come between them
+    std::lock_guard<std::mutex> g(st->tree_mu);
+    return launch_status(launch_kv4_tree(a, workspace, st->sms, pick_stream(st, stream)), what);
 }
 
 // The binding's elementwise glue (rmsnorm, silu_ffn): operands that are

@@ -1075,12 +1075,12 @@ int tile_rows(int rows, int head_dim, bool wide) {
 
 int kv4_attention_max_ctas(int sms) { return 2 * sms; }
 
+size_t kv4_attention_counter_bytes(int sms) { return (static_cast<size_t>(kv4_attention_max_ctas(sms)) * 4 + 255) / 256 * 256; }
+
 size_t kv4_attention_workspace_bytes(int q_rows, int head_dim, int sms) {
     const size_t ctas = kv4_attention_max_ctas(sms);
-    return (ctas * 4 + 255) / 256 * 256 + ctas * 2 * tile_rows(q_rows, head_dim, false) * (head_dim + 2) * 4;
+    return kv4_attention_counter_bytes(sms) + ctas * 2 * tile_rows(q_rows, head_dim, false) * (head_dim + 2) * 4;
 }
-
-size_t kv4_tree_workspace_bytes(int q_rows, int head_dim, int sms) { return kv4_attention_workspace_bytes(q_rows, head_dim, sms); }
 
 cudaError_t launch_kv4_attention(const Kv4Attn& a, void* workspace, int sms, cudaStream_t stream) {
     Kv4Attn p = a;
@@ -1092,7 +1092,7 @@ cudaError_t launch_kv4_attention(const Kv4Attn& a, void* workspace, int sms, cud
     p.group_magic = ((1u << 21) + p.group - 1) / p.group;   // row / group for row < 2048, exact as row * group < 2^21
     p.page_shift = (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctz(p.page_size) : -1;
     p.counters = static_cast<unsigned int*>(workspace);
-    p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (static_cast<size_t>(ctas) * 4 + 255) / 256 * 256);
+    p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kv4_attention_counter_bytes(sms));
 #define ALJ_KV4(NG, CT)                                                                                             \
     return p.parents ? (wide ? launch_cfg<NG, CT, 2, true>(p, sms, ctas, stream) : launch_cfg<NG, CT, 1, true>(p, sms, ctas, stream)) \
                      : (wide ? launch_cfg<NG, CT, 2, false>(p, sms, ctas, stream) : launch_cfg<NG, CT, 1, false>(p, sms, ctas, stream))

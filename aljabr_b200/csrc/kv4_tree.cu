@@ -1,0 +1,1036 @@
+// Attention of drafted trees over the 4-bit KV cache (layout and trees:
+// kv4.cuh) on tcgen05, for bf16 queries with many rows a kv head.
+//
+//   S[i, p] = scale q_i . K_p  (soft cap: S <- cap tanh(S / cap)),  P = softmax
+//   over what row i sees: positions before the tree, its node's ancestors, its
+//   node (window: the last of these);  O_i = sum_p P[i, p] V_p
+//
+// A row i is one (node, query head) pair of the nodes x group pairs that share
+// a kv head; 128 of them are an MMA's M.  A tile is KT positions.  Every code is
+// decoded once for 128 rows, into fp16 operands in shared memory:
+//   * K: d (c - 8) 2^-e, row p = the position, in the 128-byte swizzle; e, one
+//     of 32 positions, is the largest exponent of their scales, so the operand is
+//     in fp16's range whatever the cache holds, and scores are scaled back by 2^e
+//     in fp32.  d (c - 8) has 15 bits: it is rounded to fp16's 11 (2^-11 half a
+//     step; the output's own rounding is 2^-8).
+//   * V: the same, transposed on the way (a row is a dim, 8 positions 16 bytes): a
+//     word of two positions' codes is put together by one PRMT, as the codes of
+//     four dims lie in a halfword.  Its e, one of 64 positions, goes into P.
+//   * Q: scaled by a power of two into fp16's range, exact for bf16 to 2^-38 of
+//     the row's largest.
+//   * P = 2^(S - M + b + e - E) in fp16: M the running maximum, raised when a
+//     score passes it by 2^5, E the running largest e, b a bias that keeps P in
+//     the upper part of fp16's range.  P is written over S in tensor memory and is
+//     the A operand of O += P V from there.  Softmax sums are fp32, of the
+//     unrounded P.
+//   * A V group that is NaN counts as zeros in the product, and as NaN for the
+//     rows that see it: a product with a masked position's zero would be NaN too.
+//
+// Roles (one CTA an SM, persistent over the line of chunks as in
+// kv4_attention.cu): a producer warp (bulk copies of a tile's codes and scales
+// into a ring, 8 positions of V apart by 16 bytes so that transposing reads hit
+// distinct banks), 4 warps that decode K, 4 that decode V, one that issues the
+// MMAs, and a warpgroup of softmax for each of two streams: the even and the odd
+// tiles of an item have their own S, running maximum and O, so that one stream's
+// softmax runs beside the other's products.  (D 256: tiles of 64, one stream, as
+// two O do not fit tensor memory beside S.)  The streams are joined when the item
+// ends; items cut over CTAs are joined by a second small kernel, which all SMs
+// share (one CTA joining 128 rows of 10 parts would read 0.6 MB by itself).
+#include "kv4.cuh"
+#include "tc_gemm.cuh"
+
+#include <algorithm>
+
+namespace alj {
+namespace {
+
+constexpr int kRows = 128;
+constexpr int kItemCost = 2;          // tiles that an item's start and end are worth
+constexpr int kMeta = 4;              // tiles whose exponents are kept
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNone = -3.4e38f;     // running maximum of a row that has seen nothing
+// P <= 2^(kLazy + kSlack + kBias) = 2^15
+constexpr float kLazy = 5.0f;
+constexpr int kSlack = 2, kBias = 8;
+
+template <int NG>
+struct Shape {
+    static constexpr int D = 32 * NG;
+    static constexpr int KT = NG == 8 ? 64 : 128;            // positions of a tile
+    static constexpr int STREAMS = NG == 8 ? 1 : 2;
+    static constexpr int V_STAGES = NG == 8 ? 1 : 2;
+    static constexpr int RAW = NG == 2 ? 4 : NG == 4 ? 3 : 2;
+    static constexpr int SOFT = 4 * STREAMS;                 // softmax warps
+    static constexpr int WARPS = SOFT + 10;
+    static constexpr int THREADS = 32 * WARPS;
+    // a raw tile: K codes, K scales, V codes and V scales in padded blocks of 8 positions
+    static constexpr int VB = 4 * D + 16, SB = 16 * NG + 16;
+    static constexpr int K_SC = KT * D / 2, V_CODES = K_SC + KT * 2 * NG, V_SC = V_CODES + KT / 8 * VB;
+    static constexpr int RAW_BYTES = (V_SC + KT / 8 * SB + 127) / 128 * 128;
+    static constexpr int BLOCK_BYTES = 16 * (D + D / 8);     // copied for 16 positions
+    static constexpr int KHAT = KT * D * 2, VHAT = KT * D * 2, Q = kRows * D * 2;
+    static constexpr int AT_K = Q, AT_V = AT_K + 2 * KHAT, AT_RAW = AT_V + V_STAGES * VHAT, AT_SMALL = AT_RAW + RAW * RAW_BYTES;
+    static constexpr int O_COL = NG == 8 ? 128 : 256;        // tensor memory: S of two tiles, then O of each stream
+};
+
+struct Small {                        // behind the tiles in shared memory
+    uint64_t raw_full[4], raw_empty[4], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], q_full, done;
+    uint64_t ek_full[kMeta];          // K exponents: the K warps do not wait for V
+    int abort, tmem;
+    uint32_t valid[4][4];             // by raw slot: bits of the positions that some row may see
+    int ek[kMeta][4];                 // by tile: exponents of K (32 positions) and V (64)
+    int ev[kMeta][2];
+    int nan_any[kMeta][2];            // V groups that are NaN: bits by position
+    uint8_t nan[kMeta][128];
+    int sum[32];                      // prefix sums, and where this CTA starts
+    int start[4];
+    uint32_t node_ok[kKv4TreeWords];  // the producer's
+    short par_p[kKv4MaxNodes];
+    short par[kKv4MaxNodes];            // the softmax warps'
+    uint32_t see[kKv4TreeWords][kRows];
+    float fac[kRows];
+    float ml[2][kRows][2];            // M, l of each stream
+    short er[2][kRows];               // E, and the row's NaN groups
+    uint8_t row_nan[2][kRows];
+};
+
+template <int NG>
+constexpr int smem_bytes() { return 1024 + Shape<NG>::AT_SMALL + static_cast<int>(sizeof(Small)); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }   // 2^e, normal
+__device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+template <int NW>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[NW]) {
+    if constexpr (NW == 4)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
+    else if constexpr (NW == 2)
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+    else
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a));
+}
+__device__ __forceinline__ void fence_proxy_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 32 lanes x 32 columns of 32 bit from tensor memory; the wait is tied to the outputs.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+        "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// d (+)= a b, both operands in shared memory, or a in tensor memory; fp16, K = 16.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+                 : "memory");
+}
+
+// Codes to fp16.  The 8 codes of a word, each half of an output pair 16 bits
+// apart: (0, 4), (1, 5), (2, 6), (3, 7), times the pair of scales d2: (bits | 1024)
+// - 1032, or (bits | 1024) / 16 - 72 where the bits lie 4 higher, are c - 8.
+__device__ __forceinline__ void decode8(uint32_t w, __half2 d2, uint32_t (&out)[4]) {
+    const uint32_t w8 = w >> 8;
+    const __half2 off = bits_h2(0x64086408u), div16 = bits_h2(0x2C002C00u), off16 = bits_h2(0xD480D480u);
+    out[0] = h2_bits(__hmul2(__hsub2(bits_h2(lop3_and_or(w, 0x000F000Fu, 0x64006400u)), off), d2));
+    out[1] = h2_bits(__hmul2(__hfma2(bits_h2(lop3_and_or(w, 0x00F000F0u, 0x64006400u)), div16, off16), d2));
+    out[2] = h2_bits(__hmul2(__hsub2(bits_h2(lop3_and_or(w8, 0x000F000Fu, 0x64006400u)), off), d2));
+    out[3] = h2_bits(__hmul2(__hfma2(bits_h2(lop3_and_or(w8, 0x00F000F0u, 0x64006400u)), div16, off16), d2));
+}
+// Larger of m and the two fp16 magnitudes of a word of scales, NaN and infinity left out.
+__device__ __forceinline__ uint32_t top_of(uint32_t m, uint32_t w) {
+    const uint32_t a = w & 0x7FFFu, b = (w >> 16) & 0x7FFFu;
+    return max(m, max(a < 0x7C00u ? a : 0u, b < 0x7C00u ? b : 0u));
+}
+// Exponent e with 2^e <= v < 2^(e + 1) of an fp16 magnitude's bits (subnormals: that of the smallest normal).
+__device__ __forceinline__ int exponent_of(uint32_t bits) { return max(1, static_cast<int>(bits >> 10)) - 15; }
+// Two scales times 2^-e, |e| <= 16, in two exact steps.
+struct Unit {
+    __half2 a, b;
+    __device__ __forceinline__ explicit Unit(int e) {
+        const int x = -e / 2, y = -e - x;
+        a = __half2half2(__ushort_as_half(static_cast<unsigned short>((x + 15) << 10)));
+        b = __half2half2(__ushort_as_half(static_cast<unsigned short>((y + 15) << 10)));
+    }
+    __device__ __forceinline__ uint32_t of(uint32_t w) const { return h2_bits(__hmul2(__hmul2(bits_h2(w), a), b)); }
+};
+
+// ------------------------------------------------------------------ the line
+// All tiles of all (sequence, kv head, row tile) items, kItemCost places before each.
+struct Line {
+    int b, h, ch;                     // the next chunk: sequence, item of it, chunk of that
+    int left;                         // chunks of this CTA still to come
+    int chunks, len, first;           // of sequence b
+};
+struct Piece {
+    int b, kvh, row0, rows, len, base;
+    int tile0, count;                 // first tile of the cache, tiles (0: a sequence without a tree)
+    int h, ch, chunks;
+};
+__device__ __forceinline__ int window_start(const Kv4Attn& p, int end) { return p.window > 0 && end > p.window ? end - p.window : 0; }
+__device__ __forceinline__ int length_of(const Kv4Attn& p, int b, bool& bad) {
+    const int cap = static_cast<int>(min(p.table ? static_cast<long long>(p.table_stride) * p.page_size : p.page_size, 0x7fffff00LL));
+    int len = __ldg(p.lens + b);
+    bad = len < 0 || len > cap;
+    if (bad) len = len < 0 ? 0 : cap;
+    return len < p.q_len ? 0 : len;   // no tree is there
+}
+template <int KT>
+__device__ __forceinline__ int first_tile(const Kv4Attn& p, int len) { return window_start(p, len - p.q_len + 1) / KT; }
+template <int KT>
+__device__ __forceinline__ int chunks_of(const Kv4Attn& p, int len) { return max(1, (len + KT - 1) / KT - first_tile<KT>(p, len)); }
+template <int KT>
+__device__ __forceinline__ void load_seq(Line& l, const Kv4Attn& p) {
+    bool bad;
+    l.len = length_of(p, l.b, bad);
+    l.first = first_tile<KT>(p, l.len);
+    l.chunks = chunks_of<KT>(p, l.len);
+}
+template <int KT>
+__device__ __forceinline__ bool next_piece(Line& l, const Kv4Attn& p, int items, Piece& pc) {
+    if (l.left <= 0) return false;
+    const int n = min(l.chunks - l.ch, l.left);
+    pc.b = l.b;
+    pc.h = l.h;
+    pc.ch = l.ch;
+    pc.chunks = l.chunks;
+    pc.kvh = l.h / p.row_tiles;
+    pc.row0 = (l.h - pc.kvh * p.row_tiles) * kRows;
+    pc.rows = min(kRows, p.q_len * p.group - pc.row0);
+    pc.len = l.len;
+    pc.base = l.len - p.q_len;
+    pc.tile0 = l.first + l.ch;
+    pc.count = l.len > 0 ? n : 0;
+    l.left -= n;
+    l.ch += n;
+    if (l.ch >= l.chunks) {
+        l.ch = 0;
+        if (++l.h == items) {
+            l.h = 0;
+            if (++l.b < p.batch && l.left > 0) load_seq<KT>(l, p);
+        }
+    }
+    return true;
+}
+
+struct Cut {                          // an item cut over CTAs: its first CTA, their number, the item
+    int n, b, h;
+};
+
+template <int NG>
+__global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const Kv4Attn p, Cut* cuts) {
+    using F = Shape<NG>;
+    constexpr int D = F::D, KT = F::KT;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Small& s = *reinterpret_cast<Small*>(smem + F::AT_SMALL);
+    volatile int* const gave_up = &s.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(s.raw_full + i, 1);
+            mbar_init(s.raw_empty + i, 8);
+            mbar_init(s.ek_full + i, 4);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s.k_full + i, 4);
+            mbar_init(s.k_empty + i, 1);
+            mbar_init(s.v_full + i, 4);
+            mbar_init(s.v_empty + i, 1);
+            mbar_init(s.s_full + i, 1);
+            mbar_init(s.p_full + i, 4);
+            mbar_init(s.pv_done + i, 1);
+        }
+        mbar_init(&s.q_full, F::SOFT);
+        mbar_init(&s.done, 1);
+        s.abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == F::WARPS - 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tcg::tc_fence_before();
+    __syncthreads();
+    tcg::tc_fence_after();
+    const uint32_t tmem = static_cast<uint32_t>(*reinterpret_cast<volatile int*>(&s.tmem));
+    pdl_wait();
+
+    // ---------------------------------------------------------- this CTA's part of the line
+    const int items = p.kv_heads * p.row_tiles;
+    auto scan = [&](int n, int before, int& incl) {   // inclusive prefix sum of the threads' n, behind `before`; their total
+        incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        __syncthreads();
+        if (lane == 31) s.sum[warp] = incl;
+        __syncthreads();
+        int total = 0;
+        incl += before;
+        for (int w = 0; w < F::WARPS; ++w) {
+            if (w < warp) incl += s.sum[w];
+            total += s.sum[w];
+        }
+        return total;
+    };
+    auto width_of = [&](int b) {
+        bool bad = false;
+        const int n = b < p.batch ? chunks_of<KT>(p, length_of(p, b, bad)) + kItemCost : 0;
+        if (bad && blockIdx.x == 0) record_fault(ALJ_FAULT_BOUNDS);
+        return n;
+    };
+    int total = 0, incl;
+    for (int b0 = 0; b0 < p.batch; b0 += F::THREADS) total += scan(width_of(b0 + threadIdx.x), 0, incl);
+    total *= items;                   // < 2^31: checked on the host for the longest sequences
+    const int ctas = min(static_cast<int>(gridDim.x), (total + kItemCost) / (kItemCost + 1));
+    const int share = total / ctas, rem = total - share * ctas;
+    auto start_of = [&](int c) { return share * c + min(c, rem); };
+    auto cta_at = [&](int x) {
+        const int wide = rem * (share + 1);
+        return x < wide ? x / (share + 1) : rem + (x - wide) / share;
+    };
+    if (threadIdx.x == 0) cuts[blockIdx.x].n = 0;
+    Line line = {};
+    if (static_cast<int>(blockIdx.x) < ctas) {
+        const int x0 = start_of(blockIdx.x), x1 = start_of(blockIdx.x + 1);
+        int before = 0;               // line places before the sequences at hand, of one item
+        for (int b0 = 0; b0 < p.batch; b0 += F::THREADS) {
+            const int n = width_of(b0 + threadIdx.x);
+            before += scan(n, before, incl);
+            const int pre = incl - n;
+            if (n > 0 && pre * items <= x0 && x0 < incl * items) {
+                s.start[0] = b0 + threadIdx.x;
+                s.start[1] = pre;
+            }
+        }
+        __syncthreads();
+        line.b = s.start[0];
+        load_seq<KT>(line, p);
+        const int pre = s.start[1], width = line.chunks + kItemCost, rest = x0 - pre * items;
+        line.h = rest / width;
+        const int at = rest - line.h * width;
+        line.ch = max(0, at - kItemCost);
+        // the chunks between x0 and x1: places less what of the items' costs lies there
+        Line l = line;
+        int x = x0 - at + kItemCost + line.ch, n = 0;   // place of the next chunk
+        while (x < x1) {
+            const int m = min(l.chunks - l.ch, x1 - x);
+            n += m;
+            x += l.chunks - l.ch + kItemCost;
+            l.ch = 0;
+            if (++l.h == items) {
+                l.h = 0;
+                if (++l.b == p.batch) break;
+                load_seq<KT>(l, p);
+            }
+        }
+        line.left = n;
+    }
+    // place of item h's first chunk on the line; only for the piece's own sequence
+    const int my_pre = static_cast<int>(blockIdx.x) < ctas ? s.start[1] : 0;
+
+    const uint32_t at_q = smem_u32(smem), at_k = at_q + F::AT_K, at_v = at_q + F::AT_V, at_raw = at_q + F::AT_RAW;
+    Piece pc;
+    bool ok = true;
+
+    if (warp < F::SOFT) {
+        // ------------------------------------------------------ softmax
+        const int stream = warp >> 2, row = (warp & 3) * 32 + lane, thread = threadIdx.x;
+        const uint32_t tq = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const float inv_cap = p.soft_cap > 0.0f ? 1.0f / p.soft_cap : 0.0f;
+        const float size = fabsf(p.scale) * (p.soft_cap > 0.0f ? 1.0f : kLog2e);
+        auto sync = [&] { named_bar(1, 32 * F::SOFT); };
+        int tiles = 0;                // of this CTA before the piece
+        int uses0 = 0, uses1 = 0;     // uses of the two S buffers before the piece
+        int pre = my_pre, seq = line.b;
+        while (next_piece<KT>(line, p, items, pc)) {
+            if (pc.b != seq) {        // the line's places before sequence pc.b
+                for (; seq < pc.b; ++seq) {
+                    bool bad;
+                    pre += chunks_of<KT>(p, length_of(p, seq, bad)) + kItemCost;
+                }
+            }
+            const bool whole = pc.ch == 0 && (pc.count == pc.chunks || pc.count == 0);
+            const int line0 = pre * items + pc.h * (pc.chunks + kItemCost) + kItemCost;
+            // -------------------------------------------------- the rows' masks and Q
+            for (int i = thread; i < p.q_len; i += 32 * F::SOFT)
+                s.par[i] = static_cast<short>(tree_parent(p.parents + static_cast<long long>(pc.b) * p.parents_stride, i));
+            sync();
+            const int node = (pc.row0 + row) / p.group;
+            int depth = 0;
+            if (pc.count > 0 && row < pc.rows) {
+                uint32_t see[kKv4TreeWords];
+#pragma unroll
+                for (int i = 0; i < kKv4TreeWords; ++i) see[i] = 0u;
+                int t = node;
+                for (; t >= 0; t = s.par[t], ++depth)
+                    if (p.window == 0 || depth < p.window) {
+#pragma unroll
+                        for (int i = 0; i < kKv4TreeWords; ++i) see[i] |= (t >> 5) == i ? 1u << (t & 31) : 0u;
+                    }
+                if (t != -1) depth = 0;
+                if (stream == 0) {
+#pragma unroll
+                    for (int i = 0; i < kKv4TreeWords; ++i) s.see[i][row] = depth > 0 ? see[i] : 0u;
+                }
+            }
+            const bool alive = depth > 0;
+            const int row_lo = window_start(p, pc.base + depth);          // first position the row sees
+            const int all_lo = window_start(p, pc.len);
+            if (pc.count > 0) {
+                constexpr int kChunks = D / 8, kPer = 32 / kChunks;       // 16-byte chunks of a row, rows of a warp's pass
+                constexpr int kBatch = kRows / kPer / F::SOFT < 8 ? kRows / kPer / F::SOFT : 8;
+                const int j = lane % kChunks;
+                for (int r0 = 0; r0 < kRows / kPer; r0 += kBatch * F::SOFT) {
+                    uint4 x[kBatch];
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+                        const int r = (r0 + k * F::SOFT + warp) * kPer + lane / kChunks, i = pc.row0 + r;
+                        x[k] = make_uint4(0u, 0u, 0u, 0u);
+                        if (r < pc.rows) {
+                            const int t = i / p.group, hd = i - t * p.group;
+                            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) +
+                                (static_cast<long long>(pc.b) * p.q_len + t) * p.q_stride +
+                                static_cast<long long>(pc.kvh * p.group + hd) * D + 8 * j;
+                            if ((reinterpret_cast<uintptr_t>(q) & 15) == 0) {
+                                x[k] = *reinterpret_cast<const uint4*>(q);
+                            } else {
+                                const unsigned short* h = reinterpret_cast<const unsigned short*>(q);
+                                x[k] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+                        const int r = (r0 + k * F::SOFT + warp) * kPer + lane / kChunks;
+                        const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+                        float v[8], big = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            v[2 * i] = __uint_as_float(w[i] << 16);
+                            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(v[i]));
+#pragma unroll
+                        for (int o = 1; o < kChunks; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                        // the row times 2^f: its largest in [2^14, 2^15), where both 2^f and 2^-f are normal
+                        const int f = big > 0.0f ? max(-100, min(126, 14 - (static_cast<int>((__float_as_uint(big) >> 23) & 255) - 127))) : 0;
+                        const float up = p.scale < 0.0f ? -pow2i(f) : pow2i(f);
+                        if (j == 0) s.fac[r] = size * pow2i(-f);
+                        uint32_t out[4];              // as decode8 orders the dims of a chunk
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) out[i] = h2_bits(__floats2half2_rn(v[i] * up, v[i + 4] * up));
+                        sts128(at_q + (j >> 3) * (kRows * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4), make_uint4(out[0], out[1], out[2], out[3]));
+                    }
+                }
+            }
+            fence_proxy_shared();
+            __syncwarp();
+            if (lane == 0 && pc.count > 0) mbar_arrive(&s.q_full);
+            sync();                                               // masks and factors
+            const float fac = pc.count > 0 ? s.fac[row] : 0.0f;
+            float M = kNone, l = 0.0f;
+            int E = -100, nan_groups = 0;
+            const bool warp_lives = (warp & 3) * 32 < pc.rows;
+            // bits of the positions from at on that the row sees
+            auto visible = [&](int at) {
+                uint32_t bits = 0u;
+                const int rel = at - pc.base;
+                if (rel < 0 && alive) {
+                    bits = rel <= -32 ? 0xFFFFFFFFu : (1u << -rel) - 1u;
+                    const int skip = row_lo - at;
+                    if (skip > 0) bits = skip >= 32 ? 0u : bits & (0xFFFFFFFFu << skip);
+                }
+                if (rel > -32 && rel < p.q_len && alive) {
+                    const int i = max(rel, 0) >> 5, sh = rel & 31;
+                    const uint32_t a = s.see[i][row], b = i + 1 < kKv4TreeWords ? s.see[i + 1][row] : 0u;
+                    bits |= rel < 0 ? a << -rel : __funnelshift_r(a, b, sh);
+                }
+                return bits;
+            };
+            // -------------------------------------------------- its tiles
+            for (int i = stream; i < pc.count; i += F::STREAMS) {
+                const int buf = i & 1, use = (buf ? uses1 : uses0) + (i >> 1), tile = tiles + i;
+                const int meta = tile & (kMeta - 1), pos = (pc.tile0 + i) * KT;
+                const uint32_t ts = tq + buf * KT, to = tq + F::O_COL + (F::STREAMS == 2 ? stream * D : 0);
+                ok = ok && tcg::warp_wait(s.s_full + buf, use & 1, gave_up);
+                ok = ok && tcg::warp_wait(s.ek_full + meta, (tile / kMeta) & 1, gave_up);
+                ok = ok && tcg::warp_wait(s.v_full + tile % F::V_STAGES, (tile / F::V_STAGES) & 1, gave_up);
+                if (ok && warp_lives) {
+                    tcg::tc_fence_after();
+                    const bool edge = pos < all_lo || pos + KT > pc.base;
+                    float mx = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < KT / 32; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(ts + 32 * c, v);
+                        const float fc = fac * pow2i(s.ek[meta][c]);
+                        if (p.soft_cap > 0.0f) {
+#pragma unroll 4
+                            for (int k = 0; k < 32; ++k)
+                                v[k] = __float_as_uint(tanhf(__uint_as_float(v[k]) * fc * inv_cap) * (p.soft_cap * kLog2e));
+                            tcg::tmem_st32(ts + 32 * c, v);
+                            tcg::tmem_wait_st();
+                        }
+                        float m = -INFINITY;
+                        if (edge) {
+                            const uint32_t bits = visible(pos + 32 * c);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) m = fmaxf(m, (bits >> k) & 1u ? __uint_as_float(v[k]) : -INFINITY);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) m = fmaxf(m, __uint_as_float(v[k]));
+                        }
+                        mx = fmaxf(mx, m == -INFINITY || p.soft_cap > 0.0f ? m : m * fc);
+                    }
+                    const int e_new = max(s.ev[meta][0], KT == 128 ? s.ev[meta][1] : -100);
+                    const bool higher = e_new > E + kSlack, rise = mx > M + kLazy;
+                    if (__any_sync(0xffffffffu, rise) || higher) {
+                        const float now = rise ? mx : M, f = ex2(M - now);
+                        const int e = higher ? e_new : E;
+                        l *= f;
+                        if (i >= F::STREAMS) {                        // what has been summed up, to the new reference
+                            const int last = i - F::STREAMS, pb = last & 1;
+                            ok = ok && tcg::warp_wait(s.pv_done + pb, ((pb ? uses1 : uses0) + (last >> 1)) & 1, gave_up);
+                            tcg::tc_fence_after();
+                            const float g = f * pow2i(E - e);
+#pragma unroll 1
+                            for (int c = 0; c < NG; ++c) {
+                                uint32_t v[32];
+                                tmem_ld32(to + 32 * c, v);
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * g);
+                                tcg::tmem_st32(to + 32 * c, v);
+                            }
+                        }
+                        M = now;
+                        E = e;
+                    }
+#pragma unroll 1
+                    for (int c = 0; c < KT / 32; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(ts + 32 * c, v);
+                        const float fc = p.soft_cap > 0.0f ? 1.0f : fac * pow2i(s.ek[meta][c]);
+                        const int sh = kBias + s.ev[meta][c >> 1] - E;
+                        const float at = static_cast<float>(sh) - M;
+                        float part[4] = {};
+                        uint32_t out[16];
+                        if (edge) {
+                            const uint32_t bits = visible(pos + 32 * c);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k)
+                                v[k] = (bits >> k) & 1u ? v[k] : 0xFF800000u;
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) {            // a factor of zero times -infinity is no score
+                                const float y = ex2(fmaf(__uint_as_float(v[k]), fc, at));
+                                v[k] = (bits >> k) & 1u ? __float_as_uint(y) : 0u;
+                            }
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(ex2(fmaf(__uint_as_float(v[k]), fc, at)));
+                        }
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float a = __uint_as_float(v[2 * k]), b = __uint_as_float(v[2 * k + 1]);
+                            part[(2 * k) & 3] += a;
+                            part[(2 * k + 1) & 3] += b;
+                            out[k] = h2_bits(__floats2half2_rn(a, b));
+                        }
+                        l = fmaf((part[0] + part[1]) + (part[2] + part[3]), pow2i(-sh), l);
+                        tmem_st16(ts + 16 * c, out);                  // columns that this lane has read
+                    }
+                    if (s.nan_any[meta][0] || (KT == 128 && s.nan_any[meta][1])) {
+                        for (int k = 0; k < KT; ++k) {
+                            const int g = s.nan[meta][k];
+                            if (g && (edge ? (visible(pos + (k & ~31)) >> (k & 31)) & 1u : alive)) nan_groups |= g;
+                        }
+                    }
+                    tcg::tmem_wait_st();
+                }
+                tcg::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s.p_full + buf);
+            }
+            // -------------------------------------------------- the streams' results, and the rows' outputs
+            const int n0 = (pc.count + 1) >> 1, n1 = pc.count >> 1;   // uses of the buffers
+            if (n0 > 0) ok = ok && tcg::warp_wait(s.pv_done, (uses0 + n0 - 1) & 1, gave_up);
+            if (n1 > 0) ok = ok && tcg::warp_wait(s.pv_done + 1, (uses1 + n1 - 1) & 1, gave_up);
+            s.ml[stream][row][0] = M;
+            s.ml[stream][row][1] = l;
+            s.er[stream][row] = static_cast<short>(E);
+            s.row_nan[stream][row] = static_cast<uint8_t>(nan_groups);
+            sync();
+            tcg::tc_fence_after();
+            uses0 += n0;
+            uses1 += n1;
+            tiles += pc.count;
+            const int i = pc.row0 + row;
+            const bool two = F::STREAMS == 2 && pc.count > 1;
+            float w0 = 0.0f, w1 = 0.0f, L = 0.0f, top = kNone;
+            int gone = 0;
+            if (alive && pc.count > 0) {
+                const float m0 = s.ml[0][row][0], m1 = two ? s.ml[1][row][0] : kNone;
+                top = fmaxf(m0, m1);
+                w0 = ex2(m0 - top);
+                w1 = two ? ex2(m1 - top) : 0.0f;
+                L = s.ml[0][row][1] * w0 + (two ? s.ml[1][row][1] * w1 : 0.0f);
+                w0 *= pow2i(max(-126, s.er[0][row] - kBias));
+                if (two) w1 *= pow2i(max(-126, s.er[1][row] - kBias));
+                gone = s.row_nan[0][row] | (two ? s.row_nan[1][row] : 0);
+            }
+            int slot = 0;
+            if (!whole) {
+                const int cta0 = cta_at(line0), cta1 = cta_at(line0 + pc.chunks - 1);
+                slot = static_cast<int>(blockIdx.x) * 2 + (static_cast<int>(blockIdx.x) == cta0 ? 1 : 0);
+                if (static_cast<int>(blockIdx.x) == cta0 && thread == 0) cuts[cta0] = Cut{cta1 - cta0 + 1, pc.b, pc.h};
+            }
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            constexpr int kCols = D / F::STREAMS;                     // columns of a warp
+            if (ok && warp_lives) {
+#pragma unroll 1
+                for (int c = 0; c < kCols / 32; ++c) {
+                    const int d = stream * kCols + 32 * c;
+                    float o[32];
+                    uint32_t v[32];
+                    if (pc.count > 0) {
+                        tmem_ld32(tq + F::O_COL + d, v);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(v[k]) * w0;
+                    }
+                    if (two) {
+                        tmem_ld32(tq + F::O_COL + D + d, v);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = fmaf(__uint_as_float(v[k]), w1, o[k]);
+                    }
+                    const bool nan = (gone >> (d >> 5)) & 1;
+                    if (row < pc.rows) {
+                        if (whole) {
+                            const int t = i / p.group, hd = i - t * p.group;
+                            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) +
+                                (((static_cast<long long>(pc.b) * p.q_len + t) * p.kv_heads + pc.kvh) * p.group + hd) * D + d;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                uint32_t h[4];
+#pragma unroll
+                                for (int n = 0; n < 4; ++n) {
+                                    const float a = inv == 0.0f ? 0.0f : o[8 * k + 2 * n] * inv;    // a row that sees nothing
+                                    const float b = inv == 0.0f ? 0.0f : o[8 * k + 2 * n + 1] * inv;
+                                    const __nv_bfloat162 r2 = __floats2bfloat162_rn(a, b);
+                                    h[n] = nan ? 0x7FC07FC0u : *reinterpret_cast<const uint32_t*>(&r2);
+                                }
+                                reinterpret_cast<uint4*>(out)[k] = make_uint4(h[0], h[1], h[2], h[3]);
+                            }
+                        } else {
+                            float* part = p.part + static_cast<long long>(slot) * (kRows * (D + 2)) + row * D + d;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                reinterpret_cast<float4*>(part)[k] =
+                                    nan ? make_float4(NAN, NAN, NAN, NAN)
+                                    : alive ? make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3])
+                                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        }
+                    }
+                }
+                if (!whole && stream == 0 && row < pc.rows) {
+                    float* part = p.part + static_cast<long long>(slot) * (kRows * (D + 2)) + kRows * D + row * 2;
+                    part[0] = top;
+                    part[1] = L;
+                }
+            }
+            tcg::tc_fence_before();
+            sync();                                               // tensor memory and the tables are read
+        }
+    } else if (warp < F::SOFT + 4) {
+        // ------------------------------------------------------ K to fp16
+        constexpr int GW = NG == 8 ? 4 : NG;                      // groups of a warp
+        const int kw = warp - F::SOFT, span = KT == 128 ? kw : kw & 1, half = KT == 128 ? 0 : kw >> 1;
+        const int c = lane & 3, pos_in = (lane >> 3) + (lane & 4);
+        int tile = 0;
+        while (next_piece<KT>(line, p, items, pc)) {
+            for (int i = 0; i < pc.count; ++i, ++tile) {
+                const int slot = tile % F::RAW, ks = tile & 1;
+                ok = ok && tcg::warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
+                if (tile >= 2) ok = ok && tcg::warp_wait(s.k_empty + ks, ((tile >> 1) - 1) & 1, gave_up);
+                if (!ok) break;
+                const uint32_t raw = at_raw + slot * F::RAW_BYTES;
+                const uint32_t valid = s.valid[slot][span];
+                uint32_t top = 0u;
+                if ((valid >> lane) & 1u) {                       // a lane a position
+                    uint32_t w[NG / 2];
+                    lds_words<NG / 2>(raw + F::K_SC + (32 * span + lane) * (2 * NG), w);
+#pragma unroll
+                    for (int k = 0; k < NG / 2; ++k) top = top_of(top, w[k]);
+                }
+                const int e = exponent_of(__reduce_max_sync(0xffffffffu, top));
+                const Unit unit(e);
+                if (lane == 0) s.ek[tile & (kMeta - 1)][span] = e;
+                const uint32_t to = at_k + ks * F::KHAT;
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    const int at = 8 * it + pos_in, r = 32 * span + at;
+                    uint32_t w[GW], d[GW / 2];
+                    lds_words<GW>(raw + r * (D / 2) + c * (4 * NG) + half * 16, w);
+                    lds_words<GW / 2>(raw + F::K_SC + r * (2 * NG) + half * 8, d);
+                    const bool live = (valid >> at) & 1u;
+#pragma unroll
+                    for (int g = 0; g < GW; ++g) {
+                        if ((g & 1) == 0) d[g / 2] = live ? unit.of(d[g / 2]) : 0u;
+                        uint32_t out[4];
+                        decode8(w[g], bits_h2(__byte_perm(d[g / 2], 0u, g & 1 ? 0x3232 : 0x1010)), out);
+                        const int j = 4 * (4 * half + g) + c;
+                        sts128(to + (j >> 3) * (KT * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4), make_uint4(out[0], out[1], out[2], out[3]));
+                    }
+                }
+                fence_proxy_shared();
+                __syncwarp();
+                if (lane == 0) {
+                    // the exponents of tile n - kMeta have been read: S of tile n - 2 was issued after its P
+                    mbar_arrive(s.ek_full + (tile & (kMeta - 1)));
+                    mbar_arrive(s.k_full + ks);
+                    mbar_arrive(s.raw_empty + slot);
+                }
+            }
+            if (!ok) break;
+        }
+    } else if (warp < F::SOFT + 8) {
+        // ------------------------------------------------------ V to fp16, transposed
+        constexpr int WP = NG == 2 ? 1 : 2;                       // words of a thread
+        const int vw = warp - F::SOFT - 4, part = KT == 128 ? vw & 1 : 0;
+        const int wp = (KT == 128 ? vw >> 1 : vw) * 4 + (lane >> 3), j = lane & 7;
+        int tile = 0;
+        while (next_piece<KT>(line, p, items, pc)) {
+            for (int i = 0; i < pc.count; ++i, ++tile) {
+                const int slot = tile % F::RAW, vs = tile % F::V_STAGES, meta = tile & (kMeta - 1);
+                ok = ok && tcg::warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
+                if (tile >= F::V_STAGES) ok = ok && tcg::warp_wait(s.v_empty + vs, (tile / F::V_STAGES - 1) & 1, gave_up);
+                if (!ok) break;
+                const uint32_t raw = at_raw + slot * F::RAW_BYTES;
+                uint32_t top = 0u;
+                bool nan = false;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {                     // two positions a lane
+                    const int r = 64 * part + 32 * k + lane;
+                    if ((s.valid[slot][2 * part + k] >> lane) & 1u) {
+                        uint32_t w[NG / 2];
+                        lds_words<NG / 2>(raw + F::V_SC + (r >> 3) * F::SB + (r & 7) * (2 * NG), w);
+                        int bad = 0;
+#pragma unroll
+                        for (int n = 0; n < NG / 2; ++n) {
+                            top = top_of(top, w[n]);
+                            bad |= ((w[n] & 0x7FFFu) >= 0x7C00u ? 1 : 0) << (2 * n) | (((w[n] >> 16) & 0x7FFFu) >= 0x7C00u ? 1 : 0) << (2 * n + 1);
+                        }
+                        nan |= bad != 0;
+                        s.nan[meta][r] = static_cast<uint8_t>(bad);   // the two warps of these positions write the same
+                    } else {
+                        s.nan[meta][r] = 0;
+                    }
+                }
+                const int e = exponent_of(__reduce_max_sync(0xffffffffu, top));
+                const bool any_nan = __any_sync(0xffffffffu, nan);
+                const Unit unit(e);
+                if (lane == 0) {
+                    s.ev[meta][part] = e;
+                    s.nan_any[meta][part] = any_nan;
+                }
+                const uint32_t live = (s.valid[slot][2 * part + (j >> 2)] >> (8 * (j & 3))) & 255u;   // of the thread's 8 positions
+                const uint32_t blk = raw + F::V_CODES + (8 * part + j) * F::VB + wp * (4 * WP);
+                const uint32_t sc = raw + F::V_SC + (8 * part + j) * F::SB + (NG == 8 ? (wp & 1) * 8 : 0);
+                const uint32_t to = at_v + vs * F::VHAT + part * (D * 128);
+                uint32_t code[8][WP], d[8][WP];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    lds_words<WP>(blk + k * (D / 2), code[k]);
+                    lds_words<WP>(sc + k * (2 * NG), d[k]);
+#pragma unroll
+                    for (int n = 0; n < WP; ++n) {
+                        if (any_nan) {                            // NaN as zero: its rows are marked
+                            if ((d[k][n] & 0x7FFFu) >= 0x7C00u) d[k][n] &= 0xFFFF0000u;
+                            if (((d[k][n] >> 16) & 0x7FFFu) >= 0x7C00u) d[k][n] &= 0x0000FFFFu;
+                        }
+                        d[k][n] = (live >> k) & 1u ? unit.of(d[k][n]) : 0u;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < WP; ++n)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t pick = x ? 0x7632 : 0x5410;
+                        uint32_t out[4][4];                       // [dim][pair of positions]
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t v[4];
+                            decode8(__byte_perm(code[2 * k][n], code[2 * k + 1][n], pick),
+                                    bits_h2(__byte_perm(d[2 * k][n], d[2 * k + 1][n], pick)), v);
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) out[m][k] = v[m];
+                        }
+                        const int hw = 2 * (WP * wp + n) + x, dim = 32 * (hw % NG) + 4 * (hw / NG);
+#pragma unroll
+                        for (int m = 0; m < 4; ++m)
+                            sts128(to + (dim + m) * 128 + ((j ^ ((dim + m) & 7)) << 4), make_uint4(out[m][0], out[m][1], out[m][2], out[m][3]));
+                    }
+                fence_proxy_shared();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(s.v_full + vs);
+                    mbar_arrive(s.raw_empty + slot);
+                }
+            }
+            if (!ok) break;
+        }
+    } else if (warp == F::WARPS - 2) {
+        // ------------------------------------------------------ codes and scales from the cache
+        int tile = 0, seq = -1;
+        while (next_piece<KT>(line, p, items, pc)) {
+            const int lo = window_start(p, pc.base + 1);
+            for (int i = 0; i < pc.count; ++i, ++tile) {
+                const int slot = tile % F::RAW, pos0 = (pc.tile0 + i) * KT;
+                const int blk = lane >> 2, k = lane & 3, pos = pos0 + 16 * blk;
+                // lane 4 n + k copies a part of the n-th 16 positions; their page on its way while the slot empties
+                int page = -1, off = 0;
+                const bool there = 16 * blk < KT && pos < pc.len;
+                if (there) {
+                    const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
+                    page = p.table ? __ldg(p.table + static_cast<long long>(pc.b) * p.table_stride + pi) : pc.b;
+                    off = pos - pi * p.page_size;
+                }
+                const bool has = there && page >= 0 && page < p.pages;
+                if (there && !has && k == 0) record_fault(ALJ_FAULT_BOUNDS);
+                if (pos0 + KT > pc.base && seq != pc.b) {         // which nodes are there: those whose ancestors all are
+                    seq = pc.b;
+                    __syncwarp();
+                    for (int t = lane; t < p.q_len; t += 32)
+                        s.par_p[t] = static_cast<short>(tree_parent(p.parents + static_cast<long long>(pc.b) * p.parents_stride, t));
+                    __syncwarp();
+                    for (int w = 0; w < kKv4TreeWords; ++w) {
+                        int t = 32 * w + lane < p.q_len ? 32 * w + lane : -2;
+                        while (t >= 0) t = s.par_p[t];
+                        const uint32_t bits = __ballot_sync(0xffffffffu, t == -1);
+                        if (lane == 0) s.node_ok[w] = bits;
+                    }
+                    __syncwarp();
+                }
+                uint32_t bits = 0u;                               // valid ones of the 16 positions
+                if (has) {
+                    if (pos >= lo && pos + 16 <= pc.base) {
+                        bits = 0xFFFFu;
+                    } else {
+                        for (int n = 0; n < 16; ++n) {
+                            const int node = pos + n - pc.base;
+                            const bool v = pos + n >= lo && (node < 0 || (node < p.q_len && ((s.node_ok[node >> 5] >> (node & 31)) & 1u)));
+                            bits |= static_cast<uint32_t>(v) << n;
+                        }
+                    }
+                }
+                const uint32_t upper = __shfl_down_sync(0xffffffffu, bits, 4);
+                if (tile >= F::RAW) ok = ok && tcg::warp_wait(s.raw_empty + slot, (tile / F::RAW - 1) & 1, gave_up);
+                if (!ok) break;
+                if ((lane & 7) == 0) s.valid[slot][lane >> 3] = bits | upper << 16;
+                const int blocks = __popc(__ballot_sync(0xffffffffu, has)) / 4;
+                __syncwarp();
+                if (lane == 0) mbar_arrive_expect_tx(s.raw_full + slot, blocks * F::BLOCK_BYTES);
+                __syncwarp();
+                if (has && k < 3) {
+                    uint8_t* dst = smem + F::AT_RAW + slot * F::RAW_BYTES;
+                    const uint8_t* src = p.cache + (static_cast<long long>(page) * p.kv_heads + pc.kvh) * kv4_block_bytes(p.page_size, D);
+                    const long long ps = p.page_size;
+                    if (k == 0) {
+                        bulk_g2s(dst + blk * (8 * D), src + off * (D / 2LL), 8 * D, s.raw_full + slot);
+                        bulk_g2s(dst + F::K_SC + blk * (32 * NG), src + ps * D + off * (2LL * NG), 32 * NG, s.raw_full + slot);
+                    } else {
+                        const int b8 = 2 * blk + k - 1, o8 = off + 8 * (k - 1);
+                        bulk_g2s(dst + F::V_CODES + b8 * F::VB, src + (ps + o8) * (D / 2), 4 * D, s.raw_full + slot);
+                        bulk_g2s(dst + F::V_SC + b8 * F::SB, src + ps * D + (ps + o8) * (2 * NG), 16 * NG, s.raw_full + slot);
+                    }
+                }
+            }
+            if (!ok) break;
+        }
+        if (!ok)                          // the copies under way end before the CTA does
+            for (int t = max(0, tile - F::RAW); t < tile; ++t) mbar_wait(s.raw_full + t % F::RAW, (t / F::RAW) & 1);
+    } else {
+        // ------------------------------------------------------ MMA issue
+        if (lane == 0) {
+            constexpr uint32_t kS = tcg::idesc_f16(KT), kO = tcg::idesc_f16(D);
+            int tile = 0, pieces = 0, uses0 = 0, uses1 = 0;
+            while (ok && next_piece<KT>(line, p, items, pc)) {
+                if (pc.count == 0) continue;
+                auto scores = [&](int i) {
+                    const int t = tile + i, ks = t & 1, buf = i & 1;
+                    ok = ok && tcg::wait_bar(s.k_full + ks, (t >> 1) & 1, gave_up);
+                    if (!ok) return;
+                    tcg::tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        mma_ss(tmem + buf * KT, tcg::sdesc(at_q + (k >> 2) * (kRows * 128) + (k & 3) * 32),
+                               tcg::sdesc(at_k + ks * F::KHAT + (k >> 2) * (KT * 128) + (k & 3) * 32), kS, k > 0);
+                    tcg::tc_commit(s.k_empty + ks);
+                    tcg::tc_commit(s.s_full + buf);
+                };
+                ok = ok && tcg::wait_bar(&s.q_full, pieces & 1, gave_up);
+                ++pieces;
+                if (ok) scores(0);
+                if (ok && pc.count > 1) scores(1);
+                for (int i = 0; ok && i < pc.count; ++i) {
+                    const int t = tile + i, vs = t % F::V_STAGES, buf = i & 1, use = (buf ? uses1 : uses0) + (i >> 1);
+                    ok = ok && tcg::wait_bar(s.v_full + vs, (t / F::V_STAGES) & 1, gave_up);
+                    ok = ok && tcg::wait_bar(s.p_full + buf, use & 1, gave_up);
+                    if (!ok) break;
+                    tcg::tc_fence_after();
+                    const uint32_t to = tmem + F::O_COL + (F::STREAMS == 2 ? buf * D : 0);
+#pragma unroll
+                    for (int k = 0; k < KT / 16; ++k)
+                        mma_ts(to, tmem + buf * KT + 8 * k, tcg::sdesc(at_v + vs * F::VHAT + (k >> 2) * (D * 128) + (k & 3) * 32), kO,
+                               i >= F::STREAMS || k > 0);
+                    tcg::tc_commit(s.v_empty + vs);
+                    tcg::tc_commit(s.pv_done + buf);
+                    if (i + 2 < pc.count) scores(i + 2);
+                }
+                uses0 += (pc.count + 1) >> 1;
+                uses1 += pc.count >> 1;
+                tile += pc.count;
+            }
+            tcg::tc_commit(&s.done);      // every MMA issued has completed before tensor memory is released
+            mbar_wait(&s.done, 0);
+        }
+        __syncwarp();
+    }
+    tcg::tc_fence_before();
+    __syncthreads();
+    if (warp == F::WARPS - 1) {
+        tcg::tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// Items cut over CTAs: block (c, y) joins 16 rows of the item that CTA c began and others went on with, in CTA order.
+constexpr int kJoinRows = 16;
+template <int D>
+__global__ void __launch_bounds__(256) kv4_tree_join_kernel(const Kv4Attn p, const Cut* cuts) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const Cut cut = cuts[blockIdx.x];
+    if (cut.n <= 1) return;
+    const int kvh = cut.h / p.row_tiles, row0 = (cut.h - kvh * p.row_tiles) * kRows;
+    const int rows = min(kRows, p.q_len * p.group - row0);
+    const long long size = kRows * (D + 2);
+    auto base = [&](int k) { return p.part + (2 * (static_cast<long long>(blockIdx.x) + k) + (k == 0 ? 1 : 0)) * size; };
+    constexpr int kQuads = D / 4;
+    for (int i = threadIdx.x; i < kJoinRows * kQuads; i += 256) {
+        const int row = blockIdx.y * kJoinRows + i / kQuads, d = (i % kQuads) * 4;
+        if (row >= rows) break;
+        float top = kNone, L = 0.0f;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int k = 0; k < cut.n; ++k) {
+            const float* part = base(k);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + kRows * D + row * 2));
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + row * D + d));
+            const float now = fmaxf(top, ml.x), f = ex2(top - now), g = ex2(ml.x - now);
+            top = now;
+            L = fmaf(L, f, ml.y * g);
+            sum.x = fmaf(sum.x, f, v.x * g);
+            sum.y = fmaf(sum.y, f, v.y * g);
+            sum.z = fmaf(sum.z, f, v.z * g);
+            sum.w = fmaf(sum.w, f, v.w * g);
+        }
+        const float inv = 1.0f / L;
+        const bool none = L == 0.0f;
+        const __nv_bfloat162 a = __floats2bfloat162_rn(none ? 0.0f : sum.x * inv, none ? 0.0f : sum.y * inv);
+        const __nv_bfloat162 b = __floats2bfloat162_rn(none ? 0.0f : sum.z * inv, none ? 0.0f : sum.w * inv);
+        const int r = row0 + row, t = r / p.group, hd = r - t * p.group;
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) +
+                             (((static_cast<long long>(cut.b) * p.q_len + t) * p.kv_heads + kvh) * p.group + hd) * D + d;
+        *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+}
+
+template <int NG>
+cudaError_t launch_tree(const Kv4Attn& p, Cut* cuts, int sms, cudaStream_t stream) {
+    using F = Shape<NG>;
+    static_assert(smem_bytes<NG>() <= 232448, "shared memory of a CTA");
+    static bool configured[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!configured[dev & 63]) {
+        const cudaError_t e = cudaFuncSetAttribute(kv4_tree_kernel<NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<NG>());
+        if (e != cudaSuccess) return e;
+        configured[dev & 63] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms);
+    cfg.blockDim = dim3(F::THREADS);
+    cfg.dynamicSmemBytes = smem_bytes<NG>();
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_tree_kernel<NG>, p, cuts);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3(sms, (std::min(kRows, p.q_len * p.group) + kJoinRows - 1) / kJoinRows);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, kv4_tree_join_kernel<F::D>, p, static_cast<const Cut*>(cuts));
+}
+
+}  // namespace
+
+size_t kv4_tree_workspace_bytes(int q_rows, int head_dim, int sms) {
+    const size_t few = kv4_attention_workspace_bytes(q_rows, head_dim, sms);
+    const size_t many = kv4_attention_counter_bytes(sms) + (sms * sizeof(Cut) + 255) / 256 * 256 +
+                        static_cast<size_t>(sms) * 2 * kRows * (head_dim + 2) * 4;
+    return std::max(few, many);
+}
+
+cudaError_t launch_kv4_tree(const Kv4Attn& a, void* workspace, int sms, cudaStream_t stream) {
+    // fp32 queries, and few rows, run on the kernel of 8 or 16 columns
+    if (a.type != ALJ_KV_BF16 || a.q_len * a.group <= 8) return launch_kv4_attention(a, workspace, sms, stream);
+    Kv4Attn p = a;
+    p.row_tiles = (p.q_len * p.group + kRows - 1) / kRows;
+    p.page_shift = (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctz(p.page_size) : -1;
+    uint8_t* at = static_cast<uint8_t*>(workspace) + kv4_attention_counter_bytes(sms);
+    Cut* cuts = reinterpret_cast<Cut*>(at);
+    p.part = reinterpret_cast<float*>(at + (sms * sizeof(Cut) + 255) / 256 * 256);
+    if (p.head_dim == 256) return launch_tree<8>(p, cuts, sms, stream);
+    if (p.head_dim == 128) return launch_tree<4>(p, cuts, sms, stream);
+    return p.head_dim == 64 ? launch_tree<2>(p, cuts, sms, stream) : cudaErrorNotSupported;
+}
+
+}  // namespace alj
