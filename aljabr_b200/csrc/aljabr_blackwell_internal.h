@@ -281,7 +281,7 @@ size_t kv4_attention_counter_bytes(int sms);   // of the arrival counters at its
 cudaError_t launch_kv4_attention(const Kv4Attn& a, void* workspace, int sms, cudaStream_t stream);
 // The same for trees (kv4_tree.cu).  The workspace's counters are where launch_kv4_attention has them.
 size_t kv4_tree_workspace_bytes(int q_rows, int head_dim, int sms);
-cudaError_t launch_kv4_tree(const Kv4Attn& a, void* workspace, int sms, cudaStream_t stream);
+cudaError_t launch_kv4_tree(const Kv4Attn& a, void* workspace, int sms, unsigned int* fault_word, cudaStream_t stream);
 
 // Acceptance of a drafted tree (kv4_accept.cu): along each sequence's tree from node 0 to the first child whose drafted
 // token is the one picked after its parent, and so on; the path's rows move to the tree's first positions in every cache.

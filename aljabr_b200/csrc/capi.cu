@@ -117,6 +117,7 @@ using PackKey = std::tuple<uintptr_t, int, int, int>;   // device weights, type,
 struct DeviceState {
     int device = 0;
     int sms = 0;
+    unsigned int* fault_word = nullptr;     // g_fault_word of this device
     cudaStream_t stream = nullptr;
     std::mutex mu;                          // serialises the staging buffers of tb calls
     std::map<uintptr_t, Registered> reg;    // host base -> HBM copy
@@ -164,6 +165,10 @@ DeviceState* state(int* err) {
         cudaDeviceGetAttribute(&s->sms, cudaDevAttrMultiProcessorCount, d);
         if (cudaStreamCreateWithFlags(&s->stream, cudaStreamNonBlocking) != cudaSuccess) {
             *err = fail(ALJ_ERR_CUDA, "stream creation failed on device %d", d);
+            return nullptr;
+        }
+        if (cudaGetSymbolAddress(reinterpret_cast<void**>(&s->fault_word), g_fault_word) != cudaSuccess) {
+            *err = fail(ALJ_ERR_CUDA, "the library's kernels could not be loaded on device %d", d);
             return nullptr;
         }
         g_dev[d] = std::move(s);
@@ -721,7 +726,7 @@ int kv4_attend(const char* what, void* out, const void* q, int q_dtype, long lon
     if (!parents) return launch_status(launch_kv4_attention(a, workspace, st->sms, pick_stream(st, stream)), what);
     // two launches share the workspace: another thread's call on this stream must not come between them
     std::lock_guard<std::mutex> g(st->tree_mu);
-    return launch_status(launch_kv4_tree(a, workspace, st->sms, pick_stream(st, stream)), what);
+    return launch_status(launch_kv4_tree(a, workspace, st->sms, st->fault_word, pick_stream(st, stream)), what);
 }
 
 // The binding's elementwise glue (rmsnorm, silu_ffn): operands that are

@@ -15,7 +15,13 @@ namespace alj {
 // ---------------------------------------------------------------- fault word
 // Set (never cleared on the device) when a bounded wait gives up; read and
 // cleared by the host through aljabr_blackwell_device_status().
+// A file compiled without relocatable device code has a word of its own, which
+// its kernels hand on.
+#ifdef ALJ_OWN_FAULT_WORD
+static __device__ unsigned int g_fault_word;
+#else
 extern __device__ unsigned int g_fault_word;
+#endif
 
 // Upper bound for any spin on an mbarrier: ~2 s at 2 GHz.  A wait that runs
 // out records ALJ_FAULT_TIMEOUT and the CTA stops early instead of hanging.

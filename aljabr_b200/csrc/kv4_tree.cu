@@ -28,14 +28,14 @@
 //
 // Roles (one CTA an SM, persistent over the line of chunks as in
 // kv4_attention.cu): a producer warp (bulk copies of a tile's codes and scales
-// into a ring, 8 positions of V apart by 16 bytes so that transposing reads hit
-// distinct banks), 4 warps that decode K, 4 that decode V, one that issues the
-// MMAs, and a warpgroup of softmax for each of two streams: the even and the odd
+// into a ring), two that find the exponents e, 4 that decode K, 4 that decode V,
+// one that issues the MMAs, and a warpgroup of softmax for each of two streams: the even and the odd
 // tiles of an item have their own S, running maximum and O, so that one stream's
 // softmax runs beside the other's products.  (D 256: tiles of 64, one stream, as
 // two O do not fit tensor memory beside S.)  The streams are joined when the item
 // ends; items cut over CTAs are joined by a second small kernel, which all SMs
 // share (one CTA joining 128 rows of 10 parts would read 0.6 MB by itself).
+#define ALJ_OWN_FAULT_WORD     // compiled by itself, for setmaxnreg (build.py)
 #include "kv4.cuh"
 #include "tc_gemm.cuh"
 
@@ -46,7 +46,7 @@ namespace {
 
 constexpr int kRows = 128;
 constexpr int kItemCost = 2;          // tiles that an item's start and end are worth
-constexpr int kMeta = 4;              // tiles whose exponents are kept
+constexpr int kMeta = 8;              // tiles whose exponents are kept: V of tile t + 5 waits for the products of t + 3
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -3.4e38f;     // running maximum of a row that has seen nothing
 // P <= 2^(kLazy + kSlack + kBias) = 2^15
@@ -61,12 +61,13 @@ struct Shape {
     static constexpr int V_STAGES = NG == 8 ? 1 : 2;
     static constexpr int RAW = NG == 2 ? 4 : NG == 4 ? 3 : 2;
     static constexpr int SOFT = 4 * STREAMS;                 // softmax warps
-    static constexpr int WARPS = SOFT + 10;
+    static constexpr int WARPS = SOFT + 12;
+    // Registers a thread, of the launch's (96 for 5 warpgroups, 128 for 4) that they trade: 5 x 96 = 2 x 128 + 64 + 96 + 64,
+    // 4 x 128 = 192 + 72 + 128 + 120
+    static constexpr int R_SOFT = STREAMS == 2 ? 128 : 192, R_K = STREAMS == 2 ? 64 : 72, R_REST = STREAMS == 2 ? 64 : 120;
     static constexpr int THREADS = 32 * WARPS;
-    // a raw tile: K codes, K scales, V codes and V scales in padded blocks of 8 positions
-    static constexpr int VB = 4 * D + 16, SB = 16 * NG + 16;
-    static constexpr int K_SC = KT * D / 2, V_CODES = K_SC + KT * 2 * NG, V_SC = V_CODES + KT / 8 * VB;
-    static constexpr int RAW_BYTES = (V_SC + KT / 8 * SB + 127) / 128 * 128;
+    // a raw tile: K codes, V codes, K scales, V scales, each by position
+    static constexpr int V_CODES = KT * D / 2, K_SC = 2 * V_CODES, V_SC = K_SC + KT * 2 * NG, RAW_BYTES = V_SC + KT * 2 * NG;
     static constexpr int BLOCK_BYTES = 16 * (D + D / 8);     // copied for 16 positions
     static constexpr int KHAT = KT * D * 2, VHAT = KT * D * 2, Q = kRows * D * 2;
     static constexpr int AT_K = Q, AT_V = AT_K + 2 * KHAT, AT_RAW = AT_V + V_STAGES * VHAT, AT_SMALL = AT_RAW + RAW * RAW_BYTES;
@@ -75,12 +76,13 @@ struct Shape {
 
 struct Small {                        // behind the tiles in shared memory
     uint64_t raw_full[4], raw_empty[4], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], q_full, done;
-    uint64_t ek_full[kMeta];          // K exponents: the K warps do not wait for V
+    uint64_t meta_full[kMeta];
     int abort, tmem;
     uint32_t valid[4][4];             // by raw slot: bits of the positions that some row may see
     int ek[kMeta][4];                 // by tile: exponents of K (32 positions) and V (64)
     int ev[kMeta][2];
     int nan_any[kMeta][2];            // V groups that are NaN: bits by position
+    int care[kMeta];                  // V has NaN or positions that nobody sees
     uint8_t nan[kMeta][128];
     int sum[32];                      // prefix sums, and where this CTA starts
     int start[4];
@@ -117,6 +119,11 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[NW]) {
     else
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a));
 }
+__device__ __forceinline__ uint32_t lds_word(uint32_t a) {
+    uint32_t w;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(a));
+    return w;
+}
 __device__ __forceinline__ void fence_proxy_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // 32 lanes x 32 columns of 32 bit from tensor memory; the wait is tied to the outputs.
@@ -144,6 +151,24 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
+}
 // d (+)= a b, both operands in shared memory, or a in tensor memory; fp16, K = 16.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
@@ -167,10 +192,20 @@ __device__ __forceinline__ void decode8(uint32_t w, __half2 d2, uint32_t (&out)[
     out[2] = h2_bits(__hmul2(__hsub2(bits_h2(lop3_and_or(w8, 0x000F000Fu, 0x64006400u)), off), d2));
     out[3] = h2_bits(__hmul2(__hfma2(bits_h2(lop3_and_or(w8, 0x00F000F0u, 0x64006400u)), div16, off16), d2));
 }
-// Larger of m and the two fp16 magnitudes of a word of scales, NaN and infinity left out.
-__device__ __forceinline__ uint32_t top_of(uint32_t m, uint32_t w) {
-    const uint32_t a = w & 0x7FFFu, b = (w >> 16) & 0x7FFFu;
-    return max(m, max(a < 0x7C00u ? a : 0u, b < 0x7C00u ? b : 0u));
+// The largest fp16 magnitude of the words' halves; `finite` leaves NaN and infinity out.
+template <int N>
+__device__ __forceinline__ uint32_t top_of(const uint32_t (&w)[N], bool finite) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        uint32_t x = w[i] & 0x7FFF7FFFu;
+        if (finite) {
+            if ((x & 0xFFFFu) >= 0x7C00u) x &= 0xFFFF0000u;
+            if ((x >> 16) >= 0x7C00u) x &= 0xFFFFu;
+        }
+        m = __vmaxu2(m, x);
+    }
+    return max(m & 0xFFFFu, m >> 16);
 }
 // Exponent e with 2^e <= v < 2^(e + 1) of an fp16 magnitude's bits (subnormals: that of the smallest normal).
 __device__ __forceinline__ int exponent_of(uint32_t bits) { return max(1, static_cast<int>(bits >> 10)) - 15; }
@@ -255,13 +290,13 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Small& s = *reinterpret_cast<Small*>(smem + F::AT_SMALL);
     volatile int* const gave_up = &s.abort;
+    auto token_of = [&](int row) { return static_cast<int>((static_cast<unsigned int>(row) * p.group_magic) >> 21); };   // row / group
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < 4; ++i) {
             mbar_init(s.raw_full + i, 1);
-            mbar_init(s.raw_empty + i, 8);
-            mbar_init(s.ek_full + i, 4);
+            mbar_init(s.raw_empty + i, 10);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(s.k_full + i, 4);
@@ -272,12 +307,13 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             mbar_init(s.p_full + i, 4);
             mbar_init(s.pv_done + i, 1);
         }
+        for (int i = 0; i < kMeta; ++i) mbar_init(s.meta_full + i, 2);
         mbar_init(&s.q_full, F::SOFT);
         mbar_init(&s.done, 1);
         s.abort = 0;
         fence_mbar_init();
     }
-    if (warp == F::WARPS - 1) {
+    if (warp == F::SOFT + 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -369,6 +405,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
 
     if (warp < F::SOFT) {
         // ------------------------------------------------------ softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::R_SOFT));
         const int stream = warp >> 2, row = (warp & 3) * 32 + lane, thread = threadIdx.x;
         const uint32_t tq = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const float inv_cap = p.soft_cap > 0.0f ? 1.0f / p.soft_cap : 0.0f;
@@ -390,7 +427,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             for (int i = thread; i < p.q_len; i += 32 * F::SOFT)
                 s.par[i] = static_cast<short>(tree_parent(p.parents + static_cast<long long>(pc.b) * p.parents_stride, i));
             sync();
-            const int node = (pc.row0 + row) / p.group;
+            const int node = token_of(pc.row0 + row);
             int depth = 0;
             if (pc.count > 0 && row < pc.rows) {
                 uint32_t see[kKv4TreeWords];
@@ -422,7 +459,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                         const int r = (r0 + k * F::SOFT + warp) * kPer + lane / kChunks, i = pc.row0 + r;
                         x[k] = make_uint4(0u, 0u, 0u, 0u);
                         if (r < pc.rows) {
-                            const int t = i / p.group, hd = i - t * p.group;
+                            const int t = token_of(i), hd = i - t * p.group;
                             const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) +
                                 (static_cast<long long>(pc.b) * p.q_len + t) * p.q_stride +
                                 static_cast<long long>(pc.kvh * p.group + hd) * D + 8 * j;
@@ -489,93 +526,118 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 const int meta = tile & (kMeta - 1), pos = (pc.tile0 + i) * KT;
                 const uint32_t ts = tq + buf * KT, to = tq + F::O_COL + (F::STREAMS == 2 ? stream * D : 0);
                 ok = ok && tcg::warp_wait(s.s_full + buf, use & 1, gave_up);
-                ok = ok && tcg::warp_wait(s.ek_full + meta, (tile / kMeta) & 1, gave_up);
-                ok = ok && tcg::warp_wait(s.v_full + tile % F::V_STAGES, (tile / F::V_STAGES) & 1, gave_up);
+                ok = ok && tcg::warp_wait(s.meta_full + meta, (tile / kMeta) & 1, gave_up);
                 if (ok && warp_lives) {
                     tcg::tc_fence_after();
                     const bool edge = pos < all_lo || pos + KT > pc.base;
-                    float mx = -INFINITY;
+                    // O summed up so far times g
+                    auto rescale = [&](float g) {
+                        if (i < F::STREAMS) return;
+                        const int last = i - F::STREAMS, pb = last & 1;
+                        ok = ok && tcg::warp_wait(s.pv_done + pb, ((pb ? uses1 : uses0) + (last >> 1)) & 1, gave_up);
+                        tcg::tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < KT / 32; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32(ts + 32 * c, v);
-                        const float fc = fac * pow2i(s.ek[meta][c]);
-                        if (p.soft_cap > 0.0f) {
-#pragma unroll 4
-                            for (int k = 0; k < 32; ++k)
-                                v[k] = __float_as_uint(tanhf(__uint_as_float(v[k]) * fc * inv_cap) * (p.soft_cap * kLog2e));
-                            tcg::tmem_st32(ts + 32 * c, v);
-                            tcg::tmem_wait_st();
-                        }
-                        float m = -INFINITY;
-                        if (edge) {
-                            const uint32_t bits = visible(pos + 32 * c);
+                        for (int c = 0; c < NG; ++c) {
+                            uint32_t v[32];
+                            tmem_ld32(to + 32 * c, v);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) m = fmaxf(m, (bits >> k) & 1u ? __uint_as_float(v[k]) : -INFINITY);
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) m = fmaxf(m, __uint_as_float(v[k]));
+                            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * g);
+                            tcg::tmem_st32(to + 32 * c, v);
                         }
-                        mx = fmaxf(mx, m == -INFINITY || p.soft_cap > 0.0f ? m : m * fc);
-                    }
+                    };
                     const int e_new = max(s.ev[meta][0], KT == 128 ? s.ev[meta][1] : -100);
-                    const bool higher = e_new > E + kSlack, rise = mx > M + kLazy;
-                    if (__any_sync(0xffffffffu, rise) || higher) {
-                        const float now = rise ? mx : M, f = ex2(M - now);
-                        const int e = higher ? e_new : E;
-                        l *= f;
-                        if (i >= F::STREAMS) {                        // what has been summed up, to the new reference
-                            const int last = i - F::STREAMS, pb = last & 1;
-                            ok = ok && tcg::warp_wait(s.pv_done + pb, ((pb ? uses1 : uses0) + (last >> 1)) & 1, gave_up);
-                            tcg::tc_fence_after();
-                            const float g = f * pow2i(E - e);
-#pragma unroll 1
-                            for (int c = 0; c < NG; ++c) {
-                                uint32_t v[32];
-                                tmem_ld32(to + 32 * c, v);
-#pragma unroll
-                                for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * g);
-                                tcg::tmem_st32(to + 32 * c, v);
-                            }
-                        }
+                    if (e_new > E + kSlack) {                         // the same for the whole warp
+                        rescale(pow2i(max(E - e_new, -126)));
+                        E = e_new;
+                    }
+                    // A score of chunk c passes M by more than kLazy: M becomes the next integer above it, so that what is
+                    // there already, the P of the chunks before c too, is scaled by a power of two.
+                    auto raise = [&](float mx, int c) {
+                        const float now = mx > M + kLazy ? ceilf(mx) : M, f = ex2(M - now);
                         M = now;
-                        E = e;
-                    }
+                        l *= f;
+                        rescale(f);
+                        const __half2 f2 = __float2half2_rn(f);
 #pragma unroll 1
-                    for (int c = 0; c < KT / 32; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32(ts + 32 * c, v);
-                        const float fc = p.soft_cap > 0.0f ? 1.0f : fac * pow2i(s.ek[meta][c]);
-                        const int sh = kBias + s.ev[meta][c >> 1] - E;
-                        const float at = static_cast<float>(sh) - M;
-                        float part[4] = {};
-                        uint32_t out[16];
-                        if (edge) {
-                            const uint32_t bits = visible(pos + 32 * c);
+                        for (int b = 0; b < 2 * c; ++b) {
+                            uint32_t v[8];
+                            tmem_ld8(ts + 8 * b, v);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                v[k] = (bits >> k) & 1u ? v[k] : 0xFF800000u;
+                            for (int k = 0; k < 8; ++k) v[k] = h2_bits(__hmul2(bits_h2(v[k]), f2));
+                            tmem_st8(ts + 8 * b, v);
+                        }
+                    };
+                    if (!edge && p.soft_cap == 0.0f) {
+#pragma unroll 1
+                        for (int c = 0; c < KT / 32; ++c) {
+                            uint32_t v[32];
+                            tmem_ld32(ts + 32 * c, v);
+                            const float fc = fac * pow2i(s.ek[meta][c]);
+                            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) {            // a factor of zero times -infinity is no score
-                                const float y = ex2(fmaf(__uint_as_float(v[k]), fc, at));
-                                v[k] = (bits >> k) & 1u ? __float_as_uint(y) : 0u;
+                            for (int k = 0; k < 32; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
+                            const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), mx = top == -INFINITY ? top : top * fc;
+                            if (__any_sync(0xffffffffu, mx > M + kLazy)) raise(mx, c);
+                            const int sh = kBias + s.ev[meta][c >> 1] - E;
+                            const float at = static_cast<float>(sh) - M;
+                            const f2 fc2 = mk2(fc, fc), at2 = mk2(at, at);
+                            f2 sum0 = mk2(0.0f, 0.0f), sum1 = sum0;
+                            uint32_t out[16];
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                const f2 y = fma2(mk2u(v[2 * k], v[2 * k + 1]), fc2, at2);
+                                const float a = ex2(lo(y)), b = ex2(hi(y));
+                                if (k & 1) sum1 = add2(sum1, mk2(a, b));
+                                else sum0 = add2(sum0, mk2(a, b));
+                                out[k] = h2_bits(__floats2half2_rn(a, b));
                             }
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(ex2(fmaf(__uint_as_float(v[k]), fc, at)));
+                            const f2 sum = add2(sum0, sum1);
+                            l = fmaf(lo(sum) + hi(sum), pow2i(-sh), l);
+                            tmem_st16(ts + 16 * c, out);              // columns that this lane has read
                         }
+                    } else {
+#pragma unroll 1
+                        for (int c = 0; c < KT / 32; ++c) {
+                            const uint32_t bits = edge ? visible(pos + 32 * c) : 0xFFFFFFFFu;
+                            const float fc = fac * pow2i(s.ek[meta][c]);
+                            float mx = -INFINITY;
+#pragma unroll 1
+                            for (int b = 0; b < 4; ++b) {             // S becomes the scaled, capped and masked score
+                                uint32_t v[8];
+                                tmem_ld8(ts + 32 * c + 8 * b, v);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const float a = __uint_as_float(v[2 * k]), b = __uint_as_float(v[2 * k + 1]);
-                            part[(2 * k) & 3] += a;
-                            part[(2 * k + 1) & 3] += b;
-                            out[k] = h2_bits(__floats2half2_rn(a, b));
+                                for (int k = 0; k < 8; ++k) {
+                                    float y = __uint_as_float(v[k]) * fc;
+                                    if (p.soft_cap > 0.0f) y = tanhf(y * inv_cap) * (p.soft_cap * kLog2e);
+                                    y = (bits >> (8 * b + k)) & 1u ? y : -INFINITY;
+                                    mx = fmaxf(mx, y);
+                                    v[k] = __float_as_uint(y);
+                                }
+                                tmem_st8(ts + 32 * c + 8 * b, v);
+                            }
+                            tcg::tmem_wait_st();
+                            if (__any_sync(0xffffffffu, mx > M + kLazy)) raise(mx, c);
+                            const int sh = kBias + s.ev[meta][c >> 1] - E;
+                            const float at = static_cast<float>(sh) - M;
+                            float sum = 0.0f;
+#pragma unroll 1
+                            for (int b = 0; b < 4; ++b) {
+                                uint32_t v[8], out[4];
+                                tmem_ld8(ts + 32 * c + 8 * b, v);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    const float a = ex2(__uint_as_float(v[2 * k]) + at), d = ex2(__uint_as_float(v[2 * k + 1]) + at);
+                                    sum += a + d;
+                                    out[k] = h2_bits(__floats2half2_rn(a, d));
+                                }
+                                tmem_st4(ts + 16 * c + 4 * b, out);
+                            }
+                            l = fmaf(sum, pow2i(-sh), l);
                         }
-                        l = fmaf((part[0] + part[1]) + (part[2] + part[3]), pow2i(-sh), l);
-                        tmem_st16(ts + 16 * c, out);                  // columns that this lane has read
                     }
-                    if (s.nan_any[meta][0] || (KT == 128 && s.nan_any[meta][1])) {
-                        for (int k = 0; k < KT; ++k) {
+                    for (int h = 0; h < KT / 64; ++h) {
+                        if (!s.nan_any[meta][h]) continue;
+                        for (int k = 64 * h; k < 64 * h + 64; ++k) {
                             const int g = s.nan[meta][k];
                             if (g && (edge ? (visible(pos + (k & ~31)) >> (k & 31)) & 1u : alive)) nan_groups |= g;
                         }
@@ -640,7 +702,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                     const bool nan = (gone >> (d >> 5)) & 1;
                     if (row < pc.rows) {
                         if (whole) {
-                            const int t = i / p.group, hd = i - t * p.group;
+                            const int t = token_of(i), hd = i - t * p.group;
                             __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) +
                                 (((static_cast<long long>(pc.b) * p.q_len + t) * p.kv_heads + pc.kvh) * p.group + hd) * D + d;
 #pragma unroll
@@ -677,6 +739,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         }
     } else if (warp < F::SOFT + 4) {
         // ------------------------------------------------------ K to fp16
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::R_K));
         constexpr int GW = NG == 8 ? 4 : NG;                      // groups of a warp
         const int kw = warp - F::SOFT, span = KT == 128 ? kw : kw & 1, half = KT == 128 ? 0 : kw >> 1;
         const int c = lane & 3, pos_in = (lane >> 3) + (lane & 4);
@@ -685,22 +748,14 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             for (int i = 0; i < pc.count; ++i, ++tile) {
                 const int slot = tile % F::RAW, ks = tile & 1;
                 ok = ok && tcg::warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
+                ok = ok && tcg::warp_wait(s.meta_full + (tile & (kMeta - 1)), (tile / kMeta) & 1, gave_up);
                 if (tile >= 2) ok = ok && tcg::warp_wait(s.k_empty + ks, ((tile >> 1) - 1) & 1, gave_up);
                 if (!ok) break;
                 const uint32_t raw = at_raw + slot * F::RAW_BYTES;
                 const uint32_t valid = s.valid[slot][span];
-                uint32_t top = 0u;
-                if ((valid >> lane) & 1u) {                       // a lane a position
-                    uint32_t w[NG / 2];
-                    lds_words<NG / 2>(raw + F::K_SC + (32 * span + lane) * (2 * NG), w);
-#pragma unroll
-                    for (int k = 0; k < NG / 2; ++k) top = top_of(top, w[k]);
-                }
-                const int e = exponent_of(__reduce_max_sync(0xffffffffu, top));
-                const Unit unit(e);
-                if (lane == 0) s.ek[tile & (kMeta - 1)][span] = e;
+                const Unit unit(s.ek[tile & (kMeta - 1)][span]);
                 const uint32_t to = at_k + ks * F::KHAT;
-#pragma unroll
+#pragma unroll 2
                 for (int it = 0; it < 4; ++it) {
                     const int at = 8 * it + pos_in, r = 32 * span + at;
                     uint32_t w[GW], d[GW / 2];
@@ -719,8 +774,6 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 fence_proxy_shared();
                 __syncwarp();
                 if (lane == 0) {
-                    // the exponents of tile n - kMeta have been read: S of tile n - 2 was issued after its P
-                    mbar_arrive(s.ek_full + (tile & (kMeta - 1)));
                     mbar_arrive(s.k_full + ks);
                     mbar_arrive(s.raw_empty + slot);
                 }
@@ -728,82 +781,69 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             if (!ok) break;
         }
     } else if (warp < F::SOFT + 8) {
-        // ------------------------------------------------------ V to fp16, transposed
-        constexpr int WP = NG == 2 ? 1 : 2;                       // words of a thread
-        const int vw = warp - F::SOFT - 4, part = KT == 128 ? vw & 1 : 0;
-        const int wp = (KT == 128 ? vw >> 1 : vw) * 4 + (lane >> 3), j = lane & 7;
+        // ------------------------------------------------------ V to fp16, transposed (at the launch's registers)
+        // A thread has 8 positions, block j of 64, and a word (8 codes: 4 dims of groups g and g + 1) a pass.  Lanes read
+        // different words, those that would meet on a bank the other position of a pair first; eight lanes that store
+        // together have eight different j, so that their 16-byte pieces lie in different banks under the swizzle.
+        constexpr int kPasses = NG == 2 ? 1 : 2;
+        const int vw = warp - F::SOFT - 4;
+        const int word = NG == 8   ? (lane & 3) | (lane & 24) >> 1 | (lane & 4) << 2
+                         : NG == 4 ? lane & 15
+                                   : lane & 7;
+        const int part = KT == 128 ? lane >> 4 : 0, flip = NG == 8 ? 0 : lane >> 4;
+        const int hw0 = 2 * word;
         int tile = 0;
         while (next_piece<KT>(line, p, items, pc)) {
             for (int i = 0; i < pc.count; ++i, ++tile) {
                 const int slot = tile % F::RAW, vs = tile % F::V_STAGES, meta = tile & (kMeta - 1);
                 ok = ok && tcg::warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
+                ok = ok && tcg::warp_wait(s.meta_full + meta, (tile / kMeta) & 1, gave_up);
                 if (tile >= F::V_STAGES) ok = ok && tcg::warp_wait(s.v_empty + vs, (tile / F::V_STAGES - 1) & 1, gave_up);
                 if (!ok) break;
                 const uint32_t raw = at_raw + slot * F::RAW_BYTES;
-                uint32_t top = 0u;
-                bool nan = false;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {                     // two positions a lane
-                    const int r = 64 * part + 32 * k + lane;
-                    if ((s.valid[slot][2 * part + k] >> lane) & 1u) {
-                        uint32_t w[NG / 2];
-                        lds_words<NG / 2>(raw + F::V_SC + (r >> 3) * F::SB + (r & 7) * (2 * NG), w);
-                        int bad = 0;
-#pragma unroll
-                        for (int n = 0; n < NG / 2; ++n) {
-                            top = top_of(top, w[n]);
-                            bad |= ((w[n] & 0x7FFFu) >= 0x7C00u ? 1 : 0) << (2 * n) | (((w[n] >> 16) & 0x7FFFu) >= 0x7C00u ? 1 : 0) << (2 * n + 1);
-                        }
-                        nan |= bad != 0;
-                        s.nan[meta][r] = static_cast<uint8_t>(bad);   // the two warps of these positions write the same
-                    } else {
-                        s.nan[meta][r] = 0;
-                    }
-                }
-                const int e = exponent_of(__reduce_max_sync(0xffffffffu, top));
-                const bool any_nan = __any_sync(0xffffffffu, nan);
-                const Unit unit(e);
-                if (lane == 0) {
-                    s.ev[meta][part] = e;
-                    s.nan_any[meta][part] = any_nan;
-                }
-                const uint32_t live = (s.valid[slot][2 * part + (j >> 2)] >> (8 * (j & 3))) & 255u;   // of the thread's 8 positions
-                const uint32_t blk = raw + F::V_CODES + (8 * part + j) * F::VB + wp * (4 * WP);
-                const uint32_t sc = raw + F::V_SC + (8 * part + j) * F::SB + (NG == 8 ? (wp & 1) * 8 : 0);
+                const Unit unit(s.ev[meta][part]);
+                const bool care = s.care[meta] != 0;
                 const uint32_t to = at_v + vs * F::VHAT + part * (D * 128);
-                uint32_t code[8][WP], d[8][WP];
+#pragma unroll 1
+                for (int n = 0; n < kPasses; ++n) {
+                    const int j = (lane + (NG == 2 ? vw + ((lane & 8) >> 1) : 2 * vw + n)) & 7, pos = 64 * part + 8 * j;
+                    const uint32_t blk = raw + F::V_CODES + pos * (D / 2) + 4 * word;
+                    const uint32_t sc = raw + F::V_SC + pos * (2 * NG) + 4 * (word % (NG / 2));
+                    uint32_t code[8], d[8];                       // register k: position k ^ flip
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    lds_words<WP>(blk + k * (D / 2), code[k]);
-                    lds_words<WP>(sc + k * (2 * NG), d[k]);
-#pragma unroll
-                    for (int n = 0; n < WP; ++n) {
-                        if (any_nan) {                            // NaN as zero: its rows are marked
-                            if ((d[k][n] & 0x7FFFu) >= 0x7C00u) d[k][n] &= 0xFFFF0000u;
-                            if (((d[k][n] >> 16) & 0x7FFFu) >= 0x7C00u) d[k][n] &= 0x0000FFFFu;
-                        }
-                        d[k][n] = (live >> k) & 1u ? unit.of(d[k][n]) : 0u;
+                    for (int k = 0; k < 8; ++k) {
+                        code[k] = lds_word(blk + (k & 6) * (D / 2) + (k & 1 ? (flip ^ 1) : flip) * (D / 2));
+                        d[k] = lds_word(sc + (k & 6) * (2 * NG) + (k & 1 ? (flip ^ 1) : flip) * (2 * NG));
                     }
-                }
+                    if (care) {
+                        const uint32_t live = s.valid[slot][pos >> 5] >> (pos & 31);
 #pragma unroll
-                for (int n = 0; n < WP; ++n)
+                        for (int k = 0; k < 8; ++k) {
+                            if ((d[k] & 0x7FFFu) >= 0x7C00u) d[k] &= 0xFFFF0000u;
+                            if (((d[k] >> 16) & 0x7FFFu) >= 0x7C00u) d[k] &= 0x0000FFFFu;
+                            if (((live >> (k ^ flip)) & 1u) == 0u) d[k] = 0u;
+                        }
+                    }
 #pragma unroll
+                    for (int k = 0; k < 8; ++k) d[k] = unit.of(d[k]);
+#pragma unroll 1
                     for (int x = 0; x < 2; ++x) {
-                        const uint32_t pick = x ? 0x7632 : 0x5410;
+                        const uint32_t pick = flip ? (x ? 0x3276u : 0x1054u) : x ? 0x7632u : 0x5410u;
+                        const int hw = hw0 + x, dim = 32 * (hw % NG) + 4 * (hw / NG);
+                        const uint32_t row = to + dim * 128;
                         uint32_t out[4][4];                       // [dim][pair of positions]
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             uint32_t v[4];
-                            decode8(__byte_perm(code[2 * k][n], code[2 * k + 1][n], pick),
-                                    bits_h2(__byte_perm(d[2 * k][n], d[2 * k + 1][n], pick)), v);
+                            decode8(__byte_perm(code[2 * k], code[2 * k + 1], pick), bits_h2(__byte_perm(d[2 * k], d[2 * k + 1], pick)), v);
 #pragma unroll
                             for (int m = 0; m < 4; ++m) out[m][k] = v[m];
                         }
-                        const int hw = 2 * (WP * wp + n) + x, dim = 32 * (hw % NG) + 4 * (hw / NG);
 #pragma unroll
                         for (int m = 0; m < 4; ++m)
-                            sts128(to + (dim + m) * 128 + ((j ^ ((dim + m) & 7)) << 4), make_uint4(out[m][0], out[m][1], out[m][2], out[m][3]));
+                            sts128(row + m * 128 + ((j ^ ((dim + m) & 7)) << 4), make_uint4(out[m][0], out[m][1], out[m][2], out[m][3]));
                     }
+                }
                 fence_proxy_shared();
                 __syncwarp();
                 if (lane == 0) {
@@ -813,7 +853,9 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             }
             if (!ok) break;
         }
-    } else if (warp == F::WARPS - 2) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::R_REST));
+    if (warp == F::SOFT + 8) {
         // ------------------------------------------------------ codes and scales from the cache
         int tile = 0, seq = -1;
         while (next_piece<KT>(line, p, items, pc)) {
@@ -821,7 +863,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             for (int i = 0; i < pc.count; ++i, ++tile) {
                 const int slot = tile % F::RAW, pos0 = (pc.tile0 + i) * KT;
                 const int blk = lane >> 2, k = lane & 3, pos = pos0 + 16 * blk;
-                // lane 4 n + k copies a part of the n-th 16 positions; their page on its way while the slot empties
+                // lane 4 n + k sees to section k of the n-th 16 positions; their page on its way while the slot empties
                 int page = -1, off = 0;
                 const bool there = 16 * blk < KT && pos < pc.len;
                 if (there) {
@@ -865,24 +907,71 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 __syncwarp();
                 if (lane == 0) mbar_arrive_expect_tx(s.raw_full + slot, blocks * F::BLOCK_BYTES);
                 __syncwarp();
-                if (has && k < 3) {
+                // the blocks that share a page follow one another there: one copy of each section for all of them
+                if (has && (blk == 0 || off == 0)) {
+                    const int run = min(min(KT / 16 - blk, (p.page_size - off) / 16), (pc.len - pos + 15) / 16);
                     uint8_t* dst = smem + F::AT_RAW + slot * F::RAW_BYTES;
                     const uint8_t* src = p.cache + (static_cast<long long>(page) * p.kv_heads + pc.kvh) * kv4_block_bytes(p.page_size, D);
-                    const long long ps = p.page_size;
-                    if (k == 0) {
-                        bulk_g2s(dst + blk * (8 * D), src + off * (D / 2LL), 8 * D, s.raw_full + slot);
-                        bulk_g2s(dst + F::K_SC + blk * (32 * NG), src + ps * D + off * (2LL * NG), 32 * NG, s.raw_full + slot);
-                    } else {
-                        const int b8 = 2 * blk + k - 1, o8 = off + 8 * (k - 1);
-                        bulk_g2s(dst + F::V_CODES + b8 * F::VB, src + (ps + o8) * (D / 2), 4 * D, s.raw_full + slot);
-                        bulk_g2s(dst + F::V_SC + b8 * F::SB, src + ps * D + (ps + o8) * (2 * NG), 16 * NG, s.raw_full + slot);
-                    }
+                    const int row = k < 2 ? D / 2 : 2 * NG;       // bytes of a position
+                    const int to = k == 0 ? 0 : k == 1 ? F::V_CODES : k == 2 ? F::K_SC : F::V_SC;
+                    const long long section = static_cast<long long>(p.page_size) * (k < 2 ? k * (D / 2) : D + (k - 2) * (2 * NG));
+                    bulk_g2s(dst + to + 16 * blk * row, src + section + static_cast<long long>(off) * row, 16 * run * row, s.raw_full + slot);
                 }
             }
             if (!ok) break;
         }
         if (!ok)                          // the copies under way end before the CTA does
             for (int t = max(0, tile - F::RAW); t < tile; ++t) mbar_wait(s.raw_full + t % F::RAW, (t / F::RAW) & 1);
+    } else if (warp >= F::SOFT + 10) {
+        // ------------------------------------------------------ exponents of a tile's scales: one warp K's, one V's
+        const bool is_v = warp == F::SOFT + 11;
+        int tile = 0;
+        while (next_piece<KT>(line, p, items, pc)) {
+            for (int i = 0; i < pc.count; ++i, ++tile) {
+                const int slot = tile % F::RAW, meta = tile & (kMeta - 1);
+                ok = ok && tcg::warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
+                if (!ok) break;
+                uint32_t all = 0xFFFFFFFFu, top64 = 0u;
+                bool any = false;
+#pragma unroll 1
+                for (int c = 0; c < KT / 32; ++c) {               // 32 positions, a lane each
+                    const uint32_t valid = s.valid[slot][c];
+                    uint32_t w[NG / 2];
+                    lds_words<NG / 2>(at_raw + slot * F::RAW_BYTES + (is_v ? F::V_SC : F::K_SC) + (32 * c + lane) * (2 * NG), w);
+                    const bool mine = (valid >> lane) & 1u;
+                    uint32_t top = __reduce_max_sync(0xffffffffu, mine ? top_of(w, false) : 0u);
+                    const bool nan = top >= 0x7C00u;
+                    if (nan) top = __reduce_max_sync(0xffffffffu, mine ? top_of(w, true) : 0u);
+                    all &= valid;
+                    if (!is_v) {
+                        if (lane == 0) s.ek[meta][c] = exponent_of(top);
+                        continue;
+                    }
+                    // V: 64 positions share one; NaN groups count as zero, and their rows are marked
+                    if ((c & 1) == 0) top64 = 0u, any = false;
+                    top64 = max(top64, top);
+                    any |= nan;
+                    int bad = 0;
+                    if (nan && mine) {
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) bad |= ((w[g / 2] >> (16 * (g & 1))) & 0x7FFFu) >= 0x7C00u ? 1 << g : 0;
+                    }
+                    s.nan[meta][32 * c + lane] = static_cast<uint8_t>(bad);
+                    if (nan) all = 0u;
+                    if ((c & 1) == 1 && lane == 0) {
+                        s.ev[meta][c >> 1] = exponent_of(top64);
+                        s.nan_any[meta][c >> 1] = any;
+                    }
+                }
+                if (is_v && lane == 0) s.care[meta] = all != 0xFFFFFFFFu;
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(s.meta_full + meta);
+                    mbar_arrive(s.raw_empty + slot);
+                }
+            }
+            if (!ok) break;
+        }
     } else {
         // ------------------------------------------------------ MMA issue
         if (lane == 0) {
@@ -930,9 +1019,10 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         }
         __syncwarp();
     }
+    }
     tcg::tc_fence_before();
     __syncthreads();
-    if (warp == F::WARPS - 1) {
+    if (warp == F::SOFT + 9) {
         tcg::tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
@@ -941,9 +1031,11 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
 // Items cut over CTAs: block (c, y) joins 16 rows of the item that CTA c began and others went on with, in CTA order.
 constexpr int kJoinRows = 16;
 template <int D>
-__global__ void __launch_bounds__(256) kv4_tree_join_kernel(const Kv4Attn p, const Cut* cuts) {
+__global__ void __launch_bounds__(256) kv4_tree_join_kernel(const Kv4Attn p, const Cut* cuts, unsigned int* fault_word) {
     pdl_launch_dependents();
     pdl_wait();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && *static_cast<volatile unsigned int*>(&g_fault_word) != 0u)
+        atomicOr(fault_word, atomicExch(&g_fault_word, 0u));   // what the attention recorded, to the library's word
     const Cut cut = cuts[blockIdx.x];
     if (cut.n <= 1) return;
     const int kvh = cut.h / p.row_tiles, row0 = (cut.h - kvh * p.row_tiles) * kRows;
@@ -981,7 +1073,7 @@ __global__ void __launch_bounds__(256) kv4_tree_join_kernel(const Kv4Attn p, con
 }
 
 template <int NG>
-cudaError_t launch_tree(const Kv4Attn& p, Cut* cuts, int sms, cudaStream_t stream) {
+cudaError_t launch_tree(const Kv4Attn& p, Cut* cuts, int sms, unsigned int* fault_word, cudaStream_t stream) {
     using F = Shape<NG>;
     static_assert(smem_bytes<NG>() <= 232448, "shared memory of a CTA");
     static bool configured[64] = {};
@@ -1007,7 +1099,7 @@ cudaError_t launch_tree(const Kv4Attn& p, Cut* cuts, int sms, cudaStream_t strea
     cfg.gridDim = dim3(sms, (std::min(kRows, p.q_len * p.group) + kJoinRows - 1) / kJoinRows);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, kv4_tree_join_kernel<F::D>, p, static_cast<const Cut*>(cuts));
+    return cudaLaunchKernelEx(&cfg, kv4_tree_join_kernel<F::D>, p, static_cast<const Cut*>(cuts), fault_word);
 }
 
 }  // namespace
@@ -1019,18 +1111,19 @@ size_t kv4_tree_workspace_bytes(int q_rows, int head_dim, int sms) {
     return std::max(few, many);
 }
 
-cudaError_t launch_kv4_tree(const Kv4Attn& a, void* workspace, int sms, cudaStream_t stream) {
+cudaError_t launch_kv4_tree(const Kv4Attn& a, void* workspace, int sms, unsigned int* fault_word, cudaStream_t stream) {
     // fp32 queries, and few rows, run on the kernel of 8 or 16 columns
     if (a.type != ALJ_KV_BF16 || a.q_len * a.group <= 8) return launch_kv4_attention(a, workspace, sms, stream);
     Kv4Attn p = a;
     p.row_tiles = (p.q_len * p.group + kRows - 1) / kRows;
+    p.group_magic = ((1u << 21) + p.group - 1) / p.group;   // row / group for row < 2048, exact as row * group < 2^21
     p.page_shift = (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctz(p.page_size) : -1;
     uint8_t* at = static_cast<uint8_t*>(workspace) + kv4_attention_counter_bytes(sms);
     Cut* cuts = reinterpret_cast<Cut*>(at);
     p.part = reinterpret_cast<float*>(at + (sms * sizeof(Cut) + 255) / 256 * 256);
-    if (p.head_dim == 256) return launch_tree<8>(p, cuts, sms, stream);
-    if (p.head_dim == 128) return launch_tree<4>(p, cuts, sms, stream);
-    return p.head_dim == 64 ? launch_tree<2>(p, cuts, sms, stream) : cudaErrorNotSupported;
+    if (p.head_dim == 256) return launch_tree<8>(p, cuts, sms, fault_word, stream);
+    if (p.head_dim == 128) return launch_tree<4>(p, cuts, sms, fault_word, stream);
+    return p.head_dim == 64 ? launch_tree<2>(p, cuts, sms, fault_word, stream) : cudaErrorNotSupported;
 }
 
 }  // namespace alj
