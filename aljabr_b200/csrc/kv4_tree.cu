@@ -49,9 +49,10 @@ constexpr int kItemCost = 2;          // tiles that an item's start and end are 
 constexpr int kMeta = 8;              // tiles whose exponents are kept: V of tile t + 5 waits for the products of t + 3
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -3.4e38f;     // running maximum of a row that has seen nothing
-// P <= 2^(kLazy + kSlack + kBias) = 2^15
-constexpr float kLazy = 5.0f;
+// P <= 2^(kLazy + kSlack + kBias) = 2^15, or its sum over 32 positions <= kMostSum
+constexpr float kLazy = 5.0f, kMostSum = 60000.0f;
 constexpr int kSlack = 2, kBias = 8;
+constexpr float kMostM = 1048576.0f;  // where M's last place is 2^-3: S - M from the unrounded S is off by less
 
 template <int NG>
 struct Shape {
@@ -79,10 +80,10 @@ struct Small {                        // behind the tiles in shared memory
     uint64_t meta_full[kMeta];
     int abort, tmem;
     uint32_t valid[4][4];             // by raw slot: bits of the positions that some row may see
-    int ek[kMeta][4];                 // by tile: exponents of K (32 positions) and V (64)
-    int ev[kMeta][2];
-    int nan_any[kMeta][2];            // V groups that are NaN: bits by position
-    int care[kMeta];                  // V has NaN or positions that nobody sees
+    float k_unit[kMeta][4];           // by tile and 32 positions: 2^e of K, e of V, the largest of those,
+    int ev[kMeta][4];
+    int e_top[kMeta];
+    int nan_any[kMeta];               // and V groups that are NaN: bits by position
     uint8_t nan[kMeta][128];
     int sum[32];                      // prefix sums, and where this CTA starts
     int start[4];
@@ -119,10 +120,42 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[NW]) {
     else
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a));
 }
+template <int NW>
+__device__ __forceinline__ void sts_words(uint32_t a, const uint32_t (&w)[NW]) {
+    if constexpr (NW == 4)
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    else if constexpr (NW == 2)
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a), "r"(w[0]), "r"(w[1]) : "memory");
+    else
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(w[0]) : "memory");
+}
 __device__ __forceinline__ uint32_t lds_word(uint32_t a) {
     uint32_t w;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(a));
     return w;
+}
+// Waits with a limit, that also end once another role has given up.  The roles' loops have to share the instruction
+// cache, so these are kept short: a count of tries, each of which the hardware suspends for a while, in place of a clock.
+constexpr int kTries = 1 << 22;
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p, q;\n .reg .b32 n, a;\n mov.b32 n, 0;\n"
+        "WAIT:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+        " ld.volatile.shared.b32 a, [%3];\n setp.ne.b32 q, a, 0;\n @q bra DONE;\n"
+        " add.s32 n, n, 1;\n setp.lt.s32 q, n, %4;\n @q bra WAIT;\n"
+        "DONE:\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(const_cast<int*>(gave_up))), "n"(kTries)
+        : "memory");
+    if (ok == 0u && *gave_up == 0) {
+        record_fault(ALJ_FAULT_TIMEOUT);
+        *gave_up = 1;
+    }
+    return ok != 0u;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+    return __all_sync(0xffffffffu, wait_bar(bar, parity, gave_up));
 }
 __device__ __forceinline__ void fence_proxy_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -430,40 +463,38 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             const int node = token_of(pc.row0 + row);
             int depth = 0;
             if (pc.count > 0 && row < pc.rows) {
-                uint32_t see[kKv4TreeWords];
-#pragma unroll
-                for (int i = 0; i < kKv4TreeWords; ++i) see[i] = 0u;
-                int t = node;
-                for (; t >= 0; t = s.par[t], ++depth)
-                    if (p.window == 0 || depth < p.window) {
-#pragma unroll
-                        for (int i = 0; i < kKv4TreeWords; ++i) see[i] |= (t >> 5) == i ? 1u << (t & 31) : 0u;
-                    }
-                if (t != -1) depth = 0;
                 if (stream == 0) {
-#pragma unroll
-                    for (int i = 0; i < kKv4TreeWords; ++i) s.see[i][row] = depth > 0 ? see[i] : 0u;
+#pragma unroll 1
+                    for (int i = 0; i < kKv4TreeWords; ++i) s.see[i][row] = 0u;
                 }
+                int t = node;
+#pragma unroll 1
+                for (; t >= 0; t = s.par[t], ++depth)
+                    if (stream == 0 && (p.window == 0 || depth < p.window)) s.see[t >> 5][row] |= 1u << (t & 31);
+                if (t != -1) depth = 0;                               // its bits are not looked at
             }
             const bool alive = depth > 0;
             const int row_lo = window_start(p, pc.base + depth);          // first position the row sees
             const int all_lo = window_start(p, pc.len);
             if (pc.count > 0) {
-                constexpr int kChunks = D / 8, kPer = 32 / kChunks;       // 16-byte chunks of a row, rows of a warp's pass
-                constexpr int kBatch = kRows / kPer / F::SOFT < 8 ? kRows / kPer / F::SOFT : 8;
+                // 16-byte chunks of a row, rows of a warp's pass; kBatch loads are under way at a time
+                constexpr int kChunks = D / 8, kPer = 32 / kChunks, kPasses = kRows / kPer / F::SOFT, kBatch = 4;
+                static_assert(kPasses % kBatch == 0, "passes of a batch");
                 const int j = lane % kChunks;
-                for (int r0 = 0; r0 < kRows / kPer; r0 += kBatch * F::SOFT) {
+                const bool wide = ((reinterpret_cast<uintptr_t>(p.q) | static_cast<uintptr_t>(p.q_stride * 2)) & 15) == 0;
+#pragma unroll 1
+                for (int k0 = 0; k0 < kPasses; k0 += kBatch) {
                     uint4 x[kBatch];
 #pragma unroll
                     for (int k = 0; k < kBatch; ++k) {
-                        const int r = (r0 + k * F::SOFT + warp) * kPer + lane / kChunks, i = pc.row0 + r;
+                        const int r = ((k0 + k) * F::SOFT + warp) * kPer + lane / kChunks, i = pc.row0 + r;
                         x[k] = make_uint4(0u, 0u, 0u, 0u);
                         if (r < pc.rows) {
                             const int t = token_of(i), hd = i - t * p.group;
                             const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) +
                                 (static_cast<long long>(pc.b) * p.q_len + t) * p.q_stride +
                                 static_cast<long long>(pc.kvh * p.group + hd) * D + 8 * j;
-                            if ((reinterpret_cast<uintptr_t>(q) & 15) == 0) {
+                            if (wide) {
                                 x[k] = *reinterpret_cast<const uint4*>(q);
                             } else {
                                 const unsigned short* h = reinterpret_cast<const unsigned short*>(q);
@@ -471,10 +502,13 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                             }
                         }
                     }
-#pragma unroll
+#pragma unroll 1
                     for (int k = 0; k < kBatch; ++k) {
-                        const int r = (r0 + k * F::SOFT + warp) * kPer + lane / kChunks;
-                        const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+                        const uint4 y = x[0];                     // rotated through
+#pragma unroll
+                        for (int n = 0; n + 1 < kBatch; ++n) x[n] = x[n + 1];
+                        const int r = ((k0 + k) * F::SOFT + warp) * kPer + lane / kChunks;
+                        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
                         float v[8], big = 0.0f;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -525,8 +559,8 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 const int buf = i & 1, use = (buf ? uses1 : uses0) + (i >> 1), tile = tiles + i;
                 const int meta = tile & (kMeta - 1), pos = (pc.tile0 + i) * KT;
                 const uint32_t ts = tq + buf * KT, to = tq + F::O_COL + (F::STREAMS == 2 ? stream * D : 0);
-                ok = ok && tcg::warp_wait(s.s_full + buf, use & 1, gave_up);
-                ok = ok && tcg::warp_wait(s.meta_full + meta, (tile / kMeta) & 1, gave_up);
+                ok = ok && warp_wait(s.s_full + buf, use & 1, gave_up);
+                ok = ok && warp_wait(s.meta_full + meta, (tile / kMeta) & 1, gave_up);
                 if (ok && warp_lives) {
                     tcg::tc_fence_after();
                     const bool edge = pos < all_lo || pos + KT > pc.base;
@@ -534,51 +568,32 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                     auto rescale = [&](float g) {
                         if (i < F::STREAMS) return;
                         const int last = i - F::STREAMS, pb = last & 1;
-                        ok = ok && tcg::warp_wait(s.pv_done + pb, ((pb ? uses1 : uses0) + (last >> 1)) & 1, gave_up);
+                        ok = ok && warp_wait(s.pv_done + pb, ((pb ? uses1 : uses0) + (last >> 1)) & 1, gave_up);
                         tcg::tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < NG; ++c) {
-                            uint32_t v[32];
-                            tmem_ld32(to + 32 * c, v);
+                        for (int c = 0; c < 4 * NG; ++c) {
+                            uint32_t v[8];
+                            tmem_ld8(to + 8 * c, v);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * g);
-                            tcg::tmem_st32(to + 32 * c, v);
+                            for (int k = 0; k < 8; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * g);
+                            tmem_st8(to + 8 * c, v);
                         }
                     };
-                    const int e_new = max(s.ev[meta][0], KT == 128 ? s.ev[meta][1] : -100);
+                    const int e_new = s.e_top[meta];
                     if (e_new > E + kSlack) {                         // the same for the whole warp
                         rescale(pow2i(max(E - e_new, -126)));
                         E = e_new;
                     }
-                    // A score of chunk c passes M by more than kLazy: M becomes the next integer above it, so that what is
-                    // there already, the P of the chunks before c too, is scaled by a power of two.
-                    auto raise = [&](float mx, int c) {
-                        const float now = mx > M + kLazy ? ceilf(mx) : M, f = ex2(M - now);
-                        M = now;
-                        l *= f;
-                        rescale(f);
-                        const __half2 f2 = __float2half2_rn(f);
+                    const bool plain = !edge && p.soft_cap == 0.0f;
 #pragma unroll 1
-                        for (int b = 0; b < 2 * c; ++b) {
-                            uint32_t v[8];
-                            tmem_ld8(ts + 8 * b, v);
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) v[k] = h2_bits(__hmul2(bits_h2(v[k]), f2));
-                            tmem_st8(ts + 8 * b, v);
-                        }
-                    };
-                    if (!edge && p.soft_cap == 0.0f) {
-#pragma unroll 1
-                        for (int c = 0; c < KT / 32; ++c) {
+                    for (int c = 0; c < KT / 32; ++c) {
+                        const float fc = fac * s.k_unit[meta][c];
+                        const int sh = kBias + s.ev[meta][c] - E;
+                        if (plain) {
+                            // Without the maximum: P may pass 1, and the sum of 32 says whether it stays in fp16's range.
+                            // Where it does not, or M is so large that its rounding counts, the chunk goes the long way.
                             uint32_t v[32];
                             tmem_ld32(ts + 32 * c, v);
-                            const float fc = fac * pow2i(s.ek[meta][c]);
-                            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
-                            const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), mx = top == -INFINITY ? top : top * fc;
-                            if (__any_sync(0xffffffffu, mx > M + kLazy)) raise(mx, c);
-                            const int sh = kBias + s.ev[meta][c >> 1] - E;
                             const float at = static_cast<float>(sh) - M;
                             const f2 fc2 = mk2(fc, fc), at2 = mk2(at, at);
                             f2 sum0 = mk2(0.0f, 0.0f), sum1 = sum0;
@@ -591,53 +606,66 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                                 else sum0 = add2(sum0, mk2(a, b));
                                 out[k] = h2_bits(__floats2half2_rn(a, b));
                             }
-                            const f2 sum = add2(sum0, sum1);
-                            l = fmaf(lo(sum) + hi(sum), pow2i(-sh), l);
-                            tmem_st16(ts + 16 * c, out);              // columns that this lane has read
+                            const f2 sums = add2(sum0, sum1);
+                            const float sum = lo(sums) + hi(sums);
+                            if (!__any_sync(0xffffffffu, sum > kMostSum || fabsf(M) > kMostM)) {
+                                l = fmaf(sum, pow2i(-sh), l);
+                                tmem_st16(ts + 16 * c, out);          // columns that this lane has read
+                                continue;
+                            }
                         }
-                    } else {
+                        const uint32_t bits = edge ? visible(pos + 32 * c) : 0xFFFFFFFFu;
+                        float mx = -INFINITY;
 #pragma unroll 1
-                        for (int c = 0; c < KT / 32; ++c) {
-                            const uint32_t bits = edge ? visible(pos + 32 * c) : 0xFFFFFFFFu;
-                            const float fc = fac * pow2i(s.ek[meta][c]);
-                            float mx = -INFINITY;
+                        for (int b = 0; b < 4; ++b) {                 // S becomes the scaled, capped and masked score
+                            uint32_t v[8];
+                            tmem_ld8(ts + 32 * c + 8 * b, v);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                float y = __uint_as_float(v[k]) * fc;
+                                if (p.soft_cap > 0.0f) y = tanhf(y * inv_cap) * (p.soft_cap * kLog2e);
+                                y = (bits >> (8 * b + k)) & 1u ? y : -INFINITY;
+                                mx = fmaxf(mx, y);
+                                v[k] = __float_as_uint(y);
+                            }
+                            tmem_st8(ts + 32 * c + 8 * b, v);
+                        }
+                        tcg::tmem_wait_st();
+                        if (__any_sync(0xffffffffu, mx > M + kLazy)) {
+                            // M becomes the next integer above the score, so that what is there already, the P of the chunks
+                            // before c too, is scaled by a power of two
+                            const float now = mx > M + kLazy ? ceilf(mx) : M, f = ex2(M - now);
+                            M = now;
+                            l *= f;
+                            rescale(f);
+                            const __half2 f2 = __float2half2_rn(f);
 #pragma unroll 1
-                            for (int b = 0; b < 4; ++b) {             // S becomes the scaled, capped and masked score
+                            for (int b = 0; b < 2 * c; ++b) {
                                 uint32_t v[8];
-                                tmem_ld8(ts + 32 * c + 8 * b, v);
+                                tmem_ld8(ts + 8 * b, v);
 #pragma unroll
-                                for (int k = 0; k < 8; ++k) {
-                                    float y = __uint_as_float(v[k]) * fc;
-                                    if (p.soft_cap > 0.0f) y = tanhf(y * inv_cap) * (p.soft_cap * kLog2e);
-                                    y = (bits >> (8 * b + k)) & 1u ? y : -INFINITY;
-                                    mx = fmaxf(mx, y);
-                                    v[k] = __float_as_uint(y);
-                                }
-                                tmem_st8(ts + 32 * c + 8 * b, v);
+                                for (int k = 0; k < 8; ++k) v[k] = h2_bits(__hmul2(bits_h2(v[k]), f2));
+                                tmem_st8(ts + 8 * b, v);
                             }
-                            tcg::tmem_wait_st();
-                            if (__any_sync(0xffffffffu, mx > M + kLazy)) raise(mx, c);
-                            const int sh = kBias + s.ev[meta][c >> 1] - E;
-                            const float at = static_cast<float>(sh) - M;
-                            float sum = 0.0f;
-#pragma unroll 1
-                            for (int b = 0; b < 4; ++b) {
-                                uint32_t v[8], out[4];
-                                tmem_ld8(ts + 32 * c + 8 * b, v);
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    const float a = ex2(__uint_as_float(v[2 * k]) + at), d = ex2(__uint_as_float(v[2 * k + 1]) + at);
-                                    sum += a + d;
-                                    out[k] = h2_bits(__floats2half2_rn(a, d));
-                                }
-                                tmem_st4(ts + 16 * c + 4 * b, out);
-                            }
-                            l = fmaf(sum, pow2i(-sh), l);
                         }
+                        const float at = static_cast<float>(sh) - M;
+                        float sum = 0.0f;
+#pragma unroll 1
+                        for (int b = 0; b < 4; ++b) {
+                            uint32_t v[8], out[4];
+                            tmem_ld8(ts + 32 * c + 8 * b, v);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float a = ex2(__uint_as_float(v[2 * k]) + at), d = ex2(__uint_as_float(v[2 * k + 1]) + at);
+                                sum += a + d;
+                                out[k] = h2_bits(__floats2half2_rn(a, d));
+                            }
+                            tmem_st4(ts + 16 * c + 4 * b, out);
+                        }
+                        l = fmaf(sum, pow2i(-sh), l);
                     }
-                    for (int h = 0; h < KT / 64; ++h) {
-                        if (!s.nan_any[meta][h]) continue;
-                        for (int k = 64 * h; k < 64 * h + 64; ++k) {
+                    if (s.nan_any[meta]) {
+                        for (int k = 0; k < KT; ++k) {
                             const int g = s.nan[meta][k];
                             if (g && (edge ? (visible(pos + (k & ~31)) >> (k & 31)) & 1u : alive)) nan_groups |= g;
                         }
@@ -650,8 +678,8 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             }
             // -------------------------------------------------- the streams' results, and the rows' outputs
             const int n0 = (pc.count + 1) >> 1, n1 = pc.count >> 1;   // uses of the buffers
-            if (n0 > 0) ok = ok && tcg::warp_wait(s.pv_done, (uses0 + n0 - 1) & 1, gave_up);
-            if (n1 > 0) ok = ok && tcg::warp_wait(s.pv_done + 1, (uses1 + n1 - 1) & 1, gave_up);
+            if (n0 > 0) ok = ok && warp_wait(s.pv_done, (uses0 + n0 - 1) & 1, gave_up);
+            if (n1 > 0) ok = ok && warp_wait(s.pv_done + 1, (uses1 + n1 - 1) & 1, gave_up);
             s.ml[stream][row][0] = M;
             s.ml[stream][row][1] = l;
             s.er[stream][row] = static_cast<short>(E);
@@ -684,54 +712,45 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             constexpr int kCols = D / F::STREAMS;                     // columns of a warp
             if (ok && warp_lives) {
+                const int t = token_of(min(i, p.q_len * p.group - 1)), hd = i - t * p.group;
+                __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(p.out) +
+                    (((static_cast<long long>(pc.b) * p.q_len + t) * p.kv_heads + pc.kvh) * p.group + hd) * D;
+                float* const part = p.part + static_cast<long long>(slot) * (kRows * (D + 2)) + row * D;
 #pragma unroll 1
-                for (int c = 0; c < kCols / 32; ++c) {
-                    const int d = stream * kCols + 32 * c;
-                    float o[32];
-                    uint32_t v[32];
+                for (int d = stream * kCols; d < (stream + 1) * kCols; d += 8) {
+                    float o[8] = {};
+                    uint32_t v[8];
                     if (pc.count > 0) {
-                        tmem_ld32(tq + F::O_COL + d, v);
+                        tmem_ld8(tq + F::O_COL + d, v);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(v[k]) * w0;
+                        for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[k]) * w0;
                     }
                     if (two) {
-                        tmem_ld32(tq + F::O_COL + D + d, v);
+                        tmem_ld8(tq + F::O_COL + D + d, v);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = fmaf(__uint_as_float(v[k]), w1, o[k]);
+                        for (int k = 0; k < 8; ++k) o[k] = fmaf(__uint_as_float(v[k]), w1, o[k]);
                     }
                     const bool nan = (gone >> (d >> 5)) & 1;
-                    if (row < pc.rows) {
-                        if (whole) {
-                            const int t = token_of(i), hd = i - t * p.group;
-                            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) +
-                                (((static_cast<long long>(pc.b) * p.q_len + t) * p.kv_heads + pc.kvh) * p.group + hd) * D + d;
+                    if (row >= pc.rows) continue;                     // after the warp's loads
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                uint32_t h[4];
+                    for (int k = 0; k < 8; ++k) o[k] = !alive || L == 0.0f ? 0.0f : nan ? NAN : o[k];   // a row that sees nothing is zero
+                    if (whole) {
+                        uint32_t h[4];
 #pragma unroll
-                                for (int n = 0; n < 4; ++n) {
-                                    const float a = inv == 0.0f ? 0.0f : o[8 * k + 2 * n] * inv;    // a row that sees nothing
-                                    const float b = inv == 0.0f ? 0.0f : o[8 * k + 2 * n + 1] * inv;
-                                    const __nv_bfloat162 r2 = __floats2bfloat162_rn(a, b);
-                                    h[n] = nan ? 0x7FC07FC0u : *reinterpret_cast<const uint32_t*>(&r2);
-                                }
-                                reinterpret_cast<uint4*>(out)[k] = make_uint4(h[0], h[1], h[2], h[3]);
-                            }
-                        } else {
-                            float* part = p.part + static_cast<long long>(slot) * (kRows * (D + 2)) + row * D + d;
-#pragma unroll
-                            for (int k = 0; k < 8; ++k)
-                                reinterpret_cast<float4*>(part)[k] =
-                                    nan ? make_float4(NAN, NAN, NAN, NAN)
-                                    : alive ? make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3])
-                                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        for (int n = 0; n < 4; ++n) {
+                            const __nv_bfloat162 r2 = __floats2bfloat162_rn(o[2 * n] * inv, o[2 * n + 1] * inv);
+                            h[n] = *reinterpret_cast<const uint32_t*>(&r2);
                         }
+                        *reinterpret_cast<uint4*>(out + d) = make_uint4(h[0], h[1], h[2], h[3]);
+                    } else {
+                        reinterpret_cast<float4*>(part + d)[0] = make_float4(o[0], o[1], o[2], o[3]);
+                        reinterpret_cast<float4*>(part + d)[1] = make_float4(o[4], o[5], o[6], o[7]);
                     }
                 }
                 if (!whole && stream == 0 && row < pc.rows) {
-                    float* part = p.part + static_cast<long long>(slot) * (kRows * (D + 2)) + kRows * D + row * 2;
-                    part[0] = top;
-                    part[1] = L;
+                    float* const ml = p.part + static_cast<long long>(slot) * (kRows * (D + 2)) + kRows * D + row * 2;
+                    ml[0] = top;
+                    ml[1] = L;
                 }
             }
             tcg::tc_fence_before();
@@ -747,24 +766,20 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         while (next_piece<KT>(line, p, items, pc)) {
             for (int i = 0; i < pc.count; ++i, ++tile) {
                 const int slot = tile % F::RAW, ks = tile & 1;
-                ok = ok && tcg::warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
-                ok = ok && tcg::warp_wait(s.meta_full + (tile & (kMeta - 1)), (tile / kMeta) & 1, gave_up);
-                if (tile >= 2) ok = ok && tcg::warp_wait(s.k_empty + ks, ((tile >> 1) - 1) & 1, gave_up);
+                ok = ok && warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
+                ok = ok && warp_wait(s.meta_full + (tile & (kMeta - 1)), (tile / kMeta) & 1, gave_up);
+                if (tile >= 2) ok = ok && warp_wait(s.k_empty + ks, ((tile >> 1) - 1) & 1, gave_up);
                 if (!ok) break;
                 const uint32_t raw = at_raw + slot * F::RAW_BYTES;
-                const uint32_t valid = s.valid[slot][span];
-                const Unit unit(s.ek[tile & (kMeta - 1)][span]);
                 const uint32_t to = at_k + ks * F::KHAT;
 #pragma unroll 2
                 for (int it = 0; it < 4; ++it) {
-                    const int at = 8 * it + pos_in, r = 32 * span + at;
+                    const int r = 32 * span + 8 * it + pos_in;
                     uint32_t w[GW], d[GW / 2];
                     lds_words<GW>(raw + r * (D / 2) + c * (4 * NG) + half * 16, w);
                     lds_words<GW / 2>(raw + F::K_SC + r * (2 * NG) + half * 8, d);
-                    const bool live = (valid >> at) & 1u;
 #pragma unroll
                     for (int g = 0; g < GW; ++g) {
-                        if ((g & 1) == 0) d[g / 2] = live ? unit.of(d[g / 2]) : 0u;
                         uint32_t out[4];
                         decode8(w[g], bits_h2(__byte_perm(d[g / 2], 0u, g & 1 ? 0x3232 : 0x1010)), out);
                         const int j = 4 * (4 * half + g) + c;
@@ -796,13 +811,11 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         while (next_piece<KT>(line, p, items, pc)) {
             for (int i = 0; i < pc.count; ++i, ++tile) {
                 const int slot = tile % F::RAW, vs = tile % F::V_STAGES, meta = tile & (kMeta - 1);
-                ok = ok && tcg::warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
-                ok = ok && tcg::warp_wait(s.meta_full + meta, (tile / kMeta) & 1, gave_up);
-                if (tile >= F::V_STAGES) ok = ok && tcg::warp_wait(s.v_empty + vs, (tile / F::V_STAGES - 1) & 1, gave_up);
+                ok = ok && warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
+                ok = ok && warp_wait(s.meta_full + meta, (tile / kMeta) & 1, gave_up);
+                if (tile >= F::V_STAGES) ok = ok && warp_wait(s.v_empty + vs, (tile / F::V_STAGES - 1) & 1, gave_up);
                 if (!ok) break;
                 const uint32_t raw = at_raw + slot * F::RAW_BYTES;
-                const Unit unit(s.ev[meta][part]);
-                const bool care = s.care[meta] != 0;
                 const uint32_t to = at_v + vs * F::VHAT + part * (D * 128);
 #pragma unroll 1
                 for (int n = 0; n < kPasses; ++n) {
@@ -815,17 +828,6 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                         code[k] = lds_word(blk + (k & 6) * (D / 2) + (k & 1 ? (flip ^ 1) : flip) * (D / 2));
                         d[k] = lds_word(sc + (k & 6) * (2 * NG) + (k & 1 ? (flip ^ 1) : flip) * (2 * NG));
                     }
-                    if (care) {
-                        const uint32_t live = s.valid[slot][pos >> 5] >> (pos & 31);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            if ((d[k] & 0x7FFFu) >= 0x7C00u) d[k] &= 0xFFFF0000u;
-                            if (((d[k] >> 16) & 0x7FFFu) >= 0x7C00u) d[k] &= 0x0000FFFFu;
-                            if (((live >> (k ^ flip)) & 1u) == 0u) d[k] = 0u;
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) d[k] = unit.of(d[k]);
 #pragma unroll 1
                     for (int x = 0; x < 2; ++x) {
                         const uint32_t pick = flip ? (x ? 0x3276u : 0x1054u) : x ? 0x7632u : 0x5410u;
@@ -900,7 +902,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                     }
                 }
                 const uint32_t upper = __shfl_down_sync(0xffffffffu, bits, 4);
-                if (tile >= F::RAW) ok = ok && tcg::warp_wait(s.raw_empty + slot, (tile / F::RAW - 1) & 1, gave_up);
+                if (tile >= F::RAW) ok = ok && warp_wait(s.raw_empty + slot, (tile / F::RAW - 1) & 1, gave_up);
                 if (!ok) break;
                 if ((lane & 7) == 0) s.valid[slot][lane >> 3] = bits | upper << 16;
                 const int blocks = __popc(__ballot_sync(0xffffffffu, has)) / 4;
@@ -923,47 +925,57 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         if (!ok)                          // the copies under way end before the CTA does
             for (int t = max(0, tile - F::RAW); t < tile; ++t) mbar_wait(s.raw_full + t % F::RAW, (t / F::RAW) & 1);
     } else if (warp >= F::SOFT + 10) {
-        // ------------------------------------------------------ exponents of a tile's scales: one warp K's, one V's
+        // ------------------------------------------------------ exponents of a tile's scales, which become d 2^-e: one warp
+        // K's, one V's
         const bool is_v = warp == F::SOFT + 11;
         int tile = 0;
         while (next_piece<KT>(line, p, items, pc)) {
             for (int i = 0; i < pc.count; ++i, ++tile) {
                 const int slot = tile % F::RAW, meta = tile & (kMeta - 1);
-                ok = ok && tcg::warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
+                ok = ok && warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
                 if (!ok) break;
-                uint32_t all = 0xFFFFFFFFu, top64 = 0u;
+                int e_top = -100;
                 bool any = false;
 #pragma unroll 1
                 for (int c = 0; c < KT / 32; ++c) {               // 32 positions, a lane each
-                    const uint32_t valid = s.valid[slot][c];
+                    const uint32_t at = at_raw + slot * F::RAW_BYTES + (is_v ? F::V_SC : F::K_SC) + (32 * c + lane) * (2 * NG);
+                    const bool mine = (s.valid[slot][c] >> lane) & 1u;
                     uint32_t w[NG / 2];
-                    lds_words<NG / 2>(at_raw + slot * F::RAW_BYTES + (is_v ? F::V_SC : F::K_SC) + (32 * c + lane) * (2 * NG), w);
-                    const bool mine = (valid >> lane) & 1u;
+                    lds_words<NG / 2>(at, w);
                     uint32_t top = __reduce_max_sync(0xffffffffu, mine ? top_of(w, false) : 0u);
-                    const bool nan = top >= 0x7C00u;
-                    if (nan) top = __reduce_max_sync(0xffffffffu, mine ? top_of(w, true) : 0u);
-                    all &= valid;
-                    if (!is_v) {
-                        if (lane == 0) s.ek[meta][c] = exponent_of(top);
-                        continue;
-                    }
-                    // V: 64 positions share one; NaN groups count as zero, and their rows are marked
-                    if ((c & 1) == 0) top64 = 0u, any = false;
-                    top64 = max(top64, top);
-                    any |= nan;
-                    int bad = 0;
-                    if (nan && mine) {
+                    if (top >= 0x7C00u) {
+                        top = __reduce_max_sync(0xffffffffu, mine ? top_of(w, true) : 0u);
+                        if (is_v) {                               // NaN groups of V count as zero, and their rows are marked
+                            if (!any)
+                                for (int k = lane; k < KT; k += 32) s.nan[meta][k] = 0;
+                            any = true;
+                            int bad = 0;
 #pragma unroll
-                        for (int g = 0; g < NG; ++g) bad |= ((w[g / 2] >> (16 * (g & 1))) & 0x7FFFu) >= 0x7C00u ? 1 << g : 0;
+                            for (int g = 0; g < NG; ++g)
+                                if (((w[g / 2] >> (16 * (g & 1))) & 0x7FFFu) >= 0x7C00u) {
+                                    bad |= 1 << g;
+                                    w[g / 2] &= g & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                                }
+                            __syncwarp();
+                            if (mine) s.nan[meta][32 * c + lane] = static_cast<uint8_t>(bad);
+                        }
                     }
-                    s.nan[meta][32 * c + lane] = static_cast<uint8_t>(bad);
-                    if (nan) all = 0u;
-                    if ((c & 1) == 1 && lane == 0) {
-                        s.ev[meta][c >> 1] = exponent_of(top64);
-                        s.nan_any[meta][c >> 1] = any;
+                    const int e = exponent_of(top);
+                    const Unit unit(e);
+#pragma unroll
+                    for (int k = 0; k < NG / 2; ++k) w[k] = mine ? unit.of(w[k]) : 0u;
+                    sts_words<NG / 2>(at, w);
+                    e_top = max(e_top, e);
+                    if (lane == 0) {
+                        if (is_v) s.ev[meta][c] = e;
+                        else s.k_unit[meta][c] = pow2i(e);
                     }
                 }
-                if (is_v && lane == 0) s.care[meta] = all != 0xFFFFFFFFu;
+                if (is_v && lane == 0) {
+                    s.e_top[meta] = e_top;
+                    s.nan_any[meta] = any;
+                }
+                fence_proxy_shared();                             // the slot's next writer is a bulk copy
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(s.meta_full + meta);
@@ -976,39 +988,47 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         // ------------------------------------------------------ MMA issue
         if (lane == 0) {
             constexpr uint32_t kS = tcg::idesc_f16(KT), kO = tcg::idesc_f16(D);
+            // descriptors count 16-byte units: 2 for 16 values of K, an atom of 64 for its rows' 128 bytes
+            const uint64_t q_desc = tcg::sdesc(at_q), k_desc = tcg::sdesc(at_k), v_desc = tcg::sdesc(at_v);
             int tile = 0, pieces = 0, uses0 = 0, uses1 = 0;
             while (ok && next_piece<KT>(line, p, items, pc)) {
                 if (pc.count == 0) continue;
-                auto scores = [&](int i) {
-                    const int t = tile + i, ks = t & 1, buf = i & 1;
-                    ok = ok && tcg::wait_bar(s.k_full + ks, (t >> 1) & 1, gave_up);
-                    if (!ok) return;
-                    tcg::tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-                        mma_ss(tmem + buf * KT, tcg::sdesc(at_q + (k >> 2) * (kRows * 128) + (k & 3) * 32),
-                               tcg::sdesc(at_k + ks * F::KHAT + (k >> 2) * (KT * 128) + (k & 3) * 32), kS, k > 0);
-                    tcg::tc_commit(s.k_empty + ks);
-                    tcg::tc_commit(s.s_full + buf);
-                };
-                ok = ok && tcg::wait_bar(&s.q_full, pieces & 1, gave_up);
+                ok = ok && wait_bar(&s.q_full, pieces & 1, gave_up);
                 ++pieces;
-                if (ok) scores(0);
-                if (ok && pc.count > 1) scores(1);
-                for (int i = 0; ok && i < pc.count; ++i) {
-                    const int t = tile + i, vs = t % F::V_STAGES, buf = i & 1, use = (buf ? uses1 : uses0) + (i >> 1);
-                    ok = ok && tcg::wait_bar(s.v_full + vs, (t / F::V_STAGES) & 1, gave_up);
-                    ok = ok && tcg::wait_bar(s.p_full + buf, use & 1, gave_up);
-                    if (!ok) break;
-                    tcg::tc_fence_after();
-                    const uint32_t to = tmem + F::O_COL + (F::STREAMS == 2 ? buf * D : 0);
+#pragma unroll 1
+                for (int i = -2; ok && i < pc.count; ++i) {           // O of tile i, then S of tile i + 2
+                    if (i >= 0) {
+                        const int t = tile + i, vs = t % F::V_STAGES, buf = i & 1, use = (buf ? uses1 : uses0) + (i >> 1);
+                        ok = ok && wait_bar(s.v_full + vs, (t / F::V_STAGES) & 1, gave_up);
+                        ok = ok && wait_bar(s.p_full + buf, use & 1, gave_up);
+                        if (!ok) break;
+                        tcg::tc_fence_after();
+                        const uint32_t to = tmem + F::O_COL + (F::STREAMS == 2 ? buf * D : 0);
+                        const uint64_t v = v_desc + vs * (F::VHAT >> 4);
+                        bool add = i >= F::STREAMS;
+#pragma unroll 1
+                        for (int h = 0; h < KT / 64; ++h)
 #pragma unroll
-                    for (int k = 0; k < KT / 16; ++k)
-                        mma_ts(to, tmem + buf * KT + 8 * k, tcg::sdesc(at_v + vs * F::VHAT + (k >> 2) * (D * 128) + (k & 3) * 32), kO,
-                               i >= F::STREAMS || k > 0);
-                    tcg::tc_commit(s.v_empty + vs);
-                    tcg::tc_commit(s.pv_done + buf);
-                    if (i + 2 < pc.count) scores(i + 2);
+                            for (int k = 0; k < 4; ++k, add = true)
+                                mma_ts(to, tmem + buf * KT + 32 * h + 8 * k, v + h * (D * 8) + 2 * k, kO, add);
+                        tcg::tc_commit(s.v_empty + vs);
+                        tcg::tc_commit(s.pv_done + buf);
+                    }
+                    if (i + 2 < pc.count) {
+                        const int t = tile + i + 2, ks = t & 1, buf = i & 1;
+                        ok = ok && wait_bar(s.k_full + ks, (t >> 1) & 1, gave_up);
+                        if (!ok) break;
+                        tcg::tc_fence_after();
+                        const uint64_t k_at = k_desc + ks * (F::KHAT >> 4);
+                        bool add = false;
+#pragma unroll 1
+                        for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k, add = true)
+                                mma_ss(tmem + buf * KT, q_desc + h * (kRows * 8) + 2 * k, k_at + h * (KT * 8) + 2 * k, kS, add);
+                        tcg::tc_commit(s.k_empty + ks);
+                        tcg::tc_commit(s.s_full + buf);
+                    }
                 }
                 uses0 += (pc.count + 1) >> 1;
                 uses1 += pc.count >> 1;
