@@ -202,16 +202,45 @@ __device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4])
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
                  : "memory");
 }
-// d (+)= a b, both operands in shared memory, or a in tensor memory; fp16, K = 16.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
-                 : "memory");
+// d (+)= a b for 64 values of K (four MMAs, fp16): both operands in shared memory, or a in tensor memory.  The whole warp
+// comes here and `one` of it issues, so that the operands stay in uniform registers: by a lone thread an MMA took 150
+// cycles to issue.
+__device__ __forceinline__ void mma64_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t one) {
+    asm volatile(
+        "{\n .reg .pred p, q, t;\n .reg .b64 a1, a2, a3, b1, b2, b3;\n"
+        " setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n setp.eq.b32 t, %3, %3;\n"
+        " add.s64 a1, %1, 2;\n add.s64 a2, %1, 4;\n add.s64 a3, %1, 6;\n add.s64 b1, %2, 2;\n add.s64 b2, %2, 4;\n add.s64 b3, %2, 6;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(one)
+        : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-                 "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
-                 : "memory");
+__device__ __forceinline__ void mma64_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t one) {
+    asm volatile(
+        "{\n .reg .pred p, q, t;\n .reg .b32 a1, a2, a3;\n .reg .b64 b1, b2, b3;\n"
+        " setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n setp.eq.b32 t, %3, %3;\n"
+        " add.s32 a1, %1, 8;\n add.s32 a2, %1, 16;\n add.s32 a3, %1, 24;\n add.s64 b1, %2, 2;\n add.s64 b2, %2, 4;\n add.s64 b3, %2, 6;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ void commit2(uint64_t* x, uint64_t* y, uint32_t one) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n}\n" ::"r"(smem_u32(x)),
+        "r"(smem_u32(y)), "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+    return one;
 }
 
 // Codes to fp16.  The 8 codes of a word, each half of an output pair 16 bits
@@ -986,54 +1015,48 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         }
     } else {
         // ------------------------------------------------------ MMA issue
-        if (lane == 0) {
-            constexpr uint32_t kS = tcg::idesc_f16(KT), kO = tcg::idesc_f16(D);
-            // descriptors count 16-byte units: 2 for 16 values of K, an atom of 64 for its rows' 128 bytes
-            const uint64_t q_desc = tcg::sdesc(at_q), k_desc = tcg::sdesc(at_k), v_desc = tcg::sdesc(at_v);
-            int tile = 0, pieces = 0, uses0 = 0, uses1 = 0;
-            while (ok && next_piece<KT>(line, p, items, pc)) {
-                if (pc.count == 0) continue;
-                ok = ok && wait_bar(&s.q_full, pieces & 1, gave_up);
-                ++pieces;
+        constexpr uint32_t kS = tcg::idesc_f16(KT), kO = tcg::idesc_f16(D);
+        const uint32_t one = elect_one();
+        // descriptors count 16-byte units: 2 for 16 values of K, an atom of 64 for its rows' 128 bytes
+        const uint64_t q_desc = tcg::sdesc(at_q), k_desc = tcg::sdesc(at_k), v_desc = tcg::sdesc(at_v);
+        int tile = 0, pieces = 0, uses0 = 0, uses1 = 0;
+        while (ok && next_piece<KT>(line, p, items, pc)) {
+            if (pc.count == 0) continue;
+            ok = ok && warp_wait(&s.q_full, pieces & 1, gave_up);
+            ++pieces;
 #pragma unroll 1
-                for (int i = -2; ok && i < pc.count; ++i) {           // O of tile i, then S of tile i + 2
-                    if (i >= 0) {
-                        const int t = tile + i, vs = t % F::V_STAGES, buf = i & 1, use = (buf ? uses1 : uses0) + (i >> 1);
-                        ok = ok && wait_bar(s.v_full + vs, (t / F::V_STAGES) & 1, gave_up);
-                        ok = ok && wait_bar(s.p_full + buf, use & 1, gave_up);
-                        if (!ok) break;
-                        tcg::tc_fence_after();
-                        const uint32_t to = tmem + F::O_COL + (F::STREAMS == 2 ? buf * D : 0);
-                        const uint64_t v = v_desc + vs * (F::VHAT >> 4);
-                        bool add = i >= F::STREAMS;
-#pragma unroll 1
-                        for (int h = 0; h < KT / 64; ++h)
+            for (int i = -2; ok && i < pc.count; ++i) {               // O of tile i, then S of tile i + 2
+                const int buf = i & 1;
+                if (i >= 0) {
+                    const int t = tile + i, vs = t % F::V_STAGES, use = (buf ? uses1 : uses0) + (i >> 1);
+                    ok = ok && warp_wait(s.v_full + vs, (t / F::V_STAGES) & 1, gave_up);
+                    ok = ok && warp_wait(s.p_full + buf, use & 1, gave_up);
+                    if (!ok) break;
+                    tcg::tc_fence_after();
+                    const uint32_t to = tmem + F::O_COL + (F::STREAMS == 2 ? buf * D : 0);
+                    const uint64_t v = v_desc + vs * (F::VHAT >> 4);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k, add = true)
-                                mma_ts(to, tmem + buf * KT + 32 * h + 8 * k, v + h * (D * 8) + 2 * k, kO, add);
-                        tcg::tc_commit(s.v_empty + vs);
-                        tcg::tc_commit(s.pv_done + buf);
-                    }
-                    if (i + 2 < pc.count) {
-                        const int t = tile + i + 2, ks = t & 1, buf = i & 1;
-                        ok = ok && wait_bar(s.k_full + ks, (t >> 1) & 1, gave_up);
-                        if (!ok) break;
-                        tcg::tc_fence_after();
-                        const uint64_t k_at = k_desc + ks * (F::KHAT >> 4);
-                        bool add = false;
-#pragma unroll 1
-                        for (int h = 0; h < D / 64; ++h)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k, add = true)
-                                mma_ss(tmem + buf * KT, q_desc + h * (kRows * 8) + 2 * k, k_at + h * (KT * 8) + 2 * k, kS, add);
-                        tcg::tc_commit(s.k_empty + ks);
-                        tcg::tc_commit(s.s_full + buf);
-                    }
+                    for (int h = 0; h < KT / 64; ++h)
+                        mma64_ts(to, tmem + buf * KT + 32 * h, v + h * (D * 8), kO, h > 0 || i >= F::STREAMS, one);
+                    commit2(s.v_empty + vs, s.pv_done + buf, one);
                 }
-                uses0 += (pc.count + 1) >> 1;
-                uses1 += pc.count >> 1;
-                tile += pc.count;
+                if (i + 2 < pc.count) {
+                    const int t = tile + i + 2, ks = t & 1;
+                    ok = ok && warp_wait(s.k_full + ks, (t >> 1) & 1, gave_up);
+                    if (!ok) break;
+                    tcg::tc_fence_after();
+                    const uint64_t k_at = k_desc + ks * (F::KHAT >> 4);
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h)
+                        mma64_ss(tmem + buf * KT, q_desc + h * (kRows * 8), k_at + h * (KT * 8), kS, h > 0, one);
+                    commit2(s.k_empty + ks, s.s_full + buf, one);
+                }
             }
+            uses0 += (pc.count + 1) >> 1;
+            uses1 += pc.count >> 1;
+            tile += pc.count;
+        }
+        if (one) {
             tcg::tc_commit(&s.done);      // every MMA issued has completed before tensor memory is released
             mbar_wait(&s.done, 0);
         }
