@@ -888,65 +888,70 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::R_REST));
     if (warp == F::SOFT + 8) {
         // ------------------------------------------------------ codes and scales from the cache
+        // Lane 4 n + k sees to section k of the n-th 16 positions of a tile.  Page ids are asked for a tile ahead: they are
+        // all that the copies' addresses wait for.
         int tile = 0, seq = -1;
+        const int blk = lane >> 2, k = lane & 3;
+        const int row = k < 2 ? D / 2 : 2 * NG;                       // bytes of a position in the section
+        const int to = (k == 0 ? 0 : k == 1 ? F::V_CODES : k == 2 ? F::K_SC : F::V_SC) + 16 * blk * row;
+        const long long section = static_cast<long long>(p.page_size) * (k < 2 ? k * (D / 2) : D + (k - 2) * (2 * NG));
+        const long long block = kv4_block_bytes(p.page_size, D);
         while (next_piece<KT>(line, p, items, pc)) {
             const int lo = window_start(p, pc.base + 1);
+            auto page_of = [&](int pos, int& off) {                   // -1 where no position is
+                if (16 * blk >= KT || pos >= pc.len) return -1;
+                const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
+                off = pos - pi * p.page_size;
+                const int page = p.table ? __ldg(p.table + static_cast<long long>(pc.b) * p.table_stride + pi) : pc.b;
+                return page;
+            };
+            int next_off = 0, next_page = page_of(pc.tile0 * KT + 16 * blk, next_off);
+#pragma unroll 1
             for (int i = 0; i < pc.count; ++i, ++tile) {
-                const int slot = tile % F::RAW, pos0 = (pc.tile0 + i) * KT;
-                const int blk = lane >> 2, k = lane & 3, pos = pos0 + 16 * blk;
-                // lane 4 n + k sees to section k of the n-th 16 positions; their page on its way while the slot empties
-                int page = -1, off = 0;
-                const bool there = 16 * blk < KT && pos < pc.len;
-                if (there) {
-                    const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
-                    page = p.table ? __ldg(p.table + static_cast<long long>(pc.b) * p.table_stride + pi) : pc.b;
-                    off = pos - pi * p.page_size;
-                }
-                const bool has = there && page >= 0 && page < p.pages;
+                const int slot = tile % F::RAW, pos0 = (pc.tile0 + i) * KT, pos = pos0 + 16 * blk;
+                const int page = next_page, off = next_off;
+                if (i + 1 < pc.count) next_page = page_of(pos + KT, next_off);
+                const bool there = 16 * blk < KT && pos < pc.len, has = there && page >= 0 && page < p.pages;
                 if (there && !has && k == 0) record_fault(ALJ_FAULT_BOUNDS);
-                if (pos0 + KT > pc.base && seq != pc.b) {         // which nodes are there: those whose ancestors all are
-                    seq = pc.b;
-                    __syncwarp();
-                    for (int t = lane; t < p.q_len; t += 32)
-                        s.par_p[t] = static_cast<short>(tree_parent(p.parents + static_cast<long long>(pc.b) * p.parents_stride, t));
-                    __syncwarp();
-                    for (int w = 0; w < kKv4TreeWords; ++w) {
-                        int t = 32 * w + lane < p.q_len ? 32 * w + lane : -2;
-                        while (t >= 0) t = s.par_p[t];
-                        const uint32_t bits = __ballot_sync(0xffffffffu, t == -1);
-                        if (lane == 0) s.node_ok[w] = bits;
-                    }
-                    __syncwarp();
-                }
-                uint32_t bits = 0u;                               // valid ones of the 16 positions
-                if (has) {
-                    if (pos >= lo && pos + 16 <= pc.base) {
-                        bits = 0xFFFFu;
-                    } else {
-                        for (int n = 0; n < 16; ++n) {
-                            const int node = pos + n - pc.base;
-                            const bool v = pos + n >= lo && (node < 0 || (node < p.q_len && ((s.node_ok[node >> 5] >> (node & 31)) & 1u)));
-                            bits |= static_cast<uint32_t>(v) << n;
+                uint32_t bits = has ? 0xFFFFu : 0u;                   // valid ones of the 16 positions
+                if (pos0 < lo || pos0 + KT > pc.base) {               // at the window's edge, or with the tree's nodes
+                    if (seq != pc.b) {                                // which of them are there: those whose ancestors all are
+                        seq = pc.b;
+                        __syncwarp();
+#pragma unroll 1
+                        for (int t = lane; t < p.q_len; t += 32)
+                            s.par_p[t] = static_cast<short>(tree_parent(p.parents + static_cast<long long>(pc.b) * p.parents_stride, t));
+                        __syncwarp();
+#pragma unroll 1
+                        for (int w = 0; w < kKv4TreeWords; ++w) {
+                            int t = 32 * w + lane < p.q_len ? 32 * w + lane : -2;
+                            while (t >= 0) t = s.par_p[t];
+                            const uint32_t nodes = __ballot_sync(0xffffffffu, t == -1);
+                            if (lane == 0) s.node_ok[w] = nodes;
                         }
+                        __syncwarp();
+                    }
+#pragma unroll 1
+                    for (int n = 0; n < 16; ++n) {
+                        const int node = pos + n - pc.base;
+                        const bool v = pos + n >= lo && (node < 0 || (node < p.q_len && ((s.node_ok[node >> 5] >> (node & 31)) & 1u)));
+                        if (!v) bits &= ~(1u << n);
                     }
                 }
                 const uint32_t upper = __shfl_down_sync(0xffffffffu, bits, 4);
+                const int blocks = __popc(__ballot_sync(0xffffffffu, has)) / 4;
                 if (tile >= F::RAW) ok = ok && warp_wait(s.raw_empty + slot, (tile / F::RAW - 1) & 1, gave_up);
                 if (!ok) break;
                 if ((lane & 7) == 0) s.valid[slot][lane >> 3] = bits | upper << 16;
-                const int blocks = __popc(__ballot_sync(0xffffffffu, has)) / 4;
                 __syncwarp();
                 if (lane == 0) mbar_arrive_expect_tx(s.raw_full + slot, blocks * F::BLOCK_BYTES);
                 __syncwarp();
                 // the blocks that share a page follow one another there: one copy of each section for all of them
                 if (has && (blk == 0 || off == 0)) {
                     const int run = min(min(KT / 16 - blk, (p.page_size - off) / 16), (pc.len - pos + 15) / 16);
-                    uint8_t* dst = smem + F::AT_RAW + slot * F::RAW_BYTES;
-                    const uint8_t* src = p.cache + (static_cast<long long>(page) * p.kv_heads + pc.kvh) * kv4_block_bytes(p.page_size, D);
-                    const int row = k < 2 ? D / 2 : 2 * NG;       // bytes of a position
-                    const int to = k == 0 ? 0 : k == 1 ? F::V_CODES : k == 2 ? F::K_SC : F::V_SC;
-                    const long long section = static_cast<long long>(p.page_size) * (k < 2 ? k * (D / 2) : D + (k - 2) * (2 * NG));
-                    bulk_g2s(dst + to + 16 * blk * row, src + section + static_cast<long long>(off) * row, 16 * run * row, s.raw_full + slot);
+                    const uint8_t* src = p.cache + (static_cast<long long>(page) * p.kv_heads + pc.kvh) * block + section +
+                                         static_cast<long long>(off) * row;
+                    bulk_g2s(smem + F::AT_RAW + slot * F::RAW_BYTES + to, src, 16 * run * row, s.raw_full + slot);
                 }
             }
             if (!ok) break;
