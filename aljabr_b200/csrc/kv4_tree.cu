@@ -45,8 +45,8 @@ namespace alj {
 namespace {
 
 constexpr int kRows = 128;
+constexpr int kPages = 128;           // page ids read from the table at once
 constexpr int kItemCost = 2;          // tiles that an item's start and end are worth
-constexpr int kMeta = 8;              // tiles whose exponents are kept: V of tile t + 5 waits for the products of t + 3
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -3.4e38f;     // running maximum of a row that has seen nothing
 // P <= 2^(kLazy + kSlack + kBias) = 2^15, or its sum over 32 positions <= kMostSum
@@ -59,35 +59,47 @@ struct Shape {
     static constexpr int D = 32 * NG;
     static constexpr int KT = NG == 8 ? 64 : 128;            // positions of a tile
     static constexpr int STREAMS = NG == 8 ? 1 : 2;
-    static constexpr int V_STAGES = NG == 8 ? 1 : 2;
-    static constexpr int RAW = NG == 2 ? 4 : NG == 4 ? 3 : 2;
+    // tiles of scores, of K and of V as fp16, of codes.  Codes take most: they hide the time of the loads.
+    static constexpr int S_STAGES = 2, K_STAGES = 2, V_STAGES = NG == 8 ? 1 : 2, RAW = NG == 2 ? 8 : NG == 4 ? 3 : 2;
+    // tiles whose exponents are kept: those of tile t + META replace t's, and its codes come once V of t + META - RAW is
+    // decoded, for which the products of t + META - RAW - V_STAGES have been done, and t's softmax before them
+    static constexpr int META = NG == 2 ? 16 : 8;
+    static_assert(META >= RAW + V_STAGES, "exponents kept");
     static constexpr int SOFT = 4 * STREAMS;                 // softmax warps
     static constexpr int WARPS = SOFT + 12;
-    // Registers a thread, of the launch's (96 for 5 warpgroups, 128 for 4) that they trade: 5 x 96 = 2 x 128 + 64 + 96 + 64,
-    // 4 x 128 = 192 + 72 + 128 + 120
-    static constexpr int R_SOFT = STREAMS == 2 ? 128 : 192, R_K = STREAMS == 2 ? 64 : 72, R_REST = STREAMS == 2 ? 64 : 120;
-    static constexpr int THREADS = 32 * WARPS;
+    // Registers a thread, of the launch's (96 for 5 warpgroups, 128 for 4) that they trade: 5 x 96 = 2 x 120 + 64 + 96 + 80,
+    // 4 x 128 = 192 + 72 + 128 + 120.  Those who give come down to fewer (to ask for more there is an illegal instruction),
+    // those who take wait for no more than is given, V stays as it is.
+    static constexpr int R_SOFT = STREAMS == 2 ? 120 : 192, R_K = STREAMS == 2 ? 64 : 72, R_REST = STREAMS == 2 ? 80 : 120;
+    static constexpr int THREADS = 32 * WARPS, R_LAUNCH = 65536 / THREADS / 8 * 8;
+    static_assert(R_SOFT > R_LAUNCH && R_K < R_LAUNCH && R_REST < R_LAUNCH &&
+                      STREAMS * R_SOFT + R_K + R_LAUNCH + R_REST <= WARPS / 4 * R_LAUNCH, "registers that the warpgroups trade");
     // a raw tile: K codes, V codes, K scales, V scales, each by position
     static constexpr int V_CODES = KT * D / 2, K_SC = 2 * V_CODES, V_SC = K_SC + KT * 2 * NG, RAW_BYTES = V_SC + KT * 2 * NG;
     static constexpr int BLOCK_BYTES = 16 * (D + D / 8);     // copied for 16 positions
     static constexpr int KHAT = KT * D * 2, VHAT = KT * D * 2, Q = kRows * D * 2;
-    static constexpr int AT_K = Q, AT_V = AT_K + 2 * KHAT, AT_RAW = AT_V + V_STAGES * VHAT, AT_SMALL = AT_RAW + RAW * RAW_BYTES;
-    static constexpr int O_COL = NG == 8 ? 128 : 256;        // tensor memory: S of two tiles, then O of each stream
+    static constexpr int AT_K = Q, AT_V = AT_K + K_STAGES * KHAT, AT_RAW = AT_V + V_STAGES * VHAT, AT_SMALL = AT_RAW + RAW * RAW_BYTES;
+    static constexpr int O_COL = S_STAGES * KT;              // tensor memory: S of the tiles, then O of each stream
+    static_assert(O_COL + STREAMS * D <= 512, "tensor memory");
 };
 
+template <int NG>
 struct Small {                        // behind the tiles in shared memory
-    uint64_t raw_full[4], raw_empty[4], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], q_full, done;
+    using F = Shape<NG>;
+    static constexpr int kMeta = F::META;
+    uint64_t raw_full[F::RAW], raw_empty[F::RAW], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], q_full, done;
     uint64_t meta_full[kMeta];
     int abort, tmem;
-    uint32_t valid[4][4];             // by raw slot: bits of the positions that some row may see
+    uint32_t valid[F::RAW][4];           // by raw slot: bits of the positions that some row may see
     float k_unit[kMeta][4];           // by tile and 32 positions: 2^e of K, e of V, the largest of those,
     int ev[kMeta][4];
     int e_top[kMeta];
     int nan_any[kMeta];               // and V groups that are NaN: bits by position
-    uint8_t nan[kMeta][128];
+    uint8_t nan[kMeta][F::KT];
     int sum[32];                      // prefix sums, and where this CTA starts
     int start[4];
     uint32_t node_ok[kKv4TreeWords];  // the producer's
+    int pages[kPages];
     short par_p[kKv4MaxNodes];
     short par[kKv4MaxNodes];            // the softmax warps'
     uint32_t see[kKv4TreeWords][kRows];
@@ -98,7 +110,7 @@ struct Small {                        // behind the tiles in shared memory
 };
 
 template <int NG>
-constexpr int smem_bytes() { return 1024 + Shape<NG>::AT_SMALL + static_cast<int>(sizeof(Small)); }
+constexpr int smem_bytes() { return 1024 + Shape<NG>::AT_SMALL + static_cast<int>(sizeof(Small<NG>)); }
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -156,6 +168,11 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
 }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
     return __all_sync(0xffffffffu, wait_bar(bar, parity, gave_up));
+}
+__device__ __forceinline__ void bulk_to(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
 }
 __device__ __forceinline__ void fence_proxy_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -350,21 +367,26 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
     constexpr int D = F::D, KT = F::KT;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    Small& s = *reinterpret_cast<Small*>(smem + F::AT_SMALL);
+    Small<NG>& s = *reinterpret_cast<Small<NG>*>(smem + F::AT_SMALL);
+    constexpr int kMeta = F::META;
     volatile int* const gave_up = &s.abort;
     auto token_of = [&](int row) { return static_cast<int>((static_cast<unsigned int>(row) * p.group_magic) >> 21); };   // row / group
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < F::RAW; ++i) {
             mbar_init(s.raw_full + i, 1);
             mbar_init(s.raw_empty + i, 10);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < F::K_STAGES; ++i) {
             mbar_init(s.k_full + i, 4);
             mbar_init(s.k_empty + i, 1);
+        }
+        for (int i = 0; i < F::V_STAGES; ++i) {
             mbar_init(s.v_full + i, 4);
             mbar_init(s.v_empty + i, 1);
+        }
+        for (int i = 0; i < F::S_STAGES; ++i) {
             mbar_init(s.s_full + i, 1);
             mbar_init(s.p_full + i, 4);
             mbar_init(s.pv_done + i, 1);
@@ -474,7 +496,6 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         const float size = fabsf(p.scale) * (p.soft_cap > 0.0f ? 1.0f : kLog2e);
         auto sync = [&] { named_bar(1, 32 * F::SOFT); };
         int tiles = 0;                // of this CTA before the piece
-        int uses0 = 0, uses1 = 0;     // uses of the two S buffers before the piece
         int pre = my_pre, seq = line.b;
         while (next_piece<KT>(line, p, items, pc)) {
             if (pc.b != seq) {        // the line's places before sequence pc.b
@@ -584,9 +605,10 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 return bits;
             };
             // -------------------------------------------------- its tiles
-            for (int i = stream; i < pc.count; i += F::STREAMS) {
-                const int buf = i & 1, use = (buf ? uses1 : uses0) + (i >> 1), tile = tiles + i;
-                const int meta = tile & (kMeta - 1), pos = (pc.tile0 + i) * KT;
+            int last = -1;            // the stream's last tile
+            for (int tile = tiles + (F::STREAMS == 2 ? (tiles ^ stream) & 1 : 0); tile < tiles + pc.count; last = tile, tile += F::STREAMS) {
+                const int buf = tile % F::S_STAGES, use = tile / F::S_STAGES;
+                const int meta = tile & (kMeta - 1), pos = (pc.tile0 + tile - tiles) * KT;
                 const uint32_t ts = tq + buf * KT, to = tq + F::O_COL + (F::STREAMS == 2 ? stream * D : 0);
                 ok = ok && warp_wait(s.s_full + buf, use & 1, gave_up);
                 ok = ok && warp_wait(s.meta_full + meta, (tile / kMeta) & 1, gave_up);
@@ -595,9 +617,8 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                     const bool edge = pos < all_lo || pos + KT > pc.base;
                     // O summed up so far times g
                     auto rescale = [&](float g) {
-                        if (i < F::STREAMS) return;
-                        const int last = i - F::STREAMS, pb = last & 1;
-                        ok = ok && warp_wait(s.pv_done + pb, ((pb ? uses1 : uses0) + (last >> 1)) & 1, gave_up);
+                        if (last < 0) return;
+                        ok = ok && warp_wait(s.pv_done + last % F::S_STAGES, (last / F::S_STAGES) & 1, gave_up);
                         tcg::tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < 4 * NG; ++c) {
@@ -706,31 +727,30 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 if (lane == 0) mbar_arrive(s.p_full + buf);
             }
             // -------------------------------------------------- the streams' results, and the rows' outputs
-            const int n0 = (pc.count + 1) >> 1, n1 = pc.count >> 1;   // uses of the buffers
-            if (n0 > 0) ok = ok && warp_wait(s.pv_done, (uses0 + n0 - 1) & 1, gave_up);
-            if (n1 > 0) ok = ok && warp_wait(s.pv_done + 1, (uses1 + n1 - 1) & 1, gave_up);
+            // (The stream's own last products: S of that tile has been seen, so the use of its buffer before is behind us.)
+            if (last >= 0) ok = ok && warp_wait(s.pv_done + last % F::S_STAGES, (last / F::S_STAGES) & 1, gave_up);
             s.ml[stream][row][0] = M;
             s.ml[stream][row][1] = l;
             s.er[stream][row] = static_cast<short>(E);
             s.row_nan[stream][row] = static_cast<uint8_t>(nan_groups);
             sync();
             tcg::tc_fence_after();
-            uses0 += n0;
-            uses1 += n1;
+            // which streams had a tile
+            const bool has0 = pc.count > 0 && (F::STREAMS == 1 || pc.count > 1 || (tiles & 1) == 0);
+            const bool has1 = F::STREAMS == 2 && (pc.count > 1 || (pc.count == 1 && (tiles & 1) == 1));
             tiles += pc.count;
             const int i = pc.row0 + row;
-            const bool two = F::STREAMS == 2 && pc.count > 1;
             float w0 = 0.0f, w1 = 0.0f, L = 0.0f, top = kNone;
             int gone = 0;
             if (alive && pc.count > 0) {
-                const float m0 = s.ml[0][row][0], m1 = two ? s.ml[1][row][0] : kNone;
+                const float m0 = has0 ? s.ml[0][row][0] : kNone, m1 = has1 ? s.ml[1][row][0] : kNone;
                 top = fmaxf(m0, m1);
-                w0 = ex2(m0 - top);
-                w1 = two ? ex2(m1 - top) : 0.0f;
-                L = s.ml[0][row][1] * w0 + (two ? s.ml[1][row][1] * w1 : 0.0f);
-                w0 *= pow2i(max(-126, s.er[0][row] - kBias));
-                if (two) w1 *= pow2i(max(-126, s.er[1][row] - kBias));
-                gone = s.row_nan[0][row] | (two ? s.row_nan[1][row] : 0);
+                w0 = has0 ? ex2(m0 - top) : 0.0f;
+                w1 = has1 ? ex2(m1 - top) : 0.0f;
+                L = (has0 ? s.ml[0][row][1] * w0 : 0.0f) + (has1 ? s.ml[1][row][1] * w1 : 0.0f);
+                if (has0) w0 *= pow2i(max(-126, s.er[0][row] - kBias));
+                if (has1) w1 *= pow2i(max(-126, s.er[1][row] - kBias));
+                gone = (has0 ? s.row_nan[0][row] : 0) | (has1 ? s.row_nan[1][row] : 0);
             }
             int slot = 0;
             if (!whole) {
@@ -749,12 +769,12 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 for (int d = stream * kCols; d < (stream + 1) * kCols; d += 8) {
                     float o[8] = {};
                     uint32_t v[8];
-                    if (pc.count > 0) {
+                    if (has0) {
                         tmem_ld8(tq + F::O_COL + d, v);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[k]) * w0;
                     }
-                    if (two) {
+                    if (has1) {
                         tmem_ld8(tq + F::O_COL + D + d, v);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) o[k] = fmaf(__uint_as_float(v[k]), w1, o[k]);
@@ -788,16 +808,16 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
     } else if (warp < F::SOFT + 4) {
         // ------------------------------------------------------ K to fp16
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::R_K));
-        constexpr int GW = NG == 8 ? 4 : NG;                      // groups of a warp
+        constexpr int GW = KT == 128 ? NG : NG / 2;               // groups of a warp
         const int kw = warp - F::SOFT, span = KT == 128 ? kw : kw & 1, half = KT == 128 ? 0 : kw >> 1;
         const int c = lane & 3, pos_in = (lane >> 3) + (lane & 4);
         int tile = 0;
         while (next_piece<KT>(line, p, items, pc)) {
             for (int i = 0; i < pc.count; ++i, ++tile) {
-                const int slot = tile % F::RAW, ks = tile & 1;
+                const int slot = tile % F::RAW, ks = tile % F::K_STAGES;
                 ok = ok && warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
                 ok = ok && warp_wait(s.meta_full + (tile & (kMeta - 1)), (tile / kMeta) & 1, gave_up);
-                if (tile >= 2) ok = ok && warp_wait(s.k_empty + ks, ((tile >> 1) - 1) & 1, gave_up);
+                if (tile >= F::K_STAGES) ok = ok && warp_wait(s.k_empty + ks, (tile / F::K_STAGES - 1) & 1, gave_up);
                 if (!ok) break;
                 const uint32_t raw = at_raw + slot * F::RAW_BYTES;
                 const uint32_t to = at_k + ks * F::KHAT;
@@ -805,13 +825,13 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 for (int it = 0; it < 4; ++it) {
                     const int r = 32 * span + 8 * it + pos_in;
                     uint32_t w[GW], d[GW / 2];
-                    lds_words<GW>(raw + r * (D / 2) + c * (4 * NG) + half * 16, w);
-                    lds_words<GW / 2>(raw + F::K_SC + r * (2 * NG) + half * 8, d);
+                    lds_words<GW>(raw + r * (D / 2) + c * (4 * NG) + half * (4 * GW), w);
+                    lds_words<GW / 2>(raw + F::K_SC + r * (2 * NG) + half * (2 * GW), d);
 #pragma unroll
                     for (int g = 0; g < GW; ++g) {
                         uint32_t out[4];
                         decode8(w[g], bits_h2(__byte_perm(d[g / 2], 0u, g & 1 ? 0x3232 : 0x1010)), out);
-                        const int j = 4 * (4 * half + g) + c;
+                        const int j = 4 * (GW * half + g) + c;
                         sts128(to + (j >> 3) * (KT * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4), make_uint4(out[0], out[1], out[2], out[3]));
                     }
                 }
@@ -825,7 +845,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             if (!ok) break;
         }
     } else if (warp < F::SOFT + 8) {
-        // ------------------------------------------------------ V to fp16, transposed (at the launch's registers)
+        // ------------------------------------------------------ V to fp16, transposed
         // A thread has 8 positions, block j of 64, and a word (8 codes: 4 dims of groups g and g + 1) a pass.  Lanes read
         // different words, those that would meet on a bank the other position of a pair first; eight lanes that store
         // together have eight different j, so that their 16-byte pieces lie in different banks under the swizzle.
@@ -888,31 +908,40 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::R_REST));
     if (warp == F::SOFT + 8) {
         // ------------------------------------------------------ codes and scales from the cache
-        // Lane 4 n + k sees to section k of the n-th 16 positions of a tile.  Page ids are asked for a tile ahead: they are
-        // all that the copies' addresses wait for.
+        // Lane 4 n + k sees to section k of the n-th 16 positions of a tile.  Page ids come through shared memory, kPages at a
+        // time: a load from the table for every tile would take as long as the tile's products.
         int tile = 0, seq = -1;
         const int blk = lane >> 2, k = lane & 3;
         const int row = k < 2 ? D / 2 : 2 * NG;                       // bytes of a position in the section
-        const int to = (k == 0 ? 0 : k == 1 ? F::V_CODES : k == 2 ? F::K_SC : F::V_SC) + 16 * blk * row;
+        const uint32_t to = at_raw + (k == 0 ? 0 : k == 1 ? F::V_CODES : k == 2 ? F::K_SC : F::V_SC) + 16 * blk * row;
         const long long section = static_cast<long long>(p.page_size) * (k < 2 ? k * (D / 2) : D + (k - 2) * (2 * NG));
         const long long block = kv4_block_bytes(p.page_size, D);
         while (next_piece<KT>(line, p, items, pc)) {
             const int lo = window_start(p, pc.base + 1);
-            auto page_of = [&](int pos, int& off) {                   // -1 where no position is
-                if (16 * blk >= KT || pos >= pc.len) return -1;
-                const int pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
-                off = pos - pi * p.page_size;
-                const int page = p.table ? __ldg(p.table + static_cast<long long>(pc.b) * p.table_stride + pi) : pc.b;
-                return page;
-            };
-            int next_off = 0, next_page = page_of(pc.tile0 * KT + 16 * blk, next_off);
+            int pos = pc.tile0 * KT + 16 * blk, pi = pos / p.page_size, off = pos - pi * p.page_size;
+            int first = 0, last = -1;                                 // pages at hand
+            const uint8_t* const head = p.cache + static_cast<long long>(pc.kvh) * block + section;
 #pragma unroll 1
             for (int i = 0; i < pc.count; ++i, ++tile) {
-                const int slot = tile % F::RAW, pos0 = (pc.tile0 + i) * KT, pos = pos0 + 16 * blk;
-                const int page = next_page, off = next_off;
-                if (i + 1 < pc.count) next_page = page_of(pos + KT, next_off);
-                const bool there = 16 * blk < KT && pos < pc.len, has = there && page >= 0 && page < p.pages;
-                if (there && !has && k == 0) record_fault(ALJ_FAULT_BOUNDS);
+                const int slot = tile % F::RAW, pos0 = (pc.tile0 + i) * KT;
+                const bool there = 16 * blk < KT && pos < pc.len;
+                if (__any_sync(0xffffffffu, there && pi > last)) {
+                    first = __shfl_sync(0xffffffffu, pi, 0);
+                    last = first + kPages - 1;
+                    const int end = (pc.len - 1) / p.page_size;
+                    __syncwarp();
+#pragma unroll 1
+                    for (int n = lane; n < kPages && first + n <= end; n += 32) {
+                        const int page = p.table ? __ldg(p.table + static_cast<long long>(pc.b) * p.table_stride + first + n) : pc.b;
+                        const bool bad = page < 0 || page >= p.pages;
+                        if (bad) record_fault(ALJ_FAULT_BOUNDS);
+                        s.pages[n] = bad ? -1 : page;
+                    }
+                    __syncwarp();
+                }
+                const int page = there ? s.pages[pi - first] : -1;
+                const bool has = page >= 0;
+                const uint32_t any = __ballot_sync(0xffffffffu, has);
                 uint32_t bits = has ? 0xFFFFu : 0u;                   // valid ones of the 16 positions
                 if (pos0 < lo || pos0 + KT > pc.base) {               // at the window's edge, or with the tree's nodes
                     if (seq != pc.b) {                                // which of them are there: those whose ancestors all are
@@ -938,20 +967,22 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                         if (!v) bits &= ~(1u << n);
                     }
                 }
-                const uint32_t upper = __shfl_down_sync(0xffffffffu, bits, 4);
-                const int blocks = __popc(__ballot_sync(0xffffffffu, has)) / 4;
+                bits |= __shfl_down_sync(0xffffffffu, bits, 4) << 16;
+                // the blocks that share a page follow one another there: one copy of each section for all of them
+                const uint8_t* const src = head + static_cast<long long>(page) * p.kv_heads * block + static_cast<long long>(off) * row;
+                const int run = min(min(KT / 16 - blk, (p.page_size - off) >> 4), (pc.len - pos + 15) >> 4);
                 if (tile >= F::RAW) ok = ok && warp_wait(s.raw_empty + slot, (tile / F::RAW - 1) & 1, gave_up);
                 if (!ok) break;
-                if ((lane & 7) == 0) s.valid[slot][lane >> 3] = bits | upper << 16;
+                if ((lane & 7) == 0) s.valid[slot][lane >> 3] = bits;
                 __syncwarp();
-                if (lane == 0) mbar_arrive_expect_tx(s.raw_full + slot, blocks * F::BLOCK_BYTES);
+                if (lane == 0) mbar_arrive_expect_tx(s.raw_full + slot, (__popc(any) >> 2) * F::BLOCK_BYTES);
                 __syncwarp();
-                // the blocks that share a page follow one another there: one copy of each section for all of them
-                if (has && (blk == 0 || off == 0)) {
-                    const int run = min(min(KT / 16 - blk, (p.page_size - off) / 16), (pc.len - pos + 15) / 16);
-                    const uint8_t* src = p.cache + (static_cast<long long>(page) * p.kv_heads + pc.kvh) * block + section +
-                                         static_cast<long long>(off) * row;
-                    bulk_g2s(smem + F::AT_RAW + slot * F::RAW_BYTES + to, src, 16 * run * row, s.raw_full + slot);
+                if (has && (blk == 0 || off == 0)) bulk_to(to + slot * F::RAW_BYTES, src, 16 * run * row, s.raw_full + slot);
+                pos += KT;
+                off += KT;
+                while (off >= p.page_size) {
+                    off -= p.page_size;
+                    ++pi;
                 }
             }
             if (!ok) break;
@@ -1024,30 +1055,29 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         const uint32_t one = elect_one();
         // descriptors count 16-byte units: 2 for 16 values of K, an atom of 64 for its rows' 128 bytes
         const uint64_t q_desc = tcg::sdesc(at_q), k_desc = tcg::sdesc(at_k), v_desc = tcg::sdesc(at_v);
-        int tile = 0, pieces = 0, uses0 = 0, uses1 = 0;
+        int tile = 0, pieces = 0;
         while (ok && next_piece<KT>(line, p, items, pc)) {
             if (pc.count == 0) continue;
             ok = ok && warp_wait(&s.q_full, pieces & 1, gave_up);
             ++pieces;
 #pragma unroll 1
-            for (int i = -2; ok && i < pc.count; ++i) {               // O of tile i, then S of tile i + 2
-                const int buf = i & 1;
+            for (int i = -F::S_STAGES; ok && i < pc.count; ++i) {     // O of tile i, then S of tile i + S_STAGES
                 if (i >= 0) {
-                    const int t = tile + i, vs = t % F::V_STAGES, use = (buf ? uses1 : uses0) + (i >> 1);
+                    const int t = tile + i, vs = t % F::V_STAGES, buf = t % F::S_STAGES;
                     ok = ok && warp_wait(s.v_full + vs, (t / F::V_STAGES) & 1, gave_up);
-                    ok = ok && warp_wait(s.p_full + buf, use & 1, gave_up);
+                    ok = ok && warp_wait(s.p_full + buf, (t / F::S_STAGES) & 1, gave_up);
                     if (!ok) break;
                     tcg::tc_fence_after();
-                    const uint32_t to = tmem + F::O_COL + (F::STREAMS == 2 ? buf * D : 0);
+                    const uint32_t to = tmem + F::O_COL + (F::STREAMS == 2 ? (t & 1) * D : 0);
                     const uint64_t v = v_desc + vs * (F::VHAT >> 4);
 #pragma unroll
                     for (int h = 0; h < KT / 64; ++h)
                         mma64_ts(to, tmem + buf * KT + 32 * h, v + h * (D * 8), kO, h > 0 || i >= F::STREAMS, one);
                     commit2(s.v_empty + vs, s.pv_done + buf, one);
                 }
-                if (i + 2 < pc.count) {
-                    const int t = tile + i + 2, ks = t & 1;
-                    ok = ok && warp_wait(s.k_full + ks, (t >> 1) & 1, gave_up);
+                if (i + F::S_STAGES < pc.count) {
+                    const int t = tile + i + F::S_STAGES, ks = t % F::K_STAGES, buf = t % F::S_STAGES;
+                    ok = ok && warp_wait(s.k_full + ks, (t / F::K_STAGES) & 1, gave_up);
                     if (!ok) break;
                     tcg::tc_fence_after();
                     const uint64_t k_at = k_desc + ks * (F::KHAT >> 4);
@@ -1057,8 +1087,6 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                     commit2(s.k_empty + ks, s.s_full + buf, one);
                 }
             }
-            uses0 += (pc.count + 1) >> 1;
-            uses1 += pc.count >> 1;
             tile += pc.count;
         }
         if (one) {
