@@ -194,6 +194,21 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
                  :
                  : "memory");
 }
+// 16 columns asked for, and there: until then nothing may use the registers.
+__device__ __forceinline__ void tmem_ask16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_have(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
@@ -634,53 +649,71 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                         rescale(pow2i(max(E - e_new, -126)));
                         E = e_new;
                     }
-                    const bool plain = !edge && p.soft_cap == 0.0f;
+                    int c = 0;
+                    if (!edge && p.soft_cap == 0.0f) {
+                        // Without masks and without the maximum: P may pass 1, and the sum of 32 says whether it stays in
+                        // fp16's range.  Where it does not, or M is so large that its rounding counts, the rest of the tile
+                        // goes the long way.  16 columns are on their way while 16 are used.
+                        uint32_t v[16], w[16];
+                        tmem_ask16(ts, v);
 #pragma unroll 1
-                    for (int c = 0; c < KT / 32; ++c) {
-                        const float fc = fac * s.k_unit[meta][c];
-                        const int sh = kBias + s.ev[meta][c] - E;
-                        if (plain) {
-                            // Without the maximum: P may pass 1, and the sum of 32 says whether it stays in fp16's range.
-                            // Where it does not, or M is so large that its rounding counts, the chunk goes the long way.
-                            uint32_t v[32];
-                            tmem_ld32(ts + 32 * c, v);
-                            const float at = static_cast<float>(sh) - M;
+                        for (; c < KT / 32; ++c) {
+                            const int sh = kBias + s.ev[meta][c] - E;
+                            const float fc = fac * s.k_unit[meta][c], at = static_cast<float>(sh) - M;
                             const f2 fc2 = mk2(fc, fc), at2 = mk2(at, at);
                             f2 sum0 = mk2(0.0f, 0.0f), sum1 = sum0;
                             uint32_t out[16];
+                            auto half = [&](const uint32_t (&x)[16], int to) {
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) {
-                                const f2 y = fma2(mk2u(v[2 * k], v[2 * k + 1]), fc2, at2);
-                                const float a = ex2(lo(y)), b = ex2(hi(y));
-                                if (k & 1) sum1 = add2(sum1, mk2(a, b));
-                                else sum0 = add2(sum0, mk2(a, b));
-                                out[k] = h2_bits(__floats2half2_rn(a, b));
-                            }
+                                for (int k = 0; k < 8; ++k) {
+                                    const f2 y = fma2(mk2u(x[2 * k], x[2 * k + 1]), fc2, at2);
+                                    const float a = ex2(lo(y)), b = ex2(hi(y));
+                                    if (k & 1) sum1 = add2(sum1, mk2(a, b));
+                                    else sum0 = add2(sum0, mk2(a, b));
+                                    out[to + k] = h2_bits(__floats2half2_rn(a, b));
+                                }
+                            };
+                            tmem_have(v);
+                            tmem_ask16(ts + 32 * c + 16, w);
+                            half(v, 0);
+                            tmem_have(w);
+                            if (c + 1 < KT / 32) tmem_ask16(ts + 32 * c + 32, v);
+                            half(w, 8);
                             const f2 sums = add2(sum0, sum1);
                             const float sum = lo(sums) + hi(sums);
-                            if (!__any_sync(0xffffffffu, sum > kMostSum || fabsf(M) > kMostM)) {
-                                l = fmaf(sum, pow2i(-sh), l);
-                                tmem_st16(ts + 16 * c, out);          // columns that this lane has read
-                                continue;
-                            }
+                            if (__any_sync(0xffffffffu, sum > kMostSum || fabsf(M) > kMostM)) break;
+                            l = fmaf(sum, pow2i(-sh), l);
+                            tmem_st16(ts + 16 * c, out);              // columns that this lane has read
                         }
-                        const uint32_t bits = edge ? visible(pos + 32 * c) : 0xFFFFFFFFu;
-                        float mx = -INFINITY;
+                        tmem_have(v);
+                    }
 #pragma unroll 1
-                        for (int b = 0; b < 4; ++b) {                 // S becomes the scaled, capped and masked score
-                            uint32_t v[8];
-                            tmem_ld8(ts + 32 * c + 8 * b, v);
+                    for (; c < KT / 32; ++c) {
+                        const uint32_t bits = edge ? visible(pos + 32 * c) : 0xFFFFFFFFu;
+                        const int sh = kBias + s.ev[meta][c] - E;
+                        float fc = fac * s.k_unit[meta][c];
+                        if (p.soft_cap > 0.0f) {
+#pragma unroll 1
+                            for (int b = 0; b < 4; ++b) {             // S becomes the capped score
+                                uint32_t v[8];
+                                tmem_ld8(ts + 32 * c + 8 * b, v);
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) {
-                                float y = __uint_as_float(v[k]) * fc;
-                                if (p.soft_cap > 0.0f) y = tanhf(y * inv_cap) * (p.soft_cap * kLog2e);
-                                y = (bits >> (8 * b + k)) & 1u ? y : -INFINITY;
-                                mx = fmaxf(mx, y);
-                                v[k] = __float_as_uint(y);
+                                for (int k = 0; k < 8; ++k) v[k] = __float_as_uint(tanhf(__uint_as_float(v[k]) * fc * inv_cap) * (p.soft_cap * kLog2e));
+                                tmem_st8(ts + 32 * c + 8 * b, v);
                             }
-                            tmem_st8(ts + 32 * c + 8 * b, v);
+                            tcg::tmem_wait_st();
+                            fc = 1.0f;
                         }
-                        tcg::tmem_wait_st();
+                        uint32_t v[32];
+                        tmem_ld32(ts + 32 * c, v);
+                        float m[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            const float y = (bits >> k) & 1u ? __uint_as_float(v[k]) * fc : -INFINITY;
+                            m[k & 1] = fmaxf(m[k & 1], y);
+                            v[k] = __float_as_uint(y);
+                        }
+                        const float mx = fmaxf(m[0], m[1]);
                         if (__any_sync(0xffffffffu, mx > M + kLazy)) {
                             // M becomes the next integer above the score, so that what is there already, the P of the chunks
                             // before c too, is scaled by a power of two
@@ -691,28 +724,24 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                             const __half2 f2 = __float2half2_rn(f);
 #pragma unroll 1
                             for (int b = 0; b < 2 * c; ++b) {
-                                uint32_t v[8];
-                                tmem_ld8(ts + 8 * b, v);
+                                uint32_t x[8];
+                                tmem_ld8(ts + 8 * b, x);
 #pragma unroll
-                                for (int k = 0; k < 8; ++k) v[k] = h2_bits(__hmul2(bits_h2(v[k]), f2));
-                                tmem_st8(ts + 8 * b, v);
+                                for (int k = 0; k < 8; ++k) x[k] = h2_bits(__hmul2(bits_h2(x[k]), f2));
+                                tmem_st8(ts + 8 * b, x);
                             }
                         }
                         const float at = static_cast<float>(sh) - M;
-                        float sum = 0.0f;
-#pragma unroll 1
-                        for (int b = 0; b < 4; ++b) {
-                            uint32_t v[8], out[4];
-                            tmem_ld8(ts + 32 * c + 8 * b, v);
+                        float sum[2] = {};
+                        uint32_t out[16];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const float a = ex2(__uint_as_float(v[2 * k]) + at), d = ex2(__uint_as_float(v[2 * k + 1]) + at);
-                                sum += a + d;
-                                out[k] = h2_bits(__floats2half2_rn(a, d));
-                            }
-                            tmem_st4(ts + 16 * c + 4 * b, out);
+                        for (int k = 0; k < 16; ++k) {
+                            const float a = ex2(__uint_as_float(v[2 * k]) + at), b = ex2(__uint_as_float(v[2 * k + 1]) + at);
+                            sum[k & 1] += a + b;
+                            out[k] = h2_bits(__floats2half2_rn(a, b));
                         }
-                        l = fmaf(sum, pow2i(-sh), l);
+                        l = fmaf(sum[0] + sum[1], pow2i(-sh), l);
+                        tmem_st16(ts + 16 * c, out);
                     }
                     if (s.nan_any[meta]) {
                         for (int k = 0; k < KT; ++k) {
