@@ -28,7 +28,7 @@
 //
 // Roles (one CTA an SM, persistent over the line of chunks as in
 // kv4_attention.cu): a producer warp (bulk copies of a tile's codes and scales
-// into a ring), two that find the exponents e, 4 that decode K, 4 that decode V,
+// into a ring), two that find the exponents e, two warpgroups that decode, a tile each in turn,
 // one that issues the MMAs, and a warpgroup of softmax for each of two streams: the even and the odd
 // tiles of an item have their own S, running maximum and O, so that one stream's
 // softmax runs beside the other's products.  (D 256: tiles of 64, one stream, as
@@ -67,13 +67,13 @@ struct Shape {
     static_assert(META >= RAW + V_STAGES, "exponents kept");
     static constexpr int SOFT = 4 * STREAMS;                 // softmax warps
     static constexpr int WARPS = SOFT + 12;
-    // Registers a thread, of the launch's (96 for 5 warpgroups, 128 for 4) that they trade: 5 x 96 = 2 x 120 + 64 + 96 + 80,
-    // 4 x 128 = 192 + 72 + 128 + 120.  Those who give come down to fewer (to ask for more there is an illegal instruction),
-    // those who take wait for no more than is given, V stays as it is.
-    static constexpr int R_SOFT = STREAMS == 2 ? 120 : 192, R_K = STREAMS == 2 ? 64 : 72, R_REST = STREAMS == 2 ? 80 : 120;
+    // Registers a thread, of the launch's (96 for 5 warpgroups, 128 for 4) that they trade: 5 x 96 = 2 x 128 + 2 x 72 + 80,
+    // 4 x 128 = 192 + 3 x 104.  Those who give come down to fewer (to ask for more there is an illegal instruction),
+    // those who take wait for no more than is given.
+    static constexpr int R_SOFT = STREAMS == 2 ? 128 : 192, R_DECODE = STREAMS == 2 ? 72 : 104, R_REST = STREAMS == 2 ? 80 : 104;
     static constexpr int THREADS = 32 * WARPS, R_LAUNCH = 65536 / THREADS / 8 * 8;
-    static_assert(R_SOFT > R_LAUNCH && R_K < R_LAUNCH && R_REST < R_LAUNCH &&
-                      STREAMS * R_SOFT + R_K + R_LAUNCH + R_REST <= WARPS / 4 * R_LAUNCH, "registers that the warpgroups trade");
+    static_assert(R_SOFT > R_LAUNCH && R_DECODE < R_LAUNCH && R_REST < R_LAUNCH &&
+                      STREAMS * R_SOFT + 2 * R_DECODE + R_REST <= WARPS / 4 * R_LAUNCH, "registers that the warpgroups trade");
     // a raw tile: K codes, V codes, K scales, V scales, each by position
     static constexpr int V_CODES = KT * D / 2, K_SC = 2 * V_CODES, V_SC = K_SC + KT * 2 * NG, RAW_BYTES = V_SC + KT * 2 * NG;
     static constexpr int BLOCK_BYTES = 16 * (D + D / 8);     // copied for 16 positions
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
     if (threadIdx.x == 0) {
         for (int i = 0; i < F::RAW; ++i) {
             mbar_init(s.raw_full + i, 1);
-            mbar_init(s.raw_empty + i, 10);
+            mbar_init(s.raw_empty + i, 6);
         }
         for (int i = 0; i < F::K_STAGES; ++i) {
             mbar_init(s.k_full + i, 4);
@@ -834,22 +834,34 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             tcg::tc_fence_before();
             sync();                                               // tensor memory and the tables are read
         }
-    } else if (warp < F::SOFT + 4) {
-        // ------------------------------------------------------ K to fp16
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::R_K));
-        constexpr int GW = KT == 128 ? NG : NG / 2;               // groups of a warp
-        const int kw = warp - F::SOFT, span = KT == 128 ? kw : kw & 1, half = KT == 128 ? 0 : kw >> 1;
+    } else if (warp < F::SOFT + 8) {
+        // ------------------------------------------------------ K, then V, to fp16: a warpgroup every second tile
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::R_DECODE));
+        const int turn = (warp - F::SOFT) >> 2;
+        constexpr int GW = KT == 128 ? NG : NG / 2;               // K: groups of a warp
+        const int kw = warp & 3, span = KT == 128 ? kw : kw & 1, half = KT == 128 ? 0 : kw >> 1;
         const int c = lane & 3, pos_in = (lane >> 3) + (lane & 4);
+        // V: a thread has 8 positions, block j of 64, and a word (8 codes: 4 dims of groups g and g + 1) a pass.  Lanes read
+        // different words, those that would meet on a bank the other position of a pair first; eight lanes that store
+        // together have eight different j, so that their 16-byte pieces lie in different banks under the swizzle.
+        constexpr int kPasses = NG == 2 ? 1 : 2;
+        const int vw = warp & 3;
+        const int word = NG == 8   ? (lane & 3) | (lane & 24) >> 1 | (lane & 4) << 2
+                         : NG == 4 ? lane & 15
+                                   : lane & 7;
+        const int part = KT == 128 ? lane >> 4 : 0, flip = NG == 8 ? 0 : lane >> 4;
+        const int hw0 = 2 * word;
         int tile = 0;
         while (next_piece<KT>(line, p, items, pc)) {
             for (int i = 0; i < pc.count; ++i, ++tile) {
-                const int slot = tile % F::RAW, ks = tile % F::K_STAGES;
-                ok = ok && warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
+                if ((tile & 1) != turn) continue;
+                const int slot = tile % F::RAW, ks = tile % F::K_STAGES, vs = tile % F::V_STAGES;
+                // the exponents are found after the codes have arrived
                 ok = ok && warp_wait(s.meta_full + (tile & (kMeta - 1)), (tile / kMeta) & 1, gave_up);
                 if (tile >= F::K_STAGES) ok = ok && warp_wait(s.k_empty + ks, (tile / F::K_STAGES - 1) & 1, gave_up);
                 if (!ok) break;
                 const uint32_t raw = at_raw + slot * F::RAW_BYTES;
-                const uint32_t to = at_k + ks * F::KHAT;
+                const uint32_t k_to = at_k + ks * F::KHAT;
 #pragma unroll 2
                 for (int it = 0; it < 4; ++it) {
                     const int r = 32 * span + 8 * it + pos_in;
@@ -861,39 +873,16 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                         uint32_t out[4];
                         decode8(w[g], bits_h2(__byte_perm(d[g / 2], 0u, g & 1 ? 0x3232 : 0x1010)), out);
                         const int j = 4 * (GW * half + g) + c;
-                        sts128(to + (j >> 3) * (KT * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4), make_uint4(out[0], out[1], out[2], out[3]));
+                        sts128(k_to + (j >> 3) * (KT * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4), make_uint4(out[0], out[1], out[2], out[3]));
                     }
                 }
                 fence_proxy_shared();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(s.k_full + ks);
-                    mbar_arrive(s.raw_empty + slot);
-                }
-            }
-            if (!ok) break;
-        }
-    } else if (warp < F::SOFT + 8) {
-        // ------------------------------------------------------ V to fp16, transposed
-        // A thread has 8 positions, block j of 64, and a word (8 codes: 4 dims of groups g and g + 1) a pass.  Lanes read
-        // different words, those that would meet on a bank the other position of a pair first; eight lanes that store
-        // together have eight different j, so that their 16-byte pieces lie in different banks under the swizzle.
-        constexpr int kPasses = NG == 2 ? 1 : 2;
-        const int vw = warp - F::SOFT - 4;
-        const int word = NG == 8   ? (lane & 3) | (lane & 24) >> 1 | (lane & 4) << 2
-                         : NG == 4 ? lane & 15
-                                   : lane & 7;
-        const int part = KT == 128 ? lane >> 4 : 0, flip = NG == 8 ? 0 : lane >> 4;
-        const int hw0 = 2 * word;
-        int tile = 0;
-        while (next_piece<KT>(line, p, items, pc)) {
-            for (int i = 0; i < pc.count; ++i, ++tile) {
-                const int slot = tile % F::RAW, vs = tile % F::V_STAGES, meta = tile & (kMeta - 1);
-                ok = ok && warp_wait(s.raw_full + slot, (tile / F::RAW) & 1, gave_up);
-                ok = ok && warp_wait(s.meta_full + meta, (tile / kMeta) & 1, gave_up);
+                if (lane == 0) mbar_arrive(s.k_full + ks);
+                if (F::V_STAGES == 1 && tile >= 2)                // a use of the other warpgroup's: none may be passed over
+                    ok = ok && warp_wait(s.v_empty, (tile - 2) & 1, gave_up);
                 if (tile >= F::V_STAGES) ok = ok && warp_wait(s.v_empty + vs, (tile / F::V_STAGES - 1) & 1, gave_up);
                 if (!ok) break;
-                const uint32_t raw = at_raw + slot * F::RAW_BYTES;
                 const uint32_t to = at_v + vs * F::VHAT + part * (D * 128);
 #pragma unroll 1
                 for (int n = 0; n < kPasses; ++n) {
