@@ -660,16 +660,14 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                         for (; c < KT / 32; ++c) {
                             const int sh = kBias + s.ev[meta][c] - E;
                             const float fc = fac * s.k_unit[meta][c], at = static_cast<float>(sh) - M;
-                            const f2 fc2 = mk2(fc, fc), at2 = mk2(at, at);
-                            f2 sum0 = mk2(0.0f, 0.0f), sum1 = sum0;
+                            float sums[4] = {};
                             uint32_t out[16];
                             auto half = [&](const uint32_t (&x)[16], int to) {
 #pragma unroll
                                 for (int k = 0; k < 8; ++k) {
-                                    const f2 y = fma2(mk2u(x[2 * k], x[2 * k + 1]), fc2, at2);
-                                    const float a = ex2(lo(y)), b = ex2(hi(y));
-                                    if (k & 1) sum1 = add2(sum1, mk2(a, b));
-                                    else sum0 = add2(sum0, mk2(a, b));
+                                    const float a = ex2(fmaf(__uint_as_float(x[2 * k]), fc, at)), b = ex2(fmaf(__uint_as_float(x[2 * k + 1]), fc, at));
+                                    sums[2 * (k & 1)] += a;
+                                    sums[2 * (k & 1) + 1] += b;
                                     out[to + k] = h2_bits(__floats2half2_rn(a, b));
                                 }
                             };
@@ -679,8 +677,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                             tmem_have(w);
                             if (c + 1 < KT / 32) tmem_ask16(ts + 32 * c + 32, v);
                             half(w, 8);
-                            const f2 sums = add2(sum0, sum1);
-                            const float sum = lo(sums) + hi(sums);
+                            const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
                             if (__any_sync(0xffffffffu, sum > kMostSum || fabsf(M) > kMostM)) break;
                             l = fmaf(sum, pow2i(-sh), l);
                             tmem_st16(ts + 16 * c, out);              // columns that this lane has read
@@ -841,6 +838,9 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         constexpr int GW = KT == 128 ? NG : NG / 2;               // K: groups of a warp
         const int kw = warp & 3, span = KT == 128 ? kw : kw & 1, half = KT == 128 ? 0 : kw >> 1;
         const int c = lane & 3, pos_in = (lane >> 3) + (lane & 4);
+        const uint32_t k_src = (32 * span + pos_in) * (D / 2) + c * (4 * NG) + half * (4 * GW);
+        const uint32_t k_sc = F::K_SC + (32 * span + pos_in) * (2 * NG) + half * (2 * GW);
+        const uint32_t k_dst = (half * GW >> 1) * (KT * 128) + (32 * span + pos_in) * 128 + ((c ^ pos_in) << 4);
         // V: a thread has 8 positions, block j of 64, and a word (8 codes: 4 dims of groups g and g + 1) a pass.  Lanes read
         // different words, those that would meet on a bank the other position of a pair first; eight lanes that store
         // together have eight different j, so that their 16-byte pieces lie in different banks under the swizzle.
@@ -861,19 +861,17 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 if (tile >= F::K_STAGES) ok = ok && warp_wait(s.k_empty + ks, (tile / F::K_STAGES - 1) & 1, gave_up);
                 if (!ok) break;
                 const uint32_t raw = at_raw + slot * F::RAW_BYTES;
-                const uint32_t k_to = at_k + ks * F::KHAT;
+                const uint32_t k_codes = raw + k_src, k_scales = raw + k_sc, k_to0 = at_k + ks * F::KHAT + k_dst, k_to1 = k_to0 ^ 64u;
 #pragma unroll 2
                 for (int it = 0; it < 4; ++it) {
-                    const int r = 32 * span + 8 * it + pos_in;
                     uint32_t w[GW], d[GW / 2];
-                    lds_words<GW>(raw + r * (D / 2) + c * (4 * NG) + half * (4 * GW), w);
-                    lds_words<GW / 2>(raw + F::K_SC + r * (2 * NG) + half * (2 * GW), d);
+                    lds_words<GW>(k_codes + it * (4 * D), w);
+                    lds_words<GW / 2>(k_scales + it * (16 * NG), d);
 #pragma unroll
-                    for (int g = 0; g < GW; ++g) {
+                    for (int g = 0; g < GW; ++g) {                // 16-byte piece 4 g + c of the row
                         uint32_t out[4];
                         decode8(w[g], bits_h2(__byte_perm(d[g / 2], 0u, g & 1 ? 0x3232 : 0x1010)), out);
-                        const int j = 4 * (GW * half + g) + c;
-                        sts128(k_to + (j >> 3) * (KT * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4), make_uint4(out[0], out[1], out[2], out[3]));
+                        sts128((g & 1 ? k_to1 : k_to0) + (g >> 1) * (KT * 128) + it * 1024, make_uint4(out[0], out[1], out[2], out[3]));
                     }
                 }
                 fence_proxy_shared();
@@ -899,7 +897,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                     for (int x = 0; x < 2; ++x) {
                         const uint32_t pick = flip ? (x ? 0x3276u : 0x1054u) : x ? 0x7632u : 0x5410u;
                         const int hw = hw0 + x, dim = 32 * (hw % NG) + 4 * (hw / NG);
-                        const uint32_t row = to + dim * 128;
+                        const uint32_t at = to + dim * 128 + ((j ^ (dim & 4)) << 4);
                         uint32_t out[4][4];                       // [dim][pair of positions]
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
@@ -910,7 +908,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                         }
 #pragma unroll
                         for (int m = 0; m < 4; ++m)
-                            sts128(row + m * 128 + ((j ^ ((dim + m) & 7)) << 4), make_uint4(out[m][0], out[m][1], out[m][2], out[m][3]));
+                            sts128((at ^ (m << 4)) + m * 128, make_uint4(out[m][0], out[m][1], out[m][2], out[m][3]));
                     }
                 }
                 fence_proxy_shared();
