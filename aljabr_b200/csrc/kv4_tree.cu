@@ -886,23 +886,23 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 for (int n = 0; n < kPasses; ++n) {
                     const int j = (lane + (NG == 2 ? vw + ((lane & 8) >> 1) : 2 * vw + n)) & 7, pos = 64 * part + 8 * j;
                     const uint32_t blk = raw + F::V_CODES + pos * (D / 2) + 4 * word;
-                    const uint32_t sc = raw + F::V_SC + pos * (2 * NG) + 4 * (word % (NG / 2));
-                    uint32_t code[8], d[8];                       // register k: position k ^ flip
+                    const int q = pos >> 2, turned = (q >> 3) & 1;
+                    const uint32_t sc = raw + F::V_SC + ((word % (NG / 2)) * KT + 4 * (q ^ turned)) * 4;
+                    uint32_t code[8], d[2][4];                    // code k: position k ^ flip
+                    lds_words<4>(sc, d[0]);
+                    lds_words<4>(turned ? sc - 16 : sc + 16, d[1]);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        code[k] = lds_word(blk + (k & 6) * (D / 2) + (k & 1 ? (flip ^ 1) : flip) * (D / 2));
-                        d[k] = lds_word(sc + (k & 6) * (2 * NG) + (k & 1 ? (flip ^ 1) : flip) * (2 * NG));
-                    }
+                    for (int k = 0; k < 8; ++k) code[k] = lds_word(blk + (k & 6) * (D / 2) + (k & 1 ? (flip ^ 1) : flip) * (D / 2));
 #pragma unroll 1
                     for (int x = 0; x < 2; ++x) {
-                        const uint32_t pick = flip ? (x ? 0x3276u : 0x1054u) : x ? 0x7632u : 0x5410u;
+                        const uint32_t pick_d = x ? 0x7632u : 0x5410u, pick = flip ? (x ? 0x3276u : 0x1054u) : pick_d;
                         const int hw = hw0 + x, dim = 32 * (hw % NG) + 4 * (hw / NG);
                         const uint32_t at = to + dim * 128 + ((j ^ (dim & 4)) << 4);
                         uint32_t out[4][4];                       // [dim][pair of positions]
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             uint32_t v[4];
-                            decode8(__byte_perm(code[2 * k], code[2 * k + 1], pick), bits_h2(__byte_perm(d[2 * k], d[2 * k + 1], pick)), v);
+                            decode8(__byte_perm(code[2 * k], code[2 * k + 1], pick), bits_h2(__byte_perm(d[k >> 1][2 * (k & 1)], d[k >> 1][2 * (k & 1) + 1], pick_d)), v);
 #pragma unroll
                             for (int m = 0; m < 4; ++m) out[m][k] = v[m];
                         }
@@ -1017,15 +1017,17 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 if (!ok) break;
                 int e_top = -100;
                 bool any = false;
-#pragma unroll 1
-                for (int c = 0; c < KT / 32; ++c) {               // 32 positions, a lane each
-                    const uint32_t at = at_raw + slot * F::RAW_BYTES + (is_v ? F::V_SC : F::K_SC) + (32 * c + lane) * (2 * NG);
+                uint32_t w[KT / 32][NG / 2];                      // 32 positions, a lane each
+                const uint32_t at = at_raw + slot * F::RAW_BYTES + (is_v ? F::V_SC : F::K_SC);
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c) lds_words<NG / 2>(at + (32 * c + lane) * (2 * NG), w[c]);
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c) {
                     const bool mine = (s.valid[slot][c] >> lane) & 1u;
-                    uint32_t w[NG / 2];
-                    lds_words<NG / 2>(at, w);
-                    uint32_t top = __reduce_max_sync(0xffffffffu, mine ? top_of(w, false) : 0u);
+                    uint32_t top = __reduce_max_sync(0xffffffffu, mine ? top_of(w[c], false) : 0u);
                     if (top >= 0x7C00u) {
-                        top = __reduce_max_sync(0xffffffffu, mine ? top_of(w, true) : 0u);
+                        top = __reduce_max_sync(0xffffffffu, mine ? top_of(w[c], true) : 0u);
                         if (is_v) {                               // NaN groups of V count as zero, and their rows are marked
                             if (!any)
                                 for (int k = lane; k < KT; k += 32) s.nan[meta][k] = 0;
@@ -1033,9 +1035,9 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                             int bad = 0;
 #pragma unroll
                             for (int g = 0; g < NG; ++g)
-                                if (((w[g / 2] >> (16 * (g & 1))) & 0x7FFFu) >= 0x7C00u) {
+                                if (((w[c][g / 2] >> (16 * (g & 1))) & 0x7FFFu) >= 0x7C00u) {
                                     bad |= 1 << g;
-                                    w[g / 2] &= g & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                                    w[c][g / 2] &= g & 1 ? 0x0000FFFFu : 0xFFFF0000u;
                                 }
                             __syncwarp();
                             if (mine) s.nan[meta][32 * c + lane] = static_cast<uint8_t>(bad);
@@ -1044,8 +1046,16 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                     const int e = exponent_of(top);
                     const Unit unit(e);
 #pragma unroll
-                    for (int k = 0; k < NG / 2; ++k) w[k] = mine ? unit.of(w[k]) : 0u;
-                    sts_words<NG / 2>(at, w);
+                    for (int k = 0; k < NG / 2; ++k) w[c][k] = mine ? unit.of(w[c][k]) : 0u;
+                    if (is_v) {
+                        // word by word, so that a thread finds 8 positions side by side; their 16-byte halves trade places
+                        // in every second 32 positions, or eight threads' would meet on four banks
+                        const int q = 8 * c + (lane >> 2), place = 4 * (q ^ ((q >> 3) & 1)) + (lane & 3);
+#pragma unroll
+                        for (int k = 0; k < NG / 2; ++k) sts_words<1>(at + (k * KT + place) * 4, reinterpret_cast<const uint32_t(&)[1]>(w[c][k]));
+                    } else {
+                        sts_words<NG / 2>(at + (32 * c + lane) * (2 * NG), w[c]);
+                    }
                     e_top = max(e_top, e);
                     if (lane == 0) {
                         if (is_v) s.ev[meta][c] = e;
