@@ -46,7 +46,8 @@ namespace {
 
 constexpr int kRows = 128;
 constexpr int kPages = 128;           // page ids read from the table at once
-constexpr int kItemCost = 2;          // tiles that an item's start and end are worth
+constexpr int kItemCost = 4;          // tiles that an item's start and end are worth
+constexpr int kLeast = 3;             // places of a CTA: fewer, and joining them costs more than it saves
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -3.4e38f;     // running maximum of a row that has seen nothing
 // P <= 2^(kLazy + kSlack + kBias) = 2^15, or its sum over 32 positions <= kMostSum
@@ -449,9 +450,10 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         return n;
     };
     int total = 0, incl;
-    for (int b0 = 0; b0 < p.batch; b0 += F::THREADS) total += scan(width_of(b0 + threadIdx.x), 0, incl);
+    int mine = 0;                     // the thread's sequence's places
+    for (int b0 = 0; b0 < p.batch; b0 += F::THREADS) total += scan(mine = width_of(b0 + threadIdx.x), 0, incl);
     total *= items;                   // < 2^31: checked on the host for the longest sequences
-    const int ctas = min(static_cast<int>(gridDim.x), (total + kItemCost) / (kItemCost + 1));
+    const int ctas = min(static_cast<int>(gridDim.x), (total + kLeast - 1) / kLeast);
     const int share = total / ctas, rem = total - share * ctas;
     auto start_of = [&](int c) { return share * c + min(c, rem); };
     auto cta_at = [&](int x) {
@@ -464,10 +466,9 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         const int x0 = start_of(blockIdx.x), x1 = start_of(blockIdx.x + 1);
         int before = 0;               // line places before the sequences at hand, of one item
         for (int b0 = 0; b0 < p.batch; b0 += F::THREADS) {
-            const int n = width_of(b0 + threadIdx.x);
-            before += scan(n, before, incl);
-            const int pre = incl - n;
-            if (n > 0 && pre * items <= x0 && x0 < incl * items) {
+            if (p.batch > F::THREADS) before += scan(mine = width_of(b0 + threadIdx.x), before, incl);
+            const int pre = incl - mine;
+            if (mine > 0 && pre * items <= x0 && x0 < incl * items) {
                 s.start[0] = b0 + threadIdx.x;
                 s.start[1] = pre;
             }
@@ -522,6 +523,32 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             const bool whole = pc.ch == 0 && (pc.count == pc.chunks || pc.count == 0);
             const int line0 = pre * items + pc.h * (pc.chunks + kItemCost) + kItemCost;
             // -------------------------------------------------- the rows' masks and Q
+            // Q's rows come to their places in shared memory as they are, while the masks are made: a lane 16 bytes of a row,
+            // kPer rows a pass of a warp
+            constexpr int kChunks = D / 8, kPer = 32 / kChunks, kPasses = kRows / kPer / F::SOFT;
+            const int j = lane % kChunks;
+            auto place_of = [&](int k, int& r) {
+                r = (k * F::SOFT + warp) * kPer + lane / kChunks;
+                return at_q + (j >> 3) * (kRows * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4);
+            };
+            if (pc.count > 0) {
+                const bool wide = ((reinterpret_cast<uintptr_t>(p.q) | static_cast<uintptr_t>(p.q_stride * 2)) & 15) == 0;
+#pragma unroll 2
+                for (int k = 0; k < kPasses; ++k) {
+                    int r;
+                    const uint32_t place = place_of(k, r);
+                    const int i = min(pc.row0 + r, p.q_len * p.group - 1), t = token_of(i), hd = i - t * p.group;
+                    const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) + (static_cast<long long>(pc.b) * p.q_len + t) * p.q_stride +
+                                             static_cast<long long>(pc.kvh * p.group + hd) * D + 8 * j;
+                    if (wide) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place), "l"(q), "r"(r < pc.rows ? 16 : 0) : "memory");
+                    } else {
+                        const unsigned short* h = reinterpret_cast<const unsigned short*>(q);
+                        sts128(place, r < pc.rows ? make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16)
+                                                  : make_uint4(0u, 0u, 0u, 0u));
+                    }
+                }
+            }
             for (int i = thread; i < p.q_len; i += 32 * F::SOFT)
                 s.par[i] = static_cast<short>(tree_parent(p.parents + static_cast<long long>(pc.b) * p.parents_stride, i));
             sync();
@@ -542,57 +569,31 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             const int row_lo = window_start(p, pc.base + depth);          // first position the row sees
             const int all_lo = window_start(p, pc.len);
             if (pc.count > 0) {
-                // 16-byte chunks of a row, rows of a warp's pass; kBatch loads are under way at a time
-                constexpr int kChunks = D / 8, kPer = 32 / kChunks, kPasses = kRows / kPer / F::SOFT, kBatch = 4;
-                static_assert(kPasses % kBatch == 0, "passes of a batch");
-                const int j = lane % kChunks;
-                const bool wide = ((reinterpret_cast<uintptr_t>(p.q) | static_cast<uintptr_t>(p.q_stride * 2)) & 15) == 0;
+                asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
-                for (int k0 = 0; k0 < kPasses; k0 += kBatch) {
-                    uint4 x[kBatch];
+                for (int k = 0; k < kPasses; ++k) {               // each lane what it brought
+                    int r;
+                    const uint32_t place = place_of(k, r);
+                    uint32_t w[4];
+                    lds_words<4>(place, w);
+                    float v[8], big = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < kBatch; ++k) {
-                        const int r = ((k0 + k) * F::SOFT + warp) * kPer + lane / kChunks, i = pc.row0 + r;
-                        x[k] = make_uint4(0u, 0u, 0u, 0u);
-                        if (r < pc.rows) {
-                            const int t = token_of(i), hd = i - t * p.group;
-                            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) +
-                                (static_cast<long long>(pc.b) * p.q_len + t) * p.q_stride +
-                                static_cast<long long>(pc.kvh * p.group + hd) * D + 8 * j;
-                            if (wide) {
-                                x[k] = *reinterpret_cast<const uint4*>(q);
-                            } else {
-                                const unsigned short* h = reinterpret_cast<const unsigned short*>(q);
-                                x[k] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-                            }
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        v[2 * i] = __uint_as_float(w[i] << 16);
+                        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
                     }
-#pragma unroll 1
-                    for (int k = 0; k < kBatch; ++k) {
-                        const uint4 y = x[0];                     // rotated through
 #pragma unroll
-                        for (int n = 0; n + 1 < kBatch; ++n) x[n] = x[n + 1];
-                        const int r = ((k0 + k) * F::SOFT + warp) * kPer + lane / kChunks;
-                        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-                        float v[8], big = 0.0f;
+                    for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(v[i]));
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            v[2 * i] = __uint_as_float(w[i] << 16);
-                            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-                        }
+                    for (int o = 1; o < kChunks; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                    // the row times 2^f: its largest in [2^14, 2^15), where both 2^f and 2^-f are normal
+                    const int f = big > 0.0f ? max(-100, min(126, 14 - (static_cast<int>((__float_as_uint(big) >> 23) & 255) - 127))) : 0;
+                    const float up = p.scale < 0.0f ? -pow2i(f) : pow2i(f);
+                    if (j == 0) s.fac[r] = size * pow2i(-f);
+                    uint32_t out[4];                  // as decode8 orders the dims of a chunk
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(v[i]));
-#pragma unroll
-                        for (int o = 1; o < kChunks; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                        // the row times 2^f: its largest in [2^14, 2^15), where both 2^f and 2^-f are normal
-                        const int f = big > 0.0f ? max(-100, min(126, 14 - (static_cast<int>((__float_as_uint(big) >> 23) & 255) - 127))) : 0;
-                        const float up = p.scale < 0.0f ? -pow2i(f) : pow2i(f);
-                        if (j == 0) s.fac[r] = size * pow2i(-f);
-                        uint32_t out[4];              // as decode8 orders the dims of a chunk
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) out[i] = h2_bits(__floats2half2_rn(v[i] * up, v[i + 4] * up));
-                        sts128(at_q + (j >> 3) * (kRows * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4), make_uint4(out[0], out[1], out[2], out[3]));
-                    }
+                    for (int i = 0; i < 4; ++i) out[i] = h2_bits(__floats2half2_rn(v[i] * up, v[i + 4] * up));
+                    sts128(place, make_uint4(out[0], out[1], out[2], out[3]));
                 }
             }
             fence_proxy_shared();
@@ -765,7 +766,6 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             const bool has0 = pc.count > 0 && (F::STREAMS == 1 || pc.count > 1 || (tiles & 1) == 0);
             const bool has1 = F::STREAMS == 2 && (pc.count > 1 || (pc.count == 1 && (tiles & 1) == 1));
             tiles += pc.count;
-            const int i = pc.row0 + row;
             float w0 = 0.0f, w1 = 0.0f, L = 0.0f, top = kNone;
             int gone = 0;
             if (alive && pc.count > 0) {
@@ -787,40 +787,57 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             constexpr int kCols = D / F::STREAMS;                     // columns of a warp
             if (ok && warp_lives) {
-                const int t = token_of(min(i, p.q_len * p.group - 1)), hd = i - t * p.group;
-                __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(p.out) +
-                    (((static_cast<long long>(pc.b) * p.q_len + t) * p.kv_heads + pc.kvh) * p.group + hd) * D;
-                float* const part = p.part + static_cast<long long>(slot) * (kRows * (D + 2)) + row * D;
+                // kCut columns of the warp's rows at a time through its share of Q's place, so that a row's are written side by
+                // side; 16-byte pieces are swizzled by the row
+                constexpr int kCut = D == 64 ? 16 : 32, kPieces = kCut / 4;
+                const uint32_t stage = at_q + warp * (F::Q / F::SOFT);
+                float* const part = p.part + static_cast<long long>(slot) * (kRows * (D + 2));
 #pragma unroll 1
-                for (int d = stream * kCols; d < (stream + 1) * kCols; d += 8) {
-                    float o[8] = {};
-                    uint32_t v[8];
-                    if (has0) {
-                        tmem_ld8(tq + F::O_COL + d, v);
+                for (int d0 = stream * kCols; d0 < (stream + 1) * kCols; d0 += kCut) {
+                    const bool nan = (gone >> (d0 >> 5)) & 1;
+#pragma unroll 1
+                    for (int d = 0; d < kCut; d += 8) {
+                        float o[8] = {};
+                        uint32_t v[8];
+                        if (has0) {
+                            tmem_ld8(tq + F::O_COL + d0 + d, v);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[k]) * w0;
-                    }
-                    if (has1) {
-                        tmem_ld8(tq + F::O_COL + D + d, v);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) o[k] = fmaf(__uint_as_float(v[k]), w1, o[k]);
-                    }
-                    const bool nan = (gone >> (d >> 5)) & 1;
-                    if (row >= pc.rows) continue;                     // after the warp's loads
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) o[k] = !alive || L == 0.0f ? 0.0f : nan ? NAN : o[k];   // a row that sees nothing is zero
-                    if (whole) {
-                        uint32_t h[4];
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            const __nv_bfloat162 r2 = __floats2bfloat162_rn(o[2 * n] * inv, o[2 * n + 1] * inv);
-                            h[n] = *reinterpret_cast<const uint32_t*>(&r2);
+                            for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[k]) * w0;
                         }
-                        *reinterpret_cast<uint4*>(out + d) = make_uint4(h[0], h[1], h[2], h[3]);
-                    } else {
-                        reinterpret_cast<float4*>(part + d)[0] = make_float4(o[0], o[1], o[2], o[3]);
-                        reinterpret_cast<float4*>(part + d)[1] = make_float4(o[4], o[5], o[6], o[7]);
+                        if (has1) {
+                            tmem_ld8(tq + F::O_COL + D + d0 + d, v);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) o[k] = fmaf(__uint_as_float(v[k]), w1, o[k]);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float x = !alive || L == 0.0f ? 0.0f : nan ? NAN : whole ? o[k] * inv : o[k];   // what sees nothing is zero
+                            v[k] = __float_as_uint(x);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            sts128(stage + lane * (kCut * 4) + (((d / 4 + k) ^ (lane & (kPieces - 1))) << 4),
+                                   make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
                     }
+                    __syncwarp();
+#pragma unroll 1
+                    for (int n = lane; n < 32 * kPieces; n += 32) {
+                        const int r = n / kPieces, piece = n % kPieces, at = (warp & 3) * 32 + r, d = d0 + 4 * piece;
+                        uint32_t x[4];
+                        lds_words<4>(stage + r * (kCut * 4) + ((piece ^ (r & (kPieces - 1))) << 4), x);
+                        if (at >= pc.rows) continue;
+                        if (whole) {
+                            const int t = token_of(pc.row0 + at), hd = pc.row0 + at - t * p.group;
+                            const __nv_bfloat162 a = __floats2bfloat162_rn(__uint_as_float(x[0]), __uint_as_float(x[1]));
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(x[2]), __uint_as_float(x[3]));
+                            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) +
+                                (((static_cast<long long>(pc.b) * p.q_len + t) * p.kv_heads + pc.kvh) * p.group + hd) * D + d) =
+                                make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+                        } else {
+                            *reinterpret_cast<uint4*>(part + at * D + d) = make_uint4(x[0], x[1], x[2], x[3]);
+                        }
+                    }
+                    __syncwarp();
                 }
                 if (!whole && stream == 0 && row < pc.rows) {
                     float* const ml = p.part + static_cast<long long>(slot) * (kRows * (D + 2)) + kRows * D + row * 2;
