@@ -46,7 +46,7 @@ namespace {
 
 constexpr int kRows = 128;
 constexpr int kPages = 128;           // page ids read from the table at once
-constexpr int kItemCost = 4;          // tiles that an item's start and end are worth
+constexpr int kItemCost = 8;          // tiles that an item's start and end are worth
 constexpr int kLeast = 3;             // places of a CTA: fewer, and joining them costs more than it saves
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -3.4e38f;     // running maximum of a row that has seen nothing
@@ -225,6 +225,16 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
                  :
                  : "memory");
+}
+__device__ __forceinline__ void tmem_ld8x2(uint32_t at0, uint32_t at1, uint32_t (&r)[8], uint32_t (&q)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3]), "=&r"(r[4]), "=&r"(r[5]), "=&r"(r[6]), "=&r"(r[7]), "=&r"(q[0]),
+          "=&r"(q[1]), "=&r"(q[2]), "=&r"(q[3]), "=&r"(q[4]), "=&r"(q[5]), "=&r"(q[6]), "=&r"(q[7])
+        : "r"(at0), "r"(at1)
+        : "memory");
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
@@ -797,22 +807,13 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                     const bool nan = (gone >> (d0 >> 5)) & 1;
 #pragma unroll 1
                     for (int d = 0; d < kCut; d += 8) {
-                        float o[8] = {};
-                        uint32_t v[8];
-                        if (has0) {
-                            tmem_ld8(tq + F::O_COL + d0 + d, v);
+                        uint32_t v[8], w[8];
+                        tmem_ld8x2(tq + F::O_COL + d0 + d, tq + F::O_COL + (F::STREAMS - 1) * D + d0 + d, v, w);
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(v[k]) * w0;
-                        }
-                        if (has1) {
-                            tmem_ld8(tq + F::O_COL + D + d0 + d, v);
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) o[k] = fmaf(__uint_as_float(v[k]), w1, o[k]);
-                        }
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const float x = !alive || L == 0.0f ? 0.0f : nan ? NAN : whole ? o[k] * inv : o[k];   // what sees nothing is zero
-                            v[k] = __float_as_uint(x);
+                        for (int k = 0; k < 8; ++k) {             // what has not been written may be anything
+                            float o = has0 ? __uint_as_float(v[k]) * w0 : 0.0f;
+                            if (has1) o = fmaf(__uint_as_float(w[k]), w1, o);
+                            v[k] = __float_as_uint(!alive || L == 0.0f ? 0.0f : nan ? NAN : whole ? o * inv : o);   // what sees nothing is zero
                         }
 #pragma unroll
                         for (int k = 0; k < 2; ++k)
@@ -1147,8 +1148,8 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
     }
 }
 
-// Items cut over CTAs: block (c, y) joins 16 rows of the item that CTA c began and others went on with, in CTA order.
-constexpr int kJoinRows = 16;
+// Items cut over CTAs: block (c, y) joins kJoinRows rows of the item that CTA c began and others went on with, in CTA order.
+constexpr int kJoinRows = 8;
 template <int D>
 __global__ void __launch_bounds__(256) kv4_tree_join_kernel(const Kv4Attn p, const Cut* cuts, unsigned int* fault_word) {
     pdl_launch_dependents();
@@ -1167,7 +1168,7 @@ __global__ void __launch_bounds__(256) kv4_tree_join_kernel(const Kv4Attn p, con
         if (row >= rows) break;
         float top = kNone, L = 0.0f;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
         for (int k = 0; k < cut.n; ++k) {
             const float* part = base(k);
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + kRows * D + row * 2));
