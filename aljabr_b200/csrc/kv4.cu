@@ -113,9 +113,9 @@ __device__ __forceinline__ void find_block(const Kv4Rows& p, int slot, Where& w)
 }
 
 template <int D>
-__device__ __forceinline__ bool place(const Kv4Rows& p, Where& w) {
+__device__ __forceinline__ bool place(const Kv4Rows& p, Where& w, unsigned int block) {
     constexpr int kLanes = D / 8;
-    const unsigned int row = blockIdx.x * (kRowThreads / kLanes) + threadIdx.x / kLanes;   // < 2^31: checked on the host
+    const unsigned int row = block * (kRowThreads / kLanes) + threadIdx.x / kLanes;   // < 2^31: checked on the host
     w.j = threadIdx.x % kLanes;
     w.token = row / static_cast<unsigned int>(p.kv_heads);
     w.head = row - w.token * p.kv_heads;
@@ -125,6 +125,13 @@ __device__ __forceinline__ bool place(const Kv4Rows& p, Where& w) {
     }
     find_block<D>(p, __ldg(p.slots + w.token), w);
     return true;
+}
+
+// (a, b) turned by the angle of cosine c and sine s.
+__device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) {
+    const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+    b = __fadd_rn(__fmul_rn(a, s), __fmul_rn(b, c));
+    a = x;
 }
 
 // Codes of 8 values as a word, and the values they stand for back in x.
@@ -199,7 +206,7 @@ __global__ void __launch_bounds__(kRowThreads, 12) kv4_append_kernel(const Kv4Ro
     pdl_launch_dependents();
     pdl_wait();
     Where w;
-    const bool live = place<D>(p, w);
+    const bool live = place<D>(p, w, blockIdx.x);
     float k[8] = {}, v[8] = {};
     const bool write = live && w.block >= 0;
     if (write) {
@@ -221,7 +228,7 @@ __global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(const Kv4Rows p) 
     pdl_wait();
     constexpr int NG = D / 32;
     Where w;
-    if (!place<D>(p, w)) return;
+    if (!place<D>(p, w, blockIdx.x)) return;
     const int g = w.j >> 2, c = w.j & 3;
     float k[8] = {}, v[8] = {};
     if (w.block >= 0) {
@@ -242,88 +249,115 @@ __global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(const Kv4Rows p) 
     if (p.v_out) Wide<T>::store(static_cast<T*>(p.v_out) + at, p.vec_out, v);
 }
 
-// Rows of new tokens with the position rotation on the way: q is rotated into q_out, k before it is quantised.  A
-// thread owns 8 consecutive dims of a head, as above; the dims they pair with are its own (interleaved) or another
-// lane's of the same row (split halves: one shuffle a value).  A CTA stays with one token for p.span units a row of
-// threads, a unit being a q head or a kv head's K and V, so that the token's cosines and sines are loaded once.
+// Rows of new tokens with the position rotation on the way: q is rotated into q_out, k before it is quantised; the
+// products and sums are rounded one by one, as in the decode step.  The first p.q_blocks CTAs have the q rows: a thread
+// owns two runs of 8 dims that are each other's pairs (split halves) or adjacent (interleaved, and what does not turn),
+// so nothing is exchanged, and keeps their 8 cosines and sines for p.span heads of its token.  The others have K and V,
+// laid out as in kv4_append_kernel for the groups' shuffles; there a split half's pairs come by shuffle too (which for
+// q cost 16384 tokens of 32 + 8 heads 141 us in all, as one CTA a token).
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowThreads) kv4_rotate_append_kernel(const Kv4Rotate p) {
-    pdl_launch_dependents();
-    pdl_wait();
-    constexpr int kLanes = D / 8, kSlots = kRowThreads / kLanes;
-    Where w;
-    w.token = blockIdx.x / p.splits;
-    w.j = threadIdx.x % kLanes;
-    const int first = (blockIdx.x - w.token * p.splits) * (p.span * kSlots) + threadIdx.x / kLanes;
-    const int units = p.q_heads + p.rows.kv_heads;
-    int pos = __ldg(p.positions + w.token);
-    const int slot = __ldg(p.rows.slots + w.token);
+__device__ __forceinline__ void rotate_q(const Kv4Rotate& p) {
+    constexpr int kLanes = D / 16, kPer = kRowThreads / kLanes;
+    const unsigned int row = blockIdx.x * kPer + threadIdx.x / kLanes;
+    const int t = threadIdx.x % kLanes;
+    const int token = row / static_cast<unsigned int>(p.splits);
+    if (token >= p.rows.tokens) return;
+    const int head0 = (row - token * p.splits) * p.span, heads = min(p.span, p.q_heads - head0);
+    int pos = __ldg(p.positions + token);
     if (pos >= p.rope_positions) {
         record_fault(ALJ_FAULT_BOUNDS);
         pos = -1;
     }
-    // this thread's pairs: 8 (split halves) or 4 (interleaved) of (cos, sin)
-    const int half8 = p.half >> 3;                 // lanes of one half of the rotated dims
-    const bool turns = w.j < 2 * half8 && pos >= 0;
-    const bool second = !p.interleaved && w.j >= half8;
+    const int half8 = p.half >> 3;                 // runs of 8 in half of the turning dims
+    const bool turns = t < half8 && pos >= 0;
+    // its runs: with split halves t and t + half8, behind the turning dims two neighbours
+    const int run0 = p.interleaved || t >= half8 ? 2 * t : t, run1 = p.interleaved || t >= half8 ? 2 * t + 1 : t + half8;
     float cs[8], sn[8];
+    if (turns) {
+        const float4* at = reinterpret_cast<const float4*>(p.rope + static_cast<long long>(pos) * p.half + 8 * t);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) cs[i] = 1.0f, sn[i] = 0.0f;
+        for (int i = 0; i < 4; ++i) {
+            const float4 f = __ldg(at + i);
+            cs[2 * i] = f.x, sn[2 * i] = f.y, cs[2 * i + 1] = f.z, sn[2 * i + 1] = f.w;
+        }
+    }
+    const T* q = static_cast<const T*>(p.q) + token * p.q_stride + head0 * D;
+    T* out = static_cast<T*>(p.q_out) + token * p.q_out_stride + head0 * D;
+#pragma unroll 2
+    for (int h = 0; h < heads; ++h, q += D, out += D) {
+        float a[8] = {}, b[8] = {};
+        if (pos >= 0) {
+            Wide<T>::load(q + 8 * run0, p.vec_q, a);
+            Wide<T>::load(q + 8 * run1, p.vec_q, b);
+        }
+        if (turns && p.interleaved) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                turn_pair(a[2 * i], a[2 * i + 1], cs[i], sn[i]);
+                turn_pair(b[2 * i], b[2 * i + 1], cs[4 + i], sn[4 + i]);
+            }
+        } else if (turns) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) turn_pair(a[i], b[i], cs[i], sn[i]);
+        }
+        Wide<T>::store(out + 8 * run0, p.vec_q_out, a);
+        Wide<T>::store(out + 8 * run1, p.vec_q_out, b);
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowThreads) kv4_rotate_append_kernel(const Kv4Rotate p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    if (blockIdx.x < p.q_blocks) {
+        rotate_q<T, D>(p);
+        return;
+    }
+    Where w;
+    const bool live = place<D>(p.rows, w, blockIdx.x - p.q_blocks);
+    int pos = live ? __ldg(p.positions + w.token) : -1;
+    if (pos >= p.rope_positions) {
+        if (w.head == 0) record_fault(ALJ_FAULT_BOUNDS);
+        pos = -1;
+    }
+    float k[8] = {}, v[8] = {};
+    const bool write = live && w.block >= 0 && pos >= 0;
+    const int half8 = p.half >> 3;
+    const bool turns = write && w.j < 2 * half8, second = !p.interleaved && w.j >= half8;
+    float cs[8] = {}, sn[8] = {};
+    if (write) {
+        const int col = w.head * D + 8 * w.j;
+        Wide<T>::load(static_cast<const T*>(p.rows.k) + w.token * p.rows.k_stride + col, p.rows.vec, k);
+        Wide<T>::load(static_cast<const T*>(p.rows.v) + w.token * p.rows.v_stride + col, p.rows.vec, v);
+    }
     if (turns) {
         const int pair = p.interleaved ? 4 * w.j : 8 * (second ? w.j - half8 : w.j);
-        const float4* row = reinterpret_cast<const float4*>(p.rope + static_cast<long long>(pos) * p.half + pair);
+        const float4* at = reinterpret_cast<const float4*>(p.rope + static_cast<long long>(pos) * p.half + pair);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (i >= 2 && p.interleaved) break;
-            const float4 t = __ldg(row + i);
-            cs[2 * i] = t.x, sn[2 * i] = t.y, cs[2 * i + 1] = t.z, sn[2 * i + 1] = t.w;
+            const float4 f = __ldg(at + i);
+            cs[2 * i] = f.x, sn[2 * i] = f.y, cs[2 * i + 1] = f.z, sn[2 * i + 1] = f.w;
         }
     }
-    const int lane = threadIdx.x & 31;
-    const int partner = turns && !p.interleaved ? lane + (second ? -half8 : half8) : lane;
-    auto turn = [&](float (&x)[8]) {               // products and sums rounded one by one, as in the decode step
-        if (p.interleaved) {
+    if (p.interleaved) {
+        if (turns) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = x[2 * i], b = x[2 * i + 1];
-                if (turns) {
-                    x[2 * i] = __fsub_rn(__fmul_rn(a, cs[i]), __fmul_rn(b, sn[i]));
-                    x[2 * i + 1] = __fadd_rn(__fmul_rn(a, sn[i]), __fmul_rn(b, cs[i]));
-                }
-            }
-        } else {
+            for (int i = 0; i < 4; ++i) turn_pair(k[2 * i], k[2 * i + 1], cs[i], sn[i]);
+        }
+    } else {                                       // every lane takes part: a row's lanes turn together
+        const int lane = threadIdx.x & 31, partner = turns ? lane + (second ? -half8 : half8) : lane;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float other = __fmul_rn(__shfl_sync(0xffffffffu, x[i], partner), sn[i]), own = __fmul_rn(x[i], cs[i]);
-                if (turns) x[i] = second ? __fadd_rn(other, own) : __fsub_rn(own, other);
-            }
+        for (int i = 0; i < 8; ++i) {
+            const float other = __fmul_rn(__shfl_sync(0xffffffffu, k[i], partner), sn[i]), own = __fmul_rn(k[i], cs[i]);
+            if (turns) k[i] = second ? __fadd_rn(other, own) : __fsub_rn(own, other);
         }
-    };
-    for (int s = 0; s < p.span; ++s) {
-        const int unit = first + s * kSlots;
-        const bool is_q = unit < p.q_heads, live = unit < units;
-        if (!__any_sync(0xffffffffu, live)) break;
-        w.head = unit - p.q_heads;
-        w.block = -1;
-        if (live && !is_q && pos >= 0) find_block<D>(p.rows, slot, w);
-        const bool write = w.block >= 0;
-        float x[8] = {}, v[8] = {};
-        if (live && is_q && pos >= 0)
-            Wide<T>::load(static_cast<const T*>(p.q) + w.token * p.q_stride + unit * D + 8 * w.j, p.vec_q, x);
-        if (write) {
-            const int col = w.head * D + 8 * w.j;
-            Wide<T>::load(static_cast<const T*>(p.rows.k) + w.token * p.rows.k_stride + col, p.rows.vec, x);
-            Wide<T>::load(static_cast<const T*>(p.rows.v) + w.token * p.rows.v_stride + col, p.rows.vec, v);
-        }
-        turn(x);
-        if (live && is_q) Wide<T>::store(static_cast<T*>(p.q_out) + w.token * p.q_out_stride + unit * D + 8 * w.j, p.vec_q_out, x);
-        if (!__any_sync(0xffffffffu, live && !is_q)) continue;
-        put8<D>(p.rows, w, write, x, v);
-        if (live && !is_q && p.rows.k_out) {
-            const long long at = (static_cast<long long>(w.token) * p.rows.kv_heads + w.head) * D + 8 * w.j;
-            Wide<T>::store(static_cast<T*>(p.rows.k_out) + at, p.rows.vec_out, x);
-            Wide<T>::store(static_cast<T*>(p.rows.v_out) + at, p.rows.vec_out, v);
-        }
+    }
+    put8<D>(p.rows, w, write, k, v);               // a skipped row's zeros are not stored
+    if (live && p.rows.k_out) {
+        const long long at = (static_cast<long long>(w.token) * p.rows.kv_heads + w.head) * D + 8 * w.j;
+        Wide<T>::store(static_cast<T*>(p.rows.k_out) + at, p.rows.vec_out, k);
+        Wide<T>::store(static_cast<T*>(p.rows.v_out) + at, p.rows.vec_out, v);
     }
 }
 
@@ -428,13 +462,14 @@ cudaError_t launch_kv4_append(const Kv4Rows& p, cudaStream_t stream) {
 cudaError_t launch_kv4_rotate_append(const Kv4Rotate& a, int sms, cudaStream_t stream) {
     Kv4Rotate p = a;
     p.rows.page_shift = (p.rows.page_size & (p.rows.page_size - 1)) == 0 ? __builtin_ctz(p.rows.page_size) : -1;
-    const int slots = kRowThreads / (p.rows.head_dim / 8), units = p.q_heads + p.rows.kv_heads;
-    const int most = (units + slots - 1) / slots;
-    // a CTA a token where those fill the GPU, else one for every `slots` heads
-    p.span = p.rows.tokens >= 4 * sms ? most : 1;
-    p.splits = (most + p.span - 1) / p.span;
+    // q: four heads a thread where the rows still fill the GPU, else one
+    const long long tokens = p.rows.tokens;
+    const int per_q = kRowThreads / (p.rows.head_dim / 16), per_kv = kRowThreads / (p.rows.head_dim / 8);
+    p.span = tokens * ((p.q_heads + 3) / 4) / per_q >= 8LL * sms ? 4 : 1;
+    p.splits = (p.q_heads + p.span - 1) / p.span;
+    p.q_blocks = static_cast<unsigned int>((tokens * p.splits + per_q - 1) / per_q);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned int>(p.rows.tokens) * p.splits);
+    cfg.gridDim = dim3(p.q_blocks + static_cast<unsigned int>((tokens * p.rows.kv_heads + per_kv - 1) / per_kv));
     cfg.blockDim = dim3(kRowThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
