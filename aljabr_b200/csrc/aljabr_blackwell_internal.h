@@ -244,7 +244,7 @@ struct Kv4Rotate {
     int rope_positions, half, interleaved;
     int vec_q, vec_q_out;    // as rows.vec
     int span, splits;        // set by the launcher: q heads of a thread, threads a q row needs for all
-    unsigned int q_blocks;
+    unsigned int kv_step;    // 2^32 times the share of CTAs that have K and V
 };
 cudaError_t launch_kv4_rotate_append(const Kv4Rotate& a, int sms, cudaStream_t stream);
 // One token of a decode step: RoPE on q (in place) and k, then k and v (fp32, 16-byte aligned) into page 0 at *p.slots.

@@ -113,9 +113,9 @@ __device__ __forceinline__ void find_block(const Kv4Rows& p, int slot, Where& w)
 }
 
 template <int D>
-__device__ __forceinline__ bool place(const Kv4Rows& p, Where& w, unsigned int block) {
+__device__ __forceinline__ bool place(const Kv4Rows& p, Where& w) {
     constexpr int kLanes = D / 8;
-    const unsigned int row = block * (kRowThreads / kLanes) + threadIdx.x / kLanes;   // < 2^31: checked on the host
+    const unsigned int row = blockIdx.x * (kRowThreads / kLanes) + threadIdx.x / kLanes;   // < 2^31: checked on the host
     w.j = threadIdx.x % kLanes;
     w.token = row / static_cast<unsigned int>(p.kv_heads);
     w.head = row - w.token * p.kv_heads;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kRowThreads, 12) kv4_append_kernel(const Kv4Ro
     pdl_launch_dependents();
     pdl_wait();
     Where w;
-    const bool live = place<D>(p, w, blockIdx.x);
+    const bool live = place<D>(p, w);
     float k[8] = {}, v[8] = {};
     const bool write = live && w.block >= 0;
     if (write) {
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(const Kv4Rows p) 
     pdl_wait();
     constexpr int NG = D / 32;
     Where w;
-    if (!place<D>(p, w, blockIdx.x)) return;
+    if (!place<D>(p, w)) return;
     const int g = w.j >> 2, c = w.j & 3;
     float k[8] = {}, v[8] = {};
     if (w.block >= 0) {
@@ -250,28 +250,33 @@ __global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(const Kv4Rows p) 
 }
 
 // Rows of new tokens with the position rotation on the way: q is rotated into q_out, k before it is quantised; the
-// products and sums are rounded one by one, as in the decode step.  The first p.q_blocks CTAs have the q rows: a thread
-// owns two runs of 8 dims that are each other's pairs (split halves) or adjacent (interleaved, and what does not turn),
-// so nothing is exchanged, and keeps their 8 cosines and sines for p.span heads of its token.  The others have K and V,
-// laid out as in kv4_append_kernel for the groups' shuffles; there a split half's pairs come by shuffle too (which for
-// q cost 16384 tokens of 32 + 8 heads 141 us in all, as one CTA a token).
+// products and sums are rounded one by one, as in the decode step.  In the CTAs that have q rows a thread owns two runs
+// of 8 dims that are each other's pairs (split halves) or adjacent (interleaved, and what does not turn), so nothing is
+// exchanged, and keeps their 8 cosines and sines for p.span heads of its token.  The others have K and V, laid out as in
+// kv4_append_kernel for the groups' shuffles.  The former wait for memory, the latter (600 instructions a warp for
+// 2 KB) for issue slots, so they are spread among each other.
 template <typename T, int D>
-__device__ __forceinline__ void rotate_q(const Kv4Rotate& p) {
+__device__ __forceinline__ void rotate_q(const Kv4Rotate& p, unsigned int block) {
     constexpr int kLanes = D / 16, kPer = kRowThreads / kLanes;
-    const unsigned int row = blockIdx.x * kPer + threadIdx.x / kLanes;
+    const unsigned int row = block * kPer + threadIdx.x / kLanes;
     const int t = threadIdx.x % kLanes;
     const int token = row / static_cast<unsigned int>(p.splits);
     if (token >= p.rows.tokens) return;
     const int head0 = (row - token * p.splits) * p.span, heads = min(p.span, p.q_heads - head0);
-    int pos = __ldg(p.positions + token);
+    int pos = __ldg(p.positions + token);          // on its way while the first head is
+    const int half8 = p.half >> 3;                 // runs of 8 in half of the turning dims
+    // its runs: with split halves t and t + half8, behind the turning dims two neighbours
+    const int run0 = p.interleaved || t >= half8 ? 2 * t : t, run1 = p.interleaved || t >= half8 ? 2 * t + 1 : t + half8;
+    const T* q = static_cast<const T*>(p.q) + token * p.q_stride + head0 * D;
+    T* out = static_cast<T*>(p.q_out) + token * p.q_out_stride + head0 * D;
+    float a[8], b[8];
+    Wide<T>::load(q + 8 * run0, p.vec_q, a);
+    Wide<T>::load(q + 8 * run1, p.vec_q, b);
     if (pos >= p.rope_positions) {
         record_fault(ALJ_FAULT_BOUNDS);
         pos = -1;
     }
-    const int half8 = p.half >> 3;                 // runs of 8 in half of the turning dims
     const bool turns = t < half8 && pos >= 0;
-    // its runs: with split halves t and t + half8, behind the turning dims two neighbours
-    const int run0 = p.interleaved || t >= half8 ? 2 * t : t, run1 = p.interleaved || t >= half8 ? 2 * t + 1 : t + half8;
     float cs[8], sn[8];
     if (turns) {
         const float4* at = reinterpret_cast<const float4*>(p.rope + static_cast<long long>(pos) * p.half + 8 * t);
@@ -281,14 +286,15 @@ __device__ __forceinline__ void rotate_q(const Kv4Rotate& p) {
             cs[2 * i] = f.x, sn[2 * i] = f.y, cs[2 * i + 1] = f.z, sn[2 * i + 1] = f.w;
         }
     }
-    const T* q = static_cast<const T*>(p.q) + token * p.q_stride + head0 * D;
-    T* out = static_cast<T*>(p.q_out) + token * p.q_out_stride + head0 * D;
-#pragma unroll 2
+#pragma unroll 1
     for (int h = 0; h < heads; ++h, q += D, out += D) {
-        float a[8] = {}, b[8] = {};
-        if (pos >= 0) {
+        if (h > 0) {
             Wide<T>::load(q + 8 * run0, p.vec_q, a);
             Wide<T>::load(q + 8 * run1, p.vec_q, b);
+        }
+        if (pos < 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.0f;
         }
         if (turns && p.interleaved) {
 #pragma unroll
@@ -309,26 +315,44 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads) kv4_rotate_append_kernel(const Kv4Rotate p) {
     pdl_launch_dependents();
     pdl_wait();
-    if (blockIdx.x < p.q_blocks) {
-        rotate_q<T, D>(p);
+    // of every q_blocks + kv_blocks CTAs, kv_blocks evenly among the others
+    const unsigned int kv_block = __umulhi(blockIdx.x, p.kv_step);
+    if (__umulhi(blockIdx.x + 1, p.kv_step) == kv_block) {
+        rotate_q<T, D>(p, blockIdx.x - kv_block);
         return;
     }
+    // the rows are on their way while slots and positions are, whether they are used or not
+    constexpr int kLanes = D / 8;
     Where w;
-    const bool live = place<D>(p.rows, w, blockIdx.x - p.q_blocks);
-    int pos = live ? __ldg(p.positions + w.token) : -1;
+    const unsigned int row = kv_block * (kRowThreads / kLanes) + threadIdx.x / kLanes;
+    w.j = threadIdx.x % kLanes;
+    w.token = row / static_cast<unsigned int>(p.rows.kv_heads);
+    w.head = row - w.token * p.rows.kv_heads;
+    w.block = -1;
+    const bool live = w.token < p.rows.tokens;
+    const int half8 = p.half >> 3;
+    const bool second = !p.interleaved && w.j >= half8, in = w.j < 2 * half8;
+    float k[8] = {}, v[8] = {}, mate[8] = {};
+    int pos = -1;
+    if (live) {
+        const int slot = __ldg(p.rows.slots + w.token);
+        pos = __ldg(p.positions + w.token);
+        const T* const k_row = static_cast<const T*>(p.rows.k) + w.token * p.rows.k_stride + w.head * D;
+        Wide<T>::load(k_row + 8 * w.j, p.rows.vec, k);
+        // split halves: the dims that pair with these, which their own thread loads too
+        if (in && !p.interleaved) Wide<T>::load(k_row + 8 * (second ? w.j - half8 : w.j + half8), p.rows.vec, mate);
+        Wide<T>::load(static_cast<const T*>(p.rows.v) + w.token * p.rows.v_stride + w.head * D + 8 * w.j, p.rows.vec, v);
+        find_block<D>(p.rows, slot, w);
+    }
     if (pos >= p.rope_positions) {
         if (w.head == 0) record_fault(ALJ_FAULT_BOUNDS);
         pos = -1;
     }
-    float k[8] = {}, v[8] = {};
-    const bool write = live && w.block >= 0 && pos >= 0;
-    const int half8 = p.half >> 3;
-    const bool turns = write && w.j < 2 * half8, second = !p.interleaved && w.j >= half8;
+    const bool write = w.block >= 0 && pos >= 0, turns = write && in;
     float cs[8] = {}, sn[8] = {};
-    if (write) {
-        const int col = w.head * D + 8 * w.j;
-        Wide<T>::load(static_cast<const T*>(p.rows.k) + w.token * p.rows.k_stride + col, p.rows.vec, k);
-        Wide<T>::load(static_cast<const T*>(p.rows.v) + w.token * p.rows.v_stride + col, p.rows.vec, v);
+    if (!write) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.0f;
     }
     if (turns) {
         const int pair = p.interleaved ? 4 * w.j : 8 * (second ? w.j - half8 : w.j);
@@ -345,13 +369,9 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rotate_append_kernel(const Kv
 #pragma unroll
             for (int i = 0; i < 4; ++i) turn_pair(k[2 * i], k[2 * i + 1], cs[i], sn[i]);
         }
-    } else {                                       // every lane takes part: a row's lanes turn together
-        const int lane = threadIdx.x & 31, partner = turns ? lane + (second ? -half8 : half8) : lane;
+    } else if (turns) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float other = __fmul_rn(__shfl_sync(0xffffffffu, k[i], partner), sn[i]), own = __fmul_rn(k[i], cs[i]);
-            if (turns) k[i] = second ? __fadd_rn(other, own) : __fsub_rn(own, other);
-        }
+        for (int i = 0; i < 8; ++i) k[i] = __fadd_rn(__fmul_rn(k[i], cs[i]), __fmul_rn(mate[i], second ? sn[i] : -sn[i]));
     }
     put8<D>(p.rows, w, write, k, v);               // a skipped row's zeros are not stored
     if (live && p.rows.k_out) {
@@ -467,9 +487,11 @@ cudaError_t launch_kv4_rotate_append(const Kv4Rotate& a, int sms, cudaStream_t s
     const int per_q = kRowThreads / (p.rows.head_dim / 16), per_kv = kRowThreads / (p.rows.head_dim / 8);
     p.span = tokens * ((p.q_heads + 3) / 4) / per_q >= 8LL * sms ? 4 : 1;
     p.splits = (p.q_heads + p.span - 1) / p.span;
-    p.q_blocks = static_cast<unsigned int>((tokens * p.splits + per_q - 1) / per_q);
+    const long long q_blocks = (tokens * p.splits + per_q - 1) / per_q, kv_blocks = (tokens * p.rows.kv_heads + per_kv - 1) / per_kv;
+    const long long blocks = q_blocks + kv_blocks;   // < 2^31: checked on the host
+    p.kv_step = static_cast<unsigned int>(((kv_blocks << 32) + blocks - 1) / blocks);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.q_blocks + static_cast<unsigned int>((tokens * p.rows.kv_heads + per_kv - 1) / per_kv));
+    cfg.gridDim = dim3(static_cast<unsigned int>(blocks));
     cfg.blockDim = dim3(kRowThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
