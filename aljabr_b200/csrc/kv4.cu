@@ -92,6 +92,36 @@ struct Wide<__nv_bfloat16> {
     }
 };
 
+// 8 elements as they are in memory, to be on their way in few registers.
+template <typename T>
+struct Raw {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ void load(const T* p, int vec) {
+        constexpr int kWords = 2 * sizeof(T);
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < kWords / 4; ++i) {
+                const uint4 a = __ldg(reinterpret_cast<const uint4*>(p) + i);
+                w[4 * i] = a.x, w[4 * i + 1] = a.y, w[4 * i + 2] = a.z, w[4 * i + 3] = a.w;
+            }
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = __float_as_uint(__ldg(p + i));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+                w[i] = __bfloat16_as_ushort(p[2 * i]) | static_cast<uint32_t>(__bfloat16_as_ushort(p[2 * i + 1])) << 16;
+        }
+    }
+    __device__ __forceinline__ void to(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
+            else v[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+        }
+    }
+};
+
 struct Where {          // one thread's place: token, head, 8 dims 8 j ..
     int token, head, j;
     long long block;    // its page's block for the head, in bytes; -1: skip
@@ -263,15 +293,15 @@ __device__ __forceinline__ void rotate_q(const Kv4Rotate& p, unsigned int block)
     const int token = row / static_cast<unsigned int>(p.splits);
     if (token >= p.rows.tokens) return;
     const int head0 = (row - token * p.splits) * p.span, heads = min(p.span, p.q_heads - head0);
-    int pos = __ldg(p.positions + token);          // on its way while the first head is
+    int pos = __ldg(p.positions + token);          // on its way while the first head is; then always the next one
     const int half8 = p.half >> 3;                 // runs of 8 in half of the turning dims
     // its runs: with split halves t and t + half8, behind the turning dims two neighbours
     const int run0 = p.interleaved || t >= half8 ? 2 * t : t, run1 = p.interleaved || t >= half8 ? 2 * t + 1 : t + half8;
     const T* q = static_cast<const T*>(p.q) + token * p.q_stride + head0 * D;
     T* out = static_cast<T*>(p.q_out) + token * p.q_out_stride + head0 * D;
-    float a[8], b[8];
-    Wide<T>::load(q + 8 * run0, p.vec_q, a);
-    Wide<T>::load(q + 8 * run1, p.vec_q, b);
+    Raw<T> next0, next1;
+    next0.load(q + 8 * run0, p.vec_q);
+    next1.load(q + 8 * run1, p.vec_q);
     if (pos >= p.rope_positions) {
         record_fault(ALJ_FAULT_BOUNDS);
         pos = -1;
@@ -288,9 +318,12 @@ __device__ __forceinline__ void rotate_q(const Kv4Rotate& p, unsigned int block)
     }
 #pragma unroll 1
     for (int h = 0; h < heads; ++h, q += D, out += D) {
-        if (h > 0) {
-            Wide<T>::load(q + 8 * run0, p.vec_q, a);
-            Wide<T>::load(q + 8 * run1, p.vec_q, b);
+        float a[8], b[8];
+        next0.to(a);
+        next1.to(b);
+        if (h + 1 < heads) {
+            next0.load(q + D + 8 * run0, p.vec_q);
+            next1.load(q + D + 8 * run1, p.vec_q);
         }
         if (pos < 0) {
 #pragma unroll
@@ -312,7 +345,7 @@ __device__ __forceinline__ void rotate_q(const Kv4Rotate& p, unsigned int block)
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowThreads) kv4_rotate_append_kernel(const Kv4Rotate p) {
+__global__ void __launch_bounds__(kRowThreads, 8) kv4_rotate_append_kernel(const Kv4Rotate p) {
     pdl_launch_dependents();
     pdl_wait();
     // of every q_blocks + kv_blocks CTAs, kv_blocks evenly among the others
