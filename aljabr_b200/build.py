@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import glob
 import os
+import shutil
 import subprocess
 import sys
 import tempfile
@@ -18,6 +19,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libaljabr_blackwell.so")
+CALLS = os.path.join(HERE, "tensor_calls.so")     # torch tensors to the C-ABI, for kv4.py
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -36,12 +38,34 @@ def sources() -> list[str]:
 
 
 def _stale() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(CALLS):
         return True
-    t = os.path.getmtime(LIB)
-    deps = sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) \
+    t = min(os.path.getmtime(LIB), os.path.getmtime(CALLS))
+    deps = sources() + [os.path.join(CSRC, "tensor_calls.cpp")] + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) \
         + glob.glob(os.path.join(ROOT, "include", "*.h"))
     return any(os.path.getmtime(p) > t for p in deps)
+
+
+def _build_calls(tmp: str) -> str:
+    """tensor_calls.cpp against the installed torch's headers (no CUDA code)."""
+    import sysconfig
+    import torch
+    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(shutil.which(os.environ.get("NVCC", "nvcc")))))
+    obj = os.path.join(tmp, "tensor_calls.o")
+    subprocess.check_call([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-c", os.path.join(CSRC, "tensor_calls.cpp"),
+                           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", inc,
+                           "-I", os.path.join(inc, "torch", "csrc", "api", "include"), "-I", sysconfig.get_paths()["include"],
+                           "-I", os.path.join(cuda, "include"), "-o", obj])
+    return obj
+
+
+def _link_calls(obj: str) -> str:
+    import torch
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    subprocess.check_call([os.environ.get("CXX", "g++"), "-shared", obj, "-o", CALLS + ".tmp", "-Wl,-rpath,$ORIGIN", "-L", HERE,
+                           "-l:" + os.path.basename(LIB), "-L", libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"])
+    return CALLS + ".tmp"
 
 
 def build(force: bool = False, verbose_ptxas: bool = False) -> str:
@@ -55,9 +79,11 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
             rdc = "false" if os.path.basename(src) in WHOLE else "true"
             subprocess.check_call([nvcc, *flags, f"-rdc={rdc}", "-c", src, "-o", obj])
             return obj
+        calls = pool.submit(_build_calls, tmp)
         objects = list(pool.map(compile_one, sources()))
         subprocess.check_call([nvcc, *flags, "-rdc=true", "-shared", *objects, "-o", LIB + ".tmp", "-ldl"])
-    os.replace(LIB + ".tmp", LIB)
+        os.replace(LIB + ".tmp", LIB)
+        os.replace(_link_calls(calls.result()), CALLS)
     return LIB
 
 

@@ -100,6 +100,7 @@ def new_output(shape, dtype, device, index: int, stream: int) -> torch.Tensor:
 
 
 _tree_work = {}     # (device, stream) -> workspace of attend_tree, of all caches: calls on one stream follow one another
+_kinds = {}         # shapes of caches
 _captured = {}      # (device, stream) -> capture id, its workspaces
 _kept = []          # workspaces of captures on streams given by handle
 
@@ -115,6 +116,12 @@ def bad(message: str) -> native.ProviderError:
     return native.ProviderError(native.ALJ_ERR_BAD_ARG, message)
 
 
+native.lib()
+try:
+    from . import tensor_calls
+except ImportError as e:
+    raise native.ProviderError(native.ALJ_ERR_NOT_INITIALIZED, f"tensor_calls.so is missing or not this torch's ({e}): run "
+                               "`python -m aljabr_b200.build`") from e
 _rotate_append = native.lib().aljabr_blackwell_kv4_rotate_append_dev
 _attend_tree = native.lib().aljabr_blackwell_kv4_tree_attention_dev
 _accept_tree = native.lib().aljabr_blackwell_kv4_accept_tree_dev
@@ -144,6 +151,9 @@ class Kv4Cache:
         self._append, self._read = lib.aljabr_blackwell_kv4_append_dev, lib.aljabr_blackwell_kv4_read_dev
         self._attend, self._work_size = lib.aljabr_blackwell_kv4_attention_dev, lib.aljabr_blackwell_kv4_attention_workspace_size
         self._row = kv_heads * head_dim
+        self._address = data.data_ptr()
+        # one object for all caches of a shape on a device
+        self._kind = _kinds.setdefault(k := (pages, page_size, kv_heads, head_dim, self._index), k)
         self._shape = (data.data_ptr(), pages, page_size, kv_heads, head_dim)
         self._buffers = {}   # stream -> workspace: calls on one stream never overlap
         self._work = {}      # (stream, q_len, q_heads) -> its address and size
@@ -201,6 +211,10 @@ class Kv4Cache:
         token is absent (its q is zero, nothing is stored).  rope: float32 [positions, n, 2] of (cos, sin), contiguous;
         a head's first 2 n dims turn, dims i and i + n a pair, or with `interleaved` 2 i and 2 i + 1.  q_out: of q's
         shape and type, its rows may be strided, q itself will do."""
+        got = tensor_calls.rotate_append(*self._shape, self._index, q, k, v, slots, positions, rope, interleaved, q_out, k_back, v_back,
+                                         stream)
+        if got is not NotImplemented:
+            return native.check(got) if type(got) is int else got
         n, dtype = slots.numel(), k.dtype
         kind = _DTYPES.get(dtype)
         if kind is None:
@@ -380,8 +394,13 @@ def accept_tree(caches, seq_lens: torch.Tensor, parents: torch.Tensor, drafted: 
     if not caches:
         raise bad("no caches")
     first = caches[0]
-    if any(c._shape[1:] != first._shape[1:] or c._index != first._index for c in caches):
+    kind = first._kind
+    addresses = [c._address for c in caches if c._kind is kind]
+    if len(addresses) != len(caches):
         raise bad("the caches of one call must have the same shape and device")
+    got = tensor_calls.accept_tree(addresses, *kind, seq_lens, parents, drafted, picked, block_table, out, stream)
+    if got is not NotImplemented:
+        return native.check(got) if type(got) is int else got
     if drafted.dim() != 2:
         raise bad("drafted must be int32 [batch, nodes]")
     batch, nodes = drafted.shape
@@ -395,7 +414,7 @@ def accept_tree(caches, seq_lens: torch.Tensor, parents: torch.Tensor, drafted: 
         table = ints(block_table, ((batch, max(width, 1)),), "block_table")
     path, count, token, lens = (ints(t, (s,), w) for t, s, w in zip(out, ((batch, nodes),) + ((batch,),) * 3,
                                                                     ("path", "count", "token", "lens")))
-    rc = _accept_tree(path, count, token, lens, (ctypes.c_void_p * len(caches))(*[c._shape[0] for c in caches]), len(caches),
+    rc = _accept_tree(path, count, token, lens, (ctypes.c_void_p * len(caches))(*addresses), len(caches),
                       *first._shape[1:], table, width, ints(seq_lens, ((batch,),), "seq_lens"), batch,
                       ints(parents, ((nodes,), (batch, nodes)), "parents"), nodes if parents.dim() == 2 else 0, nodes,
                       ints(drafted, ((batch, nodes),), "drafted"), ints(picked, ((batch, nodes),), "picked"), stream)
