@@ -303,7 +303,7 @@ struct Kv4Accept {
     int* token;              // [batch] picked after the path's last node, -1 where there is none
     int* new_lens;           // [batch]
 };
-cudaError_t launch_kv4_accept(const Kv4Accept& a, cudaStream_t stream);
+cudaError_t launch_kv4_accept(const Kv4Accept& a, int sms, cudaStream_t stream);
 
 // Logits step (logits.cu).
 struct LogitsArgs {

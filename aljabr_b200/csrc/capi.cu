@@ -1668,7 +1668,7 @@ int aljabr_blackwell_kv4_accept_tree_dev(int* path, int* count, int* token, int*
     int err = 0;
     DeviceState* st = state(&err);
     if (!st) return err;
-    return launch_status(launch_kv4_accept(a, pick_stream(st, stream)), "kv4_accept_tree");
+    return launch_status(launch_kv4_accept(a, st->sms, pick_stream(st, stream)), "kv4_accept_tree");
 }
 
 int aljabr_blackwell_stream_capture_id(void* stream, unsigned long long* id) {
