@@ -148,8 +148,9 @@ __device__ __forceinline__ uint32_t lds_word(uint32_t a) {
     return w;
 }
 // Waits with a limit, that also end once another role has given up.  The roles' loops have to share the instruction
-// cache, so these are kept short: a count of tries, each of which the hardware suspends for a while, in place of a clock.
-constexpr int kTries = 1 << 22;
+// cache, so these are kept short: a count of tries, each of which the hardware suspends for some microseconds, in place of
+// a clock.
+constexpr int kTries = 1 << 17;
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
     uint32_t ok;
     asm volatile(
@@ -239,10 +240,6 @@ __device__ __forceinline__ void tmem_ld8x2(uint32_t at0, uint32_t at1, uint32_t 
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
                  : "memory");
 }
 // d (+)= a b for 64 values of K (four MMAs, fp16): both operands in shared memory, or a in tensor memory.  The whole warp
@@ -408,10 +405,8 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
             mbar_init(s.k_full + i, 4);
             mbar_init(s.k_empty + i, 1);
         }
-        for (int i = 0; i < F::V_STAGES; ++i) {
-            mbar_init(s.v_full + i, 4);
-            mbar_init(s.v_empty + i, 1);
-        }
+        for (int i = 0; i < F::V_STAGES; ++i) mbar_init(s.v_full + i, 4);
+        for (int i = 0; i < 2; ++i) mbar_init(s.v_empty + i, 1);
         for (int i = 0; i < F::S_STAGES; ++i) {
             mbar_init(s.s_full + i, 1);
             mbar_init(s.p_full + i, 4);
@@ -895,9 +890,9 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 fence_proxy_shared();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s.k_full + ks);
-                if (F::V_STAGES == 1 && tile >= 2)                // a use of the other warpgroup's: none may be passed over
-                    ok = ok && warp_wait(s.v_empty, (tile - 2) & 1, gave_up);
-                if (tile >= F::V_STAGES) ok = ok && warp_wait(s.v_empty + vs, (tile / F::V_STAGES - 1) & 1, gave_up);
+                // A barrier for every second tile also where V has one place: a wait by parity has to see each phase of its
+                // barrier in turn, and the other warpgroup waits for the others.
+                if (const int u = tile - F::V_STAGES; u >= 0) ok = ok && warp_wait(s.v_empty + (u & 1), (u >> 1) & 1, gave_up);
                 if (!ok) break;
                 const uint32_t to = at_v + vs * F::VHAT + part * (D * 128);
 #pragma unroll 1
@@ -1117,7 +1112,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
 #pragma unroll
                     for (int h = 0; h < KT / 64; ++h)
                         mma64_ts(to, tmem + buf * KT + 32 * h, v + h * (D * 8), kO, h > 0 || i >= F::STREAMS, one);
-                    commit2(s.v_empty + vs, s.pv_done + buf, one);
+                    commit2(s.v_empty + (t & 1), s.pv_done + buf, one);
                 }
                 if (i + F::S_STAGES < pc.count) {
                     const int t = tile + i + F::S_STAGES, ks = t % F::K_STAGES, buf = t % F::S_STAGES;

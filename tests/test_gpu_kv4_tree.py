@@ -175,6 +175,28 @@ def test_tree_attention_matches_64_bits(D, hkv, G, ps, nodes, roots, absent, len
     assert fault_bits() == 0
 
 
+@pytest.mark.parametrize("D,hkv,G,nodes,lens", [(256, 1, 4, 10, [20000, 3]), (256, 2, 2, 64, [5000, 9000]), (128, 1, 8, 17, [30000, 700]),
+                                                (64, 2, 4, 30, [25000, 40]), (128, 1, 4, 40, [2000] * 40)])
+def test_long_contexts_and_many_pieces(D, hkv, G, nodes, lens):
+    """Every stage of the pipeline goes round many times, and items are cut over CTAs: against fp32 queries, whose kernel
+    is another.  The same queries, so what differs is bf16's rounding of the output and the fp16 operands: 2^-8 in norm."""
+    p = tree.grow(np.random.default_rng(50), nodes, 1, nodes // 9)
+    rng = np.random.default_rng(51)
+    per = -(-max(lens) // 64)
+    cache = make(len(lens) * per, 64, hkv, D)
+    order = rng.permutation(len(lens) * per).reshape(len(lens), per)
+    n = len(lens) * per * 64
+    k, v = (torch.randn(n, hkv, D, device="cuda", generator=torch.Generator("cuda").manual_seed(s)) for s in (1, 2))
+    cache.append(k, v, torch.arange(n, dtype=torch.int32, device="cuda"))
+    q = cuda(rng.normal(size=(len(lens), nodes, hkv * G, D)).astype(np.float32), torch.bfloat16)
+    args = ints(lens), ints(p), cuda(order.astype(np.int32))
+    want, got = cache.attend_tree(q.float(), *args).double(), cache.attend_tree(q, *args)
+    assert float((got.double() - want).norm()) <= 2.0 ** -8 * float(want.norm())
+    gone = [t for t, path in enumerate(tree.chains(p)) if not path]
+    assert not got[:, gone].any() and torch.equal(got, cache.attend_tree(q, *args))
+    assert fault_bits() == 0
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_one_tree_for_all_and_no_table(dtype):
     p = tree.grow(np.random.default_rng(1), 12)
