@@ -1217,6 +1217,25 @@ cudaError_t launch_tree(const Kv4Attn& p, Cut* cuts, int sms, unsigned int* faul
     return cudaLaunchKernelEx(&cfg, kv4_tree_join_kernel<F::D>, p, static_cast<const Cut*>(cuts), fault_word);
 }
 
+// Which kernel.  That of 8 or 16 columns (kv4_attention.cu) has all fp32 queries, since 16-bit operands would cost them
+// their accuracy.  For bf16 its time goes with the passes over the cache, one for every 16 rows (8 at D 256), and this
+// one's hardly with the rows, but this one takes 17 to 27 us for the smallest call.  Measured with 8 KV heads, us, the few
+// columns' first and this kernel's second:
+//   8 sequences of 16384:   16 rows, D 128: 73, 108   24: 125, 110   48: 182, 113   128: 455, 115
+//                           D 64: 45, 93   76, 93   107, 93   259, 94      D 256: 156, 253   226, 255   437, 262   1137, 271
+//   32 sequences of 1024:   32 rows, D 64, 128, 256: 38, 49   60, 61   116, 114     48 rows: 50, 50   82, 61   167, 116
+//   1 sequence of 4096:     48 rows, D 64, 128, 256: 16, 21   23, 23    29, 39     128 rows: 23, 22   32, 25    53, 40
+//   1 sequence of 257:     128 rows, D 64, 128, 256: 11, 19   12, 22    12, 29
+// So this kernel has more than 32 rows, where positions times heads, rows and dims reach 160 million (D 64 and 128; they
+// meet between 100 and 200) or 640 million (D 256; 500 to 750).  The lengths are on the GPU: what counts is what the block
+// table can hold, and short sequences in a wide table cost those 10 to 20 us more.
+bool tree_is_wide(const Kv4Attn& a) {
+    const long long rows = static_cast<long long>(a.q_len) * a.group;
+    if (a.type != ALJ_KV_BF16 || rows <= 32) return false;
+    const double positions = static_cast<double>(a.batch) * a.page_size * (a.table ? a.table_stride : 1);
+    return positions * a.kv_heads * rows * a.head_dim >= (a.head_dim == 256 ? 640e6 : 160e6);
+}
+
 }  // namespace
 
 size_t kv4_tree_workspace_bytes(int q_rows, int head_dim, int sms) {
@@ -1227,8 +1246,7 @@ size_t kv4_tree_workspace_bytes(int q_rows, int head_dim, int sms) {
 }
 
 cudaError_t launch_kv4_tree(const Kv4Attn& a, void* workspace, int sms, unsigned int* fault_word, cudaStream_t stream) {
-    // fp32 queries, and few rows, run on the kernel of 8 or 16 columns
-    if (a.type != ALJ_KV_BF16 || a.q_len * a.group <= 8) return launch_kv4_attention(a, workspace, sms, stream);
+    if (!tree_is_wide(a)) return launch_kv4_attention(a, workspace, sms, stream);
     Kv4Attn p = a;
     p.row_tiles = (p.q_len * p.group + kRows - 1) / kRows;
     p.group_magic = ((1u << 21) + p.group - 1) / p.group;   // row / group for row < 2048, exact as row * group < 2^21

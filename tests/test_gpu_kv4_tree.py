@@ -95,8 +95,14 @@ def test_positions_and_slots_outside_their_ranges_are_absent():
 
 
 # ---------------------------------------------------------------- attention
-def tree_case(seed, D, hkv, G, ps, lens, trees, dtype=torch.float32, paged=True, fill=0xFF, v_size=1.0):
-    """A cache whose unused bytes, absent nodes' rows among them, are `fill` (0xFF: scales that are NaN)."""
+def widen(t, ps):
+    """More columns of absent pages: room for 131072 positions a sequence."""
+    return np.pad(t, ((0, 0), (0, 131072 // ps - t.shape[1])), constant_values=-1)
+
+
+def tree_case(seed, D, hkv, G, ps, lens, trees, dtype=torch.float32, paged=True, fill=0xFF, v_size=1.0, wide=False):
+    """A cache whose unused bytes, absent nodes' rows among them, are `fill` (0xFF: scales that are NaN).  wide: a block
+    table of many more columns, for which more than 32 rows of bf16 run on the tensor cores' kernel."""
     rng = np.random.default_rng(seed)
     B, T = len(lens), len(trees[0])
     per = max(1, -(-max(lens) // ps))
@@ -121,7 +127,7 @@ def tree_case(seed, D, hkv, G, ps, lens, trees, dtype=torch.float32, paged=True,
         t = order.astype(np.int32)
         for b, n in enumerate(lens):
             t[b, -(-n // ps):] = -1
-        table = cuda(t)
+        table = cuda(widen(t, ps) if wide else t)
     return cache, q, ints(lens), ints(trees), table, k64, v64
 
 
@@ -147,6 +153,8 @@ def check(out, q, k64, v64, lens, trees, window=0, soft_cap=0.0):
     assert off <= size * (2.0 ** -8 if bf16 else 2.0 ** -18) ** 2, (off / size) ** 0.5
 
 
+# type, absent nodes behind the tree: fp32; bf16 on the kernel of few columns; bf16 on the tensor cores' kernel
+KERNELS = [(torch.float32, 0), (torch.bfloat16, 0), (torch.bfloat16, 60)]
 CASES = [
     # D, hkv, G, page size, nodes, roots, absent, lens, window, cap
     (128, 2, 4, 16, 1, 1, 0, [1, 40, 0], 0, 0.0),
@@ -164,12 +172,12 @@ CASES = [
 ]
 
 
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dtype,wide", [(torch.float32, False), (torch.bfloat16, False), (torch.bfloat16, True)])
 @pytest.mark.parametrize("D,hkv,G,ps,nodes,roots,absent,lens,window,cap", CASES)
-def test_tree_attention_matches_64_bits(D, hkv, G, ps, nodes, roots, absent, lens, window, cap, dtype):
+def test_tree_attention_matches_64_bits(D, hkv, G, ps, nodes, roots, absent, lens, window, cap, dtype, wide):
     rng = np.random.default_rng(nodes)
     trees = [tree.grow(rng, nodes, roots, absent) for _ in lens]
-    cache, q, sl, parents, table, k64, v64 = tree_case(D + G + nodes, D, hkv, G, ps, lens, trees, dtype)
+    cache, q, sl, parents, table, k64, v64 = tree_case(D + G + nodes, D, hkv, G, ps, lens, trees, dtype, wide=wide)
     out = cache.attend_tree(q, sl, parents, table, window=window, soft_cap=cap)
     check(out, q, k64, v64, lens, trees, window, cap)
     assert fault_bits() == 0
@@ -189,12 +197,103 @@ def test_long_contexts_and_many_pieces(D, hkv, G, nodes, lens):
     k, v = (torch.randn(n, hkv, D, device="cuda", generator=torch.Generator("cuda").manual_seed(s)) for s in (1, 2))
     cache.append(k, v, torch.arange(n, dtype=torch.int32, device="cuda"))
     q = cuda(rng.normal(size=(len(lens), nodes, hkv * G, D)).astype(np.float32), torch.bfloat16)
-    args = ints(lens), ints(p), cuda(order.astype(np.int32))
+    args = ints(lens), ints(p), cuda(widen(order.astype(np.int32), 64))
     want, got = cache.attend_tree(q.float(), *args).double(), cache.attend_tree(q, *args)
     assert float((got.double() - want).norm()) <= 2.0 ** -8 * float(want.norm())
     gone = [t for t, path in enumerate(tree.chains(p)) if not path]
     assert not got[:, gone].any() and torch.equal(got, cache.attend_tree(q, *args))
     assert fault_bits() == 0
+
+
+def test_more_sequences_than_threads():
+    """1400 sequences, some of no length; against fp32, as in the test before."""
+    rng = np.random.default_rng(52)
+    lens = rng.integers(0, 130, 1400)
+    p = tree.grow(rng, 12, 2, 1)
+    cache, q, sl, parents, table, _, _ = tree_case(53, 128, 1, 4, 64, lens.tolist(), [p] * 1400, torch.bfloat16)
+    want, got = cache.attend_tree(q.float(), sl, parents, table).double(), cache.attend_tree(q, sl, parents, table)
+    assert float((got.double() - want).norm()) <= 2.0 ** -8 * float(want.norm())
+    assert torch.equal(got == 0, want == 0) and fault_bits() == 0
+
+
+@pytest.mark.parametrize("dtype,pad", KERNELS)
+def test_queries_of_a_wider_buffer_and_any_scale(dtype, pad):
+    """Rows at offsets that are no multiple of 16 bytes; scales of 0 and below; the same results as contiguous rows."""
+    p = tree.grow(np.random.default_rng(54), 20) + [-2] * pad
+    T = len(p)
+    cache, q, sl, parents, table, k64, v64 = tree_case(54, 64, 2, 2, 16, [90 + pad, 300 + pad], [p] * 2, dtype, wide=True)
+    for scale in (None, 0.0, -0.07):
+        want = cache.attend_tree(q, sl, parents, table, scale=scale)
+        for cut in (0, 1, 4, 8):
+            wide = torch.full((2 * T, 256 + 11), float("nan"), device="cuda", dtype=dtype)
+            view = wide[:, cut:cut + 256]
+            view.copy_(q.view(2 * T, 256))
+            assert torch.equal(cache.attend_tree(view.view(2, T, 4, 64), sl, parents, table, scale=scale), want)
+    check(cache.attend_tree(q, sl, parents, table, scale=-0.125), -q, k64, v64, [90 + pad, 300 + pad], [p] * 2)
+    assert fault_bits() == 0
+
+
+@pytest.mark.parametrize("nodes,lens", [(10, [4000]), (40, [4000, 900, 3000])])
+def test_two_graphs_and_calls_at_once(nodes, lens):
+    """Two captured graphs and eager calls on three streams, all in flight together: none uses another's workspace."""
+    p = tree.grow(np.random.default_rng(55), nodes)
+    cases = [tree_case(56 + i, 128, 2, 4, 64, lens, [p] * len(lens), torch.bfloat16, wide=True) for i in range(3)]
+    want = [c[0].attend_tree(*c[1:5]) for c in cases]
+    out = [torch.empty_like(w) for w in want]
+    torch.cuda.synchronize()
+    streams, graphs = [torch.cuda.Stream() for _ in cases], []
+    for c, o in zip(cases[:2], out):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=streams[0]):
+            for _ in range(3):
+                c[0].attend_tree(*c[1:5], out=o)
+    for _ in range(20):
+        for o in out:
+            o.fill_(7)
+        torch.cuda.synchronize()
+        for g, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            for _ in range(3):
+                cases[2][0].attend_tree(*cases[2][1:5], out=out[2])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, out))
+    assert fault_bits() == 0
+
+
+def test_calls_of_two_threads():
+    """On one stream, whose workspace they share, and on two."""
+    import threading
+    p = tree.grow(np.random.default_rng(57), 20)
+    cases = [tree_case(58 + i, 128, 2, 4, 64, [3000, 500], [p] * 2, torch.bfloat16, wide=True) for i in range(2)]
+    want = [c[0].attend_tree(*c[1:5]) for c in cases]
+    torch.cuda.synchronize()
+    for streams in ([torch.cuda.Stream()] * 2, [torch.cuda.Stream(), torch.cuda.Stream()]):
+        outs = [[torch.empty_like(w) for _ in range(30)] for w in want]
+
+        def work(i):
+            for o in outs[i]:
+                cases[i][0].attend_tree(*cases[i][1:5], out=o, stream=streams[i].cuda_stream)
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for os, w in zip(outs, want) for o in os)
+    assert fault_bits() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_window_far_shorter_than_the_context(dtype):
+    for window in (1, 5, 200, 4000):
+        rng = np.random.default_rng(window)
+        trees = [tree.grow(rng, 40, 1, 4) for _ in range(2)]
+        lens = [5000, 130]
+        cache, q, sl, parents, table, k64, v64 = tree_case(59, 128, 1, 4, 64, lens, trees, dtype, wide=True)
+        check(cache.attend_tree(q, sl, parents, table, window=window), q, k64, v64, lens, trees, window)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -218,12 +317,12 @@ def test_a_chain_is_attend():
         assert float((out - near).norm() / near.norm()) < 2.0 ** -18
 
 
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_nan_rows_of_other_branches_do_not_leak(dtype):
+@pytest.mark.parametrize("dtype,pad", KERNELS)
+def test_nan_rows_of_other_branches_do_not_leak(dtype, pad):
     """A node's row of NaN reaches the node and what descends from it; one before the window reaches nothing."""
-    p = [-1, 0, 0, 1, 2, 2, 3]
-    lens = [200]
-    cache, q, sl, parents, table, k64, v64 = tree_case(7, 128, 2, 4, 16, lens, [p], dtype)
+    p = [-1, 0, 0, 1, 2, 2, 3] + [-2] * pad
+    lens = [200 + pad]
+    cache, q, sl, parents, table, k64, v64 = tree_case(7, 128, 2, 4, 16, lens, [p], dtype, wide=True)
     clean = cache.attend_tree(q, sl, parents, table, window=50)
     bad = torch.full((2, 2, 128), float("nan"), device="cuda")
     cache.append(bad, bad, ints([int(table[0, w // 16]) * 16 + w % 16 for w in (100, 193 + 1)]))
@@ -232,10 +331,10 @@ def test_nan_rows_of_other_branches_do_not_leak(dtype):
     assert torch.equal(out[0, [0, 2, 4, 5]], clean[0, [0, 2, 4, 5]])
 
 
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_a_nan_group_of_v_stays_in_its_dims_and_branch(dtype):
-    p = [-1, 0, 0, 1]
-    cache, q, sl, parents, table, k64, v64 = tree_case(8, 128, 1, 2, 16, [40], [p], dtype)
+@pytest.mark.parametrize("dtype,pad", KERNELS)
+def test_a_nan_group_of_v_stays_in_its_dims_and_branch(dtype, pad):
+    p = [-1, 0, 0, 1] + [-2] * pad
+    cache, q, sl, parents, table, k64, v64 = tree_case(8, 128, 1, 2, 16, [40 + pad], [p], dtype, wide=True)
     clean = cache.attend_tree(q, sl, parents, table)
     for at, rows in ((37, [1, 3]), (20, [0, 1, 2, 3])):
         slot = ints([int(table[0, at // 16]) * 16 + at % 16])
@@ -252,18 +351,18 @@ def test_a_nan_group_of_v_stays_in_its_dims_and_branch(dtype):
         assert float((out - clean)[..., keep].double().norm()) <= 2 * tol * float(clean.double().norm())
 
 
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dtype,pad", KERNELS)
 @pytest.mark.parametrize("factor", [0.0, 1e-30, 1e-6, 1e6])
-def test_queries_of_any_size(factor, dtype):
-    p = tree.grow(np.random.default_rng(9), 20)
-    cache, q, sl, parents, table, k64, v64 = tree_case(9, 128, 2, 2, 16, [150], [p], dtype)
+def test_queries_of_any_size(factor, dtype, pad):
+    p = tree.grow(np.random.default_rng(9), 20) + [-2] * pad
+    cache, q, sl, parents, table, k64, v64 = tree_case(9, 128, 2, 2, 16, [150 + pad], [p], dtype, wide=True)
     q = (q.float() * factor).to(dtype)
     out = cache.attend_tree(q, sl, parents, table)
     if factor < 1e5:
-        check(out, q, k64, v64, [150], [p])
+        check(out, q, k64, v64, [150 + pad], [p])
     else:                                          # one position takes all: the largest score's V, where it leads by far
         qn = q.double().cpu().numpy()[0]
-        for t, rows in enumerate(tree.visible(p, 150)):
+        for t, rows in enumerate(tree.visible(p, 150 + pad)[:20]):
             for h in range(4):
                 s = k64[0][rows, h // 2] @ qn[t, h]
                 if np.sort(s)[-1] - (np.sort(s)[-2] if len(s) > 1 else -np.inf) > 2.0 ** -8 * np.abs(s).max():
@@ -271,25 +370,25 @@ def test_queries_of_any_size(factor, dtype):
                     assert np.abs(out[0, t, h].double().cpu().numpy() - want).max() <= 2.0 ** -8 * np.abs(want).max()
 
 
+@pytest.mark.parametrize("dtype,pad", KERNELS)
 @pytest.mark.parametrize("size", [1e-6, 1e-3, 3e4])
-def test_values_of_any_size(size):
-    p = tree.grow(np.random.default_rng(10), 40)
-    for dtype in (torch.float32, torch.bfloat16):
-        cache, q, sl, parents, table, k64, v64 = tree_case(10, 128, 1, 4, 16, [300], [p], dtype, v_size=size)
-        check(cache.attend_tree(q, sl, parents, table), q, k64, v64, [300], [p])
+def test_values_of_any_size(size, dtype, pad):
+    p = tree.grow(np.random.default_rng(10), 40) + [-2] * pad
+    cache, q, sl, parents, table, k64, v64 = tree_case(10, 128, 1, 4, 16, [300 + pad], [p], dtype, v_size=size, wide=pad > 0)
+    check(cache.attend_tree(q, sl, parents, table), q, k64, v64, [300 + pad], [p])
 
 
-def test_non_finite_queries_stay_in_their_rows():
-    for dtype in (torch.float32, torch.bfloat16):
-        p = tree.grow(np.random.default_rng(11), 9)
-        cache, q, sl, parents, table, _, _ = tree_case(11, 128, 2, 4, 16, [70], [p], dtype)
-        out = cache.attend_tree(q, sl, parents, table)
-        bad = q.clone()
-        bad[0, 3, 1, 5], bad[0, 4, 6, 0] = float("nan"), float("inf")
-        got = cache.attend_tree(bad, sl, parents, table)
-        hit = torch.zeros(9, 8, dtype=torch.bool)
-        hit[3, 1] = hit[4, 6] = True
-        assert torch.isnan(got[0][hit]).all() and torch.equal(got[0][~hit], out[0][~hit])
+@pytest.mark.parametrize("dtype,pad", KERNELS)
+def test_non_finite_queries_stay_in_their_rows(dtype, pad):
+    p = tree.grow(np.random.default_rng(11), 9) + [-2] * pad
+    cache, q, sl, parents, table, _, _ = tree_case(11, 128, 2, 4, 16, [70 + pad], [p], dtype, wide=True)
+    out = cache.attend_tree(q, sl, parents, table)
+    bad = q.clone()
+    bad[0, 3, 1, 5], bad[0, 4, 6, 0] = float("nan"), float("inf")
+    got = cache.attend_tree(bad, sl, parents, table)
+    hit = torch.zeros(9 + pad, 8, dtype=torch.bool)
+    hit[3, 1] = hit[4, 6] = True
+    assert torch.isnan(got[0][hit]).all() and torch.equal(got[0][~hit], out[0][~hit])
 
 
 def test_what_is_no_tree_is_absent_and_reported():
