@@ -334,6 +334,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
     // prefix of chunks and item costs
     const int cap = static_cast<int>(min(p.table ? static_cast<long long>(p.table_stride) * p.page_size : p.page_size, 0x7fffff00LL));
     int total = 0;                                 // < 2^31: checked on the host for the longest sequences
+    bool longer = false;                           // than an item that is left whole
     for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
         const int b = b0 + threadIdx.x;
         int n = 0;
@@ -346,6 +347,7 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
             if (TREE && len < p.q_len) len = 0;    // no tree is there
             s_len[b] = len;
             n = chunks_of(p, len) + kItemCost;
+            longer |= n > kItemCost + kWholeItem;
         }
         int incl = n;
 #pragma unroll
@@ -366,15 +368,18 @@ __global__ void __launch_bounds__(kThreads, NG * CT <= 4 ? 2 : 1) kv4_attn_kerne
         if (b < p.batch) s_pre[b + 1] = base + incl;
     }
     if (threadIdx.x == 0) s_pre[0] = 0;
-    __syncthreads();
+    if (TREE) longer = __syncthreads_or(longer);
+    else __syncthreads();
     const Tables tab = {s_pre, s_len};
     // A chunk costs a CTA about as much as 25 parts cost the one that joins them, so where the line is short an item
     // of n places is cut into stretches of sqrt(n / 25): one kv head of 32768 positions 23 us with 256 CTAs of a
     // chunk each, 16 so.  The join itself costs as much as three chunks, so items of up to kWholeItem chunks are left
     // whole: 257 positions 9.1 us in three parts, 7.4 whole.  n is the average item: among short sequences a long one
-    // is cut as they are, and dealt out over the CTAs all the same.
+    // is cut as they are, and dealt out over the CTAs all the same.  Of trees, whose items begin with a table of what
+    // each row sees and which come with more rows, all have to be that short: 5 ragged sequences within a window of
+    // 1024, 12 heads on 4, 21 nodes 25 us by the average and 20 so.
     const int width = (total + p.batch - 1) / p.batch;
-    const int stretch = width <= kItemCost + kWholeItem ? width : max(1, __float2int_rn(sqrtf(width / 25.0f)));
+    const int stretch = (TREE ? !longer : width <= kItemCost + kWholeItem) ? width : max(1, __float2int_rn(sqrtf(width / 25.0f)));
     total *= items;
     const int ctas = min(static_cast<int>(gridDim.x), (total + stretch - 1) / stretch);
     if (static_cast<int>(blockIdx.x) >= ctas) return;

@@ -15,7 +15,7 @@
 //     step; the output's own rounding is 2^-8).
 //   * V: the same, transposed on the way (a row is a dim, 8 positions 16 bytes): a
 //     word of two positions' codes is put together by one PRMT, as the codes of
-//     four dims lie in a halfword.  Its e, one of 64 positions, goes into P.
+//     four dims lie in a halfword.  Its e, one of 32 positions too, goes into P.
 //   * Q: scaled by a power of two into fp16's range, exact for bf16 to 2^-38 of
 //     the row's largest.
 //   * P = 2^(S - M + b + e - E) in fp16: M the running maximum, raised when a
@@ -26,15 +26,19 @@
 //   * A V group that is NaN counts as zeros in the product, and as NaN for the
 //     rows that see it: a product with a masked position's zero would be NaN too.
 //
-// Roles (one CTA an SM, persistent over the line of chunks as in
-// kv4_attention.cu): a producer warp (bulk copies of a tile's codes and scales
-// into a ring), two that find the exponents e, two warpgroups that decode, a tile each in turn,
-// one that issues the MMAs, and a warpgroup of softmax for each of two streams: the even and the odd
-// tiles of an item have their own S, running maximum and O, so that one stream's
-// softmax runs beside the other's products.  (D 256: tiles of 64, one stream, as
-// two O do not fit tensor memory beside S.)  The streams are joined when the item
-// ends; items cut over CTAs are joined by a second small kernel, which all SMs
-// share (one CTA joining 128 rows of 10 parts would read 0.6 MB by itself).
+// Roles (one CTA an SM, persistent over a line of tiles that is cut into equal parts): a producer warp (bulk copies of a
+// tile's codes and scales into a ring), two that find the exponents e of K and V, two warpgroups that decode, a tile each
+// in turn, one warp that issues the MMAs, and a warpgroup of softmax for each of two streams: the even and the odd tiles
+// of an item have their own S, running maximum and O, so that one stream's softmax runs beside the other's products.
+// (D 256: tiles of 64, one stream, as two O do not fit tensor memory beside S.)  The streams are joined when the item
+// ends; items cut over CTAs are joined by a second small kernel, which all SMs share (one CTA joining 128 rows of 10 parts
+// would read 0.6 MB by itself).
+//
+// What bounds it: the issue of instructions, most of them of the decoding and of the softmax.  A tile of 128 positions and
+// 128 rows takes about 7700 warp instructions and 3400 cycles: 64 % of the issue slots at 20 warps an SM, the tensor pipe
+// 35 % of the time, DRAM 14 %.  2 sequences of 65536, 64 query heads on 8, 61 nodes: 390 to 410 us, 650 TFLOP/s; 24 ragged
+// sequences up to 16384 with 26 nodes: 118 us.  Tried and slower for the first: tiles of 64 with 10 stages of codes (472 us),
+// 8 warps for V (465), one stage of K and four of codes (398 against 388 then).
 #define ALJ_OWN_FAULT_WORD     // compiled by itself, for setmaxnreg (build.py)
 #include "kv4.cuh"
 #include "tc_gemm.cuh"
@@ -46,8 +50,12 @@ namespace {
 
 constexpr int kRows = 128;
 constexpr int kPages = 128;           // page ids read from the table at once
-constexpr int kItemCost = 8;          // tiles that an item's start and end are worth
-constexpr int kLeast = 3;             // places of a CTA: fewer, and joining them costs more than it saves
+// Tiles that an item's start and end are worth on the line.  24 ragged sequences up to 16384, 26 nodes, us: 2 tiles 176,
+// 4 136, 6 126, 8 118, 10 120, 12 123, 16 131.
+constexpr int kItemCost = 8;
+// Places of a CTA: with fewer, joining them costs more than it saves.  1 sequence of 4096, 64 nodes, us: 2 places 29.9,
+// 3 28, 4 29.2, 6 32.1, 8 36.
+constexpr int kLeast = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -3.4e38f;     // running maximum of a row that has seen nothing
 // P <= 2^(kLazy + kSlack + kBias) = 2^15, or its sum over 32 positions <= kMostSum
