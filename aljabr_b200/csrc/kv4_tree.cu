@@ -35,7 +35,7 @@
 // would read 0.6 MB by itself).
 //
 // What bounds it: the issue of instructions, most of them of the decoding and of the softmax.  A tile of 128 positions and
-// 128 rows takes about 7700 warp instructions and 3400 cycles: 64 % of the issue slots at 20 warps an SM, the tensor pipe
+// 128 rows takes about 7400 warp instructions and 3400 cycles: 64 % of the issue slots at 20 warps an SM, the tensor pipe
 // 35 % of the time, DRAM 14 %.  2 sequences of 65536, 64 query heads on 8, 61 nodes: 390 to 410 us, 650 TFLOP/s; 24 ragged
 // sequences up to 16384 with 26 nodes: 118 us.  Tried and slower for the first: tiles of 64 with 10 stages of codes (472 us),
 // 8 warps for V (465), one stage of K and four of codes (398 against 388 then).

@@ -73,6 +73,7 @@ PyObject* rotate_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor *q = tensor(a[6]), *k = tensor(a[7]), *v = tensor(a[8]), *slots = tensor(a[9]), *positions = tensor(a[10]), *rope = tensor(a[11]);
     if (!q || !k || !slots || !rope || slots->dim() != 1 || q->dim() != 3 || rope->dim() != 3) return no();
     const int64_t tokens = slots->size(0), q_heads = q->size(1);
+    if (tokens > INT32_MAX || rope->size(0) > INT32_MAX) return no();
     const at::ScalarType type = k->scalar_type();
     if ((type != at::kFloat && type != at::kBFloat16) || !ints(slots, index, {tokens}) || !ints(positions, index, {tokens})) return no();
     const long long qs = rows(q, index, type, tokens, q_heads, D, false), ks = rows(k, index, type, tokens, heads, D, true),

@@ -227,6 +227,8 @@ class Kv4Cache:
         if rope.dtype is not torch.float32 or rope.dim() != 3 or rope.shape[2] != 2 or rope.get_device() != self._index or \
                 not rope.is_contiguous():
             raise bad(f"rope must be contiguous float32 [positions, pairs, 2] on {self.device}")
+        if max(n, rope.shape[0]) > 0x7FFFFFFF:       # ctypes would take their low 32 bits
+            raise bad(f"{n} tokens, {rope.shape[0]} positions of rope: each at most 2^31 - 1")
         kb = None if k_back is None else self._dense(k_back, n, dtype, "k_back")
         vb = None if v_back is None else self._dense(v_back, n, dtype, "v_back")
         stream = stream or current_stream(self._index)

@@ -407,6 +407,36 @@ def test_what_is_no_tree_is_absent_and_reported():
     assert not cache.attend_tree(q, ints([-5]), parents, table).any() and fault_bits() & 2
 
 
+def test_pages_lengths_and_parents_outside_their_ranges_on_both_kernels():
+    """A page that is not there reads as zeros, a length beyond the table as the table's, a wrong parent as an absent node:
+    bf16 on either kernel as fp32, within the output's rounding (2^-8 in norm)."""
+    p = tree.grow(np.random.default_rng(15), 30)
+    wrong = list(p)
+    wrong[7], wrong[20] = 7, 4000
+    cache, q, sl, parents, table, _, _ = tree_case(15, 128, 2, 4, 16, [300, 90], [p] * 2, torch.bfloat16, fill=0)
+    wide = cuda(widen(table.cpu().numpy(), 16))
+
+    def all_agree(lens, parents, edit=None):
+        outs = []
+        for x, t in ((q.float(), table), (q, table), (q, wide)):
+            t = t.clone()
+            if edit is not None:
+                t[0, 3], t[0, 10], t[1, 1] = edit
+            assert fault_bits() == 0
+            outs.append(cache.attend_tree(x, lens, parents, t).double())
+            assert fault_bits() & 2
+        for o in outs[1:]:
+            assert float((o - outs[0]).norm()) <= 2.0 ** -8 * float(outs[0].norm())
+
+    for bad in (-1, cache.pages, 2 ** 31 - 1):
+        all_agree(sl, parents, (bad, bad, bad))
+    all_agree(sl, ints([wrong, p]))
+    cut = table.shape[1] * 16
+    assert not cache.attend_tree(q, ints([-1, -2 ** 31]), parents, wide).any() and fault_bits() & 2
+    outs = [cache.attend_tree(x, ints([cut + 1, 90]), parents, table) for x in (q.float(), q)]
+    assert fault_bits() & 2 and float((outs[1].double() - outs[0].double()).norm()) <= 2.0 ** -8 * float(outs[0].double().norm())
+
+
 # ---------------------------------------------------------------- acceptance
 def read_all(cache):
     return cache.data.cpu().numpy().copy()
