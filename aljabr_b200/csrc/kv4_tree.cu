@@ -105,8 +105,6 @@ struct Small {                        // behind the tiles in shared memory
     int e_top[kMeta];
     int nan_any[kMeta];               // and V groups that are NaN: bits by position
     uint8_t nan[kMeta][F::KT];
-    int sum[32];                      // prefix sums, and where this CTA starts
-    int start[4];
     uint32_t node_ok[kKv4TreeWords];  // the producer's
     int pages[kPages];
     short par_p[kKv4MaxNodes];
@@ -438,33 +436,27 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
 
     // ---------------------------------------------------------- this CTA's part of the line
     const int items = p.kv_heads * p.row_tiles;
-    auto scan = [&](int n, int before, int& incl) {   // inclusive prefix sum of the threads' n, behind `before`; their total
-        incl = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += up;
-        }
-        __syncthreads();
-        if (lane == 31) s.sum[warp] = incl;
-        __syncthreads();
-        int total = 0;
-        incl += before;
-        for (int w = 0; w < F::WARPS; ++w) {
-            if (w < warp) incl += s.sum[w];
-            total += s.sum[w];
-        }
-        return total;
-    };
+    // Each warp adds the sequences up for itself, 32 at a time: nothing to wait for but their lengths.
     auto width_of = [&](int b) {
         bool bad = false;
         const int n = b < p.batch ? chunks_of<KT>(p, length_of(p, b, bad)) + kItemCost : 0;
-        if (bad && blockIdx.x == 0) record_fault(ALJ_FAULT_BOUNDS);
+        if (bad && blockIdx.x == 0 && warp == 0) record_fault(ALJ_FAULT_BOUNDS);
         return n;
     };
-    int total = 0, incl;
-    int mine = 0;                     // the thread's sequence's places
-    for (int b0 = 0; b0 < p.batch; b0 += F::THREADS) total += scan(mine = width_of(b0 + threadIdx.x), 0, incl);
+    auto scan = [&](int n) {          // inclusive prefix sums of the lanes' n
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, n, o);
+            if (lane >= o) n += up;
+        }
+        return n;
+    };
+    int total = 0, mine = 0, incl = 0;                    // the lane's sequence's places, and those up to its end
+#pragma unroll 1
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        incl = scan(mine = width_of(b0 + lane));
+        total += __shfl_sync(0xffffffffu, incl, 31);
+    }
     total *= items;                   // < 2^31: checked on the host for the longest sequences
     const int ctas = min(static_cast<int>(gridDim.x), (total + kLeast - 1) / kLeast);
     const int share = total / ctas, rem = total - share * ctas;
@@ -475,21 +467,24 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
     };
     if (threadIdx.x == 0) cuts[blockIdx.x].n = 0;
     Line line = {};
+    int my_pre = 0;                   // places before the sequence of the first piece
     if (static_cast<int>(blockIdx.x) < ctas) {
         const int x0 = start_of(blockIdx.x), x1 = start_of(blockIdx.x + 1);
         int before = 0;               // line places before the sequences at hand, of one item
-        for (int b0 = 0; b0 < p.batch; b0 += F::THREADS) {
-            if (p.batch > F::THREADS) before += scan(mine = width_of(b0 + threadIdx.x), before, incl);
-            const int pre = incl - mine;
-            if (mine > 0 && pre * items <= x0 && x0 < incl * items) {
-                s.start[0] = b0 + threadIdx.x;
-                s.start[1] = pre;
+#pragma unroll 1
+        for (int b0 = 0; b0 < p.batch; b0 += 32) {
+            if (p.batch > 32) incl = scan(mine = width_of(b0 + lane));
+            const int upto = before + incl, pre = upto - mine;
+            const uint32_t here = __ballot_sync(0xffffffffu, mine > 0 && pre * items <= x0 && x0 < upto * items);
+            if (here) {
+                line.b = b0 + __ffs(here) - 1;
+                my_pre = __shfl_sync(0xffffffffu, pre, __ffs(here) - 1);
+                break;
             }
+            before = __shfl_sync(0xffffffffu, upto, 31);
         }
-        __syncthreads();
-        line.b = s.start[0];
         load_seq<KT>(line, p);
-        const int pre = s.start[1], width = line.chunks + kItemCost, rest = x0 - pre * items;
+        const int width = line.chunks + kItemCost, rest = x0 - my_pre * items;
         line.h = rest / width;
         const int at = rest - line.h * width;
         line.ch = max(0, at - kItemCost);
@@ -509,9 +504,6 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         }
         line.left = n;
     }
-    // place of item h's first chunk on the line; only for the piece's own sequence
-    const int my_pre = static_cast<int>(blockIdx.x) < ctas ? s.start[1] : 0;
-
     const uint32_t at_q = smem_u32(smem), at_k = at_q + F::AT_K, at_v = at_q + F::AT_V, at_raw = at_q + F::AT_RAW;
     Piece pc;
     bool ok = true;
@@ -544,6 +536,13 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                 r = (k * F::SOFT + warp) * kPer + lane / kChunks;
                 return at_q + (j >> 3) * (kRows * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4);
             };
+            constexpr int kPar = kKv4MaxNodes / (32 * F::SOFT);      // nodes a thread brings
+            int par[kPar];
+#pragma unroll
+            for (int k = 0; k < kPar; ++k) {
+                const int i = k * (32 * F::SOFT) + thread;
+                par[k] = i < p.q_len ? tree_parent(p.parents + static_cast<long long>(pc.b) * p.parents_stride, i) : 0;
+            }
             if (pc.count > 0) {
                 const bool wide = ((reinterpret_cast<uintptr_t>(p.q) | static_cast<uintptr_t>(p.q_stride * 2)) & 15) == 0;
 #pragma unroll 2
@@ -562,8 +561,8 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                     }
                 }
             }
-            for (int i = thread; i < p.q_len; i += 32 * F::SOFT)
-                s.par[i] = static_cast<short>(tree_parent(p.parents + static_cast<long long>(pc.b) * p.parents_stride, i));
+#pragma unroll
+            for (int k = 0; k < kPar; ++k) s.par[k * (32 * F::SOFT) + thread] = static_cast<short>(par[k]);
             sync();
             const int node = token_of(pc.row0 + row);
             int depth = 0;
