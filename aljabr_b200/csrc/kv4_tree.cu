@@ -1150,47 +1150,88 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
     }
 }
 
-// Items cut over CTAs: block (c, y) joins kJoinRows rows of the item that CTA c began and others went on with, in CTA order.
-constexpr int kJoinRows = 8;
+// Items cut over CTAs: kJoinRows rows of one item at a time are joined by a block, in CTA order.  Every block lists the items
+// that were cut, so that the grid is no larger than is resident at once; parts are asked for kJoinParts at a time.  What it
+// waits for is memory.  1 x 4096 with 64 nodes, 24 ragged sequences and 2 x 65536, us: a block for each CTA and 8 rows
+// 27.7, 114.4, 379; 8 rows here 27.1, 114.0, 376; 4 rows 26.2, 115.1, 377; 4 rows and 6 blocks an SM 27.4, 115.7, 378;
+// 8 rows and 3 blocks 27.2, 117.5, 384.
+constexpr int kJoinRows = 4, kJoinParts = 4, kJoinBlocks = 4;   // blocks an SM
 template <int D>
-__global__ void __launch_bounds__(256) kv4_tree_join_kernel(const Kv4Attn p, const Cut* cuts, unsigned int* fault_word) {
+__global__ void __launch_bounds__(256, kJoinBlocks) kv4_tree_join_kernel(const Kv4Attn p, const Cut* cuts, int ctas, unsigned int* fault_word) {
+    extern __shared__ int4 s_cut[];   // [ctas] first CTA, CTAs, sequence, item
+    __shared__ int s_warp[8];
     pdl_launch_dependents();
     pdl_wait();
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && *static_cast<volatile unsigned int*>(&g_fault_word) != 0u)
+    if (blockIdx.x == 0 && threadIdx.x == 0 && *static_cast<volatile unsigned int*>(&g_fault_word) != 0u)
         atomicOr(fault_word, atomicExch(&g_fault_word, 0u));   // what the attention recorded, to the library's word
-    const Cut cut = cuts[blockIdx.x];
-    if (cut.n <= 1) return;
-    const int kvh = cut.h / p.row_tiles, row0 = (cut.h - kvh * p.row_tiles) * kRows;
-    const int rows = min(kRows, p.q_len * p.group - row0);
-    const long long size = kRows * (D + 2);
-    auto base = [&](int k) { return p.part + (2 * (static_cast<long long>(blockIdx.x) + k) + (k == 0 ? 1 : 0)) * size; };
-    constexpr int kQuads = D / 4;
-    for (int i = threadIdx.x; i < kJoinRows * kQuads; i += 256) {
-        const int row = blockIdx.y * kJoinRows + i / kQuads, d = (i % kQuads) * 4;
-        if (row >= rows) break;
-        float top = kNone, L = 0.0f;
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (int k = 0; k < cut.n; ++k) {
-            const float* part = base(k);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + kRows * D + row * 2));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + row * D + d));
-            const float now = fmaxf(top, ml.x), f = ex2(top - now), g = ex2(ml.x - now);
-            top = now;
-            L = fmaf(L, f, ml.y * g);
-            sum.x = fmaf(sum.x, f, v.x * g);
-            sum.y = fmaf(sum.y, f, v.y * g);
-            sum.z = fmaf(sum.z, f, v.z * g);
-            sum.w = fmaf(sum.w, f, v.w * g);
+    int count = 0;                    // listed in the order of the CTAs: all blocks have to number them alike
+    for (int c0 = 0; c0 < ctas; c0 += 256) {
+        const int c = c0 + threadIdx.x, warp = threadIdx.x >> 5;
+        const Cut cut = c < ctas ? cuts[c] : Cut{};
+        const uint32_t is = __ballot_sync(0xffffffffu, cut.n > 1);
+        if (c0 > 0) __syncthreads();
+        if ((threadIdx.x & 31) == 0) s_warp[warp] = __popc(is);
+        __syncthreads();
+        int at = count + __popc(is & ((1u << (threadIdx.x & 31)) - 1u));
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            if (w < warp) at += s_warp[w];
+            count += s_warp[w];
         }
-        const float inv = 1.0f / L;
-        const bool none = L == 0.0f;
-        const __nv_bfloat162 a = __floats2bfloat162_rn(none ? 0.0f : sum.x * inv, none ? 0.0f : sum.y * inv);
-        const __nv_bfloat162 b = __floats2bfloat162_rn(none ? 0.0f : sum.z * inv, none ? 0.0f : sum.w * inv);
-        const int r = row0 + row, t = r / p.group, hd = r - t * p.group;
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) +
-                             (((static_cast<long long>(cut.b) * p.q_len + t) * p.kv_heads + kvh) * p.group + hd) * D + d;
-        *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        if (cut.n > 1) s_cut[at] = make_int4(c, cut.n, cut.b, cut.h);
+    }
+    __syncthreads();
+    const int groups = (min(kRows, p.q_len * p.group) + kJoinRows - 1) / kJoinRows, units = count * groups;
+    const long long size = kRows * (D + 2);
+    constexpr int kQuads = D / 4;
+#pragma unroll 1
+    for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const int4 cut = s_cut[unit / groups];
+        const int kvh = cut.w / p.row_tiles, row0 = (cut.w - kvh * p.row_tiles) * kRows;
+        const int rows = min(kRows, p.q_len * p.group - row0);
+#pragma unroll 1
+        for (int i = threadIdx.x; i < kJoinRows * kQuads; i += 256) {
+            const int row = (unit % groups) * kJoinRows + i / kQuads, d = (i % kQuads) * 4;
+            if (row >= rows) break;
+            float top = kNone, L = 0.0f;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+            for (int k0 = 0; k0 < cut.y; k0 += kJoinParts) {
+                float2 ml[kJoinParts];
+                float4 v[kJoinParts];
+#pragma unroll
+                for (int u = 0; u < kJoinParts; ++u) {
+                    const int k = k0 + u;
+                    const float* part = p.part + (2 * (static_cast<long long>(cut.x) + k) + (k == 0 ? 1 : 0)) * size;
+                    ml[u] = k < cut.y ? __ldcg(reinterpret_cast<const float2*>(part + kRows * D + row * 2)) : make_float2(kNone, 0.0f);
+                    v[u] = k < cut.y ? __ldcg(reinterpret_cast<const float4*>(part + row * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+                float now = top;
+#pragma unroll
+                for (int u = 0; u < kJoinParts; ++u) now = fmaxf(now, ml[u].x);
+                const float f = ex2(top - now);
+                top = now;
+                L *= f;
+                sum.x *= f, sum.y *= f, sum.z *= f, sum.w *= f;
+#pragma unroll
+                for (int u = 0; u < kJoinParts; ++u) {
+                    const float g = ex2(ml[u].x - now);
+                    L = fmaf(ml[u].y, g, L);
+                    sum.x = fmaf(v[u].x, g, sum.x);
+                    sum.y = fmaf(v[u].y, g, sum.y);
+                    sum.z = fmaf(v[u].z, g, sum.z);
+                    sum.w = fmaf(v[u].w, g, sum.w);
+                }
+            }
+            const float inv = 1.0f / L;
+            const bool none = L == 0.0f;
+            const __nv_bfloat162 a = __floats2bfloat162_rn(none ? 0.0f : sum.x * inv, none ? 0.0f : sum.y * inv);
+            const __nv_bfloat162 b = __floats2bfloat162_rn(none ? 0.0f : sum.z * inv, none ? 0.0f : sum.w * inv);
+            const int r = row0 + row, t = r / p.group, hd = r - t * p.group;
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) +
+                                 (((static_cast<long long>(cut.z) * p.q_len + t) * p.kv_heads + kvh) * p.group + hd) * D + d;
+            *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        }
     }
 }
 
@@ -1218,10 +1259,10 @@ cudaError_t launch_tree(const Kv4Attn& p, Cut* cuts, int sms, unsigned int* faul
     cfg.numAttrs = 1;
     cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_tree_kernel<NG>, p, cuts);
     if (e != cudaSuccess) return e;
-    cfg.gridDim = dim3(sms, (std::min(kRows, p.q_len * p.group) + kJoinRows - 1) / kJoinRows);
+    cfg.gridDim = dim3(kJoinBlocks * sms);
     cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, kv4_tree_join_kernel<F::D>, p, static_cast<const Cut*>(cuts), fault_word);
+    cfg.dynamicSmemBytes = sms * sizeof(int4);
+    return cudaLaunchKernelEx(&cfg, kv4_tree_join_kernel<F::D>, p, static_cast<const Cut*>(cuts), sms, fault_word);
 }
 
 // Which kernel.  That of 8 or 16 columns (kv4_attention.cu) has all fp32 queries, since 16-bit operands would cost them
