@@ -36,8 +36,8 @@
 //
 // What bounds it: the issue of instructions, most of them of the decoding and of the softmax.  A tile of 128 positions and
 // 128 rows takes about 7400 warp instructions and 3400 cycles: 64 % of the issue slots at 20 warps an SM, the tensor pipe
-// 35 % of the time, DRAM 14 %.  2 sequences of 65536, 64 query heads on 8, 61 nodes: 390 to 410 us, 650 TFLOP/s; 24 ragged
-// sequences up to 16384 with 26 nodes: 118 us.  Tried and slower for the first: tiles of 64 with 10 stages of codes (472 us),
+// 35 % of the time, DRAM 14 %.  2 sequences of 65536, 64 query heads on 8, 61 nodes: 377 to 411 us, 640 to 690 TFLOP/s; 24
+// ragged sequences up to 16384 with 26 nodes: 115 us.  Tried and slower for the first: tiles of 64 with 10 stages of codes (472 us),
 // 8 warps for V (465), one stage of K and four of codes (398 against 388 then).
 #define ALJ_OWN_FAULT_WORD     // compiled by itself, for setmaxnreg (build.py)
 #include "kv4.cuh"
@@ -1267,16 +1267,17 @@ cudaError_t launch_tree(const Kv4Attn& p, Cut* cuts, int sms, unsigned int* faul
 
 // Which kernel.  That of 8 or 16 columns (kv4_attention.cu) has all fp32 queries, since 16-bit operands would cost them
 // their accuracy.  For bf16 its time goes with the passes over the cache, one for every 16 rows (8 at D 256), and this
-// one's hardly with the rows, but this one takes 17 to 27 us for the smallest call.  Measured with 8 KV heads, us, the few
+// one's hardly with the rows, but this one takes 17 to 26 us for the smallest call.  Measured with 8 KV heads, us, the few
 // columns' first and this kernel's second:
-//   8 sequences of 16384:   16 rows, D 128: 73, 108   24: 125, 110   48: 182, 113   128: 455, 115
-//                           D 64: 45, 93   76, 93   107, 93   259, 94      D 256: 156, 253   226, 255   437, 262   1137, 271
-//   32 sequences of 1024:   32 rows, D 64, 128, 256: 38, 49   60, 61   116, 114     48 rows: 50, 50   82, 61   167, 116
-//   1 sequence of 4096:     48 rows, D 64, 128, 256: 16, 21   23, 23    29, 39     128 rows: 23, 22   32, 25    53, 40
-//   1 sequence of 257:     128 rows, D 64, 128, 256: 11, 19   12, 22    12, 29
-// So this kernel has more than 32 rows, where positions times heads, rows and dims reach 160 million (D 64 and 128; they
-// meet between 100 and 200) or 640 million (D 256; 500 to 750).  The lengths are on the GPU: what counts is what the block
-// table can hold, and short sequences in a wide table cost those 10 to 20 us more.
+//   8 sequences of 16384:   16 rows, D 128: 72, 107   24: 124, 107   48: 182, 108   128: 452, 111
+//                           D 64: 45, 90   75, 90   106, 91   258, 93      D 256: 155, 242   225, 243   434, 248   1130, 256
+//   32 sequences of 1024:   32 rows, D 64, 128, 256: 38, 47   60, 58   115, 112     48 rows: 50, 48   82, 60   166, 113
+//   1 sequence of 4096:     48 rows, D 64, 128, 256: 16, 19   23, 21    29, 33     128 rows: 23, 19   32, 21    52, 34
+//   1 sequence of 257:     128 rows, D 64, 128, 256: 11, 18   12, 20    12, 27
+// So this kernel has more than 32 rows, where positions times heads, rows and dims reach 160 million (D 64 and 128: 40 rows
+// of 8 sequences of 257, D 128, 22 and 21 us; 64 of D 64, 151 million, 11 and 19) or 640 million (D 256: 64 rows there 36 and
+// 38, 80 rows 43 and 38).  The lengths are on the GPU: what counts is what the block table can hold, and short sequences in
+// a wide table cost those 7 to 15 us more.
 bool tree_is_wide(const Kv4Attn& a) {
     const long long rows = static_cast<long long>(a.q_len) * a.group;
     if (a.type != ALJ_KV_BF16 || rows <= 32) return false;
