@@ -648,6 +648,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                         if (last < 0) return;
                         ok = ok && warp_wait(s.pv_done + last % F::S_STAGES, (last / F::S_STAGES) & 1, gave_up);
                         tcg::tc_fence_after();
+                        tcg::tmem_wait_st();                          // an earlier call's stores: loads do not wait for them
 #pragma unroll 1
                         for (int c = 0; c < 4 * NG; ++c) {
                             uint32_t v[8];
@@ -731,6 +732,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                             M = now;
                             l *= f;
                             rescale(f);
+                            if (c > 0) tcg::tmem_wait_st();           // P as it was stored or scaled last
                             const __half2 f2 = __float2half2_rn(f);
 #pragma unroll 1
                             for (int b = 0; b < 2 * c; ++b) {

@@ -1,0 +1,70 @@
+"""Attention of drafted trees where its steps meet their limits: scores and
+values that rise from chunk to chunk, scales far apart, pages given back, the
+row count at which the kernel changes."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests import kv4_ref as ref
+from tests import tree_ref as tree
+from tests.test_gpu_kv4 import fault_bits, make
+from tests.test_gpu_kv4_tree import check, cuda, ints, tree_case, widen
+
+pytestmark = pytest.mark.gpu
+
+
+def one_sequence(k, v, ps=64, wide=True):
+    """A cache that holds k, v [n][hkv][D] on pages in another order, its table, and the values it stands for."""
+    n, hkv, D = k.shape
+    per = -(-n // ps)
+    order = np.random.default_rng(n).permutation(per)
+    cache = make(per, ps, hkv, D)
+    at = np.arange(n)
+    cache.append(cuda(k), cuda(v), cuda((order[at // ps] * ps + at % ps).astype(np.int32)))
+    table = order[None].astype(np.int32)
+    return cache, cuda(widen(table, ps) if wide else table), ref.values(*ref.quantise(k)), ref.values(*ref.quantise(v))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rise", [6.0, 3.0, 40.0])
+def test_scores_and_values_that_rise_from_chunk_to_chunk(D, rise):
+    """Of 32 positions to the next the scores rise by 2^rise in the weights, and every 128 positions V's scales by 2^3, so
+    that the running maximum is raised up to four times a tile and what is summed up is scaled on the way.
+
+    The scores are exact: q is 1, K one value of a position in 32 dims, a multiple of a power of two.  So what may differ is fp32's
+    rounding of a score (to 2^-22 of the largest, twice), P and V in fp16 (2^-11 each) and the output's 2^-8."""
+    T, n = 72, 72 + 1024
+    p = tree.grow(np.random.default_rng(D), T)
+    rng = np.random.default_rng(60)
+    k = np.zeros((n, 1, D), np.float32)
+    unit = rise * np.log(2.0) / 32.0              # of a score without its scale; K takes 8 bits of it
+    unit = 2.0 ** np.floor(np.log2(unit)) * np.round(256 * unit / 2.0 ** np.floor(np.log2(unit))) / 256
+    level = np.minimum(np.arange(n) // 32, 32)
+    k[:, 0, 32:64] = level[:, None]
+    v = rng.normal(size=(n, 1, D)).astype(np.float32) * (2.0 ** (np.minimum(np.arange(n) // 128, 8) * 3 - 14.0))[:, None, None].astype(np.float32)
+    cache, table, k64, v64 = one_sequence(k, v)
+    assert np.array_equal(k64, k)                 # multiples of 1/8 of the level
+    q = torch.ones(1, T, 1, D, device="cuda", dtype=torch.bfloat16)
+    got = cache.attend_tree(q, ints([n]), ints([p]), table, scale=unit).double().cpu().numpy()[0, :, 0]
+    for t, rows in enumerate(tree.visible(p, n)):
+        s = (k64[rows, 0] @ np.ones(D)) * np.float64(np.float32(unit))
+        w = np.exp(s - s.max())
+        w /= w.sum()
+        want, weight = w @ v64[rows, 0], w @ np.abs(v64[rows, 0])
+        tol = weight * (2 * 2 * np.abs(s).max() * 2.0 ** -22 + 2.0 ** -10) + np.abs(want) * 2.0 ** -8 + n * 2.0 ** -24 * np.abs(v64[rows, 0]).max(0)
+        err = np.abs(got[t] - want)
+        assert np.all(err <= tol), (t, float((err / tol).max()))
+    assert fault_bits() == 0
+
+
+@pytest.mark.parametrize("nodes,G", [(32, 1), (33, 1), (16, 2), (17, 2), (4, 8), (5, 8)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_rows_at_which_the_kernel_changes(D, nodes, G):
+    """32 rows and the next count, in a table wide enough for either kernel."""
+    lens = [700, nodes, 260]
+    trees = [tree.grow(np.random.default_rng(63 + b), nodes, 1, nodes // 8) for b in range(3)]
+    cache, q, sl, parents, table, k64, v64 = tree_case(64, D, 2, G, 16, lens, trees, torch.bfloat16, wide=True)
+    for window in (0, 90):
+        check(cache.attend_tree(q, sl, parents, table, window=window), q, k64, v64, lens, trees, window)
+    assert fault_bits() == 0
