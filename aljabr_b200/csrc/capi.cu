@@ -122,7 +122,7 @@ struct DeviceState {
     std::mutex mu;                          // serialises the staging buffers of tb calls
     std::map<uintptr_t, Registered> reg;    // host base -> HBM copy
     std::mutex reg_mu;
-    std::mutex tree_mu;                     // keeps the launches of one tree attention together
+    std::mutex tree_mu;                     // keeps the launches of one tree attention together: all of kv4_attend's
     DevBuf dx, dy, dtmp, dscratch, dgemm;
     HostBuf hx, hy;
     std::map<PackKey, PackedQ> qpack;       // guarded by mu
@@ -723,9 +723,10 @@ int kv4_attend(const char* what, void* out, const void* q, int q_dtype, long lon
     a.soft_cap = soft_cap;
     a.parents = parents;
     a.parents_stride = parents_stride;
-    if (!parents) return launch_status(launch_kv4_attention(a, workspace, st->sms, pick_stream(st, stream)), what);
-    // two launches share the workspace: another thread's call on this stream must not come between them
+    // a tree's two launches share the workspace, which may be a chain's too: no other thread's call of either kind on this
+    // stream may come between them
     std::lock_guard<std::mutex> g(st->tree_mu);
+    if (!parents) return launch_status(launch_kv4_attention(a, workspace, st->sms, pick_stream(st, stream)), what);
     return launch_status(launch_kv4_tree(a, workspace, st->sms, st->fault_word, pick_stream(st, stream)), what);
 }
 

@@ -1169,7 +1169,13 @@ __global__ void __launch_bounds__(256, kJoinBlocks) kv4_tree_join_kernel(const K
     int count = 0;                    // listed in the order of the CTAs: all blocks have to number them alike
     for (int c0 = 0; c0 < ctas; c0 += 256) {
         const int c = c0 + threadIdx.x, warp = threadIdx.x >> 5;
-        const Cut cut = c < ctas ? cuts[c] : Cut{};
+        Cut cut = c < ctas ? cuts[c] : Cut{};
+        // what another call has written over the list, on a stream that the workspace was not for, is not followed
+        if (cut.n > 1 && (cut.n > ctas - c || static_cast<unsigned int>(cut.b) >= static_cast<unsigned int>(p.batch) ||
+                          static_cast<unsigned int>(cut.h) >= static_cast<unsigned int>(p.kv_heads * p.row_tiles))) {
+            if (blockIdx.x == 0) atomicOr(fault_word, ALJ_FAULT_BOUNDS);
+            cut.n = 0;
+        }
         const uint32_t is = __ballot_sync(0xffffffffu, cut.n > 1);
         if (c0 > 0) __syncthreads();
         if ((threadIdx.x & 31) == 0) s_warp[warp] = __popc(is);

@@ -429,7 +429,9 @@ int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, lo
  * node counting as position base + its depth (a root's is 0).  A node that is
  * absent, or whose sequence holds no tree, is zero.  nodes * q_heads /
  * kv_heads is at most 1024.  The workspace may be the same as
- * kv4_attention_dev's where it is large enough.
+ * kv4_attention_dev's where it is large enough, also for several threads that
+ * call on one stream.  A call is two launches: a captured graph that another
+ * thread replays on that stream needs a workspace of its own.
  *
  * kv4_accept_tree_dev: from node 0 (a root: the token emitted last) on to the
  * first child whose drafted token is the one picked after its parent, as long
