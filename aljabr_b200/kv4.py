@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import threading
 
 import torch
 
@@ -100,6 +101,7 @@ def new_output(shape, dtype, device, index: int, stream: int) -> torch.Tensor:
 
 
 _tree_work = {}     # (device, stream) -> workspace of attend_tree, of all caches: calls on one stream follow one another
+_making = threading.Lock()      # workspaces are made once: a thread's launch may still be coming with the address of the first
 _kinds = {}         # shapes of caches
 _captured = {}      # (device, stream) -> capture id, its workspaces
 _kept = []          # workspaces of captures on streams given by handle
@@ -270,7 +272,10 @@ class Kv4Cache:
         kept as long as the cache, since kernels under way may hold its address."""
         have = self._buffers.get(stream)
         if have is None:
-            have = self._buffers[stream] = self._make_workspace(q_len, q_heads, stream)
+            with _making:
+                have = self._buffers.get(stream)
+                if have is None:
+                    have = self._buffers[stream] = self._make_workspace(q_len, q_heads, stream)
         got = self._work[stream, q_len, q_heads] = (have.data_ptr(), have.numel())
         return got
 
@@ -286,7 +291,10 @@ class Kv4Cache:
         if have is None:
             size, group = native.lib().aljabr_blackwell_kv4_tree_attention_workspace_size, native.KV4_MAX_ROWS // native.KV4_MAX_NODES
             most = max(size(native.KV4_MAX_NODES, group, 1, D) for D in (64, 128, 256))
-            have = _tree_work[self._index, stream] = self._zeros(int(most), stream)
+            with _making:
+                have = _tree_work.get((self._index, stream))
+                if have is None:
+                    have = _tree_work[self._index, stream] = self._zeros(int(most), stream)
         return have.data_ptr(), have.numel()
 
     def _zeros(self, size: int, stream: int) -> torch.Tensor:

@@ -62,3 +62,24 @@ def test_a_chain_and_a_tree_share_a_workspace():
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for os, w in zip(outs, want) for o in os)
     assert fault_bits() == 0
+
+
+def test_first_calls_of_two_threads_that_allocate():
+    """A stream's first calls come from two threads, each with caches of its own, whose outputs are made in between."""
+    p = tree.grow(np.random.default_rng(72), 20)
+    cases = [tree_case(73 + i, 128, 2, 4, 64, [1000, 500], [p] * 2, torch.bfloat16, wide=i > 1) for i in range(4)]
+    want = [c[0].attend_tree(*c[1:5]) for c in cases]
+    for _ in range(5):
+        stream, got = torch.cuda.Stream(), [[] for _ in cases]
+        torch.cuda.synchronize()
+
+        def work(i):
+            with torch.cuda.stream(stream):
+                for _ in range(8):
+                    got[i].append(cases[i][0].attend_tree(*cases[i][1:5]))
+                    got[i].append(torch.full_like(want[i], float("nan")))
+        together(*(lambda i=i: work(i) for i in range(4)))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(o, w) for o in g[::2]) and all(torch.isnan(o).all() for o in g[1::2])
+    assert fault_bits() == 0
