@@ -9,10 +9,11 @@
 // a kv head; 128 of them are an MMA's M.  A tile is KT positions.  Every code is
 // decoded once for 128 rows, into fp16 operands in shared memory:
 //   * K: d (c - 8) 2^-e, row p = the position, in the 128-byte swizzle; e, one
-//     of 32 positions, is the largest exponent of their scales, so the operand is
-//     in fp16's range whatever the cache holds, and scores are scaled back by 2^e
-//     in fp32.  d (c - 8) has 15 bits: it is rounded to fp16's 11 (2^-11 half a
-//     step; the output's own rounding is 2^-8).
+//     of 32 positions, puts the largest of their scales into [2^11, 2^12), so the
+//     operand is below 2^15 whatever the cache holds, and scores are scaled back by
+//     2^e in fp32.  d (c - 8) has 15 bits: it is rounded to fp16's 11 (2^-11 half a
+//     step; the output's own rounding is 2^-8), also where another group's or
+//     position's d is up to 2^25 times as large; from there on bits are lost.
 //   * V: the same, transposed on the way (a row is a dim, 8 positions 16 bytes): a
 //     word of two positions' codes is put together by one PRMT, as the codes of
 //     four dims lie in a halfword.  Its e, one of 32 positions too, goes into P.
@@ -315,9 +316,10 @@ __device__ __forceinline__ uint32_t top_of(const uint32_t (&w)[N], bool finite) 
     }
     return max(m & 0xFFFFu, m >> 16);
 }
-// Exponent e with 2^e <= v < 2^(e + 1) of an fp16 magnitude's bits (subnormals: that of the smallest normal).
-__device__ __forceinline__ int exponent_of(uint32_t bits) { return max(1, static_cast<int>(bits >> 10)) - 15; }
-// Two scales times 2^-e, |e| <= 16, in two exact steps.
+// Exponent e with 2^11 <= v 2^-e < 2^12 for an fp16 magnitude's bits (subnormals: that of the smallest normal), in [-25, 4]:
+// times a code, at most 8, the upper end of fp16's normal range, so that smaller scales beside it have the most of it.
+__device__ __forceinline__ int exponent_of(uint32_t bits) { return max(1, static_cast<int>(bits >> 10)) - 15 - 11; }
+// Two scales times 2^-e, -28 <= e <= 29, in two steps, exact where the result is normal.
 struct Unit {
     __half2 a, b;
     __device__ __forceinline__ explicit Unit(int e) {

@@ -68,3 +68,53 @@ def test_rows_at_which_the_kernel_changes(D, nodes, G):
     for window in (0, 90):
         check(cache.attend_tree(q, sl, parents, table, window=window), q, k64, v64, lens, trees, window)
     assert fault_bits() == 0
+
+
+@pytest.mark.parametrize("dtype,pad", [(torch.float32, 0), (torch.bfloat16, 0), (torch.bfloat16, 60)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("power,size", [(-8, 0), (-16, 0), (-20, 0), (-14, 12), (-20, 12)])
+def test_groups_of_far_smaller_scales(D, power, size, dtype, pad):
+    """V and K are of size 2^size, but their second 32 dims 2^power of that (at 2^0 scales of 2^-20 are fp16's last bits in the
+    cache itself); the queries there are as much larger.  Outputs of those dims and scores are as near as any.  A score is
+    off by 2^-11 of its products (bf16) and fp32's sums, P and V by 2^-11 each; the limits go by each dim's own values,
+    with 2^-24 of its largest for weights at fp16's lower end.  fp32: a weight times its scale enters to 2^-28 of the largest
+    V there is, whatever its dim's are, each position for itself."""
+    bf16 = dtype == torch.bfloat16
+    T, n, hkv, G = 21 + pad, 300 + pad, 2, 2
+    rng = np.random.default_rng(D)
+    p = tree.grow(rng, 21, 1, 2) + [-2] * pad
+    k, v = (rng.normal(size=(n, hkv, D)).astype(np.float32) for _ in range(2))
+    k, v = k * np.float32(2.0 ** size), v * np.float32(2.0 ** size)
+    k[..., 32:64] *= np.float32(2.0 ** power)
+    v[..., 32:64] *= np.float32(2.0 ** power)
+    q = rng.normal(size=(1, T, hkv * G, D)).astype(np.float32) * np.float32(0.5 * 2.0 ** -size)
+    q[..., 32:64] *= np.float32(2.0 ** -power)
+    cache, table, k64, v64 = one_sequence(k, v, wide=pad > 0)
+    qt = cuda(q, dtype)
+    got = cache.attend_tree(qt, ints([n]), ints([p]), table).double().cpu().numpy()[0]
+    qn = qt.double().cpu().numpy()[0]
+    off, norm, floor = np.zeros(D // 32), np.zeros(D // 32), 0.0
+    for t, rows in enumerate(tree.visible(p, n)):
+        for h in range(hkv * G):
+            if not rows:
+                assert not got[t, h].any()
+                continue
+            kk, vv = k64[rows, h // G], v64[rows, h // G]
+            s = kk @ qn[t, h] * D ** -0.5
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            want, weight = w @ vv, w @ np.abs(vv)
+            # fp32: an element of q to 2^-23 of its group's largest, whose codes enter with the offset 8
+            far = np.abs(kk) @ np.abs(qn[t, h]) if bf16 else (np.abs(qn[t, h]).reshape(-1, 32).max(-1).repeat(32) * (np.abs(kk) + 8 / 7 * np.abs(kk).reshape(len(kk), -1, 32).max(-1).repeat(32, -1))).sum(-1)
+            delta = D ** -0.5 * far.max() * 2.0 ** (-11 if bf16 else -20) + np.abs(s).max() * 2.0 ** -20
+            tol = weight * (np.expm1(2 * delta) + 2.0 ** (-10 if bf16 else -18)) + n * (2.0 ** -24 * np.abs(vv).max(0) if bf16 else 2.0 ** -28 * np.abs(vv).max())
+            floor += 32 * len(rows) * (0.0 if bf16 else 2.0 ** -28 * np.abs(vv).max()) ** 2
+            if bf16:
+                tol = tol + np.abs(want) * 2.0 ** -8
+            err = np.abs(got[t, h] - want)
+            assert np.all(err <= tol), (t, h, int((err / tol).argmax()), float((err / tol).max()))
+            off += (err ** 2).reshape(-1, 32).sum(-1)
+            norm += (want ** 2).reshape(-1, 32).sum(-1)
+    # by norm, each group for itself: rounding errors do not add up
+    assert np.all(off <= norm * (2.0 ** -8 if bf16 else 2.0 ** -18) ** 2 + floor), np.sqrt(off / norm)
+    assert fault_bits() == 0
