@@ -957,7 +957,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
         const long long section = static_cast<long long>(p.page_size) * (k < 2 ? k * (D / 2) : D + (k - 2) * (2 * NG));
         const long long block = kv4_block_bytes(p.page_size, D);
         while (next_piece<KT>(line, p, items, pc)) {
-            const int lo = window_start(p, pc.base + 1);
+            const int lo = window_start(p, pc.base + 1), kept = lo / p.page_size;   // pages before `kept` may have been given back
             int pos = pc.tile0 * KT + 16 * blk, pi = pos / p.page_size, off = pos - pi * p.page_size;
             int first = 0, last = -1;                                 // pages at hand
             const uint8_t* const head = p.cache + static_cast<long long>(pc.kvh) * block + section;
@@ -974,7 +974,7 @@ __global__ void __launch_bounds__(Shape<NG>::THREADS, 1) kv4_tree_kernel(const K
                     for (int n = lane; n < kPages && first + n <= end; n += 32) {
                         const int page = p.table ? __ldg(p.table + static_cast<long long>(pc.b) * p.table_stride + first + n) : pc.b;
                         const bool bad = page < 0 || page >= p.pages;
-                        if (bad) record_fault(ALJ_FAULT_BOUNDS);
+                        if (bad && first + n >= kept) record_fault(ALJ_FAULT_BOUNDS);
                         s.pages[n] = bad ? -1 : page;
                     }
                     __syncwarp();

@@ -363,7 +363,8 @@ int aljabr_blackwell_gemm_q_dev(int type, int nseg, float* const* y, const int* 
  * before the call: query t sees positions up to seq_lens[b] - q_len + t,
  * with window > 0 only the last `window` of them; a query that sees nothing
  * is zero.  Position p of sequence b is at block_table[b * table_stride + p /
- * page_size] (device), or with block_table NULL in page b.  soft_cap > 0
+ * page_size] (device), or with block_table NULL in page b; entries of pages
+ * that lie wholly before the first query's window may be anything.  soft_cap > 0
  * (in [1e-30, 1e30]) applies tanh(s / cap) * cap to the scaled scores.
  * Accuracy: sums and softmax statistics are fp32.  An fp32 query element
  * enters with an error of at most 2^-23 of the largest in its group of 32

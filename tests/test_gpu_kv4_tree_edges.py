@@ -118,3 +118,38 @@ def test_groups_of_far_smaller_scales(D, power, size, dtype, pad):
     # by norm, each group for itself: rounding errors do not add up
     assert np.all(off <= norm * (2.0 ** -8 if bf16 else 2.0 ** -18) ** 2 + floor), np.sqrt(off / norm)
     assert fault_bits() == 0
+
+
+@pytest.mark.parametrize("dtype,pad", [(torch.float32, 0), (torch.bfloat16, 0), (torch.bfloat16, 60)])
+@pytest.mark.parametrize("D,ps,window", [(128, 16, 100), (64, 16, 33), (256, 16, 100), (128, 64, 1), (128, 48, 500)])
+def test_pages_given_back_behind_the_window(D, ps, window, dtype, pad):
+    """A server gives pages back that no window reaches any more; their entries are -1 or no page of this pool.  That is no
+    fault, and one page further on it is."""
+    lens = [1000 + pad, 300 + pad, 22 + pad]
+    p = tree.grow(np.random.default_rng(61), 21, 2, 1) + [-2] * pad
+    T = len(p)
+    cache, q, sl, parents, table, k64, v64 = tree_case(62, D, 2, 2, ps, lens, [p] * 3, dtype, wide=pad > 0)
+    want = cache.attend_tree(q, sl, parents, table, window=window)
+    check(want, q, k64, v64, lens, [p] * 3, window)
+    first = [max(0, n - T + 1 - window) // ps for n in lens]      # the first page that a root at the tree's base may see
+    assert first[0] > 0 and fault_bits() == 0
+    for gone in (-1, cache.pages, 2 ** 31 - 1):
+        cut = table.clone()
+        for b, f in enumerate(first):
+            cut[b, :f] = gone
+        assert torch.equal(cache.attend_tree(q, sl, parents, cut, window=window), want)
+        assert fault_bits() == 0
+        cut[0, first[0]] = gone
+        cache.attend_tree(q, sl, parents, cut, window=window)
+        assert fault_bits() & 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_pages_given_back_behind_a_chain_s_window(dtype):
+    lens, T, window, ps = [1000, 300, 40], 5, 100, 16
+    cache, q, sl, _, table, _, _ = tree_case(65, 128, 2, 4, ps, lens, [list(range(-1, T - 1))] * 3, dtype)
+    want = cache.attend(q, sl, table, window=window)
+    cut = table.clone()
+    for b, n in enumerate(lens):
+        cut[b, :max(0, n - T + 1 - window) // ps] = 2 ** 31 - 1
+    assert torch.equal(cache.attend(q, sl, cut, window=window), want) and fault_bits() == 0
