@@ -54,7 +54,7 @@ def _build_calls(tmp: str) -> str:
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(shutil.which(os.environ.get("NVCC", "nvcc")))))
     obj = os.path.join(tmp, "tensor_calls.o")
     subprocess.check_call([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-c", os.path.join(CSRC, "tensor_calls.cpp"),
-                           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", inc,
+                           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DALJ_TORCH="{torch.__version__}"', "-I", inc,
                            "-I", os.path.join(inc, "torch", "csrc", "api", "include"), "-I", sysconfig.get_paths()["include"],
                            "-I", os.path.join(cuda, "include"), "-o", obj])
     return obj

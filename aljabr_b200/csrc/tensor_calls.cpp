@@ -208,4 +208,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "tensor_calls", nullptr, -1, method
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_tensor_calls(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_tensor_calls(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch", ALJ_TORCH)) {   // the torch it was built with, which kv4.py compares
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

@@ -26,7 +26,9 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import os
 import threading
+import warnings
 
 import torch
 
@@ -118,15 +120,25 @@ def bad(message: str) -> native.ProviderError:
     return native.ProviderError(native.ALJ_ERR_BAD_ARG, message)
 
 
-native.lib()
-try:
-    from . import tensor_calls
-except ImportError as e:
-    raise native.ProviderError(native.ALJ_ERR_NOT_INITIALIZED, f"tensor_calls.so is missing or not this torch's ({e}): run "
-                               "`python -m aljabr_b200.build`") from e
-_rotate_append = native.lib().aljabr_blackwell_kv4_rotate_append_dev
-_attend_tree = native.lib().aljabr_blackwell_kv4_tree_attention_dev
-_accept_tree = native.lib().aljabr_blackwell_kv4_accept_tree_dev
+def _load_calls():
+    """tensor_calls.so, where it was built and with this torch.  It takes tensors to the library in less host time; without
+    it every call goes through ctypes, to the same kernels."""
+    try:
+        from . import tensor_calls
+        made = getattr(tensor_calls, "torch", "of another version")
+        if made == torch.__version__:
+            return tensor_calls
+        why = f"it was built with torch {made}"
+    except ImportError as e:
+        if not os.path.exists(os.path.join(os.path.dirname(__file__), "tensor_calls.so")):
+            return None
+        why = str(e)
+    warnings.warn(f"tensor_calls.so is not used ({why}): calls take more host time until `python -m aljabr_b200.build`",
+                  RuntimeWarning, stacklevel=3)
+    return None
+
+
+tensor_calls = _load_calls()
 
 
 class Kv4Cache:
@@ -214,7 +226,7 @@ class Kv4Cache:
         a head's first 2 n dims turn, dims i and i + n a pair, or with `interleaved` 2 i and 2 i + 1.  q_out: of q's
         shape and type, its rows may be strided; q itself will do, elements of k or v will not."""
         got = tensor_calls.rotate_append(*self._shape, self._index, q, k, v, slots, positions, rope, interleaved, q_out, k_back, v_back,
-                                         stream)
+                                         stream) if tensor_calls else NotImplemented
         if got is not NotImplemented:
             return native.check(got) if type(got) is int else got
         n, dtype = slots.numel(), k.dtype
@@ -238,10 +250,10 @@ class Kv4Cache:
             q_out = new_output(q.shape, dtype, self.device, self._index, stream)
         elif q_out.dtype is not dtype:
             raise bad(f"q is {dtype}, q_out is {q_out.dtype}")
-        rc = _rotate_append(*self._shape, q_out.data_ptr(), self._q_rows(q_out, n, heads, "q_out"), q.data_ptr(), k.data_ptr(),
-                            v.data_ptr(), kind, qs, ks, vs, heads, self._ints(slots, n, "slots"),
-                            self._ints(positions, n, "positions"), rope.data_ptr(), rope.shape[0], 2 * rope.shape[1],
-                            bool(interleaved), n, kb, vb, stream)
+        rc = native.lib().aljabr_blackwell_kv4_rotate_append_dev(
+            *self._shape, q_out.data_ptr(), self._q_rows(q_out, n, heads, "q_out"), q.data_ptr(), k.data_ptr(), v.data_ptr(), kind,
+            qs, ks, vs, heads, self._ints(slots, n, "slots"), self._ints(positions, n, "positions"), rope.data_ptr(), rope.shape[0],
+            2 * rope.shape[1], bool(interleaved), n, kb, vb, stream)
         if rc:
             native.check(rc)
         return q_out
@@ -383,9 +395,9 @@ class Kv4Cache:
             rc = self._attend(out.data_ptr(), q.data_ptr(), kind, q_stride, *self._shape, table, width, lens, batch, q_len,
                               q_heads, window, scale, soft_cap, work, size, stream)
         else:
-            rc = _attend_tree(out.data_ptr(), q.data_ptr(), kind, q_stride, *self._shape, table, width, lens, batch,
-                              parents.data_ptr(), q_len if parents.dim() == 2 else 0, q_len, q_heads, window, scale, soft_cap,
-                              work, size, stream)
+            rc = native.lib().aljabr_blackwell_kv4_tree_attention_dev(
+                out.data_ptr(), q.data_ptr(), kind, q_stride, *self._shape, table, width, lens, batch, parents.data_ptr(),
+                q_len if parents.dim() == 2 else 0, q_len, q_heads, window, scale, soft_cap, work, size, stream)
         if rc:
             native.check(rc)
         return out
@@ -408,7 +420,8 @@ def accept_tree(caches, seq_lens: torch.Tensor, parents: torch.Tensor, drafted: 
     addresses = [c._address for c in caches if c._kind is kind]
     if len(addresses) != len(caches):
         raise bad("the caches of one call must have the same shape and device")
-    got = tensor_calls.accept_tree(addresses, *kind, seq_lens, parents, drafted, picked, block_table, out, stream)
+    got = tensor_calls.accept_tree(addresses, *kind, seq_lens, parents, drafted, picked, block_table, out, stream) \
+        if tensor_calls else NotImplemented
     if got is not NotImplemented:
         return native.check(got) if type(got) is int else got
     if drafted.dim() != 2:
@@ -424,10 +437,11 @@ def accept_tree(caches, seq_lens: torch.Tensor, parents: torch.Tensor, drafted: 
         table = ints(block_table, ((batch, max(width, 1)),), "block_table")
     path, count, token, lens = (ints(t, (s,), w) for t, s, w in zip(out, ((batch, nodes),) + ((batch,),) * 3,
                                                                     ("path", "count", "token", "lens")))
-    rc = _accept_tree(path, count, token, lens, (ctypes.c_void_p * len(caches))(*addresses), len(caches),
-                      *first._shape[1:], table, width, ints(seq_lens, ((batch,),), "seq_lens"), batch,
-                      ints(parents, ((nodes,), (batch, nodes)), "parents"), nodes if parents.dim() == 2 else 0, nodes,
-                      ints(drafted, ((batch, nodes),), "drafted"), ints(picked, ((batch, nodes),), "picked"), stream)
+    rc = native.lib().aljabr_blackwell_kv4_accept_tree_dev(
+        path, count, token, lens, (ctypes.c_void_p * len(caches))(*addresses), len(caches), *first._shape[1:], table, width,
+        ints(seq_lens, ((batch,),), "seq_lens"), batch, ints(parents, ((nodes,), (batch, nodes)), "parents"),
+        nodes if parents.dim() == 2 else 0, nodes, ints(drafted, ((batch, nodes),), "drafted"),
+        ints(picked, ((batch, nodes),), "picked"), stream)
     if rc:
         native.check(rc)
     return out
