@@ -204,7 +204,7 @@ PyMethodDef methods[] = {
     {"rotate_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<rotate_append>)), METH_FASTCALL, nullptr},
     {"accept_tree", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<accept_tree>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "tensor_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "tensor_calls", ALJ_MARK, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 
