@@ -623,6 +623,38 @@ int kv4_rows(Kv4Rows* p, void* cache, int pages, int page_size, int kv_heads, in
     return ALJ_OK;
 }
 
+// n rows of `bytes` bytes each, `step` bytes (at least `bytes`) apart.
+struct Rows {
+    uintptr_t at;
+    long long bytes, step, n;
+    Rows(const void* p, long long row_bytes, long long step_bytes, long long rows)
+        : at(reinterpret_cast<uintptr_t>(p)), bytes(row_bytes), step(step_bytes), n(rows) {}
+    Rows(const void* p, long long all) : Rows(p, all, all, 1) {}
+    bool same(const Rows& o) const { return at == o.at && bytes == o.bytes && (n == 1 || step == o.step); }
+};
+
+long long floor_div(long long a, long long b) { return a / b - (a % b != 0 && (a < 0) != (b < 0)); }
+
+// Whether two sets of rows share a byte; rows that lie between the other's rows do not.
+bool overlap(const Rows& a, const Rows& b) {
+    if (a.n < 1 || b.n < 1 || a.bytes < 1 || b.bytes < 1) return false;
+    const long long d = static_cast<long long>(b.at - a.at);
+    if (d >= (a.n - 1) * a.step + a.bytes || -d >= (b.n - 1) * b.step + b.bytes) return false;
+    if (a.step == b.step && a.n > 1 && b.n > 1) {
+        // row j of b, m = j - i rows behind row i of a, overlaps it where -b.bytes < d + m step < a.bytes
+        const long long lo = floor_div(-b.bytes - d, a.step) + 1, hi = floor_div(a.bytes - 1 - d, a.step);
+        return std::max(lo, 1 - a.n) <= std::min(hi, b.n - 1);
+    }
+    const Rows& few = a.n <= b.n ? a : b;
+    const Rows& many = a.n <= b.n ? b : a;
+    const long long off = static_cast<long long>(many.at - few.at);
+    for (long long i = 0; i < few.n; ++i) {        // rows j of `many` with off + j step < i few.step + few.bytes and > i few.step - many.bytes
+        const long long lo = floor_div(i * few.step - many.bytes - off, many.step) + 1, hi = floor_div(i * few.step + few.bytes - 1 - off, many.step);
+        if (std::max(lo, 0LL) <= std::min(hi, many.n - 1)) return true;
+    }
+    return false;
+}
+
 // Rows that enter the cache: the checks and arguments of both appends.
 int kv4_append_rows(Kv4Rows* p, const char* what, void* cache, int pages, int page_size, int kv_heads, int head_dim,
                     const void* k, const void* v, int type, long long k_stride, long long v_stride, const int* slots,
@@ -1591,6 +1623,24 @@ int aljabr_blackwell_kv4_rotate_append_dev(void* cache, int pages, int page_size
     if (q_stride < row || q_out_stride < row)
         return fail(ALJ_ERR_BAD_DIMS, "kv4_rotate_append: strides %lld, %lld < q_heads * head_dim = %lld", q_stride, q_out_stride, row);
     const uintptr_t e = kv_dtype == ALJ_KV_BF16 ? 2 : 4;
+    // CTAs of q and of K and V run side by side: what one writes the other must not read, nor a thread another's row of q
+    const long long kv = static_cast<long long>(kv_heads) * head_dim * e, eb = static_cast<long long>(e);
+    const Rows out_rows(q_out, row * eb, q_out_stride * eb, tokens), q_rows(q, row * eb, q_stride * eb, tokens);
+    const Rows k_rows(k, kv, k_stride * eb, tokens), v_rows(v, kv, v_stride * eb, tokens);
+    const Rows kb_rows(k_back, kv, kv, k_back ? tokens : 0), vb_rows(v_back, kv, kv, v_back ? tokens : 0);
+    const Rows cache_bytes(cache, kv4_cache_bytes(pages, page_size, kv_heads, head_dim));
+    const Rows small[3] = {{slots, 4LL * tokens}, {positions, 4LL * tokens}, {rope, 4LL * rope_positions * rotary_dim}};
+    if (overlap(out_rows, k_rows) || overlap(out_rows, v_rows) || (overlap(out_rows, q_rows) && !out_rows.same(q_rows)))
+        return fail(ALJ_ERR_BAD_ARG, "kv4_rotate_append: q_out must not overlap k or v, nor q unless it is q");
+    if ((overlap(kb_rows, k_rows) && !kb_rows.same(k_rows)) || (overlap(vb_rows, v_rows) && !vb_rows.same(v_rows)) ||
+        overlap(kb_rows, v_rows) || overlap(vb_rows, k_rows) || overlap(kb_rows, q_rows) || overlap(vb_rows, q_rows) ||
+        overlap(kb_rows, out_rows) || overlap(vb_rows, out_rows) || overlap(kb_rows, vb_rows))
+        return fail(ALJ_ERR_BAD_ARG, "kv4_rotate_append: k_back must not overlap other rows unless it is k, nor v_back unless it is v");
+    for (const Rows& w : {out_rows, kb_rows, vb_rows, cache_bytes})
+        for (const Rows& r : small)
+            if (overlap(w, r)) return fail(ALJ_ERR_BAD_ARG, "kv4_rotate_append: slots, positions and rope must not lie in what is written");
+    for (const Rows& w : {out_rows, kb_rows, vb_rows})
+        if (overlap(w, cache_bytes)) return fail(ALJ_ERR_BAD_ARG, "kv4_rotate_append: no rows may be written into the cache");
     if (misaligned(e, q, q_out) || misaligned(4, positions) || misaligned(16, rope))
         return fail(ALJ_ERR_BAD_ARG, "kv4_rotate_append: q, q_out and positions must be aligned to their elements, rope to 16 bytes");
     p.q = q;

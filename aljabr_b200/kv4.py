@@ -224,7 +224,8 @@ class Kv4Cache:
         q: [tokens, q_heads, head_dim] with contiguous rows, of k's type.  positions: int32 [tokens], below zero where a
         token is absent (its q is zero, nothing is stored).  rope: float32 [positions, n, 2] of (cos, sin), contiguous;
         a head's first 2 n dims turn, dims i and i + n a pair, or with `interleaved` 2 i and 2 i + 1.  q_out: of q's
-        shape and type, its rows may be strided; q itself will do, elements of k or v will not."""
+        shape and type, its rows may be strided; q itself will do.  k_back, v_back: as for append(); k and v themselves will do.
+        Outputs may lie between the rows of other arguments, but overlap none."""
         got = tensor_calls.rotate_append(*self._shape, self._index, q, k, v, slots, positions, rope, interleaved, q_out, k_back, v_back,
                                          stream) if tensor_calls else NotImplemented
         if got is not NotImplemented:

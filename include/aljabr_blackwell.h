@@ -420,8 +420,9 @@ int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, lo
  *   (a c - b s, a s + b c) for the dims a, b = pair, pair + rotary_dim / 2,
  *   or with `interleaved` 2 pair, 2 pair + 1,
  * products and sums rounded to fp32 one by one, as in the decode step.  The
- * rotated q goes to q_out (q's type, q_out_stride apart; q itself will do, but
- * no elements of k or v), K is quantised from the fp32 result.  A token at a position below zero is
+ * rotated q goes to q_out (q's type, q_out_stride apart; q itself will do, as
+ * will k for k_back and v for v_back; what is written must overlap no other
+ * argument), K is quantised from the fp32 result.  A token at a position below zero is
  * absent: q_out zero, nothing stored.  One whose slot is -1 has its q rotated.
  *
  * kv4_tree_attention_dev: as kv4_attention_dev, for the nodes of each
