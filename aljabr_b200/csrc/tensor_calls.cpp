@@ -101,13 +101,19 @@ PyObject* rotate_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const long long os = rows(out, index, type, tokens, q_heads, D, false);
     if (os < 0) return no();
+    // a tensor without memory of its own (a fake one) throws here, with the interpreter held
+    const void *qp = q->data_ptr(), *kp = k->data_ptr(), *vp = v->data_ptr();
+    void* const op = out->data_ptr();
+    const int *sp = slots->data_ptr<int>(), *pp = positions->data_ptr<int>();
+    const float* rp = rope->data_ptr<float>();
+    const int n_rope = static_cast<int>(rope->size(0)), rotary = static_cast<int>(2 * rope->size(1));
+    const int kind = type == at::kFloat ? ALJ_KV_F32 : ALJ_KV_BF16;
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = aljabr_blackwell_kv4_rotate_append_dev(
-        reinterpret_cast<void*>(address), static_cast<int>(dims[0]), static_cast<int>(dims[1]), static_cast<int>(heads), static_cast<int>(D),
-        out->data_ptr(), os, q->data_ptr(), k->data_ptr(), v->data_ptr(), type == at::kFloat ? ALJ_KV_F32 : ALJ_KV_BF16, qs, ks, vs,
-        static_cast<int>(q_heads), slots->data_ptr<int>(), positions->data_ptr<int>(), rope->data_ptr<float>(),
-        static_cast<int>(rope->size(0)), static_cast<int>(2 * rope->size(1)), inter, static_cast<int>(tokens), back[0], back[1], stream);
+    rc = aljabr_blackwell_kv4_rotate_append_dev(reinterpret_cast<void*>(address), static_cast<int>(dims[0]), static_cast<int>(dims[1]),
+                                                static_cast<int>(heads), static_cast<int>(D), op, os, qp, kp, vp, kind, qs, ks, vs,
+                                                static_cast<int>(q_heads), sp, pp, rp, n_rope, rotary, inter, static_cast<int>(tokens),
+                                                back[0], back[1], stream);
     Py_END_ALLOW_THREADS
     if (rc) return PyLong_FromLong(rc);
     if (a[13] == Py_None) return THPVariable_Wrap(made);
@@ -161,14 +167,15 @@ PyObject* accept_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
             return no();
         path = *out[0], count = *out[1], token = *out[2], left = *out[3];
     }
+    int* const outs[4] = {path.data_ptr<int>(), count.data_ptr<int>(), token.data_ptr<int>(), left.data_ptr<int>()};
+    const int *tp = table ? table->data_ptr<int>() : nullptr, *lp = lens->data_ptr<int>(), *pp = parents->data_ptr<int>(),
+              *dp = drafted->data_ptr<int>(), *kp = picked->data_ptr<int>();
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = aljabr_blackwell_kv4_accept_tree_dev(path.data_ptr<int>(), count.data_ptr<int>(), token.data_ptr<int>(), left.data_ptr<int>(), caches,
-                                              static_cast<int>(layers), static_cast<int>(dims[0]), static_cast<int>(dims[1]),
-                                              static_cast<int>(dims[2]), static_cast<int>(dims[3]), table ? table->data_ptr<int>() : nullptr,
-                                              static_cast<int>(width), lens->data_ptr<int>(), static_cast<int>(batch), parents->data_ptr<int>(),
-                                              each ? static_cast<int>(nodes) : 0, static_cast<int>(nodes), drafted->data_ptr<int>(),
-                                              picked->data_ptr<int>(), stream);
+    rc = aljabr_blackwell_kv4_accept_tree_dev(outs[0], outs[1], outs[2], outs[3], caches, static_cast<int>(layers), static_cast<int>(dims[0]),
+                                              static_cast<int>(dims[1]), static_cast<int>(dims[2]), static_cast<int>(dims[3]), tp,
+                                              static_cast<int>(width), lp, static_cast<int>(batch), pp, each ? static_cast<int>(nodes) : 0,
+                                              static_cast<int>(nodes), dp, kp, stream);
     Py_END_ALLOW_THREADS
     if (rc) return PyLong_FromLong(rc);
     if (a[11] != Py_None) {
