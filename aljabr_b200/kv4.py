@@ -328,6 +328,8 @@ class Kv4Cache:
             _captured[key] = capture, (have := [])
         size = native.lib().aljabr_blackwell_kv4_tree_attention_workspace_size if tree else self._work_size
         need = size(q_len, q_heads, self.kv_heads, self.head_dim)
+        if need < 0:
+            native.check(int(need))
         if not have or have[-1].numel() < need:
             have.append(self._zeros(int(need), stream) if tree else self._make_workspace(q_len, q_heads, stream))
             if stream != current_stream(self._index):

@@ -9,7 +9,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from aljabr_b200 import kv4
+from aljabr_b200 import kv4, native
 from tests.test_kv4_wrapper_cpu import cache  # noqa: F401
 
 
@@ -38,3 +38,14 @@ def test_threads_that_meet_at_a_stream_s_first_call_use_one_workspace(cache, mon
     gc.collect()
     alive = [t().data_ptr() for t in made if t() is not None]
     assert len(set(got)) == 1 and got[0] in alive
+
+
+@pytest.mark.parametrize("nodes,q_heads,tree", [(257, 2, True), (300, 2, True), (256, 10, True), (3, 5, True), (0, 2, True),
+                                                (1025, 2, False)])
+@pytest.mark.parametrize("size", [0, 1 << 26])
+def test_a_capture_refuses_what_a_call_refuses(cache, monkeypatch, nodes, q_heads, tree, size):  # noqa: F811
+    """With the library's error, also where the capture has a workspace already."""
+    monkeypatch.setattr(kv4, "_captured", {(-1, 7): (5, [torch.zeros(size, dtype=torch.uint8)] if size else [])})
+    cache._work_size = native.lib().aljabr_blackwell_kv4_attention_workspace_size
+    with pytest.raises(native.ProviderError):
+        cache._captured_workspace(5, nodes, q_heads, 7, tree)
