@@ -1680,22 +1680,28 @@ int aljabr_blackwell_kv4_accept_tree_dev(int* path, int* count, int* token, int*
     if (misaligned(4, path, count, token, new_lens, block_table, seq_lens, drafted, picked))
         return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: integers must be aligned to their elements");
     // every layer's blocks walk for themselves while the first one's write: an output must not be an input
-    const long long all = static_cast<long long>(batch) * nodes;
-    const int* const outs[4] = {path, count, token, new_lens};
-    const long long out_n[4] = {all, batch, batch, batch};
-    const int* const ins[5] = {seq_lens, parents, drafted, picked, block_table};
-    const long long in_n[5] = {batch, static_cast<long long>(parents_stride) * (batch - 1) + nodes, all, all,
-                               static_cast<long long>(table_stride) * batch};
-    for (int o = 0; o < 4; ++o)
-        for (int i = 0; i < 5; ++i)
-            if (ins[i] && outs[o] < ins[i] + in_n[i] && ins[i] < outs[o] + out_n[o])
-                return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: outputs must not overlap the inputs");
+    const long long all = 4LL * batch * nodes, each = 4LL * batch;
+    const Rows outs[4] = {{path, all}, {count, each}, {token, each}, {new_lens, each}};
+    const Rows ins[5] = {{seq_lens, each}, {parents, 4 * (static_cast<long long>(parents_stride) * (batch - 1) + nodes)}, {drafted, all},
+                         {picked, all}, {block_table, block_table ? table_stride * each : 0}};
+    for (int o = 0; o < 4; ++o) {
+        for (const Rows& in : ins)
+            if (overlap(outs[o], in)) return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: outputs must not overlap the inputs");
+        for (int i = 0; i < o; ++i)
+            if (overlap(outs[o], outs[i])) return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: outputs must not overlap one another");
+    }
+    const long long cache_bytes = kv4_cache_bytes(pages, page_size, kv_heads, head_dim);
     Kv4Accept a = {};
     for (int l = 0; l < layers; ++l) {
         if (!caches[l] || misaligned(16, caches[l]))
             return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: cache %d must be a 16-byte aligned device address", l);
-        for (int m = 0; m < l; ++m)
-            if (a.cache[m] == caches[l]) return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: caches %d and %d are the same", m, l);
+        for (int m = 0; m < l; ++m) {
+            const long long d = static_cast<uint8_t*>(caches[l]) - a.cache[m];
+            if (d < cache_bytes && -d < cache_bytes)      // a row would move twice
+                return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: caches %d and %d overlap", m, l);
+        }
+        for (const Rows& out : outs)
+            if (overlap(out, {caches[l], cache_bytes})) return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: cache %d overlaps an output", l);
         a.cache[l] = static_cast<uint8_t*>(caches[l]);
     }
     a.layers = layers;

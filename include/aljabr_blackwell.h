@@ -444,7 +444,8 @@ int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, lo
  * (host array of device addresses); sequences must not share the pages of
  * their trees.  A sequence without a tree, or whose node 0 is no root, keeps
  * nothing of it: count 0, token -1, new_lens base (or seq_lens[b] without a
- * tree).  Outputs must not overlap inputs.
+ * tree).  Outputs must overlap neither one another nor inputs, and caches
+ * not one another.
  *
  * Parents, pages, positions and lengths outside their ranges are not followed
  * and set bit 1 of aljabr_blackwell_device_status, as above.  All are
