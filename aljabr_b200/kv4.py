@@ -36,6 +36,7 @@ from . import native
 
 _DTYPES = {torch.float32: native.KV_F32, torch.bfloat16: native.KV_BF16}
 _LEGACY_STREAM = 1      # cudaStreamLegacy: the C-ABI reads 0 as "the library's own stream"
+_THREAD_STREAM = 2      # cudaStreamPerThread: another stream in each thread
 
 
 # torch.cuda.current_stream(device).cuda_stream without building the Stream object (2.6 us a call)
@@ -78,6 +79,11 @@ def selecting(call, index_of):
     return on_device
 
 
+def stream_key(stream: int):
+    """What tells streams apart whose calls do not follow one another."""
+    return stream if stream != _THREAD_STREAM else (stream, threading.get_ident())
+
+
 def capture_id(stream: int) -> int:
     """Id of the graph capture that `stream` takes part in; 0 where it is in none."""
     got = ctypes.c_ulonglong(0)
@@ -102,10 +108,10 @@ def new_output(shape, dtype, device, index: int, stream: int) -> torch.Tensor:
     return t
 
 
-_tree_work = {}     # (device, stream) -> workspace of attend_tree, of all caches: calls on one stream follow one another
+_tree_work = {}     # (device, stream_key) -> workspace of attend_tree, of all caches: calls on one stream follow one another
 _making = threading.Lock()      # workspaces are made once: a thread's launch may still be coming with the address of the first
 _kinds = {}         # shapes of caches
-_captured = {}      # (device, stream) -> capture id, its workspaces
+_captured = {}      # (device, stream_key) -> capture id, its workspaces
 _kept = []          # workspaces of captures on streams given by handle
 
 
@@ -169,8 +175,8 @@ class Kv4Cache:
         # one object for all caches of a shape on a device
         self._kind = _kinds.setdefault(k := (pages, page_size, kv_heads, head_dim, self._index), k)
         self._shape = (data.data_ptr(), pages, page_size, kv_heads, head_dim)
-        self._buffers = {}   # stream -> workspace: calls on one stream never overlap
-        self._work = {}      # (stream, q_len, q_heads) -> its address and size
+        self._buffers = {}   # stream_key -> workspace: calls on one stream never overlap
+        self._work = {}      # (stream_key, q_len, q_heads) -> its address and size
 
     # -- checks ----------------------------------------------------------------
     def _rows(self, t: torch.Tensor, tokens: int, what: str) -> int:
@@ -283,13 +289,14 @@ class Kv4Cache:
     def _workspace(self, q_len: int, q_heads: int, stream: int):
         """(address, bytes) of this stream's workspace: made once, as large as any accepted call needs (a few MB), and
         kept as long as the cache, since kernels under way may hold its address."""
-        have = self._buffers.get(stream)
+        key = stream_key(stream)
+        have = self._buffers.get(key)
         if have is None:
             with _making:
-                have = self._buffers.get(stream)
+                have = self._buffers.get(key)
                 if have is None:
-                    have = self._buffers[stream] = self._make_workspace(q_len, q_heads, stream)
-        got = self._work[stream, q_len, q_heads] = (have.data_ptr(), have.numel())
+                    have = self._buffers[key] = self._make_workspace(q_len, q_heads, stream)
+        got = self._work[key, q_len, q_heads] = (have.data_ptr(), have.numel())
         return got
 
     def _make_workspace(self, q_len: int, q_heads: int, stream: int) -> torch.Tensor:
@@ -300,14 +307,15 @@ class Kv4Cache:
 
     def _tree_workspace(self, stream: int):
         """(address, bytes) of this stream's workspace for trees: as large as any accepted call needs, kept for good."""
-        have = _tree_work.get((self._index, stream))
+        key = self._index, stream_key(stream)
+        have = _tree_work.get(key)
         if have is None:
             size, group = native.lib().aljabr_blackwell_kv4_tree_attention_workspace_size, native.KV4_MAX_ROWS // native.KV4_MAX_NODES
             most = max(size(native.KV4_MAX_NODES, group, 1, D) for D in (64, 128, 256))
             with _making:
-                have = _tree_work.get((self._index, stream))
+                have = _tree_work.get(key)
                 if have is None:
-                    have = _tree_work[self._index, stream] = self._zeros(int(most), stream)
+                    have = _tree_work[key] = self._zeros(int(most), stream)
         return have.data_ptr(), have.numel()
 
     def _zeros(self, size: int, stream: int) -> torch.Tensor:
@@ -322,7 +330,7 @@ class Kv4Cache:
         stream: so it belongs to this capture's calls on this stream (of all caches: they follow one another) and to
         nothing else.  torch's graph keeps the memory: here it is held until the stream's next capture, and for good
         where the stream was given by its handle, since other means of capture keep nothing."""
-        key = self._index, stream
+        key = self._index, stream_key(stream)
         owner, have = _captured.get(key, (0, []))
         if owner != capture:
             _captured[key] = capture, (have := [])
@@ -390,7 +398,7 @@ class Kv4Cache:
         elif parents is not None:
             work, size = self._tree_workspace(stream)
         else:
-            have = self._work.get((stream, q_len, q_heads))
+            have = self._work.get((stream_key(stream), q_len, q_heads))
             work, size = have if have is not None else self._workspace(q_len, q_heads, stream)
         scale = D ** -0.5 if scale is None else scale
         lens = self._ints(seq_lens, batch, "seq_lens")

@@ -49,3 +49,29 @@ def test_a_capture_refuses_what_a_call_refuses(cache, monkeypatch, nodes, q_head
     cache._work_size = native.lib().aljabr_blackwell_kv4_attention_workspace_size
     with pytest.raises(native.ProviderError):
         cache._captured_workspace(5, nodes, q_heads, 7, tree)
+
+
+@pytest.mark.parametrize("tree", [True, False])
+def test_the_per_thread_stream_is_another_in_each_thread(cache, monkeypatch, tree):  # noqa: F811
+    """Handle 2 names a stream of the calling thread: two threads' calls on it run side by side, and want two workspaces."""
+    monkeypatch.setattr(kv4.Kv4Cache, "_zeros", lambda self, size, stream: torch.zeros(64, dtype=torch.uint8))
+    monkeypatch.setattr(kv4, "_tree_work", {})
+    monkeypatch.setattr(kv4, "capture_id", lambda stream: 0)
+    got = []
+    cache._attend = lambda *a: got.append(a[-3]) or 0
+    q, lens, table = torch.zeros(1, 1, 2, 64), torch.ones(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32)
+
+    def call():
+        if tree:
+            got.append(cache._tree_workspace(2)[0])
+        else:
+            cache.attend(q, lens, table, out=q, stream=2)
+    call()
+    call()
+    gate = threading.Barrier(2)
+    threads = [threading.Thread(target=lambda: (gate.wait(), call(), call(), gate.wait())) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert got[0] == got[1] and len(set(got)) == 3 and all(got.count(g) == 2 for g in got)
