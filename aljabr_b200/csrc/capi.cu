@@ -1690,18 +1690,20 @@ int aljabr_blackwell_kv4_accept_tree_dev(int* path, int* count, int* token, int*
         for (int i = 0; i < o; ++i)
             if (overlap(outs[o], outs[i])) return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: outputs must not overlap one another");
     }
+    uintptr_t first = ~uintptr_t(0), last = 0;            // of all outputs
+    for (const Rows& out : outs) first = std::min(first, out.at), last = std::max<uintptr_t>(last, out.at + out.bytes);
     const long long cache_bytes = kv4_cache_bytes(pages, page_size, kv_heads, head_dim);
     Kv4Accept a = {};
     for (int l = 0; l < layers; ++l) {
         if (!caches[l] || misaligned(16, caches[l]))
             return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: cache %d must be a 16-byte aligned device address", l);
-        for (int m = 0; m < l; ++m) {
-            const long long d = static_cast<uint8_t*>(caches[l]) - a.cache[m];
-            if (d < cache_bytes && -d < cache_bytes)      // a row would move twice
+        const uintptr_t at = reinterpret_cast<uintptr_t>(caches[l]);
+        for (int m = 0; m < l; ++m)                       // within cache_bytes of one another: a row would move twice
+            if (at - reinterpret_cast<uintptr_t>(a.cache[m]) + (cache_bytes - 1) < 2 * static_cast<uintptr_t>(cache_bytes) - 1)
                 return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: caches %d and %d overlap", m, l);
-        }
-        for (const Rows& out : outs)
-            if (overlap(out, {caches[l], cache_bytes})) return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: cache %d overlaps an output", l);
+        if (at < last && first < at + cache_bytes)
+            for (const Rows& out : outs)
+                if (overlap(out, {caches[l], cache_bytes})) return fail(ALJ_ERR_BAD_ARG, "kv4_accept_tree: cache %d overlaps an output", l);
         a.cache[l] = static_cast<uint8_t*>(caches[l]);
     }
     a.layers = layers;
