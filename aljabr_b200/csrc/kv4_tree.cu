@@ -37,9 +37,9 @@
 //
 // What bounds it: the issue of instructions, most of them of the decoding and of the softmax.  A tile of 128 positions and
 // 128 rows takes about 7400 warp instructions and 3400 cycles: 64 % of the issue slots at 20 warps an SM, the tensor pipe
-// 35 % of the time, DRAM 14 %.  2 sequences of 65536, 64 query heads on 8, 61 nodes: 377 to 411 us, 640 to 690 TFLOP/s; 24
-// ragged sequences up to 16384 with 26 nodes: 115 us.  Tried and slower for the first: tiles of 64 with 10 stages of codes (472 us),
-// 8 warps for V (465), one stage of K and four of codes (398 against 388 then).
+// 35 % of the time, DRAM 14 %.  2 sequences of 65536, 64 query heads on 8, 61 nodes: 378 us by itself, 690 TFLOP/s, and 396 to
+// 411 among other work; 24 ragged sequences up to 16384 with 26 nodes: 114 to 117 us.  Tried and slower for the first: tiles
+// of 64 with 10 stages of codes (472 us), 8 warps for V (465), one stage of K and four of codes (398 against 388 then).
 #define ALJ_OWN_FAULT_WORD     // compiled by itself, for setmaxnreg (build.py)
 #include "kv4.cuh"
 #include "tc_gemm.cuh"
@@ -1284,10 +1284,11 @@ cudaError_t launch_tree(const Kv4Attn& p, Cut* cuts, int sms, unsigned int* faul
 //   32 sequences of 1024:   32 rows, D 64, 128, 256: 38, 47   60, 58   115, 112     48 rows: 50, 48   82, 60   166, 113
 //   1 sequence of 4096:     48 rows, D 64, 128, 256: 16, 19   23, 21    29, 33     128 rows: 23, 19   32, 21    52, 34
 //   1 sequence of 257:     128 rows, D 64, 128, 256: 11, 18   12, 20    12, 27
-// So this kernel has more than 32 rows, where positions times heads, rows and dims reach 160 million (D 64 and 128: 40 rows
+// 32 rows is where D 64 turns.  D 128 would from 17 rows on and D 256 from 25, by up to 14 % and about a fifth on long
+// contexts; up to 32 rows K's codes stay exact, as attend() has them.  So this kernel has more than 32 rows, where positions times heads, rows and dims reach 160 million (D 64 and 128: 40 rows
 // of 8 sequences of 257, D 128, 22 and 21 us; 64 of D 64, 151 million, 11 and 19) or 640 million (D 256: 64 rows there 36 and
 // 38, 80 rows 43 and 38).  The lengths are on the GPU: what counts is what the block table can hold, and short sequences in
-// a wide table cost those 7 to 15 us more.
+// a wide table cost those 7 to 15 us more, and fp16's rounding of K and V.
 bool tree_is_wide(const Kv4Attn& a) {
     const long long rows = static_cast<long long>(a.q_len) * a.group;
     if (a.type != ALJ_KV_BF16 || rows <= 32) return false;

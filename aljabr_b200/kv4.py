@@ -306,7 +306,8 @@ class Kv4Cache:
         return self._zeros(self._work_size(native.KV4_MAX_ROWS, self.kv_heads, self.kv_heads, self.head_dim), stream)
 
     def _tree_workspace(self, stream: int):
-        """(address, bytes) of this stream's workspace for trees: as large as any accepted call needs, kept for good."""
+        """(address, bytes) of this stream's workspace for trees: as large as any call of any cache needs (39 MB), and kept for
+        good, since kernels under way may hold its address."""
         key = self._index, stream_key(stream)
         have = _tree_work.get(key)
         if have is None:

@@ -372,7 +372,7 @@ int aljabr_blackwell_gemm_q_dev(int type, int nseg, float* const* y, const int* 
  * softmax weights with 2^-22 of themselves or 2^-28 of the largest V.
  * Queries of 2^115 and more leave its range and may give NaN.  For
  * bf16 queries the weights and their products with V's scales are rounded to
- * fp16 (2^-11 each), below the output's own rounding of 2^-9.
+ * fp16 (2^-11 each), below the output's own rounding of 2^-8.
  * q_len * q_heads / kv_heads is at most 1024, batch at most 2048.  The results
  * do not depend on timing.
  * workspace: kv4_attention_workspace_size bytes of device memory (it does not
@@ -430,10 +430,19 @@ int aljabr_blackwell_kv4_attention_dev(void* out, const void* q, int q_dtype, lo
  * its ancestors and itself; with window > 0 of these the last `window`, a
  * node counting as position base + its depth (a root's is 0).  A node that is
  * absent, or whose sequence holds no tree, is zero.  nodes * q_heads /
- * kv_heads is at most 1024.  The workspace may be the same as
- * kv4_attention_dev's where it is large enough, also for several threads that
- * call on one stream.  A call is two launches: a captured graph that another
- * thread replays on that stream needs a workspace of its own.
+ * kv_heads (rows) is at most 1024.
+ * Accuracy: as kv4_attention_dev's for fp32 queries and for up to 32 rows.
+ * bf16 queries with more rows and enough work (by the sizes given and what the
+ * block table can hold, so not by the data) run on the tensor cores, whose
+ * operands are fp16: values of K and V too are rounded, by 2^-11 each, and with
+ * them a score by up to 2^-11 of its products' magnitudes, which scores in the
+ * hundreds feel.  Values whose scale is more than 2^25 below the largest of
+ * their 32 positions lose more, as do weights of positions whose V scales are
+ * more than 2^22 below the largest so far.
+ * The workspace may be the same as kv4_attention_dev's where it is large
+ * enough, also for several threads that call on one stream.  A call is two
+ * launches: a captured graph that another thread replays on that stream needs
+ * a workspace of its own.
  *
  * kv4_accept_tree_dev: from node 0 (a root: the token emitted last) on to the
  * first child whose drafted token is the one picked after its parent, as long
