@@ -1285,10 +1285,11 @@ cudaError_t launch_tree(const Kv4Attn& p, Cut* cuts, int sms, unsigned int* faul
 //   1 sequence of 4096:     48 rows, D 64, 128, 256: 16, 19   23, 21    29, 33     128 rows: 23, 19   32, 21    52, 34
 //   1 sequence of 257:     128 rows, D 64, 128, 256: 11, 18   12, 20    12, 27
 // 32 rows is where D 64 turns.  D 128 would from 17 rows on and D 256 from 25, by up to 14 % and about a fifth on long
-// contexts; up to 32 rows K's codes stay exact, as attend() has them.  So this kernel has more than 32 rows, where positions times heads, rows and dims reach 160 million (D 64 and 128: 40 rows
-// of 8 sequences of 257, D 128, 22 and 21 us; 64 of D 64, 151 million, 11 and 19) or 640 million (D 256: 64 rows there 36 and
-// 38, 80 rows 43 and 38).  The lengths are on the GPU: what counts is what the block table can hold, and short sequences in
-// a wide table cost those 7 to 15 us more, and fp16's rounding of K and V.
+// contexts; up to 32 rows K's codes stay exact, as attend() has them.  So this kernel has more than 32 rows, where positions
+// times heads, rows and dims reach 160 million (D 64 and 128: 40 rows of 8 sequences of 257, D 128, 22 and 21 us; 64 of D 64,
+// 151 million, 11 and 19) or 640 million (D 256: 64 rows there 36 and 38, 80 rows 43 and 38).  The lengths are on the GPU: what
+// counts is what the block table can hold, and short sequences in a wide table cost those 7 to 15 us more, and fp16's
+// rounding of K and V.
 bool tree_is_wide(const Kv4Attn& a) {
     const long long rows = static_cast<long long>(a.q_len) * a.group;
     if (a.type != ALJ_KV_BF16 || rows <= 32) return false;
