@@ -42,7 +42,7 @@ def refused(**kw):
     # what is read by all, and the cache (4 pages of 16 positions, 2 heads of 128: 18432 bytes)
     (dict(qo=6 * M), True), (dict(slots=2 * M + 12284), True), (dict(slots=2 * M + 12288), False), (dict(pos=9 * M, kb=9 * M, vb=10 * M), True),
     (dict(rope=2 * M - 100 * 128 * 4 - 8), False), (dict(rope=2 * M - 100 * 128 * 4 + 8), True), (dict(slots=M + 18428), True),
-    (dict(qo=M + 18432), False), (dict(qo=M + 18428), True), (dict(kb=M - 3072, vb=10 * M), False), (dict(kb=M - 3068, vb=10 * M), True),
+    (dict(qo=M + 18432), False), (dict(qo=M + 18428), True), (dict(kb=M - 3 * 1024, vb=10 * M), False), (dict(kb=M - 3 * 1024 + 4, vb=10 * M), True),
 ])
 def test_overlaps(kw, want):
     assert refused(**kw) == want
